@@ -302,7 +302,7 @@ def _exact_mx(x):
         b = x[r0:r0 + 8192].double().unflatten(-1, (-1, 32))
         amax = b.abs().max(-1, keepdim=True).values
         e = torch.where(amax > 0, torch.floor(torch.log2(amax)), torch.full_like(amax, -1e9)) - 2.0
-        s = torch.pow(2.0, e.clamp(min=-126.0))
+        s = torch.exp2(e.clamp(min=-126.0))  # exact, which pow(2, e) is not on the GPU
         t = (b.abs() / s).clamp(max=6.0)
         best, near = torch.zeros_like(t), t.clone()
         for i in range(1, 8):
