@@ -429,6 +429,85 @@ int t2t_gram_strided(const void* x, int x_dtype, long long x_head_stride, long l
 int t2t_fit_chol(const double* Mq, const double* Mk, double* L, int32_t* small, int H, int D,
                  double floor, void* stream);
 
+/* ---- rotary positions -------------------------------------------------- */
+/* The block's steps between the q / k projections and attention; no
+ * counterpart in the reference, whose models run them in torch.
+ *
+ * cosv[t, i] = factor * cos(p[t, a] * freqs[i]), sinv likewise ([T, pairs]
+ * fp32, pairs = the sum of axis_pairs): positions [T, axes] int32 or int64
+ * (pos_bits), 1 <= axes <= 4; axis a has axis_pairs[a] pairs (1 .. 4096; host
+ * memory), one after the other.  freqs [pairs] fp64.  Angles, sines and
+ * cosines are taken in fp64.  Product magnitudes up to 2^31. */
+int t2t_rotary_table(const void* positions, int pos_bits, long long T, int axes,
+                     const int* axis_pairs, const double* freqs, double factor, float* cosv,
+                     float* sinv, void* stream);
+#define T2T_ROPE_INTERLEAVED 0 /* pairs (2 i, 2 i + 1)   */
+#define T2T_ROPE_HALF        1 /* pairs (i, i + R / 2)   */
+#define T2T_NORM_NONE  0
+#define T2T_NORM_TOKEN 1 /* RMS over a token's heads * D values, weight [heads * D] */
+#define T2T_NORM_HEAD  2 /* RMS over a head's D values, weight [D]                  */
+/* Element (b, n, h, d) of x at b x_batch + n x_row + h x_head + d (elements;
+ * any strides), of out likewise.  out may be x with the same strides; apart
+ * from that no output shares memory with an input or the other output. */
+typedef struct t2t_rotary_tensor {
+  const void* x;
+  long long x_batch, x_row, x_head;
+  void* out;
+  long long out_batch, out_row, out_head;
+  const void* weight; /* of the norm, in the tensors' type; else unused */
+  int heads;
+} t2t_rotary_tensor;
+/* q [B, N, Hq, D] and (k not NULL) k [B, N, Hk, D], fp16 or bf16, both in one
+ * launch: out = rotate(x * rsqrt(mean(x^2) + eps) * weight), without the norm
+ * out = rotate(x); fp32 inside, rounded once.  The first R channels of a head
+ * are turned, pair i by (cosv, sinv)[b, n, i] ([B, N, R / 2] where
+ * table_batched, else [N, R / 2]; contiguous), the others are not.  inverse:
+ * by the negative angle, which is also the gradient's way back (no norm).
+ * 1 <= D <= 256, R even, 2 <= R <= D. */
+int t2t_rotary(const t2t_rotary_tensor* q, const t2t_rotary_tensor* k, int dtype, const float* cosv,
+               const float* sinv, int table_batched, int B, int N, int D, int R, int layout,
+               int inverse, int norm, float eps, void* stream);
+
+/* ---- MXFP4 linear layers ------------------------------------------------ */
+/* Matrices [M, K] (K a multiple of 32) of 4-bit E2M1 values (0, .5, 1, 1.5, 2,
+ * 3, 4, 6 and their negatives) in blocks of 32 columns with one scale byte
+ * each (E8M0: 2^(byte - 127); 255 stands for NaN).  No counterpart in the
+ * reference.  Codes and scales are held in the operand order of the scaled
+ * MFMA, rows in blocks of 32 and columns padded to 256 with zeros:
+ *   codes  [ceil(M / 32)][K / 64][64][16] bytes: lane l of a chunk holds row
+ *          l % 32, columns 32 (l / 32) + j of the chunk's 64, column j in
+ *          nibble j % 2 of byte j / 2
+ *   scales [ceil(M / 32)][K / 256][64][4] bytes: byte j of lane l belongs to
+ *          row l % 32, columns 64 j + 32 (l / 32) .. + 31 of the group's 256
+ * Byte counts of both (0 for an empty matrix). */
+size_t t2t_mxfp4_code_bytes(int M, int K);
+size_t t2t_mxfp4_scale_bytes(int M, int K);
+/* x [M, K] fp16 / bf16, row m at m * row_stride (elements, a multiple of 8; x
+ * 16-byte aligned).  A block's scale is 2^e, e = floor(log2 max|x|) - 2, at
+ * least -126; codes are x / 2^e to nearest, ties to even, held to 6; a block
+ * with an inf or NaN gets byte 255. */
+int t2t_mxfp4_quantize(const void* x, int dtype, long long row_stride, void* codes, void* scales,
+                       int M, int K, void* stream);
+/* The values that codes and scales stand for -> out [M, K] fp16 / bf16 (exact
+ * in the type that was quantised). */
+int t2t_mxfp4_dequantize(const void* codes, const void* scales, void* out, int dtype,
+                         long long row_stride, int M, int K, void* stream);
+#define T2T_ACT_NONE      0
+#define T2T_ACT_GELU_TANH 1 /* x / 2 (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) */
+/* out [M, N] (dtype) = act(A W^T + bias): A [M, K] and W [N, K] in MXFP4,
+ * bias [N] in dtype or NULL; fp32 sums, rounded once.  Row m of out at
+ * m * out_row_stride. */
+int t2t_mxfp4_product(const void* a_codes, const void* a_scales, const void* w_codes,
+                      const void* w_scales, const void* bias, int act, void* out, int dtype,
+                      long long out_row_stride, int M, int N, int K, void* stream);
+/* t2t_mxfp4_quantize of x into the workspace and t2t_mxfp4_product.  out
+ * shares no memory with x. */
+size_t t2t_mxfp4_linear_ws_bytes(int M, int N, int K);
+int t2t_mxfp4_linear(const void* x, int dtype, long long x_row_stride, const void* w_codes,
+                     const void* w_scales, const void* bias, int act, void* out,
+                     long long out_row_stride, int M, int N, int K, void* ws, size_t ws_bytes,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -35,6 +35,13 @@ class StepArgs(ctypes.Structure):
                                            "ws_split_bytes")])
 
 
+class RotaryTensor(ctypes.Structure):
+    """t2t_rotary_tensor of include/t2t_hip.h."""
+    _fields_ = ([("x", _P)] + [(f"x_{s}", c_longlong) for s in ("batch", "row", "head")]
+                + [("out", _P)] + [(f"out_{s}", c_longlong) for s in ("batch", "row", "head")]
+                + [("weight", _P), ("heads", c_int)])
+
+
 # the stages of t2t_step, in order
 (STEP_PROJECT_Q, STEP_PROJECT_K, STEP_KMEANS, STEP_VSTATS, STEP_FINALIZE, STEP_SELECT,
  STEP_GATHER_K, STEP_PLAN, STEP_EXACT, STEP_TILES, STEP_RESIDUAL) = (1 << i for i in range(11))
@@ -123,6 +130,18 @@ SIGNATURES = {
     "t2t_gram_strided": (c_int, [_P, c_int, c_longlong, c_longlong, _P, _P, c_int, c_int, c_int, _P,
                                  c_size_t, _P]),
     "t2t_fit_chol": (c_int, [_P, _P, _P, _P, c_int, c_int, c_double, _P]),
+    "t2t_rotary_table": (c_int, [_P, c_int, c_longlong, c_int, ctypes.POINTER(c_int), _P, c_double, _P,
+                                 _P, _P]),
+    "t2t_rotary": (c_int, [ctypes.POINTER(RotaryTensor)] * 2 + [c_int, _P, _P] + [c_int] * 8 +
+                   [c_float, _P]),
+    "t2t_mxfp4_code_bytes": (c_size_t, [c_int, c_int]),
+    "t2t_mxfp4_scale_bytes": (c_size_t, [c_int, c_int]),
+    "t2t_mxfp4_quantize": (c_int, [_P, c_int, c_longlong, _P, _P, c_int, c_int, _P]),
+    "t2t_mxfp4_dequantize": (c_int, [_P, _P, _P, c_int, c_longlong, c_int, c_int, _P]),
+    "t2t_mxfp4_product": (c_int, [_P] * 5 + [c_int, _P, c_int, c_longlong] + [c_int] * 3 + [_P]),
+    "t2t_mxfp4_linear_ws_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "t2t_mxfp4_linear": (c_int, [_P, c_int, c_longlong, _P, _P, _P, c_int, _P, c_longlong, c_int, c_int,
+                                 c_int, _P, c_size_t, _P]),
 }
 
 _lib = None

@@ -7,8 +7,11 @@ library and CUDA (ROCm) tensors.
 """
 from __future__ import annotations
 
+import ctypes
 import math
-from contextlib import nullcontext
+from contextlib import contextmanager, nullcontext
+from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -704,3 +707,348 @@ def fit_chol(Mq, Mk, floor, small, stream=None):
     L = _new(stream, H, D, D, dtype=torch.float64, device=dev)
     call("t2t_fit_chol", Mq, Mk, L, small, H, D, float(floor), stream_handle(stream))
     return L
+
+
+# ---------------------------------------------------------------------------
+# the block's steps around attention: rotary positions, MXFP4 linear layers
+# ---------------------------------------------------------------------------
+@contextmanager
+def _launch(dev, stream, *tensors):
+    """A call on ``stream`` (default: ``dev``'s current one) with ``dev``
+    current; yields the stream's handle.  On a stream of the caller's choice the
+    tensors' memory is not reused before the stream is done with it."""
+    if stream is not None and stream.device != dev:
+        raise ValueError(f"t2t: the stream is on {stream.device}, the tensors on {dev}")
+    with torch.cuda.device(dev) if torch.cuda.current_device() != dev.index else nullcontext():
+        if stream is not None:
+            for t in tensors:
+                if t is not None:
+                    t.record_stream(stream)
+        yield stream_handle(stream)
+
+
+def _check_vec(t, n, dtype, name, dev):
+    if t is not None:
+        _check(t, (n,), dtype, name, dev)
+
+
+def _scattered(t):
+    """Whether a view's elements all have an address of their own."""
+    last = 0
+    for st, sz in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
+        if st <= last:
+            return False
+        last += st * (sz - 1)
+    return True
+
+
+@dataclass(frozen=True)
+class RotaryScaling:
+    """How the frequencies f[i] = base^(-2 i / d) are stretched for contexts
+    ``factor`` times as long as the ``original`` one:
+
+    - ``linear``: f[i] / factor;
+    - ``ntk``: base * factor^(d / (d - 2)) in the place of base;
+    - ``yarn``: f[i] (1 - r) + f[i] / factor r, r rising from 0 to 1 between
+      the pairs that turn ``beta_fast`` and ``beta_slow`` times over the
+      original length; cos and sin times ``attention`` (default
+      0.1 ln(factor) + 1)."""
+
+    kind: str
+    factor: float
+    original: int = 0
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    attention: float | None = None
+
+
+class RotaryFrequencies(NamedTuple):
+    """Frequencies of every pair (fp64, on the device), the pairs of each
+    position axis and the factor of cos and sin."""
+
+    freqs: torch.Tensor
+    pairs: tuple[int, ...]
+    factor: float
+
+
+def rotary_frequencies(dims, *, base=10000.0, scaling=None, device):
+    """The frequencies of rotated channels ``dims`` (an even number, or one
+    for each of up to four position axes), to be kept by the program."""
+    dims = (dims,) if isinstance(dims, int) else tuple(dims)
+    if not 1 <= len(dims) <= 4 or any(int(d) != d or d < 2 or d % 2 or d > 8192 for d in dims):
+        raise ValueError(f"t2t: dims must be one to four even numbers in [2, 8192], got {dims}")
+    if not (math.isfinite(base) and base > 1.0):
+        raise ValueError(f"t2t: base must be above 1, got {base}")
+    factor = 1.0
+    if scaling is not None:
+        if scaling.kind not in ("linear", "ntk", "yarn"):
+            raise ValueError(f"t2t: scaling kind {scaling.kind!r} (linear, ntk or yarn)")
+        if not (math.isfinite(scaling.factor) and scaling.factor >= 1.0):
+            raise ValueError(f"t2t: scaling factor must be at least 1, got {scaling.factor}")
+        if scaling.kind == "yarn":
+            if scaling.original < 1 or not scaling.beta_fast > scaling.beta_slow > 0:
+                raise ValueError("t2t: yarn needs the original length and beta_fast > beta_slow > 0")
+            factor = scaling.attention
+            if factor is None:
+                factor = 0.1 * math.log(scaling.factor) + 1.0
+    f = []
+    for d in dims:
+        b = base
+        if scaling is not None and scaling.kind == "ntk":
+            if d == 2:
+                raise ValueError("t2t: ntk scaling needs more than one pair an axis")
+            b = base * scaling.factor ** (d / (d - 2.0))
+        fd = [b ** (-2.0 * i / d) for i in range(d // 2)]
+        if scaling is not None and scaling.kind == "linear":
+            fd = [x / scaling.factor for x in fd]
+        elif scaling is not None and scaling.kind == "yarn":
+            # pair d ln(L / (2 pi t)) / (2 ln base) makes t turns over length L
+            lo, hi = (d * math.log(scaling.original / (2.0 * math.pi * t)) / (2.0 * math.log(base))
+                      for t in (scaling.beta_fast, scaling.beta_slow))
+            lo, hi = max(math.floor(lo), 0), min(math.ceil(hi), d - 1)
+            width = (hi - lo) or 0.001
+            r = [min(max((i - lo) / width, 0.0), 1.0) for i in range(d // 2)]
+            fd = [x * y / scaling.factor + x * (1.0 - y) for x, y in zip(fd, r)]
+        f += fd
+    return RotaryFrequencies(torch.tensor(f, dtype=torch.float64, device=device),
+                             tuple(d // 2 for d in dims), float(factor))
+
+
+def rotary_table(positions, frequencies, out=None, stream=None):
+    """(cos, sin) of ``positions`` (int32 or int64, [...] for one axis, [...,
+    axes] for several) times the frequencies: fp32 [..., pairs] each.  Angles
+    are taken in 64 bits; |position * frequency| stays below 2^31."""
+    freqs, pairs, factor = frequencies
+    dev = _dev(positions)
+    lead = tuple(positions.shape)
+    if len(pairs) > 1:
+        if not lead or lead[-1] != len(pairs):
+            raise ValueError(f"t2t: positions must end in {len(pairs)} axes, got {lead}")
+        lead = lead[:-1]
+    _check(positions, positions.shape, (torch.int32, torch.int64), "positions", dev)
+    n = sum(pairs)
+    _check(freqs, (n,), torch.float64, "frequencies", dev)
+    with _launch(dev, stream, positions, freqs, *(out or ())) as st:
+        if out is None:
+            out = tuple(_new(stream, *lead, n, dtype=_f32, device=dev) for _ in range(2))
+        for t, name in zip(out, ("cos", "sin")):
+            _check(t, (*lead, n), _f32, name, dev)
+        call("t2t_rotary_table", positions, 32 if positions.dtype == _i32 else 64, math.prod(lead),
+             len(pairs), (ctypes.c_int * len(pairs))(*pairs), freqs, factor, *out, st)
+    return tuple(out)
+
+
+_ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
+_ROPE_NORMS = {None: 0, "token": 1, "head": 2}
+
+
+def _rotary_arg(x, out, weight, norm, name, dev, B, N, D, dtype):
+    if (not isinstance(x, torch.Tensor) or x.dtype != dtype or x.device != dev or x.dim() not in (3, 4)
+            or (x.shape[0] if x.dim() == 4 else 1) != B or x.shape[-3] != N or x.shape[-1] != D
+            or not 1 <= x.shape[-2] <= 65536 or (D > 1 and x.stride(-1) != 1)):
+        raise ValueError(f"t2t: {name} must be a {dtype} [{B}, {N}, heads, {D}] tensor on {dev} with "
+                         f"contiguous channels")
+    if (not isinstance(out, torch.Tensor) or out.shape != x.shape or out.dtype != dtype
+            or out.device != dev or (D > 1 and out.stride(-1) != 1) or not _scattered(out)):
+        raise ValueError(f"t2t: the output of {name} must be a {dtype} {tuple(x.shape)} tensor on {dev} "
+                         f"with contiguous channels and no element twice")
+    H = x.shape[-2]
+    if norm is not None:
+        _check(weight, (H * D,) if norm == "token" else (D,), dtype, f"{name}_weight", dev)
+    elif weight is not None:
+        raise ValueError(f"t2t: {name}_weight without a norm")
+    sb = lambda t: t.stride(0) if t.dim() == 4 else 0  # noqa: E731
+    return _lib.RotaryTensor(x.data_ptr(), sb(x), x.stride(-3), x.stride(-2), out.data_ptr(), sb(out),
+                             out.stride(-3), out.stride(-2),
+                             weight.data_ptr() if weight is not None else None, H)
+
+
+def rotary(q, k, cos, sin, *, layout="interleaved", inverse=False, norm=None, q_weight=None,
+           k_weight=None, eps=1e-6, out=None, stream=None):
+    """Rotated q [B, N, Hq, D] and k [B, N, Hk, D] (or [N, H, D]; fp16 or bf16;
+    any strides with contiguous channels; k may be None), one launch.
+
+    cos, sin fp32 [N, R / 2] or [B, N, R / 2]: the first R <= D channels of every
+    head are turned, pairs (2i, 2i + 1) with ``layout`` "interleaved", (i, i +
+    R / 2) with "half"; the others pass.  ``inverse`` turns back (the rotation's
+    transpose, so also its gradient).  ``norm``: an RMS norm before the turn,
+    x * rsqrt(mean(x^2) + eps) * weight, over all heads of a token ("token",
+    weight [H * D]) or each head ("head", weight [D]).  fp32 inside, rounded
+    once.  ``out``: (out_q, out_k); an output may be its input, and otherwise
+    shares no memory with any other argument.  Returns (out_q, out_k)."""
+    dev = _dev(q)
+    if q.dim() not in (3, 4) or q.dtype not in _HALF:
+        raise ValueError("t2t: q must be an fp16 or bf16 [B, N, H, D] or [N, H, D] tensor")
+    B, (N, _, D) = q.shape[0] if q.dim() == 4 else 1, q.shape[-3:]
+    if layout not in _ROPE_LAYOUTS or norm not in _ROPE_NORMS:
+        raise ValueError(f"t2t: layout {layout!r} (interleaved or half), norm {norm!r} (None, token or head)")
+    if inverse and norm is not None:
+        raise ValueError("t2t: the inverse rotation takes no norm")
+    if not (math.isfinite(eps) and eps >= 0.0):
+        raise ValueError(f"t2t: eps must be at least 0, got {eps}")
+    R = 2 * cos.shape[-1] if isinstance(cos, torch.Tensor) and cos.dim() else 0
+    if not (1 <= D <= 256 and 2 <= R <= D):
+        raise ValueError(f"t2t: {R} of {D} channels rotated (2 <= R <= D <= 256)")
+    batched = cos.dim() == 3
+    for t, name in ((cos, "cos"), (sin, "sin")):
+        _check(t, (B, N, R // 2) if batched else (N, R // 2), _f32, name, dev)
+    if B * N >= 2 ** 31:
+        raise ValueError(f"t2t: {B} x {N} tokens")
+    with _launch(dev, stream, q, k, cos, sin, q_weight, k_weight, *(out or ())) as st:
+        if out is None:
+            out = tuple(None if x is None else _new(stream, *x.shape, dtype=x.dtype, device=dev)
+                        for x in (q, k))
+        tq = _rotary_arg(q, out[0], q_weight, norm, "q", dev, B, N, D, q.dtype)
+        tk = None
+        if k is not None:
+            tk = _rotary_arg(k, out[1], k_weight, norm, "k", dev, B, N, D, q.dtype)
+        call("t2t_rotary", ctypes.byref(tq), ctypes.byref(tk) if tk is not None else None,
+             dtype_code(q.dtype), cos, sin, int(batched), B, N, D, R, _ROPE_LAYOUTS[layout],
+             int(bool(inverse)), _ROPE_NORMS[norm], float(eps), st)
+    return out[0], out[1] if k is not None else None
+
+
+class MxFp4:
+    """A matrix [rows, cols] in MXFP4 (``mxfp4_quantize``): E2M1 codes in blocks
+    of 32 columns with a power-of-two scale each, in the order of the matrix
+    operands (include/t2t_hip.h).  ``codes`` and ``scales`` are uint8 buffers."""
+
+    __slots__ = ("codes", "scales", "rows", "cols")
+
+    def __init__(self, codes, scales, rows, cols):
+        self.codes, self.scales, self.rows, self.cols = codes, scales, rows, cols
+
+    @property
+    def shape(self):
+        return (self.rows, self.cols)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def __repr__(self):
+        return f"MxFp4({self.rows} x {self.cols}, {self.device})"
+
+
+def _mx_size(rows, cols, name):
+    if not (0 <= rows < 2 ** 31 and 32 <= cols < 2 ** 31 - 255 and cols % 32 == 0):
+        raise ValueError(f"t2t: {name} must have columns in multiples of 32, got {rows} x {cols}")
+
+
+def _check_mx(t, name, dev):
+    if not isinstance(t, MxFp4):
+        raise ValueError(f"t2t: {name} must be an MxFp4 matrix (mxfp4_quantize)")
+    _mx_size(t.rows, t.cols, name)
+    for buf, size in ((t.codes, "t2t_mxfp4_code_bytes"), (t.scales, "t2t_mxfp4_scale_bytes")):
+        _check(buf, (size_query(size, t.rows, t.cols),), torch.uint8, name, dev)
+
+
+def _mx_rows(t, name, dev, align):
+    """A [..., K] tensor of 16-bit values as rows: (rows, K, row stride)."""
+    if (not isinstance(t, torch.Tensor) or t.dtype not in _HALF or t.device != dev or t.dim() < 1):
+        raise ValueError(f"t2t: {name} must be an fp16 or bf16 tensor on {dev}")
+    cols = t.shape[-1]
+    try:
+        v = t.view(math.prod(t.shape[:-1]), cols)
+    except RuntimeError:
+        raise ValueError(f"t2t: the rows of {name} {tuple(t.shape)} must have one stride, got "
+                         f"{tuple(t.stride())}") from None
+    rows = v.shape[0]
+    stride = v.stride(0) if rows > 1 else cols
+    if cols > 1 and v.numel() and v.stride(1) != 1 or stride < cols \
+            or rows and (t.data_ptr() % align or rows > 1 and stride * 2 % align):
+        raise ValueError(f"t2t: {name} must have contiguous {align}-byte aligned rows that do not "
+                         f"overlap, got strides {tuple(t.stride())}")
+    return rows, cols, stride
+
+
+def _mx_new(stream, rows, cols, dev):
+    return MxFp4(*(_new(stream, size_query(size, rows, cols), dtype=torch.uint8, device=dev)
+                   for size in ("t2t_mxfp4_code_bytes", "t2t_mxfp4_scale_bytes")), rows, cols)
+
+
+def mxfp4_quantize(x, out=None, stream=None):
+    """x [..., K] (fp16 or bf16, contiguous 16-byte aligned rows, K a multiple of
+    32) in MXFP4, rows flattened.  A block's scale is 2^(floor(log2 max|x|) - 2)
+    (at least 2^-126); values are rounded to nearest, ties to even, and held to
+    6 scales; a block with an inf or NaN stands for NaN."""
+    dev = _dev(x)
+    M, K, stride = _mx_rows(x, "x", dev, 16)
+    _mx_size(M, K, "x")
+    if out is not None:
+        _check_mx(out, "out", dev)
+        if out.shape != (M, K):
+            raise ValueError(f"t2t: out is {out.rows} x {out.cols}, x {M} x {K}")
+    with _launch(dev, stream, x, *((out.codes, out.scales) if out is not None else ())) as st:
+        if out is None:
+            out = _mx_new(stream, M, K, dev)
+        call("t2t_mxfp4_quantize", _lib.RowView(x), dtype_code(x.dtype), stride, out.codes, out.scales,
+             M, K, st)
+    return out
+
+
+def mxfp4_dequantize(t, dtype=torch.bfloat16, out=None, stream=None):
+    """The values that an MxFp4 matrix stands for, [rows, cols]: exact in the
+    type that was quantised, and in bf16 where no scale is below 2^-126."""
+    if not isinstance(t, MxFp4):
+        raise ValueError("t2t: expected an MxFp4 matrix")
+    dev = _dev(t.codes)
+    _check_mx(t, "t", dev)
+    dtype_code(dtype)
+    with _launch(dev, stream, t.codes, t.scales, out) as st:
+        if out is None:
+            out = _new(stream, t.rows, t.cols, dtype=dtype, device=dev)
+        if _mx_rows(out, "out", dev, 16)[:2] != t.shape or out.dtype != dtype:
+            raise ValueError(f"t2t: out must be {dtype} {t.shape}, got {out.dtype} {tuple(out.shape)}")
+        stride = _mx_rows(out, "out", dev, 16)[2]
+        call("t2t_mxfp4_dequantize", t.codes, t.scales, _lib.RowView(out), dtype_code(dtype), stride,
+             t.rows, t.cols, st)
+    return out
+
+
+_ACTIVATIONS = {None: 0, "gelu_tanh": 1}
+
+
+def mxfp4_linear(x, weight, bias=None, *, activation=None, dtype=None, out=None, ws=None, stream=None):
+    """act(x W^T + bias) with both operands in MXFP4: x [..., K] fp16 or bf16
+    (quantised as by mxfp4_quantize; contiguous 16-byte aligned rows), or an
+    MxFp4 matrix that several layers share; weight MxFp4 [N, K]; bias [N] in the
+    output's type.  fp32 sums, one rounding to x's type (``dtype``, default
+    bf16, for an MxFp4 x) -> [..., N].  ``activation``: None or "gelu_tanh".
+    ``out``: contiguous rows, no memory shared with x."""
+    if not isinstance(weight, MxFp4):
+        raise ValueError("t2t: weight must be an MxFp4 matrix (mxfp4_quantize)")
+    dev = _dev(weight.codes)
+    _check_mx(weight, "weight", dev)
+    N = weight.rows
+    quantised = isinstance(x, MxFp4)
+    if quantised:
+        _check_mx(x, "x", dev)
+        (M, K), lead = x.shape, (x.rows,)
+        dt = torch.bfloat16 if dtype is None else dtype
+    else:
+        M, K, stride = _mx_rows(x, "x", dev, 16)
+        lead, dt = tuple(x.shape[:-1]), x.dtype
+        if dtype not in (None, dt):
+            raise ValueError(f"t2t: the output of a {dt} input is {dt}, not {dtype}")
+    code = dtype_code(dt)
+    if K != weight.cols or N < 1:
+        raise ValueError(f"t2t: x has {K} columns, weight {N} x {weight.cols}")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"t2t: activation {activation!r} (None or gelu_tanh)")
+    _check_vec(bias, N, dt, "bias", dev)
+    src = (x.codes, x.scales) if quantised else (x,)
+    with _launch(dev, stream, *src, weight.codes, weight.scales, bias, out) as st:
+        if out is None:
+            out = _new(stream, *lead, N, dtype=dt, device=dev)
+        om, on, ostride = _mx_rows(out, "out", dev, 2)
+        if tuple(out.shape) != (*lead, N) or out.dtype != dt:
+            raise ValueError(f"t2t: out must be {dt} {(*lead, N)}, got {out.dtype} {tuple(out.shape)}")
+        args = (weight.codes, weight.scales, bias, _ACTIVATIONS[activation], _lib.RowView(out))
+        if quantised:
+            call("t2t_mxfp4_product", *src, *args, code, ostride, M, N, K, st)
+        else:
+            ws = _ws_for(ws, size_query("t2t_mxfp4_linear_ws_bytes", M, N, K), dev, stream)
+            call("t2t_mxfp4_linear", _lib.RowView(x), code, stride, *args, ostride, M, N, K, ws,
+                 ws.numel(), st)
+    return out
