@@ -14,6 +14,7 @@
 // Rows past M and columns past K hold zero codes and zero scale bytes (a zero
 // code under a scale of 255, which stands for NaN, would be NaN).
 #include "t2t_common.h"
+#include <type_traits>
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
@@ -222,45 +223,195 @@ struct MxMat {
   int rows, blocks;  // rows, row blocks of 32
 };
 
-// One wave per 32 x 32 outputs, fragments straight from memory.  The weights
-// are the A operand, so a lane holds one token's features 8 (i / 4) +
-// 4 (l / 32) + i % 4.
-template <typename T>
-__global__ __launch_bounds__(256) void mx_linear_kernel(MxMat a, MxMat w,
-                                                        const uint16_t* __restrict__ bias, int act,
-                                                        uint16_t* __restrict__ out, long long ldo,
-                                                        int groups, long long tiles) {
-  const int lane = threadIdx.x & 63;
-  const long long tile = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (tile >= tiles) return;
-  const long long mb = tile / w.blocks;
-  const int nb = (int)(tile - mb * w.blocks);
-  const char* ap = a.codes + mb * groups * 4096 + lane * 16;
-  const char* wp = w.codes + (long long)nb * groups * 4096 + lane * 16;
-  const uint32_t* as = a.scales + mb * groups * 64 + lane;
-  const uint32_t* wsc = w.scales + (long long)nb * groups * 64 + lane;
-  f32x16 acc = zero16();
-  for (int g = 0; g < groups; ++g) {
-    const uint32_t sa = as[g * 64], sw = wsc[g * 64];
-    const u32x4* pa = (const u32x4*)(ap + (size_t)g * 4096);
-    const u32x4* pw = (const u32x4*)(wp + (size_t)g * 4096);
-    acc = mx_mfma<0>(pw[0], pa[0], acc, sw, sa);
-    acc = mx_mfma<1>(pw[64], pa[64], acc, sw, sa);
-    acc = mx_mfma<2>(pw[128], pa[128], acc, sw, sa);
-    acc = mx_mfma<3>(pw[192], pa[192], acc, sw, sa);
-  }
-  const long long m = mb * 32 + (lane & 31);
-  if (m >= a.rows) return;
+// Tiles of 64 TW features x 64 TA tokens, four waves of 32 TW x 32 TA each (2 x
+// 2).  The weights are the A operand, so a lane holds one token's features 8
+// (i / 4) + 4 (l / 32) + i % 4 of a block.  Operands are staged through LDS by
+// DMA, in the order they are held in memory, which is the order of the
+// fragments: both the DMA and the fragment reads are linear (no conflicts, no
+// address arithmetic).  A stage is 128 columns (two fragments a row block) and
+// four stages are kept, so a stage's loads have the time of three to land.
+typedef __attribute__((address_space(3))) void mx_lds_t;
+typedef __attribute__((address_space(1))) void mx_glb_t;
+
+template <int TW, int TA> struct MxTile {
+  static constexpr int RB = 2 * (TW + TA);          // row blocks: 2 TW of weights, 2 TA of tokens
+  static constexpr int CODES = RB * 2048;           // a stage's codes
+  static constexpr int PITCH = 64 * TW + 16;        // a token's staged outputs (bytes)
+  static constexpr int SCALES = RB * 256;
+  static constexpr int STAGE = CODES + SCALES > 4 * 32 * PITCH ? CODES + SCALES : 4 * 32 * PITCH;
+};
+
+template <typename T, int TW, int TA, bool GELU>
+__global__ __launch_bounds__(256, TW * TA >= 16 ? 1 : 2) void mx_tile_kernel(
+    MxMat a, MxMat w, const uint16_t* __restrict__ bias, uint16_t* __restrict__ out, long long ldo, int vec,
+    int groups, int mt, int nt, int per_xcd) {
+  using C = MxTile<TW, TA>;
+  __shared__ __attribute__((aligned(1024))) char st0[C::STAGE];
+  __shared__ __attribute__((aligned(1024))) char st1[C::STAGE];
+  __shared__ __attribute__((aligned(1024))) char st2[C::STAGE];
+  __shared__ __attribute__((aligned(1024))) char st3[C::STAGE];
+  // consecutive work-groups go to the eight XCDs in turn: each takes a run of
+  // tiles, eight token tiles by all feature tiles, so that the 32 tiles an XCD
+  // has under way share their panels in its L2
+  const int id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  if (id >= mt * nt) return;
+  const int grp = id / (8 * nt), in = id - grp * 8 * nt;
+  const int gm = min(8, mt - grp * 8);
+  const int m0 = (grp * 8 + in % gm) * 2 * TA, n0 = (in / gm) * 2 * TW;  // row blocks
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wn = wave & 1, wm = wave >> 1, hh = lane >> 5;
+  // this wave's share of the stage's DMA: TW + TA KB of codes, and 1 KB of scales (four row
+  // blocks; with fewer than sixteen some waves fetch the same)
+  const char* src[TW + TA];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int n = nb * 32 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
-    if (n < w.rows) {
-      float v = acc[i];
-      if (bias) v += T::to_f(bias[n]);
-      if (act) v = mx_gelu(v);
-      out[m * ldo + n] = T::from_f(v);
+  for (int i = 0; i < TW + TA; ++i) {
+    const int q = wave * (TW + TA) + i, rb = q >> 1;
+    const long long row = rb < 2 * TW ? min(n0 + rb, w.blocks - 1) : min(m0 + rb - 2 * TW, a.blocks - 1);
+    src[i] = (rb < 2 * TW ? w.codes : a.codes) + row * groups * 4096 + (q & 1) * 1024;
+  }
+  constexpr int SI = (C::RB + 3) / 4;
+  const int srb = min(4 * (wave % SI) + (lane >> 4), C::RB - 1);
+  const long long srow = srb < 2 * TW ? min(n0 + srb, w.blocks - 1) : min(m0 + srb - 2 * TW, a.blocks - 1);
+  const char* ssrc = (const char*)(srb < 2 * TW ? w.scales : a.scales) + srow * groups * 256 + (lane & 15) * 16;
+  const int n = 2 * groups;  // stages
+  // Stages past the last keep the counts of loads in flight what they are, at the price of one
+  // line each: every lane reads the same 16 bytes of the last stage.
+  auto issue = [&](int s, char* st, auto ODD) {
+    constexpr int O = decltype(ODD)::value;
+    const int t = min(s, n - 2 + O);
+    const uint32_t voff = s < n ? lane * 16 : 0;
+#pragma unroll
+    for (int i = 0; i < TW + TA; ++i)
+      __builtin_amdgcn_global_load_lds((const mx_glb_t*)(src[i] + (size_t)t * 2048 + voff),
+                                       (mx_lds_t*)(st + (wave * (TW + TA) + i) * 1024), 16, 0, 0);
+    if constexpr (!O)
+      __builtin_amdgcn_global_load_lds((const mx_glb_t*)(ssrc + (size_t)(t >> 1) * 256),
+                                       (mx_lds_t*)(st + C::CODES + (wave % SI) * 1024), 16, 0, 0);
+  };
+  f32x16 acc[TW][TA];
+#pragma unroll
+  for (int i = 0; i < TW; ++i) {
+    f32x16 b0 = zero16();
+    if (bias)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        b0[e] = T::to_f(bias[min((n0 + wn * TW + i) * 32 + 8 * (e >> 2) + 4 * hh + (e & 3), w.rows - 1)]);
+#pragma unroll
+    for (int j = 0; j < TA; ++j) acc[i][j] = b0;
+  }
+  u32x4 fw[2][TW], fa[2][TA];
+  uint32_t sw[TW], sa[TA];
+  auto frags = [&](const char* st, int c) {
+#pragma unroll
+    for (int i = 0; i < TW; ++i)
+      fw[c][i] = *(const u32x4*)(st + ((wn * TW + i) * 2 + c) * 1024 + lane * 16);
+#pragma unroll
+    for (int j = 0; j < TA; ++j)
+      fa[c][j] = *(const u32x4*)(st + ((2 * TW + wm * TA + j) * 2 + c) * 1024 + lane * 16);
+  };
+  auto mul = [&](auto S, int c) {
+#pragma unroll
+    for (int i = 0; i < TW; ++i)
+#pragma unroll
+      for (int j = 0; j < TA; ++j)
+        acc[i][j] = mx_mfma<decltype(S)::value>(fw[c][i], fa[c][j], acc[i][j], sw[i], sa[j]);
+  };
+  // one stage: its first fragments are in registers; the second ones are read under the first
+  // products, the next stage's first ones under the second products
+  auto stage = [&](int s, char* cur, const char* nxt, auto ODD) {
+    constexpr int O = decltype(ODD)::value;
+    if constexpr (!O) {
+#pragma unroll
+      for (int i = 0; i < TW; ++i) sw[i] = *(const uint32_t*)(cur + C::CODES + (wn * TW + i) * 256 + lane * 4);
+#pragma unroll
+      for (int j = 0; j < TA; ++j)
+        sa[j] = *(const uint32_t*)(cur + C::CODES + (2 * TW + wm * TA + j) * 256 + lane * 4);
+    }
+    frags(cur, 1);
+    mul(std::integral_constant<int, 2 * O>{}, 0);
+    // stage s + 1 of every wave has landed and this stage's reads are done; the two stages
+    // after it may still be under way
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * (TW + TA) + 1) : "memory");
+    issue(s + 4, cur, ODD);
+    frags(nxt, 0);
+    mul(std::integral_constant<int, 2 * O + 1>{}, 1);
+  };
+  using Even = std::integral_constant<int, 0>;
+  using Odd = std::integral_constant<int, 1>;
+  issue(0, st0, Even{});
+  issue(1, st1, Odd{});
+  issue(2, st2, Even{});
+  issue(3, st3, Odd{});
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(3 * (TW + TA) + 1) : "memory");
+  frags(st0, 0);
+  for (int s = 0;; s += 4) {
+    stage(s, st0, st1, Even{});
+    stage(s + 1, st1, st2, Odd{});
+    if (s + 2 >= n) break;
+    stage(s + 2, st2, st3, Even{});
+    stage(s + 3, st3, st0, Odd{});
+    if (s + 4 >= n) break;
+  }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  // epilogue: 32 tokens at a time through a staging area of the wave's own, then whole rows
+  char* so = st0 + wave * 32 * C::PITCH;
+  constexpr int LR = 4 * TW;  // lanes per row, 8 features each
+  const int f0 = (n0 + wn * TW) * 32 + (lane % LR) * 8;
+  const bool whole = vec && f0 + 8 <= w.rows;
+#pragma unroll
+  for (int j = 0; j < TA; ++j) {
+#pragma unroll
+    for (int i = 0; i < TW; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = GELU ? mx_gelu(acc[i][j][4 * q + e]) : acc[i][j][4 * q + e];
+        *(u32x2*)(so + (lane & 31) * C::PITCH + (32 * i + 8 * q + 4 * hh) * 2) =
+            u32x2{Pk<T>::pack(v[0], v[1]), Pk<T>::pack(v[2], v[3])};
+      }
+    const int mb = (m0 + wm * TA + j) * 32;
+#pragma unroll 1
+    for (int t = lane / LR; t < 32 && mb + t < a.rows; t += 64 / LR) {
+      const u32x4 v = *(const u32x4*)(so + t * C::PITCH + (lane % LR) * 16);
+      uint16_t* o = out + (long long)(mb + t) * ldo + f0;
+      if (whole)
+        *(u32x4*)o = v;
+      else
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (f0 + e < w.rows) o[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
     }
   }
+}
+
+template <typename T, int TW, int TA>
+static int mx_tile_launch(const MxMat& a, const MxMat& w, const uint16_t* bias, int act, uint16_t* out,
+                          long long ldo, int groups, hipStream_t st) {
+  const int mt = cdiv(a.blocks, 2 * TA), nt = cdiv(w.blocks, 2 * TW);
+  const long long tiles = (long long)mt * nt;
+  T2T_REQUIRE(tiles <= INT_MAX / 2, "mxfp4_product: M=%d N=%d", a.rows, w.rows);
+  const int per = cdiv(tiles, 8);
+  const int vec = ldo % 8 == 0 && (uintptr_t)out % 16 == 0;
+  if (act == T2T_ACT_GELU_TANH)
+    hipLaunchKernelGGL((mx_tile_kernel<T, TW, TA, true>), dim3(8 * per), dim3(256), 0, st, a, w, bias, out,
+                       ldo, vec, groups, mt, nt, per);
+  else
+    hipLaunchKernelGGL((mx_tile_kernel<T, TW, TA, false>), dim3(8 * per), dim3(256), 0, st, a, w, bias, out,
+                       ldo, vec, groups, mt, nt, per);
+  T2T_LAUNCH_CHECK("mxfp4_product");
+  return T2T_OK;
+}
+
+template <typename T>
+static int mx_product(const MxMat& a, const MxMat& w, const uint16_t* bias, int act, uint16_t* out,
+                      long long ldo, int groups, hipStream_t st) {
+  if ((long long)a.blocks * w.blocks >= 64 * 256)
+    return mx_tile_launch<T, 4, 4>(a, w, bias, act, out, ldo, groups, st);
+  if ((long long)a.blocks * w.blocks >= 16 * 256)
+    return mx_tile_launch<T, 2, 2>(a, w, bias, act, out, ldo, groups, st);
+  return mx_tile_launch<T, 1, 1>(a, w, bias, act, out, ldo, groups, st);
 }
 
 static int mx_check_product(const char* what, const void* a_codes, const void* a_scales,
@@ -286,17 +437,12 @@ extern "C" int t2t_mxfp4_product(const void* a_codes, const void* a_scales, cons
   if (rc != T2T_OK || M == 0) return rc;
   const MxMat a{(const char*)a_codes, (const uint32_t*)a_scales, M, (int)mx_row_blocks(M)};
   const MxMat w{(const char*)w_codes, (const uint32_t*)w_scales, N, (int)mx_row_blocks(N)};
-  const long long tiles = (long long)a.blocks * w.blocks;
-  const long long wgs = (tiles + 3) / 4;
-  T2T_REQUIRE(wgs <= INT_MAX, "mxfp4_product: M=%d N=%d", M, N);
+  const int groups = mx_kp(K) / 256;
   if (dtype == T2T_BF16)
-    hipLaunchKernelGGL(mx_linear_kernel<BF16T>, dim3((unsigned)wgs), dim3(256), 0, (hipStream_t)stream, a,
-                       w, (const uint16_t*)bias, act, (uint16_t*)out, out_row_stride, mx_kp(K) / 256, tiles);
-  else
-    hipLaunchKernelGGL(mx_linear_kernel<F16T>, dim3((unsigned)wgs), dim3(256), 0, (hipStream_t)stream, a,
-                       w, (const uint16_t*)bias, act, (uint16_t*)out, out_row_stride, mx_kp(K) / 256, tiles);
-  T2T_LAUNCH_CHECK("mxfp4_product");
-  return T2T_OK;
+    return mx_product<BF16T>(a, w, (const uint16_t*)bias, act, (uint16_t*)out, out_row_stride, groups,
+                             (hipStream_t)stream);
+  return mx_product<F16T>(a, w, (const uint16_t*)bias, act, (uint16_t*)out, out_row_stride, groups,
+                          (hipStream_t)stream);
 }
 
 // codes, then scales
