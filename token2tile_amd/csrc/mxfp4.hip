@@ -241,6 +241,70 @@ template <int TW, int TA> struct MxTile {
   static constexpr int STAGE = CODES + SCALES > 4 * 32 * PITCH ? CODES + SCALES : 4 * 32 * PITCH;
 };
 
+// Consecutive work-groups go to the eight XCDs in turn: each takes a run of
+// tiles, eight token tiles by all feature tiles, so that the 32 tiles an XCD
+// has under way share their panels in its L2.  -> first row blocks
+__device__ inline bool mx_place(int mt, int nt, int per_xcd, int mb, int nb, int& m0, int& n0) {
+  const int id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  if (id >= mt * nt) return false;
+  const int grp = id / (8 * nt), in = id - grp * 8 * nt;
+  const int gm = min(8, mt - grp * 8);
+  m0 = (grp * 8 + in % gm) * mb;
+  n0 = (in / gm) * nb;
+  return true;
+}
+
+// the sums start at the bias
+template <typename T, int TW, int TA>
+__device__ inline void mx_bias_init(f32x16 (&acc)[TW][TA], const uint16_t* __restrict__ bias, int f0, int rows) {
+  const int hh = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int i = 0; i < TW; ++i) {
+    f32x16 b0 = zero16();
+    if (bias)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        b0[e] = T::to_f(bias[min(f0 + 32 * i + 8 * (e >> 2) + 4 * hh + (e & 3), rows - 1)]);
+#pragma unroll
+    for (int j = 0; j < TA; ++j) acc[i][j] = b0;
+  }
+}
+
+// 32 tokens at a time through a staging area of the wave's own, then whole rows: a wave's 32 TA
+// tokens from m on, 32 TW features from n on
+template <typename T, int TW, int TA, bool GELU>
+__device__ inline void mx_store(const f32x16 (&acc)[TW][TA], char* so, uint16_t* __restrict__ out,
+                                long long ldo, int vec, int m, int M, int n, int N) {
+  constexpr int PITCH = 64 * TW + 16, LR = 4 * TW;  // lanes per row, 8 features each
+  const int lane = threadIdx.x & 63, hh = lane >> 5;
+  const int f0 = n + (lane % LR) * 8;
+  const bool whole = vec && f0 + 8 <= N;
+#pragma unroll
+  for (int j = 0; j < TA; ++j) {
+#pragma unroll
+    for (int i = 0; i < TW; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = GELU ? mx_gelu(acc[i][j][4 * q + e]) : acc[i][j][4 * q + e];
+        *(u32x2*)(so + (lane & 31) * PITCH + (32 * i + 8 * q + 4 * hh) * 2) =
+            u32x2{Pk<T>::pack(v[0], v[1]), Pk<T>::pack(v[2], v[3])};
+      }
+#pragma unroll 1
+    for (int t = lane / LR; t < 32 && m + 32 * j + t < M; t += 64 / LR) {
+      const u32x4 v = *(const u32x4*)(so + t * PITCH + (lane % LR) * 16);
+      uint16_t* o = out + (long long)(m + 32 * j + t) * ldo + f0;
+      if (whole)
+        *(u32x4*)o = v;
+      else
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (f0 + e < N) o[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+    }
+  }
+}
+
 template <typename T, int TW, int TA, bool GELU>
 __global__ __launch_bounds__(256, TW * TA >= 16 ? 1 : 2) void mx_tile_kernel(
     MxMat a, MxMat w, const uint16_t* __restrict__ bias, uint16_t* __restrict__ out, long long ldo, int vec,
@@ -250,17 +314,10 @@ __global__ __launch_bounds__(256, TW * TA >= 16 ? 1 : 2) void mx_tile_kernel(
   __shared__ __attribute__((aligned(1024))) char st1[C::STAGE];
   __shared__ __attribute__((aligned(1024))) char st2[C::STAGE];
   __shared__ __attribute__((aligned(1024))) char st3[C::STAGE];
-  // consecutive work-groups go to the eight XCDs in turn: each takes a run of
-  // tiles, eight token tiles by all feature tiles, so that the 32 tiles an XCD
-  // has under way share their panels in its L2
-  const int id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-  if (id >= mt * nt) return;
-  const int grp = id / (8 * nt), in = id - grp * 8 * nt;
-  const int gm = min(8, mt - grp * 8);
-  const int m0 = (grp * 8 + in % gm) * 2 * TA, n0 = (in / gm) * 2 * TW;  // row blocks
-
+  int m0, n0;
+  if (!mx_place(mt, nt, per_xcd, 2 * TA, 2 * TW, m0, n0)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wn = wave & 1, wm = wave >> 1, hh = lane >> 5;
+  const int wn = wave & 1, wm = wave >> 1;
   // this wave's share of the stage's DMA: TW + TA KB of codes, and 1 KB of scales (four row
   // blocks; with fewer than sixteen some waves fetch the same)
   const char* src[TW + TA];
@@ -290,16 +347,7 @@ __global__ __launch_bounds__(256, TW * TA >= 16 ? 1 : 2) void mx_tile_kernel(
                                        (mx_lds_t*)(st + C::CODES + (wave % SI) * 1024), 16, 0, 0);
   };
   f32x16 acc[TW][TA];
-#pragma unroll
-  for (int i = 0; i < TW; ++i) {
-    f32x16 b0 = zero16();
-    if (bias)
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        b0[e] = T::to_f(bias[min((n0 + wn * TW + i) * 32 + 8 * (e >> 2) + 4 * hh + (e & 3), w.rows - 1)]);
-#pragma unroll
-    for (int j = 0; j < TA; ++j) acc[i][j] = b0;
-  }
+  mx_bias_init<T, TW, TA>(acc, bias, (n0 + wn * TW) * 32, w.rows);
   u32x4 fw[2][TW], fa[2][TA];
   uint32_t sw[TW], sa[TA];
   auto frags = [&](const char* st, int c) {
@@ -354,37 +402,210 @@ __global__ __launch_bounds__(256, TW * TA >= 16 ? 1 : 2) void mx_tile_kernel(
     if (s + 4 >= n) break;
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-  // epilogue: 32 tokens at a time through a staging area of the wave's own, then whole rows
-  char* so = st0 + wave * 32 * C::PITCH;
-  constexpr int LR = 4 * TW;  // lanes per row, 8 features each
-  const int f0 = (n0 + wn * TW) * 32 + (lane % LR) * 8;
-  const bool whole = vec && f0 + 8 <= w.rows;
-#pragma unroll
-  for (int j = 0; j < TA; ++j) {
-#pragma unroll
-    for (int i = 0; i < TW; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = GELU ? mx_gelu(acc[i][j][4 * q + e]) : acc[i][j][4 * q + e];
-        *(u32x2*)(so + (lane & 31) * C::PITCH + (32 * i + 8 * q + 4 * hh) * 2) =
-            u32x2{Pk<T>::pack(v[0], v[1]), Pk<T>::pack(v[2], v[3])};
-      }
-    const int mb = (m0 + wm * TA + j) * 32;
-#pragma unroll 1
-    for (int t = lane / LR; t < 32 && mb + t < a.rows; t += 64 / LR) {
-      const u32x4 v = *(const u32x4*)(so + t * C::PITCH + (lane % LR) * 16);
-      uint16_t* o = out + (long long)(mb + t) * ldo + f0;
-      if (whole)
-        *(u32x4*)o = v;
-      else
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (f0 + e < w.rows) o[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
-    }
-  }
+  mx_store<T, TW, TA, GELU>(acc, st0 + wave * 32 * C::PITCH, out, ldo, vec, (m0 + wm * TA) * 32, a.rows,
+                            (n0 + wn * TW) * 32, w.rows);
 }
+
+// ---- the 256 x 256 tile: its inner loop is written out ----------------------
+// With 256 accumulators a SIMD holds one wave, so no other wave covers a wait,
+// and left to itself the compiler issues a fragment read right before the
+// product that needs it.  A step is one asm block of sixteen products (64
+// columns): the next step's eight fragment reads go between the first eight,
+// the stage's DMA between the others, and the one wait at its end finds the
+// reads 256 cycles old.
+#define MX_P(i, j)                                                                                      \
+  "v_mfma_scale_f32_32x32x64_f8f6f4 %[c" #i #j "], %[w" #i "], %[a" #j "], %[c" #i #j "], %[p" #i     \
+  "], %[q" #j "] " MX_SEL " cbsz:4 blgp:4\n\t"
+#define MX_R(d, base, o) "ds_read_b128 %[" d "], %[" base "] offset:%c[" o "]\n\t"
+#define MX_RS(d, base, o) "ds_read_b32 %[" d "], %[" base "] offset:%c[" o "]\n\t"
+// 1 KB (16 bytes a lane) to LDS at m0, which moves on
+#define MX_D(i) "global_load_lds_dwordx4 %[v], %[g" #i "]\n\ts_add_u32 m0, m0, 0x400\n\t"
+#define MX_ACC                                                                                          \
+  [c00] "+a"(acc[0][0]), [c01] "+a"(acc[0][1]), [c02] "+a"(acc[0][2]), [c03] "+a"(acc[0][3]),           \
+      [c10] "+a"(acc[1][0]), [c11] "+a"(acc[1][1]), [c12] "+a"(acc[1][2]), [c13] "+a"(acc[1][3]),       \
+      [c20] "+a"(acc[2][0]), [c21] "+a"(acc[2][1]), [c22] "+a"(acc[2][2]), [c23] "+a"(acc[2][3]),       \
+      [c30] "+a"(acc[3][0]), [c31] "+a"(acc[3][1]), [c32] "+a"(acc[3][2]), [c33] "+a"(acc[3][3])
+#define MX_NEXT(f)                                                                                      \
+  [x0] "=&v"(f.w[0]), [x1] "=&v"(f.w[1]), [x2] "=&v"(f.w[2]), [x3] "=&v"(f.w[3]), [y0] "=&v"(f.a[0]),   \
+      [y1] "=&v"(f.a[1]), [y2] "=&v"(f.a[2]), [y3] "=&v"(f.a[3])
+#define MX_CUR(f, sc)                                                                                   \
+  [w0] "v"(f.w[0]), [w1] "v"(f.w[1]), [w2] "v"(f.w[2]), [w3] "v"(f.w[3]), [a0] "v"(f.a[0]),             \
+      [a1] "v"(f.a[1]), [a2] "v"(f.a[2]), [a3] "v"(f.a[3]), [p0] "v"(sc.w[0]), [p1] "v"(sc.w[1]),       \
+      [p2] "v"(sc.w[2]), [p3] "v"(sc.w[3]), [q0] "v"(sc.a[0]), [q1] "v"(sc.a[1]), [q2] "v"(sc.a[2]),    \
+      [q3] "v"(sc.a[3])
+#define MX_READS(OFF)                                                                                   \
+  [bw] "v"(bw), [ba] "v"(ba), [o0] "n"(OFF), [o1] "n"((OFF) + 2048), [o2] "n"((OFF) + 4096),            \
+      [o3] "n"((OFF) + 6144)
+#define MX_FIRST8                                                                                       \
+  MX_P(0, 0) MX_R("x0", "bw", "o0") MX_P(0, 1) MX_R("y0", "ba", "o0") MX_P(0, 2) MX_R("x1", "bw", "o1") \
+      MX_P(0, 3) MX_R("y1", "ba", "o1") MX_P(1, 0) MX_R("x2", "bw", "o2") MX_P(1, 1)                    \
+          MX_R("y2", "ba", "o2") MX_P(1, 2) MX_R("x3", "bw", "o3") MX_P(1, 3) MX_R("y3", "ba", "o3")
+#define MX_LAST8                                                                                        \
+  MX_P(2, 0) MX_P(2, 1) MX_P(2, 2) MX_P(2, 3) MX_P(3, 0) MX_P(3, 1) MX_P(3, 2) MX_P(3, 3)
+#define MX_LAST8_DMA                                                                                    \
+  MX_P(2, 0) MX_D(0) MX_P(2, 1) MX_D(1) MX_P(2, 2) MX_D(2) MX_P(2, 3) MX_D(3) MX_P(3, 0) MX_D(4)        \
+      MX_P(3, 1) MX_D(5) MX_P(3, 2) MX_D(6) MX_P(3, 3) MX_D(7)
+
+struct MxFrags {
+  u32x4 w[4], a[4];
+};
+struct MxScales {
+  uint32_t w[4], a[4];
+};
+struct MxDma {
+  const char* g[8];     // this wave's eight KB of a stage, at stage 0
+  const char* scales;   // its KB of scales, per lane
+  uint32_t lds, lds_scales;
+};
+
+// first step of a stage: reads the stage's second fragments at OFF
+template <int ODD, int OFF>
+__device__ inline void mx_step0(f32x16 (&acc)[4][4], const MxFrags& f, MxFrags& nx, const MxScales& sc,
+                                uint32_t bw, uint32_t ba) {
+#define MX_BODY "s_nop 1\n\t" MX_FIRST8 MX_LAST8 "s_waitcnt lgkmcnt(0)"
+  if constexpr (!ODD) {
+#define MX_SEL "op_sel:[0,0,0] op_sel_hi:[0,0,0]"
+    asm volatile(MX_BODY : MX_ACC, MX_NEXT(nx) : MX_CUR(f, sc), MX_READS(OFF) : "memory");
+#undef MX_SEL
+  } else {
+#define MX_SEL "op_sel:[0,0,0] op_sel_hi:[1,1,0]"
+    asm volatile(MX_BODY : MX_ACC, MX_NEXT(nx) : MX_CUR(f, sc), MX_READS(OFF) : "memory");
+#undef MX_SEL
+  }
+#undef MX_BODY
+}
+
+// second step of a stage: once the next stage has landed for every wave (the two after it may
+// be under way) and this one's reads are done, reads the next stage's first fragments at OFF
+// (after an odd stage also the next group's scales at SOFF) and fetches the stage four further
+// on into this one's place (v: its column offset; before an even one also scales)
+template <int ODD, int OFF, int SOFF>
+__device__ inline void mx_step1(f32x16 (&acc)[4][4], const MxFrags& f, MxFrags& nx, const MxScales& sc,
+                                MxScales& nsc, uint32_t bw, uint32_t ba, uint32_t sbw, uint32_t sba,
+                                const MxDma& d, uint32_t lds, uint32_t lds_scales, uint32_t v,
+                                const char* scales) {
+#define MX_DMA_IN                                                                                       \
+  [v] "v"(v), [m] "s"(lds), [g0] "s"(d.g[0]), [g1] "s"(d.g[1]), [g2] "s"(d.g[2]), [g3] "s"(d.g[3]),     \
+      [g4] "s"(d.g[4]), [g5] "s"(d.g[5]), [g6] "s"(d.g[6]), [g7] "s"(d.g[7])
+  if constexpr (!ODD) {
+#define MX_SEL "op_sel:[1,1,0] op_sel_hi:[0,0,0]"
+    asm volatile("s_mov_b32 m0, %[m]\n\ts_waitcnt vmcnt(17)\n\ts_barrier\n\t" MX_FIRST8 MX_LAST8_DMA
+                 "s_mov_b32 m0, %[ms]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[vs], off\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : MX_ACC, MX_NEXT(nx)
+                 : MX_CUR(f, sc), MX_READS(OFF), MX_DMA_IN, [ms] "s"(lds_scales), [vs] "v"(scales)
+                 : "memory", "scc");
+#undef MX_SEL
+  } else {
+#define MX_SEL "op_sel:[1,1,0] op_sel_hi:[1,1,0]"
+    asm volatile("s_mov_b32 m0, %[m]\n\ts_waitcnt vmcnt(17)\n\ts_barrier\n\t" MX_FIRST8
+                 MX_RS("n0", "sbw", "t0") MX_RS("n1", "sbw", "t1") MX_RS("n2", "sbw", "t2")
+                 MX_RS("n3", "sbw", "t3") MX_RS("r0", "sba", "t0") MX_RS("r1", "sba", "t1")
+                 MX_RS("r2", "sba", "t2") MX_RS("r3", "sba", "t3") MX_LAST8_DMA "s_waitcnt lgkmcnt(0)"
+                 : MX_ACC, MX_NEXT(nx), [n0] "=&v"(nsc.w[0]), [n1] "=&v"(nsc.w[1]), [n2] "=&v"(nsc.w[2]),
+                   [n3] "=&v"(nsc.w[3]), [r0] "=&v"(nsc.a[0]), [r1] "=&v"(nsc.a[1]), [r2] "=&v"(nsc.a[2]),
+                   [r3] "=&v"(nsc.a[3])
+                 : MX_CUR(f, sc), MX_READS(OFF), MX_DMA_IN, [sbw] "v"(sbw), [sba] "v"(sba), [t0] "n"(SOFF),
+                   [t1] "n"(SOFF + 256), [t2] "n"(SOFF + 512), [t3] "n"(SOFF + 768)
+                 : "memory", "scc");
+#undef MX_SEL
+  }
+#undef MX_DMA_IN
+}
+
+template <typename T, bool GELU>
+__global__ __launch_bounds__(256, 1) void mx_big_kernel(MxMat a, MxMat w, const uint16_t* __restrict__ bias,
+                                                        uint16_t* __restrict__ out, long long ldo, int vec,
+                                                        int groups, int mt, int nt, int per_xcd) {
+  using C = MxTile<4, 4>;
+  static_assert(C::STAGE + 8192 < 65536 && C::CODES + 1024 < 65536, "LDS offsets of 16 bits");
+  __shared__ __attribute__((aligned(1024))) char lds[4 * C::STAGE];
+  int m0, n0;
+  if (!mx_place(mt, nt, per_xcd, 8, 8, m0, n0)) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wn = wave & 1, wm = wave >> 1;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(mx_lds_t*)lds;
+  MxDma d;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int rb = wave * 4 + (i >> 1);
+    const long long row = rb < 8 ? min(n0 + rb, w.blocks - 1) : min(m0 + rb - 8, a.blocks - 1);
+    d.g[i] = (rb < 8 ? w.codes : a.codes) + row * groups * 4096 + (i & 1) * 1024;
+  }
+  {
+    const int rb = 4 * wave + (lane >> 4);
+    const long long row = rb < 8 ? min(n0 + rb, w.blocks - 1) : min(m0 + rb - 8, a.blocks - 1);
+    d.scales = (const char*)(rb < 8 ? w.scales : a.scales) + row * groups * 256 + (lane & 15) * 16;
+  }
+  d.lds = lds0 + wave * 8192;
+  d.lds_scales = lds0 + C::CODES + wave * 1024;
+  const int n = 2 * groups;
+  const uint32_t l16 = lane * 16;
+  // the column offset of stage s; past the last stage every lane reads the same line of it, so
+  // that the counts of loads in flight stay what they are
+  auto col = [&](int s, int odd) { return (uint32_t)min(s, n - 2 + odd) * 2048 + (s < n ? l16 : 0); };
+  auto issue = [&](int s, int odd) {
+    const uint32_t v = col(s, odd);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[v], %[g]" ::[m] "s"(
+                       d.lds + s * C::STAGE + i * 1024),
+                   [v] "v"(v), [g] "s"(d.g[i])
+                   : "memory");
+    if (!odd)
+      asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[v], off" ::[m] "s"(
+                       d.lds_scales + s * C::STAGE),
+                   [v] "v"(d.scales + (size_t)(min(s, n - 2) >> 1) * 256)
+                   : "memory");
+  };
+  f32x16 acc[4][4];
+  mx_bias_init<T, 4, 4>(acc, bias, (n0 + wn * 4) * 32, w.rows);
+  issue(0, 0);
+  issue(1, 1);
+  issue(2, 0);
+  issue(3, 1);
+  // fragment and scale addresses of stages 0, 1 and of stages 2, 3
+  const uint32_t bw0 = lds0 + wn * 8192 + l16, ba0 = lds0 + 16384 + wm * 8192 + l16;
+  const uint32_t sw0 = lds0 + wn * 1024 + lane * 4, sa0 = lds0 + 2048 + wm * 1024 + lane * 4;
+  const uint32_t bw2 = bw0 + 2 * C::STAGE, ba2 = ba0 + 2 * C::STAGE;
+  const uint32_t sw2 = sw0 + 2 * C::STAGE, sa2 = sa0 + 2 * C::STAGE;
+  MxFrags f0, f1;
+  MxScales s0, s2;
+  asm volatile("s_waitcnt vmcnt(25)\n\ts_barrier\n\t" MX_R("x0", "bw", "o0") MX_R("y0", "ba", "o0")
+               MX_R("x1", "bw", "o1") MX_R("y1", "ba", "o1") MX_R("x2", "bw", "o2") MX_R("y2", "ba", "o2")
+               MX_R("x3", "bw", "o3") MX_R("y3", "ba", "o3") MX_RS("n0", "sbw", "t0") MX_RS("n1", "sbw", "t1")
+               MX_RS("n2", "sbw", "t2") MX_RS("n3", "sbw", "t3") MX_RS("r0", "sba", "t0")
+               MX_RS("r1", "sba", "t1") MX_RS("r2", "sba", "t2") MX_RS("r3", "sba", "t3")
+               "s_waitcnt lgkmcnt(0)"
+               : MX_NEXT(f0), [n0] "=&v"(s0.w[0]), [n1] "=&v"(s0.w[1]), [n2] "=&v"(s0.w[2]),
+                 [n3] "=&v"(s0.w[3]), [r0] "=&v"(s0.a[0]), [r1] "=&v"(s0.a[1]), [r2] "=&v"(s0.a[2]),
+                 [r3] "=&v"(s0.a[3])
+               : [bw] "v"(bw0), [ba] "v"(ba0), [o0] "n"(0), [o1] "n"(2048), [o2] "n"(4096), [o3] "n"(6144),
+                 [sbw] "v"(sw0), [sba] "v"(sa0), [t0] "n"(C::CODES), [t1] "n"(C::CODES + 256),
+                 [t2] "n"(C::CODES + 512), [t3] "n"(C::CODES + 768)
+               : "memory");
+  constexpr int ST = C::STAGE;
+  for (int s = 0;; s += 4) {
+    const char* sp = d.scales + (size_t)(min(s + 4, n - 2) >> 1) * 256;
+    mx_step0<0, 1024>(acc, f0, f1, s0, bw0, ba0);
+    mx_step1<0, ST, 0>(acc, f1, f0, s0, s2, bw0, ba0, sw2, sa2, d, d.lds, d.lds_scales, col(s + 4, 0), sp);
+    mx_step0<1, ST + 1024>(acc, f0, f1, s0, bw0, ba0);
+    mx_step1<1, 0, C::CODES>(acc, f1, f0, s0, s2, bw2, ba2, sw2, sa2, d, d.lds + ST, 0, col(s + 5, 1), sp);
+    if (s + 2 >= n) break;
+    sp = d.scales + (size_t)(min(s + 6, n - 2) >> 1) * 256;
+    mx_step0<0, 1024>(acc, f0, f1, s2, bw2, ba2);
+    mx_step1<0, ST, 0>(acc, f1, f0, s2, s0, bw2, ba2, sw0, sa0, d, d.lds + 2 * ST, d.lds_scales + 2 * ST,
+                       col(s + 6, 0), sp);
+    mx_step0<1, ST + 1024>(acc, f0, f1, s2, bw2, ba2);
+    mx_step1<1, 0, C::CODES>(acc, f1, f0, s2, s0, bw0, ba0, sw0, sa0, d, d.lds + 3 * ST, 0, col(s + 7, 1), sp);
+    if (s + 4 >= n) break;
+  }
+  // the last products' registers are readable after 18 cycles of issue
+  asm volatile("s_nop 15\n\ts_nop 15\n\ts_waitcnt vmcnt(0)\n\ts_barrier" : MX_ACC : : "memory");
+  mx_store<T, 4, 4, GELU>(acc, lds + wave * 32 * C::PITCH, out, ldo, vec, (m0 + wm * 4) * 32, a.rows,
+                          (n0 + wn * 4) * 32, w.rows);
+}
+// ---- end of the 256 x 256 tile
 
 template <typename T, int TW, int TA>
 static int mx_tile_launch(const MxMat& a, const MxMat& w, const uint16_t* bias, int act, uint16_t* out,
@@ -394,12 +615,9 @@ static int mx_tile_launch(const MxMat& a, const MxMat& w, const uint16_t* bias, 
   T2T_REQUIRE(tiles <= INT_MAX / 2, "mxfp4_product: M=%d N=%d", a.rows, w.rows);
   const int per = cdiv(tiles, 8);
   const int vec = ldo % 8 == 0 && (uintptr_t)out % 16 == 0;
-  if (act == T2T_ACT_GELU_TANH)
-    hipLaunchKernelGGL((mx_tile_kernel<T, TW, TA, true>), dim3(8 * per), dim3(256), 0, st, a, w, bias, out,
-                       ldo, vec, groups, mt, nt, per);
-  else
-    hipLaunchKernelGGL((mx_tile_kernel<T, TW, TA, false>), dim3(8 * per), dim3(256), 0, st, a, w, bias, out,
-                       ldo, vec, groups, mt, nt, per);
+  auto kernel = act == T2T_ACT_GELU_TANH ? mx_tile_kernel<T, TW, TA, true> : mx_tile_kernel<T, TW, TA, false>;
+  if constexpr (TW * TA == 16) kernel = act == T2T_ACT_GELU_TANH ? mx_big_kernel<T, true> : mx_big_kernel<T, false>;
+  hipLaunchKernelGGL(kernel, dim3(8 * per), dim3(256), 0, st, a, w, bias, out, ldo, vec, groups, mt, nt, per);
   T2T_LAUNCH_CHECK("mxfp4_product");
   return T2T_OK;
 }
@@ -419,7 +637,8 @@ static int mx_check_product(const char* what, const void* a_codes, const void* a
                             long long out_row_stride, int M, int N, int K) {
   T2T_REQUIRE(dtype == T2T_F16 || dtype == T2T_BF16, "%s: dtype %d", what, dtype);
   T2T_REQUIRE(act == T2T_ACT_NONE || act == T2T_ACT_GELU_TANH, "%s: activation %d", what, act);
-  T2T_REQUIRE(M >= 0 && N >= 1 && K >= 32 && K % 32 == 0, "%s: M=%d N=%d K=%d (K a multiple of 32)", what, M,
+  T2T_REQUIRE(M >= 0 && N >= 1 && K >= 32 && K % 32 == 0 && K <= (1 << 27),
+              "%s: M=%d N=%d K=%d (K a multiple of 32, at most 2^27)", what, M,
               N, K);
   if (M == 0) return T2T_OK;
   T2T_REQUIRE(a_codes && a_scales && w_codes && w_scales && out, "%s: null pointer", what);
