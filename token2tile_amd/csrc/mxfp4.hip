@@ -211,10 +211,11 @@ __device__ inline f32x16 mx_mfma(const u32x4& a, const u32x4& b, const f32x16& c
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, c, 4, 4, S, (int)sa, S, (int)sb);
 }
 
-// gelu(x) = x / 2 (1 + tanh u) = x / (1 + e^(-2 u)), u = sqrt(2 / pi) (x + 0.044715 x^3)
+// gelu(x) = x / 2 (1 + tanh u) = x / (1 + e^(-2 u)), u = sqrt(2 / pi) (x + 0.044715 x^3), with the
+// constants of e^(-2 u) = 2^(x (c0 + c1 x^2)).  v_exp_f32 and v_rcp_f32 are within 1 ulp.
 __device__ inline float mx_gelu(float x) {
-  const float u2 = 1.5957691216057308f * x * (1.f + 0.044715f * x * x);
-  return x / (1.f + __expf(-u2));
+  const float z = x * __builtin_fmaf(-0.10294324f, x * x, -2.3022082f);
+  return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z));
 }
 
 struct MxMat {
@@ -243,28 +244,38 @@ template <int TW, int TA> struct MxTile {
 
 // Consecutive work-groups go to the eight XCDs in turn: each takes a run of
 // tiles, eight token tiles by all feature tiles, so that the 32 tiles an XCD
-// has under way share their panels in its L2.  -> first row blocks
-__device__ inline bool mx_place(int mt, int nt, int per_xcd, int mb, int nb, int& m0, int& n0) {
-  const int id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-  if (id >= mt * nt) return false;
+// has under way share their panels in its L2.
+__device__ inline int mx_first(int per_xcd) { return (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3); }
+__device__ inline int mx_end(int mt, int nt, int per_xcd) {
+  return min(mt * nt, ((int)(blockIdx.x & 7) + 1) * per_xcd);
+}
+// a tile's first row blocks
+__device__ inline void mx_place(int id, int mt, int nt, int mb, int nb, int& m0, int& n0) {
   const int grp = id / (8 * nt), in = id - grp * 8 * nt;
   const int gm = min(8, mt - grp * 8);
   m0 = (grp * 8 + in % gm) * mb;
   n0 = (in / gm) * nb;
-  return true;
 }
 
-// the sums start at the bias
+// the sums start at the bias, which comes through LDS of the wave's own (128 TW bytes): a lane
+// needs 16 TW of the wave's 32 TW features
 template <typename T, int TW, int TA>
-__device__ inline void mx_bias_init(f32x16 (&acc)[TW][TA], const uint16_t* __restrict__ bias, int f0, int rows) {
-  const int hh = (threadIdx.x >> 5) & 1;
+__device__ inline void mx_bias_init(f32x16 (&acc)[TW][TA], const uint16_t* __restrict__ bias, float* own,
+                                    int f0, int rows) {
+  const int lane = threadIdx.x & 63, hh = lane >> 5;
+  if (bias)
+#pragma unroll
+    for (int i = lane; i < 32 * TW; i += 64) own[i] = T::to_f(bias[min(f0 + i, rows - 1)]);
 #pragma unroll
   for (int i = 0; i < TW; ++i) {
     f32x16 b0 = zero16();
     if (bias)
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        b0[e] = T::to_f(bias[min(f0 + 32 * i + 8 * (e >> 2) + 4 * hh + (e & 3), rows - 1)]);
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 v = *(const f32x4*)(own + 32 * i + 8 * q + 4 * hh);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b0[4 * q + e] = v[e];
+      }
 #pragma unroll
     for (int j = 0; j < TA; ++j) acc[i][j] = b0;
   }
@@ -305,6 +316,52 @@ __device__ inline void mx_store(const f32x16 (&acc)[TW][TA], char* so, uint16_t*
   }
 }
 
+// the same through 4 KB: 32 tokens x 64 features at a time, 16-byte chunk c of token t at
+// c ^ (t & 7)
+template <typename T, bool GELU>
+__device__ inline void mx_store_big(const f32x16 (&acc)[4][4], char* so, uint16_t* __restrict__ out,
+                                    long long ldo, int vec, int m, int M, int n, int N) {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // (or its addresses are kept in registers through the products)
+  const int hh = lane >> 5, c = lane & 7;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int ii = 0; ii < 4; ii += 2) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            v[e] = GELU ? mx_gelu(acc[ii + i][j][4 * q + e]) : acc[ii + i][j][4 * q + e];
+          *(u32x2*)(so + (lane & 31) * 128 + (((4 * i + q) ^ (lane & 7)) * 16) + 8 * hh) =
+              u32x2{Pk<T>::pack(v[0], v[1]), Pk<T>::pack(v[2], v[3])};
+        }
+      const int f0 = n + 32 * ii + 8 * c;
+      if (vec && f0 + 8 <= N) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int t = 8 * r + (lane >> 3);
+          if (m + 32 * j + t < M)
+            *(u32x4*)(out + (long long)(m + 32 * j + t) * ldo + f0) =
+                *(const u32x4*)(so + t * 128 + ((c ^ (t & 7)) * 16));
+        }
+      } else {
+#pragma unroll 1
+        for (int t = lane >> 3; t < 32 && m + 32 * j + t < M; t += 8) {
+          const u32x4 v = *(const u32x4*)(so + t * 128 + ((c ^ (t & 7)) * 16));
+          uint16_t* o = out + (long long)(m + 32 * j + t) * ldo + f0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (f0 + e < N) o[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+        }
+      }
+    }
+}
+
 template <typename T, int TW, int TA, bool GELU>
 __global__ __launch_bounds__(256, TW * TA >= 16 ? 1 : 2) void mx_tile_kernel(
     MxMat a, MxMat w, const uint16_t* __restrict__ bias, uint16_t* __restrict__ out, long long ldo, int vec,
@@ -314,8 +371,10 @@ __global__ __launch_bounds__(256, TW * TA >= 16 ? 1 : 2) void mx_tile_kernel(
   __shared__ __attribute__((aligned(1024))) char st1[C::STAGE];
   __shared__ __attribute__((aligned(1024))) char st2[C::STAGE];
   __shared__ __attribute__((aligned(1024))) char st3[C::STAGE];
+  const int id = mx_first(per_xcd);
+  if (id >= mx_end(mt, nt, per_xcd)) return;
   int m0, n0;
-  if (!mx_place(mt, nt, per_xcd, 2 * TA, 2 * TW, m0, n0)) return;
+  mx_place(id, mt, nt, 2 * TA, 2 * TW, m0, n0);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wn = wave & 1, wm = wave >> 1;
   // this wave's share of the stage's DMA: TW + TA KB of codes, and 1 KB of scales (four row
@@ -347,7 +406,8 @@ __global__ __launch_bounds__(256, TW * TA >= 16 ? 1 : 2) void mx_tile_kernel(
                                        (mx_lds_t*)(st + C::CODES + (wave % SI) * 1024), 16, 0, 0);
   };
   f32x16 acc[TW][TA];
-  mx_bias_init<T, TW, TA>(acc, bias, (n0 + wn * TW) * 32, w.rows);
+  mx_bias_init<T>(acc, bias, (float*)(st3 + wave * 128 * TW), (n0 + wn * TW) * 32, w.rows);
+  __syncthreads();
   u32x4 fw[2][TW], fa[2][TA];
   uint32_t sw[TW], sa[TA];
   auto frags = [&](const char* st, int c) {
@@ -453,9 +513,8 @@ struct MxScales {
   uint32_t w[4], a[4];
 };
 struct MxDma {
-  const char* g[8];     // this wave's eight KB of a stage, at stage 0
-  const char* scales;   // its KB of scales, per lane
-  uint32_t lds, lds_scales;
+  const char* g[8];    // this wave's eight KB of a stage, at stage 0
+  const char* scales;  // its KB of scales, per lane
 };
 
 // first step of a stage: reads the stage's second fragments at OFF
@@ -513,97 +572,119 @@ __device__ inline void mx_step1(f32x16 (&acc)[4][4], const MxFrags& f, MxFrags& 
 #undef MX_DMA_IN
 }
 
+// Work-groups stay for many tiles.  The DMA runs four stages ahead of the
+// products as one stream over all of them, so a tile's first stages are loaded
+// under the last products and the epilogue of the one before; the epilogue has
+// LDS of its own (4 KB a wave).
 template <typename T, bool GELU>
 __global__ __launch_bounds__(256, 1) void mx_big_kernel(MxMat a, MxMat w, const uint16_t* __restrict__ bias,
                                                         uint16_t* __restrict__ out, long long ldo, int vec,
                                                         int groups, int mt, int nt, int per_xcd) {
   using C = MxTile<4, 4>;
-  static_assert(C::STAGE + 8192 < 65536 && C::CODES + 1024 < 65536, "LDS offsets of 16 bits");
-  __shared__ __attribute__((aligned(1024))) char lds[4 * C::STAGE];
-  int m0, n0;
-  if (!mx_place(mt, nt, per_xcd, 8, 8, m0, n0)) return;
+  constexpr int ST = C::CODES + C::SCALES, PAIR = 2 * ST;
+  static_assert(ST + 8192 < 65536 && C::CODES + 1024 < 65536, "LDS offsets of 16 bits");
+  __shared__ __attribute__((aligned(1024))) char lds[4 * ST + 4 * 4096];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wn = wave & 1, wm = wave >> 1;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(mx_lds_t*)lds;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(mx_lds_t*)lds, l16 = lane * 16;
+  const int n = 2 * groups, step = gridDim.x >> 3;
+  int id = mx_first(per_xcd);
+  const int end = mx_end(mt, nt, per_xcd);
+  if (id >= end) return;
+
+  // the stream of stages: tile ld, its stage ls
   MxDma d;
+  int ld = id, ls = 0;
+  auto aim = [&]() {
+    int m0, n0;
+    mx_place(ld, mt, nt, 8, 8, m0, n0);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int rb = wave * 4 + (i >> 1);
-    const long long row = rb < 8 ? min(n0 + rb, w.blocks - 1) : min(m0 + rb - 8, a.blocks - 1);
-    d.g[i] = (rb < 8 ? w.codes : a.codes) + row * groups * 4096 + (i & 1) * 1024;
-  }
-  {
+    for (int i = 0; i < 8; ++i) {
+      const int rb = wave * 4 + (i >> 1);
+      const long long row = rb < 8 ? min(n0 + rb, w.blocks - 1) : min(m0 + rb - 8, a.blocks - 1);
+      d.g[i] = (rb < 8 ? w.codes : a.codes) + row * groups * 4096 + (i & 1) * 1024;
+    }
     const int rb = 4 * wave + (lane >> 4);
     const long long row = rb < 8 ? min(n0 + rb, w.blocks - 1) : min(m0 + rb - 8, a.blocks - 1);
     d.scales = (const char*)(rb < 8 ? w.scales : a.scales) + row * groups * 256 + (lane & 15) * 16;
-  }
-  d.lds = lds0 + wave * 8192;
-  d.lds_scales = lds0 + C::CODES + wave * 1024;
-  const int n = 2 * groups;
-  const uint32_t l16 = lane * 16;
-  // the column offset of stage s; past the last stage every lane reads the same line of it, so
-  // that the counts of loads in flight stay what they are
-  auto col = [&](int s, int odd) { return (uint32_t)min(s, n - 2 + odd) * 2048 + (s < n ? l16 : 0); };
-  auto issue = [&](int s, int odd) {
-    const uint32_t v = col(s, odd);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[v], %[g]" ::[m] "s"(
-                       d.lds + s * C::STAGE + i * 1024),
-                   [v] "v"(v), [g] "s"(d.g[i])
-                   : "memory");
-    if (!odd)
-      asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[v], off" ::[m] "s"(
-                       d.lds_scales + s * C::STAGE),
-                   [v] "v"(d.scales + (size_t)(min(s, n - 2) >> 1) * 256)
-                   : "memory");
   };
-  f32x16 acc[4][4];
-  mx_bias_init<T, 4, 4>(acc, bias, (n0 + wn * 4) * 32, w.rows);
-  issue(0, 0);
-  issue(1, 1);
-  issue(2, 0);
-  issue(3, 1);
-  // fragment and scale addresses of stages 0, 1 and of stages 2, 3
-  const uint32_t bw0 = lds0 + wn * 8192 + l16, ba0 = lds0 + 16384 + wm * 8192 + l16;
-  const uint32_t sw0 = lds0 + wn * 1024 + lane * 4, sa0 = lds0 + 2048 + wm * 1024 + lane * 4;
-  const uint32_t bw2 = bw0 + 2 * C::STAGE, ba2 = ba0 + 2 * C::STAGE;
-  const uint32_t sw2 = sw0 + 2 * C::STAGE, sa2 = sa0 + 2 * C::STAGE;
+  // column offset of stage ls (+ 1); after the last tile every lane reads one line of its last
+  // stage, so that the counts of loads in flight stay what they are
+  auto col = [&](int odd) { return (uint32_t)(ls + odd) * 2048 + (ld < end ? l16 : 0); };
+  auto next_pair = [&]() {
+    if (ld >= end) return;
+    ls += 2;
+    if (ls < n) return;
+    ld += step;
+    if (ld < end) {
+      ls = 0;
+      aim();
+    } else {
+      ls = n - 2;
+    }
+  };
+  const uint32_t dst = lds0 + wave * 8192, sdst = lds0 + C::CODES + wave * 1024;
+  auto issue_pair = [&](uint32_t off) {  // in the order of the steps below: the scales after the first eight
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[v], %[g]" ::[m] "s"(
+                       dst + off + (i >> 3) * ST + (i & 7) * 1024),
+                   [v] "v"(col(i >> 3)), [g] "s"(d.g[i & 7])
+                   : "memory");
+      if (i == 7)
+        asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[v], off" ::[m] "s"(sdst + off),
+                     [v] "v"(d.scales + (size_t)ls * 128)
+                     : "memory");
+    }
+    next_pair();
+  };
+  aim();
+  issue_pair(0);
+  issue_pair(PAIR);
+  // fragment and scale addresses of the pair in use and of the other one
+  uint32_t bw = lds0 + wn * 8192 + l16, ba = lds0 + 16384 + wm * 8192 + l16;
+  uint32_t sw = lds0 + wn * 1024 + lane * 4, sa = lds0 + 2048 + wm * 1024 + lane * 4;
+  uint32_t off = 0;
   MxFrags f0, f1;
-  MxScales s0, s2;
-  asm volatile("s_waitcnt vmcnt(25)\n\ts_barrier\n\t" MX_R("x0", "bw", "o0") MX_R("y0", "ba", "o0")
+  MxScales sc, nsc;
+  asm volatile("s_waitcnt vmcnt(17)\n\ts_barrier\n\t" MX_R("x0", "bw", "o0") MX_R("y0", "ba", "o0")
                MX_R("x1", "bw", "o1") MX_R("y1", "ba", "o1") MX_R("x2", "bw", "o2") MX_R("y2", "ba", "o2")
                MX_R("x3", "bw", "o3") MX_R("y3", "ba", "o3") MX_RS("n0", "sbw", "t0") MX_RS("n1", "sbw", "t1")
                MX_RS("n2", "sbw", "t2") MX_RS("n3", "sbw", "t3") MX_RS("r0", "sba", "t0")
                MX_RS("r1", "sba", "t1") MX_RS("r2", "sba", "t2") MX_RS("r3", "sba", "t3")
                "s_waitcnt lgkmcnt(0)"
-               : MX_NEXT(f0), [n0] "=&v"(s0.w[0]), [n1] "=&v"(s0.w[1]), [n2] "=&v"(s0.w[2]),
-                 [n3] "=&v"(s0.w[3]), [r0] "=&v"(s0.a[0]), [r1] "=&v"(s0.a[1]), [r2] "=&v"(s0.a[2]),
-                 [r3] "=&v"(s0.a[3])
-               : [bw] "v"(bw0), [ba] "v"(ba0), [o0] "n"(0), [o1] "n"(2048), [o2] "n"(4096), [o3] "n"(6144),
-                 [sbw] "v"(sw0), [sba] "v"(sa0), [t0] "n"(C::CODES), [t1] "n"(C::CODES + 256),
+               : MX_NEXT(f0), [n0] "=&v"(sc.w[0]), [n1] "=&v"(sc.w[1]), [n2] "=&v"(sc.w[2]),
+                 [n3] "=&v"(sc.w[3]), [r0] "=&v"(sc.a[0]), [r1] "=&v"(sc.a[1]), [r2] "=&v"(sc.a[2]),
+                 [r3] "=&v"(sc.a[3])
+               : MX_READS(0), [sbw] "v"(sw), [sba] "v"(sa), [t0] "n"(C::CODES), [t1] "n"(C::CODES + 256),
                  [t2] "n"(C::CODES + 512), [t3] "n"(C::CODES + 768)
                : "memory");
-  constexpr int ST = C::STAGE;
-  for (int s = 0;; s += 4) {
-    const char* sp = d.scales + (size_t)(min(s + 4, n - 2) >> 1) * 256;
-    mx_step0<0, 1024>(acc, f0, f1, s0, bw0, ba0);
-    mx_step1<0, ST, 0>(acc, f1, f0, s0, s2, bw0, ba0, sw2, sa2, d, d.lds, d.lds_scales, col(s + 4, 0), sp);
-    mx_step0<1, ST + 1024>(acc, f0, f1, s0, bw0, ba0);
-    mx_step1<1, 0, C::CODES>(acc, f1, f0, s0, s2, bw2, ba2, sw2, sa2, d, d.lds + ST, 0, col(s + 5, 1), sp);
-    if (s + 2 >= n) break;
-    sp = d.scales + (size_t)(min(s + 6, n - 2) >> 1) * 256;
-    mx_step0<0, 1024>(acc, f0, f1, s2, bw2, ba2);
-    mx_step1<0, ST, 0>(acc, f1, f0, s2, s0, bw2, ba2, sw0, sa0, d, d.lds + 2 * ST, d.lds_scales + 2 * ST,
-                       col(s + 6, 0), sp);
-    mx_step0<1, ST + 1024>(acc, f0, f1, s2, bw2, ba2);
-    mx_step1<1, 0, C::CODES>(acc, f1, f0, s2, s0, bw0, ba0, sw0, sa0, d, d.lds + 3 * ST, 0, col(s + 7, 1), sp);
-    if (s + 4 >= n) break;
+  char* own = lds + 4 * ST + wave * 4096;
+  f32x16 acc[4][4];
+  for (;;) {
+    int m0, n0;
+    mx_place(id, mt, nt, 8, 8, m0, n0);
+    mx_bias_init<T>(acc, bias, (float*)own, (n0 + wn * 4) * 32, w.rows);
+    for (int g = groups; g > 0; --g) {
+      const uint32_t other = PAIR - 2 * off;  // from this pair to the other one (off: 0 or PAIR)
+      mx_step0<0, 1024>(acc, f0, f1, sc, bw, ba);
+      mx_step1<0, ST, 0>(acc, f1, f0, sc, nsc, bw, ba, sw, sa, d, dst + off, sdst + off, col(0),
+                         d.scales + (size_t)ls * 128);
+      mx_step0<1, ST + 1024>(acc, f0, f1, sc, bw, ba);
+      const uint32_t o_bw = bw + other, o_ba = ba + other, o_sw = sw + other, o_sa = sa + other;
+      mx_step1<1, 0, C::CODES>(acc, f1, f0, sc, nsc, o_bw, o_ba, o_sw, o_sa, d, dst + off + ST, 0, col(1),
+                               nullptr);
+      next_pair();
+      sc = nsc;
+      bw = o_bw, ba = o_ba, sw = o_sw, sa = o_sa, off = PAIR - off;
+    }
+    // the last products' registers are readable after 18 cycles of issue
+    asm volatile("s_nop 15\n\ts_nop 15" : MX_ACC);
+    mx_store_big<T, GELU>(acc, own, out, ldo, vec, (m0 + wm * 4) * 32, a.rows, (n0 + wn * 4) * 32, w.rows);
+    id += step;
+    if (id >= end) break;
   }
-  // the last products' registers are readable after 18 cycles of issue
-  asm volatile("s_nop 15\n\ts_nop 15\n\ts_waitcnt vmcnt(0)\n\ts_barrier" : MX_ACC : : "memory");
-  mx_store<T, 4, 4, GELU>(acc, lds + wave * 32 * C::PITCH, out, ldo, vec, (m0 + wm * 4) * 32, a.rows,
-                          (n0 + wn * 4) * 32, w.rows);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 // ---- end of the 256 x 256 tile
 
@@ -617,7 +698,9 @@ static int mx_tile_launch(const MxMat& a, const MxMat& w, const uint16_t* bias, 
   const int vec = ldo % 8 == 0 && (uintptr_t)out % 16 == 0;
   auto kernel = act == T2T_ACT_GELU_TANH ? mx_tile_kernel<T, TW, TA, true> : mx_tile_kernel<T, TW, TA, false>;
   if constexpr (TW * TA == 16) kernel = act == T2T_ACT_GELU_TANH ? mx_big_kernel<T, true> : mx_big_kernel<T, false>;
-  hipLaunchKernelGGL(kernel, dim3(8 * per), dim3(256), 0, st, a, w, bias, out, ldo, vec, groups, mt, nt, per);
+  // the 256 x 256 tile fills a CU: 32 of its work-groups an XCD, which go through the tiles
+  const int slots = TW * TA == 16 && per > 32 ? 32 : per;
+  hipLaunchKernelGGL(kernel, dim3(8 * slots), dim3(256), 0, st, a, w, bias, out, ldo, vec, groups, mt, nt, per);
   T2T_LAUNCH_CHECK("mxfp4_product");
   return T2T_OK;
 }
