@@ -559,7 +559,7 @@ def test_linear_views_and_buffers(dev, M):
     for off, width in ((8, 96), (3, 77)):                        # aligned rows, odd ones
         buf = torch.full((2 * M + 2, width), 5.0, device=dev, dtype=dt)
         out = buf[1:2 * M + 1, off:off + N].unflatten(0, (2, M))
-        ws = torch.empty(ops.size_query("t2t_mxfp4_linear_ws_bytes", 2 * M, N, K), dtype=torch.uint8, device=dev)
+        ws = torch.empty(ops.mxfp4_linear_ws_bytes(2 * M, N, K), dtype=torch.uint8, device=dev)
         assert ops.mxfp4_linear(x, W, b, out=out, ws=ws) is out
         assert torch.equal(out, y)
         out.fill_(5.0)
@@ -673,7 +673,7 @@ def test_the_chain_captured_and_replayed(dev):
     fr = ops.rotary_frequencies(64, device=dev)
     x = _randn(g, N, K).to(dt)
     pos = torch.arange(N, device=dev)
-    ws = torch.empty(ops.size_query("t2t_mxfp4_linear_ws_bytes", N, H * 64, K), dtype=torch.uint8, device=dev)
+    ws = torch.empty(ops.mxfp4_linear_ws_bytes(N, H * 64, K), dtype=torch.uint8, device=dev)
 
     def chain(i):
         cos, sin = ops.rotary_table(pos, fr)

@@ -65,45 +65,232 @@ extern "C" int t2t_rotary_table(const void* positions, int pos_bits, long long T
 
 // ---------------------------------------------------------------------------
 // y = rotate(x rsqrt(mean(x^2) + eps) w), fp32 inside, one rounding at the
-// end.  One work-group of 256 threads per token and tensor (blockIdx.y: q or
-// k); the norm's sums are taken first (over the token's H D values, or one
-// wave per head), then every thread turns pairs.  Any strides, widths and
-// alignment.
+// end.  Bound: one read and one write of every element.
+//
+// A head is cut into units of 16 channels that turn together: with paired
+// halves channels 8 u .. + 7 and R / 2 + 8 u .. + 7, else 16 u .. + 15; unit u
+// reads entries 8 u .. + 7 of the tables in both layouts.  Lane l of a wave
+// holds unit l % L (L: units rounded up to a power of two) of heads l / L, l /
+// L + 64 / L, ...: its entries are read once a token, and the norm's sum over a
+// head is one over L neighbouring lanes.  A token's heads stay in registers
+// (ITS of them a lane) between the sum and the turn.
 // ---------------------------------------------------------------------------
-static __device__ inline float rope_sum64(float v) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
+struct RotaryArgs {
+  const float* cosv;
+  const float* sinv;
+  long long table_batch;  // table rows from one sequence to the next
+  long long tokens;
+  int N, D, R, half;
+  float sign, eps;
+  int units, shift;  // units of a head, log2(L)
+};
+
+// What every form below computes alike, so that a view's result does not depend on the form that its
+// strides take: the turn (one product rounded, one fused), and the norm's sum, fp32 over each eight
+// channels of a head in their order and fp64 over these (no order of which shows in fp32).
+__device__ inline void rope_turn(float a, float e, float c, float s, float& y0, float& y1) {
+  y0 = __builtin_fmaf(a, c, -(e * s));
+  y1 = __builtin_fmaf(a, s, e * c);
+}
+__device__ inline double rope_sum(double v, int lanes) {  // over groups of `lanes` neighbours
+  for (int d = 1; d < lanes; d <<= 1) v += __shfl_xor(v, d, 64);
   return v;
+}
+__device__ inline float rope_squares(const float (&f)[8], int n) {
+  float s = f[0] * f[0];
+#pragma unroll
+  for (int e = 1; e < 8; ++e)
+    if (e < n) s = __builtin_fmaf(f[e], f[e], s);
+  return s;
+}
+__device__ inline float rope_inv(double sum, double one_over_n, float eps) {
+  return rsqrtf((float)(sum * one_over_n) + eps);
+}
+
+template <typename T>
+__device__ inline void rope_unpack(const u32x4& v, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = T::to_f((uint16_t)(v[i] & 0xffff));
+    f[2 * i + 1] = T::to_f((uint16_t)(v[i] >> 16));
+  }
+}
+template <typename T>
+__device__ inline u32x4 rope_pack(const float (&f)[8]) {
+  u32x4 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = Pk<T>::pack(f[2 * i], f[2 * i + 1]);
+  return v;
+}
+
+// WPT waves per token (the heads dealt over them), one wave for the ordinary call; NORM as
+// T2T_NORM_*; heads in rounds of ITS (with the token norm there is one round)
+template <typename T, int NORM, int WPT, int ITS>
+__global__ __launch_bounds__(256) void rotary_kernel(t2t_rotary_tensor q, t2t_rotary_tensor k, RotaryArgs A) {
+  const t2t_rotary_tensor& g = blockIdx.y ? k : q;
+  __shared__ double part[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int L = 1 << A.shift, u = lane & (L - 1);
+  const int wpos = WPT == 1 ? 0 : wave;
+  const int head0 = wpos * (64 >> A.shift) + (lane >> A.shift), hstep = WPT * (64 >> A.shift);
+  // the unit's two halves: where they lie, whether they are there and turn
+  const int tu = A.half ? A.R >> 4 : (A.R + 15) >> 4;  // units that turn
+  const bool pair = A.half && u < tu;
+  const int rest = A.R + 16 * (u - tu);
+  const int c0 = pair ? 8 * u : A.half ? rest : 16 * u;
+  const int c1 = pair ? A.R / 2 + 8 * u : c0 + 8;
+  const bool on0 = u < A.units, on1 = on0 && c1 < A.D;
+  const bool turn0 = on0 && (A.half ? u < tu : c0 < A.R), turn1 = on1 && (A.half ? u < tu : c1 < A.R);
+  const int H = g.heads;
+  const double one_over_n = 1.0 / (NORM == T2T_NORM_TOKEN ? (double)H * A.D : (double)A.D);
+  const uint16_t* w = (const uint16_t*)g.weight;
+  u32x4 wr[ITS][2];  // the token norm's weights, the same for every token
+  if constexpr (NORM == T2T_NORM_TOKEN) {
+#pragma unroll
+    for (int i = 0; i < ITS; ++i) {
+      const int h = head0 + i * hstep;
+      wr[i][0] = wr[i][1] = u32x4{0u, 0u, 0u, 0u};
+      if (on0 && h < H) wr[i][0] = *(const u32x4*)(w + (long long)h * A.D + c0);
+      if (on1 && h < H) wr[i][1] = *(const u32x4*)(w + (long long)h * A.D + c1);
+    }
+  } else if constexpr (NORM == T2T_NORM_HEAD) {
+    wr[0][0] = wr[0][1] = u32x4{0u, 0u, 0u, 0u};
+    if (on0) wr[0][0] = *(const u32x4*)(w + c0);
+    if (on1) wr[0][1] = *(const u32x4*)(w + c1);
+  }
+  constexpr int TPB = 4 / WPT;  // tokens under way in a work-group
+  for (long long tok = (long long)blockIdx.x * TPB + (WPT == 1 ? wave : 0); tok < A.tokens;
+       tok += (long long)gridDim.x * TPB) {
+    const int b = (int)(tok / A.N), n = (int)(tok - (long long)b * A.N);
+    const uint16_t* x = (const uint16_t*)g.x + b * g.x_batch + n * g.x_row;
+    uint16_t* o = (uint16_t*)g.out + b * g.out_batch + n * g.out_row;
+    float cs[8], sn[8];
+    {
+      const long long row = (b * A.table_batch + n) * (A.R / 2) + 8 * u;
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        f32x4 cv{1.f, 1.f, 1.f, 1.f}, sv{0.f, 0.f, 0.f, 0.f};
+        if (v ? turn1 : turn0) {
+          cv = *(const f32x4*)(A.cosv + row + 4 * v);
+          sv = *(const f32x4*)(A.sinv + row + 4 * v);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) cs[4 * v + i] = cv[i], sn[4 * v + i] = A.sign * sv[i];
+      }
+    }
+    for (int h0 = head0; NORM == T2T_NORM_TOKEN ? h0 == head0 : h0 - (lane >> A.shift) < H;
+         h0 += ITS * hstep) {
+      u32x4 r[ITS][2];
+#pragma unroll
+      for (int i = 0; i < ITS; ++i) {
+        const int h = h0 + i * hstep;
+        r[i][0] = r[i][1] = u32x4{0u, 0u, 0u, 0u};
+        if (on0 && h < H) r[i][0] = *(const u32x4*)(x + h * g.x_head + c0);
+        if (on1 && h < H) r[i][1] = *(const u32x4*)(x + h * g.x_head + c1);
+      }
+      float inv[ITS];
+      if constexpr (NORM != T2T_NORM_NONE) {
+        double sum[ITS], all = 0.0;
+#pragma unroll
+        for (int i = 0; i < ITS; ++i) {
+          float f0[8], f1[8];
+          rope_unpack<T>(r[i][0], f0);
+          rope_unpack<T>(r[i][1], f1);
+          sum[i] = (double)rope_squares(f0, 8) + (double)rope_squares(f1, 8);
+          all += sum[i];
+        }
+        if constexpr (NORM == T2T_NORM_TOKEN) {
+          all = rope_sum(all, 64);
+          if constexpr (WPT > 1) {
+            __syncthreads();  // the last token's sums are read
+            if (lane == 0) part[wave] = all;
+            __syncthreads();
+            all = part[0] + part[1] + part[2] + part[3];
+          }
+          const float v = rope_inv(all, one_over_n, A.eps);
+#pragma unroll
+          for (int i = 0; i < ITS; ++i) inv[i] = v;
+        } else {
+#pragma unroll
+          for (int i = 0; i < ITS; ++i) inv[i] = rope_inv(rope_sum(sum[i], L), one_over_n, A.eps);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < ITS; ++i) {
+        const int h = h0 + i * hstep;
+        // the packed values are kept, not their fp32 forms from the sum or the last token
+        asm volatile("" : "+v"(r[i][0]), "+v"(r[i][1]));
+        if constexpr (NORM != T2T_NORM_NONE) {
+          constexpr int last = NORM == T2T_NORM_TOKEN ? ITS - 1 : 0;
+          asm volatile("" : "+v"(wr[i < last ? i : last][0]), "+v"(wr[i < last ? i : last][1]));
+        }
+        float f0[8], f1[8], y0[8], y1[8];
+        rope_unpack<T>(r[i][0], f0);
+        rope_unpack<T>(r[i][1], f1);
+        if constexpr (NORM != T2T_NORM_NONE) {
+          float w0[8], w1[8];
+          const int wi = NORM == T2T_NORM_TOKEN ? i : 0;
+          rope_unpack<T>(wr[wi][0], w0);
+          rope_unpack<T>(wr[wi][1], w1);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f0[e] *= inv[i] * w0[e], f1[e] *= inv[i] * w1[e];
+        }
+        if (pair) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) rope_turn(f0[e], f1[e], cs[e], sn[e], y0[e], y1[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            y0[2 * e] = f0[2 * e], y0[2 * e + 1] = f0[2 * e + 1];
+            y1[2 * e] = f1[2 * e], y1[2 * e + 1] = f1[2 * e + 1];
+            if (turn0) rope_turn(f0[2 * e], f0[2 * e + 1], cs[e], sn[e], y0[2 * e], y0[2 * e + 1]);
+            if (turn1) rope_turn(f1[2 * e], f1[2 * e + 1], cs[4 + e], sn[4 + e], y1[2 * e], y1[2 * e + 1]);
+          }
+        }
+        if (on0 && h < H) *(u32x4*)(o + h * g.out_head + c0) = rope_pack<T>(y0);
+        if (on1 && h < H) *(u32x4*)(o + h * g.out_head + c1) = rope_pack<T>(y1);
+      }
+    }
+  }
+}
+
+// Any strides, widths and alignment: one work-group per token and tensor, pair by pair, a wave to
+// a head; the token norm's sum comes first.
+// the sum of a head's squares, by a wave
+template <typename T>
+__device__ inline double rope_head_squares(const uint16_t* x, int D, int lane) {
+  double sum = 0.0;
+  for (int c = 8 * lane; c < D; c += 512) {
+    const int n = min(8, D - c);
+    float f[8];
+    for (int e = 0; e < 8; ++e) f[e] = e < n ? T::to_f(x[c + e]) : 0.f;
+    sum += (double)rope_squares(f, n);
+  }
+  return sum;
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void rotary_any_kernel(t2t_rotary_tensor q, t2t_rotary_tensor k,
-                                                         const float* __restrict__ cosv,
-                                                         const float* __restrict__ sinv,
-                                                         long long table_batch, int N, int D, int R,
-                                                         int half, float sign, int norm, float eps) {
+                                                         RotaryArgs A, int norm) {
   const t2t_rotary_tensor& g = blockIdx.y ? k : q;
-  __shared__ float part[4];
+  __shared__ double part[4];
   const long long tok = blockIdx.x;
-  const int b = (int)(tok / N), n = (int)(tok - (long long)b * N);
+  const int D = A.D, R = A.R;
+  const int b = (int)(tok / A.N), n = (int)(tok - (long long)b * A.N);
   const uint16_t* x = (const uint16_t*)g.x + b * g.x_batch + n * g.x_row;
   uint16_t* o = (uint16_t*)g.out + b * g.out_batch + n * g.out_row;
   const uint16_t* w = (const uint16_t*)g.weight;
-  const float* c = cosv + (b * table_batch + n) * (R / 2);
-  const float* s = sinv + (b * table_batch + n) * (R / 2);
+  const float* c = A.cosv + (b * A.table_batch + n) * (R / 2);
+  const float* s = A.sinv + (b * A.table_batch + n) * (R / 2);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float inv = 1.f;
   if (norm == T2T_NORM_TOKEN) {
-    float sum = 0.f;
-    for (int h = wave; h < g.heads; h += 4)
-      for (int d = lane; d < D; d += 64) {
-        const float v = T::to_f(x[h * g.x_head + d]);
-        sum += v * v;
-      }
-    sum = rope_sum64(sum);
+    double sum = 0.0;
+    for (int h = wave; h < g.heads; h += 4) sum += rope_head_squares<T>(x + h * g.x_head, D, lane);
+    sum = rope_sum(sum, 64);
     if (lane == 0) part[wave] = sum;
     __syncthreads();
-    inv = rsqrtf((part[0] + part[1] + part[2] + part[3]) / ((float)g.heads * D) + eps);
+    inv = rope_inv(part[0] + part[1] + part[2] + part[3], 1.0 / ((double)g.heads * D), A.eps);
   }
   const int units = R / 2 + (D - R);  // pairs, then channels that are not turned
   for (int h = wave; h < g.heads; h += 4) {
@@ -111,32 +298,88 @@ __global__ __launch_bounds__(256) void rotary_any_kernel(t2t_rotary_tensor q, t2
     uint16_t* oh = o + h * g.out_head;
     const uint16_t* wh = norm == T2T_NORM_TOKEN ? w + (long long)h * D : w;
     if (norm == T2T_NORM_HEAD) {
-      float sum = 0.f;
-      for (int d = lane; d < D; d += 64) {
-        const float v = T::to_f(xh[d]);
-        sum += v * v;
-      }
-      inv = rsqrtf(rope_sum64(sum) / D + eps);
+      inv = rope_inv(rope_sum(rope_head_squares<T>(xh, D, lane), 64), 1.0 / D, A.eps);
     }
     for (int u = lane; u < units; u += 64) {
       if (u < R / 2) {
-        const int i0 = half ? u : 2 * u, i1 = half ? u + R / 2 : 2 * u + 1;
+        const int i0 = A.half ? u : 2 * u, i1 = A.half ? u + R / 2 : 2 * u + 1;
         float a = T::to_f(xh[i0]), e = T::to_f(xh[i1]);
         if (norm) {
-          a = a * inv * T::to_f(wh[i0]);
-          e = e * inv * T::to_f(wh[i1]);
+          a *= inv * T::to_f(wh[i0]);
+          e *= inv * T::to_f(wh[i1]);
         }
-        const float cc = c[u], ss = sign * s[u];
-        oh[i0] = T::from_f(a * cc - e * ss);
-        oh[i1] = T::from_f(a * ss + e * cc);
+        float y0, y1;
+        rope_turn(a, e, c[u], A.sign * s[u], y0, y1);
+        oh[i0] = T::from_f(y0);
+        oh[i1] = T::from_f(y1);
       } else {
         const int d = R + (u - R / 2);
         float a = T::to_f(xh[d]);
-        if (norm) a = a * inv * T::to_f(wh[d]);
+        if (norm) a *= inv * T::to_f(wh[d]);
         oh[d] = T::from_f(a);
       }
     }
   }
+}
+
+// 16-byte vectors: all strides, widths and pointers allow them
+static bool rope_vectors(const t2t_rotary_tensor& t, bool weight) {
+  return ((t.x_batch | t.x_row | t.x_head | t.out_batch | t.out_row | t.out_head) & 7) == 0 &&
+         (((uintptr_t)t.x | (uintptr_t)t.out | (weight ? (uintptr_t)t.weight : 0)) & 15) == 0;
+}
+
+template <typename T, int NORM, int WPT, int ITS>
+static void rope_launch(const t2t_rotary_tensor& q, const t2t_rotary_tensor& k, const RotaryArgs& A, int tensors,
+                        hipStream_t st) {
+  const long long wgs = (A.tokens + 4 / WPT - 1) / (4 / WPT);
+  // a few rounds of work-groups, so that the weights are read once for several tokens
+  hipLaunchKernelGGL((rotary_kernel<T, NORM, WPT, ITS>), dim3((unsigned)(wgs < 4096 ? wgs : 4096), tensors),
+                     dim3(256), 0, st, q, k, A);
+}
+
+template <typename T, int NORM, int WPT>
+static bool rope_rounds(const t2t_rotary_tensor& q, const t2t_rotary_tensor& k, const RotaryArgs& A, int tensors,
+                        int its, hipStream_t st) {
+  switch (its) {
+    case 1: rope_launch<T, NORM, WPT, 1>(q, k, A, tensors, st); return true;
+    case 2: rope_launch<T, NORM, WPT, 2>(q, k, A, tensors, st); return true;
+    case 3: rope_launch<T, NORM, WPT, 3>(q, k, A, tensors, st); return true;
+    case 4: rope_launch<T, NORM, WPT, 4>(q, k, A, tensors, st); return true;
+    case 5: rope_launch<T, NORM, WPT, 5>(q, k, A, tensors, st); return true;
+    case 6: rope_launch<T, NORM, WPT, 6>(q, k, A, tensors, st); return true;
+    case 7: rope_launch<T, NORM, WPT, 7>(q, k, A, tensors, st); return true;
+    case 8: rope_launch<T, NORM, WPT, 8>(q, k, A, tensors, st); return true;
+  }
+  return false;
+}
+
+template <typename T>
+static void rope_run(const t2t_rotary_tensor& q, const t2t_rotary_tensor& k, RotaryArgs A, int norm, int tensors,
+                     hipStream_t st) {
+  const int H = tensors == 2 && k.heads > q.heads ? k.heads : q.heads;
+  bool vec = A.D % 8 == 0 && A.R % (A.half ? 16 : 8) == 0 && rope_vectors(q, norm) &&
+             (tensors == 1 || rope_vectors(k, norm)) && (((uintptr_t)A.cosv | (uintptr_t)A.sinv) & 15) == 0;
+  A.units = A.half ? A.R / 16 + (A.D - A.R + 15) / 16 : (A.D + 15) / 16;
+  for (A.shift = 0; (1 << A.shift) < A.units;) ++A.shift;
+  const int per = 64 >> A.shift;  // heads a wave holds at once
+  // a whole work-group takes a token where the tokens are few (latency) or a wave's registers
+  // cannot hold the heads that one norm spans
+  const bool wide = A.tokens < 1024 || (norm == T2T_NORM_TOKEN && H > 8 * per);
+  int its = cdiv(H, wide ? 4 * per : per);
+  if (norm != T2T_NORM_TOKEN) its = cdiv(its, cdiv(its, 8));
+  if (vec && its <= 8) {
+    if (norm == T2T_NORM_TOKEN)
+      wide ? rope_rounds<T, T2T_NORM_TOKEN, 4>(q, k, A, tensors, its, st)
+           : rope_rounds<T, T2T_NORM_TOKEN, 1>(q, k, A, tensors, its, st);
+    else if (norm == T2T_NORM_HEAD)
+      wide ? rope_rounds<T, T2T_NORM_HEAD, 4>(q, k, A, tensors, its, st)
+           : rope_rounds<T, T2T_NORM_HEAD, 1>(q, k, A, tensors, its, st);
+    else
+      wide ? rope_rounds<T, T2T_NORM_NONE, 4>(q, k, A, tensors, its, st)
+           : rope_rounds<T, T2T_NORM_NONE, 1>(q, k, A, tensors, its, st);
+    return;
+  }
+  hipLaunchKernelGGL(rotary_any_kernel<T>, dim3((unsigned)A.tokens, tensors), dim3(256), 0, st, q, k, A, norm);
 }
 
 extern "C" int t2t_rotary(const t2t_rotary_tensor* q, const t2t_rotary_tensor* k, int dtype,
@@ -158,14 +401,16 @@ extern "C" int t2t_rotary(const t2t_rotary_tensor* q, const t2t_rotary_tensor* k
   const long long tokens = (long long)B * N;
   if (tokens == 0) return T2T_OK;
   T2T_REQUIRE(cosv && sinv && ts[0]->x && ts[0]->out && ts[1]->x && ts[1]->out, "rotary: null pointer");
-  const dim3 grid((unsigned)tokens, k ? 2 : 1);
-  const long long tb = table_batched ? N : 0;
+  RotaryArgs A{};
+  A.cosv = cosv, A.sinv = sinv;
+  A.table_batch = table_batched ? N : 0;
+  A.tokens = tokens, A.N = N, A.D = D, A.R = R;
+  A.half = layout == T2T_ROPE_HALF;
+  A.sign = inverse ? -1.f : 1.f, A.eps = eps;
   if (dtype == T2T_BF16)
-    hipLaunchKernelGGL(rotary_any_kernel<BF16T>, grid, dim3(256), 0, (hipStream_t)stream, *ts[0], *ts[1],
-                       cosv, sinv, tb, N, D, R, layout == T2T_ROPE_HALF, inverse ? -1.f : 1.f, norm, eps);
+    rope_run<BF16T>(*ts[0], *ts[1], A, norm, k ? 2 : 1, (hipStream_t)stream);
   else
-    hipLaunchKernelGGL(rotary_any_kernel<F16T>, grid, dim3(256), 0, (hipStream_t)stream, *ts[0], *ts[1],
-                       cosv, sinv, tb, N, D, R, layout == T2T_ROPE_HALF, inverse ? -1.f : 1.f, norm, eps);
+    rope_run<F16T>(*ts[0], *ts[1], A, norm, k ? 2 : 1, (hipStream_t)stream);
   T2T_LAUNCH_CHECK("rotary");
   return T2T_OK;
 }

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from contextlib import contextmanager, nullcontext
+from contextlib import nullcontext
 from dataclasses import dataclass
 from typing import NamedTuple
 
@@ -712,28 +712,49 @@ def fit_chol(Mq, Mk, floor, small, stream=None):
 # ---------------------------------------------------------------------------
 # the block's steps around attention: rotary positions, MXFP4 linear layers
 # ---------------------------------------------------------------------------
-@contextmanager
-def _launch(dev, stream, *tensors):
-    """A call on ``stream`` (default: ``dev``'s current one) with ``dev``
-    current; yields the stream's handle.  On a stream of the caller's choice the
-    tensors' memory is not reused before the stream is done with it."""
+# (single-token calls are bound by the host: checks are written for few
+# operations, and a matrix in MXFP4 is checked once, when it is made)
+_functions = {}
+
+
+def _launch(name, dev, stream, tensors, *args):
+    """Call an entry point on ``stream`` (default: ``dev``'s current one) with
+    ``dev`` current.  On a stream of the caller's choice the memory of
+    ``tensors`` is not reused before the stream is done with it."""
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _launch(name, dev, stream, tensors, *args)
+    if stream is None:
+        handle = torch._C._cuda_getCurrentRawStream(dev.index)
+    else:
+        handle = stream.cuda_stream
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(_lib.lib(), name)
+    rc = fn(*args, handle)
+    if rc:
+        raise RuntimeError(f"{name} failed (code {rc}): "
+                           f"{_lib.lib().t2t_last_error().decode(errors='replace')}")
+
+
+def _on(stream, dev):
     if stream is not None and stream.device != dev:
         raise ValueError(f"t2t: the stream is on {stream.device}, the tensors on {dev}")
-    with torch.cuda.device(dev) if torch.cuda.current_device() != dev.index else nullcontext():
-        if stream is not None:
-            for t in tensors:
-                if t is not None:
-                    t.record_stream(stream)
-        yield stream_handle(stream)
 
 
-def _check_vec(t, n, dtype, name, dev):
-    if t is not None:
-        _check(t, (n,), dtype, name, dev)
+def _empty(stream, shape, dtype, dev):
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    return _new(stream, *shape, dtype=dtype, device=dev)
 
 
 def _scattered(t):
     """Whether a view's elements all have an address of their own."""
+    if t.is_contiguous():
+        return True
     last = 0
     for st, sz in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
         if st <= last:
@@ -820,22 +841,25 @@ def rotary_table(positions, frequencies, out=None, stream=None):
     are taken in 64 bits; |position * frequency| stays below 2^31."""
     freqs, pairs, factor = frequencies
     dev = _dev(positions)
+    _on(stream, dev)
     lead = tuple(positions.shape)
     if len(pairs) > 1:
         if not lead or lead[-1] != len(pairs):
             raise ValueError(f"t2t: positions must end in {len(pairs)} axes, got {lead}")
         lead = lead[:-1]
-    _check(positions, positions.shape, (torch.int32, torch.int64), "positions", dev)
-    n = sum(pairs)
-    _check(freqs, (n,), torch.float64, "frequencies", dev)
-    with _launch(dev, stream, positions, freqs, *(out or ())) as st:
-        if out is None:
-            out = tuple(_new(stream, *lead, n, dtype=_f32, device=dev) for _ in range(2))
-        for t, name in zip(out, ("cos", "sin")):
-            _check(t, (*lead, n), _f32, name, dev)
-        call("t2t_rotary_table", positions, 32 if positions.dtype == _i32 else 64, math.prod(lead),
-             len(pairs), (ctypes.c_int * len(pairs))(*pairs), freqs, factor, *out, st)
-    return tuple(out)
+    _check(positions, positions.shape, (_i32, torch.int64), "positions", dev)
+    shape = (*lead, sum(pairs))
+    _check(freqs, shape[-1:], torch.float64, "frequencies", dev)
+    if out is None:
+        cos, sin = _empty(stream, shape, _f32, dev), _empty(stream, shape, _f32, dev)
+    else:
+        cos, sin = out
+        _check(cos, shape, _f32, "cos", dev)
+        _check(sin, shape, _f32, "sin", dev)
+    _launch("t2t_rotary_table", dev, stream, (positions, freqs, cos, sin), positions.data_ptr(),
+            32 if positions.dtype == _i32 else 64, math.prod(lead), len(pairs),
+            (ctypes.c_int * len(pairs))(*pairs), freqs.data_ptr(), factor, cos.data_ptr(), sin.data_ptr())
+    return cos, sin
 
 
 _ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
@@ -843,9 +867,11 @@ _ROPE_NORMS = {None: 0, "token": 1, "head": 2}
 
 
 def _rotary_arg(x, out, weight, norm, name, dev, B, N, D, dtype):
-    if (not isinstance(x, torch.Tensor) or x.dtype != dtype or x.device != dev or x.dim() not in (3, 4)
-            or (x.shape[0] if x.dim() == 4 else 1) != B or x.shape[-3] != N or x.shape[-1] != D
-            or not 1 <= x.shape[-2] <= 65536 or (D > 1 and x.stride(-1) != 1)):
+    """The argument struct of one tensor, checked."""
+    nd = x.dim() if isinstance(x, torch.Tensor) else 0
+    if (nd not in (3, 4) or x.dtype != dtype or x.device != dev or (x.shape[0] if nd == 4 else 1) != B
+            or x.shape[-3] != N or x.shape[-1] != D or not 1 <= x.shape[-2] <= 65536
+            or (D > 1 and x.stride(-1) != 1)):
         raise ValueError(f"t2t: {name} must be a {dtype} [{B}, {N}, heads, {D}] tensor on {dev} with "
                          f"contiguous channels")
     if (not isinstance(out, torch.Tensor) or out.shape != x.shape or out.dtype != dtype
@@ -857,10 +883,10 @@ def _rotary_arg(x, out, weight, norm, name, dev, B, N, D, dtype):
         _check(weight, (H * D,) if norm == "token" else (D,), dtype, f"{name}_weight", dev)
     elif weight is not None:
         raise ValueError(f"t2t: {name}_weight without a norm")
-    sb = lambda t: t.stride(0) if t.dim() == 4 else 0  # noqa: E731
-    return _lib.RotaryTensor(x.data_ptr(), sb(x), x.stride(-3), x.stride(-2), out.data_ptr(), sb(out),
-                             out.stride(-3), out.stride(-2),
-                             weight.data_ptr() if weight is not None else None, H)
+    xs, os = x.stride(), out.stride()
+    return _lib.RotaryTensor(x.data_ptr(), xs[0] if nd == 4 else 0, xs[-3], xs[-2], out.data_ptr(),
+                             os[0] if nd == 4 else 0, os[-3], os[-2],
+                             None if weight is None else weight.data_ptr(), H)
 
 
 def rotary(q, k, cos, sin, *, layout="interleaved", inverse=False, norm=None, q_weight=None,
@@ -877,6 +903,7 @@ def rotary(q, k, cos, sin, *, layout="interleaved", inverse=False, norm=None, q_
     once.  ``out``: (out_q, out_k); an output may be its input, and otherwise
     shares no memory with any other argument.  Returns (out_q, out_k)."""
     dev = _dev(q)
+    _on(stream, dev)
     if q.dim() not in (3, 4) or q.dtype not in _HALF:
         raise ValueError("t2t: q must be an fp16 or bf16 [B, N, H, D] or [N, H, D] tensor")
     B, (N, _, D) = q.shape[0] if q.dim() == 4 else 1, q.shape[-3:]
@@ -890,81 +917,85 @@ def rotary(q, k, cos, sin, *, layout="interleaved", inverse=False, norm=None, q_
     if not (1 <= D <= 256 and 2 <= R <= D):
         raise ValueError(f"t2t: {R} of {D} channels rotated (2 <= R <= D <= 256)")
     batched = cos.dim() == 3
-    for t, name in ((cos, "cos"), (sin, "sin")):
-        _check(t, (B, N, R // 2) if batched else (N, R // 2), _f32, name, dev)
+    shape = (B, N, R // 2) if batched else (N, R // 2)
+    _check(cos, shape, _f32, "cos", dev)
+    _check(sin, shape, _f32, "sin", dev)
     if B * N >= 2 ** 31:
         raise ValueError(f"t2t: {B} x {N} tokens")
-    with _launch(dev, stream, q, k, cos, sin, q_weight, k_weight, *(out or ())) as st:
-        if out is None:
-            out = tuple(None if x is None else _new(stream, *x.shape, dtype=x.dtype, device=dev)
-                        for x in (q, k))
-        tq = _rotary_arg(q, out[0], q_weight, norm, "q", dev, B, N, D, q.dtype)
-        tk = None
-        if k is not None:
-            tk = _rotary_arg(k, out[1], k_weight, norm, "k", dev, B, N, D, q.dtype)
-        call("t2t_rotary", ctypes.byref(tq), ctypes.byref(tk) if tk is not None else None,
-             dtype_code(q.dtype), cos, sin, int(batched), B, N, D, R, _ROPE_LAYOUTS[layout],
-             int(bool(inverse)), _ROPE_NORMS[norm], float(eps), st)
-    return out[0], out[1] if k is not None else None
+    oq, ok = out if out is not None else (None, None)
+    if oq is None:
+        oq = _empty(stream, q.shape, q.dtype, dev)
+    tq = _rotary_arg(q, oq, q_weight, norm, "q", dev, B, N, D, q.dtype)
+    tk = None
+    if k is not None:
+        if ok is None and isinstance(k, torch.Tensor):
+            ok = _empty(stream, k.shape, k.dtype, dev)
+        tk = _rotary_arg(k, ok, k_weight, norm, "k", dev, B, N, D, q.dtype)
+    _launch("t2t_rotary", dev, stream, (q, k, cos, sin, q_weight, k_weight, oq, ok), tq, tk,
+            dtype_code(q.dtype), cos.data_ptr(), sin.data_ptr(), batched, B, N, D, R,
+            _ROPE_LAYOUTS[layout], bool(inverse), _ROPE_NORMS[norm], eps)
+    return oq, ok if k is not None else None
+
+
+def _mx_bytes(rows, cols):
+    """Bytes of the codes and of the scales (t2t_mxfp4_code_bytes, _scale_bytes)."""
+    scales = -(-rows // 32) * (-(-cols // 256) * 256)
+    return scales * 16, scales
 
 
 class MxFp4:
     """A matrix [rows, cols] in MXFP4 (``mxfp4_quantize``): E2M1 codes in blocks
     of 32 columns with a power-of-two scale each, in the order of the matrix
-    operands (include/t2t_hip.h).  ``codes`` and ``scales`` are uint8 buffers."""
+    operands (include/t2t_hip.h).  ``codes`` and ``scales`` are the uint8
+    buffers on the GPU; they are checked here, once."""
 
-    __slots__ = ("codes", "scales", "rows", "cols")
+    __slots__ = ("_codes", "_scales", "_rows", "_cols", "_device", "_ptrs")
 
     def __init__(self, codes, scales, rows, cols):
-        self.codes, self.scales, self.rows, self.cols = codes, scales, rows, cols
+        rows, cols = int(rows), int(cols)
+        if not (0 <= rows < 2 ** 31 and 32 <= cols <= 2 ** 27 and cols % 32 == 0):
+            raise ValueError(f"t2t: an MXFP4 matrix has columns in multiples of 32, got {rows} x {cols}")
+        dev = _dev(codes)
+        for t, n, name in zip((codes, scales), _mx_bytes(rows, cols), ("codes", "scales")):
+            _check(t, (n,), torch.uint8, name, dev)
+            if n and t.data_ptr() % 16:
+                raise ValueError(f"t2t: {name} must be 16-byte aligned")
+        self._codes, self._scales, self._rows, self._cols = codes, scales, rows, cols
+        self._device, self._ptrs = dev, (codes.data_ptr(), scales.data_ptr())
 
-    @property
-    def shape(self):
-        return (self.rows, self.cols)
-
-    @property
-    def device(self):
-        return self.codes.device
+    codes = property(lambda self: self._codes)
+    scales = property(lambda self: self._scales)
+    rows = property(lambda self: self._rows)
+    cols = property(lambda self: self._cols)
+    shape = property(lambda self: (self._rows, self._cols))
+    device = property(lambda self: self._device)
 
     def __repr__(self):
-        return f"MxFp4({self.rows} x {self.cols}, {self.device})"
-
-
-def _mx_size(rows, cols, name):
-    if not (0 <= rows < 2 ** 31 and 32 <= cols < 2 ** 31 - 255 and cols % 32 == 0):
-        raise ValueError(f"t2t: {name} must have columns in multiples of 32, got {rows} x {cols}")
-
-
-def _check_mx(t, name, dev):
-    if not isinstance(t, MxFp4):
-        raise ValueError(f"t2t: {name} must be an MxFp4 matrix (mxfp4_quantize)")
-    _mx_size(t.rows, t.cols, name)
-    for buf, size in ((t.codes, "t2t_mxfp4_code_bytes"), (t.scales, "t2t_mxfp4_scale_bytes")):
-        _check(buf, (size_query(size, t.rows, t.cols),), torch.uint8, name, dev)
+        return f"MxFp4({self._rows} x {self._cols}, {self._device})"
 
 
 def _mx_rows(t, name, dev, align):
     """A [..., K] tensor of 16-bit values as rows: (rows, K, row stride)."""
-    if (not isinstance(t, torch.Tensor) or t.dtype not in _HALF or t.device != dev or t.dim() < 1):
+    if not isinstance(t, torch.Tensor) or t.dtype not in _HALF or t.device != dev or t.dim() < 1:
         raise ValueError(f"t2t: {name} must be an fp16 or bf16 tensor on {dev}")
     cols = t.shape[-1]
-    try:
-        v = t.view(math.prod(t.shape[:-1]), cols)
-    except RuntimeError:
-        raise ValueError(f"t2t: the rows of {name} {tuple(t.shape)} must have one stride, got "
-                         f"{tuple(t.stride())}") from None
-    rows = v.shape[0]
-    stride = v.stride(0) if rows > 1 else cols
-    if cols > 1 and v.numel() and v.stride(1) != 1 or stride < cols \
-            or rows and (t.data_ptr() % align or rows > 1 and stride * 2 % align):
-        raise ValueError(f"t2t: {name} must have contiguous {align}-byte aligned rows that do not "
-                         f"overlap, got strides {tuple(t.stride())}")
+    if t.is_contiguous():
+        rows, stride = (t.numel() // cols if cols else 0), cols
+    else:
+        try:
+            v = t.view(math.prod(t.shape[:-1]), cols)
+        except RuntimeError:
+            raise ValueError(f"t2t: the rows of {name} {tuple(t.shape)} must have one stride, got "
+                             f"{tuple(t.stride())}") from None
+        rows = v.shape[0]
+        stride = v.stride(0) if rows > 1 else cols
+        if cols > 1 and v.stride(1) != 1 or stride < cols:
+            raise ValueError(f"t2t: {name} must have contiguous rows that do not overlap, got strides "
+                             f"{tuple(t.stride())}")
+    if t.data_ptr() % align or rows > 1 and stride * 2 % align:
+        raise ValueError(f"t2t: the rows of {name} must be {align}-byte aligned, got strides "
+                         f"{tuple(t.stride())}")
     return rows, cols, stride
-
-
-def _mx_new(stream, rows, cols, dev):
-    return MxFp4(*(_new(stream, size_query(size, rows, cols), dtype=torch.uint8, device=dev)
-                   for size in ("t2t_mxfp4_code_bytes", "t2t_mxfp4_scale_bytes")), rows, cols)
 
 
 def mxfp4_quantize(x, out=None, stream=None):
@@ -973,17 +1004,17 @@ def mxfp4_quantize(x, out=None, stream=None):
     (at least 2^-126); values are rounded to nearest, ties to even, and held to
     6 scales; a block with an inf or NaN stands for NaN."""
     dev = _dev(x)
+    _on(stream, dev)
     M, K, stride = _mx_rows(x, "x", dev, 16)
-    _mx_size(M, K, "x")
-    if out is not None:
-        _check_mx(out, "out", dev)
-        if out.shape != (M, K):
-            raise ValueError(f"t2t: out is {out.rows} x {out.cols}, x {M} x {K}")
-    with _launch(dev, stream, x, *((out.codes, out.scales) if out is not None else ())) as st:
-        if out is None:
-            out = _mx_new(stream, M, K, dev)
-        call("t2t_mxfp4_quantize", _lib.RowView(x), dtype_code(x.dtype), stride, out.codes, out.scales,
-             M, K, st)
+    if out is None:
+        if K < 32 or K % 32:
+            raise ValueError(f"t2t: x must have columns in multiples of 32, got {K}")
+        nc, ns = _mx_bytes(M, K)
+        out = MxFp4(_empty(stream, (nc,), torch.uint8, dev), _empty(stream, (ns,), torch.uint8, dev), M, K)
+    elif not isinstance(out, MxFp4) or out.shape != (M, K) or out.device != dev:
+        raise ValueError(f"t2t: out must be an MxFp4 matrix {M} x {K} on {dev}, got {out!r}")
+    _launch("t2t_mxfp4_quantize", dev, stream, (x, out._codes, out._scales), x.data_ptr(),
+            dtype_code(x.dtype), stride, *out._ptrs, M, K)
     return out
 
 
@@ -992,21 +1023,27 @@ def mxfp4_dequantize(t, dtype=torch.bfloat16, out=None, stream=None):
     type that was quantised, and in bf16 where no scale is below 2^-126."""
     if not isinstance(t, MxFp4):
         raise ValueError("t2t: expected an MxFp4 matrix")
-    dev = _dev(t.codes)
-    _check_mx(t, "t", dev)
-    dtype_code(dtype)
-    with _launch(dev, stream, t.codes, t.scales, out) as st:
-        if out is None:
-            out = _new(stream, t.rows, t.cols, dtype=dtype, device=dev)
-        if _mx_rows(out, "out", dev, 16)[:2] != t.shape or out.dtype != dtype:
+    dev = t._device
+    _on(stream, dev)
+    code = dtype_code(dtype)
+    if out is None:
+        out = _empty(stream, t.shape, dtype, dev)
+        stride = t._cols
+    else:
+        M, K, stride = _mx_rows(out, "out", dev, 16)
+        if (M, K) != t.shape or out.dtype != dtype:
             raise ValueError(f"t2t: out must be {dtype} {t.shape}, got {out.dtype} {tuple(out.shape)}")
-        stride = _mx_rows(out, "out", dev, 16)[2]
-        call("t2t_mxfp4_dequantize", t.codes, t.scales, _lib.RowView(out), dtype_code(dtype), stride,
-             t.rows, t.cols, st)
+    _launch("t2t_mxfp4_dequantize", dev, stream, (t._codes, t._scales, out), *t._ptrs, out.data_ptr(), code,
+            stride, *t.shape)
     return out
 
 
 _ACTIVATIONS = {None: 0, "gelu_tanh": 1}
+
+
+def mxfp4_linear_ws_bytes(M, N, K):
+    """Workspace of mxfp4_linear for a 16-bit x of M rows."""
+    return size_query("t2t_mxfp4_linear_ws_bytes", M, N, K)
 
 
 def mxfp4_linear(x, weight, bias=None, *, activation=None, dtype=None, out=None, ws=None, stream=None):
@@ -1018,37 +1055,42 @@ def mxfp4_linear(x, weight, bias=None, *, activation=None, dtype=None, out=None,
     ``out``: contiguous rows, no memory shared with x."""
     if not isinstance(weight, MxFp4):
         raise ValueError("t2t: weight must be an MxFp4 matrix (mxfp4_quantize)")
-    dev = _dev(weight.codes)
-    _check_mx(weight, "weight", dev)
-    N = weight.rows
-    quantised = isinstance(x, MxFp4)
-    if quantised:
-        _check_mx(x, "x", dev)
-        (M, K), lead = x.shape, (x.rows,)
+    dev = weight._device
+    _on(stream, dev)
+    N = weight._rows
+    if isinstance(x, MxFp4):
+        if x._device != dev:
+            raise ValueError(f"t2t: x must be on {dev}")
+        M, K = x.shape
+        shape = (M, N)
         dt = torch.bfloat16 if dtype is None else dtype
     else:
         M, K, stride = _mx_rows(x, "x", dev, 16)
-        lead, dt = tuple(x.shape[:-1]), x.dtype
+        shape, dt = (*x.shape[:-1], N), x.dtype
         if dtype not in (None, dt):
             raise ValueError(f"t2t: the output of a {dt} input is {dt}, not {dtype}")
     code = dtype_code(dt)
-    if K != weight.cols or N < 1:
-        raise ValueError(f"t2t: x has {K} columns, weight {N} x {weight.cols}")
+    if K != weight._cols or N < 1:
+        raise ValueError(f"t2t: x has {K} columns, weight {N} x {weight._cols}")
     if activation not in _ACTIVATIONS:
         raise ValueError(f"t2t: activation {activation!r} (None or gelu_tanh)")
-    _check_vec(bias, N, dt, "bias", dev)
-    src = (x.codes, x.scales) if quantised else (x,)
-    with _launch(dev, stream, *src, weight.codes, weight.scales, bias, out) as st:
-        if out is None:
-            out = _new(stream, *lead, N, dtype=dt, device=dev)
-        om, on, ostride = _mx_rows(out, "out", dev, 2)
-        if tuple(out.shape) != (*lead, N) or out.dtype != dt:
-            raise ValueError(f"t2t: out must be {dt} {(*lead, N)}, got {out.dtype} {tuple(out.shape)}")
-        args = (weight.codes, weight.scales, bias, _ACTIVATIONS[activation], _lib.RowView(out))
-        if quantised:
-            call("t2t_mxfp4_product", *src, *args, code, ostride, M, N, K, st)
-        else:
-            ws = _ws_for(ws, size_query("t2t_mxfp4_linear_ws_bytes", M, N, K), dev, stream)
-            call("t2t_mxfp4_linear", _lib.RowView(x), code, stride, *args, ostride, M, N, K, ws,
-                 ws.numel(), st)
+    if bias is not None:
+        _check(bias, (N,), dt, "bias", dev)
+    if out is None:
+        out = _empty(stream, shape, dt, dev)
+        ostride = N
+    else:
+        ostride = _mx_rows(out, "out", dev, 2)[2]
+        if tuple(out.shape) != shape or out.dtype != dt:
+            raise ValueError(f"t2t: out must be {dt} {shape}, got {out.dtype} {tuple(out.shape)}")
+    args = (*weight._ptrs, None if bias is None else bias.data_ptr(), _ACTIVATIONS[activation],
+            out.data_ptr())
+    if isinstance(x, MxFp4):
+        _launch("t2t_mxfp4_product", dev, stream,
+                (x._codes, x._scales, weight._codes, weight._scales, bias, out), *x._ptrs, *args, code,
+                ostride, M, N, K)
+    else:
+        ws = _ws_for(ws, mxfp4_linear_ws_bytes(M, N, K), dev, stream)
+        _launch("t2t_mxfp4_linear", dev, stream, (x, weight._codes, weight._scales, bias, out), x.data_ptr(),
+                code, stride, *args, ostride, M, N, K, ws.data_ptr(), ws.numel())
     return out
