@@ -237,9 +237,8 @@ typedef __attribute__((address_space(1))) void mx_glb_t;
 template <int TW, int TA> struct MxTile {
   static constexpr int RB = 2 * (TW + TA);          // row blocks: 2 TW of weights, 2 TA of tokens
   static constexpr int CODES = RB * 2048;           // a stage's codes
-  static constexpr int PITCH = 64 * TW + 16;        // a token's staged outputs (bytes)
   static constexpr int SCALES = RB * 256;
-  static constexpr int STAGE = CODES + SCALES > 4 * 32 * PITCH ? CODES + SCALES : 4 * 32 * PITCH;
+  static constexpr int STAGE = CODES + SCALES > 16384 ? CODES + SCALES : 16384;  // or 4 KB a wave, at the end
 };
 
 // Consecutive work-groups go to the eight XCDs in turn: each takes a run of
@@ -281,90 +280,67 @@ __device__ inline void mx_bias_init(f32x16 (&acc)[TW][TA], const uint16_t* __res
   }
 }
 
-// 32 tokens at a time through a staging area of the wave's own, then whole rows: a wave's 32 TA
-// tokens from m on, 32 TW features from n on
+// The values of one row, the first n of which are inside, to an o of any alignment (rows of odd
+// widths: the store takes 16 bytes at any address, two at a time it cost 16 us at 4099 x 2041)
+template <typename VT>
+__device__ inline void mx_put(uint16_t* o, const VT& v, int n) {
+  if (n >= (int)sizeof(VT) / 2)
+    __builtin_memcpy(o, &v, sizeof(VT));
+  else
+#pragma unroll
+    for (int e = 0; e < (int)sizeof(VT) / 2; ++e)
+      if (e < n) o[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+}
+
+// A wave's 32 TA tokens from m on, 32 TW features from n on: 32 tokens x 64 features at a time (32
+// where TW is 1) are packed, turned through LDS of the wave's own (16-byte chunk c of token t at c ^
+// (t & 7)) and stored as rows, a step behind, so that the reads have the next step's packing to land.
+// (DS operations of a wave run in order: the next writes follow the last reads.)
 template <typename T, int TW, int TA, bool GELU>
 __device__ inline void mx_store(const f32x16 (&acc)[TW][TA], char* so, uint16_t* __restrict__ out,
-                                long long ldo, int vec, int m, int M, int n, int N) {
-  constexpr int PITCH = 64 * TW + 16, LR = 4 * TW;  // lanes per row, 8 features each
-  const int lane = threadIdx.x & 63, hh = lane >> 5;
-  const int f0 = n + (lane % LR) * 8;
-  const bool whole = vec && f0 + 8 <= N;
-#pragma unroll
-  for (int j = 0; j < TA; ++j) {
-#pragma unroll
-    for (int i = 0; i < TW; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = GELU ? mx_gelu(acc[i][j][4 * q + e]) : acc[i][j][4 * q + e];
-        *(u32x2*)(so + (lane & 31) * PITCH + (32 * i + 8 * q + 4 * hh) * 2) =
-            u32x2{Pk<T>::pack(v[0], v[1]), Pk<T>::pack(v[2], v[3])};
-      }
-#pragma unroll 1
-    for (int t = lane / LR; t < 32 && m + 32 * j + t < M; t += 64 / LR) {
-      const u32x4 v = *(const u32x4*)(so + t * PITCH + (lane % LR) * 16);
-      uint16_t* o = out + (long long)(m + 32 * j + t) * ldo + f0;
-      if (whole)
-        *(u32x4*)o = v;
-      else
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (f0 + e < N) o[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
-    }
-  }
-}
-
-// the same through 4 KB: 32 tokens x 64 features at a time, 16-byte chunk c of token t at
-// c ^ (t & 7)
-template <typename T, bool GELU>
-__device__ inline void mx_store_big(const f32x16 (&acc)[4][4], char* so, uint16_t* __restrict__ out,
-                                    long long ldo, int vec, int m, int M, int n, int N) {
+                                long long ldo, int m, int M, int n, int N) {
+  constexpr int IW = TW == 1 ? 1 : 2, LR = 4 * IW, RT = 64 / LR, RS = 32 / RT;  // lanes a row, rows a store
   int lane = threadIdx.x & 63;
   asm volatile("" : "+v"(lane));  // (or its addresses are kept in registers through the products)
-  const int hh = lane >> 5, c = lane & 7;
+  const int hh = lane >> 5, c = lane % LR, t0 = lane / LR;
+  u32x4 v[RS];
+  uint16_t* row = out + (long long)(m + t0) * ldo + n + 8 * c;
+  auto put = [&](int j, int i) {
+    const int left = N - (n + 32 * i + 8 * c);
+    uint16_t* o = row + (long long)(32 * j) * ldo + 32 * i;
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+    for (int r = 0; r < RS; ++r, o += RT * ldo)
+      if (m + 32 * j + RT * r + t0 < M) mx_put(o, v[r], left);
+  };
 #pragma unroll
-    for (int ii = 0; ii < 4; ii += 2) {
-      __builtin_amdgcn_sched_barrier(0);
+  for (int k = 0; k < TA * (TW / IW); ++k) {
+    const int j = k / (TW / IW), ii = k % (TW / IW) * IW;
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < IW; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float v[4];
+      for (int q = 0; q < 4; ++q) {
+        float f[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            v[e] = GELU ? mx_gelu(acc[ii + i][j][4 * q + e]) : acc[ii + i][j][4 * q + e];
-          *(u32x2*)(so + (lane & 31) * 128 + (((4 * i + q) ^ (lane & 7)) * 16) + 8 * hh) =
-              u32x2{Pk<T>::pack(v[0], v[1]), Pk<T>::pack(v[2], v[3])};
-        }
-      const int f0 = n + 32 * ii + 8 * c;
-      if (vec && f0 + 8 <= N) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int t = 8 * r + (lane >> 3);
-          if (m + 32 * j + t < M)
-            *(u32x4*)(out + (long long)(m + 32 * j + t) * ldo + f0) =
-                *(const u32x4*)(so + t * 128 + ((c ^ (t & 7)) * 16));
-        }
-      } else {
-#pragma unroll 1
-        for (int t = lane >> 3; t < 32 && m + 32 * j + t < M; t += 8) {
-          const u32x4 v = *(const u32x4*)(so + t * 128 + ((c ^ (t & 7)) * 16));
-          uint16_t* o = out + (long long)(m + 32 * j + t) * ldo + f0;
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (f0 + e < N) o[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
-        }
+        for (int e = 0; e < 4; ++e)
+          f[e] = GELU ? mx_gelu(acc[ii + i][j][4 * q + e]) : acc[ii + i][j][4 * q + e];
+        *(u32x2*)(so + (lane & 31) * (16 * LR) + (((4 * i + q) ^ (lane & (LR - 1))) * 16) + 8 * hh) =
+            u32x2{Pk<T>::pack(f[0], f[1]), Pk<T>::pack(f[2], f[3])};
       }
+    __builtin_amdgcn_sched_barrier(0);
+    if (k) put((k - 1) / (TW / IW), (k - 1) % (TW / IW) * IW);
+#pragma unroll
+    for (int r = 0; r < RS; ++r) {
+      const int t = RT * r + t0;
+      v[r] = *(const u32x4*)(so + t * (16 * LR) + ((c ^ (t & (LR - 1))) * 16));
     }
+  }
+  put(TA - 1, TW - IW);
 }
 
 template <typename T, int TW, int TA, bool GELU>
-__global__ __launch_bounds__(256, TW * TA >= 16 ? 1 : 2) void mx_tile_kernel(
-    MxMat a, MxMat w, const uint16_t* __restrict__ bias, uint16_t* __restrict__ out, long long ldo, int vec,
+__global__ __launch_bounds__(256, 2) void mx_tile_kernel(
+    MxMat a, MxMat w, const uint16_t* __restrict__ bias, uint16_t* __restrict__ out, long long ldo,
     int groups, int mt, int nt, int per_xcd) {
   using C = MxTile<TW, TA>;
   __shared__ __attribute__((aligned(1024))) char st0[C::STAGE];
@@ -462,7 +438,7 @@ __global__ __launch_bounds__(256, TW * TA >= 16 ? 1 : 2) void mx_tile_kernel(
     if (s + 4 >= n) break;
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-  mx_store<T, TW, TA, GELU>(acc, st0 + wave * 32 * C::PITCH, out, ldo, vec, (m0 + wm * TA) * 32, a.rows,
+  mx_store<T, TW, TA, GELU>(acc, st0 + wave * 4096, out, ldo, (m0 + wm * TA) * 32, a.rows,
                             (n0 + wn * TW) * 32, w.rows);
 }
 
@@ -470,9 +446,10 @@ __global__ __launch_bounds__(256, TW * TA >= 16 ? 1 : 2) void mx_tile_kernel(
 // With 256 accumulators a SIMD holds one wave, so no other wave covers a wait,
 // and left to itself the compiler issues a fragment read right before the
 // product that needs it.  A step is one asm block of sixteen products (64
-// columns): the next step's eight fragment reads go between the first eight,
-// the stage's DMA between the others, and the one wait at its end finds the
-// reads 256 cycles old.
+// columns): the next step's eight fragment reads and half a stage's DMA go
+// between them, and the one wait at its end finds the reads old.  The DMA is
+// spread over both steps of a stage: the CU takes a KB in 16 cycles, and eight
+// of each wave's within 256 cycles held the products up.
 #define MX_P(i, j)                                                                                      \
   "v_mfma_scale_f32_32x32x64_f8f6f4 %[c" #i #j "], %[w" #i "], %[a" #j "], %[c" #i #j "], %[p" #i     \
   "], %[q" #j "] " MX_SEL " cbsz:4 blgp:4\n\t"
@@ -496,15 +473,14 @@ __global__ __launch_bounds__(256, TW * TA >= 16 ? 1 : 2) void mx_tile_kernel(
 #define MX_READS(OFF)                                                                                   \
   [bw] "v"(bw), [ba] "v"(ba), [o0] "n"(OFF), [o1] "n"((OFF) + 2048), [o2] "n"((OFF) + 4096),            \
       [o3] "n"((OFF) + 6144)
-#define MX_FIRST8                                                                                       \
+// where the reads and the DMA of a step go; D0 .. D3: a DMA, X: what else the step has to issue
+// (products in an order that changes one operand at a time)
+#define MX_STEP(X0, X1, X2, X3)                                                                         \
   MX_P(0, 0) MX_R("x0", "bw", "o0") MX_P(0, 1) MX_R("y0", "ba", "o0") MX_P(0, 2) MX_R("x1", "bw", "o1") \
-      MX_P(0, 3) MX_R("y1", "ba", "o1") MX_P(1, 0) MX_R("x2", "bw", "o2") MX_P(1, 1)                    \
-          MX_R("y2", "ba", "o2") MX_P(1, 2) MX_R("x3", "bw", "o3") MX_P(1, 3) MX_R("y3", "ba", "o3")
-#define MX_LAST8                                                                                        \
-  MX_P(2, 0) MX_P(2, 1) MX_P(2, 2) MX_P(2, 3) MX_P(3, 0) MX_P(3, 1) MX_P(3, 2) MX_P(3, 3)
-#define MX_LAST8_DMA                                                                                    \
-  MX_P(2, 0) MX_D(0) MX_P(2, 1) MX_D(1) MX_P(2, 2) MX_D(2) MX_P(2, 3) MX_D(3) MX_P(3, 0) MX_D(4)        \
-      MX_P(3, 1) MX_D(5) MX_P(3, 2) MX_D(6) MX_P(3, 3) MX_D(7)
+      MX_P(0, 3) MX_D(0) X0 MX_P(1, 3) MX_R("y1", "ba", "o1") MX_P(1, 2) MX_R("x2", "bw", "o2")         \
+          MX_P(1, 1) MX_R("y2", "ba", "o2") MX_P(1, 0) MX_D(1) X1 MX_P(2, 0) MX_R("x3", "bw", "o3")     \
+              MX_P(2, 1) MX_R("y3", "ba", "o3") MX_P(2, 2) X2 MX_P(2, 3) MX_D(2) MX_P(3, 3) X3          \
+                  MX_P(3, 2) MX_D(3) MX_P(3, 1) MX_P(3, 0) "s_waitcnt lgkmcnt(0)"
 
 struct MxFrags {
   u32x4 w[4], a[4];
@@ -517,50 +493,56 @@ struct MxDma {
   const char* scales;  // its KB of scales, per lane
 };
 
-// first step of a stage: reads the stage's second fragments at OFF
+// half a stage's DMA: four KB from g[0 .. 3] + v to LDS at m
+#define MX_DMA_IN                                                                                       \
+  [v] "v"(v), [m] "s"(m), [g0] "s"(g[0]), [g1] "s"(g[1]), [g2] "s"(g[2]), [g3] "s"(g[3])
+
+// First step of a stage: reads the stage's second fragments at OFF; fetches the second half of the
+// stage three further on (after an odd stage, that is of an even one, its scales too).
 template <int ODD, int OFF>
 __device__ inline void mx_step0(f32x16 (&acc)[4][4], const MxFrags& f, MxFrags& nx, const MxScales& sc,
-                                uint32_t bw, uint32_t ba) {
-#define MX_BODY "s_nop 1\n\t" MX_FIRST8 MX_LAST8 "s_waitcnt lgkmcnt(0)"
+                                uint32_t bw, uint32_t ba, const char* const* g, uint32_t m, uint32_t v,
+                                uint32_t ms, const char* vs) {
   if constexpr (!ODD) {
 #define MX_SEL "op_sel:[0,0,0] op_sel_hi:[0,0,0]"
-    asm volatile(MX_BODY : MX_ACC, MX_NEXT(nx) : MX_CUR(f, sc), MX_READS(OFF) : "memory");
+    asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 1\n\t" MX_STEP("", "", "", "")
+                 : MX_ACC, MX_NEXT(nx)
+                 : MX_CUR(f, sc), MX_READS(OFF), MX_DMA_IN
+                 : "memory", "scc");
 #undef MX_SEL
   } else {
 #define MX_SEL "op_sel:[0,0,0] op_sel_hi:[1,1,0]"
-    asm volatile(MX_BODY : MX_ACC, MX_NEXT(nx) : MX_CUR(f, sc), MX_READS(OFF) : "memory");
+    asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 1\n\t" MX_STEP("", "", "", "")
+                 "\n\ts_mov_b32 m0, %[ms]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[vs], off"
+                 : MX_ACC, MX_NEXT(nx)
+                 : MX_CUR(f, sc), MX_READS(OFF), MX_DMA_IN, [ms] "s"(ms), [vs] "v"(vs)
+                 : "memory", "scc");
 #undef MX_SEL
   }
-#undef MX_BODY
 }
 
-// second step of a stage: once the next stage has landed for every wave (the two after it may
-// be under way) and this one's reads are done, reads the next stage's first fragments at OFF
-// (after an odd stage also the next group's scales at SOFF) and fetches the stage four further
-// on into this one's place (v: its column offset; before an even one also scales)
+// Second step of a stage: once the next stage has landed for every wave (the two after it may be
+// under way) and this one's reads are done, reads the next stage's first fragments at OFF (after an
+// odd stage also the next group's scales at SOFF) and fetches the first half of the stage four
+// further on into this one's place.
 template <int ODD, int OFF, int SOFF>
 __device__ inline void mx_step1(f32x16 (&acc)[4][4], const MxFrags& f, MxFrags& nx, const MxScales& sc,
                                 MxScales& nsc, uint32_t bw, uint32_t ba, uint32_t sbw, uint32_t sba,
-                                const MxDma& d, uint32_t lds, uint32_t lds_scales, uint32_t v,
-                                const char* scales) {
-#define MX_DMA_IN                                                                                       \
-  [v] "v"(v), [m] "s"(lds), [g0] "s"(d.g[0]), [g1] "s"(d.g[1]), [g2] "s"(d.g[2]), [g3] "s"(d.g[3]),     \
-      [g4] "s"(d.g[4]), [g5] "s"(d.g[5]), [g6] "s"(d.g[6]), [g7] "s"(d.g[7])
+                                const char* const* g, uint32_t m, uint32_t v) {
   if constexpr (!ODD) {
 #define MX_SEL "op_sel:[1,1,0] op_sel_hi:[0,0,0]"
-    asm volatile("s_mov_b32 m0, %[m]\n\ts_waitcnt vmcnt(17)\n\ts_barrier\n\t" MX_FIRST8 MX_LAST8_DMA
-                 "s_mov_b32 m0, %[ms]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[vs], off\n\t"
-                 "s_waitcnt lgkmcnt(0)"
+    asm volatile("s_mov_b32 m0, %[m]\n\ts_waitcnt vmcnt(17)\n\ts_barrier\n\t" MX_STEP("", "", "", "")
                  : MX_ACC, MX_NEXT(nx)
-                 : MX_CUR(f, sc), MX_READS(OFF), MX_DMA_IN, [ms] "s"(lds_scales), [vs] "v"(scales)
+                 : MX_CUR(f, sc), MX_READS(OFF), MX_DMA_IN
                  : "memory", "scc");
 #undef MX_SEL
   } else {
 #define MX_SEL "op_sel:[1,1,0] op_sel_hi:[1,1,0]"
-    asm volatile("s_mov_b32 m0, %[m]\n\ts_waitcnt vmcnt(17)\n\ts_barrier\n\t" MX_FIRST8
-                 MX_RS("n0", "sbw", "t0") MX_RS("n1", "sbw", "t1") MX_RS("n2", "sbw", "t2")
-                 MX_RS("n3", "sbw", "t3") MX_RS("r0", "sba", "t0") MX_RS("r1", "sba", "t1")
-                 MX_RS("r2", "sba", "t2") MX_RS("r3", "sba", "t3") MX_LAST8_DMA "s_waitcnt lgkmcnt(0)"
+    asm volatile("s_mov_b32 m0, %[m]\n\ts_waitcnt vmcnt(17)\n\ts_barrier\n\t" MX_STEP(
+                     MX_RS("n0", "sbw", "t0") MX_RS("n1", "sbw", "t1"),
+                     MX_RS("n2", "sbw", "t2") MX_RS("n3", "sbw", "t3"),
+                     MX_RS("r0", "sba", "t0") MX_RS("r1", "sba", "t1"),
+                     MX_RS("r2", "sba", "t2") MX_RS("r3", "sba", "t3"))
                  : MX_ACC, MX_NEXT(nx), [n0] "=&v"(nsc.w[0]), [n1] "=&v"(nsc.w[1]), [n2] "=&v"(nsc.w[2]),
                    [n3] "=&v"(nsc.w[3]), [r0] "=&v"(nsc.a[0]), [r1] "=&v"(nsc.a[1]), [r2] "=&v"(nsc.a[2]),
                    [r3] "=&v"(nsc.a[3])
@@ -569,8 +551,8 @@ __device__ inline void mx_step1(f32x16 (&acc)[4][4], const MxFrags& f, MxFrags& 
                  : "memory", "scc");
 #undef MX_SEL
   }
-#undef MX_DMA_IN
 }
+#undef MX_DMA_IN
 
 // Work-groups stay for many tiles.  The DMA runs four stages ahead of the
 // products as one stream over all of them, so a tile's first stages are loaded
@@ -578,7 +560,7 @@ __device__ inline void mx_step1(f32x16 (&acc)[4][4], const MxFrags& f, MxFrags& 
 // LDS of its own (4 KB a wave).
 template <typename T, bool GELU>
 __global__ __launch_bounds__(256, 1) void mx_big_kernel(MxMat a, MxMat w, const uint16_t* __restrict__ bias,
-                                                        uint16_t* __restrict__ out, long long ldo, int vec,
+                                                        uint16_t* __restrict__ out, long long ldo,
                                                         int groups, int mt, int nt, int per_xcd) {
   using C = MxTile<4, 4>;
   constexpr int ST = C::CODES + C::SCALES, PAIR = 2 * ST;
@@ -624,30 +606,30 @@ __global__ __launch_bounds__(256, 1) void mx_big_kernel(MxMat a, MxMat w, const 
     }
   };
   const uint32_t dst = lds0 + wave * 8192, sdst = lds0 + C::CODES + wave * 1024;
-  auto issue_pair = [&](uint32_t off) {  // in the order of the steps below: the scales after the first eight
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[v], %[g]" ::[m] "s"(
-                       dst + off + (i >> 3) * ST + (i & 7) * 1024),
-                   [v] "v"(col(i >> 3)), [g] "s"(d.g[i & 7])
+  auto issue = [&](uint32_t off, int i) {  // KB i of a pair
+    asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[v], %[g]" ::[m] "s"(
+                     dst + off + (i >> 3) * ST + (i & 7) * 1024),
+                 [v] "v"(col(i >> 3)), [g] "s"(d.g[i & 7])
+                 : "memory");
+    if (i == 7)  // in the order of the steps: the scales after the even stage
+      asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[v], off" ::[m] "s"(sdst + off),
+                   [v] "v"(d.scales + (size_t)ls * 128)
                    : "memory");
-      if (i == 7)
-        asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[v], off" ::[m] "s"(sdst + off),
-                     [v] "v"(d.scales + (size_t)ls * 128)
-                     : "memory");
-    }
-    next_pair();
   };
+  // two pairs but for the last half stage, which the first step fetches
   aim();
-  issue_pair(0);
-  issue_pair(PAIR);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) issue(0, i);
+  next_pair();
+#pragma unroll
+  for (int i = 0; i < 12; ++i) issue(PAIR, i);
   // fragment and scale addresses of the pair in use and of the other one
   uint32_t bw = lds0 + wn * 8192 + l16, ba = lds0 + 16384 + wm * 8192 + l16;
   uint32_t sw = lds0 + wn * 1024 + lane * 4, sa = lds0 + 2048 + wm * 1024 + lane * 4;
   uint32_t off = 0;
   MxFrags f0, f1;
   MxScales sc, nsc;
-  asm volatile("s_waitcnt vmcnt(17)\n\ts_barrier\n\t" MX_R("x0", "bw", "o0") MX_R("y0", "ba", "o0")
+  asm volatile("s_waitcnt vmcnt(13)\n\ts_barrier\n\t" MX_R("x0", "bw", "o0") MX_R("y0", "ba", "o0")
                MX_R("x1", "bw", "o1") MX_R("y1", "ba", "o1") MX_R("x2", "bw", "o2") MX_R("y2", "ba", "o2")
                MX_R("x3", "bw", "o3") MX_R("y3", "ba", "o3") MX_RS("n0", "sbw", "t0") MX_RS("n1", "sbw", "t1")
                MX_RS("n2", "sbw", "t2") MX_RS("n3", "sbw", "t3") MX_RS("r0", "sba", "t0")
@@ -667,26 +649,154 @@ __global__ __launch_bounds__(256, 1) void mx_big_kernel(MxMat a, MxMat w, const 
     mx_bias_init<T>(acc, bias, (float*)own, (n0 + wn * 4) * 32, w.rows);
     for (int g = groups; g > 0; --g) {
       const uint32_t other = PAIR - 2 * off;  // from this pair to the other one (off: 0 or PAIR)
-      mx_step0<0, 1024>(acc, f0, f1, sc, bw, ba);
-      mx_step1<0, ST, 0>(acc, f1, f0, sc, nsc, bw, ba, sw, sa, d, dst + off, sdst + off, col(0),
-                         d.scales + (size_t)ls * 128);
-      mx_step0<1, ST + 1024>(acc, f0, f1, sc, bw, ba);
-      const uint32_t o_bw = bw + other, o_ba = ba + other, o_sw = sw + other, o_sa = sa + other;
-      mx_step1<1, 0, C::CODES>(acc, f1, f0, sc, nsc, o_bw, o_ba, o_sw, o_sa, d, dst + off + ST, 0, col(1),
-                               nullptr);
+      mx_step0<0, 1024>(acc, f0, f1, sc, bw, ba, d.g + 4, dst + PAIR - off + ST + 4096, col(1), 0, nullptr);
       next_pair();
+      mx_step1<0, ST, 0>(acc, f1, f0, sc, nsc, bw, ba, sw, sa, d.g, dst + off, col(0));
+      mx_step0<1, ST + 1024>(acc, f0, f1, sc, bw, ba, d.g + 4, dst + off + 4096, col(0), sdst + off,
+                             d.scales + (size_t)ls * 128);
+      const uint32_t o_bw = bw + other, o_ba = ba + other, o_sw = sw + other, o_sa = sa + other;
+      mx_step1<1, 0, C::CODES>(acc, f1, f0, sc, nsc, o_bw, o_ba, o_sw, o_sa, d.g, dst + off + ST, col(1));
       sc = nsc;
       bw = o_bw, ba = o_ba, sw = o_sw, sa = o_sa, off = PAIR - off;
     }
     // the last products' registers are readable after 18 cycles of issue
     asm volatile("s_nop 15\n\ts_nop 15" : MX_ACC);
-    mx_store_big<T, GELU>(acc, own, out, ldo, vec, (m0 + wm * 4) * 32, a.rows, (n0 + wn * 4) * 32, w.rows);
+    mx_store<T, 4, 4, GELU>(acc, own, out, ldo, (m0 + wm * 4) * 32, a.rows, (n0 + wn * 4) * 32, w.rows);
     id += step;
     if (id >= end) break;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 // ---- end of the 256 x 256 tile
+
+// ---- small launches: the columns split over the waves ------------------------
+// NB x MB blocks of 32 x 32 a work-group; its waves take units of 128 columns in
+// turn, so every fragment is loaded once, straight into registers (no staging,
+// no barrier in the loop), DEPTH units ahead.  The waves' sums meet in LDS, in
+// the order of the waves, and each wave finishes the blocks of its number.
+template <int NB, int MB> struct MxUnit {
+  u32x4 w[2][NB], a[2][MB];
+  uint32_t sw[NB], sa[MB];
+};
+
+template <typename T, int NB, int MB, int WAVES, int DEPTH, bool GELU>
+__global__ __launch_bounds__(64 * WAVES, NB * MB >= 8 ? 1 : 2) void mx_split_kernel(
+    MxMat a, MxMat w, const uint16_t* __restrict__ bias, uint16_t* __restrict__ out, long long ldo,
+    int groups, int mt, int nt, int per_xcd) {
+  constexpr int P = NB * MB, ROUND = 128 / (4 * WAVES) < P ? 128 / (4 * WAVES) : P;  // blocks in 128 KB
+  __shared__ f32x4 part[WAVES][ROUND][4][64];
+  const int id = mx_first(per_xcd);
+  if (id >= mx_end(mt, nt, per_xcd)) return;
+  int m0, n0;
+  mx_place(id, mt, nt, MB, NB, m0, n0);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = 2 * groups;
+  const char *pw[NB], *pa[MB];
+  const uint32_t *qw[NB], *qa[MB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {
+    const long long row = min(n0 + i, w.blocks - 1);
+    pw[i] = w.codes + row * groups * 4096;
+    qw[i] = w.scales + row * groups * 64;
+  }
+#pragma unroll
+  for (int j = 0; j < MB; ++j) {
+    const long long row = min(m0 + j, a.blocks - 1);
+    pa[j] = a.codes + row * groups * 4096;
+    qa[j] = a.scales + row * groups * 64;
+  }
+  auto load = [&](int s, MxUnit<NB, MB>& t) {
+    const size_t o = (size_t)s * 2048 + lane * 16, os = (size_t)(s >> 1) * 64 + lane;
+    const int sh = 16 * (s & 1);  // an odd unit's scales are the upper half
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      t.w[0][i] = *(const u32x4*)(pw[i] + o);
+      t.w[1][i] = *(const u32x4*)(pw[i] + o + 1024);
+      t.sw[i] = qw[i][os] >> sh;
+    }
+#pragma unroll
+    for (int j = 0; j < MB; ++j) {
+      t.a[0][j] = *(const u32x4*)(pa[j] + o);
+      t.a[1][j] = *(const u32x4*)(pa[j] + o + 1024);
+      t.sa[j] = qa[j][os] >> sh;
+    }
+  };
+  f32x16 acc[NB][MB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int j = 0; j < MB; ++j) acc[i][j] = zero16();
+  auto mul = [&](const MxUnit<NB, MB>& t) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int j = 0; j < MB; ++j) acc[i][j] = mx_mfma<0>(t.w[0][i], t.a[0][j], acc[i][j], t.sw[i], t.sa[j]);
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int j = 0; j < MB; ++j) acc[i][j] = mx_mfma<1>(t.w[1][i], t.a[1][j], acc[i][j], t.sw[i], t.sa[j]);
+  };
+  MxUnit<NB, MB> ring[DEPTH];
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d)
+    if (wave + d * WAVES < n) load(wave + d * WAVES, ring[d]);
+  for (int s = wave; s < n; s += DEPTH * WAVES) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      if (s + d * WAVES < n) mul(ring[d]);
+      if (s + (d + DEPTH) * WAVES < n) load(s + (d + DEPTH) * WAVES, ring[d]);
+    }
+  }
+#pragma unroll
+  for (int p0 = 0; p0 < P; p0 += ROUND) {
+    if (p0) __syncthreads();
+#pragma unroll
+    for (int p = p0; p < p0 + ROUND && p < P; ++p)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x16& c = acc[p / MB][p % MB];
+        part[wave][p - p0][q][lane] = f32x4{c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]};
+      }
+    __syncthreads();
+    // quarter q of block p: four features of each token
+    const int quarters = 4 * (P - p0 < ROUND ? P - p0 : ROUND);
+    for (int pq = wave; pq < quarters; pq += WAVES) {
+      const int p = pq >> 2, q = pq & 3;
+      f32x4 v = part[0][p][q][lane];
+#pragma unroll
+      for (int x = 1; x < WAVES; ++x) {
+        const f32x4 y = part[x][p][q][lane];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += y[e];
+      }
+      const int m = (m0 + (p + p0) % MB) * 32 + (lane & 31);
+      const int f = (n0 + (p + p0) / MB) * 32 + 8 * q + 4 * (lane >> 5);
+      if (m < a.rows && f < w.rows) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (bias) v[e] += T::to_f(bias[min(f + e, w.rows - 1)]);
+          if (GELU) v[e] = mx_gelu(v[e]);
+        }
+        mx_put(out + m * ldo + f, u32x2{Pk<T>::pack(v[0], v[1]), Pk<T>::pack(v[2], v[3])}, w.rows - f);
+      }
+    }
+  }
+}
+
+template <typename T, int NB, int MB, int WAVES, int DEPTH>
+static int mx_split_launch(const MxMat& a, const MxMat& w, const uint16_t* bias, int act, uint16_t* out,
+                           long long ldo, int groups, hipStream_t st) {
+  const int mt = cdiv(a.blocks, MB), nt = cdiv(w.blocks, NB);
+  const long long tiles = (long long)mt * nt;
+  T2T_REQUIRE(tiles <= INT_MAX / 2, "mxfp4_product: M=%d N=%d", a.rows, w.rows);
+  const int per = cdiv(tiles, 8);
+  auto kernel = act == T2T_ACT_GELU_TANH ? mx_split_kernel<T, NB, MB, WAVES, DEPTH, true>
+                                         : mx_split_kernel<T, NB, MB, WAVES, DEPTH, false>;
+  hipLaunchKernelGGL(kernel, dim3(8 * per), dim3(64 * WAVES), 0, st, a, w, bias, out, ldo, groups, mt, nt,
+                     per);
+  T2T_LAUNCH_CHECK("mxfp4_product");
+  return T2T_OK;
+}
 
 template <typename T, int TW, int TA>
 static int mx_tile_launch(const MxMat& a, const MxMat& w, const uint16_t* bias, int act, uint16_t* out,
@@ -695,12 +805,13 @@ static int mx_tile_launch(const MxMat& a, const MxMat& w, const uint16_t* bias, 
   const long long tiles = (long long)mt * nt;
   T2T_REQUIRE(tiles <= INT_MAX / 2, "mxfp4_product: M=%d N=%d", a.rows, w.rows);
   const int per = cdiv(tiles, 8);
-  const int vec = ldo % 8 == 0 && (uintptr_t)out % 16 == 0;
-  auto kernel = act == T2T_ACT_GELU_TANH ? mx_tile_kernel<T, TW, TA, true> : mx_tile_kernel<T, TW, TA, false>;
-  if constexpr (TW * TA == 16) kernel = act == T2T_ACT_GELU_TANH ? mx_big_kernel<T, true> : mx_big_kernel<T, false>;
-  // the 256 x 256 tile fills a CU: 32 of its work-groups an XCD, which go through the tiles
-  const int slots = TW * TA == 16 && per > 32 ? 32 : per;
-  hipLaunchKernelGGL(kernel, dim3(8 * slots), dim3(256), 0, st, a, w, bias, out, ldo, vec, groups, mt, nt, per);
+  auto launch = [&](auto kernel, int slots) {
+    hipLaunchKernelGGL(kernel, dim3(8 * slots), dim3(256), 0, st, a, w, bias, out, ldo, groups, mt, nt, per);
+  };
+  if constexpr (TW * TA == 16)  // fills a CU: 32 work-groups an XCD, which go through the tiles
+    launch(act == T2T_ACT_GELU_TANH ? mx_big_kernel<T, true> : mx_big_kernel<T, false>, per < 32 ? per : 32);
+  else
+    launch(act == T2T_ACT_GELU_TANH ? mx_tile_kernel<T, TW, TA, true> : mx_tile_kernel<T, TW, TA, false>, per);
   T2T_LAUNCH_CHECK("mxfp4_product");
   return T2T_OK;
 }
