@@ -129,9 +129,9 @@ def test_mxfp4_entries_reject_bad_arguments():
 
     def linear(x=p, dt=1, xs=64, act=0, M=4, N=8, K=64, rs=8, ws=p, nb=1 << 20):
         return L.t2t_mxfp4_linear(x, dt, xs, p, p, None, act, p, rs, M, N, K, ws, nb, None)
-    need = L.t2t_mxfp4_linear_ws_bytes(4, 8, 64)
-    assert linear(nb=need - 1) == 2 and b"workspace" in L.t2t_last_error()
-    assert linear(ws=None) == 2 and linear(x=None) == 1 and linear(xs=60) == 1 and linear(dt=3) == 1
+    need = L.t2t_mxfp4_linear_ws_bytes(400, 8, 64)
+    assert linear(M=400, nb=need - 1) == 2 and b"workspace" in L.t2t_last_error()
+    assert linear(M=400, ws=None) == 2 and linear(x=None) == 1 and linear(xs=60) == 1 and linear(dt=3) == 1
     assert linear(act=7) == 1 and linear(rs=4) == 1 and linear(K=31) == 1 and linear(x=odd) == 1
     assert linear(M=0) == 0
 

@@ -17,6 +17,7 @@
 #include <type_traits>
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 static inline long long mx_row_blocks(int M) { return ((long long)M + 31) / 32; }
 static inline int mx_kp(int K) { return (K + 255) / 256 * 256; }
@@ -72,14 +73,13 @@ template <> struct MxCvt<F16T> {
 // [4, 8); the conversion rounds to nearest even and saturates at 6.
 template <typename T>
 __device__ inline void mx_block(const u32x4 (&x)[4], u32x4& codes, uint32_t& byte) {
-  uint32_t top = 0;
+  u16x2 both{0, 0};
 #pragma unroll
   for (int v = 0; v < 4; ++v)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t lo = x[v][i] & 0x7fffu, hi = (x[v][i] >> 16) & 0x7fffu;
-      top = max(top, max(lo, hi));
-    }
+    for (int i = 0; i < 4; ++i)
+      both = __builtin_elementwise_max(both, __builtin_bit_cast(u16x2, x[v][i] & 0x7fff7fffu));
+  const uint32_t top = max((uint32_t)both[0], (uint32_t)both[1]);
   if (top >= MxCvt<T>::inf) {
     byte = 255;
     codes = u32x4{0u, 0u, 0u, 0u};
@@ -237,8 +237,7 @@ typedef __attribute__((address_space(1))) void mx_glb_t;
 template <int TW, int TA> struct MxTile {
   static constexpr int RB = 2 * (TW + TA);          // row blocks: 2 TW of weights, 2 TA of tokens
   static constexpr int CODES = RB * 2048;           // a stage's codes
-  static constexpr int SCALES = RB * 256;
-  static constexpr int STAGE = CODES + SCALES > 16384 ? CODES + SCALES : 16384;  // or 4 KB a wave, at the end
+  static constexpr int STAGE = CODES + RB * 256;    // with its scales (of every second stage)
 };
 
 // Consecutive work-groups go to the eight XCDs in turn: each takes a run of
@@ -256,28 +255,25 @@ __device__ inline void mx_place(int id, int mt, int nt, int mb, int nb, int& m0,
   n0 = (in / gm) * nb;
 }
 
-// the sums start at the bias, which comes through LDS of the wave's own (128 TW bytes): a lane
-// needs 16 TW of the wave's 32 TW features
+// Adds the bias, which comes through LDS of the wave's own (128 TW bytes): a lane needs 16 TW of the
+// wave's 32 TW features.
 template <typename T, int TW, int TA>
-__device__ inline void mx_bias_init(f32x16 (&acc)[TW][TA], const uint16_t* __restrict__ bias, float* own,
-                                    int f0, int rows) {
+__device__ inline void mx_bias_add(f32x16 (&acc)[TW][TA], const uint16_t* __restrict__ bias, float* own, int f0,
+                                   int rows) {
+  if (!bias) return;
   const int lane = threadIdx.x & 63, hh = lane >> 5;
-  if (bias)
 #pragma unroll
-    for (int i = lane; i < 32 * TW; i += 64) own[i] = T::to_f(bias[min(f0 + i, rows - 1)]);
+  for (int i = lane; i < 32 * TW; i += 64) own[i] = T::to_f(bias[min(f0 + i, rows - 1)]);
 #pragma unroll
-  for (int i = 0; i < TW; ++i) {
-    f32x16 b0 = zero16();
-    if (bias)
+  for (int i = 0; i < TW; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f32x4 v = *(const f32x4*)(own + 32 * i + 8 * q + 4 * hh);
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 v = *(const f32x4*)(own + 32 * i + 8 * q + 4 * hh);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) b0[4 * q + e] = v[e];
-      }
+      for (int j = 0; j < TA; ++j)
 #pragma unroll
-    for (int j = 0; j < TA; ++j) acc[i][j] = b0;
-  }
+        for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += v[e];
+    }
 }
 
 // The values of one row, the first n of which are inside, to an o of any alignment (rows of odd
@@ -336,110 +332,6 @@ __device__ inline void mx_store(const f32x16 (&acc)[TW][TA], char* so, uint16_t*
     }
   }
   put(TA - 1, TW - IW);
-}
-
-template <typename T, int TW, int TA, bool GELU>
-__global__ __launch_bounds__(256, 2) void mx_tile_kernel(
-    MxMat a, MxMat w, const uint16_t* __restrict__ bias, uint16_t* __restrict__ out, long long ldo,
-    int groups, int mt, int nt, int per_xcd) {
-  using C = MxTile<TW, TA>;
-  __shared__ __attribute__((aligned(1024))) char st0[C::STAGE];
-  __shared__ __attribute__((aligned(1024))) char st1[C::STAGE];
-  __shared__ __attribute__((aligned(1024))) char st2[C::STAGE];
-  __shared__ __attribute__((aligned(1024))) char st3[C::STAGE];
-  const int id = mx_first(per_xcd);
-  if (id >= mx_end(mt, nt, per_xcd)) return;
-  int m0, n0;
-  mx_place(id, mt, nt, 2 * TA, 2 * TW, m0, n0);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wn = wave & 1, wm = wave >> 1;
-  // this wave's share of the stage's DMA: TW + TA KB of codes, and 1 KB of scales (four row
-  // blocks; with fewer than sixteen some waves fetch the same)
-  const char* src[TW + TA];
-#pragma unroll
-  for (int i = 0; i < TW + TA; ++i) {
-    const int q = wave * (TW + TA) + i, rb = q >> 1;
-    const long long row = rb < 2 * TW ? min(n0 + rb, w.blocks - 1) : min(m0 + rb - 2 * TW, a.blocks - 1);
-    src[i] = (rb < 2 * TW ? w.codes : a.codes) + row * groups * 4096 + (q & 1) * 1024;
-  }
-  constexpr int SI = (C::RB + 3) / 4;
-  const int srb = min(4 * (wave % SI) + (lane >> 4), C::RB - 1);
-  const long long srow = srb < 2 * TW ? min(n0 + srb, w.blocks - 1) : min(m0 + srb - 2 * TW, a.blocks - 1);
-  const char* ssrc = (const char*)(srb < 2 * TW ? w.scales : a.scales) + srow * groups * 256 + (lane & 15) * 16;
-  const int n = 2 * groups;  // stages
-  // Stages past the last keep the counts of loads in flight what they are, at the price of one
-  // line each: every lane reads the same 16 bytes of the last stage.
-  auto issue = [&](int s, char* st, auto ODD) {
-    constexpr int O = decltype(ODD)::value;
-    const int t = min(s, n - 2 + O);
-    const uint32_t voff = s < n ? lane * 16 : 0;
-#pragma unroll
-    for (int i = 0; i < TW + TA; ++i)
-      __builtin_amdgcn_global_load_lds((const mx_glb_t*)(src[i] + (size_t)t * 2048 + voff),
-                                       (mx_lds_t*)(st + (wave * (TW + TA) + i) * 1024), 16, 0, 0);
-    if constexpr (!O)
-      __builtin_amdgcn_global_load_lds((const mx_glb_t*)(ssrc + (size_t)(t >> 1) * 256),
-                                       (mx_lds_t*)(st + C::CODES + (wave % SI) * 1024), 16, 0, 0);
-  };
-  f32x16 acc[TW][TA];
-  mx_bias_init<T>(acc, bias, (float*)(st3 + wave * 128 * TW), (n0 + wn * TW) * 32, w.rows);
-  __syncthreads();
-  u32x4 fw[2][TW], fa[2][TA];
-  uint32_t sw[TW], sa[TA];
-  auto frags = [&](const char* st, int c) {
-#pragma unroll
-    for (int i = 0; i < TW; ++i)
-      fw[c][i] = *(const u32x4*)(st + ((wn * TW + i) * 2 + c) * 1024 + lane * 16);
-#pragma unroll
-    for (int j = 0; j < TA; ++j)
-      fa[c][j] = *(const u32x4*)(st + ((2 * TW + wm * TA + j) * 2 + c) * 1024 + lane * 16);
-  };
-  auto mul = [&](auto S, int c) {
-#pragma unroll
-    for (int i = 0; i < TW; ++i)
-#pragma unroll
-      for (int j = 0; j < TA; ++j)
-        acc[i][j] = mx_mfma<decltype(S)::value>(fw[c][i], fa[c][j], acc[i][j], sw[i], sa[j]);
-  };
-  // one stage: its first fragments are in registers; the second ones are read under the first
-  // products, the next stage's first ones under the second products
-  auto stage = [&](int s, char* cur, const char* nxt, auto ODD) {
-    constexpr int O = decltype(ODD)::value;
-    if constexpr (!O) {
-#pragma unroll
-      for (int i = 0; i < TW; ++i) sw[i] = *(const uint32_t*)(cur + C::CODES + (wn * TW + i) * 256 + lane * 4);
-#pragma unroll
-      for (int j = 0; j < TA; ++j)
-        sa[j] = *(const uint32_t*)(cur + C::CODES + (2 * TW + wm * TA + j) * 256 + lane * 4);
-    }
-    frags(cur, 1);
-    mul(std::integral_constant<int, 2 * O>{}, 0);
-    // stage s + 1 of every wave has landed and this stage's reads are done; the two stages
-    // after it may still be under way
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * (TW + TA) + 1) : "memory");
-    issue(s + 4, cur, ODD);
-    frags(nxt, 0);
-    mul(std::integral_constant<int, 2 * O + 1>{}, 1);
-  };
-  using Even = std::integral_constant<int, 0>;
-  using Odd = std::integral_constant<int, 1>;
-  issue(0, st0, Even{});
-  issue(1, st1, Odd{});
-  issue(2, st2, Even{});
-  issue(3, st3, Odd{});
-  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(3 * (TW + TA) + 1) : "memory");
-  frags(st0, 0);
-  for (int s = 0;; s += 4) {
-    stage(s, st0, st1, Even{});
-    stage(s + 1, st1, st2, Odd{});
-    if (s + 2 >= n) break;
-    stage(s + 2, st2, st3, Even{});
-    stage(s + 3, st3, st0, Odd{});
-    if (s + 4 >= n) break;
-  }
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-  mx_store<T, TW, TA, GELU>(acc, st0 + wave * 4096, out, ldo, (m0 + wm * TA) * 32, a.rows,
-                            (n0 + wn * TW) * 32, w.rows);
 }
 
 // ---- the 256 x 256 tile: its inner loop is written out ----------------------
@@ -563,7 +455,7 @@ __global__ __launch_bounds__(256, 1) void mx_big_kernel(MxMat a, MxMat w, const 
                                                         uint16_t* __restrict__ out, long long ldo,
                                                         int groups, int mt, int nt, int per_xcd) {
   using C = MxTile<4, 4>;
-  constexpr int ST = C::CODES + C::SCALES, PAIR = 2 * ST;
+  constexpr int ST = C::STAGE, PAIR = 2 * ST;
   static_assert(ST + 8192 < 65536 && C::CODES + 1024 < 65536, "LDS offsets of 16 bits");
   __shared__ __attribute__((aligned(1024))) char lds[4 * ST + 4 * 4096];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -646,7 +538,11 @@ __global__ __launch_bounds__(256, 1) void mx_big_kernel(MxMat a, MxMat w, const 
   for (;;) {
     int m0, n0;
     mx_place(id, mt, nt, 8, 8, m0, n0);
-    mx_bias_init<T>(acc, bias, (float*)own, (n0 + wn * 4) * 32, w.rows);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = zero16();
+    mx_bias_add<T>(acc, bias, (float*)own, (n0 + wn * 4) * 32, w.rows);  // the sums start at the bias
     for (int g = groups; g > 0; --g) {
       const uint32_t other = PAIR - 2 * off;  // from this pair to the other one (off: 0 or PAIR)
       mx_step0<0, 1024>(acc, f0, f1, sc, bw, ba, d.g + 4, dst + PAIR - off + ST + 4096, col(1), 0, nullptr);
@@ -669,43 +565,191 @@ __global__ __launch_bounds__(256, 1) void mx_big_kernel(MxMat a, MxMat w, const 
 }
 // ---- end of the 256 x 256 tile
 
-// ---- small launches: the columns split over the waves ------------------------
-// NB x MB blocks of 32 x 32 a work-group; its waves take units of 128 columns in
-// turn, so every fragment is loaded once, straight into registers (no staging,
-// no barrier in the loop), DEPTH units ahead.  The waves' sums meet in LDS, in
-// the order of the waves, and each wave finishes the blocks of its number.
-template <int NB, int MB> struct MxUnit {
-  u32x4 w[2][NB], a[2][MB];
-  uint32_t sw[NB], sa[MB];
+// ---- the 128 x 128 tile ------------------------------------------------------
+// The same with a whole stage a step: eight products, the next stage's eight
+// fragment reads and the DMA of the stage four further on.  Bound by LDS: at 128
+// bytes a cycle a stage's reads (32 KB) and the DMA's writes (18 KB) take 400
+// cycles, its products 256.  Two work-groups fit a CU; eight stages instead
+// (one work-group a CU) gained nothing at 512 x 5120 x 5120 (11.5 and 12.3 us).
+#define MX_Q(c, i, j, SEL)                                                                              \
+  "v_mfma_scale_f32_32x32x64_f8f6f4 %[c" #i #j "], %[w" #c #i "], %[a" #c #j "], %[c" #i #j           \
+  "], %[p" #i "], %[q" #j "] " SEL " cbsz:4 blgp:4\n\t"
+#define MX_MID_STEP(S0, S1, X)                                                                          \
+  "s_mov_b32 m0, %[m]\n\ts_waitcnt vmcnt(9)\n\ts_barrier\n\t" MX_Q(0, 0, 0, S0) MX_R("x00", "bw", "o0") \
+      MX_R("y00", "ba", "o0") MX_Q(0, 0, 1, S0) MX_R("x01", "bw", "o1") MX_R("y01", "ba", "o1")         \
+          MX_Q(0, 1, 1, S0) MX_D(0) MX_R("x10", "bw", "o2") MX_Q(0, 1, 0, S0) MX_R("y10", "ba", "o2")   \
+              MX_D(1) MX_Q(1, 0, 0, S1) MX_R("x11", "bw", "o3") MX_R("y11", "ba", "o3") X               \
+                  MX_Q(1, 0, 1, S1) MX_D(2) MX_Q(1, 1, 1, S1) MX_D(3) MX_Q(1, 1, 0, S1)
+struct MxMidFrags {
+  u32x4 w[2][2], a[2][2];  // [fragment of the stage][block]
 };
+struct MxMidScales {
+  uint32_t w[2], a[2];
+};
+// OFF: where the next stage lies; after an odd stage its scales are read too (SOFF), with an even
+// one the DMA fetches scales
+template <int ODD, int OFF, int SOFF>
+__device__ inline void mx_mid_step(f32x16 (&acc)[2][2], const MxMidFrags& f, MxMidFrags& nx,
+                                   const MxMidScales& sc, MxMidScales& nsc, uint32_t bw, uint32_t ba,
+                                   uint32_t sbw, uint32_t sba, const char* const (&g)[4], uint32_t m, uint32_t v,
+                                   uint32_t ms, const char* vs) {
+#define MX_MID_OUT                                                                                      \
+  [c00] "+v"(acc[0][0]), [c01] "+v"(acc[0][1]), [c10] "+v"(acc[1][0]), [c11] "+v"(acc[1][1]),           \
+      [x00] "=&v"(nx.w[0][0]), [x01] "=&v"(nx.w[0][1]), [x10] "=&v"(nx.w[1][0]), [x11] "=&v"(nx.w[1][1]), \
+      [y00] "=&v"(nx.a[0][0]), [y01] "=&v"(nx.a[0][1]), [y10] "=&v"(nx.a[1][0]), [y11] "=&v"(nx.a[1][1])
+#define MX_MID_IN                                                                                       \
+  [w00] "v"(f.w[0][0]), [w01] "v"(f.w[0][1]), [w10] "v"(f.w[1][0]), [w11] "v"(f.w[1][1]),               \
+      [a00] "v"(f.a[0][0]), [a01] "v"(f.a[0][1]), [a10] "v"(f.a[1][0]), [a11] "v"(f.a[1][1]),           \
+      [p0] "v"(sc.w[0]), [p1] "v"(sc.w[1]), [q0] "v"(sc.a[0]), [q1] "v"(sc.a[1]), [bw] "v"(bw),         \
+      [ba] "v"(ba), [o0] "n"(OFF), [o1] "n"(OFF + 2048), [o2] "n"(OFF + 1024), [o3] "n"(OFF + 3072),    \
+      [m] "s"(m), [v] "v"(v), [g0] "s"(g[0]), [g1] "s"(g[1]), [g2] "s"(g[2]), [g3] "s"(g[3])
+  if constexpr (!ODD)
+    asm volatile(MX_MID_STEP("op_sel:[0,0,0] op_sel_hi:[0,0,0]", "op_sel:[1,1,0] op_sel_hi:[0,0,0]", "")
+                 "s_mov_b32 m0, %[ms]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[vs], off\n\ts_waitcnt lgkmcnt(0)"
+                 : MX_MID_OUT
+                 : MX_MID_IN, [ms] "s"(ms), [vs] "v"(vs)
+                 : "memory", "scc");
+  else
+    asm volatile(MX_MID_STEP("op_sel:[0,0,0] op_sel_hi:[1,1,0]", "op_sel:[1,1,0] op_sel_hi:[1,1,0]",
+                             MX_RS("n0", "sbw", "t0") MX_RS("n1", "sbw", "t1") MX_RS("r0", "sba", "t0")
+                                 MX_RS("r1", "sba", "t1")) "s_waitcnt lgkmcnt(0)"
+                 : MX_MID_OUT, [n0] "=&v"(nsc.w[0]), [n1] "=&v"(nsc.w[1]), [r0] "=&v"(nsc.a[0]),
+                   [r1] "=&v"(nsc.a[1])
+                 : MX_MID_IN, [sbw] "v"(sbw), [sba] "v"(sba), [t0] "n"(SOFF), [t1] "n"(SOFF + 256)
+                 : "memory", "scc");
+#undef MX_MID_OUT
+#undef MX_MID_IN
+}
 
-template <typename T, int NB, int MB, int WAVES, int DEPTH, bool GELU>
-__global__ __launch_bounds__(64 * WAVES, NB * MB >= 8 ? 1 : 2) void mx_split_kernel(
-    MxMat a, MxMat w, const uint16_t* __restrict__ bias, uint16_t* __restrict__ out, long long ldo,
-    int groups, int mt, int nt, int per_xcd) {
-  constexpr int P = NB * MB, ROUND = 128 / (4 * WAVES) < P ? 128 / (4 * WAVES) : P;  // blocks in 128 KB
-  __shared__ f32x4 part[WAVES][ROUND][4][64];
+template <typename T, bool GELU>
+__global__ __launch_bounds__(256, 2) void mx_mid_kernel(MxMat a, MxMat w, const uint16_t* __restrict__ bias,
+                                                        uint16_t* __restrict__ out, long long ldo, int groups,
+                                                        int mt, int nt, int per_xcd) {
+  using C = MxTile<2, 2>;
+  constexpr int ST = C::STAGE, PAIR = 2 * ST;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * ST];
   const int id = mx_first(per_xcd);
   if (id >= mx_end(mt, nt, per_xcd)) return;
   int m0, n0;
-  mx_place(id, mt, nt, MB, NB, m0, n0);
+  mx_place(id, mt, nt, 4, 4, m0, n0);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wn = wave & 1, wm = wave >> 1, n = 2 * groups;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(mx_lds_t*)lds, l16 = lane * 16;
+  const char* g[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int rb = wave * 2 + (i >> 1);
+    const long long row = rb < 4 ? min(n0 + rb, w.blocks - 1) : min(m0 + rb - 4, a.blocks - 1);
+    g[i] = (rb < 4 ? w.codes : a.codes) + row * groups * 4096 + (i & 1) * 1024;
+  }
+  // 1 KB of scales, four row blocks; waves 0 and 2, 1 and 3 fetch the same
+  const int srb = 4 * wn + (lane >> 4);
+  const long long srow = srb < 4 ? min(n0 + srb, w.blocks - 1) : min(m0 + srb - 4, a.blocks - 1);
+  const char* gs = (const char*)(srb < 4 ? w.scales : a.scales) + srow * groups * 256 + (lane & 15) * 16;
+  const uint32_t dst = lds0 + wave * 4096, sdst = lds0 + C::CODES + wn * 1024;
+  // past the last stage every lane reads one line of it, so that the counts of loads in flight stay
+  auto col = [&](int s) { return (uint32_t)min(s, n - 2 + (s & 1)) * 2048 + (s < n ? l16 : 0); };
+  auto scol = [&](int s) { return gs + (size_t)(min(s, n - 2) >> 1) * 256; };
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[v], %[g]" ::[m] "s"(
+                       dst + s * ST + i * 1024),
+                   [v] "v"(col(s)), [g] "s"(g[i])
+                   : "memory");
+    if (!(s & 1))
+      asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[v], off" ::[m] "s"(sdst + s * ST),
+                   [v] "v"(scol(s))
+                   : "memory");
+  }
+  uint32_t bw = lds0 + wn * 4096 + l16, ba = lds0 + 8192 + wm * 4096 + l16;
+  uint32_t sw = lds0 + wn * 512 + lane * 4, sa = lds0 + 1024 + wm * 512 + lane * 4;
+  uint32_t off = 0;
+  MxMidFrags f0, f1;
+  MxMidScales sc, nsc;
+  asm volatile("s_waitcnt vmcnt(13)\n\ts_barrier\n\t" MX_R("x00", "bw", "o0") MX_R("x01", "bw", "o1")
+               MX_R("x10", "bw", "o2") MX_R("x11", "bw", "o3") MX_R("y00", "ba", "o0") MX_R("y01", "ba", "o1")
+               MX_R("y10", "ba", "o2") MX_R("y11", "ba", "o3") MX_RS("n0", "sbw", "t0") MX_RS("n1", "sbw", "t1")
+               MX_RS("r0", "sba", "t0") MX_RS("r1", "sba", "t1") "s_waitcnt lgkmcnt(0)"
+               : [x00] "=&v"(f0.w[0][0]), [x01] "=&v"(f0.w[0][1]), [x10] "=&v"(f0.w[1][0]),
+                 [x11] "=&v"(f0.w[1][1]), [y00] "=&v"(f0.a[0][0]), [y01] "=&v"(f0.a[0][1]),
+                 [y10] "=&v"(f0.a[1][0]), [y11] "=&v"(f0.a[1][1]), [n0] "=&v"(sc.w[0]), [n1] "=&v"(sc.w[1]),
+                 [r0] "=&v"(sc.a[0]), [r1] "=&v"(sc.a[1])
+               : [bw] "v"(bw), [ba] "v"(ba), [o0] "n"(0), [o1] "n"(2048), [o2] "n"(1024), [o3] "n"(3072),
+                 [sbw] "v"(sw), [sba] "v"(sa), [t0] "n"(C::CODES), [t1] "n"(C::CODES + 256)
+               : "memory");
+  f32x16 acc[2][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) acc[i][j] = zero16();
+  for (int s = 0; s < n; s += 2) {
+    const uint32_t other = PAIR - 2 * off;  // from this pair of stages to the other one
+    mx_mid_step<0, ST, 0>(acc, f0, f1, sc, nsc, bw, ba, sw, sa, g, dst + off, col(s + 4), sdst + off,
+                          scol(s + 4));
+    const uint32_t o_bw = bw + other, o_ba = ba + other, o_sw = sw + other, o_sa = sa + other;
+    mx_mid_step<1, 0, C::CODES>(acc, f1, f0, sc, nsc, o_bw, o_ba, o_sw, o_sa, g, dst + off + ST, col(s + 5), 0,
+                                nullptr);
+    sc = nsc;
+    bw = o_bw, ba = o_ba, sw = o_sw, sa = o_sa, off = PAIR - off;
+  }
+  // every load has landed and every wave's reads are done: LDS is free; the products' registers are
+  // readable
+  asm volatile("s_nop 15\n\ts_nop 15\n\ts_waitcnt vmcnt(0)\n\ts_barrier"
+               : "+v"(acc[0][0]), "+v"(acc[0][1]), "+v"(acc[1][0]), "+v"(acc[1][1])
+               :
+               : "memory");
+  char* own = lds + wave * 4096;
+  mx_bias_add<T>(acc, bias, (float*)own, (n0 + wn * 2) * 32, w.rows);
+  mx_store<T, 2, 2, GELU>(acc, own, out, ldo, (m0 + wm * 2) * 32, a.rows, (n0 + wn * 2) * 32, w.rows);
+}
+
+// ---- small launches: the columns split over the waves ------------------------
+// 32 NB features x 32 tokens a work-group; its waves take units of 128 columns in
+// turn, so every fragment is loaded once, straight into registers (no staging,
+// no barrier in the loop), DEPTH units ahead.  The waves' sums meet in LDS, in
+// the order of the waves.  With X16 the tokens come in 16 bits and every
+// work-group quantises them into LDS first (MX_X16_BLOCKS blocks at most), under
+// the loads of its first weights, in the place of a launch before this one.
+#define MX_X16_BLOCKS 2048
+struct MxSrc {
+  MxMat m;            // in MXFP4 (its row count in either case), or
+  const uint16_t* x;  // in 16 bits
+  long long stride;
+  int K;
+};
+
+template <typename T, int NB, int WAVES, int DEPTH, bool GELU, bool X16>
+__global__ __launch_bounds__(64 * WAVES) void mx_split_kernel(MxSrc a, MxMat w,
+                                                              const uint16_t* __restrict__ bias,
+                                                              uint16_t* __restrict__ out, long long ldo,
+                                                              int groups, int mt, int nt, int per_xcd) {
+  __shared__ f32x4 part[WAVES][NB][4][64];
+  __shared__ u32x4 xc[X16 ? MX_X16_BLOCKS : 1];
+  __shared__ uint8_t xs[X16 ? MX_X16_BLOCKS : 1];
+  const int id = mx_first(per_xcd);
+  if (id >= mx_end(mt, nt, per_xcd)) return;
+  int mb, n0;
+  mx_place(id, mt, nt, 1, NB, mb, n0);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = 2 * groups;
-  const char *pw[NB], *pa[MB];
-  const uint32_t *qw[NB], *qa[MB];
+  const char* pw[NB];
+  const uint32_t* qw[NB];
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
     const long long row = min(n0 + i, w.blocks - 1);
     pw[i] = w.codes + row * groups * 4096;
     qw[i] = w.scales + row * groups * 64;
   }
-#pragma unroll
-  for (int j = 0; j < MB; ++j) {
-    const long long row = min(m0 + j, a.blocks - 1);
-    pa[j] = a.codes + row * groups * 4096;
-    qa[j] = a.scales + row * groups * 64;
-  }
-  auto load = [&](int s, MxUnit<NB, MB>& t) {
+  const char* pa = X16 ? nullptr : a.m.codes + (long long)mb * groups * 4096;
+  const uint32_t* qa = X16 ? nullptr : a.m.scales + (long long)mb * groups * 64;
+  const int row = mb * 32 + (lane & 31);
+  struct Unit {
+    u32x4 w[2][NB], a[2];
+    uint32_t sw[NB], sa;
+  };
+  auto load = [&](int s, Unit& t) {
     const size_t o = (size_t)s * 2048 + lane * 16, os = (size_t)(s >> 1) * 64 + lane;
     const int sh = 16 * (s & 1);  // an odd unit's scales are the upper half
 #pragma unroll
@@ -714,104 +758,119 @@ __global__ __launch_bounds__(64 * WAVES, NB * MB >= 8 ? 1 : 2) void mx_split_ker
       t.w[1][i] = *(const u32x4*)(pw[i] + o + 1024);
       t.sw[i] = qw[i][os] >> sh;
     }
-#pragma unroll
-    for (int j = 0; j < MB; ++j) {
-      t.a[0][j] = *(const u32x4*)(pa[j] + o);
-      t.a[1][j] = *(const u32x4*)(pa[j] + o + 1024);
-      t.sa[j] = qa[j][os] >> sh;
+    if constexpr (!X16) {
+      t.a[0] = *(const u32x4*)(pa + o);
+      t.a[1] = *(const u32x4*)(pa + o + 1024);
+      t.sa = qa[os] >> sh;
     }
   };
-  f32x16 acc[NB][MB];
-#pragma unroll
-  for (int i = 0; i < NB; ++i)
-#pragma unroll
-    for (int j = 0; j < MB; ++j) acc[i][j] = zero16();
-  auto mul = [&](const MxUnit<NB, MB>& t) {
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-#pragma unroll
-      for (int j = 0; j < MB; ++j) acc[i][j] = mx_mfma<0>(t.w[0][i], t.a[0][j], acc[i][j], t.sw[i], t.sa[j]);
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-#pragma unroll
-      for (int j = 0; j < MB; ++j) acc[i][j] = mx_mfma<1>(t.w[1][i], t.a[1][j], acc[i][j], t.sw[i], t.sa[j]);
+  // X16: block b of row r at r 8 groups + b
+  auto fetch = [&](int s, Unit& t) {
+    const int b = row * 8 * groups + 4 * s + (lane >> 5);
+    t.a[0] = t.a[1] = u32x4{0u, 0u, 0u, 0u};
+    t.sa = 0;
+    if (row < a.m.rows) {
+      t.a[0] = xc[b], t.a[1] = xc[b + 2];
+      t.sa = xs[b] | (xs[b + 2] << 8);
+    }
   };
-  MxUnit<NB, MB> ring[DEPTH];
+  f32x16 acc[NB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i) acc[i] = zero16();
+  auto mul = [&](const Unit& t) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i) acc[i] = mx_mfma<0>(t.w[0][i], t.a[0], acc[i], t.sw[i], t.sa);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) acc[i] = mx_mfma<1>(t.w[1][i], t.a[1], acc[i], t.sw[i], t.sa);
+  };
+  Unit ring[DEPTH];
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d)
     if (wave + d * WAVES < n) load(wave + d * WAVES, ring[d]);
+  if constexpr (X16) {
+    for (int b = threadIdx.x; b < a.m.rows * 8 * groups; b += 64 * WAVES) {
+      const int r = b / (8 * groups), c = 32 * (b - r * 8 * groups);
+      u32x4 v[4], codes{0u, 0u, 0u, 0u};
+      uint32_t byte = 0;
+      if (c < a.K) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = *(const u32x4*)(a.x + r * a.stride + c + 8 * i);
+        mx_block<T>(v, codes, byte);
+      }
+      xc[b] = codes;
+      xs[b] = (uint8_t)byte;
+    }
+    __syncthreads();
+  }
   for (int s = wave; s < n; s += DEPTH * WAVES) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
-      if (s + d * WAVES < n) mul(ring[d]);
+      if (s + d * WAVES < n) {
+        if constexpr (X16) fetch(s + d * WAVES, ring[d]);
+        mul(ring[d]);
+      }
       if (s + (d + DEPTH) * WAVES < n) load(s + (d + DEPTH) * WAVES, ring[d]);
     }
   }
 #pragma unroll
-  for (int p0 = 0; p0 < P; p0 += ROUND) {
-    if (p0) __syncthreads();
+  for (int i = 0; i < NB; ++i)
 #pragma unroll
-    for (int p = p0; p < p0 + ROUND && p < P; ++p)
+    for (int q = 0; q < 4; ++q)
+      part[wave][i][q][lane] = f32x4{acc[i][4 * q], acc[i][4 * q + 1], acc[i][4 * q + 2], acc[i][4 * q + 3]};
+  __syncthreads();
+  // quarter q of a block: four features of each token
+  for (int iq = wave; iq < 4 * NB; iq += WAVES) {
+    const int i = iq >> 2, q = iq & 3;
+    f32x4 v = part[0][i][q][lane];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f32x16& c = acc[p / MB][p % MB];
-        part[wave][p - p0][q][lane] = f32x4{c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]};
+    for (int x = 1; x < WAVES; ++x) {
+      const f32x4 y = part[x][i][q][lane];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += y[e];
+    }
+    const int f = (n0 + i) * 32 + 8 * q + 4 * (lane >> 5);
+    if (row < a.m.rows && f < w.rows) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (bias) v[e] += T::to_f(bias[min(f + e, w.rows - 1)]);
+        if (GELU) v[e] = mx_gelu(v[e]);
       }
-    __syncthreads();
-    // quarter q of block p: four features of each token
-    const int quarters = 4 * (P - p0 < ROUND ? P - p0 : ROUND);
-    for (int pq = wave; pq < quarters; pq += WAVES) {
-      const int p = pq >> 2, q = pq & 3;
-      f32x4 v = part[0][p][q][lane];
-#pragma unroll
-      for (int x = 1; x < WAVES; ++x) {
-        const f32x4 y = part[x][p][q][lane];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += y[e];
-      }
-      const int m = (m0 + (p + p0) % MB) * 32 + (lane & 31);
-      const int f = (n0 + (p + p0) / MB) * 32 + 8 * q + 4 * (lane >> 5);
-      if (m < a.rows && f < w.rows) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (bias) v[e] += T::to_f(bias[min(f + e, w.rows - 1)]);
-          if (GELU) v[e] = mx_gelu(v[e]);
-        }
-        mx_put(out + m * ldo + f, u32x2{Pk<T>::pack(v[0], v[1]), Pk<T>::pack(v[2], v[3])}, w.rows - f);
-      }
+      mx_put(out + row * ldo + f, u32x2{Pk<T>::pack(v[0], v[1]), Pk<T>::pack(v[2], v[3])}, w.rows - f);
     }
   }
 }
 
-template <typename T, int NB, int MB, int WAVES, int DEPTH>
-static int mx_split_launch(const MxMat& a, const MxMat& w, const uint16_t* bias, int act, uint16_t* out,
+template <typename T, int NB, int WAVES, int DEPTH, bool X16>
+static int mx_split_launch(const MxSrc& a, const MxMat& w, const uint16_t* bias, int act, uint16_t* out,
                            long long ldo, int groups, hipStream_t st) {
-  const int mt = cdiv(a.blocks, MB), nt = cdiv(w.blocks, NB);
-  const long long tiles = (long long)mt * nt;
-  T2T_REQUIRE(tiles <= INT_MAX / 2, "mxfp4_product: M=%d N=%d", a.rows, w.rows);
+  const int nt = cdiv(w.blocks, NB);
+  const long long tiles = (long long)a.m.blocks * nt;
+  T2T_REQUIRE(tiles <= INT_MAX / 16, "mxfp4_product: M=%d N=%d", a.m.rows, w.rows);
   const int per = cdiv(tiles, 8);
-  auto kernel = act == T2T_ACT_GELU_TANH ? mx_split_kernel<T, NB, MB, WAVES, DEPTH, true>
-                                         : mx_split_kernel<T, NB, MB, WAVES, DEPTH, false>;
-  hipLaunchKernelGGL(kernel, dim3(8 * per), dim3(64 * WAVES), 0, st, a, w, bias, out, ldo, groups, mt, nt,
-                     per);
+  auto kernel = act == T2T_ACT_GELU_TANH ? mx_split_kernel<T, NB, WAVES, DEPTH, true, X16>
+                                         : mx_split_kernel<T, NB, WAVES, DEPTH, false, X16>;
+  hipLaunchKernelGGL(kernel, dim3(8 * per), dim3(64 * WAVES), 0, st, a, w, bias, out, ldo, groups, a.m.blocks,
+                     nt, per);
   T2T_LAUNCH_CHECK("mxfp4_product");
   return T2T_OK;
 }
 
+// tiles of 64 TW x 64 TA
 template <typename T, int TW, int TA>
 static int mx_tile_launch(const MxMat& a, const MxMat& w, const uint16_t* bias, int act, uint16_t* out,
                           long long ldo, int groups, hipStream_t st) {
   const int mt = cdiv(a.blocks, 2 * TA), nt = cdiv(w.blocks, 2 * TW);
   const long long tiles = (long long)mt * nt;
-  T2T_REQUIRE(tiles <= INT_MAX / 2, "mxfp4_product: M=%d N=%d", a.rows, w.rows);
+  T2T_REQUIRE(tiles <= INT_MAX / 16, "mxfp4_product: M=%d N=%d", a.rows, w.rows);
   const int per = cdiv(tiles, 8);
   auto launch = [&](auto kernel, int slots) {
     hipLaunchKernelGGL(kernel, dim3(8 * slots), dim3(256), 0, st, a, w, bias, out, ldo, groups, mt, nt, per);
   };
-  if constexpr (TW * TA == 16)  // fills a CU: 32 work-groups an XCD, which go through the tiles
-    launch(act == T2T_ACT_GELU_TANH ? mx_big_kernel<T, true> : mx_big_kernel<T, false>, per < 32 ? per : 32);
+  const bool gelu = act == T2T_ACT_GELU_TANH;
+  if constexpr (TW == 4)  // fills a CU: 32 work-groups an XCD, which go through the tiles
+    launch(gelu ? mx_big_kernel<T, true> : mx_big_kernel<T, false>, per < 32 ? per : 32);
   else
-    launch(act == T2T_ACT_GELU_TANH ? mx_tile_kernel<T, TW, TA, true> : mx_tile_kernel<T, TW, TA, false>, per);
+    launch(gelu ? mx_mid_kernel<T, true> : mx_mid_kernel<T, false>, per);
   T2T_LAUNCH_CHECK("mxfp4_product");
   return T2T_OK;
 }
@@ -819,11 +878,12 @@ static int mx_tile_launch(const MxMat& a, const MxMat& w, const uint16_t* bias, 
 template <typename T>
 static int mx_product(const MxMat& a, const MxMat& w, const uint16_t* bias, int act, uint16_t* out,
                       long long ldo, int groups, hipStream_t st) {
-  if ((long long)a.blocks * w.blocks >= 64 * 256)
+  const long long big = (long long)cdiv(a.blocks, 8) * cdiv(w.blocks, 8);
+  const long long mid = (long long)cdiv(a.blocks, 4) * cdiv(w.blocks, 4);
+  if (big >= 256 && groups >= 4 && 4 * big <= mid + mid / 4)
     return mx_tile_launch<T, 4, 4>(a, w, bias, act, out, ldo, groups, st);
-  if ((long long)a.blocks * w.blocks >= 16 * 256)
-    return mx_tile_launch<T, 2, 2>(a, w, bias, act, out, ldo, groups, st);
-  return mx_tile_launch<T, 1, 1>(a, w, bias, act, out, ldo, groups, st);
+  if (a.blocks > 2) return mx_tile_launch<T, 2, 2>(a, w, bias, act, out, ldo, groups, st);
+  return mx_split_launch<T, 1, 8, 4, false>(MxSrc{a, nullptr, 0, 0}, w, bias, act, out, ldo, groups, st);
 }
 
 static int mx_check_product(const char* what, const void* a_codes, const void* a_scales,
@@ -858,10 +918,13 @@ extern "C" int t2t_mxfp4_product(const void* a_codes, const void* a_scales, cons
                           (hipStream_t)stream);
 }
 
+// few rows are quantised by the product itself
+static bool mx_few(int M, int K) { return M <= 32 && (long long)M * (mx_kp(K) / 32) <= MX_X16_BLOCKS; }
+
 // codes, then scales
 extern "C" size_t t2t_mxfp4_linear_ws_bytes(int M, int N, int K) {
   (void)N;
-  return t2t_align256(t2t_mxfp4_code_bytes(M, K)) + t2t_mxfp4_scale_bytes(M, K);
+  return mx_few(M, K) ? 0 : t2t_align256(t2t_mxfp4_code_bytes(M, K)) + t2t_mxfp4_scale_bytes(M, K);
 }
 
 extern "C" int t2t_mxfp4_linear(const void* x, int dtype, long long x_row_stride, const void* w_codes,
@@ -872,13 +935,20 @@ extern "C" int t2t_mxfp4_linear(const void* x, int dtype, long long x_row_stride
   int rc = mx_check_product("mxfp4_linear", x, x, w_codes, w_scales, act, out, dtype, out_row_stride, M, N, K);
   if (rc == T2T_OK) rc = mx_check_rows("mxfp4_linear", x, dtype, x_row_stride, w_codes, w_scales, M, K);
   if (rc != T2T_OK || M == 0) return rc;
+  if (mx_few(M, K)) {
+    const MxSrc a{MxMat{nullptr, nullptr, M, (int)mx_row_blocks(M)}, (const uint16_t*)x, x_row_stride, K};
+    const MxMat w{(const char*)w_codes, (const uint32_t*)w_scales, N, (int)mx_row_blocks(N)};
+    auto run = dtype == T2T_BF16 ? mx_split_launch<BF16T, 1, 8, 2, true> : mx_split_launch<F16T, 1, 8, 2, true>;
+    return run(a, w, (const uint16_t*)bias, act, (uint16_t*)out, out_row_stride, mx_kp(K) / 256,
+               (hipStream_t)stream);
+  }
   if (!ws || ws_bytes < t2t_mxfp4_linear_ws_bytes(M, N, K)) {
     t2t_set_error("mxfp4_linear: workspace %zu < %zu bytes", ws ? ws_bytes : (size_t)0,
                   t2t_mxfp4_linear_ws_bytes(M, N, K));
     return T2T_ERR_WORKSPACE;
   }
-  char* scales = (char*)ws + t2t_align256(t2t_mxfp4_code_bytes(M, K));
   T2T_REQUIRE((uintptr_t)ws % 16 == 0, "mxfp4_linear: workspace must be 16-byte aligned");
+  char* scales = (char*)ws + t2t_align256(t2t_mxfp4_code_bytes(M, K));
   rc = t2t_mxfp4_quantize(x, dtype, x_row_stride, ws, scales, M, K, stream);
   if (rc != T2T_OK) return rc;
   return t2t_mxfp4_product(ws, scales, w_codes, w_scales, bias, act, out, dtype, out_row_stride, M, N, K,

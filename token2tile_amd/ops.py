@@ -1042,7 +1042,8 @@ _ACTIVATIONS = {None: 0, "gelu_tanh": 1}
 
 
 def mxfp4_linear_ws_bytes(M, N, K):
-    """Workspace of mxfp4_linear for a 16-bit x of M rows."""
+    """Workspace of mxfp4_linear for a 16-bit x of M rows (0 where the product
+    quantises them itself)."""
     return size_query("t2t_mxfp4_linear_ws_bytes", M, N, K)
 
 
@@ -1090,7 +1091,10 @@ def mxfp4_linear(x, weight, bias=None, *, activation=None, dtype=None, out=None,
                 (x._codes, x._scales, weight._codes, weight._scales, bias, out), *x._ptrs, *args, code,
                 ostride, M, N, K)
     else:
-        ws = _ws_for(ws, mxfp4_linear_ws_bytes(M, N, K), dev, stream)
+        need = mxfp4_linear_ws_bytes(M, N, K)
+        if need or ws is not None:
+            ws = _ws_for(ws, need, dev, stream)
         _launch("t2t_mxfp4_linear", dev, stream, (x, weight._codes, weight._scales, bias, out), x.data_ptr(),
-                code, stride, *args, ostride, M, N, K, ws.data_ptr(), ws.numel())
+                code, stride, *args, ostride, M, N, K, None if ws is None else ws.data_ptr(),
+                0 if ws is None else ws.numel())
     return out
