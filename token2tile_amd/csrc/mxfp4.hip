@@ -33,8 +33,8 @@ extern "C" size_t t2t_mxfp4_scale_bytes(int M, int K) {
 static int mx_check_rows(const char* what, const void* x, int dtype, long long row_stride,
                          const void* codes, const void* scales, int M, int K) {
   T2T_REQUIRE(dtype == T2T_F16 || dtype == T2T_BF16, "%s: dtype %d", what, dtype);
-  T2T_REQUIRE(M >= 0 && K >= 32 && K % 32 == 0 && K <= INT_MAX - 255, "%s: M=%d K=%d (K a multiple of 32)",
-              what, M, K);
+  T2T_REQUIRE(M >= 0 && K >= 32 && K % 32 == 0 && K <= (1 << 27),
+              "%s: M=%d K=%d (K a multiple of 32, at most 2^27)", what, M, K);
   if (M == 0) return T2T_OK;
   T2T_REQUIRE(x && codes && scales, "%s: null pointer", what);
   T2T_REQUIRE(((uintptr_t)x | (uintptr_t)codes | (uintptr_t)scales) % 16 == 0 && row_stride % 8 == 0 &&
@@ -149,35 +149,41 @@ extern "C" int t2t_mxfp4_quantize(const void* x, int dtype, long long row_stride
 }
 
 // ---------------------------------------------------------------------------
-// the values back: the same thread per block
+// the values back: 32 lanes take a row of the 256 columns, eight values each, so
+// that the stores are whole rows (a thread per block, with its four stores 64
+// bytes apart from its neighbour's, took 260 us at 75,600 x 5,120)
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint32_t* __restrict__ codes,
-                                                            const uint32_t* __restrict__ scales,
+                                                            const uint8_t* __restrict__ scales,
                                                             uint16_t* __restrict__ out,
                                                             long long row_stride, int M, int K,
                                                             int groups) {
   const long long rb = blockIdx.x / groups;
   const int g = (int)(blockIdx.x - rb * groups);
-  const int r = threadIdx.x >> 3, blk = threadIdx.x & 7;
-  const long long row = rb * 32 + r;
-  const int col = 256 * g + 32 * blk;
-  if (row >= M || col >= K) return;
-  const int half = blk & 1, j = blk >> 1;
-  const u32x4 c = *(const u32x4*)((const char*)codes + (rb * groups + g) * 4096 + j * 1024 +
-                                  (r + 32 * half) * 16);
-  const uint32_t byte = (scales[(rb * groups + g) * 64 + r + 32 * half] >> (8 * j)) & 255u;
-  const float scale = __builtin_bit_cast(float, byte << 23);
-  u32x4* dst = (u32x4*)(out + row * row_stride + col);
+  const int part = threadIdx.x & 31, blk = part >> 2, half = blk & 1, j = blk >> 1;
+  const int col = 256 * g + 8 * part;
+  if (col >= K) return;
+  const uint32_t* cp = codes + (rb * groups + g) * 1024 + j * 256 + half * 128 + (part & 3);
+  const uint8_t* sp = scales + (rb * groups + g) * 256 + half * 128 + j;
+  uint32_t c[4], byte[4];
 #pragma unroll
-  for (int v = 0; v < 4; ++v) {
+  for (int i = 0; i < 4; ++i) {
+    const int r = 8 * i + (threadIdx.x >> 5);
+    c[i] = cp[4 * r];
+    byte[i] = sp[4 * r];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const long long row = rb * 32 + 8 * i + (threadIdx.x >> 5);
+    const float scale = __builtin_bit_cast(float, byte[i] << 23);
     u32x4 o;
-    o[0] = MxCvt<T>::template dec<0>(c[v], scale);
-    o[1] = MxCvt<T>::template dec<1>(c[v], scale);
-    o[2] = MxCvt<T>::template dec<2>(c[v], scale);
-    o[3] = MxCvt<T>::template dec<3>(c[v], scale);
-    if (byte == 255) o = u32x4{MxCvt<T>::nan_pair, MxCvt<T>::nan_pair, MxCvt<T>::nan_pair, MxCvt<T>::nan_pair};
-    dst[v] = o;
+    o[0] = MxCvt<T>::template dec<0>(c[i], scale);
+    o[1] = MxCvt<T>::template dec<1>(c[i], scale);
+    o[2] = MxCvt<T>::template dec<2>(c[i], scale);
+    o[3] = MxCvt<T>::template dec<3>(c[i], scale);
+    if (byte[i] == 255) o = u32x4{MxCvt<T>::nan_pair, MxCvt<T>::nan_pair, MxCvt<T>::nan_pair, MxCvt<T>::nan_pair};
+    if (row < M) *(u32x4*)(out + row * row_stride + col) = o;
   }
 }
 
@@ -189,11 +195,11 @@ extern "C" int t2t_mxfp4_dequantize(const void* codes, const void* scales, void*
   const long long wgs = mx_row_blocks(M) * groups;
   if (dtype == T2T_BF16)
     hipLaunchKernelGGL(mx_dequantize_kernel<BF16T>, dim3((unsigned)wgs), dim3(256), 0,
-                       (hipStream_t)stream, (const uint32_t*)codes, (const uint32_t*)scales,
+                       (hipStream_t)stream, (const uint32_t*)codes, (const uint8_t*)scales,
                        (uint16_t*)out, row_stride, M, K, groups);
   else
     hipLaunchKernelGGL(mx_dequantize_kernel<F16T>, dim3((unsigned)wgs), dim3(256), 0,
-                       (hipStream_t)stream, (const uint32_t*)codes, (const uint32_t*)scales,
+                       (hipStream_t)stream, (const uint32_t*)codes, (const uint8_t*)scales,
                        (uint16_t*)out, row_stride, M, K, groups);
   T2T_LAUNCH_CHECK("mxfp4_dequantize");
   return T2T_OK;

@@ -7,12 +7,46 @@
 // with start[a] <= i < start[a + 1].  The angle is one fp64 product (a far
 // position leaves no fraction in fp32) and its sine and cosine are taken in
 // fp64, so the fp32 entries are off by one rounding.  Bound: writing the
-// tables.
+// tables.  A thread keeps one pair and goes through the positions.
 // ---------------------------------------------------------------------------
 struct TableAxes {
   int n;
   int start[5];
 };
+
+// m sin x and m cos x by the Taylor series on [-pi/4, pi/4], to below 1e-15 (r^15, r^14), after taking
+// the nearest multiple of pi/2 off in two parts; |x| < 2^31.  The coefficients are kept in scalar
+// registers (left to itself the compiler moves each into vector registers at every use).
+struct TableCoef {
+  double s[7], c[6];
+  __device__ TableCoef()
+      : s{-1.0 / 1307674368000.0, 1.0 / 6227020800.0, -1.0 / 39916800.0, 1.0 / 362880.0, -1.0 / 5040.0,
+          1.0 / 120.0, -1.0 / 6.0},
+        c{-1.0 / 87178291200.0, 1.0 / 479001600.0, -1.0 / 3628800.0, 1.0 / 40320.0, -1.0 / 720.0, 1.0 / 24.0} {
+#pragma unroll
+    for (int i = 0; i < 7; ++i) asm("" : "+s"(s[i]));
+#pragma unroll
+    for (int i = 0; i < 6; ++i) asm("" : "+s"(c[i]));
+  }
+};
+__device__ inline void table_sincos(const TableCoef& k_, double x, double m, float& s, float& c) {
+  const double k = __builtin_rint(x * 0.6366197723675814);
+  double r = __builtin_fma(-k, 1.5707963267948966, x);
+  r = __builtin_fma(-k, 6.123233995736766e-17, r);
+  const double t = r * r;
+  double u = k_.s[0], v = k_.c[0];
+#pragma unroll
+  for (int i = 1; i < 7; ++i) u = __builtin_fma(u, t, k_.s[i]);
+#pragma unroll
+  for (int i = 1; i < 6; ++i) v = __builtin_fma(v, t, k_.c[i]);
+  u = __builtin_fma(u * t, r, r);
+  v = __builtin_fma(__builtin_fma(v, t, -0.5), t, 1.0);
+  // which is which, and the signs, after the rounding to fp32
+  const uint32_t q = (uint32_t)(int)k;
+  const uint32_t fu = __builtin_bit_cast(uint32_t, (float)(m * u)), fv = __builtin_bit_cast(uint32_t, (float)(m * v));
+  s = __builtin_bit_cast(float, (q & 1 ? fv : fu) ^ ((q & 2) << 30));
+  c = __builtin_bit_cast(float, (q & 1 ? fu : fv) ^ (((q + 1) & 2) << 30));
+}
 
 template <typename P>
 __global__ __launch_bounds__(256) void rotary_table_kernel(const P* __restrict__ pos,
@@ -20,17 +54,28 @@ __global__ __launch_bounds__(256) void rotary_table_kernel(const P* __restrict__
                                                            TableAxes ax, double m,
                                                            float* __restrict__ cosv,
                                                            float* __restrict__ sinv, int pairs,
-                                                           long long total) {
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total;
-       i += (long long)gridDim.x * 256) {
-    const long long t = i / pairs;
-    const int p = (int)(i - t * pairs);
+                                                           long long T) {
+  const int rows = pairs < 256 ? 256 / pairs : 1;  // positions a work-group takes at once
+  const int r = pairs < 256 ? threadIdx.x / pairs : 0;
+  if (r >= rows) return;
+  const TableCoef coef;
+  for (int p = pairs < 256 ? threadIdx.x - r * pairs : threadIdx.x; p < pairs; p += pairs < 256 ? pairs : 256) {
     int a = 0;
     for (int k = 1; k < ax.n; ++k) a += p >= ax.start[k];
-    double s, c;
-    sincos((double)pos[t * ax.n + a] * freqs[p], &s, &c);
-    cosv[i] = (float)(m * c);
-    sinv[i] = (float)(m * s);
+    const double f = freqs[p];
+    const long long step = (long long)gridDim.x * rows;
+    for (long long t0 = (long long)blockIdx.x * rows + r; t0 < T; t0 += 4 * step) {
+      P at[4];  // four positions' loads under way at once
+#pragma unroll
+      for (int i = 0; i < 4; ++i) at[i] = pos[min(t0 + i * step, T - 1) * ax.n + a];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const long long t = t0 + i * step;
+        float s, c;
+        table_sincos(coef, (double)at[i] * f, m, s, c);
+        if (t < T) cosv[t * pairs + p] = c, sinv[t * pairs + p] = s;
+      }
+    }
   }
 }
 
@@ -50,15 +95,16 @@ extern "C" int t2t_rotary_table(const void* positions, int pos_bits, long long T
   T2T_REQUIRE(T <= LLONG_MAX / 4 / pairs, "rotary_table: T=%lld", T);
   if (T == 0) return T2T_OK;
   T2T_REQUIRE(positions && freqs && cosv && sinv, "rotary_table: null pointer");
-  const long long total = T * pairs;
-  const long long g = (total + 255) / 256;
-  const dim3 grid((unsigned)(g < 16384 ? g : 16384));
+  const long long rows = pairs < 256 ? 256 / pairs : 1, g = (T + rows - 1) / rows;
+  // four positions a thread, where that leaves enough work-groups
+  const long long wgs = g < 2048 ? g : (g + 3) / 4;
+  const dim3 grid((unsigned)(wgs < (1 << 20) ? wgs : 1 << 20));
   if (pos_bits == 32)
     hipLaunchKernelGGL(rotary_table_kernel<int32_t>, grid, dim3(256), 0, (hipStream_t)stream,
-                       (const int32_t*)positions, freqs, ax, factor, cosv, sinv, pairs, total);
+                       (const int32_t*)positions, freqs, ax, factor, cosv, sinv, pairs, T);
   else
     hipLaunchKernelGGL(rotary_table_kernel<long long>, grid, dim3(256), 0, (hipStream_t)stream,
-                       (const long long*)positions, freqs, ax, factor, cosv, sinv, pairs, total);
+                       (const long long*)positions, freqs, ax, factor, cosv, sinv, pairs, T);
   T2T_LAUNCH_CHECK("rotary_table");
   return T2T_OK;
 }

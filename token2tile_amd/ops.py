@@ -751,6 +751,12 @@ def _empty(stream, shape, dtype, dev):
     return _new(stream, *shape, dtype=dtype, device=dev)
 
 
+def _is(t, shape, dtype, dev):
+    """_check without its message."""
+    return (isinstance(t, torch.Tensor) and t.shape == shape and t.dtype == dtype and t.device == dev
+            and t.is_contiguous())
+
+
 def _scattered(t):
     """Whether a view's elements all have an address of their own."""
     if t.is_contiguous():
@@ -847,9 +853,12 @@ def rotary_table(positions, frequencies, out=None, stream=None):
         if not lead or lead[-1] != len(pairs):
             raise ValueError(f"t2t: positions must end in {len(pairs)} axes, got {lead}")
         lead = lead[:-1]
-    _check(positions, positions.shape, (_i32, torch.int64), "positions", dev)
+    bits = {_i32: 32, torch.int64: 64}.get(positions.dtype)
+    if bits is None or not positions.is_contiguous():
+        _check(positions, positions.shape, (_i32, torch.int64), "positions", dev)
     shape = (*lead, sum(pairs))
-    _check(freqs, shape[-1:], torch.float64, "frequencies", dev)
+    if not _is(freqs, shape[-1:], torch.float64, dev):
+        _check(freqs, shape[-1:], torch.float64, "frequencies", dev)
     if out is None:
         cos, sin = _empty(stream, shape, _f32, dev), _empty(stream, shape, _f32, dev)
     else:
@@ -857,8 +866,7 @@ def rotary_table(positions, frequencies, out=None, stream=None):
         _check(cos, shape, _f32, "cos", dev)
         _check(sin, shape, _f32, "sin", dev)
     _launch("t2t_rotary_table", dev, stream, (positions, freqs, cos, sin), positions.data_ptr(),
-            32 if positions.dtype == _i32 else 64, math.prod(lead), len(pairs),
-            (ctypes.c_int * len(pairs))(*pairs), freqs.data_ptr(), factor, cos.data_ptr(), sin.data_ptr())
+            bits, math.prod(lead), len(pairs), (ctypes.c_int * len(pairs))(*pairs), freqs.data_ptr(), factor, cos.data_ptr(), sin.data_ptr())
     return cos, sin
 
 
@@ -866,27 +874,35 @@ _ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
 _ROPE_NORMS = {None: 0, "token": 1, "head": 2}
 
 
-def _rotary_arg(x, out, weight, norm, name, dev, B, N, D, dtype):
-    """The argument struct of one tensor, checked."""
-    nd = x.dim() if isinstance(x, torch.Tensor) else 0
-    if (nd not in (3, 4) or x.dtype != dtype or x.device != dev or (x.shape[0] if nd == 4 else 1) != B
-            or x.shape[-3] != N or x.shape[-1] != D or not 1 <= x.shape[-2] <= 65536
-            or (D > 1 and x.stride(-1) != 1)):
+def _rotary_arg(x, out, weight, norm, name, dev, stream, B, N, D, dtype):
+    """The argument struct of one tensor, checked (out None: made by the caller)."""
+    if not isinstance(x, torch.Tensor):
+        raise ValueError(f"t2t: {name} must be a tensor")
+    shape, xs = x.shape, x.stride()
+    nd = len(shape)
+    if (nd not in (3, 4) or x.dtype != dtype or x.device != dev or (shape[0] if nd == 4 else 1) != B
+            or shape[-3] != N or shape[-1] != D or not 1 <= shape[-2] <= 65536 or (D > 1 and xs[-1] != 1)):
         raise ValueError(f"t2t: {name} must be a {dtype} [{B}, {N}, heads, {D}] tensor on {dev} with "
                          f"contiguous channels")
-    if (not isinstance(out, torch.Tensor) or out.shape != x.shape or out.dtype != dtype
-            or out.device != dev or (D > 1 and out.stride(-1) != 1) or not _scattered(out)):
-        raise ValueError(f"t2t: the output of {name} must be a {dtype} {tuple(x.shape)} tensor on {dev} "
-                         f"with contiguous channels and no element twice")
+    fresh = out is None
+    if fresh:
+        out = _empty(stream, shape, dtype, dev)
+    os = out.stride() if isinstance(out, torch.Tensor) else ()
+    if not fresh and out is not x and (len(os) != nd or out.shape != shape or out.dtype != dtype
+                                       or out.device != dev):
+        raise ValueError(f"t2t: the output of {name} must be a {dtype} {tuple(shape)} tensor on {dev}")
+    if not fresh and ((D > 1 and os[-1] != 1) or not _scattered(out)):
+        raise ValueError(f"t2t: the output of {name} must have contiguous channels and no element twice")
     H = x.shape[-2]
     if norm is not None:
-        _check(weight, (H * D,) if norm == "token" else (D,), dtype, f"{name}_weight", dev)
+        wshape = (H * D,) if norm == "token" else (D,)
+        if not _is(weight, wshape, dtype, dev):
+            _check(weight, wshape, dtype, f"{name}_weight", dev)
     elif weight is not None:
         raise ValueError(f"t2t: {name}_weight without a norm")
-    xs, os = x.stride(), out.stride()
-    return _lib.RotaryTensor(x.data_ptr(), xs[0] if nd == 4 else 0, xs[-3], xs[-2], out.data_ptr(),
-                             os[0] if nd == 4 else 0, os[-3], os[-2],
-                             None if weight is None else weight.data_ptr(), H)
+    return out, _lib.RotaryTensor(x.data_ptr(), xs[0] if nd == 4 else 0, xs[-3], xs[-2], out.data_ptr(),
+                                  os[0] if nd == 4 else 0, os[-3], os[-2],
+                                  None if weight is None else weight.data_ptr(), H)
 
 
 def rotary(q, k, cos, sin, *, layout="interleaved", inverse=False, norm=None, q_weight=None,
@@ -918,19 +934,16 @@ def rotary(q, k, cos, sin, *, layout="interleaved", inverse=False, norm=None, q_
         raise ValueError(f"t2t: {R} of {D} channels rotated (2 <= R <= D <= 256)")
     batched = cos.dim() == 3
     shape = (B, N, R // 2) if batched else (N, R // 2)
-    _check(cos, shape, _f32, "cos", dev)
-    _check(sin, shape, _f32, "sin", dev)
+    for t, name in ((cos, "cos"), (sin, "sin")):
+        if not _is(t, shape, _f32, dev):
+            _check(t, shape, _f32, name, dev)
     if B * N >= 2 ** 31:
         raise ValueError(f"t2t: {B} x {N} tokens")
     oq, ok = out if out is not None else (None, None)
-    if oq is None:
-        oq = _empty(stream, q.shape, q.dtype, dev)
-    tq = _rotary_arg(q, oq, q_weight, norm, "q", dev, B, N, D, q.dtype)
+    oq, tq = _rotary_arg(q, oq, q_weight, norm, "q", dev, stream, B, N, D, q.dtype)
     tk = None
     if k is not None:
-        if ok is None and isinstance(k, torch.Tensor):
-            ok = _empty(stream, k.shape, k.dtype, dev)
-        tk = _rotary_arg(k, ok, k_weight, norm, "k", dev, B, N, D, q.dtype)
+        ok, tk = _rotary_arg(k, ok, k_weight, norm, "k", dev, stream, B, N, D, q.dtype)
     _launch("t2t_rotary", dev, stream, (q, k, cos, sin, q_weight, k_weight, oq, ok), tq, tk,
             dtype_code(q.dtype), cos.data_ptr(), sin.data_ptr(), batched, B, N, D, R,
             _ROPE_LAYOUTS[layout], bool(inverse), _ROPE_NORMS[norm], eps)
@@ -960,8 +973,12 @@ class MxFp4:
             _check(t, (n,), torch.uint8, name, dev)
             if n and t.data_ptr() % 16:
                 raise ValueError(f"t2t: {name} must be 16-byte aligned")
+        self._set(codes, scales, rows, cols, dev)
+
+    def _set(self, codes, scales, rows, cols, dev):
         self._codes, self._scales, self._rows, self._cols = codes, scales, rows, cols
         self._device, self._ptrs = dev, (codes.data_ptr(), scales.data_ptr())
+        return self
 
     codes = property(lambda self: self._codes)
     scales = property(lambda self: self._scales)
@@ -1007,10 +1024,11 @@ def mxfp4_quantize(x, out=None, stream=None):
     _on(stream, dev)
     M, K, stride = _mx_rows(x, "x", dev, 16)
     if out is None:
-        if K < 32 or K % 32:
+        if K < 32 or K % 32 or K > 2 ** 27:
             raise ValueError(f"t2t: x must have columns in multiples of 32, got {K}")
         nc, ns = _mx_bytes(M, K)
-        out = MxFp4(_empty(stream, (nc,), torch.uint8, dev), _empty(stream, (ns,), torch.uint8, dev), M, K)
+        out = MxFp4.__new__(MxFp4)._set(_empty(stream, (nc,), torch.uint8, dev),
+                                        _empty(stream, (ns,), torch.uint8, dev), M, K, dev)
     elif not isinstance(out, MxFp4) or out.shape != (M, K) or out.device != dev:
         raise ValueError(f"t2t: out must be an MxFp4 matrix {M} x {K} on {dev}, got {out!r}")
     _launch("t2t_mxfp4_quantize", dev, stream, (x, out._codes, out._scales), x.data_ptr(),
@@ -1075,7 +1093,7 @@ def mxfp4_linear(x, weight, bias=None, *, activation=None, dtype=None, out=None,
         raise ValueError(f"t2t: x has {K} columns, weight {N} x {weight._cols}")
     if activation not in _ACTIVATIONS:
         raise ValueError(f"t2t: activation {activation!r} (None or gelu_tanh)")
-    if bias is not None:
+    if bias is not None and not _is(bias, (N,), dt, dev):
         _check(bias, (N,), dt, "bias", dev)
     if out is None:
         out = _empty(stream, shape, dt, dev)
