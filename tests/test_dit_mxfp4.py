@@ -1,0 +1,118 @@
+"""The DiT harness with MXFP4 linear layers and the fused norm and rotary
+embedding: the blocks call the operators as documented, the defaults are what
+they were, and the whole stack runs both ways."""
+import math
+
+import pytest
+import torch
+
+from token2tile_amd import dit, ops
+
+CFG = dict(blocks=2, hidden=768, heads=6, ffn=1056, context_tokens=40, grid=(3, 8, 10))
+
+
+def _model(dev, seed=0, **kw):
+    torch.manual_seed(seed)
+    return dit.WanDiT(dit.DiTConfig(**CFG, **kw), sparse=False, device=dev)
+
+
+def _inputs(dev, cfg):
+    g = torch.Generator(device=dev).manual_seed(5)
+    r = lambda *s: torch.randn(*s, generator=g, device=dev, dtype=torch.bfloat16)  # noqa: E731
+    return r(1, cfg.tokens, cfg.hidden), 0.1 * r(1, cfg.hidden), r(1, cfg.context_tokens, cfg.hidden)
+
+
+def test_defaults_are_the_plain_forms():
+    cfg = dit.DiTConfig()
+    assert not cfg.mxfp4 and not cfg.fused_rope
+    torch.manual_seed(0)
+    blk = dit.Block(dit.DiTConfig(blocks=1, hidden=256, heads=2, ffn=64, context_tokens=4, grid=(2, 3, 4)), 0)
+    rope = dit.rope_tables(blk.cfg, "cpu")
+    x = torch.randn(1, 24, 256)
+    q, k, v = blk.qkv(x, rope)
+    want = dit.apply_rope(dit.rms_norm(blk.q(x), blk.norm_q, 1e-6).view(1, 24, 2, 128), *rope)
+    assert torch.equal(q, want) and torch.equal(v, blk.v(x).view(1, 24, 2, 128)) and k.shape == q.shape
+
+
+@pytest.mark.gpu
+def test_fused_tables_equal_the_harness_tables(dev):
+    cfg = dit.DiTConfig(**CFG)
+    for a, b in zip(dit.rope_tables(cfg, dev), dit.rope_tables(dit.DiTConfig(**CFG, fused_rope=True), dev)):
+        # two 64-bit angles, each rounded once to fp32 (half a step each)
+        assert bool(((a - b).abs() <= a.abs() * 2.0 ** -23 + 1e-12).all())
+
+
+@pytest.mark.gpu
+def test_fused_rope_block(dev):
+    """q and k of a block against the 64-bit norm and rotation of its own
+    projections, one rounding."""
+    model = _model(dev, fused_rope=True)
+    blk = model.blocks[0]
+    x, _, _ = _inputs(dev, model.cfg)
+    with torch.no_grad():
+        q, k, v = blk.qkv(x, model.rope)
+        cos, sin = (t.double()[None, :, None] for t in model.rope)
+        for y, lin, w in ((q, blk.q, blk.norm_q), (k, blk.k, blk.norm_k)):
+            f = lin(x).double()
+            f = (f / (f.square().mean(-1, keepdim=True) + 1e-6).sqrt() * w.double()).view(y.shape)
+            a, b = f[..., 0::2], f[..., 1::2]
+            ref = torch.stack((a * cos - b * sin, a * sin + b * cos), -1).flatten(-2)
+            # a bf16 rounding of the result, fp32 inside (2^-17 of the pair)
+            mag = torch.stack((a.abs() + b.abs(),) * 2, -1).flatten(-2)
+            assert bool(((y.double() - ref).abs() <= ref.abs() * 2.0 ** -8 + 2.0 ** -17 * mag).all())
+        assert torch.equal(v, blk.v(x).view(v.shape))
+
+
+@pytest.mark.gpu
+def test_mxfp4_block_calls(dev):
+    """The quantised block's layers are the operators on the model's weights."""
+    plain, model = _model(dev), _model(dev, mxfp4=True)
+    x, _, ctx = _inputs(dev, model.cfg)
+    with torch.no_grad():
+        for name in ("q", "k", "v", "o", "cq", "ck", "cv", "co", "ffn1", "ffn2"):
+            lin, mx = getattr(plain.blocks[1], name), getattr(model.blocks[1], name)
+            assert isinstance(mx, dit.MxFp4Linear) and mx.weight.shape == tuple(lin.weight.shape)
+            assert torch.equal(ops.mxfp4_dequantize(mx.weight),
+                               ops.mxfp4_dequantize(ops.mxfp4_quantize(lin.weight.detach())))
+        blk = model.blocks[1]
+        q, k, v = blk.qkv(x, model.rope)
+        assert torch.equal(v, blk.v(x).view(v.shape))           # shared or own quantisation: the same
+        f = dit.rms_norm(blk.q(x), blk.norm_q, model.cfg.eps).view(q.shape)
+        assert torch.equal(q, dit.apply_rope(f, *model.rope))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(fused_rope=True), dict(mxfp4=True), dict(mxfp4=True, fused_rope=True)])
+def test_stack_runs(dev, kw):
+    plain, model = _model(dev), _model(dev, **kw)
+    args = _inputs(dev, model.cfg)
+    y, z = plain(*args), model(*args)
+    assert z.shape == y.shape and z.dtype == y.dtype and bool(torch.isfinite(z).all())
+    assert torch.equal(model(*args), z)
+    c = torch.nn.functional.cosine_similarity(y.float().flatten(), z.float().flatten(), dim=0)
+    assert c > (0.9 if kw.get("mxfp4") else 0.99)
+
+
+@pytest.mark.gpu
+def test_sparse_attention_takes_the_fused_rows(dev):
+    """The chain into the sparse attention call: MXFP4 projections, fused norm
+    and rotation, the T2T backend's rebuilding and reuse steps."""
+    cfg = dit.DiTConfig(blocks=1, hidden=12 * 128, heads=12, ffn=2048, context_tokens=64, grid=(4, 32, 32),
+                        mxfp4=True, fused_rope=True)
+    budget = dict(ns_base=4096, dense_prefix_steps=1, cq=32, ck=2048, step_profile=(1.0,) * 4,
+                  layer_profile=(1.0,) * 6, cfg_mult=(1.0, 1.0))
+    from token2tile_amd.backend.t2t_attn import T2TAttentionMetadataBuilder, T2TRequestCache
+    torch.manual_seed(0)
+    model = dit.WanDiT(cfg, sparse=True, device=dev)
+    x, t, ctx = _inputs(dev, cfg)
+    b, cache = T2TAttentionMetadataBuilder(), T2TRequestCache()
+    outs = []
+    for step in range(3):
+        md = b.build(step_index=step, total_steps=50, cache=cache, profile_name="manual", **budget)
+        outs.append(model(x, t, ctx, lambda i, m=md: m).float())
+    # a budget of every key: the sparse steps are dense attention up to bf16 roundings of its output
+    # (2^-8 of it twice), which the block's MXFP4 layers then carry on
+    for y in outs[1:]:
+        assert bool(torch.isfinite(y).all())
+        assert torch.nn.functional.cosine_similarity(y.flatten(), outs[0].flatten(), dim=0) > 0.99
+    assert math.isfinite(float(outs[0].abs().max()))

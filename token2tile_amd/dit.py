@@ -8,6 +8,9 @@ Its self-attention runs either dense (torch SDPA) or through
 profile, dense prefix and mask-refresh reuse, so one denoising step can be
 timed both ways on the same weights and inputs.
 
+With ``mxfp4`` the blocks' linear layers run on MXFP4 operands, and with
+``fused_rope`` the RMSNorm and rotary embedding of q and k in one launch.
+
 ``python -m token2tile_amd.dit`` prints one JSON line with the per-step times
 at the Wan2.1-14B 720p shape (40 blocks, hidden 5120, 40 heads, FFN 13824,
 75,600 latent tokens, 512 context tokens).
@@ -36,6 +39,8 @@ class DiTConfig:
     context_tokens: int = 512
     grid: tuple[int, int, int] = (21, 45, 80)  # latent frames x height x width (720p)
     eps: float = 1e-6
+    mxfp4: bool = False       # the blocks' linear layers in MXFP4 (ops.mxfp4_linear)
+    fused_rope: bool = False  # q/k RMSNorm and rotary embedding in one launch (ops.rotary)
 
     @property
     def head_dim(self) -> int:
@@ -56,6 +61,9 @@ def rope_tables(cfg: DiTConfig, device) -> tuple[torch.Tensor, torch.Tensor]:
     f, h, w = cfg.grid
     pos = torch.stack(torch.meshgrid(torch.arange(f), torch.arange(h), torch.arange(w),
                                      indexing="ij"), dim=-1).reshape(-1, 3).to(device)
+    if cfg.fused_rope:
+        from token2tile_amd import ops
+        return ops.rotary_table(pos, ops.rotary_frequencies(parts, device=device))
     angles = []
     for axis, ch in enumerate(parts):
         inv = 1.0 / (10000.0 ** (torch.arange(0, ch, 2, device=device, dtype=torch.float64) / ch))
@@ -76,6 +84,31 @@ def apply_rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.T
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
     xf = x.float()
     return (xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps)).to(x.dtype) * weight
+
+
+class MxFp4Linear(torch.nn.Module):
+    """A linear layer whose weight is kept in MXFP4; its input is quantised at
+    the call, or comes as an ``ops.MxFp4`` that several layers share (the
+    output's leading dimensions are then flattened)."""
+
+    def __init__(self, linear: torch.nn.Linear):
+        super().__init__()
+        from token2tile_amd import ops
+        self.weight = ops.mxfp4_quantize(linear.weight.detach())
+        self.bias = linear.bias
+
+    def forward(self, x, activation=None):
+        from token2tile_amd import ops
+        return ops.mxfp4_linear(x, self.weight, self.bias, activation=activation,
+                                dtype=None if self.bias is None else self.bias.dtype)
+
+
+def _shared(x, layer):
+    """x as ``layer`` and its neighbours take it: in MXFP4 once for all of them."""
+    if isinstance(layer, MxFp4Linear):
+        from token2tile_amd import ops
+        return ops.mxfp4_quantize(x)
+    return x
 
 
 class Block(torch.nn.Module):
@@ -102,13 +135,30 @@ class Block(torch.nn.Module):
         self.ffn2 = torch.nn.Linear(Fh, D)
         self.attn_impl = attn_impl  # None: dense SDPA
 
-    def self_attention(self, x, rope, attn_metadata):
+    def quantize_(self):
+        """The block's linear layers in MXFP4, in the place of the 16-bit ones."""
+        for name in ("q", "k", "v", "o", "cq", "ck", "cv", "co", "ffn1", "ffn2"):
+            setattr(self, name, MxFp4Linear(getattr(self, name)))
+
+    def qkv(self, x, rope):
+        """q, k (normed and rotated) and v [B, N, H, d] of the self-attention."""
         B, N, D = x.shape
         H, d = self.cfg.heads, self.cfg.head_dim
-        q = rms_norm(self.q(x), self.norm_q, self.cfg.eps).view(B, N, H, d)
-        k = rms_norm(self.k(x), self.norm_k, self.cfg.eps).view(B, N, H, d)
-        v = self.v(x).view(B, N, H, d)
-        q, k = apply_rope(q, *rope), apply_rope(k, *rope)
+        x = _shared(x, self.q)
+        q, k, v = self.q(x), self.k(x), self.v(x).view(B, N, H, d)
+        if self.cfg.fused_rope:
+            from token2tile_amd import ops
+            q, k = q.view(B, N, H, d), k.view(B, N, H, d)
+            q, k = ops.rotary(q, k, *rope, norm="token", q_weight=self.norm_q, k_weight=self.norm_k,
+                              eps=self.cfg.eps, out=(q, k))
+            return q, k, v
+        q = rms_norm(q, self.norm_q, self.cfg.eps).view(B, N, H, d)
+        k = rms_norm(k, self.norm_k, self.cfg.eps).view(B, N, H, d)
+        return apply_rope(q, *rope), apply_rope(k, *rope), v
+
+    def self_attention(self, x, rope, attn_metadata):
+        B, N, D = x.shape
+        q, k, v = self.qkv(x, rope)
         if self.attn_impl is None:
             o = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2),
                                                v.transpose(1, 2)).transpose(1, 2)
@@ -120,6 +170,7 @@ class Block(torch.nn.Module):
         B, N, D = x.shape
         H, d = self.cfg.heads, self.cfg.head_dim
         q = rms_norm(self.cq(x), self.cnorm_q, self.cfg.eps).view(B, N, H, d).transpose(1, 2)
+        ctx = _shared(ctx, self.ck)
         k = rms_norm(self.ck(ctx), self.cnorm_k, self.cfg.eps).view(B, -1, H, d).transpose(1, 2)
         v = self.cv(ctx).view(B, -1, H, d).transpose(1, 2)
         o = F.scaled_dot_product_attention(q, k, v).transpose(1, 2).reshape(B, N, D)
@@ -132,7 +183,11 @@ class Block(torch.nn.Module):
         x = x + self.self_attention(h, rope, attn_metadata) * e[2]
         x = x + self.cross_attention(self.norm3(x), ctx)
         h = F.layer_norm(x, (D,), eps=self.cfg.eps) * (1 + e[4]) + e[3]
-        x = x + self.ffn2(F.gelu(self.ffn1(h), approximate="tanh")) * e[5]
+        if isinstance(self.ffn1, MxFp4Linear):
+            y = self.ffn1(h, activation="gelu_tanh")
+        else:
+            y = F.gelu(self.ffn1(h), approximate="tanh")
+        x = x + self.ffn2(y) * e[5]
         return x
 
 
@@ -163,6 +218,9 @@ class WanDiT(torch.nn.Module):
                 for blk in self.blocks:
                     blk.k.weight.mul_(math.sqrt(1.0 - tie * tie)).add_(tie * blk.q.weight)
         self.to(dtype)
+        if cfg.mxfp4:
+            for blk in self.blocks:
+                blk.quantize_()
         self.rope = rope_tables(cfg, device)
 
     @torch.no_grad()
@@ -240,11 +298,15 @@ def main(argv=None):
                    help="sparse steps timed per budget window (after the initial step 12)")
     p.add_argument("--structured", action="store_true",
                    help="tied q/k weights and a smooth latent (local attention); default: random")
+    p.add_argument("--mxfp4", action="store_true",
+                   help="the blocks' linear layers in MXFP4; default: bf16")
+    p.add_argument("--fused-rope", action="store_true",
+                   help="q/k norm and rotary embedding in one launch; default: torch")
     args = p.parse_args(argv)
     if not torch.cuda.is_available():
         sys.exit("the DiT harness needs a ROCm GPU")
     dev = torch.device("cuda", 0)
-    cfg = DiTConfig(blocks=args.blocks)
+    cfg = DiTConfig(blocks=args.blocks, mxfp4=args.mxfp4, fused_rope=args.fused_rope)
     dense = run(cfg, [0, 1, 2], dev, sparse=False, structured=args.structured)
     d_ms = (dense[1] + dense[2]) / 2
     torch.cuda.empty_cache()
@@ -271,6 +333,7 @@ def main(argv=None):
                       "dtype": "bf16",
                       "weights": "random, k tied to q (0.9), smooth latent" if args.structured
                       else "random", "attention_profile": "auto"},
+           **({"linear": "mxfp4"} if cfg.mxfp4 else {}), **({"rope": "fused"} if cfg.fused_rope else {}),
            "dense_ms_per_step": round(d_ms, 1),
            "t2t_step_ms": {str(k): round(v, 1) for k, v in sparse.items()},
            "t2t_ms_per_step_by_window": [round(w, 1) for w in win_ms],
