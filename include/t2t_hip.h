@@ -469,7 +469,7 @@ int t2t_rotary(const t2t_rotary_tensor* q, const t2t_rotary_tensor* k, int dtype
                int inverse, int norm, float eps, void* stream);
 
 /* ---- MXFP4 linear layers ------------------------------------------------ */
-/* Matrices [M, K] (K a multiple of 32) of 4-bit E2M1 values (0, .5, 1, 1.5, 2,
+/* Matrices [M, K] (M <= 2^30; K a multiple of 32, <= 2^27) of 4-bit E2M1 values (0, .5, 1, 1.5, 2,
  * 3, 4, 6 and their negatives) in blocks of 32 columns with one scale byte
  * each (E8M0: 2^(byte - 127); 255 stands for NaN).  No counterpart in the
  * reference.  Codes and scales are held in the operand order of the scaled

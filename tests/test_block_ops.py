@@ -158,6 +158,31 @@ def test_cpu_tensors_are_refused():
             f()
 
 
+def test_calls_run_under_their_tensors_device(monkeypatch):
+    """With another GPU current, the launch and its stream are the tensors' GPU's."""
+    now, seen = [0], []
+
+    class Guard:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            self.was, now[0] = now[0], self.device.index
+
+        def __exit__(self, *exc):
+            now[0] = self.was
+
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 100 + i, raising=False)
+    monkeypatch.setitem(ops._functions, "t2t_probe", lambda *a: seen.append((now[0], a)) or 0)
+    ops._launch("t2t_probe", torch.device("cuda", 1), None, (), 5)
+    ops._launch("t2t_probe", torch.device("cuda", 0), None, (), 6)
+    assert seen == [(1, (5, 101)), (0, (6, 100))] and now == [0]
+    with pytest.raises(ValueError, match="stream"):
+        ops._on(type("S", (), {"device": torch.device("cuda", 1)})(), torch.device("cuda", 0))
+
+
 # ---------------------------------------------------------------------------
 # rotary tables
 # ---------------------------------------------------------------------------
@@ -299,6 +324,34 @@ def test_rotary_views(dev, kind, layout, norm):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shift", [0, 1])
+def test_rotary_of_more_tokens_than_work_groups(dev, shift):
+    """The kernels go through the tokens; the last ones are as the first."""
+    g, dt = _gen(dev, shift), torch.float16
+    N = 70001
+    q = _randn(g, N * 2 * 16 + shift).to(dt)[shift:].view(N, 2, 16)
+    cos, sin = _tables(g, (N,), 16)
+    w = (1 + 0.3 * _randn(g, 32)).to(dt)
+    got = ops.rotary(q, None, cos, sin, norm="token", q_weight=w)[0]
+    _check_rotary(got, q, cos, sin, "interleaved", False, "token", w)
+
+
+@pytest.mark.gpu
+def test_rotary_results_do_not_depend_on_the_company(dev):
+    """A token's result is the same bits alone and among many, whatever the form
+    its call takes."""
+    g, dt = _gen(dev, 21), torch.bfloat16
+    for D, H, norm in ((128, 40, "token"), (96, 12, "token"), (128, 12, "head"), (64, 70, "token")):
+        q = _randn(g, 2000, H, D).to(dt)
+        cos, sin = _tables(g, (2000,), D)
+        w = (1 + 0.2 * _randn(g, H * D if norm == "token" else D)).to(dt)
+        f = lambda a, b: ops.rotary(q[a:b], None, cos[a:b], sin[a:b], norm=norm, q_weight=w)[0]  # noqa: E731
+        whole = f(0, 2000)
+        for a, b in ((0, 1), (777, 778), (1500, 1517)):
+            assert torch.equal(whole[a:b], f(a, b))
+
+
+@pytest.mark.gpu
 def test_rotary_of_no_tokens_nan_and_far_values(dev):
     c = torch.ones(0, 32, device=dev)
     q = torch.empty(0, 3, 64, device=dev, dtype=torch.float16)
@@ -345,7 +398,7 @@ def test_inverse_rotation_is_the_transpose(dev):
 @pytest.mark.parametrize("bad", ["cos_shape", "cos_dtype", "sin_shape", "weight_shape", "weight_dtype",
                                  "no_weight", "weight_without_norm", "layout", "norm", "inverse", "k_width",
                                  "k_tokens", "k_type", "channel_stride", "out_shape", "out_twice", "wide",
-                                 "eps", "rotated"])
+                                 "eps", "rotated", "out_same", "out_other"])
 def test_rotary_refused(dev, bad):
     dt = torch.bfloat16
     z = lambda *s, dtype=dt: torch.zeros(*s, device=dev, dtype=dtype)  # noqa: E731
@@ -383,6 +436,12 @@ def test_rotary_refused(dev, bad):
         a[0] = z(6, 4, 128)[..., ::2]
     elif bad == "out_shape":
         kw = dict(out=(z(6, 4, 65), z(6, 2, 64)))
+    elif bad == "out_same":
+        a[1] = z(6, 4, 64)
+        kw = dict(out=(z(6, 4, 64),) * 2)
+    elif bad == "out_other":
+        a[1] = z(6, 4, 64)
+        kw = dict(out=(a[1], z(6, 4, 64)))
     elif bad == "out_twice":
         kw = dict(out=(z(1, 4, 64).expand(6, 4, 64), z(6, 2, 64)))
     else:
@@ -439,6 +498,16 @@ def test_quantize(dev, M, K, dt):
     got = tab[m & 7] * torch.where(m > 7, -1.0, 1.0) * torch.exp2(s - 127).repeat_interleave(32, 1)
     assert _same(got, v)
     assert not bool(t.codes.view(-1, G, 4, 2, 32, 16)[-1, :, :, :, (M - 1) % 32 + 1:].any())
+
+
+@pytest.mark.gpu
+def test_quantize_more_tiles_than_work_groups(dev):
+    g = _gen(dev, 1)
+    x = _randn(g, 65537 * 32 + 5, 32).to(torch.float16)
+    y = ops.mxfp4_dequantize(ops.mxfp4_quantize(x), torch.float16)
+    for part in (slice(0, 4096), slice(-4096, None)):
+        assert _same(y[part].double(), mx_ref(x[part]))
+    assert bool(((y - x).abs() <= x.abs().amax(1, keepdim=True) / 4).all())
 
 
 @pytest.mark.gpu
@@ -519,9 +588,12 @@ def _check_linear(got, x, w, b, act):
     assert not bool(bad.any()), (int(bad.sum()), bad.nonzero()[:4].tolist())
 
 
+# (33, 20481, 256) and on: 128 x 128 tiles; (16385, 1030, 1056) and on: 256 x 256 tiles
 SIZES = [(1, 1, 32), (1, 64, 64), (1, 5120, 512), (2, 33, 96), (5, 96, 256), (31, 100, 288), (32, 32, 1568),
          (33, 257, 512), (64, 640, 2048), (100, 72, 5120), (129, 130, 160), (257, 513, 256), (600, 1000, 320),
-         (1000, 1536, 1536), (2049, 776, 64), (4099, 2041, 1568)]
+         (1000, 1536, 1536), (2049, 776, 64), (4099, 2041, 1568),
+         (33, 20481, 256), (700, 1100, 512), (300, 1700, 800), (16385, 1030, 1056), (4100, 4200, 1024),
+         (70000, 1025, 96)]
 
 
 @pytest.mark.gpu

@@ -33,16 +33,19 @@ extern "C" size_t t2t_mxfp4_scale_bytes(int M, int K) {
 static int mx_check_rows(const char* what, const void* x, int dtype, long long row_stride,
                          const void* codes, const void* scales, int M, int K) {
   T2T_REQUIRE(dtype == T2T_F16 || dtype == T2T_BF16, "%s: dtype %d", what, dtype);
-  T2T_REQUIRE(M >= 0 && K >= 32 && K % 32 == 0 && K <= (1 << 27),
-              "%s: M=%d K=%d (K a multiple of 32, at most 2^27)", what, M, K);
+  T2T_REQUIRE(M >= 0 && M <= (1 << 30) && K >= 32 && K % 32 == 0 && K <= (1 << 27),
+              "%s: M=%d K=%d (M <= 2^30, K a multiple of 32, K <= 2^27)", what, M, K);
   if (M == 0) return T2T_OK;
   T2T_REQUIRE(x && codes && scales, "%s: null pointer", what);
   T2T_REQUIRE(((uintptr_t)x | (uintptr_t)codes | (uintptr_t)scales) % 16 == 0 && row_stride % 8 == 0 &&
                   (M == 1 || row_stride >= K),
               "%s: rows must be 16-byte aligned, row stride %lld >= K", what, row_stride);
-  T2T_REQUIRE(mx_row_blocks(M) * (mx_kp(K) / 256) <= INT_MAX, "%s: M=%d K=%d", what, M, K);
   return T2T_OK;
 }
+
+// work-groups of the two conversions, which go through the tiles of 32 rows x 256 columns (a grid
+// may not hold 2^32 threads)
+static inline dim3 mx_grid(long long wgs) { return dim3((unsigned)(wgs < 65536 ? wgs : 65536)); }
 
 template <typename T> struct MxCvt;
 template <> struct MxCvt<BF16T> {
@@ -107,29 +110,27 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const uint16_t* __rest
                                                           long long row_stride,
                                                           uint32_t* __restrict__ codes,
                                                           uint32_t* __restrict__ scales, int M, int K,
-                                                          int groups) {
-  const long long rb = blockIdx.x / groups;
-  const int g = (int)(blockIdx.x - rb * groups);
-  const int r = threadIdx.x >> 3, blk = threadIdx.x & 7;
-  const long long row = rb * 32 + r;
-  const int col = 256 * g + 32 * blk;
-  u32x4 c{0u, 0u, 0u, 0u};
-  uint32_t byte = 0;
-  if (row < M && col < K) {
-    const u32x4* src = (const u32x4*)(x + row * row_stride + col);
-    u32x4 v[4];
+                                                          int groups, long long wgs) {
+  const int r = threadIdx.x >> 3, blk = threadIdx.x & 7, half = blk & 1, j = blk >> 1;
+  for (long long wg = blockIdx.x; wg < wgs; wg += gridDim.x) {
+    const long long row = wg / groups * 32 + r;
+    const int col = 256 * (int)(wg % groups) + 32 * blk;
+    u32x4 c{0u, 0u, 0u, 0u};
+    uint32_t byte = 0;
+    if (row < M && col < K) {
+      const u32x4* src = (const u32x4*)(x + row * row_stride + col);
+      u32x4 v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = src[i];
-    mx_block<T>(v, c, byte);
+      for (int i = 0; i < 4; ++i) v[i] = src[i];
+      mx_block<T>(v, c, byte);
+    }
+    *(u32x4*)((char*)codes + wg * 4096 + j * 1024 + (r + 32 * half) * 16) = c;
+    // the four bytes of a lane's dword sit in blocks half, half + 2, ...
+    uint32_t word = byte << (8 * j);
+    word |= __shfl_xor(word, 2, 64);
+    word |= __shfl_xor(word, 4, 64);
+    if (j == 0) scales[wg * 64 + r + 32 * half] = word;
   }
-  const int half = blk & 1, j = blk >> 1;
-  char* cp = (char*)codes + (rb * groups + g) * 4096 + j * 1024 + (r + 32 * half) * 16;
-  *(u32x4*)cp = c;
-  // the four bytes of a lane's dword sit in blocks half, half + 2, ...
-  uint32_t word = byte << (8 * j);
-  word |= __shfl_xor(word, 2, 64);
-  word |= __shfl_xor(word, 4, 64);
-  if (j == 0) scales[(rb * groups + g) * 64 + r + 32 * half] = word;
 }
 
 extern "C" int t2t_mxfp4_quantize(const void* x, int dtype, long long row_stride, void* codes,
@@ -139,11 +140,13 @@ extern "C" int t2t_mxfp4_quantize(const void* x, int dtype, long long row_stride
   const int groups = mx_kp(K) / 256;
   const long long wgs = mx_row_blocks(M) * groups;
   if (dtype == T2T_BF16)
-    hipLaunchKernelGGL(mx_quantize_kernel<BF16T>, dim3((unsigned)wgs), dim3(256), 0, (hipStream_t)stream,
-                       (const uint16_t*)x, row_stride, (uint32_t*)codes, (uint32_t*)scales, M, K, groups);
+    hipLaunchKernelGGL(mx_quantize_kernel<BF16T>, mx_grid(wgs), dim3(256), 0, (hipStream_t)stream,
+                       (const uint16_t*)x, row_stride, (uint32_t*)codes, (uint32_t*)scales, M, K, groups,
+                       wgs);
   else
-    hipLaunchKernelGGL(mx_quantize_kernel<F16T>, dim3((unsigned)wgs), dim3(256), 0, (hipStream_t)stream,
-                       (const uint16_t*)x, row_stride, (uint32_t*)codes, (uint32_t*)scales, M, K, groups);
+    hipLaunchKernelGGL(mx_quantize_kernel<F16T>, mx_grid(wgs), dim3(256), 0, (hipStream_t)stream,
+                       (const uint16_t*)x, row_stride, (uint32_t*)codes, (uint32_t*)scales, M, K, groups,
+                       wgs);
   T2T_LAUNCH_CHECK("mxfp4_quantize");
   return T2T_OK;
 }
@@ -158,32 +161,33 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint32_t* __re
                                                             const uint8_t* __restrict__ scales,
                                                             uint16_t* __restrict__ out,
                                                             long long row_stride, int M, int K,
-                                                            int groups) {
-  const long long rb = blockIdx.x / groups;
-  const int g = (int)(blockIdx.x - rb * groups);
+                                                            int groups, long long wgs) {
   const int part = threadIdx.x & 31, blk = part >> 2, half = blk & 1, j = blk >> 1;
-  const int col = 256 * g + 8 * part;
-  if (col >= K) return;
-  const uint32_t* cp = codes + (rb * groups + g) * 1024 + j * 256 + half * 128 + (part & 3);
-  const uint8_t* sp = scales + (rb * groups + g) * 256 + half * 128 + j;
-  uint32_t c[4], byte[4];
+  for (long long wg = blockIdx.x; wg < wgs; wg += gridDim.x) {
+    const int col = 256 * (int)(wg % groups) + 8 * part;
+    if (col >= K) continue;
+    const uint32_t* cp = codes + wg * 1024 + j * 256 + half * 128 + (part & 3);
+    const uint8_t* sp = scales + wg * 256 + half * 128 + j;
+    uint32_t c[4], byte[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = 8 * i + (threadIdx.x >> 5);
-    c[i] = cp[4 * r];
-    byte[i] = sp[4 * r];
-  }
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + (threadIdx.x >> 5);
+      c[i] = cp[4 * r];
+      byte[i] = sp[4 * r];
+    }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const long long row = rb * 32 + 8 * i + (threadIdx.x >> 5);
-    const float scale = __builtin_bit_cast(float, byte[i] << 23);
-    u32x4 o;
-    o[0] = MxCvt<T>::template dec<0>(c[i], scale);
-    o[1] = MxCvt<T>::template dec<1>(c[i], scale);
-    o[2] = MxCvt<T>::template dec<2>(c[i], scale);
-    o[3] = MxCvt<T>::template dec<3>(c[i], scale);
-    if (byte[i] == 255) o = u32x4{MxCvt<T>::nan_pair, MxCvt<T>::nan_pair, MxCvt<T>::nan_pair, MxCvt<T>::nan_pair};
-    if (row < M) *(u32x4*)(out + row * row_stride + col) = o;
+    for (int i = 0; i < 4; ++i) {
+      const long long row = wg / groups * 32 + 8 * i + (threadIdx.x >> 5);
+      const float scale = __builtin_bit_cast(float, byte[i] << 23);
+      u32x4 o;
+      o[0] = MxCvt<T>::template dec<0>(c[i], scale);
+      o[1] = MxCvt<T>::template dec<1>(c[i], scale);
+      o[2] = MxCvt<T>::template dec<2>(c[i], scale);
+      o[3] = MxCvt<T>::template dec<3>(c[i], scale);
+      if (byte[i] == 255)
+        o = u32x4{MxCvt<T>::nan_pair, MxCvt<T>::nan_pair, MxCvt<T>::nan_pair, MxCvt<T>::nan_pair};
+      if (row < M) *(u32x4*)(out + row * row_stride + col) = o;
+    }
   }
 }
 
@@ -194,13 +198,15 @@ extern "C" int t2t_mxfp4_dequantize(const void* codes, const void* scales, void*
   const int groups = mx_kp(K) / 256;
   const long long wgs = mx_row_blocks(M) * groups;
   if (dtype == T2T_BF16)
-    hipLaunchKernelGGL(mx_dequantize_kernel<BF16T>, dim3((unsigned)wgs), dim3(256), 0,
+    hipLaunchKernelGGL(mx_dequantize_kernel<BF16T>, mx_grid(wgs), dim3(256), 0,
                        (hipStream_t)stream, (const uint32_t*)codes, (const uint8_t*)scales,
-                       (uint16_t*)out, row_stride, M, K, groups);
+                       (uint16_t*)out, row_stride, M, K, groups,
+                       wgs);
   else
-    hipLaunchKernelGGL(mx_dequantize_kernel<F16T>, dim3((unsigned)wgs), dim3(256), 0,
+    hipLaunchKernelGGL(mx_dequantize_kernel<F16T>, mx_grid(wgs), dim3(256), 0,
                        (hipStream_t)stream, (const uint32_t*)codes, (const uint8_t*)scales,
-                       (uint16_t*)out, row_stride, M, K, groups);
+                       (uint16_t*)out, row_stride, M, K, groups,
+                       wgs);
   T2T_LAUNCH_CHECK("mxfp4_dequantize");
   return T2T_OK;
 }
@@ -851,7 +857,6 @@ static int mx_split_launch(const MxSrc& a, const MxMat& w, const uint16_t* bias,
                            long long ldo, int groups, hipStream_t st) {
   const int nt = cdiv(w.blocks, NB);
   const long long tiles = (long long)a.m.blocks * nt;
-  T2T_REQUIRE(tiles <= INT_MAX / 16, "mxfp4_product: M=%d N=%d", a.m.rows, w.rows);
   const int per = cdiv(tiles, 8);
   auto kernel = act == T2T_ACT_GELU_TANH ? mx_split_kernel<T, NB, WAVES, DEPTH, true, X16>
                                          : mx_split_kernel<T, NB, WAVES, DEPTH, false, X16>;
@@ -867,7 +872,10 @@ static int mx_tile_launch(const MxMat& a, const MxMat& w, const uint16_t* bias, 
                           long long ldo, int groups, hipStream_t st) {
   const int mt = cdiv(a.blocks, 2 * TA), nt = cdiv(w.blocks, 2 * TW);
   const long long tiles = (long long)mt * nt;
-  T2T_REQUIRE(tiles <= INT_MAX / 16, "mxfp4_product: M=%d N=%d", a.rows, w.rows);
+  if (tiles > (1 << 23)) {  // 2^32 threads
+    t2t_set_error("mxfp4_product: M=%d N=%d", a.rows, w.rows);
+    return T2T_ERR_UNSUPPORTED;
+  }
   const int per = cdiv(tiles, 8);
   auto launch = [&](auto kernel, int slots) {
     hipLaunchKernelGGL(kernel, dim3(8 * slots), dim3(256), 0, st, a, w, bias, out, ldo, groups, mt, nt, per);
@@ -886,10 +894,11 @@ static int mx_product(const MxMat& a, const MxMat& w, const uint16_t* bias, int 
                       long long ldo, int groups, hipStream_t st) {
   const long long big = (long long)cdiv(a.blocks, 8) * cdiv(w.blocks, 8);
   const long long mid = (long long)cdiv(a.blocks, 4) * cdiv(w.blocks, 4);
-  if (big >= 256 && groups >= 4 && 4 * big <= mid + mid / 4)
+  if ((long long)a.blocks * w.blocks <= 512)
+    return mx_split_launch<T, 1, 8, 4, false>(MxSrc{a, nullptr, 0, 0}, w, bias, act, out, ldo, groups, st);
+  if (big >= 256 && (groups >= 4 || big >= 1024) && 4 * big <= mid + mid / 4)
     return mx_tile_launch<T, 4, 4>(a, w, bias, act, out, ldo, groups, st);
-  if (a.blocks > 2) return mx_tile_launch<T, 2, 2>(a, w, bias, act, out, ldo, groups, st);
-  return mx_split_launch<T, 1, 8, 4, false>(MxSrc{a, nullptr, 0, 0}, w, bias, act, out, ldo, groups, st);
+  return mx_tile_launch<T, 2, 2>(a, w, bias, act, out, ldo, groups, st);
 }
 
 static int mx_check_product(const char* what, const void* a_codes, const void* a_scales,
@@ -897,9 +906,8 @@ static int mx_check_product(const char* what, const void* a_codes, const void* a
                             long long out_row_stride, int M, int N, int K) {
   T2T_REQUIRE(dtype == T2T_F16 || dtype == T2T_BF16, "%s: dtype %d", what, dtype);
   T2T_REQUIRE(act == T2T_ACT_NONE || act == T2T_ACT_GELU_TANH, "%s: activation %d", what, act);
-  T2T_REQUIRE(M >= 0 && N >= 1 && K >= 32 && K % 32 == 0 && K <= (1 << 27),
-              "%s: M=%d N=%d K=%d (K a multiple of 32, at most 2^27)", what, M,
-              N, K);
+  T2T_REQUIRE(M >= 0 && M <= (1 << 30) && N >= 1 && N <= (1 << 30) && K >= 32 && K % 32 == 0 && K <= (1 << 27),
+              "%s: M=%d N=%d K=%d (M, N <= 2^30, K a multiple of 32, K <= 2^27)", what, M, N, K);
   if (M == 0) return T2T_OK;
   T2T_REQUIRE(a_codes && a_scales && w_codes && w_scales && out, "%s: null pointer", what);
   T2T_REQUIRE(((uintptr_t)a_codes | (uintptr_t)a_scales | (uintptr_t)w_codes | (uintptr_t)w_scales) % 16 == 0,

@@ -320,49 +320,51 @@ __global__ __launch_bounds__(256) void rotary_any_kernel(t2t_rotary_tensor q, t2
                                                          RotaryArgs A, int norm) {
   const t2t_rotary_tensor& g = blockIdx.y ? k : q;
   __shared__ double part[4];
-  const long long tok = blockIdx.x;
   const int D = A.D, R = A.R;
-  const int b = (int)(tok / A.N), n = (int)(tok - (long long)b * A.N);
-  const uint16_t* x = (const uint16_t*)g.x + b * g.x_batch + n * g.x_row;
-  uint16_t* o = (uint16_t*)g.out + b * g.out_batch + n * g.out_row;
-  const uint16_t* w = (const uint16_t*)g.weight;
-  const float* c = A.cosv + (b * A.table_batch + n) * (R / 2);
-  const float* s = A.sinv + (b * A.table_batch + n) * (R / 2);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  float inv = 1.f;
-  if (norm == T2T_NORM_TOKEN) {
-    double sum = 0.0;
-    for (int h = wave; h < g.heads; h += 4) sum += rope_head_squares<T>(x + h * g.x_head, D, lane);
-    sum = rope_sum(sum, 64);
-    if (lane == 0) part[wave] = sum;
-    __syncthreads();
-    inv = rope_inv(part[0] + part[1] + part[2] + part[3], 1.0 / ((double)g.heads * D), A.eps);
-  }
-  const int units = R / 2 + (D - R);  // pairs, then channels that are not turned
-  for (int h = wave; h < g.heads; h += 4) {
-    const uint16_t* xh = x + h * g.x_head;
-    uint16_t* oh = o + h * g.out_head;
-    const uint16_t* wh = norm == T2T_NORM_TOKEN ? w + (long long)h * D : w;
-    if (norm == T2T_NORM_HEAD) {
-      inv = rope_inv(rope_sum(rope_head_squares<T>(xh, D, lane), 64), 1.0 / D, A.eps);
+  for (long long tok = blockIdx.x; tok < A.tokens; tok += gridDim.x) {
+    const int b = (int)(tok / A.N), n = (int)(tok - (long long)b * A.N);
+    const uint16_t* x = (const uint16_t*)g.x + b * g.x_batch + n * g.x_row;
+    uint16_t* o = (uint16_t*)g.out + b * g.out_batch + n * g.out_row;
+    const uint16_t* w = (const uint16_t*)g.weight;
+    const float* c = A.cosv + (b * A.table_batch + n) * (R / 2);
+    const float* s = A.sinv + (b * A.table_batch + n) * (R / 2);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float inv = 1.f;
+    if (norm == T2T_NORM_TOKEN) {
+      double sum = 0.0;
+      for (int h = wave; h < g.heads; h += 4) sum += rope_head_squares<T>(x + h * g.x_head, D, lane);
+      sum = rope_sum(sum, 64);
+      __syncthreads();  // the last token's sums are read
+      if (lane == 0) part[wave] = sum;
+      __syncthreads();
+      inv = rope_inv(part[0] + part[1] + part[2] + part[3], 1.0 / ((double)g.heads * D), A.eps);
     }
-    for (int u = lane; u < units; u += 64) {
-      if (u < R / 2) {
-        const int i0 = A.half ? u : 2 * u, i1 = A.half ? u + R / 2 : 2 * u + 1;
-        float a = T::to_f(xh[i0]), e = T::to_f(xh[i1]);
-        if (norm) {
-          a *= inv * T::to_f(wh[i0]);
-          e *= inv * T::to_f(wh[i1]);
+    const int units = R / 2 + (D - R);  // pairs, then channels that are not turned
+    for (int h = wave; h < g.heads; h += 4) {
+      const uint16_t* xh = x + h * g.x_head;
+      uint16_t* oh = o + h * g.out_head;
+      const uint16_t* wh = norm == T2T_NORM_TOKEN ? w + (long long)h * D : w;
+      if (norm == T2T_NORM_HEAD) {
+        inv = rope_inv(rope_sum(rope_head_squares<T>(xh, D, lane), 64), 1.0 / D, A.eps);
+      }
+      for (int u = lane; u < units; u += 64) {
+        if (u < R / 2) {
+          const int i0 = A.half ? u : 2 * u, i1 = A.half ? u + R / 2 : 2 * u + 1;
+          float a = T::to_f(xh[i0]), e = T::to_f(xh[i1]);
+          if (norm) {
+            a *= inv * T::to_f(wh[i0]);
+            e *= inv * T::to_f(wh[i1]);
+          }
+          float y0, y1;
+          rope_turn(a, e, c[u], A.sign * s[u], y0, y1);
+          oh[i0] = T::from_f(y0);
+          oh[i1] = T::from_f(y1);
+        } else {
+          const int d = R + (u - R / 2);
+          float a = T::to_f(xh[d]);
+          if (norm) a *= inv * T::to_f(wh[d]);
+          oh[d] = T::from_f(a);
         }
-        float y0, y1;
-        rope_turn(a, e, c[u], A.sign * s[u], y0, y1);
-        oh[i0] = T::from_f(y0);
-        oh[i1] = T::from_f(y1);
-      } else {
-        const int d = R + (u - R / 2);
-        float a = T::to_f(xh[d]);
-        if (norm) a *= inv * T::to_f(wh[d]);
-        oh[d] = T::from_f(a);
       }
     }
   }
@@ -425,7 +427,8 @@ static void rope_run(const t2t_rotary_tensor& q, const t2t_rotary_tensor& k, Rot
            : rope_rounds<T, T2T_NORM_NONE, 1>(q, k, A, tensors, its, st);
     return;
   }
-  hipLaunchKernelGGL(rotary_any_kernel<T>, dim3((unsigned)A.tokens, tensors), dim3(256), 0, st, q, k, A, norm);
+  hipLaunchKernelGGL(rotary_any_kernel<T>, dim3((unsigned)(A.tokens < 65536 ? A.tokens : 65536), tensors),
+                     dim3(256), 0, st, q, k, A, norm);
 }
 
 extern "C" int t2t_rotary(const t2t_rotary_tensor* q, const t2t_rotary_tensor* k, int dtype,

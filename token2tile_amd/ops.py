@@ -886,7 +886,7 @@ def _rotary_arg(x, out, weight, norm, name, dev, stream, B, N, D, dtype):
                          f"contiguous channels")
     fresh = out is None
     if fresh:
-        out = _empty(stream, shape, dtype, dev)
+        out = x.new_empty(shape) if stream is None else _empty(stream, shape, dtype, dev)
     os = out.stride() if isinstance(out, torch.Tensor) else ()
     if not fresh and out is not x and (len(os) != nd or out.shape != shape or out.dtype != dtype
                                        or out.device != dev):
@@ -944,6 +944,8 @@ def rotary(q, k, cos, sin, *, layout="interleaved", inverse=False, norm=None, q_
     tk = None
     if k is not None:
         ok, tk = _rotary_arg(k, ok, k_weight, norm, "k", dev, stream, B, N, D, q.dtype)
+        if out is not None and B * N and (tq.out == tk.out or tq.out == tk.x or tk.out == tq.x):
+            raise ValueError("t2t: the outputs of q and k must be two, and neither the other's input")
     _launch("t2t_rotary", dev, stream, (q, k, cos, sin, q_weight, k_weight, oq, ok), tq, tk,
             dtype_code(q.dtype), cos.data_ptr(), sin.data_ptr(), batched, B, N, D, R,
             _ROPE_LAYOUTS[layout], bool(inverse), _ROPE_NORMS[norm], eps)
@@ -966,7 +968,7 @@ class MxFp4:
 
     def __init__(self, codes, scales, rows, cols):
         rows, cols = int(rows), int(cols)
-        if not (0 <= rows < 2 ** 31 and 32 <= cols <= 2 ** 27 and cols % 32 == 0):
+        if not (0 <= rows <= 2 ** 30 and 32 <= cols <= 2 ** 27 and cols % 32 == 0):
             raise ValueError(f"t2t: an MXFP4 matrix has columns in multiples of 32, got {rows} x {cols}")
         dev = _dev(codes)
         for t, n, name in zip((codes, scales), _mx_bytes(rows, cols), ("codes", "scales")):
@@ -1024,8 +1026,8 @@ def mxfp4_quantize(x, out=None, stream=None):
     _on(stream, dev)
     M, K, stride = _mx_rows(x, "x", dev, 16)
     if out is None:
-        if K < 32 or K % 32 or K > 2 ** 27:
-            raise ValueError(f"t2t: x must have columns in multiples of 32, got {K}")
+        if K < 32 or K % 32 or K > 2 ** 27 or M > 2 ** 30:
+            raise ValueError(f"t2t: x must have columns in multiples of 32, got {M} x {K}")
         nc, ns = _mx_bytes(M, K)
         out = MxFp4.__new__(MxFp4)._set(_empty(stream, (nc,), torch.uint8, dev),
                                         _empty(stream, (ns,), torch.uint8, dev), M, K, dev)
@@ -1096,7 +1098,7 @@ def mxfp4_linear(x, weight, bias=None, *, activation=None, dtype=None, out=None,
     if bias is not None and not _is(bias, (N,), dt, dev):
         _check(bias, (N,), dt, "bias", dev)
     if out is None:
-        out = _empty(stream, shape, dt, dev)
+        out = _empty(stream, shape, dt, dev) if stream is not None or isinstance(x, MxFp4) else x.new_empty(shape)
         ostride = N
     else:
         ostride = _mx_rows(out, "out", dev, 2)[2]
@@ -1110,8 +1112,10 @@ def mxfp4_linear(x, weight, bias=None, *, activation=None, dtype=None, out=None,
                 ostride, M, N, K)
     else:
         need = mxfp4_linear_ws_bytes(M, N, K)
-        if need or ws is not None:
+        if ws is not None:
             ws = _ws_for(ws, need, dev, stream)
+        elif need:
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if stream is None else _ws(need, dev, stream)
         _launch("t2t_mxfp4_linear", dev, stream, (x, weight._codes, weight._scales, bias, out), x.data_ptr(),
                 code, stride, *args, ostride, M, N, K, None if ws is None else ws.data_ptr(),
                 0 if ws is None else ws.numel())
