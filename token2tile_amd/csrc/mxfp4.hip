@@ -267,25 +267,31 @@ __device__ inline void mx_place(int id, int mt, int nt, int mb, int nb, int& m0,
   n0 = (in / gm) * nb;
 }
 
-// Adds the bias, which comes through LDS of the wave's own (128 TW bytes): a lane needs 16 TW of the
-// wave's 32 TW features.
+// The sums start at the bias, which comes through LDS of the wave's own (128 TW bytes): a lane needs
+// 16 TW of the wave's 32 TW features.
 template <typename T, int TW, int TA>
-__device__ inline void mx_bias_add(f32x16 (&acc)[TW][TA], const uint16_t* __restrict__ bias, float* own, int f0,
-                                   int rows) {
-  if (!bias) return;
+__device__ inline void mx_start(f32x16 (&acc)[TW][TA], const uint16_t* __restrict__ bias, float* own, int f0,
+                                int rows) {
   const int lane = threadIdx.x & 63, hh = lane >> 5;
+  if (bias)
 #pragma unroll
-  for (int i = lane; i < 32 * TW; i += 64) own[i] = T::to_f(bias[min(f0 + i, rows - 1)]);
+    for (int i = lane; i < 32 * TW; i += 64) own[i] = T::to_f(bias[min(f0 + i, rows - 1)]);
 #pragma unroll
-  for (int i = 0; i < TW; ++i)
+  for (int i = 0; i < TW; ++i) {
+    f32x16 b0 = zero16();
+    if (bias)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const f32x4 v = *(const f32x4*)(own + 32 * i + 8 * q + 4 * hh);
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 v = *(const f32x4*)(own + 32 * i + 8 * q + 4 * hh);
 #pragma unroll
-      for (int j = 0; j < TA; ++j)
+        for (int e = 0; e < 4; ++e) b0[4 * q + e] = v[e];
+      }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += v[e];
+    for (int j = 0; j < TA; ++j) {
+      acc[i][j] = b0;
+      if constexpr (TW == 4) asm volatile("" : "+a"(acc[i][j]));  // a register set each, now
     }
+  }
 }
 
 // The values of one row, the first n of which are inside, to an o of any alignment (rows of odd
@@ -300,50 +306,57 @@ __device__ inline void mx_put(uint16_t* o, const VT& v, int n) {
       if (e < n) o[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
 }
 
-// A wave's 32 TA tokens from m on, 32 TW features from n on: 32 tokens x 64 features at a time (32
-// where TW is 1) are packed, turned through LDS of the wave's own (16-byte chunk c of token t at c ^
-// (t & 7)) and stored as rows, a step behind, so that the reads have the next step's packing to land.
-// (DS operations of a wave run in order: the next writes follow the last reads.)
-template <typename T, int TW, int TA, bool GELU>
+// A wave's 32 TA tokens from m on, 32 TW features from n on: 32 tokens x 64 features at a time are
+// packed, turned through 4 KB of LDS of the wave's own (16-byte chunk c of token t at c ^ (t & 7)) and
+// stored as rows, a step behind, so that the reads have the next step's packing to land.  (DS
+// operations of a wave run in order: the next writes follow the last reads.)  VEC: widths and strides
+// are multiples of eight and out is 16-byte aligned, so a chunk is inside or outside as a whole, and a
+// store takes one scalar address, one offset a lane for all of them and one comparison.
+template <typename T, int TW, int TA, bool GELU, bool VEC>
 __device__ inline void mx_store(const f32x16 (&acc)[TW][TA], char* so, uint16_t* __restrict__ out,
                                 long long ldo, int m, int M, int n, int N) {
-  constexpr int IW = TW == 1 ? 1 : 2, LR = 4 * IW, RT = 64 / LR, RS = 32 / RT;  // lanes a row, rows a store
   int lane = threadIdx.x & 63;
   asm volatile("" : "+v"(lane));  // (or its addresses are kept in registers through the products)
-  const int hh = lane >> 5, c = lane % LR, t0 = lane / LR;
-  u32x4 v[RS];
-  uint16_t* row = out + (long long)(m + t0) * ldo + n + 8 * c;
+  const int hh = lane >> 5, c = lane & 7, t0 = lane >> 3;
+  const long long lane_at = t0 * ldo + 8 * c;
+  u32x4 v[4];
   auto put = [&](int j, int i) {
-    const int left = N - (n + 32 * i + 8 * c);
-    uint16_t* o = row + (long long)(32 * j) * ldo + 32 * i;
+    const int left = N - (n + 32 * i + 8 * c), rows = left > 0 ? M - (m + 32 * j) : 0;
 #pragma unroll
-    for (int r = 0; r < RS; ++r, o += RT * ldo)
-      if (m + 32 * j + RT * r + t0 < M) mx_put(o, v[r], left);
+    for (int r = 0; r < 4; ++r) {
+      uint16_t* o = out + ((long long)(m + 32 * j + 8 * r) * ldo + n + 32 * i);
+      if (8 * r + t0 < rows) {
+        if constexpr (VEC)
+          *(u32x4*)(o + lane_at) = v[r];
+        else
+          mx_put(o + lane_at, v[r], left);
+      }
+    }
   };
 #pragma unroll
-  for (int k = 0; k < TA * (TW / IW); ++k) {
-    const int j = k / (TW / IW), ii = k % (TW / IW) * IW;
+  for (int k = 0; k < TA * (TW / 2); ++k) {
+    const int j = k / (TW / 2), ii = k % (TW / 2) * 2;
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < IW; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         float f[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           f[e] = GELU ? mx_gelu(acc[ii + i][j][4 * q + e]) : acc[ii + i][j][4 * q + e];
-        *(u32x2*)(so + (lane & 31) * (16 * LR) + (((4 * i + q) ^ (lane & (LR - 1))) * 16) + 8 * hh) =
+        *(u32x2*)(so + (lane & 31) * 128 + (((4 * i + q) ^ (lane & 7)) * 16) + 8 * hh) =
             u32x2{Pk<T>::pack(f[0], f[1]), Pk<T>::pack(f[2], f[3])};
       }
     __builtin_amdgcn_sched_barrier(0);
-    if (k) put((k - 1) / (TW / IW), (k - 1) % (TW / IW) * IW);
+    if (k) put((k - 1) / (TW / 2), (k - 1) % (TW / 2) * 2);
 #pragma unroll
-    for (int r = 0; r < RS; ++r) {
-      const int t = RT * r + t0;
-      v[r] = *(const u32x4*)(so + t * (16 * LR) + ((c ^ (t & (LR - 1))) * 16));
+    for (int r = 0; r < 4; ++r) {
+      const int t = 8 * r + t0;
+      v[r] = *(const u32x4*)(so + t * 128 + ((c ^ (t & 7)) * 16));
     }
   }
-  put(TA - 1, TW - IW);
+  put(TA - 1, TW - 2);
 }
 
 // ---- the 256 x 256 tile: its inner loop is written out ----------------------
@@ -462,7 +475,7 @@ __device__ inline void mx_step1(f32x16 (&acc)[4][4], const MxFrags& f, MxFrags& 
 // products as one stream over all of them, so a tile's first stages are loaded
 // under the last products and the epilogue of the one before; the epilogue has
 // LDS of its own (4 KB a wave).
-template <typename T, bool GELU>
+template <typename T, bool GELU, bool VEC>
 __global__ __launch_bounds__(256, 1) void mx_big_kernel(MxMat a, MxMat w, const uint16_t* __restrict__ bias,
                                                         uint16_t* __restrict__ out, long long ldo,
                                                         int groups, int mt, int nt, int per_xcd) {
@@ -511,7 +524,7 @@ __global__ __launch_bounds__(256, 1) void mx_big_kernel(MxMat a, MxMat w, const 
   };
   const uint32_t dst = lds0 + wave * 8192, sdst = lds0 + C::CODES + wave * 1024;
   auto issue = [&](uint32_t off, int i) {  // KB i of a pair
-    asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[v], %[g]" ::[m] "s"(
+    asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %[v], %[g]" ::[m] "s"(
                      dst + off + (i >> 3) * ST + (i & 7) * 1024),
                  [v] "v"(col(i >> 3)), [g] "s"(d.g[i & 7])
                  : "memory");
@@ -550,11 +563,7 @@ __global__ __launch_bounds__(256, 1) void mx_big_kernel(MxMat a, MxMat w, const 
   for (;;) {
     int m0, n0;
     mx_place(id, mt, nt, 8, 8, m0, n0);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = zero16();
-    mx_bias_add<T>(acc, bias, (float*)own, (n0 + wn * 4) * 32, w.rows);  // the sums start at the bias
+    mx_start<T>(acc, bias, (float*)own, (n0 + wn * 4) * 32, w.rows);
     for (int g = groups; g > 0; --g) {
       const uint32_t other = PAIR - 2 * off;  // from this pair to the other one (off: 0 or PAIR)
       mx_step0<0, 1024>(acc, f0, f1, sc, bw, ba, d.g + 4, dst + PAIR - off + ST + 4096, col(1), 0, nullptr);
@@ -569,7 +578,7 @@ __global__ __launch_bounds__(256, 1) void mx_big_kernel(MxMat a, MxMat w, const 
     }
     // the last products' registers are readable after 18 cycles of issue
     asm volatile("s_nop 15\n\ts_nop 15" : MX_ACC);
-    mx_store<T, 4, 4, GELU>(acc, own, out, ldo, (m0 + wm * 4) * 32, a.rows, (n0 + wn * 4) * 32, w.rows);
+    mx_store<T, 4, 4, GELU, VEC>(acc, own, out, ldo, (m0 + wm * 4) * 32, a.rows, (n0 + wn * 4) * 32, w.rows);
     id += step;
     if (id >= end) break;
   }
@@ -633,13 +642,14 @@ __device__ inline void mx_mid_step(f32x16 (&acc)[2][2], const MxMidFrags& f, MxM
 #undef MX_MID_IN
 }
 
-template <typename T, bool GELU>
+template <typename T, bool GELU, bool VEC>
 __global__ __launch_bounds__(256, 2) void mx_mid_kernel(MxMat a, MxMat w, const uint16_t* __restrict__ bias,
                                                         uint16_t* __restrict__ out, long long ldo, int groups,
                                                         int mt, int nt, int per_xcd) {
   using C = MxTile<2, 2>;
   constexpr int ST = C::STAGE, PAIR = 2 * ST;
   __shared__ __attribute__((aligned(1024))) char lds[4 * ST];
+  __shared__ __attribute__((aligned(16))) float sbias[4][64];
   const int id = mx_first(per_xcd);
   if (id >= mx_end(mt, nt, per_xcd)) return;
   int m0, n0;
@@ -666,7 +676,7 @@ __global__ __launch_bounds__(256, 2) void mx_mid_kernel(MxMat a, MxMat w, const 
   for (int s = 0; s < 4; ++s) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[v], %[g]" ::[m] "s"(
+      asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %[v], %[g]" ::[m] "s"(
                        dst + s * ST + i * 1024),
                    [v] "v"(col(s)), [g] "s"(g[i])
                    : "memory");
@@ -675,6 +685,8 @@ __global__ __launch_bounds__(256, 2) void mx_mid_kernel(MxMat a, MxMat w, const 
                    [v] "v"(scol(s))
                    : "memory");
   }
+  f32x16 acc[2][2];
+  mx_start<T>(acc, bias, sbias[wave], (n0 + wn * 2) * 32, w.rows);
   uint32_t bw = lds0 + wn * 4096 + l16, ba = lds0 + 8192 + wm * 4096 + l16;
   uint32_t sw = lds0 + wn * 512 + lane * 4, sa = lds0 + 1024 + wm * 512 + lane * 4;
   uint32_t off = 0;
@@ -691,11 +703,6 @@ __global__ __launch_bounds__(256, 2) void mx_mid_kernel(MxMat a, MxMat w, const 
                : [bw] "v"(bw), [ba] "v"(ba), [o0] "n"(0), [o1] "n"(2048), [o2] "n"(1024), [o3] "n"(3072),
                  [sbw] "v"(sw), [sba] "v"(sa), [t0] "n"(C::CODES), [t1] "n"(C::CODES + 256)
                : "memory");
-  f32x16 acc[2][2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = zero16();
   for (int s = 0; s < n; s += 2) {
     const uint32_t other = PAIR - 2 * off;  // from this pair of stages to the other one
     mx_mid_step<0, ST, 0>(acc, f0, f1, sc, nsc, bw, ba, sw, sa, g, dst + off, col(s + 4), sdst + off,
@@ -713,8 +720,7 @@ __global__ __launch_bounds__(256, 2) void mx_mid_kernel(MxMat a, MxMat w, const 
                :
                : "memory");
   char* own = lds + wave * 4096;
-  mx_bias_add<T>(acc, bias, (float*)own, (n0 + wn * 2) * 32, w.rows);
-  mx_store<T, 2, 2, GELU>(acc, own, out, ldo, (m0 + wm * 2) * 32, a.rows, (n0 + wn * 2) * 32, w.rows);
+  mx_store<T, 2, 2, GELU, VEC>(acc, own, out, ldo, (m0 + wm * 2) * 32, a.rows, (n0 + wn * 2) * 32, w.rows);
 }
 
 // ---- small launches: the columns split over the waves ------------------------
@@ -880,11 +886,19 @@ static int mx_tile_launch(const MxMat& a, const MxMat& w, const uint16_t* bias, 
   auto launch = [&](auto kernel, int slots) {
     hipLaunchKernelGGL(kernel, dim3(8 * slots), dim3(256), 0, st, a, w, bias, out, ldo, groups, mt, nt, per);
   };
+  auto form = [&](auto G, auto V) {
+    constexpr bool GELU = decltype(G)::value, VEC = decltype(V)::value;
+    if constexpr (TW == 4)  // fills a CU: 32 work-groups an XCD, which go through the tiles
+      launch(mx_big_kernel<T, GELU, VEC>, per < 32 ? per : 32);
+    else
+      launch(mx_mid_kernel<T, GELU, VEC>, per);
+  };
   const bool gelu = act == T2T_ACT_GELU_TANH;
-  if constexpr (TW == 4)  // fills a CU: 32 work-groups an XCD, which go through the tiles
-    launch(gelu ? mx_big_kernel<T, true> : mx_big_kernel<T, false>, per < 32 ? per : 32);
+  const bool vec = w.rows % 8 == 0 && ldo % 8 == 0 && (uintptr_t)out % 16 == 0;
+  if (gelu)
+    vec ? form(std::true_type{}, std::true_type{}) : form(std::true_type{}, std::false_type{});
   else
-    launch(gelu ? mx_mid_kernel<T, true> : mx_mid_kernel<T, false>, per);
+    vec ? form(std::false_type{}, std::true_type{}) : form(std::false_type{}, std::false_type{});
   T2T_LAUNCH_CHECK("mxfp4_product");
   return T2T_OK;
 }
