@@ -489,7 +489,7 @@ size_t t2t_mxfp4_scale_bytes(int M, int K);
 int t2t_mxfp4_quantize(const void* x, int dtype, long long row_stride, void* codes, void* scales,
                        int M, int K, void* stream);
 /* The values that codes and scales stand for -> out [M, K] fp16 / bf16 (exact
- * in the type that was quantised). */
+ * in the type that was quantised, and in bf16). */
 int t2t_mxfp4_dequantize(const void* codes, const void* scales, void* out, int dtype,
                          long long row_stride, int M, int K, void* stream);
 #define T2T_ACT_NONE      0

@@ -22,12 +22,10 @@ typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 static inline long long mx_row_blocks(int M) { return ((long long)M + 31) / 32; }
 static inline int mx_kp(int K) { return (K + 255) / 256 * 256; }
 
-extern "C" size_t t2t_mxfp4_code_bytes(int M, int K) {
-  return M <= 0 || K <= 0 ? 0 : (size_t)mx_row_blocks(M) * mx_kp(K) * 16;
-}
 extern "C" size_t t2t_mxfp4_scale_bytes(int M, int K) {
-  return M <= 0 || K <= 0 ? 0 : (size_t)mx_row_blocks(M) * mx_kp(K);
+  return M <= 0 || K <= 0 ? 0 : (size_t)mx_row_blocks(M) * (((size_t)K + 255) / 256 * 256);
 }
+extern "C" size_t t2t_mxfp4_code_bytes(int M, int K) { return 16 * t2t_mxfp4_scale_bytes(M, K); }
 
 // a 16-bit matrix beside its codes and scales
 static int mx_check_rows(const char* what, const void* x, int dtype, long long row_stride,
@@ -103,7 +101,9 @@ __device__ inline void mx_block(const u32x4 (&x)[4], u32x4& codes, uint32_t& byt
 }
 
 // ---------------------------------------------------------------------------
-// quantise: a work-group per 32 rows x 256 columns, a thread per block
+// quantise: a work-group per 32 rows x 256 columns, a thread per block (64 bytes
+// of a row; the four loads' lines meet in L1).  Bound: reading x, 75,600 x 5,120
+// in 183 us, 5.4 TB/s with the codes written.
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const uint16_t* __restrict__ x,
@@ -154,7 +154,8 @@ extern "C" int t2t_mxfp4_quantize(const void* x, int dtype, long long row_stride
 // ---------------------------------------------------------------------------
 // the values back: 32 lanes take a row of the 256 columns, eight values each, so
 // that the stores are whole rows (a thread per block, with its four stores 64
-// bytes apart from its neighbour's, took 260 us at 75,600 x 5,120)
+// bytes apart from its neighbour's, took 260 us at 75,600 x 5,120; this takes
+// 194, 5.0 TB/s).  Bound: writing the values.
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint32_t* __restrict__ codes,
@@ -362,11 +363,17 @@ __device__ inline void mx_store(const f32x16 (&acc)[TW][TA], char* so, uint16_t*
 // ---- the 256 x 256 tile: its inner loop is written out ----------------------
 // With 256 accumulators a SIMD holds one wave, so no other wave covers a wait,
 // and left to itself the compiler issues a fragment read right before the
-// product that needs it.  A step is one asm block of sixteen products (64
-// columns): the next step's eight fragment reads and half a stage's DMA go
-// between them, and the one wait at its end finds the reads old.  The DMA is
-// spread over both steps of a stage: the CU takes a KB in 16 cycles, and eight
-// of each wave's within 256 cycles held the products up.
+// product that needs it (2.93 ms at 75,600 x 13,824 x 5,120; 2.52 written out).
+// A step is one asm block of sixteen products (64 columns): the next step's eight
+// fragment reads and half a stage's DMA go between them, and the one wait at its
+// end finds the reads old.  A block waits for its own reads, so none of its
+// outputs is in flight outside it.
+// Why this tile: per stage a CU moves 36 KB to LDS (64 bytes a cycle at most) and
+// reads 64 KB from it for 1024 cycles of products; with 128 x 128 it is LDS that
+// bounds.  Measured: 1203 cycles a stage and 12,000 a tile, 4.4 PFLOP/s at K =
+// 5120, 4.9 at 13,824.  Bound: power.  The card holds 1.5 GHz of 2.4 on random
+// codes; with loads that always hit L2, or reads and DMA placed otherwise, the
+// time is the same, and with zero codes it is 1.3 times shorter.
 #define MX_P(i, j)                                                                                      \
   "v_mfma_scale_f32_32x32x64_f8f6f4 %[c" #i #j "], %[w" #i "], %[a" #j "], %[c" #i #j "], %[p" #i     \
   "], %[q" #j "] " MX_SEL " cbsz:4 blgp:4\n\t"
@@ -390,8 +397,8 @@ __device__ inline void mx_store(const f32x16 (&acc)[TW][TA], char* so, uint16_t*
 #define MX_READS(OFF)                                                                                   \
   [bw] "v"(bw), [ba] "v"(ba), [o0] "n"(OFF), [o1] "n"((OFF) + 2048), [o2] "n"((OFF) + 4096),            \
       [o3] "n"((OFF) + 6144)
-// where the reads and the DMA of a step go; D0 .. D3: a DMA, X: what else the step has to issue
-// (products in an order that changes one operand at a time)
+// where the reads and the DMA of a step go; X0 .. X3: what else it has to issue (products in an order
+// that changes one operand at a time)
 #define MX_STEP(X0, X1, X2, X3)                                                                         \
   MX_P(0, 0) MX_R("x0", "bw", "o0") MX_P(0, 1) MX_R("y0", "ba", "o0") MX_P(0, 2) MX_R("x1", "bw", "o1") \
       MX_P(0, 3) MX_D(0) X0 MX_P(1, 3) MX_R("y1", "ba", "o1") MX_P(1, 2) MX_R("x2", "bw", "o2")         \
@@ -584,14 +591,14 @@ __global__ __launch_bounds__(256, 1) void mx_big_kernel(MxMat a, MxMat w, const 
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
-// ---- end of the 256 x 256 tile
 
 // ---- the 128 x 128 tile ------------------------------------------------------
 // The same with a whole stage a step: eight products, the next stage's eight
 // fragment reads and the DMA of the stage four further on.  Bound by LDS: at 128
 // bytes a cycle a stage's reads (32 KB) and the DMA's writes (18 KB) take 400
 // cycles, its products 256.  Two work-groups fit a CU; eight stages instead
-// (one work-group a CU) gained nothing at 512 x 5120 x 5120 (11.5 and 12.3 us).
+// (one work-group a CU) gained nothing at 512 x 5120 x 5120 (11.5 and 12.3 us;
+// 17.0 with the compiler's schedule).
 #define MX_Q(c, i, j, SEL)                                                                              \
   "v_mfma_scale_f32_32x32x64_f8f6f4 %[c" #i #j "], %[w" #c #i "], %[a" #c #j "], %[c" #i #j           \
   "], %[p" #i "], %[q" #j "] " SEL " cbsz:4 blgp:4\n\t"
@@ -724,12 +731,15 @@ __global__ __launch_bounds__(256, 2) void mx_mid_kernel(MxMat a, MxMat w, const 
 }
 
 // ---- small launches: the columns split over the waves ------------------------
-// 32 NB features x 32 tokens a work-group; its waves take units of 128 columns in
-// turn, so every fragment is loaded once, straight into registers (no staging,
+// 32 features x 32 tokens a work-group; its eight waves take units of 128 columns
+// in turn, so every fragment is loaded once, straight into registers (no staging,
 // no barrier in the loop), DEPTH units ahead.  The waves' sums meet in LDS, in
 // the order of the waves.  With X16 the tokens come in 16 bits and every
 // work-group quantises them into LDS first (MX_X16_BLOCKS blocks at most), under
 // the loads of its first weights, in the place of a launch before this one.
+// Bound: one round of loads and the exchange (1 x 5120 x 5120: 5.8 us, with X16
+// 6.4 and 8.3 in two launches); with more tokens the bytes from L2, which every
+// 32 x 32 block reads for itself.
 #define MX_X16_BLOCKS 2048
 struct MxSrc {
   MxMat m;            // in MXFP4 (its row count in either case), or
@@ -738,44 +748,35 @@ struct MxSrc {
   int K;
 };
 
-template <typename T, int NB, int WAVES, int DEPTH, bool GELU, bool X16>
-__global__ __launch_bounds__(64 * WAVES) void mx_split_kernel(MxSrc a, MxMat w,
-                                                              const uint16_t* __restrict__ bias,
-                                                              uint16_t* __restrict__ out, long long ldo,
-                                                              int groups, int mt, int nt, int per_xcd) {
-  __shared__ f32x4 part[WAVES][NB][4][64];
+template <typename T, int DEPTH, bool GELU, bool X16>
+__global__ __launch_bounds__(512) void mx_split_kernel(MxSrc a, MxMat w, const uint16_t* __restrict__ bias,
+                                                       uint16_t* __restrict__ out, long long ldo, int groups,
+                                                       int mt, int nt, int per_xcd) {
+  constexpr int WAVES = 8;
+  __shared__ f32x4 part[WAVES][4][64];
   __shared__ u32x4 xc[X16 ? MX_X16_BLOCKS : 1];
   __shared__ uint8_t xs[X16 ? MX_X16_BLOCKS : 1];
   const int id = mx_first(per_xcd);
   if (id >= mx_end(mt, nt, per_xcd)) return;
-  int mb, n0;
-  mx_place(id, mt, nt, 1, NB, mb, n0);
+  int mb, nb;
+  mx_place(id, mt, nt, 1, 1, mb, nb);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = 2 * groups;
-  const char* pw[NB];
-  const uint32_t* qw[NB];
-#pragma unroll
-  for (int i = 0; i < NB; ++i) {
-    const long long row = min(n0 + i, w.blocks - 1);
-    pw[i] = w.codes + row * groups * 4096;
-    qw[i] = w.scales + row * groups * 64;
-  }
+  const char* pw = w.codes + (long long)nb * groups * 4096;
+  const uint32_t* qw = w.scales + (long long)nb * groups * 64;
   const char* pa = X16 ? nullptr : a.m.codes + (long long)mb * groups * 4096;
   const uint32_t* qa = X16 ? nullptr : a.m.scales + (long long)mb * groups * 64;
   const int row = mb * 32 + (lane & 31);
   struct Unit {
-    u32x4 w[2][NB], a[2];
-    uint32_t sw[NB], sa;
+    u32x4 w[2], a[2];
+    uint32_t sw, sa;
   };
   auto load = [&](int s, Unit& t) {
     const size_t o = (size_t)s * 2048 + lane * 16, os = (size_t)(s >> 1) * 64 + lane;
     const int sh = 16 * (s & 1);  // an odd unit's scales are the upper half
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      t.w[0][i] = *(const u32x4*)(pw[i] + o);
-      t.w[1][i] = *(const u32x4*)(pw[i] + o + 1024);
-      t.sw[i] = qw[i][os] >> sh;
-    }
+    t.w[0] = *(const u32x4*)(pw + o);
+    t.w[1] = *(const u32x4*)(pw + o + 1024);
+    t.sw = qw[os] >> sh;
     if constexpr (!X16) {
       t.a[0] = *(const u32x4*)(pa + o);
       t.a[1] = *(const u32x4*)(pa + o + 1024);
@@ -792,15 +793,7 @@ __global__ __launch_bounds__(64 * WAVES) void mx_split_kernel(MxSrc a, MxMat w,
       t.sa = xs[b] | (xs[b + 2] << 8);
     }
   };
-  f32x16 acc[NB];
-#pragma unroll
-  for (int i = 0; i < NB; ++i) acc[i] = zero16();
-  auto mul = [&](const Unit& t) {
-#pragma unroll
-    for (int i = 0; i < NB; ++i) acc[i] = mx_mfma<0>(t.w[0][i], t.a[0], acc[i], t.sw[i], t.sa);
-#pragma unroll
-    for (int i = 0; i < NB; ++i) acc[i] = mx_mfma<1>(t.w[1][i], t.a[1], acc[i], t.sw[i], t.sa);
-  };
+  f32x16 acc = zero16();
   Unit ring[DEPTH];
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d)
@@ -823,51 +816,52 @@ __global__ __launch_bounds__(64 * WAVES) void mx_split_kernel(MxSrc a, MxMat w,
   for (int s = wave; s < n; s += DEPTH * WAVES) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
+      Unit& t = ring[d];
       if (s + d * WAVES < n) {
-        if constexpr (X16) fetch(s + d * WAVES, ring[d]);
-        mul(ring[d]);
+        if constexpr (X16) fetch(s + d * WAVES, t);
+        acc = mx_mfma<0>(t.w[0], t.a[0], acc, t.sw, t.sa);
+        acc = mx_mfma<1>(t.w[1], t.a[1], acc, t.sw, t.sa);
       }
-      if (s + (d + DEPTH) * WAVES < n) load(s + (d + DEPTH) * WAVES, ring[d]);
+      if (s + (d + DEPTH) * WAVES < n) load(s + (d + DEPTH) * WAVES, t);
     }
   }
 #pragma unroll
-  for (int i = 0; i < NB; ++i)
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      part[wave][i][q][lane] = f32x4{acc[i][4 * q], acc[i][4 * q + 1], acc[i][4 * q + 2], acc[i][4 * q + 3]};
+  for (int q = 0; q < 4; ++q)
+    part[wave][q][lane] = f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
   __syncthreads();
-  // quarter q of a block: four features of each token
-  for (int iq = wave; iq < 4 * NB; iq += WAVES) {
-    const int i = iq >> 2, q = iq & 3;
-    f32x4 v = part[0][i][q][lane];
+  if (wave >= 4) return;
+  // quarter q: four features of each token
+  const int q = wave, f = nb * 32 + 8 * q + 4 * (lane >> 5);
+  f32x4 v = part[0][q][lane];
 #pragma unroll
-    for (int x = 1; x < WAVES; ++x) {
-      const f32x4 y = part[x][i][q][lane];
+  for (int x = 1; x < WAVES; ++x) {
+    const f32x4 y = part[x][q][lane];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += y[e];
+    for (int e = 0; e < 4; ++e) v[e] += y[e];
+  }
+  if (row < a.m.rows && f < w.rows) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (bias) v[e] += T::to_f(bias[min(f + e, w.rows - 1)]);
+      if (GELU) v[e] = mx_gelu(v[e]);
     }
-    const int f = (n0 + i) * 32 + 8 * q + 4 * (lane >> 5);
-    if (row < a.m.rows && f < w.rows) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (bias) v[e] += T::to_f(bias[min(f + e, w.rows - 1)]);
-        if (GELU) v[e] = mx_gelu(v[e]);
-      }
-      mx_put(out + row * ldo + f, u32x2{Pk<T>::pack(v[0], v[1]), Pk<T>::pack(v[2], v[3])}, w.rows - f);
-    }
+    mx_put(out + row * ldo + f, u32x2{Pk<T>::pack(v[0], v[1]), Pk<T>::pack(v[2], v[3])}, w.rows - f);
   }
 }
 
-template <typename T, int NB, int WAVES, int DEPTH, bool X16>
+template <typename T, int DEPTH, bool X16>
 static int mx_split_launch(const MxSrc& a, const MxMat& w, const uint16_t* bias, int act, uint16_t* out,
                            long long ldo, int groups, hipStream_t st) {
-  const int nt = cdiv(w.blocks, NB);
-  const long long tiles = (long long)a.m.blocks * nt;
+  const long long tiles = (long long)a.m.blocks * w.blocks;
   const int per = cdiv(tiles, 8);
-  auto kernel = act == T2T_ACT_GELU_TANH ? mx_split_kernel<T, NB, WAVES, DEPTH, true, X16>
-                                         : mx_split_kernel<T, NB, WAVES, DEPTH, false, X16>;
-  hipLaunchKernelGGL(kernel, dim3(8 * per), dim3(64 * WAVES), 0, st, a, w, bias, out, ldo, groups, a.m.blocks,
-                     nt, per);
+  if (per > (1 << 19)) {  // 2^31 threads
+    t2t_set_error("mxfp4_product: M=%d N=%d", a.m.rows, w.rows);
+    return T2T_ERR_UNSUPPORTED;
+  }
+  auto kernel =
+      act == T2T_ACT_GELU_TANH ? mx_split_kernel<T, DEPTH, true, X16> : mx_split_kernel<T, DEPTH, false, X16>;
+  hipLaunchKernelGGL(kernel, dim3(8 * per), dim3(512), 0, st, a, w, bias, out, ldo, groups, a.m.blocks,
+                     w.blocks, per);
   T2T_LAUNCH_CHECK("mxfp4_product");
   return T2T_OK;
 }
@@ -903,13 +897,19 @@ static int mx_tile_launch(const MxMat& a, const MxMat& w, const uint16_t* bias, 
   return T2T_OK;
 }
 
+// Which product: by the number of outputs.  Below 512 blocks of 32 x 32 too few tiles would go through
+// all of K one stage after another (64 x 5120 x 5120: split 7.6 us, 128 x 128 tiles 10.6; 128 x 5120 x
+// 5120: 10.7 and 10.8; 256 x: 15.8 and 11.0).  From 256 large tiles on they fill the chip (4096^3: 37.4
+// us, 128 x 128 tiles 42.1; 1500 x 5120 x 5120, 120 large tiles: 33.3 and 25.9), unless K is short and
+// they are few (9000 x 2048 x 512: 20.4 and 15.8; 75,600 x 5120 x 128: 172 and 208) or they would be
+// padded by more than a quarter over the small ones (75,600 x 96 x 1536: 34.1 and 17.7).
 template <typename T>
 static int mx_product(const MxMat& a, const MxMat& w, const uint16_t* bias, int act, uint16_t* out,
                       long long ldo, int groups, hipStream_t st) {
   const long long big = (long long)cdiv(a.blocks, 8) * cdiv(w.blocks, 8);
   const long long mid = (long long)cdiv(a.blocks, 4) * cdiv(w.blocks, 4);
   if ((long long)a.blocks * w.blocks <= 512)
-    return mx_split_launch<T, 1, 8, 4, false>(MxSrc{a, nullptr, 0, 0}, w, bias, act, out, ldo, groups, st);
+    return mx_split_launch<T, 4, false>(MxSrc{a, nullptr, 0, 0}, w, bias, act, out, ldo, groups, st);
   if (big >= 256 && (groups >= 4 || big >= 1024) && 4 * big <= mid + mid / 4)
     return mx_tile_launch<T, 4, 4>(a, w, bias, act, out, ldo, groups, st);
   return mx_tile_launch<T, 2, 2>(a, w, bias, act, out, ldo, groups, st);
@@ -946,7 +946,8 @@ extern "C" int t2t_mxfp4_product(const void* a_codes, const void* a_scales, cons
                           (hipStream_t)stream);
 }
 
-// few rows are quantised by the product itself
+// Few rows are quantised by the product itself, as far as its LDS holds them: every work-group does it
+// again, which costs what the saved launch gains at 12 x 5120 (8.2 us either way; 1 x: 6.4 and 8.3).
 static bool mx_few(int M, int K) { return M <= 32 && (long long)M * (mx_kp(K) / 32) <= MX_X16_BLOCKS; }
 
 // codes, then scales
@@ -966,7 +967,7 @@ extern "C" int t2t_mxfp4_linear(const void* x, int dtype, long long x_row_stride
   if (mx_few(M, K)) {
     const MxSrc a{MxMat{nullptr, nullptr, M, (int)mx_row_blocks(M)}, (const uint16_t*)x, x_row_stride, K};
     const MxMat w{(const char*)w_codes, (const uint32_t*)w_scales, N, (int)mx_row_blocks(N)};
-    auto run = dtype == T2T_BF16 ? mx_split_launch<BF16T, 1, 8, 2, true> : mx_split_launch<F16T, 1, 8, 2, true>;
+    auto run = dtype == T2T_BF16 ? mx_split_launch<BF16T, 2, true> : mx_split_launch<F16T, 2, true>;
     return run(a, w, (const uint16_t*)bias, act, (uint16_t*)out, out_row_stride, mx_kp(K) / 256,
                (hipStream_t)stream);
   }

@@ -1040,7 +1040,7 @@ def mxfp4_quantize(x, out=None, stream=None):
 
 def mxfp4_dequantize(t, dtype=torch.bfloat16, out=None, stream=None):
     """The values that an MxFp4 matrix stands for, [rows, cols]: exact in the
-    type that was quantised, and in bf16 where no scale is below 2^-126."""
+    type that was quantised, and in bf16 always."""
     if not isinstance(t, MxFp4):
         raise ValueError("t2t: expected an MxFp4 matrix")
     dev = t._device
