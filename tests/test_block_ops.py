@@ -250,7 +250,9 @@ ROTARY = [  # B, N, HQ, HK, D, R
     (1, 1, 40, 40, 128, 128), (4, 1, 12, 2, 128, 128), (1, 5, 1, 1, 2, 2), (2, 33, 5, 3, 64, 32),
     (1, 130, 7, 1, 80, 80), (1, 9, 3, 3, 96, 48), (3, 17, 33, 8, 128, 96), (1, 40, 65, 9, 128, 128),
     (1, 7, 4, 2, 256, 256), (1, 7, 4, 2, 256, 64), (1, 6, 2, 2, 88, 24), (1, 6, 3, 1, 77, 20),
-    (1, 3, 300, 130, 128, 128), (2, 300, 12, 12, 128, 64), (1, 4, 700, 1, 64, 64)]
+    (1, 3, 300, 130, 128, 128), (2, 300, 12, 12, 128, 64), (1, 4, 700, 1, 64, 64), (1, 1501, 3, 1, 64, 32),
+    (2, 1100, 1, 1, 40, 40), (1, 1203, 32, 8, 256, 128), (1, 1025, 40, 5, 128, 128), (3, 701, 5, 2, 20, 12),
+    (1, 1300, 33, 2, 80, 40)]
 
 
 @pytest.mark.gpu
@@ -341,7 +343,8 @@ def test_rotary_results_do_not_depend_on_the_company(dev):
     """A token's result is the same bits alone and among many, whatever the form
     its call takes."""
     g, dt = _gen(dev, 21), torch.bfloat16
-    for D, H, norm in ((128, 40, "token"), (96, 12, "token"), (128, 12, "head"), (64, 70, "token")):
+    for D, H, norm in ((128, 40, "token"), (96, 12, "token"), (128, 12, "head"), (64, 70, "token"),
+                       (64, 1, "token"), (40, 3, "token"), (20, 2, "head"), (256, 32, "token")):
         q = _randn(g, 2000, H, D).to(dt)
         cos, sin = _tables(g, (2000,), D)
         w = (1 + 0.2 * _randn(g, H * D if norm == "token" else D)).to(dt)

@@ -629,7 +629,7 @@ __device__ inline void mx_mid_step(f32x16 (&acc)[2][2], const MxMidFrags& f, MxM
   [w00] "v"(f.w[0][0]), [w01] "v"(f.w[0][1]), [w10] "v"(f.w[1][0]), [w11] "v"(f.w[1][1]),               \
       [a00] "v"(f.a[0][0]), [a01] "v"(f.a[0][1]), [a10] "v"(f.a[1][0]), [a11] "v"(f.a[1][1]),           \
       [p0] "v"(sc.w[0]), [p1] "v"(sc.w[1]), [q0] "v"(sc.a[0]), [q1] "v"(sc.a[1]), [bw] "v"(bw),         \
-      [ba] "v"(ba), [o0] "n"(OFF), [o1] "n"(OFF + 2048), [o2] "n"(OFF + 1024), [o3] "n"(OFF + 3072),    \
+      [ba] "v"(ba), [o0] "n"(OFF), [o1] "n"(OFF + 2048), [o2] "n"(OFF + 1024), [o3] "n"(OFF + 3 * 1024),    \
       [m] "s"(m), [v] "v"(v), [g0] "s"(g[0]), [g1] "s"(g[1]), [g2] "s"(g[2]), [g3] "s"(g[3])
   if constexpr (!ODD)
     asm volatile(MX_MID_STEP("op_sel:[0,0,0] op_sel_hi:[0,0,0]", "op_sel:[1,1,0] op_sel_hi:[0,0,0]", "")
@@ -707,7 +707,7 @@ __global__ __launch_bounds__(256, 2) void mx_mid_kernel(MxMat a, MxMat w, const 
                  [x11] "=&v"(f0.w[1][1]), [y00] "=&v"(f0.a[0][0]), [y01] "=&v"(f0.a[0][1]),
                  [y10] "=&v"(f0.a[1][0]), [y11] "=&v"(f0.a[1][1]), [n0] "=&v"(sc.w[0]), [n1] "=&v"(sc.w[1]),
                  [r0] "=&v"(sc.a[0]), [r1] "=&v"(sc.a[1])
-               : [bw] "v"(bw), [ba] "v"(ba), [o0] "n"(0), [o1] "n"(2048), [o2] "n"(1024), [o3] "n"(3072),
+               : [bw] "v"(bw), [ba] "v"(ba), [o0] "n"(0), [o1] "n"(2048), [o2] "n"(1024), [o3] "n"(3 * 1024),
                  [sbw] "v"(sw), [sba] "v"(sa), [t0] "n"(C::CODES), [t1] "n"(C::CODES + 256)
                : "memory");
   for (int s = 0; s < n; s += 2) {

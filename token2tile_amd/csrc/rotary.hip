@@ -117,14 +117,17 @@ extern "C" int t2t_rotary_table(const void* positions, int pos_bits, long long T
 // x 40 heads x 128: 575 us, 5.4 TB/s; pair by pair in the general form below 2.1
 // ms; 4 tokens: 4.8 us).
 //
-// A head is cut into units of 16 channels that turn together: with paired
-// halves channels 8 u .. + 7 and R / 2 + 8 u .. + 7, else 16 u .. + 15; unit u
-// reads entries 8 u .. + 7 of the tables in both layouts.  Lane l of a wave
-// holds unit l % L (L: units rounded up to a power of two) of heads l / L, l /
-// L + 64 / L, ...: its entries are read once a token, and the norm's sum over a
-// head is one over L neighbouring lanes.  A token's heads stay in registers
-// (ITS of them a lane) between the sum and the turn, and the token norm's weights
-// from token to token: a work-group goes through many.
+// A head is cut into units of 2 V channels that turn together (V: 8, or 4 where
+// widths, strides or addresses ask for it): with paired halves channels V u .. +
+// V - 1 and R / 2 + V u .. + V - 1, else 2 V u .. + 2 V - 1; unit u reads entries
+// V u .. + V - 1 of the tables in both layouts.  The lanes of a wave are units of
+// heads of tokens: L lanes a head (units rounded up to a power of two), then as
+// many heads as there are or fit, then tokens, where few heads leave lanes over.
+// A lane's table entries are read once a token, the norm's sums run over
+// neighbouring lanes, and a token's heads stay in registers (ITS of them a lane)
+// between the sum and the turn, as do the token norm's weights from token to
+// token: a work-group goes through many.  (One head of 64 in 75,600 tokens: 15 us,
+// 73 with a token a wave; 32 + 8 heads of 96 in 20,000: 77 us.)
 // ---------------------------------------------------------------------------
 struct RotaryArgs {
   const float* cosv;
@@ -133,12 +136,13 @@ struct RotaryArgs {
   long long tokens;
   int N, D, R, half;
   float sign, eps;
-  int units, shift;  // units of a head, log2(L)
+  int units, shift;          // units of a head, log2(L)
+  int hshift[2], chunks[2];  // q and k: log2 of a wave's heads, rounds of ITS that a token takes
 };
 
-// What every form below computes alike, so that a view's result does not depend on the form that its
-// strides take: the turn (one product rounded, one fused), and the norm's sum, fp32 over each eight
-// channels of a head in their order and fp64 over these (no order of which shows in fp32).
+// What every form below computes alike, so that a result does not depend on the form that its call's
+// shape and strides take: the turn (one product rounded, one fused), and the norm's sum, fp32 over
+// each four channels of a head in their order and fp64 over these (no order of which shows in fp32).
 __device__ inline void rope_turn(float a, float e, float c, float s, float& y0, float& y1) {
   y0 = __builtin_fmaf(a, c, -(e * s));
   y1 = __builtin_fmaf(a, s, e * c);
@@ -147,160 +151,179 @@ __device__ inline double rope_sum(double v, int lanes) {  // over groups of `lan
   for (int d = 1; d < lanes; d <<= 1) v += __shfl_xor(v, d, 64);
   return v;
 }
-__device__ inline float rope_squares(const float (&f)[8], int n) {
-  float s = f[0] * f[0];
-#pragma unroll
-  for (int e = 1; e < 8; ++e)
-    if (e < n) s = __builtin_fmaf(f[e], f[e], s);
-  return s;
+__device__ inline double rope_squares(float a, float b, float c, float d) {
+  return (double)__builtin_fmaf(d, d, __builtin_fmaf(c, c, __builtin_fmaf(b, b, a * a)));
 }
 __device__ inline float rope_inv(double sum, double one_over_n, float eps) {
   return rsqrtf((float)(sum * one_over_n) + eps);
 }
 
-template <typename T>
-__device__ inline void rope_unpack(const u32x4& v, float (&f)[8]) {
+template <int V> struct RopeVec;
+template <> struct RopeVec<8> {
+  typedef u32x4 type;
+};
+template <> struct RopeVec<4> {
+  typedef u32x2 type;
+};
+template <typename T, int V>
+__device__ inline void rope_unpack(const typename RopeVec<V>::type& v, float (&f)[V]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < V / 2; ++i) {
     f[2 * i] = T::to_f((uint16_t)(v[i] & 0xffff));
     f[2 * i + 1] = T::to_f((uint16_t)(v[i] >> 16));
   }
 }
-template <typename T>
-__device__ inline u32x4 rope_pack(const float (&f)[8]) {
-  u32x4 v;
+template <typename T, int V>
+__device__ inline typename RopeVec<V>::type rope_pack(const float (&f)[V]) {
+  typename RopeVec<V>::type v;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = Pk<T>::pack(f[2 * i], f[2 * i + 1]);
+  for (int i = 0; i < V / 2; ++i) v[i] = Pk<T>::pack(f[2 * i], f[2 * i + 1]);
   return v;
 }
 
-// WPT waves per token (the heads dealt over them), one wave for the ordinary call; NORM as
-// T2T_NORM_*; heads in rounds of ITS (with the token norm there is one round)
-template <typename T, int NORM, int WPT, int ITS>
+// NORM as T2T_NORM_*.  WPT waves to a token: 1, or 4 under the token norm where the tokens are few
+// or a wave's registers do not hold their heads.
+template <typename T, int NORM, int WPT, int ITS, int V>
 __global__ __launch_bounds__(256) void rotary_kernel(t2t_rotary_tensor q, t2t_rotary_tensor k, RotaryArgs A) {
+  typedef typename RopeVec<V>::type vec;
   const t2t_rotary_tensor& g = blockIdx.y ? k : q;
   __shared__ double part[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int L = 1 << A.shift, u = lane & (L - 1);
-  const int wpos = WPT == 1 ? 0 : wave;
-  const int head0 = wpos * (64 >> A.shift) + (lane >> A.shift), hstep = WPT * (64 >> A.shift);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hshift = A.hshift[blockIdx.y], chunks = A.chunks[blockIdx.y];
+  const int L = 1 << A.shift, per = 1 << hshift, span = A.shift + hshift;  // 2^span lanes a token
+  const int u = lane & (L - 1), hl = (lane >> A.shift) & (per - 1), slot = lane >> span;
+  const int hstep = WPT * per;
   // the unit's two halves: where they lie, whether they are there and turn
-  const int tu = A.half ? A.R >> 4 : (A.R + 15) >> 4;  // units that turn
+  const int tu = A.half ? A.R / (2 * V) : (A.R + 2 * V - 1) / (2 * V);  // units that turn
   const bool pair = A.half && u < tu;
-  const int rest = A.R + 16 * (u - tu);
-  const int c0 = pair ? 8 * u : A.half ? rest : 16 * u;
-  const int c1 = pair ? A.R / 2 + 8 * u : c0 + 8;
+  const int rest = A.R + 2 * V * (u - tu);
+  const int c0 = pair ? V * u : A.half ? rest : 2 * V * u;
+  const int c1 = pair ? A.R / 2 + V * u : c0 + V;
   const bool on0 = u < A.units, on1 = on0 && c1 < A.D;
   const bool turn0 = on0 && (A.half ? u < tu : c0 < A.R), turn1 = on1 && (A.half ? u < tu : c1 < A.R);
   const int H = g.heads;
   const double one_over_n = 1.0 / (NORM == T2T_NORM_TOKEN ? (double)H * A.D : (double)A.D);
   const uint16_t* w = (const uint16_t*)g.weight;
-  u32x4 wr[ITS][2];  // the token norm's weights, the same for every token
+  const vec none = {};
+  vec wr[ITS][2];  // the token norm's weights, the same for every token
   if constexpr (NORM == T2T_NORM_TOKEN) {
 #pragma unroll
     for (int i = 0; i < ITS; ++i) {
-      const int h = head0 + i * hstep;
-      wr[i][0] = wr[i][1] = u32x4{0u, 0u, 0u, 0u};
-      if (on0 && h < H) wr[i][0] = *(const u32x4*)(w + (long long)h * A.D + c0);
-      if (on1 && h < H) wr[i][1] = *(const u32x4*)(w + (long long)h * A.D + c1);
+      const int h = (WPT == 1 ? 0 : wave * per) + hl + i * hstep;
+      wr[i][0] = wr[i][1] = none;
+      if (on0 && h < H) wr[i][0] = *(const vec*)(w + (long long)h * A.D + c0);
+      if (on1 && h < H) wr[i][1] = *(const vec*)(w + (long long)h * A.D + c1);
     }
   } else if constexpr (NORM == T2T_NORM_HEAD) {
-    wr[0][0] = wr[0][1] = u32x4{0u, 0u, 0u, 0u};
-    if (on0) wr[0][0] = *(const u32x4*)(w + c0);
-    if (on1) wr[0][1] = *(const u32x4*)(w + c1);
+    wr[0][0] = wr[0][1] = none;
+    if (on0) wr[0][0] = *(const vec*)(w + c0);
+    if (on1) wr[0][1] = *(const vec*)(w + c1);
   }
-  constexpr int TPB = 4 / WPT;  // tokens under way in a work-group
-  for (long long tok = (long long)blockIdx.x * TPB + (WPT == 1 ? wave : 0); tok < A.tokens;
-       tok += (long long)gridDim.x * TPB) {
-    const int b = (int)(tok / A.N), n = (int)(tok - (long long)b * A.N);
+  const long long items = ((A.tokens + (64 >> span) - 1) >> (6 - span)) * chunks;
+  constexpr int IPB = 4 / WPT;  // items under way in a work-group
+  for (long long item = (long long)blockIdx.x * IPB + (WPT == 1 ? wave : 0); item < items;
+       item += (long long)gridDim.x * IPB) {
+    // (chunks is 1 but where the heads of a token go in several items)
+    const long long group = chunks == 1 ? item : item / chunks;
+    const int first = WPT == 1 ? (int)(item - group * chunks) * ITS * per : wave * per;  // the wave's heads
+    const long long tok = (group << (6 - span)) + slot;
+    const bool live = tok < A.tokens;
+    const uint32_t t32 = (uint32_t)(live ? tok : A.tokens - 1), b = t32 / (uint32_t)A.N, n = t32 - b * A.N;
     const uint16_t* x = (const uint16_t*)g.x + b * g.x_batch + n * g.x_row;
     uint16_t* o = (uint16_t*)g.out + b * g.out_batch + n * g.out_row;
-    float cs[8], sn[8];
+    float cs[V], sn[V];
     {
-      const long long row = (b * A.table_batch + n) * (A.R / 2) + 8 * u;
+      const long long row = (b * A.table_batch + n) * (A.R / 2) + V * u;
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
-        f32x4 cv{1.f, 1.f, 1.f, 1.f}, sv{0.f, 0.f, 0.f, 0.f};
-        if (v ? turn1 : turn0) {
-          cv = *(const f32x4*)(A.cosv + row + 4 * v);
-          sv = *(const f32x4*)(A.sinv + row + 4 * v);
-        }
+        // (the unit's first and second half of entries)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) cs[4 * v + i] = cv[i], sn[4 * v + i] = A.sign * sv[i];
+        for (int i = 0; i < V / 2; ++i) cs[V / 2 * v + i] = 1.f, sn[V / 2 * v + i] = 0.f;
+        if (v ? turn1 : turn0) {
+          typedef float fvec __attribute__((ext_vector_type(V / 2)));
+          const fvec cv = *(const fvec*)(A.cosv + row + V / 2 * v), sv = *(const fvec*)(A.sinv + row + V / 2 * v);
+#pragma unroll
+          for (int i = 0; i < V / 2; ++i) cs[V / 2 * v + i] = cv[i], sn[V / 2 * v + i] = A.sign * sv[i];
+        }
       }
     }
-    for (int h0 = head0; NORM == T2T_NORM_TOKEN ? h0 == head0 : h0 - (lane >> A.shift) < H;
-         h0 += ITS * hstep) {
-      u32x4 r[ITS][2];
+    vec r[ITS][2];
+#pragma unroll
+    for (int i = 0; i < ITS; ++i) {
+      const int h = first + hl + i * hstep;
+      r[i][0] = r[i][1] = none;
+      if (on0 && h < H) r[i][0] = *(const vec*)(x + h * g.x_head + c0);
+      if (on1 && h < H) r[i][1] = *(const vec*)(x + h * g.x_head + c1);
+    }
+    float inv[ITS];
+    if constexpr (NORM != T2T_NORM_NONE) {
+      double sum[ITS], all = 0.0;
 #pragma unroll
       for (int i = 0; i < ITS; ++i) {
-        const int h = h0 + i * hstep;
-        r[i][0] = r[i][1] = u32x4{0u, 0u, 0u, 0u};
-        if (on0 && h < H) r[i][0] = *(const u32x4*)(x + h * g.x_head + c0);
-        if (on1 && h < H) r[i][1] = *(const u32x4*)(x + h * g.x_head + c1);
+        sum[i] = 0.0;
+        if (first + i * hstep < H) {  // (the same for the wave)
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            float f[V];
+            rope_unpack<T, V>(r[i][v], f);
+#pragma unroll
+            for (int e = 0; e < V; e += 4) sum[i] += rope_squares(f[e], f[e + 1], f[e + 2], f[e + 3]);
+          }
+        }
+        all += sum[i];
       }
-      float inv[ITS];
+      if constexpr (NORM == T2T_NORM_TOKEN) {
+        all = rope_sum(all, 1 << span);
+        if constexpr (WPT > 1) {
+          __syncthreads();  // the last token's sums are read
+          if (lane == 0) part[wave] = all;
+          __syncthreads();
+          all = part[0] + part[1] + part[2] + part[3];
+        }
+        const float v = rope_inv(all, one_over_n, A.eps);
+#pragma unroll
+        for (int i = 0; i < ITS; ++i) inv[i] = v;
+      } else {
+#pragma unroll
+        for (int i = 0; i < ITS; ++i) inv[i] = rope_inv(rope_sum(sum[i], L), one_over_n, A.eps);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < ITS; ++i) {
+      if (first + i * hstep >= H) break;
+      const int h = first + hl + i * hstep;
+      // the packed values are kept, not their fp32 forms from the sum or the last token
+      asm volatile("" : "+v"(r[i][0]), "+v"(r[i][1]));
       if constexpr (NORM != T2T_NORM_NONE) {
-        double sum[ITS], all = 0.0;
+        constexpr int last = NORM == T2T_NORM_TOKEN ? ITS - 1 : 0;
+        asm volatile("" : "+v"(wr[i < last ? i : last][0]), "+v"(wr[i < last ? i : last][1]));
+      }
+      float f0[V], f1[V], y0[V], y1[V];
+      rope_unpack<T, V>(r[i][0], f0);
+      rope_unpack<T, V>(r[i][1], f1);
+      if constexpr (NORM != T2T_NORM_NONE) {
+        float w0[V], w1[V];
+        const int wi = NORM == T2T_NORM_TOKEN ? i : 0;
+        rope_unpack<T, V>(wr[wi][0], w0);
+        rope_unpack<T, V>(wr[wi][1], w1);
 #pragma unroll
-        for (int i = 0; i < ITS; ++i) {
-          float f0[8], f1[8];
-          rope_unpack<T>(r[i][0], f0);
-          rope_unpack<T>(r[i][1], f1);
-          sum[i] = (double)rope_squares(f0, 8) + (double)rope_squares(f1, 8);
-          all += sum[i];
-        }
-        if constexpr (NORM == T2T_NORM_TOKEN) {
-          all = rope_sum(all, 64);
-          if constexpr (WPT > 1) {
-            __syncthreads();  // the last token's sums are read
-            if (lane == 0) part[wave] = all;
-            __syncthreads();
-            all = part[0] + part[1] + part[2] + part[3];
-          }
-          const float v = rope_inv(all, one_over_n, A.eps);
+        for (int e = 0; e < V; ++e) f0[e] *= inv[i] * w0[e], f1[e] *= inv[i] * w1[e];
+      }
+      if (pair) {
 #pragma unroll
-          for (int i = 0; i < ITS; ++i) inv[i] = v;
-        } else {
+        for (int e = 0; e < V; ++e) rope_turn(f0[e], f1[e], cs[e], sn[e], y0[e], y1[e]);
+      } else {
 #pragma unroll
-          for (int i = 0; i < ITS; ++i) inv[i] = rope_inv(rope_sum(sum[i], L), one_over_n, A.eps);
+        for (int e = 0; e < V / 2; ++e) {
+          y0[2 * e] = f0[2 * e], y0[2 * e + 1] = f0[2 * e + 1];
+          y1[2 * e] = f1[2 * e], y1[2 * e + 1] = f1[2 * e + 1];
+          if (turn0) rope_turn(f0[2 * e], f0[2 * e + 1], cs[e], sn[e], y0[2 * e], y0[2 * e + 1]);
+          if (turn1)
+            rope_turn(f1[2 * e], f1[2 * e + 1], cs[V / 2 + e], sn[V / 2 + e], y1[2 * e], y1[2 * e + 1]);
         }
       }
-#pragma unroll
-      for (int i = 0; i < ITS; ++i) {
-        const int h = h0 + i * hstep;
-        // the packed values are kept, not their fp32 forms from the sum or the last token
-        asm volatile("" : "+v"(r[i][0]), "+v"(r[i][1]));
-        if constexpr (NORM != T2T_NORM_NONE) {
-          constexpr int last = NORM == T2T_NORM_TOKEN ? ITS - 1 : 0;
-          asm volatile("" : "+v"(wr[i < last ? i : last][0]), "+v"(wr[i < last ? i : last][1]));
-        }
-        float f0[8], f1[8], y0[8], y1[8];
-        rope_unpack<T>(r[i][0], f0);
-        rope_unpack<T>(r[i][1], f1);
-        if constexpr (NORM != T2T_NORM_NONE) {
-          float w0[8], w1[8];
-          const int wi = NORM == T2T_NORM_TOKEN ? i : 0;
-          rope_unpack<T>(wr[wi][0], w0);
-          rope_unpack<T>(wr[wi][1], w1);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) f0[e] *= inv[i] * w0[e], f1[e] *= inv[i] * w1[e];
-        }
-        if (pair) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) rope_turn(f0[e], f1[e], cs[e], sn[e], y0[e], y1[e]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            y0[2 * e] = f0[2 * e], y0[2 * e + 1] = f0[2 * e + 1];
-            y1[2 * e] = f1[2 * e], y1[2 * e + 1] = f1[2 * e + 1];
-            if (turn0) rope_turn(f0[2 * e], f0[2 * e + 1], cs[e], sn[e], y0[2 * e], y0[2 * e + 1]);
-            if (turn1) rope_turn(f1[2 * e], f1[2 * e + 1], cs[4 + e], sn[4 + e], y1[2 * e], y1[2 * e + 1]);
-          }
-        }
-        if (on0 && h < H) *(u32x4*)(o + h * g.out_head + c0) = rope_pack<T>(y0);
-        if (on1 && h < H) *(u32x4*)(o + h * g.out_head + c1) = rope_pack<T>(y1);
-      }
+      if (on0 && h < H && live) *(vec*)(o + h * g.out_head + c0) = rope_pack<T, V>(y0);
+      if (on1 && h < H && live) *(vec*)(o + h * g.out_head + c1) = rope_pack<T, V>(y1);
     }
   }
 }
@@ -309,11 +332,10 @@ __global__ __launch_bounds__(256) void rotary_kernel(t2t_rotary_tensor q, t2t_ro
 template <typename T>
 __device__ inline double rope_head_squares(const uint16_t* x, int D, int lane) {
   double sum = 0.0;
-  for (int c = 8 * lane; c < D; c += 512) {
-    const int n = min(8, D - c);
-    float f[8];
-    for (int e = 0; e < 8; ++e) f[e] = e < n ? T::to_f(x[c + e]) : 0.f;
-    sum += (double)rope_squares(f, n);
+  for (int c = 4 * lane; c < D; c += 256) {
+    float f[4];
+    for (int e = 0; e < 4; ++e) f[e] = c + e < D ? T::to_f(x[c + e]) : 0.f;
+    sum += rope_squares(f[0], f[1], f[2], f[3]);
   }
   return sum;
 }
@@ -375,63 +397,86 @@ __global__ __launch_bounds__(256) void rotary_any_kernel(t2t_rotary_tensor q, t2
   }
 }
 
-// 16-byte vectors: all strides, widths and pointers allow them
-static bool rope_vectors(const t2t_rotary_tensor& t, bool weight) {
-  return ((t.x_batch | t.x_row | t.x_head | t.out_batch | t.out_row | t.out_head) & 7) == 0 &&
-         (((uintptr_t)t.x | (uintptr_t)t.out | (weight ? (uintptr_t)t.weight : 0)) & 15) == 0;
+// vectors of V channels: widths, strides and pointers allow them
+static bool rope_vectors(const t2t_rotary_tensor& t, bool weight, int V) {
+  return ((t.x_batch | t.x_row | t.x_head | t.out_batch | t.out_row | t.out_head) & (V - 1)) == 0 &&
+         (((uintptr_t)t.x | (uintptr_t)t.out | (weight ? (uintptr_t)t.weight : 0)) & (2 * V - 1)) == 0;
 }
 
-template <typename T, int NORM, int WPT, int ITS>
+template <typename T, int NORM, int WPT, int ITS, int V>
 static void rope_launch(const t2t_rotary_tensor& q, const t2t_rotary_tensor& k, const RotaryArgs& A, int tensors,
                         hipStream_t st) {
-  const long long wgs = (A.tokens + 4 / WPT - 1) / (4 / WPT);
+  long long items = 0;
+  for (int i = 0; i < tensors; ++i) {
+    const int span = A.shift + A.hshift[i];
+    const long long n = ((A.tokens + (64 >> span) - 1) >> (6 - span)) * A.chunks[i];
+    items = n > items ? n : items;
+  }
+  const long long wgs = (items + 4 / WPT - 1) / (4 / WPT);
   // a few rounds of work-groups, so that the weights are read once for several tokens
-  hipLaunchKernelGGL((rotary_kernel<T, NORM, WPT, ITS>), dim3((unsigned)(wgs < 4096 ? wgs : 4096), tensors),
+  hipLaunchKernelGGL((rotary_kernel<T, NORM, WPT, ITS, V>), dim3((unsigned)(wgs < 4096 ? wgs : 4096), tensors),
                      dim3(256), 0, st, q, k, A);
 }
 
-template <typename T, int NORM, int WPT>
-static bool rope_rounds(const t2t_rotary_tensor& q, const t2t_rotary_tensor& k, const RotaryArgs& A, int tensors,
-                        int its, hipStream_t st) {
-  switch (its) {
-    case 1: rope_launch<T, NORM, WPT, 1>(q, k, A, tensors, st); return true;
-    case 2: rope_launch<T, NORM, WPT, 2>(q, k, A, tensors, st); return true;
-    case 3: rope_launch<T, NORM, WPT, 3>(q, k, A, tensors, st); return true;
-    case 4: rope_launch<T, NORM, WPT, 4>(q, k, A, tensors, st); return true;
-    case 5: rope_launch<T, NORM, WPT, 5>(q, k, A, tensors, st); return true;
-    case 6: rope_launch<T, NORM, WPT, 6>(q, k, A, tensors, st); return true;
-    case 7: rope_launch<T, NORM, WPT, 7>(q, k, A, tensors, st); return true;
-    case 8: rope_launch<T, NORM, WPT, 8>(q, k, A, tensors, st); return true;
+// the vector kernel, if it takes the call
+template <typename T, int V>
+static bool rope_vector_run(const t2t_rotary_tensor& q, const t2t_rotary_tensor& k, RotaryArgs A, int norm,
+                            int tensors, hipStream_t st) {
+  if (A.D % V || A.R % (A.half ? 2 * V : V) || !rope_vectors(q, norm, V) ||
+      (tensors == 2 && !rope_vectors(k, norm, V)) || (((uintptr_t)A.cosv | (uintptr_t)A.sinv) & (2 * V - 1)))
+    return false;
+  A.units = A.half ? A.R / (2 * V) + (A.D - A.R + 2 * V - 1) / (2 * V) : (A.D + 2 * V - 1) / (2 * V);
+  for (A.shift = 0; (1 << A.shift) < A.units;) ++A.shift;
+  if (A.shift > 6) return false;
+  int its = 1;  // rounds of a token's heads
+  const int heads[2] = {q.heads, k.heads};
+  for (int i = 0; i < tensors; ++i) {
+    for (A.hshift[i] = 0; A.hshift[i] < 6 - A.shift && (1 << A.hshift[i]) < heads[i];) ++A.hshift[i];
+    its = max(its, cdiv(heads[i], 1 << A.hshift[i]));
+    A.chunks[i] = 1;
   }
-  return false;
+  if (norm == T2T_NORM_TOKEN) {
+    // a whole work-group takes a token where the tokens are few (latency) or its heads too many for
+    // a wave's registers (3000 tokens of 32 + 8 heads x 256: eight rounds in a wave 43 us, two in four
+    // waves 28)
+    if (A.tokens >= 1024 && its <= 5) {
+      switch (its) {
+        case 1: rope_launch<T, T2T_NORM_TOKEN, 1, 1, V>(q, k, A, tensors, st); return true;
+        case 2: rope_launch<T, T2T_NORM_TOKEN, 1, 2, V>(q, k, A, tensors, st); return true;
+        case 3: rope_launch<T, T2T_NORM_TOKEN, 1, 3, V>(q, k, A, tensors, st); return true;
+        case 4: rope_launch<T, T2T_NORM_TOKEN, 1, 4, V>(q, k, A, tensors, st); return true;
+        default: rope_launch<T, T2T_NORM_TOKEN, 1, 5, V>(q, k, A, tensors, st); return true;
+      }
+    }
+    A.hshift[0] = A.hshift[1] = 6 - A.shift;
+    its = cdiv(max(heads[0], tensors == 2 ? heads[1] : 0), 4 << (6 - A.shift));
+    if (its <= 1) rope_launch<T, T2T_NORM_TOKEN, 4, 1, V>(q, k, A, tensors, st);
+    else if (its <= 2) rope_launch<T, T2T_NORM_TOKEN, 4, 2, V>(q, k, A, tensors, st);
+    else if (its <= 4) rope_launch<T, T2T_NORM_TOKEN, 4, 4, V>(q, k, A, tensors, st);
+    else if (its <= 8) rope_launch<T, T2T_NORM_TOKEN, 4, 8, V>(q, k, A, tensors, st);
+    return its <= 8;
+  }
+  // heads on their own: up to four rounds an item (table entries serve them all), one where the items
+  // would be few
+  const int r = its >= 4 ? 4 : its >= 2 ? 2 : 1, rounds = A.tokens * cdiv(its, r) < 8192 ? 1 : r;
+  for (int i = 0; i < tensors; ++i) A.chunks[i] = cdiv(heads[i], rounds << A.hshift[i]);
+  if (norm == T2T_NORM_HEAD) {
+    if (rounds == 4) rope_launch<T, T2T_NORM_HEAD, 1, 4, V>(q, k, A, tensors, st);
+    else if (rounds == 2) rope_launch<T, T2T_NORM_HEAD, 1, 2, V>(q, k, A, tensors, st);
+    else rope_launch<T, T2T_NORM_HEAD, 1, 1, V>(q, k, A, tensors, st);
+  } else {
+    if (rounds == 4) rope_launch<T, T2T_NORM_NONE, 1, 4, V>(q, k, A, tensors, st);
+    else if (rounds == 2) rope_launch<T, T2T_NORM_NONE, 1, 2, V>(q, k, A, tensors, st);
+    else rope_launch<T, T2T_NORM_NONE, 1, 1, V>(q, k, A, tensors, st);
+  }
+  return true;
 }
 
 template <typename T>
-static void rope_run(const t2t_rotary_tensor& q, const t2t_rotary_tensor& k, RotaryArgs A, int norm, int tensors,
-                     hipStream_t st) {
-  const int H = tensors == 2 && k.heads > q.heads ? k.heads : q.heads;
-  bool vec = A.D % 8 == 0 && A.R % (A.half ? 16 : 8) == 0 && rope_vectors(q, norm) &&
-             (tensors == 1 || rope_vectors(k, norm)) && (((uintptr_t)A.cosv | (uintptr_t)A.sinv) & 15) == 0;
-  A.units = A.half ? A.R / 16 + (A.D - A.R + 15) / 16 : (A.D + 15) / 16;
-  for (A.shift = 0; (1 << A.shift) < A.units;) ++A.shift;
-  const int per = 64 >> A.shift;  // heads a wave holds at once
-  // a whole work-group takes a token where the tokens are few (latency) or a wave's registers
-  // cannot hold the heads that one norm spans
-  const bool wide = A.tokens < 1024 || (norm == T2T_NORM_TOKEN && H > 8 * per);
-  int its = cdiv(H, wide ? 4 * per : per);
-  if (norm != T2T_NORM_TOKEN) its = cdiv(its, cdiv(its, 8));
-  if (vec && its <= 8) {
-    if (norm == T2T_NORM_TOKEN)
-      wide ? rope_rounds<T, T2T_NORM_TOKEN, 4>(q, k, A, tensors, its, st)
-           : rope_rounds<T, T2T_NORM_TOKEN, 1>(q, k, A, tensors, its, st);
-    else if (norm == T2T_NORM_HEAD)
-      wide ? rope_rounds<T, T2T_NORM_HEAD, 4>(q, k, A, tensors, its, st)
-           : rope_rounds<T, T2T_NORM_HEAD, 1>(q, k, A, tensors, its, st);
-    else
-      wide ? rope_rounds<T, T2T_NORM_NONE, 4>(q, k, A, tensors, its, st)
-           : rope_rounds<T, T2T_NORM_NONE, 1>(q, k, A, tensors, its, st);
+static void rope_run(const t2t_rotary_tensor& q, const t2t_rotary_tensor& k, const RotaryArgs& A, int norm,
+                     int tensors, hipStream_t st) {
+  if (rope_vector_run<T, 8>(q, k, A, norm, tensors, st) || rope_vector_run<T, 4>(q, k, A, norm, tensors, st))
     return;
-  }
   hipLaunchKernelGGL(rotary_any_kernel<T>, dim3((unsigned)(A.tokens < 65536 ? A.tokens : 65536), tensors),
                      dim3(256), 0, st, q, k, A, norm);
 }
