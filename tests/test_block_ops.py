@@ -1,8 +1,11 @@
 """Rotary positions and MXFP4 linear layers: every operator against plain
 64-bit forms of its definition, at the sizes, layouts and values where it can
 go wrong, and what the entry points refuse."""
+import copy
 import ctypes
+import io
 import math
+import pickle
 
 import pytest
 import torch
@@ -181,6 +184,81 @@ def test_calls_run_under_their_tensors_device(monkeypatch):
     assert seen == [(1, (5, 101)), (0, (6, 100))] and now == [0]
     with pytest.raises(ValueError, match="stream"):
         ops._on(type("S", (), {"device": torch.device("cuda", 1)})(), torch.device("cuda", 0))
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """CPU tensors in the place of GPU ones; the launches, which are not made:
+    (entry point, tensors recorded on the stream, arguments)."""
+    seen = []
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True, raising=False)
+    monkeypatch.setattr(ops, "_launch", lambda name, dev, stream, tensors, *a: seen.append((name, tensors, a)))
+    return seen
+
+
+def _mx_cpu(rows, cols, fill=0):
+    n = -(-rows // 32) * -(-cols // 256) * 256
+    return ops.MxFp4(torch.full((16 * n,), fill, dtype=torch.uint8), torch.full((n,), fill, dtype=torch.uint8),
+                     rows, cols)
+
+
+def _saved(x):
+    f = io.BytesIO()
+    torch.save(x, f)
+    f.seek(0)
+    return torch.load(f, weights_only=False)
+
+
+COPIES = {"copy": copy.copy, "deepcopy": copy.deepcopy, "pickle": lambda x: pickle.loads(pickle.dumps(x)),
+          "save": _saved}
+
+
+@pytest.mark.parametrize("how", COPIES)
+def test_a_copied_matrix_is_read_at_its_own_address(launches, how):
+    W = _mx_cpu(40, 64, 3)
+    c = COPIES[how](W)
+    assert c.shape == (40, 64) and torch.equal(c.codes, W.codes) and torch.equal(c.scales, W.scales)
+    assert (c.codes.data_ptr() == W.codes.data_ptr()) == (how == "copy")
+    x = torch.zeros(40, 64, dtype=torch.bfloat16)
+    ops.mxfp4_dequantize(c)
+    ops.mxfp4_quantize(x, out=c)
+    ops.mxfp4_linear(x, c)
+    ops.mxfp4_linear(c, c)
+    mine = [c.codes.data_ptr(), c.scales.data_ptr()]
+    at = {"t2t_mxfp4_dequantize": [0], "t2t_mxfp4_quantize": [3], "t2t_mxfp4_linear": [3],
+          "t2t_mxfp4_product": [0, 2]}
+    assert [name for name, _, _ in launches] == list(at)
+    for name, _, args in launches:
+        for i in at[name]:
+            assert list(args[i:i + 2]) == mine, name
+
+
+def test_a_matrix_off_the_gpu_is_refused(monkeypatch):
+    """A matrix saved on a GPU and loaded to the host goes to no kernel."""
+    with monkeypatch.context() as m:
+        m.setattr(torch.Tensor, "is_cuda", True, raising=False)
+        W = _mx_cpu(40, 64)
+    monkeypatch.setattr(ops, "_launch", lambda *a: pytest.fail("launched"))
+    x = torch.zeros(40, 64, dtype=torch.bfloat16)
+    for f in (lambda: ops.mxfp4_dequantize(W), lambda: ops.mxfp4_linear(x, W), lambda: ops.mxfp4_linear(W, W),
+              lambda: ops.mxfp4_quantize(x, out=W)):
+        with pytest.raises(ValueError, match="t2t"):
+            f()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("how", COPIES)
+def test_a_copied_matrix_outlives_its_source(dev, how):
+    g, dt = _gen(dev, 4), torch.bfloat16
+    x = _randn(g, 50, 96).to(dt)
+    W = ops.mxfp4_quantize(_randn(g, 70, 96).to(dt))
+    want = ops.mxfp4_linear(x, W), ops.mxfp4_dequantize(W)
+    c = COPIES[how](W)
+    if how != "copy":
+        W.codes.fill_(0)
+        W.scales.fill_(255)
+    assert c.device == dev and torch.equal(ops.mxfp4_linear(x, c), want[0])
+    assert torch.equal(ops.mxfp4_dequantize(c), want[1])
 
 
 # ---------------------------------------------------------------------------

@@ -964,7 +964,8 @@ class MxFp4:
     operands (include/t2t_hip.h).  ``codes`` and ``scales`` are the uint8
     buffers on the GPU; they are checked here, once."""
 
-    __slots__ = ("_codes", "_scales", "_rows", "_cols", "_device", "_ptrs")
+    # (addresses and device are the buffers' at each call: a copied, pickled or loaded matrix has others)
+    __slots__ = ("_codes", "_scales", "_rows", "_cols")
 
     def __init__(self, codes, scales, rows, cols):
         rows, cols = int(rows), int(cols)
@@ -975,22 +976,24 @@ class MxFp4:
             _check(t, (n,), torch.uint8, name, dev)
             if n and t.data_ptr() % 16:
                 raise ValueError(f"t2t: {name} must be 16-byte aligned")
-        self._set(codes, scales, rows, cols, dev)
+        self._set(codes, scales, rows, cols)
 
-    def _set(self, codes, scales, rows, cols, dev):
+    def _set(self, codes, scales, rows, cols):
         self._codes, self._scales, self._rows, self._cols = codes, scales, rows, cols
-        self._device, self._ptrs = dev, (codes.data_ptr(), scales.data_ptr())
         return self
+
+    def _ptrs(self):
+        return self._codes.data_ptr(), self._scales.data_ptr()
 
     codes = property(lambda self: self._codes)
     scales = property(lambda self: self._scales)
     rows = property(lambda self: self._rows)
     cols = property(lambda self: self._cols)
     shape = property(lambda self: (self._rows, self._cols))
-    device = property(lambda self: self._device)
+    device = property(lambda self: self._codes.device)
 
     def __repr__(self):
-        return f"MxFp4({self._rows} x {self._cols}, {self._device})"
+        return f"MxFp4({self._rows} x {self._cols}, {self.device})"
 
 
 def _mx_rows(t, name, dev, align):
@@ -1030,11 +1033,11 @@ def mxfp4_quantize(x, out=None, stream=None):
             raise ValueError(f"t2t: x must have columns in multiples of 32, got {M} x {K}")
         nc, ns = _mx_bytes(M, K)
         out = MxFp4.__new__(MxFp4)._set(_empty(stream, (nc,), torch.uint8, dev),
-                                        _empty(stream, (ns,), torch.uint8, dev), M, K, dev)
-    elif not isinstance(out, MxFp4) or out.shape != (M, K) or out.device != dev:
+                                        _empty(stream, (ns,), torch.uint8, dev), M, K)
+    elif not isinstance(out, MxFp4) or out.shape != (M, K) or _dev(out._codes) != dev:
         raise ValueError(f"t2t: out must be an MxFp4 matrix {M} x {K} on {dev}, got {out!r}")
     _launch("t2t_mxfp4_quantize", dev, stream, (x, out._codes, out._scales), x.data_ptr(),
-            dtype_code(x.dtype), stride, *out._ptrs, M, K)
+            dtype_code(x.dtype), stride, *out._ptrs(), M, K)
     return out
 
 
@@ -1043,7 +1046,7 @@ def mxfp4_dequantize(t, dtype=torch.bfloat16, out=None, stream=None):
     type that was quantised, and in bf16 always."""
     if not isinstance(t, MxFp4):
         raise ValueError("t2t: expected an MxFp4 matrix")
-    dev = t._device
+    dev = _dev(t._codes)
     _on(stream, dev)
     code = dtype_code(dtype)
     if out is None:
@@ -1053,7 +1056,7 @@ def mxfp4_dequantize(t, dtype=torch.bfloat16, out=None, stream=None):
         M, K, stride = _mx_rows(out, "out", dev, 16)
         if (M, K) != t.shape or out.dtype != dtype:
             raise ValueError(f"t2t: out must be {dtype} {t.shape}, got {out.dtype} {tuple(out.shape)}")
-    _launch("t2t_mxfp4_dequantize", dev, stream, (t._codes, t._scales, out), *t._ptrs, out.data_ptr(), code,
+    _launch("t2t_mxfp4_dequantize", dev, stream, (t._codes, t._scales, out), *t._ptrs(), out.data_ptr(), code,
             stride, *t.shape)
     return out
 
@@ -1076,11 +1079,11 @@ def mxfp4_linear(x, weight, bias=None, *, activation=None, dtype=None, out=None,
     ``out``: contiguous rows, no memory shared with x."""
     if not isinstance(weight, MxFp4):
         raise ValueError("t2t: weight must be an MxFp4 matrix (mxfp4_quantize)")
-    dev = weight._device
+    dev = _dev(weight._codes)
     _on(stream, dev)
     N = weight._rows
     if isinstance(x, MxFp4):
-        if x._device != dev:
+        if x.device != dev:
             raise ValueError(f"t2t: x must be on {dev}")
         M, K = x.shape
         shape = (M, N)
@@ -1104,11 +1107,11 @@ def mxfp4_linear(x, weight, bias=None, *, activation=None, dtype=None, out=None,
         ostride = _mx_rows(out, "out", dev, 2)[2]
         if tuple(out.shape) != shape or out.dtype != dt:
             raise ValueError(f"t2t: out must be {dt} {shape}, got {out.dtype} {tuple(out.shape)}")
-    args = (*weight._ptrs, None if bias is None else bias.data_ptr(), _ACTIVATIONS[activation],
+    args = (*weight._ptrs(), None if bias is None else bias.data_ptr(), _ACTIVATIONS[activation],
             out.data_ptr())
     if isinstance(x, MxFp4):
         _launch("t2t_mxfp4_product", dev, stream,
-                (x._codes, x._scales, weight._codes, weight._scales, bias, out), *x._ptrs, *args, code,
+                (x._codes, x._scales, weight._codes, weight._scales, bias, out), *x._ptrs(), *args, code,
                 ostride, M, N, K)
     else:
         need = mxfp4_linear_ws_bytes(M, N, K)
