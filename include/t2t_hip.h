@@ -437,7 +437,8 @@ int t2t_fit_chol(const double* Mq, const double* Mk, double* L, int32_t* small, 
  * fp32, pairs = the sum of axis_pairs): positions [T, axes] int32 or int64
  * (pos_bits), 1 <= axes <= 4; axis a has axis_pairs[a] pairs (1 .. 4096; host
  * memory), one after the other.  freqs [pairs] fp64.  Angles, sines and
- * cosines are taken in fp64.  Product magnitudes up to 2^31. */
+ * cosines are taken in fp64.  Products below 2^51 in magnitude; from there on
+ * both entries are NaN. */
 int t2t_rotary_table(const void* positions, int pos_bits, long long T, int axes,
                      const int* axis_pairs, const double* freqs, double factor, float* cosv,
                      float* sinv, void* stream);

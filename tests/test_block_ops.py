@@ -287,6 +287,26 @@ def test_rotary_table(dev, pdt, T, dims, scaling, last):
         assert bool(((got.double() - ref).abs() <= ref.abs() * 2.0 ** -24 + 2e-15).all())
 
 
+@pytest.mark.gpu
+def test_rotary_table_of_far_positions(dev):
+    """Angles beyond 2^31: the host's sine and cosine of the same 64-bit angle;
+    beyond 2^51 (half a radian between neighbours) NaN, not some number."""
+    fr = ops.rotary_frequencies(64, device=dev)
+    pos = [2 ** 31 - 1, 2 ** 31 + 1, 3 * 2 ** 31 + 5, 2 ** 32 + 12345, 5 * 2 ** 32 + 7, 2 ** 40 + 1, -(2 ** 33) - 1,
+           -(2 ** 45) - 3, 2 ** 51 - 1, 2 ** 51, -(2 ** 51), 2 ** 53 + 2, 2 ** 62, -(2 ** 63)]
+    cos, sin = (t.double().cpu() for t in ops.rotary_table(torch.tensor(pos, device=dev), fr))
+    for i, p in enumerate(pos):
+        for j, f in enumerate(fr.freqs.tolist()):
+            a = float(p) * f
+            if abs(a) >= 2.0 ** 51:
+                assert math.isnan(cos[i, j]) and math.isnan(sin[i, j]), (p, j)
+                continue
+            # one rounding to fp32; the reduction's remainder is off by 2^-53, the series by less than
+            # 1.2^16 / 16! = 9e-13 (the quotient x 2 / pi is off by up to 0.2, so |r| <= 1.2)
+            for got, ref in ((cos[i, j], math.cos(a)), (sin[i, j], math.sin(a))):
+                assert abs(float(got) - ref) <= abs(ref) * 2.0 ** -24 + 2e-12, (p, j)
+
+
 # ---------------------------------------------------------------------------
 # rotation and norm
 # ---------------------------------------------------------------------------

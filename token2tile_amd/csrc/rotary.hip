@@ -17,7 +17,7 @@ struct TableAxes {
 };
 
 // m sin x and m cos x by the Taylor series on [-pi/4, pi/4], to below 1e-15 (r^15, r^14), after taking
-// the nearest multiple of pi/2 off in two parts; |x| < 2^31.  The coefficients are kept in scalar
+// the nearest multiple of pi/2 off in two parts; |x| < 2^51.  The coefficients are kept in scalar
 // registers (left to itself the compiler moves each into vector registers at every use).
 struct TableCoef {
   double s[7], c[6];
@@ -43,8 +43,9 @@ __device__ inline void table_sincos(const TableCoef& k_, double x, double m, flo
   for (int i = 1; i < 6; ++i) v = __builtin_fma(v, t, k_.c[i]);
   u = __builtin_fma(u * t, r, r);
   v = __builtin_fma(__builtin_fma(v, t, -0.5), t, 1.0);
-  // which is which, and the signs, after the rounding to fp32
-  const uint32_t q = (uint32_t)(int)k;
+  // which is which, and the signs, after the rounding to fp32; k modulo 2^32 stands in the low bits of
+  // k + 1.5 2^52 (a conversion to an integer ends at 2^31)
+  const uint32_t q = (uint32_t)__builtin_bit_cast(uint64_t, k + 0x1.8p52);
   const uint32_t fu = __builtin_bit_cast(uint32_t, (float)(m * u)), fv = __builtin_bit_cast(uint32_t, (float)(m * v));
   s = __builtin_bit_cast(float, (q & 1 ? fv : fu) ^ ((q & 2) << 30));
   c = __builtin_bit_cast(float, (q & 1 ? fu : fv) ^ (((q + 1) & 2) << 30));
@@ -70,12 +71,25 @@ __global__ __launch_bounds__(256) void rotary_table_kernel(const P* __restrict__
       P at[4];  // four positions' loads under way at once
 #pragma unroll
       for (int i = 0; i < 4; ++i) at[i] = pos[min(t0 + i * step, T - 1) * ax.n + a];
+      // neighbouring fp64 angles are half a radian apart from 2^51 on: these entries are NaN (a choice
+      // at every entry instead of the rare second store takes 15.4 for 14.9 us)
+      bool far = false;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const long long t = t0 + i * step;
+        const double x = (double)at[i] * f;
+        far |= !(__builtin_fabs(x) < 0x1p51);
         float s, c;
-        table_sincos(coef, (double)at[i] * f, m, s, c);
+        table_sincos(coef, x, m, s, c);
         if (t < T) cosv[t * pairs + p] = c, sinv[t * pairs + p] = s;
+      }
+      if (far) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const long long t = t0 + i * step;
+          if (t < T && !(__builtin_fabs((double)at[i] * f) < 0x1p51))
+            cosv[t * pairs + p] = sinv[t * pairs + p] = __builtin_nanf("");
+        }
       }
     }
   }

@@ -844,7 +844,8 @@ def rotary_frequencies(dims, *, base=10000.0, scaling=None, device):
 def rotary_table(positions, frequencies, out=None, stream=None):
     """(cos, sin) of ``positions`` (int32 or int64, [...] for one axis, [...,
     axes] for several) times the frequencies: fp32 [..., pairs] each.  Angles
-    are taken in 64 bits; |position * frequency| stays below 2^31."""
+    are taken in 64 bits; from |position * frequency| = 2^51 on, where they
+    are too coarse, the entries are NaN."""
     freqs, pairs, factor = frequencies
     dev = _dev(positions)
     _on(stream, dev)
