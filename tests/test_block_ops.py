@@ -246,6 +246,21 @@ def test_a_matrix_off_the_gpu_is_refused(monkeypatch):
             f()
 
 
+@pytest.mark.parametrize("M", [4, 400])
+def test_every_tensor_of_a_call_is_recorded_on_its_stream(launches, M):
+    """A caller's workspace too: it may be freed while the stream still writes it."""
+    K, N = 64, 40
+    dt = torch.bfloat16
+    W, x, b, out = _mx_cpu(N, K), torch.zeros(M, K, dtype=dt), torch.zeros(N, dtype=dt), torch.zeros(M, N, dtype=dt)
+    ws = torch.empty(max(ops.mxfp4_linear_ws_bytes(M, N, K), 256), dtype=torch.uint8)
+    stream = type("S", (), {"device": x.device})()
+    ops.mxfp4_linear(x, W, b, out=out, ws=ws, stream=stream)
+    (_, tensors, args), = launches
+    assert ws.data_ptr() in args
+    for t in (x, W.codes, W.scales, b, out, ws):
+        assert any(u is t for u in tensors)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("how", COPIES)
 def test_a_copied_matrix_outlives_its_source(dev, how):

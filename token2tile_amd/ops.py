@@ -1120,7 +1120,7 @@ def mxfp4_linear(x, weight, bias=None, *, activation=None, dtype=None, out=None,
             ws = _ws_for(ws, need, dev, stream)
         elif need:
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if stream is None else _ws(need, dev, stream)
-        _launch("t2t_mxfp4_linear", dev, stream, (x, weight._codes, weight._scales, bias, out), x.data_ptr(),
+        _launch("t2t_mxfp4_linear", dev, stream, (x, weight._codes, weight._scales, bias, out, ws), x.data_ptr(),
                 code, stride, *args, ostride, M, N, K, None if ws is None else ws.data_ptr(),
                 0 if ws is None else ws.numel())
     return out
