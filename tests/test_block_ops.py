@@ -59,6 +59,32 @@ def test_frequencies_of_every_scaling():
     assert three.freqs[22] == 1.0 and three.freqs[43] == 1.0
 
 
+@pytest.mark.parametrize("d,base,L,fast,slow", [
+    (64, 10000.0, 4096, 32.0, 1.0), (128, 10000.0, 32768, 32.0, 1.0), (96, 500000.0, 8192, 16.0, 2.0),
+    (2, 10000.0, 4096, 32.0, 1.0), (42, 10000.0, 81, 32.0, 1.0), (8, 10000.0, 1, 32.0, 1.0),
+    (64, 10000.0, 2, 32.0, 1.0), (64, 10000.0, 7, 32.0, 1.0), (16, 100.0, 5_000_000, 32.0, 1.0),
+    (16, 100.0, 100_000, 32.0, 1.0), (44, 10000.0, 21, 4.0, 3.9)])
+def test_yarn_ramp(d, base, L, fast, slow):
+    """The ramp's borders are found by counting turns, pair by pair, not from
+    logarithms; a context so short (long) that every pair turns fewer (more)
+    times than both borders is stretched (kept) throughout."""
+    s = 8.0
+    turns = lambda j: L * base ** (-2.0 * j / d) / (2.0 * math.pi)  # noqa: E731
+    lo = max(j for j in range(-4 * d, 4 * d) if turns(j) >= fast)
+    hi = min(j for j in range(-4 * d, 4 * d) if turns(j) <= slow)
+    got = ops.rotary_frequencies(d, base=base, scaling=ops.RotaryScaling("yarn", s, L, fast, slow), device="cpu")
+    for i, f in enumerate(got.freqs.tolist()):
+        plain = base ** (-2.0 * i / d)
+        if hi < 0:
+            r = 1.0
+        elif lo > d - 1:
+            r = 0.0
+        else:
+            a, b = max(lo, 0), min(hi, d - 1)
+            r = min(max((i - a) / (b - a), 0.0), 1.0) if b > a else float(i > a)
+        assert abs(f - (plain * (1 - r) + plain / s * r)) <= 1e-13 * plain, (i, lo, hi)
+
+
 @pytest.mark.parametrize("kw", [
     dict(dims=0), dict(dims=7), dict(dims=()), dict(dims=(2, 2, 2, 2, 2)), dict(dims=64, base=1.0),
     dict(dims=64, base=math.inf), dict(dims=64, scaling=ops.RotaryScaling("other", 2.0)),

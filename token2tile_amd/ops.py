@@ -832,9 +832,13 @@ def rotary_frequencies(dims, *, base=10000.0, scaling=None, device):
             # pair d ln(L / (2 pi t)) / (2 ln base) makes t turns over length L
             lo, hi = (d * math.log(scaling.original / (2.0 * math.pi * t)) / (2.0 * math.log(base))
                       for t in (scaling.beta_fast, scaling.beta_slow))
-            lo, hi = max(math.floor(lo), 0), min(math.ceil(hi), d - 1)
-            width = (hi - lo) or 0.001
-            r = [min(max((i - lo) / width, 0.0), 1.0) for i in range(d // 2)]
+            lo, hi = math.floor(lo), math.ceil(hi)
+            if hi < 0 or lo > d - 1:  # every pair beyond both borders, the slow or the fast one
+                r = [1.0 if hi < 0 else 0.0] * (d // 2)
+            else:
+                lo, hi = max(lo, 0), min(hi, d - 1)
+                width = (hi - lo) or 0.001
+                r = [min(max((i - lo) / width, 0.0), 1.0) for i in range(d // 2)]
             fd = [x * y / scaling.factor + x * (1.0 - y) for x, y in zip(fd, r)]
         f += fd
     return RotaryFrequencies(torch.tensor(f, dtype=torch.float64, device=device),
