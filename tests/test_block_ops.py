@@ -6,6 +6,7 @@ import ctypes
 import io
 import math
 import pickle
+import random
 
 import pytest
 import torch
@@ -285,6 +286,126 @@ def test_every_tensor_of_a_call_is_recorded_on_its_stream(launches, M):
     assert ws.data_ptr() in args
     for t in (x, W.codes, W.scales, b, out, ws):
         assert any(u is t for u in tensors)
+
+
+def _walk(t):
+    """The addresses of a tensor's bytes."""
+    at = torch.zeros((), dtype=torch.int64)
+    for st, sz in zip(t.stride(), t.shape):
+        at = at.unsqueeze(-1) + st * torch.arange(sz)
+    e = t.element_size()
+    return set((t.data_ptr() + at.reshape(-1, 1) * e + torch.arange(e)).flatten().tolist())
+
+
+def test_shared_memory_is_found():
+    """Random views of one buffer: what the search over the strides says is what
+    the lists of addresses say."""
+    r = random.Random(3)
+    buf = torch.zeros(4000, dtype=torch.bfloat16)
+    met = 0
+    for _ in range(600):
+        views = []
+        for _ in range(2):
+            shape = [r.randint(1, 4) for _ in range(r.randint(1, 3))] + [r.randint(1, 6)]
+            stride = [r.choice([0, 1, 3, 7, 8, 24, 25, 48, 96, 200]) for _ in shape[:-1]] + [1]
+            v = buf.as_strided(shape, stride, r.randint(0, 300))
+            views.append(v.view(torch.uint8) if r.random() < 0.2 else v)
+        a, b = views
+        want = bool(_walk(a) & _walk(b))
+        met += want
+        assert ops._meet(a, b) == want, (a.shape, a.stride(), b.shape, b.stride(), b.data_ptr() - a.data_ptr())
+        (lo, hi), at = ops._span(a), _walk(a)
+        assert min(at) == lo and max(at) == hi - 1
+    assert 100 < met < 500
+
+
+@pytest.mark.parametrize("kind", ["own", "fused", "slots", "head_major", "moved", "step", "twice", "rows", "table",
+                                  "weight", "other", "one", "same", "swapped"])
+def test_outputs_of_a_rotation_share_no_memory(launches, kind):
+    dt, N, H, D = torch.bfloat16, 6, 4, 32
+    buf = torch.zeros(8 * N * H * D, dtype=dt)
+    cos = torch.zeros(N, D // 2)
+    q, k = torch.zeros(N, H, D, dtype=dt), torch.zeros(N, H, D, dtype=dt)
+    view = lambda at, sn=H * D, sh=D: buf.as_strided((N, H, D), (sn, sh, 1), at)  # noqa: E731
+    kw, fine = {}, True
+    if kind == "own":                # in place
+        out = (q, k)
+    elif kind == "fused":            # both in place in one projection's rows
+        q, k = view(0, 2 * H * D), view(H * D, 2 * H * D)
+        out = (q, view(H * D, 2 * H * D))
+    elif kind == "slots":            # heads of q and k in turn
+        out = (view(0, 2 * H * D, 2 * D), view(D, 2 * H * D, 2 * D))
+    elif kind == "head_major":
+        out = (view(0, D, 2 * N * D), view(N * D, D, 2 * N * D))
+    else:
+        fine = False
+        if kind == "moved":          # k's rows are q's, one token on
+            out = (view(0), view(H * D))
+        elif kind == "step":         # an output is its input one token on
+            q = view(0)
+            out = (view(H * D), k)
+        elif kind == "twice":        # in place by another stride
+            q = view(0)
+            out = (view(0, 2 * H * D), k)
+        elif kind == "rows":
+            out = (view(0, 2 * H * D), view(H * D - 1, 2 * H * D))
+        elif kind == "table":
+            cos = buf.view(torch.float32)[:N * D // 2].view(N, D // 2)
+            out = (view(0), k)
+        elif kind == "weight":
+            kw = dict(norm="head", q_weight=buf[:D], k_weight=torch.zeros(D, dtype=dt))
+            out = (q, view(0))
+        elif kind == "one":          # q for k as well, one of them in place
+            k = q
+            out = (q, view(0))
+        elif kind == "same":
+            k = q
+            out = (q, q)
+        elif kind == "swapped":
+            out = (k, q)
+        else:                        # the other's input
+            k = view(64)
+            out = (view(0), torch.zeros(N, H, D, dtype=dt))
+    call = lambda: ops.rotary(q, k, cos, torch.zeros(N, D // 2), out=out, **kw)  # noqa: E731
+    if fine:
+        assert call() == out and len(launches) == 1
+    else:
+        with pytest.raises(ValueError, match="shares memory"):
+            call()
+        assert not launches
+
+
+def test_outputs_of_tables_and_linears_share_no_memory(launches):
+    dt, M, K, N = torch.bfloat16, 6, 64, 40
+    fr = ops.rotary_frequencies(32, device="cpu")
+    pos, c = torch.zeros(M, dtype=torch.int64), torch.zeros(2 * M, 16)
+    ops.rotary_table(pos, fr, out=(c[:M], c[M:]))
+    buf = torch.zeros(400 * 128, dtype=dt)
+    W, x, rows = _mx_cpu(N, K), buf[:M * 128].view(M, 128)[:, :K], buf[:M * 128].view(M, 128)
+    ops.mxfp4_linear(x, W, out=rows[:, K:K + N])                 # beside x in its rows
+    raw = torch.zeros(1 << 17, dtype=torch.uint8)
+    n = ops._mx_bytes(N, K)
+    R = ops.MxFp4(raw[:n[0]], raw[n[0]:sum(n)], N, K)
+    X = ops.MxFp4(raw[:n[0]], raw[n[0]:sum(n)], N, K)
+    big = buf[:400 * K].view(400, K)
+    need = ops.mxfp4_linear_ws_bytes(400, N, K)
+    assert 0 < need < 1 << 16
+    ops.mxfp4_linear(big, W, ws=raw[:need])
+    done = len(launches)
+    other = raw[1 << 16:].view(dt)
+    for f in (lambda: ops.rotary_table(pos, fr, out=(c[:M], c[:M])),
+              lambda: ops.rotary_table(pos, fr, out=(c[:M], c[1:M + 1])),
+              lambda: ops.mxfp4_linear(x, W, out=rows[:, K - 1:K - 1 + N]),
+              lambda: ops.mxfp4_linear(X, W, out=raw[:2 * N * N].view(dt).view(N, N)),
+              lambda: ops.mxfp4_linear(other[:M * K].view(M, K), R, out=raw[:2 * M * N].view(dt).view(M, N)),
+              lambda: ops.mxfp4_linear(x, W, other[:N], out=other[:M * N].view(M, N)),
+              lambda: ops.mxfp4_linear(big, W, ws=buf.view(torch.uint8)),
+              lambda: ops.mxfp4_linear(big, W, out=other[:400 * N].view(400, N), ws=raw[(1 << 16):]),
+              lambda: ops.mxfp4_dequantize(X, out=raw[:2 * N * K].view(dt).view(N, K)),
+              lambda: ops.mxfp4_quantize(raw[:2 * N * K].view(dt).view(N, K), out=X)):
+        with pytest.raises(ValueError, match="shares memory"):
+            f()
+    assert len(launches) == done
 
 
 @pytest.mark.gpu

@@ -757,6 +757,11 @@ def _is(t, shape, dtype, dev):
             and t.is_contiguous())
 
 
+def _same_view(a, b):
+    return a is b or (a.data_ptr() == b.data_ptr()
+                      and all(n < 2 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride())))
+
+
 def _scattered(t):
     """Whether a view's elements all have an address of their own."""
     if t.is_contiguous():
@@ -767,6 +772,86 @@ def _scattered(t):
             return False
         last += st * (sz - 1)
     return True
+
+
+def _span(t):
+    """First address and the one behind the last of a tensor's elements."""
+    p = t.data_ptr()
+    if t.is_contiguous():
+        return p, p + t.nbytes
+    if t.numel() == 0:
+        return p, p
+    return p, p + (sum(st * (sz - 1) for st, sz in zip(t.stride(), t.shape)) + 1) * t.element_size()
+
+
+def _in_slots(a, b):
+    """Whether the two lie in parts of their own of slots of one stride (the usual
+    interleaved views, without the search)."""
+    d, ea, eb = b.data_ptr() - a.data_ptr(), a.element_size(), b.element_size()
+    da = [(s * ea, n - 1) for s, n in zip(a.stride(), a.shape) if n > 1]
+    db = [(s * eb, n - 1) for s, n in zip(b.stride(), b.shape) if n > 1]
+    for st, _ in da:
+        if st:
+            at = d % st
+            if (ea + sum(s * n for s, n in da if s % st) <= at
+                    and eb + sum(s * n for s, n in db if s % st) <= st - at):
+                return True
+    return False
+
+
+def _meet(a, b):
+    """Whether two tensors whose spans meet share memory (interleaved views, such
+    as q and k of one projection, do not).  An element of each has the same
+    address where the difference of the bases is a sum of multiples of all
+    strides: the multiples are searched from the largest stride down, within what
+    the smaller ones can make up for."""
+    if _in_slots(a, b):
+        return False
+    mul = {1: [1 - b.element_size(), a.element_size() - 1]}  # stride in bytes: lowest, highest multiple
+    for t, side in ((a, 1), (b, 0)):
+        for st, sz in zip(t.stride(), t.shape):
+            if st and sz > 1:
+                mul.setdefault(st * t.element_size(), [0, 0])[side] += (sz - 1) if side else (1 - sz)
+    strides = sorted(mul, reverse=True)
+    low, high = [0], [0]  # reach of the strides from i on
+    for st in reversed(strides):
+        low.insert(0, low[0] + st * mul[st][0])
+        high.insert(0, high[0] + st * mul[st][1])
+    work = 4096  # (odd combinations of strides are left to the caller)
+
+    def search(d, i):
+        nonlocal work
+        if i == len(strides):
+            return d == 0
+        st = strides[i]
+        for k in range(max(mul[st][0], -((high[i + 1] - d) // st)), min(mul[st][1], (d - low[i + 1]) // st) + 1):
+            work -= 1
+            if work < 0:
+                return False
+            if search(d - k * st, i + 1):
+                return True
+        return False
+
+    return search(b.data_ptr() - a.data_ptr(), 0)
+
+
+def _apart(outs, names, ins):
+    """The outputs share no memory with one another or with the inputs, but that
+    outs[i] may be ins[i]."""
+    at = [(0, 0) if t is None else _span(t) for t in ins]
+    to = [at[i] if o is ins[i] else _span(o) for i, o in enumerate(outs)]
+    for i, (lo, hi) in enumerate(to):
+        o, meets = outs[i], False
+        for j, (a, b) in enumerate(at):
+            if a < hi and lo < b:
+                t = ins[j]
+                if t is o if j == i else j < len(outs) and outs[j] is t:
+                    continue  # in its own input's place; the place of an output, which comes below
+                meets = meets or not (j == i and _same_view(o, t)) and _meet(o, t)
+        for j in range(i):
+            meets = meets or to[j][0] < hi and lo < to[j][1] and _meet(o, outs[j])
+        if meets:
+            raise ValueError(f"t2t: {names[i]} shares memory with another argument of the call")
 
 
 @dataclass(frozen=True)
@@ -870,6 +955,7 @@ def rotary_table(positions, frequencies, out=None, stream=None):
         cos, sin = out
         _check(cos, shape, _f32, "cos", dev)
         _check(sin, shape, _f32, "sin", dev)
+        _apart((cos, sin), ("cos", "sin"), (None, None, positions, freqs))
     _launch("t2t_rotary_table", dev, stream, (positions, freqs, cos, sin), positions.data_ptr(),
             bits, math.prod(lead), len(pairs), (ctypes.c_int * len(pairs))(*pairs), freqs.data_ptr(), factor, cos.data_ptr(), sin.data_ptr())
     return cos, sin
@@ -949,8 +1035,9 @@ def rotary(q, k, cos, sin, *, layout="interleaved", inverse=False, norm=None, q_
     tk = None
     if k is not None:
         ok, tk = _rotary_arg(k, ok, k_weight, norm, "k", dev, stream, B, N, D, q.dtype)
-        if out is not None and B * N and (tq.out == tk.out or tq.out == tk.x or tk.out == tq.x):
-            raise ValueError("t2t: the outputs of q and k must be two, and neither the other's input")
+    if out is not None:
+        _apart((oq,) if k is None else (oq, ok), ("the output of q", "the output of k"),
+               (q, k, cos, sin, q_weight, k_weight))
     _launch("t2t_rotary", dev, stream, (q, k, cos, sin, q_weight, k_weight, oq, ok), tq, tk,
             dtype_code(q.dtype), cos.data_ptr(), sin.data_ptr(), batched, B, N, D, R,
             _ROPE_LAYOUTS[layout], bool(inverse), _ROPE_NORMS[norm], eps)
@@ -1041,6 +1128,8 @@ def mxfp4_quantize(x, out=None, stream=None):
                                         _empty(stream, (ns,), torch.uint8, dev), M, K)
     elif not isinstance(out, MxFp4) or out.shape != (M, K) or _dev(out._codes) != dev:
         raise ValueError(f"t2t: out must be an MxFp4 matrix {M} x {K} on {dev}, got {out!r}")
+    else:
+        _apart((out._codes, out._scales), ("out.codes", "out.scales"), (None, None, x))
     _launch("t2t_mxfp4_quantize", dev, stream, (x, out._codes, out._scales), x.data_ptr(),
             dtype_code(x.dtype), stride, *out._ptrs(), M, K)
     return out
@@ -1061,6 +1150,7 @@ def mxfp4_dequantize(t, dtype=torch.bfloat16, out=None, stream=None):
         M, K, stride = _mx_rows(out, "out", dev, 16)
         if (M, K) != t.shape or out.dtype != dtype:
             raise ValueError(f"t2t: out must be {dtype} {t.shape}, got {out.dtype} {tuple(out.shape)}")
+        _apart((out,), ("out",), (None, t._codes, t._scales))
     _launch("t2t_mxfp4_dequantize", dev, stream, (t._codes, t._scales, out), *t._ptrs(), out.data_ptr(), code,
             stride, *t.shape)
     return out
@@ -1081,7 +1171,7 @@ def mxfp4_linear(x, weight, bias=None, *, activation=None, dtype=None, out=None,
     MxFp4 matrix that several layers share; weight MxFp4 [N, K]; bias [N] in the
     output's type.  fp32 sums, one rounding to x's type (``dtype``, default
     bf16, for an MxFp4 x) -> [..., N].  ``activation``: None or "gelu_tanh".
-    ``out``: contiguous rows, no memory shared with x."""
+    ``out``: contiguous rows; it and ``ws`` share no memory with another argument."""
     if not isinstance(weight, MxFp4):
         raise ValueError("t2t: weight must be an MxFp4 matrix (mxfp4_quantize)")
     dev = _dev(weight._codes)
@@ -1112,6 +1202,8 @@ def mxfp4_linear(x, weight, bias=None, *, activation=None, dtype=None, out=None,
         ostride = _mx_rows(out, "out", dev, 2)[2]
         if tuple(out.shape) != shape or out.dtype != dt:
             raise ValueError(f"t2t: out must be {dt} {shape}, got {out.dtype} {tuple(out.shape)}")
+        _apart((out,), ("out",), (None, *((x._codes, x._scales) if isinstance(x, MxFp4) else (x,)),
+                                  weight._codes, weight._scales, bias))
     args = (*weight._ptrs(), None if bias is None else bias.data_ptr(), _ACTIVATIONS[activation],
             out.data_ptr())
     if isinstance(x, MxFp4):
@@ -1122,6 +1214,8 @@ def mxfp4_linear(x, weight, bias=None, *, activation=None, dtype=None, out=None,
         need = mxfp4_linear_ws_bytes(M, N, K)
         if ws is not None:
             ws = _ws_for(ws, need, dev, stream)
+            if need:
+                _apart((ws[:need],), ("ws",), (None, x, weight._codes, weight._scales, bias, out))
         elif need:
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if stream is None else _ws(need, dev, stream)
         _launch("t2t_mxfp4_linear", dev, stream, (x, weight._codes, weight._scales, bias, out, ws), x.data_ptr(),
