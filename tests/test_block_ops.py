@@ -288,6 +288,15 @@ def test_every_tensor_of_a_call_is_recorded_on_its_stream(launches, M):
         assert any(u is t for u in tensors)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.int8, "bf16"])
+def test_other_output_types_are_refused(launches, dtype):
+    W = _mx_cpu(40, 64)
+    for f in (lambda: ops.mxfp4_dequantize(W, dtype), lambda: ops.mxfp4_linear(W, W, dtype=dtype)):
+        with pytest.raises(ValueError, match="t2t"):
+            f()
+    assert not launches
+
+
 def _walk(t):
     """The addresses of a tensor's bytes."""
     at = torch.zeros((), dtype=torch.int64)

@@ -1112,6 +1112,12 @@ def _mx_rows(t, name, dev, align):
     return rows, cols, stride
 
 
+def _mx_dtype(dtype):
+    if dtype not in _HALF:
+        raise ValueError(f"t2t: the output's type must be torch.float16 or torch.bfloat16, got {dtype}")
+    return dtype_code(dtype)
+
+
 def mxfp4_quantize(x, out=None, stream=None):
     """x [..., K] (fp16 or bf16, contiguous 16-byte aligned rows, K a multiple of
     32) in MXFP4, rows flattened.  A block's scale is 2^(floor(log2 max|x|) - 2)
@@ -1142,7 +1148,7 @@ def mxfp4_dequantize(t, dtype=torch.bfloat16, out=None, stream=None):
         raise ValueError("t2t: expected an MxFp4 matrix")
     dev = _dev(t._codes)
     _on(stream, dev)
-    code = dtype_code(dtype)
+    code = _mx_dtype(dtype)
     if out is None:
         out = _empty(stream, t.shape, dtype, dev)
         stride = t._cols
@@ -1188,7 +1194,7 @@ def mxfp4_linear(x, weight, bias=None, *, activation=None, dtype=None, out=None,
         shape, dt = (*x.shape[:-1], N), x.dtype
         if dtype not in (None, dt):
             raise ValueError(f"t2t: the output of a {dt} input is {dt}, not {dtype}")
-    code = dtype_code(dt)
+    code = _mx_dtype(dt)
     if K != weight._cols or N < 1:
         raise ValueError(f"t2t: x has {K} columns, weight {N} x {weight._cols}")
     if activation not in _ACTIVATIONS:
