@@ -1,6 +1,8 @@
 """The DiT harness with MXFP4 linear layers and the fused norm and rotary
 embedding: the blocks call the operators as documented, the defaults are what
 they were, and the whole stack runs both ways."""
+import copy
+import io
 import math
 
 import pytest
@@ -32,6 +34,54 @@ def test_defaults_are_the_plain_forms():
     q, k, v = blk.qkv(x, rope)
     want = dit.apply_rope(dit.rms_norm(blk.q(x), blk.norm_q, 1e-6).view(1, 24, 2, 128), *rope)
     assert torch.equal(q, want) and torch.equal(v, blk.v(x).view(1, 24, 2, 128)) and k.shape == q.shape
+
+
+def _layer(dev, dtype, bias, seed=0):
+    torch.manual_seed(seed)
+    return dit.MxFp4Linear(torch.nn.Linear(64, 40, bias=bias).to(dev, dtype))
+
+
+@pytest.mark.parametrize("bias", [True, False])
+def test_the_layer_is_a_module(monkeypatch, bias):
+    """Its weight is saved, loaded, copied and moved with it, and its output's
+    type follows the module's (CPU tensors in the place of GPU ones)."""
+    seen = []
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True, raising=False)
+    monkeypatch.setattr(ops, "_launch", lambda name, dev, stream, tensors, *a: seen.append((name, a)))
+    a, b = _layer("cpu", torch.float16, bias), _layer("cpu", torch.float16, bias)
+    a.weight.codes.fill_(3), a.weight.scales.fill_(4)
+    assert {t.data_ptr() for t in a.state_dict().values()} >= {a.weight.codes.data_ptr(), a.weight.scales.data_ptr()}
+    b.load_state_dict(a.state_dict())
+    c = copy.deepcopy(a)
+    for m in (b, c):
+        assert torch.equal(m.weight.codes, a.weight.codes) and torch.equal(m.weight.scales, a.weight.scales)
+        assert m.weight.codes.data_ptr() != a.weight.codes.data_ptr() and m.weight.shape == (40, 64)
+    X = ops.MxFp4(*(torch.zeros(n, dtype=torch.uint8) for n in ops._mx_bytes(6, 64)), 6, 64)
+    assert a(X).dtype == torch.float16 and a.to(torch.bfloat16)(X).dtype == torch.bfloat16
+    assert c(torch.zeros(2, 3, 64, dtype=torch.float16)).shape == (2, 3, 40)
+    assert seen[-1][0] == "t2t_mxfp4_linear" and c.weight.codes.data_ptr() in seen[-1][1]
+    c.to("meta")
+    assert c.weight.codes.device.type == "meta" and c.weight.scales.device.type == "meta"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,bias", [(torch.float16, False), (torch.bfloat16, True)])
+def test_a_saved_and_moved_layer_gives_the_same(dev, dtype, bias):
+    a, b = _layer(dev, dtype, bias), _layer(dev, dtype, bias, seed=1)
+    x = torch.randn(2, 9, 64, generator=torch.Generator(device=dev).manual_seed(1), device=dev).to(dtype)
+    want = a(x)
+    assert a(ops.mxfp4_quantize(x)).dtype == dtype
+    f = io.BytesIO()
+    torch.save(a.state_dict(), f)
+    f.seek(0)
+    b.load_state_dict(torch.load(f, weights_only=True))
+    c = copy.deepcopy(a)
+    a.weight.codes.fill_(0)
+    assert torch.equal(b(x), want) and torch.equal(c(x), want)
+    c.cpu()
+    with pytest.raises(ValueError, match="t2t"):
+        c(x)
+    assert torch.equal(c.to(dev)(x), want)
 
 
 @pytest.mark.gpu

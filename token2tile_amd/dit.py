@@ -87,20 +87,31 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
 
 
 class MxFp4Linear(torch.nn.Module):
-    """A linear layer whose weight is kept in MXFP4; its input is quantised at
-    the call, or comes as an ``ops.MxFp4`` that several layers share (the
-    output's leading dimensions are then flattened)."""
+    """A linear layer whose weight is kept in MXFP4 (its codes and scales are
+    buffers: moved, copied, saved and loaded with the module); its input is
+    quantised at the call, or comes as an ``ops.MxFp4`` that several layers share
+    (the output's leading dimensions are then flattened)."""
 
     def __init__(self, linear: torch.nn.Linear):
         super().__init__()
         from token2tile_amd import ops
-        self.weight = ops.mxfp4_quantize(linear.weight.detach())
+        w = ops.mxfp4_quantize(linear.weight.detach())
+        self.out_features, self.in_features = w.shape
+        self.register_buffer("weight_codes", w.codes)
+        self.register_buffer("weight_scales", w.scales)
+        # of the outputs' type, which the module's conversions change with the bias
+        self.register_buffer("_like", linear.weight.detach().new_empty(0), persistent=False)
         self.bias = linear.bias
+
+    @property
+    def weight(self):
+        from token2tile_amd import ops
+        return ops.MxFp4(self.weight_codes, self.weight_scales, self.out_features, self.in_features)
 
     def forward(self, x, activation=None):
         from token2tile_amd import ops
         return ops.mxfp4_linear(x, self.weight, self.bias, activation=activation,
-                                dtype=None if self.bias is None else self.bias.dtype)
+                                dtype=self._like.dtype if isinstance(x, ops.MxFp4) else None)
 
 
 def _shared(x, layer):
