@@ -979,6 +979,105 @@ def test_mxfp4_refused(dev, bad):
         calls[bad]()
 
 
+# 128 x 128 tiles (32 x 48 blocks; the last group of 256 columns padded in the second), 256 x 256 tiles
+# (17 x 17 of them, the last ones with a single block of rows or one of 96 columns)
+TILES = [(1000, 1536, 512), (1000, 1531, 800), (4100, 4200, 1024), (4100, 4195, 1056)]
+
+
+def _operands(dev, M, N, K, dt, seed):
+    g = _gen(dev, seed)
+    return _randn(g, M, K).to(dt), (_randn(g, N, K) * K ** -0.5).to(dt), _randn(g, N).to(dt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,act", [("bf16", "gelu_tanh"), ("fp16", None)])
+@pytest.mark.parametrize("M,N,K", TILES)
+def test_tiles_into_views(dev, M, N, K, dt, act):
+    """Outputs of any stride and address get the bits of a contiguous one, and
+    nothing around them is written."""
+    dt = HALF[dt]
+    x, w, b = _operands(dev, M, N, K, dt, M + N)
+    W = ops.mxfp4_quantize(w)
+    y = ops.mxfp4_linear(x, W, b, activation=act)
+    _check_linear(y, x, w, b, act)
+    X = ops.mxfp4_quantize(x)
+    # aligned rows, an address off by 8 bytes, an odd stride, an odd stride and address
+    for off, width in ((16, N + 24 - N % 8), (4, N + 24 - N % 8), (8, N + 17 - N % 2), (3, N + 17 - N % 2)):
+        buf = torch.full((M + 2, width), 5.0, device=dev, dtype=dt)
+        out = buf[1:M + 1, off:off + N]
+        for src in (x, X):
+            assert ops.mxfp4_linear(src, W, b, activation=act, dtype=dt, out=out) is out
+            assert torch.equal(out, y), (off, width)
+            out.fill_(5.0)
+            assert bool((buf == 5.0).all()), (off, width)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("col", [40, 168, -1])
+@pytest.mark.parametrize("M,N,K", TILES)
+def test_tiles_of_nonfinite_blocks(dev, M, N, K, col):
+    """In an even stage of 128 columns, an odd one and the last: an inf or NaN
+    turns its row or column of the result to NaN and leaves the rest; a row of
+    zeros gives the bias."""
+    x, w, b = _operands(dev, M, N, K, torch.float16, col + 2)
+    x[0] = 0
+    clean = ops.mxfp4_linear(x, ops.mxfp4_quantize(w), b)
+    assert torch.equal(clean[0], b)
+    bad = torch.zeros(M, N, device=dev, dtype=torch.bool)
+    for r in (7, N // 2, N - 1):
+        w[r, col] = float("inf")
+        bad[:, r] = True
+    for r in (130, M - 1):
+        x[r, col] = float("nan")
+        bad[r] = True
+    y = ops.mxfp4_linear(x, ops.mxfp4_quantize(w), b)
+    assert torch.equal(y.isnan(), bad) and torch.equal(y[~bad], clean[~bad])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N", [(600, 1000), (4100, 4200)])
+def test_tiles_of_long_sums(dev, M, N):
+    """13,824 products of one sign, as in the split form."""
+    K = 13824
+    x = torch.full((M, K), 6.0, device=dev, dtype=torch.bfloat16)
+    w = torch.full((N, K), 0.5, device=dev, dtype=torch.bfloat16)
+    x[1::2] = 1.5
+    y = ops.mxfp4_linear(x, ops.mxfp4_quantize(w))
+    want = (torch.tensor([3.0, 0.75], device=dev) * K).to(torch.bfloat16)
+    assert torch.equal(y, want.repeat(M // 2)[:, None].expand(M, N))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", TILES)
+def test_tiles_on_a_side_stream_and_captured(dev, M, N, K):
+    """Two graphs that share a workspace, replayed in turn with new inputs and
+    eager work on another stream between, against the eager results."""
+    dt = torch.bfloat16
+    x, w, b = _operands(dev, M, N, K, dt, 3)
+    W = [ops.mxfp4_quantize(w), ops.mxfp4_quantize(w.flip(0))]
+    ws = torch.empty(ops.mxfp4_linear_ws_bytes(M, N, K), dtype=torch.uint8, device=dev)
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        for i in range(2):
+            ops.mxfp4_linear(x, W[i], b, ws=ws)
+    torch.cuda.current_stream(dev).wait_stream(side)
+    graphs, outs = [], []
+    for i in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(ops.mxfp4_linear(x, W[i], b, activation="gelu_tanh", ws=ws))
+        graphs.append(gr)
+    for r in range(3):
+        x.copy_(_randn(_gen(dev, r), M, K))
+        side.wait_stream(torch.cuda.current_stream(dev))
+        for i in range(2):
+            graphs[i].replay()
+            want = ops.mxfp4_linear(x, W[i], b, activation="gelu_tanh", stream=side)
+            torch.cuda.synchronize(dev)
+            assert torch.equal(outs[i], want), (r, i)
+
+
 # ---------------------------------------------------------------------------
 # streams, captures and the operators together
 # ---------------------------------------------------------------------------
