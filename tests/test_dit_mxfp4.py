@@ -131,6 +131,80 @@ def test_mxfp4_block_calls(dev):
         assert torch.equal(q, dit.apply_rope(f, *model.rope))
 
 
+LAYERS = ("q", "k", "v", "o", "cq", "ck", "cv", "co", "ffn1", "ffn2")
+
+
+def _check_layer(layer, x, got, gelu=False):
+    """A layer's output against the values of its weight and input in 64 bits."""
+    if not isinstance(x, ops.MxFp4):
+        x = ops.mxfp4_quantize(x)
+    a, w = ops.mxfp4_dequantize(x).double(), ops.mxfp4_dequantize(layer.weight).double()
+    b = layer.bias.double()
+    y, mag = a @ w.t() + b, a.abs() @ w.abs().t() + b.abs()
+    # fp32 sums: chains of at most K / 32 + 64 additions, 2^-23 of the terms' magnitudes each; the
+    # activation (slope up to 1.13) adds 2^-18 of its argument; one rounding to bf16
+    tol = (x.cols / 32 + 64) * 2.0 ** -23 * mag
+    if gelu:
+        u = math.sqrt(2 / math.pi) * (y + 0.044715 * y ** 3)
+        tol, y = 1.13 * tol + 2.0 ** -18 * y.abs(), 0.5 * y * (1 + torch.tanh(u))
+    tol = tol + y.abs() * 2.0 ** -8 * (1 + 2.0 ** -7) + 1e-30
+    assert bool(((got.double().view(y.shape) - y).abs() <= tol).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fused", [False, True])
+def test_every_layer_of_a_quantised_block(dev, fused):
+    """Each linear layer is called once, on what the block's definition makes of
+    the layers before it (bit for bit), gives the product of its own weight, and
+    the block's output is the sum of all three parts."""
+    model = _model(dev, mxfp4=True, fused_rope=fused)
+    blk, cfg = model.blocks[1], model.cfg
+    x, t, ctx = _inputs(dev, cfg)
+    B, N, D = x.shape
+    calls = {n: [] for n in LAYERS}
+    for n in LAYERS:   # (outputs as they were: the fused rotation works in place)
+        getattr(blk, n).register_forward_hook(lambda m, a, y, n=n: calls[n].append((a[0], y.clone())))
+    with torch.no_grad():
+        out = blk(x, t, ctx, model.rope, None)
+        assert all(len(c) == 1 for c in calls.values())
+        src, y = ({n: c[0][i] for n, c in calls.items()} for i in range(2))
+        for n in LAYERS:
+            _check_layer(getattr(blk, n), src[n], y[n], gelu=n == "ffn1")
+
+        def quantised(n, want):
+            q = ops.mxfp4_quantize(want)
+            assert torch.equal(src[n].codes, q.codes) and torch.equal(src[n].scales, q.scales), n
+
+        heads = lambda z: z.reshape(B, -1, cfg.heads, cfg.head_dim)  # noqa: E731
+        attend = lambda q, k, v: torch.nn.functional.scaled_dot_product_attention(  # noqa: E731
+            q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)).transpose(1, 2).reshape(B, N, D)
+        e = (blk.modulation + t[:, None, :]).chunk(6, dim=1)
+        h = torch.nn.functional.layer_norm(x, (D,), eps=cfg.eps) * (1 + e[1]) + e[0]
+        for n in "qkv":
+            quantised(n, h)
+        if fused:
+            q, k = ops.rotary(heads(y["q"]), heads(y["k"]), *model.rope, norm="token", q_weight=blk.norm_q,
+                              k_weight=blk.norm_k, eps=cfg.eps)
+        else:
+            q, k = (dit.apply_rope(heads(dit.rms_norm(z, g, cfg.eps)), *model.rope)
+                    for z, g in ((y["q"], blk.norm_q), (y["k"], blk.norm_k)))
+        assert torch.equal(src["o"], attend(q, k, heads(y["v"])))
+        x1 = x + y["o"] * e[2]
+        assert torch.equal(src["cq"], blk.norm3(x1))
+        for n in ("ck", "cv"):
+            quantised(n, ctx)
+        q, k = (heads(dit.rms_norm(z, g, cfg.eps)) for z, g in ((y["cq"], blk.cnorm_q), (y["ck"], blk.cnorm_k)))
+        assert torch.equal(src["co"], attend(q, k, heads(y["cv"])))
+        x2 = x1 + y["co"]
+        assert torch.equal(src["ffn1"],
+                           torch.nn.functional.layer_norm(x2, (D,), eps=cfg.eps) * (1 + e[4]) + e[3])
+        assert torch.equal(src["ffn2"], y["ffn1"])
+        assert torch.equal(out, x2 + y["ffn2"] * e[5])
+        # every part counts: none is lost in the residual's rounding
+        for part in (y["o"] * e[2], y["co"], y["ffn2"] * e[5]):
+            assert float(part.float().norm()) > 2.0 ** -8 * float(x.float().norm())
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kw", [dict(fused_rope=True), dict(mxfp4=True), dict(mxfp4=True, fused_rope=True)])
 def test_stack_runs(dev, kw):
