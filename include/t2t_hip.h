@@ -502,7 +502,8 @@ int t2t_mxfp4_product(const void* a_codes, const void* a_scales, const void* w_c
                       const void* w_scales, const void* bias, int act, void* out, int dtype,
                       long long out_row_stride, int M, int N, int K, void* stream);
 /* t2t_mxfp4_quantize of x into the workspace and t2t_mxfp4_product (one launch
- * and no workspace where the rows are few).  out shares no memory with x. */
+ * and no workspace where M <= 32 and M * ceil(K / 256) * 8 <= 2048).  out and ws
+ * share no memory with another argument. */
 size_t t2t_mxfp4_linear_ws_bytes(int M, int N, int K);
 int t2t_mxfp4_linear(const void* x, int dtype, long long x_row_stride, const void* w_codes,
                      const void* w_scales, const void* bias, int act, void* out,

@@ -103,7 +103,7 @@ __device__ inline void mx_block(const u32x4 (&x)[4], u32x4& codes, uint32_t& byt
 // ---------------------------------------------------------------------------
 // quantise: a work-group per 32 rows x 256 columns, a thread per block (64 bytes
 // of a row; the four loads' lines meet in L1).  Bound: reading x, 75,600 x 5,120
-// in 183 us, 5.4 TB/s with the codes written.
+// in 185 us, 5.3 TB/s with the codes written.
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const uint16_t* __restrict__ x,
@@ -370,10 +370,13 @@ __device__ inline void mx_store(const f32x16 (&acc)[TW][TA], char* so, uint16_t*
 // outputs is in flight outside it.
 // Why this tile: per stage a CU moves 36 KB to LDS (64 bytes a cycle at most) and
 // reads 64 KB from it for 1024 cycles of products; with 128 x 128 it is LDS that
-// bounds.  Measured: 1203 cycles a stage and 12,000 a tile, 4.4 PFLOP/s at K =
-// 5120, 4.9 at 13,824.  Bound: power.  The card holds 1.5 GHz of 2.4 on random
-// codes; with loads that always hit L2, or reads and DMA placed otherwise, the
-// time is the same, and with zero codes it is 1.3 times shorter.
+// bounds.  Measured: 1203 cycles a stage, 1024 of them products, and 12,000 a tile
+// beside them (its start and its epilogue, which only DMA overlaps: a fifth of the
+// time at K = 5120); 4.4 PFLOP/s at K = 5120, 4.9 at 13,824.  Bounds: those idle
+// cycles, and power: the card holds 1.5 to 1.75 GHz of 2.4 on random codes, and
+// with zero codes the time is 1.3 times shorter.  With loads that always hit L2, or
+// reads and DMA placed otherwise, it is the same.  How much of the idle fifth the
+// clock would take back is not measured.
 #define MX_P(i, j)                                                                                      \
   "v_mfma_scale_f32_32x32x64_f8f6f4 %[c" #i #j "], %[w" #i "], %[a" #j "], %[c" #i #j "], %[p" #i     \
   "], %[q" #j "] " MX_SEL " cbsz:4 blgp:4\n\t"
@@ -737,9 +740,9 @@ __global__ __launch_bounds__(256, 2) void mx_mid_kernel(MxMat a, MxMat w, const 
 // the order of the waves.  With X16 the tokens come in 16 bits and every
 // work-group quantises them into LDS first (MX_X16_BLOCKS blocks at most), under
 // the loads of its first weights, in the place of a launch before this one.
-// Bound: one round of loads and the exchange (1 x 5120 x 5120: 5.8 us, with X16
-// 6.4 and 8.3 in two launches); with more tokens the bytes from L2, which every
-// 32 x 32 block reads for itself.
+// Bound: one round of loads and the exchange (1 x 5120 x 5120, 160 work-groups for
+// 256 CUs: 5.3 us, with X16 5.4, against 2.7 more for a launch that quantises); with
+// more tokens the bytes from L2, which every 32 x 32 block reads for itself.
 #define MX_X16_BLOCKS 2048
 struct MxSrc {
   MxMat m;            // in MXFP4 (its row count in either case), or
@@ -872,7 +875,7 @@ static int mx_tile_launch(const MxMat& a, const MxMat& w, const uint16_t* bias, 
                           long long ldo, int groups, hipStream_t st) {
   const int mt = cdiv(a.blocks, 2 * TA), nt = cdiv(w.blocks, 2 * TW);
   const long long tiles = (long long)mt * nt;
-  if (tiles > (1 << 23)) {  // 2^32 threads
+  if (tiles > (1 << 23)) {  // 2^31 threads of 128 x 128 tiles; as many large ones are a TB of outputs
     t2t_set_error("mxfp4_product: M=%d N=%d", a.rows, w.rows);
     return T2T_ERR_UNSUPPORTED;
   }
@@ -900,9 +903,11 @@ static int mx_tile_launch(const MxMat& a, const MxMat& w, const uint16_t* bias, 
 // Which product: by the number of outputs.  Below 512 blocks of 32 x 32 too few tiles would go through
 // all of K one stage after another (64 x 5120 x 5120: split 7.6 us, 128 x 128 tiles 10.6; 128 x 5120 x
 // 5120: 10.7 and 10.8; 256 x: 15.8 and 11.0).  From 256 large tiles on they fill the chip (4096^3: 37.4
-// us, 128 x 128 tiles 42.1; 1500 x 5120 x 5120, 120 large tiles: 33.3 and 25.9), unless K is short and
+// us, 128 x 128 tiles 38.4; 1500 x 5120 x 5120, 120 large tiles: 33.3 and 25.9), unless K is short and
 // they are few (9000 x 2048 x 512: 20.4 and 15.8; 75,600 x 5120 x 128: 172 and 208) or they would be
-// padded by more than a quarter over the small ones (75,600 x 96 x 1536: 34.1 and 17.7).
+// padded by more than a quarter over the small ones (75,600 x 96 x 1536: 34.1 and 17.7).  Rounds of 256
+// work-groups are not counted, which loses where the second holds few tiles (K = 4096, 289 of them: 52.7
+// and 42.5; 324: 51.9 and 50.3; 400: 55.6 and 58.5; 504: 62.2 and 69.8; 576: 83.2 and 78.8).
 template <typename T>
 static int mx_product(const MxMat& a, const MxMat& w, const uint16_t* bias, int act, uint16_t* out,
                       long long ldo, int groups, hipStream_t st) {
@@ -947,7 +952,7 @@ extern "C" int t2t_mxfp4_product(const void* a_codes, const void* a_scales, cons
 }
 
 // Few rows are quantised by the product itself, as far as its LDS holds them: every work-group does it
-// again, which costs what the saved launch gains at 12 x 5120 (8.2 us either way; 1 x: 6.4 and 8.3).
+// again, which costs what the saved launch gains at 12 x 5120 (8.2 us either way; 1 x: 5.4 and 8.0).
 static bool mx_few(int M, int K) { return M <= 32 && (long long)M * (mx_kp(K) / 32) <= MX_X16_BLOCKS; }
 
 // codes, then scales

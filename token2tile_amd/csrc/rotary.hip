@@ -7,9 +7,11 @@
 // with start[a] <= i < start[a + 1].  The angle is one fp64 product (a far
 // position leaves no fraction in fp32) and its sine and cosine are taken in
 // fp64, so the fp32 entries are off by one rounding.  A thread keeps one pair
-// and goes through the positions.  75,600 x 64 entries take 16 us (2.4 TB/s of
-// writes), bound by the issue of 23 fp64 operations an entry; with the device
-// library's sincos, which takes any angle, 24 us.
+// and goes through the positions.  75,600 x 64 entries take 15 us into the same
+// buffers again, 17 into others (2.6 and 2.3 TB/s of writes).  Counted: 77 vector
+// instructions an entry, 9.5 us of issue, of which the 23 in fp64 are 3; the
+// others are addresses and a thread's setup for its four positions.  With the
+// device library's sincos, which takes any angle, 24 us.
 // ---------------------------------------------------------------------------
 struct TableAxes {
   int n;
@@ -128,8 +130,8 @@ extern "C" int t2t_rotary_table(const void* positions, int pos_bits, long long T
 // ---------------------------------------------------------------------------
 // y = rotate(x rsqrt(mean(x^2) + eps) w), fp32 inside, one rounding at the
 // end.  Bound: one read and one write of every element (q and k of 75,600 tokens
-// x 40 heads x 128: 575 us, 5.4 TB/s; pair by pair in the general form below 2.1
-// ms; 4 tokens: 4.8 us).
+// x 40 heads x 128: 575 us, 5.4 TB/s; one element off their alignment, pair by
+// pair in the general form below, 2.5 ms; 4 tokens: 4.8 us).
 //
 // A head is cut into units of 2 V channels that turn together (V: 8, or 4 where
 // widths, strides or addresses ask for it): with paired halves channels V u .. +
@@ -154,9 +156,10 @@ struct RotaryArgs {
   int hshift[2], chunks[2];  // q and k: log2 of a wave's heads, rounds of ITS that a token takes
 };
 
-// What every form below computes alike, so that a result does not depend on the form that its call's
+// What every form below computes alike, so that a result hardly depends on the form that its call's
 // shape and strides take: the turn (one product rounded, one fused), and the norm's sum, fp32 over
-// each four channels of a head in their order and fp64 over these (no order of which shows in fp32).
+// each four channels of a head in their order and fp64 over these (the order differs between the forms,
+// which shows only where two sums a few fp64 steps apart round to different fp32 values).
 __device__ inline void rope_turn(float a, float e, float c, float s, float& y0, float& y1) {
   y0 = __builtin_fmaf(a, c, -(e * s));
   y1 = __builtin_fmaf(a, s, e * c);
