@@ -410,6 +410,7 @@ def test_outputs_of_tables_and_linears_share_no_memory(launches):
               lambda: ops.mxfp4_linear(x, W, other[:N], out=other[:M * N].view(M, N)),
               lambda: ops.mxfp4_linear(big, W, ws=buf.view(torch.uint8)),
               lambda: ops.mxfp4_linear(big, W, out=other[:400 * N].view(400, N), ws=raw[(1 << 16):]),
+              lambda: ops.MxFp4(raw[:n[0]], raw[n[0] - 16:sum(n) - 16], N, K),
               lambda: ops.mxfp4_dequantize(X, out=raw[:2 * N * K].view(dt).view(N, K)),
               lambda: ops.mxfp4_quantize(raw[:2 * N * K].view(dt).view(N, K), out=X)):
         with pytest.raises(ValueError, match="shares memory"):

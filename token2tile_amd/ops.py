@@ -835,6 +835,14 @@ def _meet(a, b):
     return search(b.data_ptr() - a.data_ptr(), 0)
 
 
+def _near(lo, hi, spans):
+    """Whether addresses [lo, hi) meet one of spans ((address, bytes) each)."""
+    for p, n in spans:
+        if p < hi and lo < p + n:
+            return True
+    return False
+
+
 def _apart(outs, names, ins):
     """The outputs share no memory with one another or with the inputs, but that
     outs[i] may be ins[i]."""
@@ -1068,14 +1076,13 @@ class MxFp4:
             _check(t, (n,), torch.uint8, name, dev)
             if n and t.data_ptr() % 16:
                 raise ValueError(f"t2t: {name} must be 16-byte aligned")
+        if _near(*_span(codes), ((scales.data_ptr(), scales.nbytes),)):
+            raise ValueError("t2t: scales shares memory with codes")
         self._set(codes, scales, rows, cols)
 
     def _set(self, codes, scales, rows, cols):
         self._codes, self._scales, self._rows, self._cols = codes, scales, rows, cols
         return self
-
-    def _ptrs(self):
-        return self._codes.data_ptr(), self._scales.data_ptr()
 
     codes = property(lambda self: self._codes)
     scales = property(lambda self: self._scales)
@@ -1126,7 +1133,8 @@ def mxfp4_quantize(x, out=None, stream=None):
     dev = _dev(x)
     _on(stream, dev)
     M, K, stride = _mx_rows(x, "x", dev, 16)
-    if out is None:
+    given = out is not None
+    if not given:
         if K < 32 or K % 32 or K > 2 ** 27 or M > 2 ** 30:
             raise ValueError(f"t2t: x must have columns in multiples of 32, got {M} x {K}")
         nc, ns = _mx_bytes(M, K)
@@ -1134,10 +1142,11 @@ def mxfp4_quantize(x, out=None, stream=None):
                                         _empty(stream, (ns,), torch.uint8, dev), M, K)
     elif not isinstance(out, MxFp4) or out.shape != (M, K) or _dev(out._codes) != dev:
         raise ValueError(f"t2t: out must be an MxFp4 matrix {M} x {K} on {dev}, got {out!r}")
-    else:
-        _apart((out._codes, out._scales), ("out.codes", "out.scales"), (None, None, x))
-    _launch("t2t_mxfp4_quantize", dev, stream, (x, out._codes, out._scales), x.data_ptr(),
-            dtype_code(x.dtype), stride, *out._ptrs(), M, K)
+    px, codes, scales = x.data_ptr(), out._codes, out._scales
+    pc, ps = codes.data_ptr(), scales.data_ptr()
+    if given and _near(px, px + 2 * ((M - 1) * stride + K), ((pc, codes.nbytes), (ps, scales.nbytes))):
+        _apart((codes, scales), ("out.codes", "out.scales"), (None, None, x))
+    _launch("t2t_mxfp4_quantize", dev, stream, (x, codes, scales), px, dtype_code(x.dtype), stride, pc, ps, M, K)
     return out
 
 
@@ -1146,7 +1155,8 @@ def mxfp4_dequantize(t, dtype=torch.bfloat16, out=None, stream=None):
     type that was quantised, and in bf16 always."""
     if not isinstance(t, MxFp4):
         raise ValueError("t2t: expected an MxFp4 matrix")
-    dev = _dev(t._codes)
+    codes, scales = t._codes, t._scales
+    dev = codes.device if codes.is_cuda else _dev(codes)
     _on(stream, dev)
     code = _mx_dtype(dtype)
     if out is None:
@@ -1156,9 +1166,9 @@ def mxfp4_dequantize(t, dtype=torch.bfloat16, out=None, stream=None):
         M, K, stride = _mx_rows(out, "out", dev, 16)
         if (M, K) != t.shape or out.dtype != dtype:
             raise ValueError(f"t2t: out must be {dtype} {t.shape}, got {out.dtype} {tuple(out.shape)}")
-        _apart((out,), ("out",), (None, t._codes, t._scales))
-    _launch("t2t_mxfp4_dequantize", dev, stream, (t._codes, t._scales, out), *t._ptrs(), out.data_ptr(), code,
-            stride, *t.shape)
+        _apart((out,), ("out",), (None, codes, scales))
+    _launch("t2t_mxfp4_dequantize", dev, stream, (codes, scales, out), codes.data_ptr(), scales.data_ptr(),
+            out.data_ptr(), code, stride, *t.shape)
     return out
 
 
@@ -1180,13 +1190,16 @@ def mxfp4_linear(x, weight, bias=None, *, activation=None, dtype=None, out=None,
     ``out``: contiguous rows; it and ``ws`` share no memory with another argument."""
     if not isinstance(weight, MxFp4):
         raise ValueError("t2t: weight must be an MxFp4 matrix (mxfp4_quantize)")
-    dev = _dev(weight._codes)
+    wc, wsc = weight._codes, weight._scales
+    dev = wc.device if wc.is_cuda else _dev(wc)
     _on(stream, dev)
     N = weight._rows
-    if isinstance(x, MxFp4):
-        if x.device != dev:
+    shared = isinstance(x, MxFp4)
+    if shared:
+        xs = x._codes, x._scales
+        if xs[0].device != dev:
             raise ValueError(f"t2t: x must be on {dev}")
-        M, K = x.shape
+        M, K = x._rows, x._cols
         shape = (M, N)
         dt = torch.bfloat16 if dtype is None else dtype
     else:
@@ -1194,37 +1207,43 @@ def mxfp4_linear(x, weight, bias=None, *, activation=None, dtype=None, out=None,
         shape, dt = (*x.shape[:-1], N), x.dtype
         if dtype not in (None, dt):
             raise ValueError(f"t2t: the output of a {dt} input is {dt}, not {dtype}")
-    code = _mx_dtype(dt)
+    code = _mx_dtype(dt) if shared else dtype_code(dt)
     if K != weight._cols or N < 1:
         raise ValueError(f"t2t: x has {K} columns, weight {N} x {weight._cols}")
     if activation not in _ACTIVATIONS:
         raise ValueError(f"t2t: activation {activation!r} (None or gelu_tanh)")
     if bias is not None and not _is(bias, (N,), dt, dev):
         _check(bias, (N,), dt, "bias", dev)
+    args = wc.data_ptr(), wsc.data_ptr(), None if bias is None else bias.data_ptr()
+    spans = None  # of the inputs, where the caller brings an output or a workspace
+    if out is not None or ws is not None:
+        spans = [(args[0], wc.nbytes), (args[1], wsc.nbytes)] + [(args[2], 2 * N)] * (bias is not None)
+        spans += ([(t.data_ptr(), t.nbytes) for t in xs] if shared else
+                  [(x.data_ptr(), 2 * ((M - 1) * stride + K))])
     if out is None:
-        out = _empty(stream, shape, dt, dev) if stream is not None or isinstance(x, MxFp4) else x.new_empty(shape)
-        ostride = N
+        out = _empty(stream, shape, dt, dev) if stream is not None or shared else x.new_empty(shape)
+        ostride, po = N, out.data_ptr()
     else:
         ostride = _mx_rows(out, "out", dev, 2)[2]
         if tuple(out.shape) != shape or out.dtype != dt:
             raise ValueError(f"t2t: out must be {dt} {shape}, got {out.dtype} {tuple(out.shape)}")
-        _apart((out,), ("out",), (None, *((x._codes, x._scales) if isinstance(x, MxFp4) else (x,)),
-                                  weight._codes, weight._scales, bias))
-    args = (*weight._ptrs(), None if bias is None else bias.data_ptr(), _ACTIVATIONS[activation],
-            out.data_ptr())
-    if isinstance(x, MxFp4):
-        _launch("t2t_mxfp4_product", dev, stream,
-                (x._codes, x._scales, weight._codes, weight._scales, bias, out), *x._ptrs(), *args, code,
-                ostride, M, N, K)
+        po = out.data_ptr()
+        if _near(po, po + 2 * ((M - 1) * ostride + N), spans):
+            _apart((out,), ("out",), (None, *(xs if shared else (x,)), wc, wsc, bias))
+    args = *args, _ACTIVATIONS[activation], po
+    if shared:
+        _launch("t2t_mxfp4_product", dev, stream, (*xs, wc, wsc, bias, out), xs[0].data_ptr(),
+                xs[1].data_ptr(), *args, code, ostride, M, N, K)
     else:
         need = mxfp4_linear_ws_bytes(M, N, K)
         if ws is not None:
             ws = _ws_for(ws, need, dev, stream)
-            if need:
-                _apart((ws[:need],), ("ws",), (None, x, weight._codes, weight._scales, bias, out))
+            at = ws.data_ptr()
+            if need and _near(at, at + need, (*spans, (po, 2 * ((M - 1) * ostride + N)))):
+                _apart((ws[:need],), ("ws",), (None, x, wc, wsc, bias, out))
         elif need:
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if stream is None else _ws(need, dev, stream)
-        _launch("t2t_mxfp4_linear", dev, stream, (x, weight._codes, weight._scales, bias, out, ws), x.data_ptr(),
+        _launch("t2t_mxfp4_linear", dev, stream, (x, wc, wsc, bias, out, ws), x.data_ptr(),
                 code, stride, *args, ostride, M, N, K, None if ws is None else ws.data_ptr(),
                 0 if ws is None else ws.numel())
     return out
