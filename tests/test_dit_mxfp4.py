@@ -61,7 +61,7 @@ def test_the_layer_is_a_module(monkeypatch, bias):
     assert c(torch.zeros(2, 3, 64, dtype=torch.float16)).shape == (2, 3, 40)
     assert seen[-1][0] == "t2t_mxfp4_linear" and c.weight.codes.data_ptr() in seen[-1][1]
     c.to("meta")
-    assert c.weight.codes.device.type == "meta" and c.weight.scales.device.type == "meta"
+    assert c.weight_codes.device.type == "meta" and c.weight_scales.device.type == "meta"
 
 
 @pytest.mark.gpu
