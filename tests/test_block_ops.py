@@ -8,6 +8,7 @@ import math
 import pickle
 import random
 
+import numpy as np
 import pytest
 import torch
 
@@ -58,6 +59,18 @@ def test_frequencies_of_every_scaling():
     three = ops.rotary_frequencies((44, 42, 42), device="cpu")
     assert three.pairs == (22, 21, 21) and three.freqs.shape == (64,)
     assert three.freqs[22] == 1.0 and three.freqs[43] == 1.0
+
+
+@pytest.mark.parametrize("dims", [64.0, np.int64(64), (64.0,), [np.int32(64)], torch.tensor(64)])
+def test_frequencies_of_whole_numbers_of_any_type(dims):
+    f = ops.rotary_frequencies(dims, device="cpu")
+    assert f.pairs == (32,) and type(f.pairs[0]) is int
+    assert torch.equal(f.freqs, ops.rotary_frequencies(64, device="cpu").freqs)
+    for three in (np.array([44, 42, 42]), (d for d in (44, 42, 42)), torch.tensor([44, 42, 42])):
+        assert ops.rotary_frequencies(three, device="cpu").pairs == (22, 21, 21)
+    for bad in (63.5, "64", None, (64, None), math.nan, math.inf):
+        with pytest.raises(ValueError, match="t2t"):
+            ops.rotary_frequencies(bad, device="cpu")
 
 
 @pytest.mark.parametrize("d,base,L,fast,slow", [

@@ -894,9 +894,19 @@ class RotaryFrequencies(NamedTuple):
 def rotary_frequencies(dims, *, base=10000.0, scaling=None, device):
     """The frequencies of rotated channels ``dims`` (an even number, or one
     for each of up to four position axes), to be kept by the program."""
-    dims = (dims,) if isinstance(dims, int) else tuple(dims)
-    if not 1 <= len(dims) <= 4 or any(int(d) != d or d < 2 or d % 2 or d > 8192 for d in dims):
-        raise ValueError(f"t2t: dims must be one to four even numbers in [2, 8192], got {dims}")
+    given = dims
+    try:
+        dims = tuple(dims)
+    except TypeError:
+        dims = (dims,)
+    try:
+        whole = [int(d) for d in dims]
+        fits = 1 <= len(whole) <= 4 and all(w == d and 2 <= w <= 8192 and w % 2 == 0 for w, d in zip(whole, dims))
+    except (TypeError, ValueError, OverflowError):
+        fits = False
+    if not fits:
+        raise ValueError(f"t2t: dims must be one to four even numbers in [2, 8192], got {given}")
+    dims = tuple(whole)
     if not (math.isfinite(base) and base > 1.0):
         raise ValueError(f"t2t: base must be above 1, got {base}")
     factor = 1.0
