@@ -1,0 +1,470 @@
+"""Performance cases of the block operators for 8-bit weights and for generation
+chunk by chunk: 8-bit quantisation by rows, the 8-bit linear layer, the append
+of keys and values to a paged cache (with the norm and rotation of q and k), and
+attention of new tokens over such a cache.
+
+With ``own`` false, ``run`` computes each operator in its plain form, out of
+elementary torch operations; with ``own`` true it makes the calls of
+``token2tile_amd.ops`` that ``token2tile_amd/dit.py`` makes.
+
+``kind`` of a case:
+  quantize  ``int8_quantize`` and ``int8_dequantize``: the values that the 8-bit
+            codes and their scales stand for
+  linear    ``int8_linear``: a 16-bit input, a weight kept in 8 bits
+  append    ``cache_append``: q, k and v of new tokens; k and v into their slots
+  attend    ``cache_attention``: new tokens over the keys and values of their
+            sequences, the new ones among them
+"""
+import math
+
+import torch
+
+own = False
+
+DEV = torch.device("cuda", 0)
+F32, F64, I32 = torch.float32, torch.float64, torch.int32
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16}
+EPS = 1e-6
+LOWEST = 2.0 ** -120  # of a row's scale
+
+
+def _quantize(name, M, K, dtype="bf16"):
+    return dict(name=name, kind="quantize", M=M, K=K, dtype=dtype)
+
+
+def _linear(name, M, N, K, act="none", bias=True, dtype="bf16"):
+    return dict(name=name, kind="linear", M=M, N=N, K=K, act=act, bias=bias, dtype=dtype)
+
+
+def _append(name, T, B, HQ, HK, D, R, layout, norm, page, pad=0, dtype="bf16"):
+    """T tokens of B sequences, the last ``pad`` of them stored nowhere."""
+    return dict(name=name, kind="append", T=T, B=B, HQ=HQ, HK=HK, D=D, R=R, layout=layout, norm=norm,
+                page=page, pad=pad, dtype=dtype)
+
+
+def _attend(name, B, N, L, HQ, HK, D, mask, page, ragged=False, dtype="bf16"):
+    """B sequences of up to N new tokens and up to L keys, those of the new ones included."""
+    return dict(name=name, kind="attend", B=B, N=N, L=L, HQ=HQ, HK=HK, D=D, mask=mask, page=page,
+                ragged=ragged, dtype=dtype)
+
+
+def listed():
+    return [
+        # the activations that enter the projections of a 720p block
+        _quantize("quantize_720p", 75600, 5120),
+        # ragged rows of an odd width
+        _quantize("quantize_odd", 4099, 1531, "fp16"),
+        # one row through a projection: a single token, weight reading
+        _linear("linear_token", 1, 5120, 5120),
+        # three latent frames at 480p through a projection of the small model
+        _linear("linear_chunk", 4680, 1536, 1536),
+        # ragged in every size, no bias
+        _linear("linear_odd", 4099, 2041, 1571, "none", False, "fp16"),
+        # the first feed-forward layer of a 720p block
+        _linear("linear_ffn_720p", 75600, 13824, 5120, "gelu"),
+        # a batch of four single tokens: latency
+        _append("append_token", 4, 4, 40, 40, 128, 128, "interleaved", "token", 64),
+        # three latent frames at 480p, as the block stack makes them
+        _append("append_chunk", 4680, 1, 40, 40, 128, 128, "interleaved", "token", 64),
+        # ragged prompts with shared key heads, norm of each head, part of the head rotated, padded
+        _append("append_shared", 10007, 5, 32, 8, 128, 96, "half", "head", 16, 23, "fp16"),
+        # single tokens of sixteen sequences over long caches: key and value reading
+        _attend("attend_token", 16, 1, 32760, 40, 8, 128, "none", 64),
+        # trees of drafted tokens, a ragged batch
+        _attend("attend_tree", 3, 61, 16001, 32, 8, 128, "tree", 16, True),
+        # three latent frames at 480p over 21 frames
+        _attend("attend_chunk", 1, 4680, 32760, 40, 40, 128, "none", 64),
+    ]
+
+
+def _log(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    kind = rng.choice(["quantize", "linear", "linear", "linear", "append", "append", "attend", "attend",
+                       "attend", "attend"])
+    dtype = rng.choice(["bf16", "bf16", "fp16"])
+    while True:
+        if kind == "quantize":
+            c = _quantize("", _log(rng, 1, 75600), _log(rng, 16, 5120), dtype)
+        elif kind == "linear":
+            M, N, K = _log(rng, 1, 75600), _log(rng, 64, 13824), _log(rng, 64, 13824)
+            if rng.random() < 0.5:
+                K = (K + 31) // 32 * 32
+            if M * N * K > 75600 * 13824 * 5120:
+                continue
+            c = _linear("", M, N, K, rng.choice(["none", "gelu"]), rng.random() < 0.7, dtype)
+        else:
+            HQ = rng.choice([1, 2, 5, 8, 12, 16, 24, 32, 40])
+            HK = rng.choice([HQ, HQ, HQ // 4 if HQ % 4 == 0 else HQ, 1])
+            D, page = rng.choice([64, 128, 128, 128]), rng.choice([1, 16, 16, 48, 64, 64, 256])
+            if kind == "append":
+                T = _log(rng, 1, 75600)
+                if T * (2 * HQ + 4 * HK) * D > 32760 * 240 * 128:
+                    continue
+                pad = rng.choice([0, 0, min(T - 1, _log(rng, 1, 64))])
+                c = _append("", T, min(T, _log(rng, 1, 32)), HQ, HK, D, rng.choice([D, D, D // 2]),
+                            rng.choice(["interleaved", "half"]), rng.choice(["token", "token", "head", "none"]),
+                            page, pad, dtype)
+            else:
+                mask = rng.choice(["none", "none", "causal", "tree", "frames"])
+                B, N, L = _log(rng, 1, 32), _log(rng, 1, 160 if mask == "tree" else 8192), _log(rng, 1, 65536)
+                L = max(L, N)
+                if B * N * L * HQ * D > 4680 * 32760 * 40 * 128 or B * L * HK * D > 16 * 65536 * 8 * 128:
+                    continue
+                if mask == "frames" and B * N * N > 1 << 28:
+                    continue
+                c = _attend("", B, N, L, HQ, HK, D, mask, page, rng.random() < 0.5, dtype)
+        del c["name"]
+        return c
+
+
+# ---------------------------------------------------------------------------
+# inputs
+# ---------------------------------------------------------------------------
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _randn(g, *shape):
+    return torch.randn(*shape, generator=g, device=DEV, dtype=F32)
+
+
+def _activations(g, rows, cols, dt):
+    """Rows whose channels have scales of their own, a few far above the rest."""
+    scale = torch.exp(0.5 * _randn(g, cols))
+    scale[torch.randint(0, cols, (max(1, cols // 256),), generator=g, device=DEV)] *= 20.0
+    return _randn(g, rows, cols).mul_(scale).to(dt)
+
+
+def _pages(lengths, page, g):
+    """Pages in no order for sequences of these lengths: how many there are (a few are no one's),
+    and each sequence's row of the table (-1 behind its last page)."""
+    need = [-(-n // page) for n in lengths]
+    total = sum(need) + 3
+    order, table, at = torch.randperm(total, generator=g, device=DEV).to(I32), [], 0
+    for n in need:
+        row = torch.full((max(need),), -1, dtype=I32, device=DEV)
+        row[:n] = order[at:at + n]
+        table.append(row)
+        at += n
+    return total, torch.stack(table)
+
+
+def _shares(case):
+    """Tokens of each sequence of an append."""
+    T, B = case["T"], case["B"]
+    return [T // B + (b < T % B) for b in range(B)]
+
+
+def _sizes(case):
+    """New tokens and keys of each sequence of an attention call."""
+    B, N, L = case["B"], case["N"], case["L"]
+    rows = [max(1, N - b * N // (2 * B)) if case["ragged"] else N for b in range(B)]
+    return rows, [max(rows[b], L - b * L // (2 * B)) for b in range(B)]
+
+
+def _mask(case, rows, g):
+    """bool [rows of all sequences, N]: which new tokens of its sequence a new token sees."""
+    out = []
+    for n in rows:
+        see = torch.zeros(n, case["N"], dtype=torch.bool, device=DEV)
+        i = torch.arange(n, device=DEV)
+        if case["mask"] == "frames":  # frames of an eighth of the chunk, every one sees itself and those before it
+            f = i // max(1, n // 8)
+            see[:, :n] = f[None, :] <= f[:, None]
+        else:                         # a tree: every token but the first hangs below one of those before it
+            up = (torch.rand(n, generator=g, device=DEV) * i).long().clamp_(max=n - 1)
+            eye = torch.eye(n, dtype=F32, device=DEV)
+            step = torch.zeros(n, n, dtype=F32, device=DEV)
+            step[i[1:], up[1:]] = 1.0
+            reach = eye + step
+            for _ in range(max(1, (n - 1).bit_length())):
+                reach = (reach @ reach > 0).float()
+            see[:, :n] = reach > 0
+        out.append(see)
+    return torch.cat(out)
+
+
+def prepare(case, seed):
+    g = _gen(seed)
+    st = dict(case=case)
+    dt = DT[case["dtype"]]
+    if case["kind"] == "quantize":
+        st["x"] = _activations(g, case["M"], case["K"], dt)
+    elif case["kind"] == "linear":
+        M, N, K = case["M"], case["N"], case["K"]
+        st["x"] = _activations(g, M, K, dt)
+        w = (_randn(g, N, K) * K ** -0.5).to(dt)
+        st["b"] = (0.1 * _randn(g, N)).to(dt) if case["bias"] else None
+        if own:  # a program keeps its weights in 8 bits ...
+            from token2tile_amd import ops
+            st["w"] = ops.int8_quantize(w)
+        else:    # ... or as whole numbers beside the channels' scales
+            st["w"] = tuple(t.to(torch.int8) if i == 0 else t for i, t in enumerate(_codes(w)))
+    elif case["kind"] == "append":
+        T, D, R = case["T"], case["D"], case["R"]
+        for x, H in (("q", case["HQ"]), ("k", case["HK"]), ("v", case["HK"])):
+            st[x] = _activations(g, T, H * D, dt).view(T, H, D)
+            if case["norm"] != "none" and x != "v":
+                n = H * D if case["norm"] == "token" else D
+                st["w" + x] = (1.0 + 0.2 * _randn(g, n)).to(dt)
+        shares = _shares(case)
+        start = torch.randint(0, 4096, (len(shares),), generator=g, device=DEV)
+        first = start % case["page"]       # a sequence goes on inside a page
+        total, table = _pages([n + case["page"] - 1 for n in shares], case["page"], g)
+        seq = torch.repeat_interleave(torch.arange(len(shares), device=DEV),
+                                      torch.tensor(shares, device=DEV), output_size=T)
+        ends = torch.tensor(shares, device=DEV).cumsum(0)
+        i = torch.arange(T, device=DEV) - (ends - torch.tensor(shares, device=DEV))[seq]
+        at = first[seq] + i
+        st["slots"] = table.long()[seq, at // case["page"]] * case["page"] + at % case["page"]
+        if case["pad"]:
+            st["slots"][-case["pad"]:] = -1
+        freq = 10000.0 ** (-2.0 * torch.arange(R // 2, device=DEV, dtype=F64) / R)
+        ang = (start[seq] + i)[:, None].double() * freq
+        st["cos"], st["sin"] = ang.cos().float(), ang.sin().float()
+        shape = (total, case["page"], case["HK"], D)
+        st["ck"], st["cv"] = _randn(g, *shape).to(dt), _randn(g, *shape).to(dt)
+    else:
+        rows, lens = _sizes(case)
+        total, st["table"] = _pages(lens, case["page"], g)
+        shape = (total, case["page"], case["HK"], case["D"])
+        st["ck"], st["cv"] = _randn(g, *shape).to(dt), _randn(g, *shape).to(dt)
+        st["q"] = (1.5 * _randn(g, sum(rows), case["HQ"], case["D"])).to(dt)
+        st["lengths"] = torch.tensor(lens, dtype=I32, device=DEV)
+        st["mask"] = _mask(case, rows, g) if case["mask"] in ("tree", "frames") else None
+        st["offsets"] = None
+        if case["ragged"]:
+            st["offsets"] = torch.tensor([0] + rows, device=DEV).cumsum(0).to(I32)
+        else:
+            st["q"] = st["q"].view(case["B"], case["N"], case["HQ"], case["D"])
+            if st["mask"] is not None:
+                st["mask"] = st["mask"].view(case["B"], case["N"], case["N"])
+    if own and case["kind"] in ("append", "attend"):
+        from token2tile_amd import ops
+        st["cache"] = ops.PagedCache(st["ck"], st["cv"])
+    return st
+
+
+# ---------------------------------------------------------------------------
+# plain forms
+# ---------------------------------------------------------------------------
+def _codes(x):
+    """Whole numbers -127 .. 127 (in 32 bits) and a scale for each row of x [M, K].  The quotients
+    are taken in 64 bits: one in 32 may fall on the other side of a border."""
+    top = x.abs().amax(-1).float()
+    scale = (top / 127.0).clamp_(min=LOWEST)
+    code = torch.cat([torch.round(a.double() / s[:, None].double()).float()
+                      for a, s in zip(x.split(8192), scale.split(8192))])
+    return code.clamp_(-127.0, 127.0), scale
+
+
+def _gelu(x):
+    return 0.5 * x * (1.0 + torch.tanh(math.sqrt(2.0 / math.pi) * (x + 0.044715 * x * x * x)))
+
+
+def _turn(st, x, w, case):
+    y = x.float()
+    if case["norm"] == "token":
+        f = y.flatten(1)
+        y = (f * torch.rsqrt(f.pow(2).mean(-1, keepdim=True) + EPS) * w.float()).view(y.shape)
+    elif case["norm"] == "head":
+        y = y * torch.rsqrt(y.pow(2).mean(-1, keepdim=True) + EPS) * w.float()
+    R = case["R"]
+    c, s = st["cos"][:, None], st["sin"][:, None]
+    r, rest = y[..., :R], y[..., R:]
+    if case["layout"] == "half":
+        a, b = r[..., :R // 2], r[..., R // 2:]
+        r = torch.cat((a * c - b * s, a * s + b * c), dim=-1)
+    else:
+        a, b = r[..., 0::2], r[..., 1::2]
+        r = torch.stack((a * c - b * s, a * s + b * c), dim=-1).flatten(-2)
+    return torch.cat((r, rest), dim=-1).to(x.dtype)
+
+
+def _sequence(st, case, b, length):
+    """Keys and values [heads, length, D] of a sequence, in 32 bits."""
+    pos = torch.arange(length, device=DEV)
+    page, row = st["table"][b, pos // case["page"]].long(), pos % case["page"]
+    return (st["ck"][page, row].float().transpose(0, 1).contiguous(),
+            st["cv"][page, row].float().transpose(0, 1).contiguous())
+
+
+def _attention(st, case):
+    rows, lens = _sizes(case)
+    HQ, HK, D = case["HQ"], case["HK"], case["D"]
+    G, q, out, at = HQ // HK, st["q"].view(-1, HQ, D), [], 0
+    for b, (n, length) in enumerate(zip(rows, lens)):
+        k, v = _sequence(st, case, b, length)
+        x = q[at:at + n].float().view(n, HK, G, D).permute(1, 2, 0, 3).reshape(HK, G * n, D)
+        hide = None
+        if case["mask"] == "causal":
+            hide = torch.ones(n, n, dtype=torch.bool, device=DEV).triu(1)
+        elif case["mask"] != "none":
+            hide = ~st["mask"].view(-1, case["N"])[at:at + n, :n]
+        o = torch.empty(HK, G * n, D, device=DEV)
+        step = max(1, (1 << 30) // (G * n * length))
+        for h in range(0, HK, step):
+            s = torch.matmul(x[h:h + step], k[h:h + step].transpose(1, 2)).mul_(D ** -0.5)
+            if hide is not None:
+                s.view(-1, G, n, length)[..., length - n:].masked_fill_(hide, -math.inf)
+            p = s.sub_(s.amax(-1, keepdim=True)).exp_()
+            o[h:h + step] = torch.matmul(p, v[h:h + step]) / p.sum(-1, keepdim=True)
+        out.append(o.view(HK, G, n, D).permute(2, 0, 1, 3).reshape(n, HQ, D))
+        at += n
+    return torch.cat(out).to(st["q"].dtype).view(st["q"].shape)
+
+
+def _plain(st, case):
+    if case["kind"] == "quantize":
+        code, scale = _codes(st["x"])
+        return (code * scale[:, None]).to(st["x"].dtype)
+    if case["kind"] == "linear":
+        code, scale = _codes(st["x"])
+        w, ws = st["w"]
+        y = torch.matmul(code, w.float().t()) * ws * scale[:, None]
+        if st["b"] is not None:
+            y += st["b"].float()
+        if case["act"] == "gelu":
+            y = _gelu(y)
+        return y.to(st["x"].dtype)
+    if case["kind"] == "append":
+        q, k = _turn(st, st["q"], st.get("wq"), case), _turn(st, st["k"], st.get("wk"), case)
+        n = case["T"] - case["pad"]  # (the tokens that are stored: their number is the program's own)
+        for cache, x in ((st["ck"], k), (st["cv"], st["v"])):
+            cache.view(-1, *cache.shape[2:])[st["slots"][:n]] = x[:n]
+        return q, st["ck"], st["cv"]
+    return _attention(st, case)
+
+
+def run(state):
+    st, case = state, state["case"]
+    if not own:
+        return _plain(st, case)
+    from token2tile_amd import ops
+    if case["kind"] == "quantize":
+        return ops.int8_dequantize(ops.int8_quantize(st["x"]), st["x"].dtype)
+    if case["kind"] == "linear":
+        return ops.int8_linear(st["x"], st["w"], st["b"],
+                               activation="gelu_tanh" if case["act"] == "gelu" else None)
+    if case["kind"] == "append":
+        q = ops.cache_append(st["q"], st["k"], st["v"], st["cos"], st["sin"], st["cache"], st["slots"],
+                             layout=case["layout"], norm=None if case["norm"] == "none" else case["norm"],
+                             q_weight=st.get("wq"), k_weight=st.get("wk"), eps=EPS)
+        return q, st["ck"], st["cv"]
+    return ops.cache_attention(st["q"], st["cache"], st["table"], st["lengths"], offsets=st["offsets"],
+                               mask=st["mask"], causal=case["mask"] == "causal")
+
+
+# ---------------------------------------------------------------------------
+# definitions in 64 bits
+# ---------------------------------------------------------------------------
+def _exact_codes(x):
+    """The nearest whole multiple of the row's scale, the even one on ties."""
+    scale = torch.maximum((x.abs().max(-1, keepdim=True).values.to(F32) / 127).to(F64),
+                          torch.full((), LOWEST, dtype=F64, device=x.device))
+    t = x.to(F64) / scale
+    low = t.floor()
+    up = (t - low > 0.5) | ((t - low == 0.5) & (low % 2 != 0))
+    return (low + up).clamp(-127, 127), scale
+
+
+def _exact_attention(st, case):
+    rows, lens = _sizes(case)
+    HQ, HK, D, page = case["HQ"], case["HK"], case["D"], case["page"]
+    q = st["q"].reshape(-1, HQ, D)
+    out = torch.empty(q.shape, dtype=F64, device=DEV)
+    r0 = 0
+    for b in range(case["B"]):
+        n, length = rows[b], lens[b]
+        used = st["table"][b, :(length + page - 1) // page].long()
+        i, j = torch.arange(n, device=DEV)[:, None], torch.arange(length, device=DEV)[None] - (length - n)
+        seen = None
+        if case["mask"] == "causal":
+            seen = j <= i
+        elif case["mask"] != "none":
+            seen = (j < 0).expand(n, length).clone()
+            seen[:, length - n:] = st["mask"].reshape(-1, case["N"])[r0:r0 + n, :n]
+        for h in range(HQ):
+            k = st["ck"][used, :, h * HK // HQ].flatten(0, 1)[:length].to(F64)
+            v = st["cv"][used, :, h * HK // HQ].flatten(0, 1)[:length].to(F64)
+            logit = q[r0:r0 + n, h].to(F64) @ k.T / math.sqrt(D)
+            if seen is not None:
+                logit = torch.where(seen, logit, torch.full((), -math.inf, dtype=F64, device=DEV))
+            out[r0:r0 + n, h] = torch.exp(logit - torch.logsumexp(logit, 1, keepdim=True)) @ v
+        r0 += n
+    return out.view(st["q"].shape)
+
+
+def exact(case, seed):
+    global own
+    was, own = own, False
+    try:
+        st = prepare(case, seed)
+    finally:
+        own = was
+    if case["kind"] == "quantize":
+        out = []
+        for x in st["x"].split(8192):
+            code, scale = _exact_codes(x)
+            out.append(code * scale)
+        return torch.cat(out)
+    if case["kind"] == "linear":
+        w, out = st["w"][0].to(F64).T.contiguous(), []
+        for x in st["x"].split(16384):
+            code, scale = _exact_codes(x)
+            y = code.mm(w).mul_(scale).mul_(st["w"][1].to(F64))
+            if st["b"] is not None:
+                y += st["b"].to(F64)
+            if case["act"] == "gelu":
+                y *= 0.5 + 0.5 * torch.tanh(0.7978845608028654 * y * (1.0 + 0.044715 * y ** 2))
+            out.append(y)
+        return torch.cat(out)
+    if case["kind"] == "attend":
+        return _exact_attention(st, case)
+    R, turned = case["R"], []
+    phase = torch.complex(st["cos"].double(), st["sin"].double()).unsqueeze(1)
+    for name in ("q", "k"):
+        x = st[name].to(F64)
+        if case["norm"] != "none":
+            w = st["w" + name].to(F64)
+            over = (-2, -1) if case["norm"] == "token" else (-1,)
+            x = x / torch.sqrt((x * x).mean(over, keepdim=True) + EPS)
+            x *= w.view(x.shape[1:]) if case["norm"] == "token" else w
+        i = torch.arange(R // 2, device=DEV)
+        re, im = (i, i + R // 2) if case["layout"] == "half" else (2 * i, 2 * i + 1)
+        z = torch.complex(x[..., re], x[..., im]) * phase
+        x[..., re], x[..., im] = z.real, z.imag
+        turned.append(x)
+    keep = st["slots"] >= 0
+    caches = []
+    for cache, x in ((st["ck"], turned[1]), (st["cv"], st["v"].to(F64))):
+        c = cache.to(F64)
+        c.flatten(0, 1)[st["slots"][keep]] = x[keep]
+        caches.append(c)
+    return turned[0], caches[0], caches[1]
+
+
+def work(case):
+    if case["kind"] == "quantize":
+        return {"bytes": 4 * case["M"] * case["K"], "flops": 2 * case["M"] * case["K"]}
+    if case["kind"] == "linear":
+        M, N, K = case["M"], case["N"], case["K"]
+        return {"bytes": 2 * M * K + N * K + 4 * N + 2 * N * case["bias"] + 2 * M * N, "flops": 2 * M * N * K}
+    HQ, HK, D = case["HQ"], case["HK"], case["D"]
+    if case["kind"] == "append":
+        T = case["T"]
+        n = T * (HQ + HK) * D
+        w = {"token": 2 * (HQ + HK) * D, "head": 4 * D, "none": 0}[case["norm"]]
+        return {"bytes": 4 * n + 4 * T * HK * D + 4 * T * case["R"] + 8 * T + w,
+                "flops": 3 * T * (HQ + HK) * case["R"] + (4 * n if case["norm"] != "none" else 0)}
+    rows, lens = _sizes(case)
+    pairs = sum(n * length for n, length in zip(rows, lens))
+    if case["mask"] != "none":  # about half of the new tokens are seen by one of them
+        pairs -= sum(n * (n - 1) // 2 for n in rows)
+    masks = sum(rows) * case["N"] if case["mask"] in ("tree", "frames") else 0
+    return {"bytes": 4 * sum(rows) * HQ * D + 4 * sum(lens) * HK * D
+            + 4 * sum(-(-n // case["page"]) for n in lens) + masks,
+            "flops": 4 * HQ * D * pairs}
