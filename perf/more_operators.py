@@ -253,9 +253,10 @@ def prepare(case, seed):
 # ---------------------------------------------------------------------------
 def _codes(x):
     """Whole numbers -127 .. 127 (in 32 bits) and a scale for each row of x [M, K].  The quotients
-    are taken in 64 bits: one in 32 may fall on the other side of a border."""
-    top = x.abs().amax(-1).float()
-    scale = (top / 127.0).clamp_(min=LOWEST)
+    are taken in 64 bits: in 32 a code may fall on the other side of a border, and a scale's last
+    bit goes by how the division is made."""
+    top = x.abs().amax(-1).double()
+    scale = (top / 127.0).float().clamp_(min=LOWEST)
     code = torch.cat([torch.round(a.double() / s[:, None].double()).float()
                       for a, s in zip(x.split(8192), scale.split(8192))])
     return code.clamp_(-127.0, 127.0), scale
@@ -363,7 +364,7 @@ def run(state):
 # ---------------------------------------------------------------------------
 def _exact_codes(x):
     """The nearest whole multiple of the row's scale, the even one on ties."""
-    scale = torch.maximum((x.abs().max(-1, keepdim=True).values.to(F32) / 127).to(F64),
+    scale = torch.maximum((x.abs().max(-1, keepdim=True).values.to(F64) / 127).to(F32).to(F64),
                           torch.full((), LOWEST, dtype=F64, device=x.device))
     t = x.to(F64) / scale
     low = t.floor()
