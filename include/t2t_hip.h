@@ -510,6 +510,90 @@ int t2t_mxfp4_linear(const void* x, int dtype, long long x_row_stride, const voi
                      long long out_row_stride, int M, int N, int K, void* ws, size_t ws_bytes,
                      void* stream);
 
+/* ---- 8-bit linear layers -------------------------------------------------- */
+/* Matrices [M, K] (M <= 2^30, K < 2^17) of whole numbers -127 .. 127 with one
+ * fp32 scale a row.  No counterpart in the reference.  codes: row m at m *
+ * stride bytes (16-byte aligned, a multiple of 16), columns K .. Kp - 1 of
+ * every row zero, Kp = t2t_int8_row_bytes(K) = K rounded up to 128 <= stride.
+ * Code -128 is taken as it stands. */
+size_t t2t_int8_row_bytes(int K);
+/* x [M, K] fp16 / bf16, row m at m * row_stride (elements; any alignment).  A
+ * row's scale is max|x| / 127 in fp32, at least 2^-120; codes are x / scale to
+ * nearest, ties to even (the exact quotient); a row with an inf or NaN gets
+ * scale NaN and codes 0.  Columns K .. Kp - 1 of codes are written (0). */
+int t2t_int8_quantize(const void* x, int dtype, long long row_stride, void* codes,
+                      long long code_stride, float* scales, int M, int K, void* stream);
+/* code * scale, rounded once -> out [M, K] fp16 / bf16. */
+int t2t_int8_dequantize(const void* codes, long long code_stride, const float* scales, void* out,
+                        int dtype, long long row_stride, int M, int K, void* stream);
+/* out [M, N] (dtype) = act((sum_k A W) w_scales[n] a_scales[m] + bias[n]): A [M, K]
+ * and W [N, K] in 8 bits, bias [N] in dtype or NULL, act as for MXFP4; sums in
+ * 32-bit integers (exact), the rest in fp32, rounded once.  Row m of out at m *
+ * out_row_stride. */
+int t2t_int8_product(const void* a_codes, long long a_stride, const float* a_scales,
+                     const void* w_codes, long long w_stride, const float* w_scales,
+                     const void* bias, int act, void* out, int dtype, long long out_row_stride,
+                     int M, int N, int K, void* stream);
+/* t2t_int8_quantize of x into the workspace and t2t_int8_product.  out and ws
+ * share no memory with another argument. */
+size_t t2t_int8_linear_ws_bytes(int M, int N, int K);
+int t2t_int8_linear(const void* x, int dtype, long long x_row_stride, const void* w_codes,
+                    long long w_stride, const float* w_scales, const void* bias, int act, void* out,
+                    long long out_row_stride, int M, int N, int K, void* ws, size_t ws_bytes,
+                    void* stream);
+
+/* ---- paged cache of keys and values -------------------------------------- */
+/* Keys and values in pages of page_size tokens: element (page, in, head, d) of
+ * k and v at page kv_page + in kv_row + head kv_head + d (elements).  Slot
+ * page page_size + in is a token's place.  No counterpart in the reference.
+ *
+ * Append of T tokens in one launch: k [T, Hk, D], normed and rotated as by
+ * t2t_rotary (k->out: the cache's keys; out_batch, out_row and out_head: kv_page,
+ * kv_row and kv_head), and v (v->out likewise, no norm, weight unused) into the
+ * tokens' slots [T] (int32 or int64, slot_bits); a token whose slot lies outside
+ * [0, pages * page_size) is stored nowhere.  Slots inside must be distinct.  q (or
+ * NULL) [T, Hq, D] is normed and rotated into q->out.  x_batch is unused.  cosv,
+ * sinv [T, R / 2] fp32; dtype, D, R, layout, norm and eps as in t2t_rotary. */
+int t2t_cache_append(const t2t_rotary_tensor* q, const t2t_rotary_tensor* k,
+                     const t2t_rotary_tensor* v, int dtype, const float* cosv, const float* sinv,
+                     const void* slots, int slot_bits, int pages, int page_size, long long T, int D,
+                     int R, int layout, int norm, float eps, void* stream);
+/* Attention of new tokens over the keys of their sequences, the new ones among
+ * them (append first): sequence b has lengths[b] keys, at positions j of page
+ * table[b table_row + j / page_size].  Its n rows of q are its last n tokens:
+ * without offsets rows [B, N], n = N; with offsets [B + 1] rows offsets[b] ..
+ * offsets[b + 1] - 1 of N in all (rows behind the last sequence are left as they
+ * were).  out = softmax(scale q k^T) v per head; query head h reads key head h /
+ * (HQ / HK).  A row sees all older keys, and of the n new ones all; with causal
+ * those up to itself; with mask (one byte each, row i at i mask_row bytes, in
+ * sequence b without offsets at b mask_batch + i mask_row) those whose byte is not
+ * 0 (none from mask_cols on).  Rows that see nothing are zeros.  Lengths are held
+ * to [0, width page_size]; keys under table entries outside [0, pages) are left
+ * out; hidden keys and what is past the length have no part whatever they hold.
+ * lse (or NULL) [rows, HQ] fp32 contiguous: natural log of the softmax's sum, -inf
+ * for rows that see nothing.  fp16 or bf16, D 64 or 128, all strides multiples of
+ * 8 elements and pointers 16-byte aligned, one head's keys within 64 GiB; sums and
+ * softmax in fp32, weights rounded to the type for the second product.  out and ws
+ * share no memory with another argument. */
+typedef struct t2t_cache_attention_args {
+  size_t struct_bytes; /* sizeof(t2t_cache_attention_args) */
+  const void *q, *k, *v;
+  void* out;
+  float* lse;
+  const int32_t *table, *lengths, *offsets;
+  const uint8_t* mask;
+  long long q_batch, q_row, q_head, out_batch, out_row, out_head, kv_page, kv_row, kv_head;
+  long long table_row, mask_batch, mask_row;
+  int B, N, HQ, HK, D, dtype, pages, page_size, width, mask_cols, causal;
+  float scale;
+} t2t_cache_attention_args;
+/* T: rows of q in all; keys: width * page_size.  (With less, or none, a long
+ * sequence's keys go to fewer work-groups.) */
+size_t t2t_cache_attention_ws_bytes(int ragged, int B, long long T, int HQ, int HK, int D,
+                                    long long keys);
+int t2t_cache_attention(const t2t_cache_attention_args* args, void* ws, size_t ws_bytes,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -42,6 +42,19 @@ class RotaryTensor(ctypes.Structure):
                 + [("weight", _P), ("heads", c_int)])
 
 
+class CacheAttentionArgs(ctypes.Structure):
+    """t2t_cache_attention_args of include/t2t_hip.h."""
+    _fields_ = ([("struct_bytes", c_size_t)]
+                + [(n, _P) for n in ("q", "k", "v", "out", "lse", "table", "lengths", "offsets", "mask")]
+                + [(f"{t}_{s}", c_longlong) for t, ss in (
+                    ("q", ("batch", "row", "head")), ("out", ("batch", "row", "head")),
+                    ("kv", ("page", "row", "head")), ("table", ("row",)), ("mask", ("batch", "row")))
+                   for s in ss]
+                + [(n, c_int) for n in ("B", "N", "HQ", "HK", "D", "dtype", "pages", "page_size", "width",
+                                        "mask_cols", "causal")]
+                + [("scale", c_float)])
+
+
 # the stages of t2t_step, in order
 (STEP_PROJECT_Q, STEP_PROJECT_K, STEP_KMEANS, STEP_VSTATS, STEP_FINALIZE, STEP_SELECT,
  STEP_GATHER_K, STEP_PLAN, STEP_EXACT, STEP_TILES, STEP_RESIDUAL) = (1 << i for i in range(11))
@@ -142,6 +155,18 @@ SIGNATURES = {
     "t2t_mxfp4_linear_ws_bytes": (c_size_t, [c_int, c_int, c_int]),
     "t2t_mxfp4_linear": (c_int, [_P, c_int, c_longlong, _P, _P, _P, c_int, _P, c_longlong, c_int, c_int,
                                  c_int, _P, c_size_t, _P]),
+    "t2t_int8_row_bytes": (c_size_t, [c_int]),
+    "t2t_int8_quantize": (c_int, [_P, c_int, c_longlong, _P, c_longlong, _P, c_int, c_int, _P]),
+    "t2t_int8_dequantize": (c_int, [_P, c_longlong, _P, _P, c_int, c_longlong, c_int, c_int, _P]),
+    "t2t_int8_product": (c_int, [_P, c_longlong, _P, _P, c_longlong, _P, _P, c_int, _P, c_int, c_longlong,
+                                 c_int, c_int, c_int, _P]),
+    "t2t_int8_linear_ws_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "t2t_int8_linear": (c_int, [_P, c_int, c_longlong, _P, c_longlong, _P, _P, c_int, _P, c_longlong, c_int,
+                                c_int, c_int, _P, c_size_t, _P]),
+    "t2t_cache_append": (c_int, [ctypes.POINTER(RotaryTensor)] * 3 + [c_int, _P, _P, _P, c_int, c_int, c_int,
+                                                                     c_longlong] + [c_int] * 4 + [c_float, _P]),
+    "t2t_cache_attention_ws_bytes": (c_size_t, [c_int, c_int, c_longlong, c_int, c_int, c_int, c_longlong]),
+    "t2t_cache_attention": (c_int, [ctypes.POINTER(CacheAttentionArgs), _P, c_size_t, _P]),
 }
 
 _lib = None

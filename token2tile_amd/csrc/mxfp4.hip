@@ -13,7 +13,7 @@
 //           group g: the block of row l % 32, columns 256 g + 64 j + 32 (l / 32)
 // Rows past M and columns past K hold zero codes and zero scale bytes (a zero
 // code under a scale of 255, which stands for NaN, would be NaN).
-#include "t2t_common.h"
+#include "t2t_linear.h"
 #include <type_traits>
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -224,13 +224,6 @@ __device__ inline f32x16 mx_mfma(const u32x4& a, const u32x4& b, const f32x16& c
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, c, 4, 4, S, (int)sa, S, (int)sb);
 }
 
-// gelu(x) = x / 2 (1 + tanh u) = x / (1 + e^(-2 u)), u = sqrt(2 / pi) (x + 0.044715 x^3), with the
-// constants of e^(-2 u) = 2^(x (c0 + c1 x^2)).  v_exp_f32 and v_rcp_f32 are within 1 ulp.
-__device__ inline float mx_gelu(float x) {
-  const float z = x * __builtin_fmaf(-0.10294324f, x * x, -2.3022082f);
-  return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z));
-}
-
 struct MxMat {
   const char* codes;
   const uint32_t* scales;
@@ -244,29 +237,11 @@ struct MxMat {
 // fragments: both the DMA and the fragment reads are linear (no conflicts, no
 // address arithmetic).  A stage is 128 columns (two fragments a row block) and
 // four stages are kept, so a stage's loads have the time of three to land.
-typedef __attribute__((address_space(3))) void mx_lds_t;
-typedef __attribute__((address_space(1))) void mx_glb_t;
-
 template <int TW, int TA> struct MxTile {
   static constexpr int RB = 2 * (TW + TA);          // row blocks: 2 TW of weights, 2 TA of tokens
   static constexpr int CODES = RB * 2048;           // a stage's codes
   static constexpr int STAGE = CODES + RB * 256;    // with its scales (of every second stage)
 };
-
-// Consecutive work-groups go to the eight XCDs in turn: each takes a run of
-// tiles, eight token tiles by all feature tiles, so that the 32 tiles an XCD
-// has under way share their panels in its L2.
-__device__ inline int mx_first(int per_xcd) { return (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3); }
-__device__ inline int mx_end(int mt, int nt, int per_xcd) {
-  return min(mt * nt, ((int)(blockIdx.x & 7) + 1) * per_xcd);
-}
-// a tile's first row blocks
-__device__ inline void mx_place(int id, int mt, int nt, int mb, int nb, int& m0, int& n0) {
-  const int grp = id / (8 * nt), in = id - grp * 8 * nt;
-  const int gm = min(8, mt - grp * 8);
-  m0 = (grp * 8 + in % gm) * mb;
-  n0 = (in / gm) * nb;
-}
 
 // The sums start at the bias, which comes through LDS of the wave's own (128 TW bytes): a lane needs
 // 16 TW of the wave's 32 TW features.
@@ -295,18 +270,6 @@ __device__ inline void mx_start(f32x16 (&acc)[TW][TA], const uint16_t* __restric
   }
 }
 
-// The values of one row, the first n of which are inside, to an o of any alignment (rows of odd
-// widths: the store takes 16 bytes at any address, two at a time it cost 16 us at 4099 x 2041)
-template <typename VT>
-__device__ inline void mx_put(uint16_t* o, const VT& v, int n) {
-  if (n >= (int)sizeof(VT) / 2)
-    __builtin_memcpy(o, &v, sizeof(VT));
-  else
-#pragma unroll
-    for (int e = 0; e < (int)sizeof(VT) / 2; ++e)
-      if (e < n) o[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
-}
-
 // A wave's 32 TA tokens from m on, 32 TW features from n on: 32 tokens x 64 features at a time are
 // packed, turned through 4 KB of LDS of the wave's own (16-byte chunk c of token t at c ^ (t & 7)) and
 // stored as rows, a step behind, so that the reads have the next step's packing to land.  (DS
@@ -330,7 +293,7 @@ __device__ inline void mx_store(const f32x16 (&acc)[TW][TA], char* so, uint16_t*
         if constexpr (VEC)
           *(u32x4*)(o + lane_at) = v[r];
         else
-          mx_put(o + lane_at, v[r], left);
+          lin_put(o + lane_at, v[r], left);
       }
     }
   };
@@ -345,7 +308,7 @@ __device__ inline void mx_store(const f32x16 (&acc)[TW][TA], char* so, uint16_t*
         float f[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          f[e] = GELU ? mx_gelu(acc[ii + i][j][4 * q + e]) : acc[ii + i][j][4 * q + e];
+          f[e] = GELU ? lin_gelu(acc[ii + i][j][4 * q + e]) : acc[ii + i][j][4 * q + e];
         *(u32x2*)(so + (lane & 31) * 128 + (((4 * i + q) ^ (lane & 7)) * 16) + 8 * hh) =
             u32x2{Pk<T>::pack(f[0], f[1]), Pk<T>::pack(f[2], f[3])};
       }
@@ -495,10 +458,10 @@ __global__ __launch_bounds__(256, 1) void mx_big_kernel(MxMat a, MxMat w, const 
   __shared__ __attribute__((aligned(1024))) char lds[4 * ST + 4 * 4096];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wn = wave & 1, wm = wave >> 1;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(mx_lds_t*)lds, l16 = lane * 16;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lin_lds_t*)lds, l16 = lane * 16;
   const int n = 2 * groups, step = gridDim.x >> 3;
-  int id = mx_first(per_xcd);
-  const int end = mx_end(mt, nt, per_xcd);
+  int id = lin_first(per_xcd);
+  const int end = lin_end(mt, nt, per_xcd);
   if (id >= end) return;
 
   // the stream of stages: tile ld, its stage ls
@@ -506,7 +469,7 @@ __global__ __launch_bounds__(256, 1) void mx_big_kernel(MxMat a, MxMat w, const 
   int ld = id, ls = 0;
   auto aim = [&]() {
     int m0, n0;
-    mx_place(ld, mt, nt, 8, 8, m0, n0);
+    lin_place(ld, mt, nt, 8, 8, m0, n0);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int rb = wave * 4 + (i >> 1);
@@ -572,7 +535,7 @@ __global__ __launch_bounds__(256, 1) void mx_big_kernel(MxMat a, MxMat w, const 
   f32x16 acc[4][4];
   for (;;) {
     int m0, n0;
-    mx_place(id, mt, nt, 8, 8, m0, n0);
+    lin_place(id, mt, nt, 8, 8, m0, n0);
     mx_start<T>(acc, bias, (float*)own, (n0 + wn * 4) * 32, w.rows);
     for (int g = groups; g > 0; --g) {
       const uint32_t other = PAIR - 2 * off;  // from this pair to the other one (off: 0 or PAIR)
@@ -660,13 +623,13 @@ __global__ __launch_bounds__(256, 2) void mx_mid_kernel(MxMat a, MxMat w, const 
   constexpr int ST = C::STAGE, PAIR = 2 * ST;
   __shared__ __attribute__((aligned(1024))) char lds[4 * ST];
   __shared__ __attribute__((aligned(16))) float sbias[4][64];
-  const int id = mx_first(per_xcd);
-  if (id >= mx_end(mt, nt, per_xcd)) return;
+  const int id = lin_first(per_xcd);
+  if (id >= lin_end(mt, nt, per_xcd)) return;
   int m0, n0;
-  mx_place(id, mt, nt, 4, 4, m0, n0);
+  lin_place(id, mt, nt, 4, 4, m0, n0);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wn = wave & 1, wm = wave >> 1, n = 2 * groups;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(mx_lds_t*)lds, l16 = lane * 16;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lin_lds_t*)lds, l16 = lane * 16;
   const char* g[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -759,10 +722,10 @@ __global__ __launch_bounds__(512) void mx_split_kernel(MxSrc a, MxMat w, const u
   __shared__ f32x4 part[WAVES][4][64];
   __shared__ u32x4 xc[X16 ? MX_X16_BLOCKS : 1];
   __shared__ uint8_t xs[X16 ? MX_X16_BLOCKS : 1];
-  const int id = mx_first(per_xcd);
-  if (id >= mx_end(mt, nt, per_xcd)) return;
+  const int id = lin_first(per_xcd);
+  if (id >= lin_end(mt, nt, per_xcd)) return;
   int mb, nb;
-  mx_place(id, mt, nt, 1, 1, mb, nb);
+  lin_place(id, mt, nt, 1, 1, mb, nb);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = 2 * groups;
   const char* pw = w.codes + (long long)nb * groups * 4096;
@@ -846,9 +809,9 @@ __global__ __launch_bounds__(512) void mx_split_kernel(MxSrc a, MxMat w, const u
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if (bias) v[e] += T::to_f(bias[min(f + e, w.rows - 1)]);
-      if (GELU) v[e] = mx_gelu(v[e]);
+      if (GELU) v[e] = lin_gelu(v[e]);
     }
-    mx_put(out + row * ldo + f, u32x2{Pk<T>::pack(v[0], v[1]), Pk<T>::pack(v[2], v[3])}, w.rows - f);
+    lin_put(out + row * ldo + f, u32x2{Pk<T>::pack(v[0], v[1]), Pk<T>::pack(v[2], v[3])}, w.rows - f);
   }
 }
 

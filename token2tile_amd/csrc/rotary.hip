@@ -1,6 +1,7 @@
 // Rotary positions: the cos / sin tables of a set of positions, and the
 // rotation of q and k with the RMS norm that stands before it.
 #include "t2t_common.h"
+#include <type_traits>
 
 // ---------------------------------------------------------------------------
 // cos[t, i] = m cos(p[t, a] f[i]), sin likewise; pair i belongs to the axis a
@@ -198,11 +199,64 @@ __device__ inline typename RopeVec<V>::type rope_pack(const float (&f)[V]) {
   return v;
 }
 
+// ---- into a paged cache ------------------------------------------------------
+// The forms with SLOTS are those of an append: the first tensor's rows go to their slots (its out
+// strides are the cache's), the second, if any, is an ordinary one, and the grid's last row of
+// work-groups stores v.
+struct RopeSlots {
+  const void* slots;
+  int wide;               // 64-bit slots
+  int page;
+  unsigned long long all;  // slots there are
+  t2t_rotary_tensor v;
+  // the place of a token's row; false where it has none
+  __device__ bool place(long long tok, long long out_batch, long long out_row, long long& at) const {
+    const unsigned long long s = wide ? (unsigned long long)((const long long*)slots)[tok]
+                                      : (unsigned long long)(long long)((const int32_t*)slots)[tok];
+    if (s >= all) return false;
+    // (fewer than 2^32 in nearly every cache: a division of 32 bits)
+    const long long p = all >> 32 ? (long long)(s / page) : (long long)((uint32_t)s / (uint32_t)page);
+    at = p * out_batch + ((long long)s - p * page) * out_row;
+    return true;
+  }
+};
+// v [T, H, D] into its slots, V channels a thread
+template <int V>
+__device__ inline void rope_store_v(const RopeSlots& S, long long tokens, int D) {
+  const t2t_rotary_tensor& g = S.v;
+  const int per_head = D / V, per = per_head * g.heads;
+  const long long units = tokens * per, step = (long long)gridDim.x * 256;
+  for (long long u0 = (long long)blockIdx.x * 256 + threadIdx.x; u0 < units; u0 += 4 * step) {
+    typedef uint16_t vec __attribute__((ext_vector_type(V)));
+    vec x[4];
+    long long at[4];
+    bool on[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long long u = u0 + i * step;
+      on[i] = u < units;
+      const long long tok = on[i] ? u / per : 0;
+      const int in = on[i] ? (int)(u - tok * per) : 0, h = in / per_head, c = (in - h * per_head) * V;
+      on[i] = on[i] && S.place(tok, g.out_batch, g.out_row, at[i]);
+      if (!on[i]) continue;
+      at[i] += h * g.out_head + c;
+      x[i] = *(const vec*)((const uint16_t*)g.x + tok * g.x_row + h * g.x_head + c);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (on[i]) *(vec*)((uint16_t*)g.out + at[i]) = x[i];
+  }
+}
+
 // NORM as T2T_NORM_*.  WPT waves to a token: 1, or 4 under the token norm where the tokens are few
 // or a wave's registers do not hold their heads.
-template <typename T, int NORM, int WPT, int ITS, int V>
-__global__ __launch_bounds__(256) void rotary_kernel(t2t_rotary_tensor q, t2t_rotary_tensor k, RotaryArgs A) {
+template <typename T, int NORM, int WPT, int ITS, int V, typename SLOTS>
+__global__ __launch_bounds__(256) void rotary_kernel(t2t_rotary_tensor q, t2t_rotary_tensor k, RotaryArgs A,
+                                                     SLOTS slots) {
   typedef typename RopeVec<V>::type vec;
+  constexpr bool APPEND = std::is_same<SLOTS, RopeSlots>::value;
+  if constexpr (APPEND)
+    if (blockIdx.y + 1 == gridDim.y) return rope_store_v<V>(slots, A.tokens, A.D);
   const t2t_rotary_tensor& g = blockIdx.y ? k : q;
   __shared__ double part[4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -244,10 +298,16 @@ __global__ __launch_bounds__(256) void rotary_kernel(t2t_rotary_tensor q, t2t_ro
     const long long group = chunks == 1 ? item : item / chunks;
     const int first = WPT == 1 ? (int)(item - group * chunks) * ITS * per : wave * per;  // the wave's heads
     const long long tok = (group << (6 - span)) + slot;
-    const bool live = tok < A.tokens;
+    bool live = tok < A.tokens;
     const uint32_t t32 = (uint32_t)(live ? tok : A.tokens - 1), b = t32 / (uint32_t)A.N, n = t32 - b * A.N;
     const uint16_t* x = (const uint16_t*)g.x + b * g.x_batch + n * g.x_row;
     uint16_t* o = (uint16_t*)g.out + b * g.out_batch + n * g.out_row;
+    if constexpr (APPEND)
+      if (blockIdx.y == 0) {
+        long long at = 0;
+        live = slots.place(t32, g.out_batch, g.out_row, at) && live;
+        o = (uint16_t*)g.out + at;
+      }
     float cs[V], sn[V];
     {
       const long long row = (b * A.table_batch + n) * (A.R / 2) + V * u;
@@ -359,9 +419,12 @@ __device__ inline double rope_head_squares(const uint16_t* x, int D, int lane) {
 
 // Any strides, widths and alignment: one work-group per token and tensor, pair by pair, a wave to
 // a head; the token norm's sum comes first.
-template <typename T>
+template <typename T, typename SLOTS>
 __global__ __launch_bounds__(256) void rotary_any_kernel(t2t_rotary_tensor q, t2t_rotary_tensor k,
-                                                         RotaryArgs A, int norm) {
+                                                         RotaryArgs A, int norm, SLOTS slots) {
+  constexpr bool APPEND = std::is_same<SLOTS, RopeSlots>::value;
+  if constexpr (APPEND)
+    if (blockIdx.y + 1 == gridDim.y) return rope_store_v<1>(slots, A.tokens, A.D);
   const t2t_rotary_tensor& g = blockIdx.y ? k : q;
   __shared__ double part[4];
   const int D = A.D, R = A.R;
@@ -369,6 +432,12 @@ __global__ __launch_bounds__(256) void rotary_any_kernel(t2t_rotary_tensor q, t2
     const int b = (int)(tok / A.N), n = (int)(tok - (long long)b * A.N);
     const uint16_t* x = (const uint16_t*)g.x + b * g.x_batch + n * g.x_row;
     uint16_t* o = (uint16_t*)g.out + b * g.out_batch + n * g.out_row;
+    if constexpr (APPEND)
+      if (blockIdx.y == 0) {
+        long long at = 0;
+        if (!slots.place(tok, g.out_batch, g.out_row, at)) continue;  // (the same for the work-group)
+        o = (uint16_t*)g.out + at;
+      }
     const uint16_t* w = (const uint16_t*)g.weight;
     const float* c = A.cosv + (b * A.table_batch + n) * (R / 2);
     const float* s = A.sinv + (b * A.table_batch + n) * (R / 2);
@@ -420,9 +489,14 @@ static bool rope_vectors(const t2t_rotary_tensor& t, bool weight, int V) {
          (((uintptr_t)t.x | (uintptr_t)t.out | (weight ? (uintptr_t)t.weight : 0)) & (2 * V - 1)) == 0;
 }
 
-template <typename T, int NORM, int WPT, int ITS, int V>
+struct RopeInPlace {};  // an ordinary call: no slots
+template <typename SLOTS> static constexpr int rope_rows(int tensors) {
+  return tensors + std::is_same<SLOTS, RopeSlots>::value;
+}
+
+template <typename T, int NORM, int WPT, int ITS, int V, typename SLOTS>
 static void rope_launch(const t2t_rotary_tensor& q, const t2t_rotary_tensor& k, const RotaryArgs& A, int tensors,
-                        hipStream_t st) {
+                        hipStream_t st, const SLOTS& slots) {
   long long items = 0;
   for (int i = 0; i < tensors; ++i) {
     const int span = A.shift + A.hshift[i];
@@ -433,14 +507,16 @@ static void rope_launch(const t2t_rotary_tensor& q, const t2t_rotary_tensor& k, 
   // evenly several items a work-group from 16,384 of them on, so that the weights are read once for
   // several tokens (75,600 tokens of 40 + 40 heads: two each 578 us, one 599, up to five 590)
   const long long turns = (wgs + 16383) / 16384, grid = (wgs + turns - 1) / turns;
-  hipLaunchKernelGGL((rotary_kernel<T, NORM, WPT, ITS, V>), dim3((unsigned)grid, tensors), dim3(256), 0, st, q, k,
-                     A);
+  hipLaunchKernelGGL((rotary_kernel<T, NORM, WPT, ITS, V, SLOTS>), dim3((unsigned)grid, rope_rows<SLOTS>(tensors)),
+                     dim3(256), 0, st, q, k, A, slots);
 }
 
 // the vector kernel, if it takes the call
-template <typename T, int V>
+template <typename T, int V, typename SLOTS>
 static bool rope_vector_run(const t2t_rotary_tensor& q, const t2t_rotary_tensor& k, RotaryArgs A, int norm,
-                            int tensors, hipStream_t st) {
+                            int tensors, hipStream_t st, const SLOTS& slots) {
+  if constexpr (std::is_same<SLOTS, RopeSlots>::value)
+    if (!rope_vectors(slots.v, false, V)) return false;
   if (A.D % V || A.R % (A.half ? 2 * V : V) || !rope_vectors(q, norm, V) ||
       (tensors == 2 && !rope_vectors(k, norm, V)) || (((uintptr_t)A.cosv | (uintptr_t)A.sinv) & (2 * V - 1)))
     return false;
@@ -460,19 +536,19 @@ static bool rope_vector_run(const t2t_rotary_tensor& q, const t2t_rotary_tensor&
     // waves 28)
     if (A.tokens >= 1024 && its <= 5) {
       switch (its) {
-        case 1: rope_launch<T, T2T_NORM_TOKEN, 1, 1, V>(q, k, A, tensors, st); return true;
-        case 2: rope_launch<T, T2T_NORM_TOKEN, 1, 2, V>(q, k, A, tensors, st); return true;
-        case 3: rope_launch<T, T2T_NORM_TOKEN, 1, 3, V>(q, k, A, tensors, st); return true;
-        case 4: rope_launch<T, T2T_NORM_TOKEN, 1, 4, V>(q, k, A, tensors, st); return true;
-        default: rope_launch<T, T2T_NORM_TOKEN, 1, 5, V>(q, k, A, tensors, st); return true;
+        case 1: rope_launch<T, T2T_NORM_TOKEN, 1, 1, V>(q, k, A, tensors, st, slots); return true;
+        case 2: rope_launch<T, T2T_NORM_TOKEN, 1, 2, V>(q, k, A, tensors, st, slots); return true;
+        case 3: rope_launch<T, T2T_NORM_TOKEN, 1, 3, V>(q, k, A, tensors, st, slots); return true;
+        case 4: rope_launch<T, T2T_NORM_TOKEN, 1, 4, V>(q, k, A, tensors, st, slots); return true;
+        default: rope_launch<T, T2T_NORM_TOKEN, 1, 5, V>(q, k, A, tensors, st, slots); return true;
       }
     }
     A.hshift[0] = A.hshift[1] = 6 - A.shift;
     its = cdiv(max(heads[0], tensors == 2 ? heads[1] : 0), 4 << (6 - A.shift));
-    if (its <= 1) rope_launch<T, T2T_NORM_TOKEN, 4, 1, V>(q, k, A, tensors, st);
-    else if (its <= 2) rope_launch<T, T2T_NORM_TOKEN, 4, 2, V>(q, k, A, tensors, st);
-    else if (its <= 4) rope_launch<T, T2T_NORM_TOKEN, 4, 4, V>(q, k, A, tensors, st);
-    else if (its <= 8) rope_launch<T, T2T_NORM_TOKEN, 4, 8, V>(q, k, A, tensors, st);
+    if (its <= 1) rope_launch<T, T2T_NORM_TOKEN, 4, 1, V>(q, k, A, tensors, st, slots);
+    else if (its <= 2) rope_launch<T, T2T_NORM_TOKEN, 4, 2, V>(q, k, A, tensors, st, slots);
+    else if (its <= 4) rope_launch<T, T2T_NORM_TOKEN, 4, 4, V>(q, k, A, tensors, st, slots);
+    else if (its <= 8) rope_launch<T, T2T_NORM_TOKEN, 4, 8, V>(q, k, A, tensors, st, slots);
     return its <= 8;
   }
   // heads on their own: up to four rounds an item (table entries serve them all), one where the items
@@ -480,24 +556,26 @@ static bool rope_vector_run(const t2t_rotary_tensor& q, const t2t_rotary_tensor&
   const int r = its >= 4 ? 4 : its >= 2 ? 2 : 1, rounds = A.tokens * cdiv(its, r) < 8192 ? 1 : r;
   for (int i = 0; i < tensors; ++i) A.chunks[i] = cdiv(heads[i], rounds << A.hshift[i]);
   if (norm == T2T_NORM_HEAD) {
-    if (rounds == 4) rope_launch<T, T2T_NORM_HEAD, 1, 4, V>(q, k, A, tensors, st);
-    else if (rounds == 2) rope_launch<T, T2T_NORM_HEAD, 1, 2, V>(q, k, A, tensors, st);
-    else rope_launch<T, T2T_NORM_HEAD, 1, 1, V>(q, k, A, tensors, st);
+    if (rounds == 4) rope_launch<T, T2T_NORM_HEAD, 1, 4, V>(q, k, A, tensors, st, slots);
+    else if (rounds == 2) rope_launch<T, T2T_NORM_HEAD, 1, 2, V>(q, k, A, tensors, st, slots);
+    else rope_launch<T, T2T_NORM_HEAD, 1, 1, V>(q, k, A, tensors, st, slots);
   } else {
-    if (rounds == 4) rope_launch<T, T2T_NORM_NONE, 1, 4, V>(q, k, A, tensors, st);
-    else if (rounds == 2) rope_launch<T, T2T_NORM_NONE, 1, 2, V>(q, k, A, tensors, st);
-    else rope_launch<T, T2T_NORM_NONE, 1, 1, V>(q, k, A, tensors, st);
+    if (rounds == 4) rope_launch<T, T2T_NORM_NONE, 1, 4, V>(q, k, A, tensors, st, slots);
+    else if (rounds == 2) rope_launch<T, T2T_NORM_NONE, 1, 2, V>(q, k, A, tensors, st, slots);
+    else rope_launch<T, T2T_NORM_NONE, 1, 1, V>(q, k, A, tensors, st, slots);
   }
   return true;
 }
 
-template <typename T>
+template <typename T, typename SLOTS>
 static void rope_run(const t2t_rotary_tensor& q, const t2t_rotary_tensor& k, const RotaryArgs& A, int norm,
-                     int tensors, hipStream_t st) {
-  if (rope_vector_run<T, 8>(q, k, A, norm, tensors, st) || rope_vector_run<T, 4>(q, k, A, norm, tensors, st))
+                     int tensors, hipStream_t st, const SLOTS& slots) {
+  if (rope_vector_run<T, 8>(q, k, A, norm, tensors, st, slots) ||
+      rope_vector_run<T, 4>(q, k, A, norm, tensors, st, slots))
     return;
-  hipLaunchKernelGGL(rotary_any_kernel<T>, dim3((unsigned)(A.tokens < 65536 ? A.tokens : 65536), tensors),
-                     dim3(256), 0, st, q, k, A, norm);
+  hipLaunchKernelGGL((rotary_any_kernel<T, SLOTS>),
+                     dim3((unsigned)(A.tokens < 65536 ? A.tokens : 65536), rope_rows<SLOTS>(tensors)), dim3(256), 0,
+                     st, q, k, A, norm, slots);
 }
 
 extern "C" int t2t_rotary(const t2t_rotary_tensor* q, const t2t_rotary_tensor* k, int dtype,
@@ -526,9 +604,49 @@ extern "C" int t2t_rotary(const t2t_rotary_tensor* q, const t2t_rotary_tensor* k
   A.half = layout == T2T_ROPE_HALF;
   A.sign = inverse ? -1.f : 1.f, A.eps = eps;
   if (dtype == T2T_BF16)
-    rope_run<BF16T>(*ts[0], *ts[1], A, norm, k ? 2 : 1, (hipStream_t)stream);
+    rope_run<BF16T>(*ts[0], *ts[1], A, norm, k ? 2 : 1, (hipStream_t)stream, RopeInPlace{});
   else
-    rope_run<F16T>(*ts[0], *ts[1], A, norm, k ? 2 : 1, (hipStream_t)stream);
+    rope_run<F16T>(*ts[0], *ts[1], A, norm, k ? 2 : 1, (hipStream_t)stream, RopeInPlace{});
   T2T_LAUNCH_CHECK("rotary");
+  return T2T_OK;
+}
+
+extern "C" int t2t_cache_append(const t2t_rotary_tensor* q, const t2t_rotary_tensor* k, const t2t_rotary_tensor* v,
+                                int dtype, const float* cosv, const float* sinv, const void* slots, int slot_bits,
+                                int pages, int page_size, long long T, int D, int R, int layout, int norm, float eps,
+                                void* stream) {
+  T2T_REQUIRE(k && v, "cache_append: null pointer");
+  T2T_REQUIRE(dtype == T2T_F16 || dtype == T2T_BF16, "cache_append: dtype %d", dtype);
+  T2T_REQUIRE(slot_bits == 32 || slot_bits == 64, "cache_append: slots of %d bits", slot_bits);
+  T2T_REQUIRE(pages >= 1 && page_size >= 1, "cache_append: %d pages of %d", pages, page_size);
+  T2T_REQUIRE(T >= 0 && T <= INT_MAX, "cache_append: T=%lld", T);
+  T2T_REQUIRE(D >= 1 && D <= 256 && R >= 2 && R <= D && R % 2 == 0,
+              "cache_append: D=%d R=%d (1 <= D <= 256, R even, 2 <= R <= D)", D, R);
+  T2T_REQUIRE(layout == T2T_ROPE_INTERLEAVED || layout == T2T_ROPE_HALF, "cache_append: layout %d", layout);
+  T2T_REQUIRE(norm >= T2T_NORM_NONE && norm <= T2T_NORM_HEAD, "cache_append: norm %d", norm);
+  const t2t_rotary_tensor* ts[3] = {k, v, q ? q : k};
+  for (int i = 0; i < 3; ++i) {
+    T2T_REQUIRE(ts[i]->heads >= 1 && ts[i]->heads <= 65536, "cache_append: heads=%d", ts[i]->heads);
+    T2T_REQUIRE(!norm || i == 1 || ts[i]->weight, "cache_append: the norm needs a weight");
+  }
+  T2T_REQUIRE(k->heads == v->heads, "cache_append: %d heads of keys, %d of values", k->heads, v->heads);
+  if (T == 0) return T2T_OK;
+  T2T_REQUIRE(cosv && sinv && slots, "cache_append: null pointer");
+  for (int i = 0; i < 3; ++i) T2T_REQUIRE(ts[i]->x && ts[i]->out, "cache_append: null pointer");
+  t2t_rotary_tensor kt = *k, qt = q ? *q : *k;
+  kt.x_batch = 0, qt.x_batch = 0;  // one sequence
+  if (q) qt.out_batch = 0;
+  RotaryArgs A{};
+  A.cosv = cosv, A.sinv = sinv;
+  A.tokens = T, A.N = (int)T, A.D = D, A.R = R;
+  A.half = layout == T2T_ROPE_HALF;
+  A.sign = 1.f, A.eps = eps;
+  RopeSlots S{slots, slot_bits == 64, page_size, (unsigned long long)pages * page_size, *v};
+  S.v.x_batch = 0;
+  if (dtype == T2T_BF16)
+    rope_run<BF16T>(kt, qt, A, norm, q ? 2 : 1, (hipStream_t)stream, S);
+  else
+    rope_run<F16T>(kt, qt, A, norm, q ? 2 : 1, (hipStream_t)stream, S);
+  T2T_LAUNCH_CHECK("cache_append");
   return T2T_OK;
 }

@@ -1257,3 +1257,435 @@ def mxfp4_linear(x, weight, bias=None, *, activation=None, dtype=None, out=None,
                 code, stride, *args, ostride, M, N, K, None if ws is None else ws.data_ptr(),
                 0 if ws is None else ws.numel())
     return out
+
+
+# ---------------------------------------------------------------------------
+# 8-bit linear layers
+# ---------------------------------------------------------------------------
+_I8_MAX_COLS = 2 ** 17 - 1  # the sums stay in 32 bits
+
+
+class Int8:
+    """A matrix [rows, cols] in 8 bits (``int8_quantize``, or the codes and scales of
+    a checkpoint): ``codes`` int8 [rows, cols rounded up to 128] with zeros from
+    column ``cols`` on (which is not checked), rows of contiguous codes, 16-byte
+    aligned; ``scales`` fp32 [rows].  Element (i, j) stands for codes[i, j] *
+    scales[i].  Both are on the GPU and are checked here, once."""
+
+    # (addresses and device are the buffers' at each call: a copied, pickled or loaded matrix has others)
+    __slots__ = ("_codes", "_scales", "_cols")
+
+    def __init__(self, codes, scales, cols=None):
+        dev = _dev(codes)
+        if codes.dtype != torch.int8 or codes.dim() != 2:
+            raise ValueError(f"t2t: codes must be an int8 matrix, got {codes.dtype} {tuple(codes.shape)}")
+        rows, wide = codes.shape
+        cols = wide if cols is None else int(cols)
+        if not (0 <= rows <= 2 ** 30 and 1 <= cols <= _I8_MAX_COLS and wide == _i8_cols(cols)):
+            raise ValueError(f"t2t: {cols} columns (1 to 2^17 - 1) are held as {_i8_cols(max(cols, 1))} with zeros "
+                             f"behind them, got {rows} x {wide}")
+        _check(scales, (rows,), _f32, "scales", dev)
+        stride = codes.stride(0) if rows > 1 else wide
+        if codes.stride(1) != 1 or stride < wide or stride % 16 or codes.data_ptr() % 16:
+            raise ValueError(f"t2t: the rows of codes must be contiguous, 16-byte aligned and apart, got strides "
+                             f"{tuple(codes.stride())}")
+        if rows and _near(*_span(codes), ((scales.data_ptr(), scales.nbytes),)) and _meet(codes, scales):
+            raise ValueError("t2t: scales shares memory with codes")
+        self._set(codes, scales, cols)
+
+    def _set(self, codes, scales, cols):
+        self._codes, self._scales, self._cols = codes, scales, cols
+        return self
+
+    codes = property(lambda self: self._codes)
+    scales = property(lambda self: self._scales)
+    rows = property(lambda self: self._codes.shape[0])
+    cols = property(lambda self: self._cols)
+    shape = property(lambda self: (self._codes.shape[0], self._cols))
+    device = property(lambda self: self._codes.device)
+
+    def __repr__(self):
+        return f"Int8({self.rows} x {self._cols}, {self.device})"
+
+
+def _i8_cols(cols):
+    """Columns that are held (t2t_int8_row_bytes)."""
+    return (cols + 127) & ~127
+
+
+def _i8_args(t):
+    """Addresses and row stride of an Int8 matrix."""
+    codes = t._codes
+    return codes.data_ptr(), codes.stride(0) if codes.shape[0] > 1 else codes.shape[1], t._scales.data_ptr()
+
+
+def _i8_spans(t):
+    p, end = _span(t._codes)
+    return [(p, end - p), (t._scales.data_ptr(), t._scales.nbytes)]
+
+
+def _x_span(x, rows, cols, stride):
+    return x.data_ptr(), 2 * ((rows - 1) * stride + cols)
+
+
+def int8_quantize(x, out=None, stream=None):
+    """x [..., K] (fp16 or bf16, contiguous rows, K < 2^17) in 8 bits, rows
+    flattened.  A row's scale is max|x| / 127 in fp32 (at least 2^-120); codes are
+    the nearest whole multiples, ties to even; a row with an inf or NaN stands for
+    NaN."""
+    dev = _dev(x)
+    _on(stream, dev)
+    M, K, stride = _mx_rows(x, "x", dev, 2)
+    if not (1 <= K <= _I8_MAX_COLS and M <= 2 ** 30):
+        raise ValueError(f"t2t: x must have 1 to 2^17 - 1 columns, got {M} x {K}")
+    if out is None:
+        out = Int8.__new__(Int8)._set(_empty(stream, (M, _i8_cols(K)), torch.int8, dev),
+                                      _empty(stream, (M,), _f32, dev), K)
+    elif not isinstance(out, Int8) or out.shape != (M, K) or _dev(out._codes) != dev:
+        raise ValueError(f"t2t: out must be an Int8 matrix {M} x {K} on {dev}, got {out!r}")
+    elif _near(*_span(x), _i8_spans(out)):
+        _apart((out._codes, out._scales), ("out.codes", "out.scales"), (None, None, x))
+    pc, cs, ps = _i8_args(out)
+    _launch("t2t_int8_quantize", dev, stream, (x, out._codes, out._scales), x.data_ptr(), dtype_code(x.dtype),
+            stride, pc, cs, ps, M, K)
+    return out
+
+
+def int8_dequantize(t, dtype=torch.bfloat16, out=None, stream=None):
+    """The values that an Int8 matrix stands for, [rows, cols] in fp16 or bf16,
+    rounded once."""
+    if not isinstance(t, Int8):
+        raise ValueError("t2t: expected an Int8 matrix")
+    dev = _dev(t._codes)
+    _on(stream, dev)
+    code = _mx_dtype(dtype)
+    if out is None:
+        out = _empty(stream, t.shape, dtype, dev)
+        stride = t._cols
+    else:
+        M, K, stride = _mx_rows(out, "out", dev, 2)
+        if (M, K) != t.shape or out.dtype != dtype:
+            raise ValueError(f"t2t: out must be {dtype} {t.shape}, got {out.dtype} {tuple(out.shape)}")
+        _apart((out,), ("out",), (None, t._codes, t._scales))
+    pc, cs, ps = _i8_args(t)
+    _launch("t2t_int8_dequantize", dev, stream, (t._codes, t._scales, out), pc, cs, ps, out.data_ptr(), code,
+            stride, *t.shape)
+    return out
+
+
+def int8_linear_ws_bytes(M, N, K):
+    """Workspace of int8_linear for a 16-bit x of M rows."""
+    return size_query("t2t_int8_linear_ws_bytes", M, N, K)
+
+
+def int8_linear(x, weight, bias=None, *, activation=None, dtype=None, out=None, ws=None, stream=None):
+    """act(x W^T + bias) with both operands in 8 bits, a scale for each token and
+    channel: x [..., K] fp16 or bf16 (quantised as by int8_quantize; contiguous
+    rows), or an Int8 matrix that several layers share; weight Int8 [N, K]; bias
+    [N] in the output's type.  Integer sums (exact), scales, bias and activation in
+    fp32, one rounding to x's type (``dtype``, default bf16, for an Int8 x) ->
+    [..., N].  ``activation``: None or "gelu_tanh".  ``out``: contiguous rows; it
+    and ``ws`` share no memory with another argument."""
+    if not isinstance(weight, Int8):
+        raise ValueError("t2t: weight must be an Int8 matrix (int8_quantize)")
+    wc, wsc = weight._codes, weight._scales
+    dev = wc.device if wc.is_cuda else _dev(wc)
+    _on(stream, dev)
+    N = wc.shape[0]
+    shared = isinstance(x, Int8)
+    if shared:
+        xs = x._codes, x._scales
+        if xs[0].device != dev:
+            raise ValueError(f"t2t: x must be on {dev}")
+        M, K = x.shape
+        shape = (M, N)
+        dt = torch.bfloat16 if dtype is None else dtype
+        code = _mx_dtype(dt)
+    else:
+        M, K, stride = _mx_rows(x, "x", dev, 2)
+        shape, dt = (*x.shape[:-1], N), x.dtype
+        if dtype not in (None, dt):
+            raise ValueError(f"t2t: the output of a {dt} input is {dt}, not {dtype}")
+        code = dtype_code(dt)
+    if K != weight._cols or N < 1:
+        raise ValueError(f"t2t: x has {K} columns, weight {N} x {weight._cols}")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"t2t: activation {activation!r} (None or gelu_tanh)")
+    if bias is not None and not _is(bias, (N,), dt, dev):
+        _check(bias, (N,), dt, "bias", dev)
+    args = *_i8_args(weight), None if bias is None else bias.data_ptr()
+    spans = None  # of the inputs, where the caller brings an output or a workspace
+    if out is not None or ws is not None:
+        spans = _i8_spans(weight) + [(args[3], 2 * N)] * (bias is not None)
+        spans += _i8_spans(x) if shared else [_x_span(x, M, K, stride)]
+    if out is None:
+        out = _empty(stream, shape, dt, dev) if stream is not None or shared else x.new_empty(shape)
+        ostride, po = N, out.data_ptr()
+    else:
+        ostride = _mx_rows(out, "out", dev, 2)[2]
+        if tuple(out.shape) != shape or out.dtype != dt:
+            raise ValueError(f"t2t: out must be {dt} {shape}, got {out.dtype} {tuple(out.shape)}")
+        po = out.data_ptr()
+        if _near(*_span(out), spans):
+            _apart((out,), ("out",), (None, *(xs if shared else (x,)), wc, wsc, bias))
+    args = *args, _ACTIVATIONS[activation], po
+    if shared:
+        _launch("t2t_int8_product", dev, stream, (*xs, wc, wsc, bias, out), *_i8_args(x), *args, code, ostride,
+                M, N, K)
+    else:
+        need = int8_linear_ws_bytes(M, N, K)
+        if ws is not None:
+            ws = _ws_for(ws, need, dev, stream)
+            at = ws.data_ptr()
+            if need and _near(at, at + need, (*spans, _x_span(out, M, N, ostride))):
+                _apart((ws[:need],), ("ws",), (None, x, wc, wsc, bias, out))
+        elif need:
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if stream is None else _ws(need, dev, stream)
+        _launch("t2t_int8_linear", dev, stream, (x, wc, wsc, bias, out, ws), x.data_ptr(), code, stride, *args,
+                ostride, M, N, K, None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
+    return out
+
+
+# ---------------------------------------------------------------------------
+# paged cache of keys and values
+# ---------------------------------------------------------------------------
+class PagedCache:
+    """Keys and values of tokens in pages: ``k`` and ``v`` fp16 or bf16 [pages,
+    page_size, heads, D], D 64 or 128, of the same strides (multiples of 8;
+    contiguous channels; both may be views of one tensor), 16-byte aligned.  Slot
+    page * page_size + i is row i of a page.  They are checked here, once."""
+
+    __slots__ = ("_k", "_v")
+
+    def __init__(self, k, v):
+        dev = _dev(k)
+        if (k.dtype not in _HALF or k.dim() != 4 or not isinstance(v, torch.Tensor) or v.shape != k.shape
+                or v.dtype != k.dtype or v.device != dev):
+            raise ValueError(f"t2t: k and v must be fp16 or bf16 [pages, page_size, heads, D] tensors of one shape "
+                             f"on {dev}")
+        pages, page, heads, D = k.shape
+        if D not in (64, 128) or not (1 <= pages < 2 ** 31 and 1 <= page < 2 ** 31 and 1 <= heads <= 65536):
+            raise ValueError(f"t2t: a cache of {tuple(k.shape)} (at least one page, row and head, D 64 or 128)")
+        st = _cache_strides(k)
+        if (st != _cache_strides(v) or k.stride(3) != 1 or v.stride(3) != 1 or any(s % 8 for s in st)
+                or (k.data_ptr() | v.data_ptr()) % 16):
+            raise ValueError(f"t2t: k and v must have the same strides, in multiples of 8, contiguous channels and "
+                             f"16-byte alignment, got {tuple(k.stride())} and {tuple(v.stride())}")
+        if (pages - 1) * st[0] + (page - 1) * st[1] >= 2 ** 35:
+            raise ValueError("t2t: one head's keys must span less than 64 GiB")
+        if not (_scattered(k) and _scattered(v)) or _near(*_span(k), ((_span(v)[0], _span(v)[1] - _span(v)[0]),)) \
+                and (_same_view(k, v) or _meet(k, v)):
+            raise ValueError("t2t: the cache holds an element twice")
+        self._k, self._v = k, v
+
+    k = property(lambda self: self._k)
+    v = property(lambda self: self._v)
+    shape = property(lambda self: tuple(self._k.shape))
+    page_size = property(lambda self: self._k.shape[1])
+    device = property(lambda self: self._k.device)
+    dtype = property(lambda self: self._k.dtype)
+
+    def __repr__(self):
+        return f"PagedCache({self.shape}, {self.dtype}, {self.device})"
+
+
+def _cache_strides(t):
+    """Strides of pages, rows and heads (0 where there is one)."""
+    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape))
+
+
+def _cache_of(cache):
+    if not isinstance(cache, PagedCache):
+        raise ValueError("t2t: cache must be a PagedCache")
+    k = cache._k
+    return k, cache._v, k.device if k.is_cuda else _dev(k)
+
+
+def cache_append(q, k, v, cos, sin, cache, slots, *, layout="interleaved", norm=None, q_weight=None,
+                 k_weight=None, eps=1e-6, out=None, stream=None):
+    """New tokens' k, normed and rotated as by ``rotary``, and v into their slots of
+    a PagedCache, and q (or None) normed and rotated, one launch.  Returns the
+    rotated q (``out``, which may be q; else shares no memory with another
+    argument).
+
+    q [T, Hq, D], k and v [T, Hk, D] of the cache's type (any strides with
+    contiguous channels); cos, sin fp32 [T, R / 2]; slots int32 or int64 [T]: a
+    token whose slot lies outside the cache (-1) is stored nowhere; the others'
+    must differ.  ``norm`` "token", "head" or None, weights, ``layout`` and eps as
+    in ``rotary``."""
+    ck, cv, dev = _cache_of(cache)
+    _on(stream, dev)
+    pages, page, H, D = ck.shape
+    dt = ck.dtype
+    if not isinstance(k, torch.Tensor) or k.dim() != 3:
+        raise ValueError("t2t: k must be a [T, heads, D] tensor")
+    T = k.shape[0]
+    for t, name in ((k, "k"), (v, "v")):
+        if (not isinstance(t, torch.Tensor) or t.shape != (T, H, D) or t.dtype != dt or t.device != dev
+                or t.stride(2) != 1):
+            raise ValueError(f"t2t: {name} must be a {dt} [{T}, {H}, {D}] tensor on {dev} with contiguous channels")
+    if layout not in _ROPE_LAYOUTS or norm not in _ROPE_NORMS:
+        raise ValueError(f"t2t: layout {layout!r} (interleaved or half), norm {norm!r} (None, token or head)")
+    if not (math.isfinite(eps) and eps >= 0.0):
+        raise ValueError(f"t2t: eps must be at least 0, got {eps}")
+    R = 2 * cos.shape[-1] if isinstance(cos, torch.Tensor) and cos.dim() else 0
+    if not 2 <= R <= D:
+        raise ValueError(f"t2t: {R} of {D} channels rotated (2 <= R <= D)")
+    for t, name in ((cos, "cos"), (sin, "sin")):
+        if not _is(t, (T, R // 2), _f32, dev):
+            _check(t, (T, R // 2), _f32, name, dev)
+    if T >= 2 ** 31:
+        raise ValueError(f"t2t: {T} tokens")
+    bits = {_i32: 32, torch.int64: 64}.get(slots.dtype) if isinstance(slots, torch.Tensor) else None
+    if bits is None or not _is(slots, (T,), slots.dtype, dev):
+        _check(slots, (T,), (_i32, torch.int64), "slots", dev)
+    if norm is not None:
+        wshape = (H * D,) if norm == "token" else (D,)
+        if not _is(k_weight, wshape, dt, dev):
+            _check(k_weight, wshape, dt, "k_weight", dev)
+    elif k_weight is not None:
+        raise ValueError("t2t: k_weight without a norm")
+    cs = _cache_strides(ck)
+    ks, vs = k.stride(), v.stride()
+    tk = _lib.RotaryTensor(k.data_ptr(), 0, ks[0], ks[1], ck.data_ptr(), *cs,
+                           None if k_weight is None else k_weight.data_ptr(), H)
+    tv = _lib.RotaryTensor(v.data_ptr(), 0, vs[0], vs[1], cv.data_ptr(), *cs, None, H)
+    oq = tq = None
+    if q is not None:
+        if not isinstance(q, torch.Tensor) or q.dim() != 3:
+            raise ValueError("t2t: q must be a [T, heads, D] tensor")
+        oq, tq = _rotary_arg(q, out, q_weight, norm, "q", dev, stream, 1, T, D, dt)
+    elif out is not None or q_weight is not None:
+        raise ValueError("t2t: out and q_weight belong to q")
+    # the cache (and a caller's output) apart from everything that is read
+    ins = (q, k, v, cos, sin, q_weight, k_weight, slots)
+    at = [(p, e - p) for p, e in (_span(t) for t in ins if t is not None)]
+    if out is not None and q is not out:
+        at.append((lambda p, e: (p, e - p))(*_span(oq)))
+    if out is not None or _near(*_span(ck), at) or _near(*_span(cv), at):
+        if out is not None:
+            _apart((oq, ck, cv), ("the output of q", "the cache", "the cache"), ins[:1] + (None, None) + ins[1:])
+        else:
+            _apart((ck, cv), ("the cache", "the cache"), (None, None) + ins)
+    _launch("t2t_cache_append", dev, stream, (*ins, ck, cv, oq), tq, tk, tv, dtype_code(dt), cos.data_ptr(),
+            sin.data_ptr(), slots.data_ptr(), bits, pages, page, T, D, R, _ROPE_LAYOUTS[layout], _ROPE_NORMS[norm],
+            eps)
+    return oq
+
+
+def cache_attention_ws_bytes(B, T, Hq, cache, width, ragged=False):
+    """Workspace of cache_attention for T rows in all of B sequences (``ragged``: with
+    offsets) whose page tables are ``width`` pages wide."""
+    k = cache._k
+    return size_query("t2t_cache_attention_ws_bytes", bool(ragged), B, T, Hq, k.shape[2], k.shape[3],
+                      width * k.shape[1])
+
+
+def cache_attention(q, cache, page_table, lengths, *, offsets=None, mask=None, causal=False, scale=None,
+                    return_lse=False, out=None, ws=None, stream=None):
+    """Attention of new tokens over the cached keys and values of their sequences,
+    the new tokens' own among them (``cache_append`` first).
+
+    q [B, N, Hq, D]: N new tokens a sequence, or with ``offsets`` (int32 [B + 1]) [T,
+    Hq, D]: rows offsets[b] .. offsets[b + 1] - 1 are sequence b's (rows behind the
+    last sequence's stay as they are in ``out``, undefined in a fresh one).  page_table
+    int32 [B, width], lengths int32 [B]: the keys of sequence b, positions 0 ..
+    lengths[b] - 1, the last ones those of its new tokens, position j in page
+    page_table[b, j // page_size].  Query head h reads key head h // (Hq / Hk).
+
+    A token sees all older keys, and of the new ones all, or with ``causal`` those up
+    to itself, or those of ``mask`` (bool [B, N, C] or [T, C]: its row's column j is
+    the sequence's new token j; none from column C on), such as the tree that drafted
+    tokens form or the frames of a chunk.  A token that sees nothing gets zeros.  What
+    is not seen has no part whatever it holds; keys in pages outside the cache are not
+    seen, and lengths are held to what the table has room for.
+
+    ``scale`` (default D^-0.5) above 0.  fp32 sums and softmax, its weights rounded to
+    the type for the second product.  Returns out (of q's shape), or (out, lse) with
+    the natural logarithms of the softmax's sums, fp32 [..., Hq].  ``out``: contiguous
+    channels, 16-byte aligned rows; it and ``ws`` share no memory with another
+    argument."""
+    ck, cv, dev = _cache_of(cache)
+    _on(stream, dev)
+    pages, page, Hk, D = ck.shape
+    dt = ck.dtype
+    ragged = offsets is not None
+    if (not isinstance(q, torch.Tensor) or q.dim() != (3 if ragged else 4) or q.dtype != dt or q.device != dev
+            or q.shape[-1] != D):
+        raise ValueError(f"t2t: q must be a {dt} [{'T' if ragged else 'B, N'}, heads, {D}] tensor on {dev}")
+    Hq, N = q.shape[-2], q.shape[-3]
+    if Hq < 1 or Hq % Hk or Hq > 65536:
+        raise ValueError(f"t2t: {Hq} query heads over {Hk} of keys")
+    if not isinstance(lengths, torch.Tensor) or lengths.dim() != 1:
+        raise ValueError("t2t: lengths must be an int32 [B] tensor")
+    B = lengths.shape[0]
+    if not _is(lengths, (B,), _i32, dev):
+        _check(lengths, (B,), _i32, "lengths", dev)
+    if ragged:
+        if not _is(offsets, (B + 1,), _i32, dev):
+            _check(offsets, (B + 1,), _i32, "offsets", dev)
+        T, lead = N, (N,)
+    else:
+        if q.shape[0] != B:
+            raise ValueError(f"t2t: q of {q.shape[0]} sequences, {B} lengths")
+        T, lead = B * N, (B, N)
+    if (not isinstance(page_table, torch.Tensor) or page_table.dim() != 2 or page_table.shape[0] != B
+            or page_table.dtype != _i32 or page_table.device != dev
+            or (page_table.shape[1] > 1 and page_table.stride(1) != 1)):
+        raise ValueError(f"t2t: page_table must be an int32 [{B}, width] tensor on {dev} with contiguous rows")
+    width = page_table.shape[1]
+    if width * page >= 2 ** 31 - 64 or T * Hq >= 2 ** 31 or B > 2 ** 20:
+        raise ValueError(f"t2t: {B} sequences of {width} pages of {page}, {T} tokens of {Hq} heads")
+    if mask is not None:
+        if causal:
+            raise ValueError("t2t: a mask and causal")
+        if (not isinstance(mask, torch.Tensor) or mask.dtype != torch.bool or mask.device != dev
+                or mask.dim() != len(lead) + 1 or tuple(mask.shape[:-1]) != lead
+                or (mask.shape[-1] > 1 and mask.stride(-1) != 1)):
+            raise ValueError(f"t2t: mask must be a bool {[*lead, 'columns']} tensor on {dev} with contiguous rows")
+    if scale is None:
+        scale = D ** -0.5
+    elif not (math.isfinite(scale) and scale > 0.0):
+        raise ValueError(f"t2t: scale must be above 0, got {scale}")
+    qs = _attn_strides(q, "q")
+    if out is None:
+        o = q.new_empty(q.shape) if stream is None else _empty(stream, q.shape, dt, dev)
+    else:
+        o = out
+        if not isinstance(o, torch.Tensor) or o.shape != q.shape or o.dtype != dt or o.device != dev:
+            raise ValueError(f"t2t: out must be a {dt} {tuple(q.shape)} tensor on {dev}")
+        if not _scattered(o):
+            raise ValueError("t2t: out holds an element twice")
+    os = _attn_strides(o, "out")
+    lse = _empty(stream, (*lead, Hq), _f32, dev) if return_lse else None
+    need = cache_attention_ws_bytes(B, T, Hq, cache, width, ragged) if T and B else 0
+    if ws is not None:
+        ws = _ws_for(ws, need, dev, stream)
+    elif need:
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if stream is None else _ws(need, dev, stream)
+    ins = (q, ck, cv, page_table, lengths, offsets, mask)
+    if out is not None:
+        _apart((o,), ("out",), (None, *ins))
+    if ws is not None and need:
+        at = ws.data_ptr()
+        if _near(at, at + need, [(p, e - p) for p, e in (_span(t) for t in (*ins, o) if t is not None)]):
+            _apart((ws[:need],), ("ws",), (None, *ins, o))
+    ms = mask.stride() if mask is not None else (0, 0, 0)
+    args = _lib.CacheAttentionArgs(
+        ctypes.sizeof(_lib.CacheAttentionArgs), q.data_ptr(), ck.data_ptr(), cv.data_ptr(), o.data_ptr(),
+        None if lse is None else lse.data_ptr(), page_table.data_ptr() or None, lengths.data_ptr() or None,
+        offsets.data_ptr() if ragged else None, None if mask is None else mask.data_ptr() or q.data_ptr(), *qs, *os,
+        *_cache_strides(ck), page_table.stride(0), 0 if ragged else ms[0], ms[-2], B, N, Hq, Hk, D, dtype_code(dt),
+        pages, page, width, mask.shape[-1] if mask is not None else 0, bool(causal), scale)
+    _launch("t2t_cache_attention", dev, stream, (*ins, o, lse, ws), args, None if ws is None else ws.data_ptr(),
+            0 if ws is None else ws.numel())
+    return (o, lse) if return_lse else o
+
+
+def _attn_strides(t, name):
+    """Strides of sequences, tokens and heads of [B, N, H, D] or [T, H, D]."""
+    st = tuple(s if n > 1 else 0 for s, n in zip(t.stride(), t.shape))[:-1]
+    if (t.stride(-1) != 1 or any(s % 8 for s in st) or t.data_ptr() % 16) and t.numel():
+        raise ValueError(f"t2t: {name} must have contiguous channels and 16-byte aligned rows, got strides "
+                         f"{tuple(t.stride())}")
+    return st if len(st) == 3 else (0, *st)
