@@ -513,7 +513,7 @@ int t2t_mxfp4_linear(const void* x, int dtype, long long x_row_stride, const voi
 /* ---- 8-bit linear layers -------------------------------------------------- */
 /* Matrices [M, K] (M <= 2^30, K < 2^17) of whole numbers -127 .. 127 with one
  * fp32 scale a row.  No counterpart in the reference.  codes: row m at m *
- * stride bytes (16-byte aligned, a multiple of 16), columns K .. Kp - 1 of
+ * stride bytes (16-byte aligned, a multiple of 16, at most 2^23), columns K .. Kp - 1 of
  * every row zero, Kp = t2t_int8_row_bytes(K) = K rounded up to 128 <= stride.
  * Code -128 is taken as it stands. */
 size_t t2t_int8_row_bytes(int K);

@@ -24,8 +24,11 @@ static int i8_check_sizes(const char* what, int M, int K) {
 static int i8_check_matrix(const char* what, const void* codes, long long stride, const void* scales, int M,
                            int K) {
   T2T_REQUIRE(codes && scales, "%s: null pointer", what);
-  T2T_REQUIRE((uintptr_t)codes % 16 == 0 && stride % 16 == 0 && stride >= i8_kp(K) && (uintptr_t)scales % 4 == 0,
-              "%s: rows of codes must be 16-byte aligned and hold K rounded up to 128, stride %lld", what, stride);
+  // (a tile's rows are addressed by 32-bit offsets)
+  T2T_REQUIRE((uintptr_t)codes % 16 == 0 && stride % 16 == 0 && stride >= i8_kp(K) && stride <= (1 << 23) &&
+                  (uintptr_t)scales % 4 == 0,
+              "%s: rows of codes must be 16-byte aligned, hold K rounded up to 128 and lie within 8 MiB, stride %lld",
+              what, stride);
   return T2T_OK;
 }
 // a 16-bit matrix
@@ -323,10 +326,402 @@ static int i8_split_launch(const I8Mat& a, const I8Mat& w, const uint16_t* bias,
   return T2T_OK;
 }
 
+// ---- tiles staged through LDS ------------------------------------------------
+// Tiles of 64 TW features x 64 TA tokens, four waves of 32 TW x 32 TA each (2 x 2).
+// The weights are the A operand, so a lane holds one token's features 8 (i / 4) +
+// 4 (l / 32) + i % 4 of a block.  A stage is 64 columns: rows of 64 bytes, weights
+// before tokens, fetched by DMA (1 KB, sixteen rows, an instruction; the lane fetches
+// the 16 bytes that belong at its place).  16-byte chunk c of row r lies at c ^ ((r
+// >> 2) & 3), so that the fragment reads (row l % 32, chunk 2 s + l / 32 in lane l for
+// step s) meet all banks.  Four stages are kept.
+template <int TW, int TA> struct I8Tile {
+  static constexpr int STAGE = 64 * (TW + TA) * 64;
+};
+__device__ inline int i8_swz(int row) { return (row >> 2) & 3; }
+
+// A wave's 32 TA tokens from m on, 32 TW features from n on: 32 tokens x 64 features at a time are
+// scaled, packed, turned through 4 KB of LDS of the wave's own (16-byte chunk c of token t at c ^ (t &
+// 7)) and stored as rows, a step behind, so that the reads have the next step's packing to land.  (DS
+// operations of a wave run in order: the next writes follow the last reads.)  VEC: widths and strides
+// are multiples of eight and out is 16-byte aligned, so a chunk is inside or outside as a whole.
+// `par`: the wave's 32 TW channel scales and as many biases, in LDS.
+template <typename T, int TW, int TA, bool GELU, bool VEC>
+__device__ inline void i8_store(const i32x16 (&acc)[TW][TA], char* so, const float* par, const I8Mat& a,
+                                uint16_t* __restrict__ out, long long ldo, int m, int n, int N) {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // (or its addresses are kept in registers through the products)
+  const int hh = lane >> 5, c = lane & 7, t0 = lane >> 3, M = a.rows;
+  const long long lane_at = t0 * ldo + 8 * c;
+  float sa[TA];
+#pragma unroll
+  for (int j = 0; j < TA; ++j) sa[j] = a.scales[min(m + 32 * j + (lane & 31), M - 1)];
+  u32x4 v[4];
+  auto put = [&](int j, int i) {
+    const int left = N - (n + 32 * i + 8 * c), rows = left > 0 ? M - (m + 32 * j) : 0;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      uint16_t* o = out + ((long long)(m + 32 * j + 8 * r) * ldo + n + 32 * i);
+      if (8 * r + t0 < rows) {
+        if constexpr (VEC)
+          *(u32x4*)(o + lane_at) = v[r];
+        else
+          lin_put(o + lane_at, v[r], left);
+      }
+    }
+  };
+#pragma unroll
+  for (int ii = 0; ii < TW; ii += 2) {
+    f32x4 sw[2][4], sb[2][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        sw[i][q] = *(const f32x4*)(par + 32 * (ii + i) + 8 * q + 4 * hh);
+        sb[i][q] = *(const f32x4*)(par + 32 * (TW + ii + i) + 8 * q + 4 * hh);
+      }
+#pragma unroll
+    for (int j = 0; j < TA; ++j) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float f[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) f[e] = i8_out<T, GELU>(acc[ii + i][j][4 * q + e], sw[i][q][e], sa[j], sb[i][q][e]);
+          *(u32x2*)(so + (lane & 31) * 128 + (((4 * i + q) ^ (lane & 7)) * 16) + 8 * hh) =
+              u32x2{Pk<T>::pack(f[0], f[1]), Pk<T>::pack(f[2], f[3])};
+        }
+      __builtin_amdgcn_sched_barrier(0);
+      if (ii || j) put(j ? j - 1 : TA - 1, j ? ii : ii - 2);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int t = 8 * r + t0;
+        v[r] = *(const u32x4*)(so + t * 128 + ((c ^ (t & 7)) * 16));
+      }
+    }
+  }
+  put(TA - 1, TW - 2);
+}
+// the wave's scales and biases to LDS of its own
+template <typename T, int TW>
+__device__ inline void i8_params(float* par, const I8Mat& w, const uint16_t* __restrict__ bias, int n) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = lane; i < 32 * TW; i += 64) {
+    const int f = min(n + i, w.rows - 1);
+    par[i] = w.scales[f];
+    par[32 * TW + i] = bias ? T::to_f(bias[f]) : 0.f;
+  }
+}
+
+// ---- the 256 x 256 tile: its inner loop is written out ----------------------
+// With 256 accumulators a SIMD holds one wave, so no other wave covers a wait.  A
+// step is one asm block of sixteen products (32 columns): the next step's eight
+// fragment reads and half a stage's DMA go between them, and the one wait at its
+// end finds the reads old.  A block waits for its own reads, so none of its
+// outputs is in flight outside it.
+#define I8_P(i, j) "v_mfma_i32_32x32x32_i8 %[c" #i #j "], %[w" #i "], %[a" #j "], %[c" #i #j "]\n\t"
+#define I8_R(d, base, o) "ds_read_b128 %[" d "], %[" base "] offset:%c[" o "]\n\t"
+// 1 KB (16 bytes a lane) to LDS at m0, which moves on
+#define I8_D(i) "global_load_lds_dwordx4 %[v" #i "], %[g]\n\ts_add_u32 m0, m0, 0x400\n\t"
+#define I8_ACC                                                                                          \
+  [c00] "+a"(acc[0][0]), [c01] "+a"(acc[0][1]), [c02] "+a"(acc[0][2]), [c03] "+a"(acc[0][3]),           \
+      [c10] "+a"(acc[1][0]), [c11] "+a"(acc[1][1]), [c12] "+a"(acc[1][2]), [c13] "+a"(acc[1][3]),       \
+      [c20] "+a"(acc[2][0]), [c21] "+a"(acc[2][1]), [c22] "+a"(acc[2][2]), [c23] "+a"(acc[2][3]),       \
+      [c30] "+a"(acc[3][0]), [c31] "+a"(acc[3][1]), [c32] "+a"(acc[3][2]), [c33] "+a"(acc[3][3])
+#define I8_NEXT(f)                                                                                      \
+  [x0] "=&v"(f.w[0]), [x1] "=&v"(f.w[1]), [x2] "=&v"(f.w[2]), [x3] "=&v"(f.w[3]), [y0] "=&v"(f.a[0]),   \
+      [y1] "=&v"(f.a[1]), [y2] "=&v"(f.a[2]), [y3] "=&v"(f.a[3])
+#define I8_CUR(f)                                                                                       \
+  [w0] "v"(f.w[0]), [w1] "v"(f.w[1]), [w2] "v"(f.w[2]), [w3] "v"(f.w[3]), [a0] "v"(f.a[0]),             \
+      [a1] "v"(f.a[1]), [a2] "v"(f.a[2]), [a3] "v"(f.a[3])
+#define I8_READS(OFF)                                                                                   \
+  [bw] "v"(bw), [ba] "v"(ba), [o0] "n"(OFF), [o1] "n"((OFF) + 2048), [o2] "n"((OFF) + 4096),            \
+      [o3] "n"((OFF) + 6144)
+#define I8_DMA_IN [v0] "v"(v[0]), [v1] "v"(v[1]), [v2] "v"(v[2]), [v3] "v"(v[3]), [g] "s"(g), [m] "s"(m)
+#define I8_STEP                                                                                         \
+  I8_P(0, 0) I8_R("x0", "bw", "o0") I8_P(0, 1) I8_R("y0", "ba", "o0") I8_P(0, 2) I8_R("x1", "bw", "o1") \
+      I8_P(0, 3) I8_D(0) I8_P(1, 3) I8_R("y1", "ba", "o1") I8_P(1, 2) I8_R("x2", "bw", "o2")            \
+          I8_P(1, 1) I8_R("y2", "ba", "o2") I8_P(1, 0) I8_D(1) I8_P(2, 0) I8_R("x3", "bw", "o3")        \
+              I8_P(2, 1) I8_R("y3", "ba", "o3") I8_P(2, 2) I8_P(2, 3) I8_D(2) I8_P(3, 3)                \
+                  I8_P(3, 2) I8_D(3) I8_P(3, 1) I8_P(3, 0) "s_waitcnt lgkmcnt(0)"
+
+struct I8Frags {
+  i32x4 w[4], a[4];
+};
+// First step of a stage: reads the stage's second fragments at OFF; fetches the second half of the
+// stage three further on.
+template <int OFF>
+__device__ inline void i8_step0(i32x16 (&acc)[4][4], const I8Frags& f, I8Frags& nx, uint32_t bw, uint32_t ba,
+                                const uint32_t* v, const char* g, uint32_t m) {
+  asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 1\n\t" I8_STEP
+               : I8_ACC, I8_NEXT(nx)
+               : I8_CUR(f), I8_READS(OFF), I8_DMA_IN
+               : "memory", "scc");
+}
+// Second step: once the next stage has landed for every wave (the two after it may be under way) and
+// this one's reads are done, reads the next stage's first fragments at OFF and fetches the first half
+// of the stage four further on into this one's place.
+template <int OFF>
+__device__ inline void i8_step1(i32x16 (&acc)[4][4], const I8Frags& f, I8Frags& nx, uint32_t bw, uint32_t ba,
+                                const uint32_t* v, const char* g, uint32_t m) {
+  asm volatile("s_mov_b32 m0, %[m]\n\ts_waitcnt vmcnt(16)\n\ts_barrier\n\t" I8_STEP
+               : I8_ACC, I8_NEXT(nx)
+               : I8_CUR(f), I8_READS(OFF), I8_DMA_IN
+               : "memory", "scc");
+}
+
+// Work-groups stay for many tiles.  The DMA runs four stages ahead of the products
+// as one stream over all of them, so a tile's first stages are loaded under the last
+// products and the epilogue of the one before; the epilogue has LDS of its own.
+template <typename T, bool GELU, bool VEC>
+__global__ __launch_bounds__(256, 1) void i8_big_kernel(I8Mat a, I8Mat w, const uint16_t* __restrict__ bias,
+                                                        uint16_t* __restrict__ out, long long ldo, int n,
+                                                        int mt, int nt, int per_xcd) {
+  constexpr int ST = I8Tile<4, 4>::STAGE, PAIR = 2 * ST, OWN = 4096 + 1024;
+  static_assert(ST + 8192 < 65536, "LDS offsets of 16 bits");
+  __shared__ __attribute__((aligned(1024))) char lds[4 * ST + 4 * OWN];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wn = wave & 1, wm = wave >> 1;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lin_lds_t*)lds;
+  const int step = gridDim.x >> 3;
+  int id = lin_first(per_xcd);
+  const int end = lin_end(mt, nt, per_xcd);
+  if (id >= end) return;
+
+  // the stream of stages (n a tile, an even number): tile ld, its stage ls; this wave fetches 128 rows
+  // of the weights (waves 0 and 1) or the tokens, KB i those from 16 i on
+  const char* g;
+  uint32_t v[8];
+  int ld = id, ls = 0;
+  auto aim = [&]() {
+    int m0, n0;
+    lin_place(ld, mt, nt, 8, 8, m0, n0);
+    const I8Mat& x = wave < 2 ? w : a;
+    const int first = 32 * (wave < 2 ? n0 : m0), last = x.rows - 1 - first;
+    g = x.codes + first * x.stride;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = 128 * (wave & 1) + 16 * i + (lane >> 2);
+      v[i] = (uint32_t)(min(row, last) * x.stride) + 16 * ((lane & 3) ^ i8_swz(row));
+    }
+  };
+  auto next_pair = [&]() {
+    if (ld >= end) return;
+    ls += 2;
+    if (ls < n) return;
+    ld += step;
+    if (ld < end) {
+      ls = 0;
+      aim();
+    } else {  // after the last tile every lane reads one place, so that the counts of loads stay
+      ls = n - 2;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0;
+    }
+  };
+  auto at = [&](int odd) { return g + (size_t)(ls + odd) * 64; };
+  const uint32_t dst = lds0 + wave * 8192;
+  auto issue = [&](uint32_t off, int i) {  // KB i of a pair
+    asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %[v], %[g]" ::[m] "s"(
+                     dst + off + (i >> 3) * ST + (i & 7) * 1024),
+                 [v] "v"(v[i & 7]), [g] "s"(at(i >> 3))
+                 : "memory");
+  };
+  // two pairs but for the last half stage, which the first step fetches
+  aim();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) issue(0, i);
+  next_pair();
+#pragma unroll
+  for (int i = 0; i < 12; ++i) issue(PAIR, i);
+  // fragment addresses in the pair in use: of a stage's first and second steps
+  const uint32_t row = (lane & 31) * 64, hh = lane >> 5, z = i8_swz(lane & 31);
+  const uint32_t f0at = row + 16 * (hh ^ z), f1at = row + 16 * ((2 + hh) ^ z);
+  uint32_t bw = lds0 + wn * 8192, ba = lds0 + 16384 + wm * 8192, off = 0;
+  I8Frags f0, f1;
+  {
+    const uint32_t w0 = bw + f0at, a0 = ba + f0at;
+    asm volatile("s_waitcnt vmcnt(20)\n\ts_barrier\n\t" I8_R("x0", "bw", "o0") I8_R("y0", "ba", "o0")
+                 I8_R("x1", "bw", "o1") I8_R("y1", "ba", "o1") I8_R("x2", "bw", "o2") I8_R("y2", "ba", "o2")
+                 I8_R("x3", "bw", "o3") I8_R("y3", "ba", "o3") "s_waitcnt lgkmcnt(0)"
+                 : I8_NEXT(f0)
+                 : [bw] "v"(w0), [ba] "v"(a0), [o0] "n"(0), [o1] "n"(2048), [o2] "n"(4096), [o3] "n"(6144)
+                 : "memory");
+  }
+  char* own = lds + 4 * ST + wave * OWN;
+  i32x16 acc[4][4];
+  for (;;) {
+    int m0, n0;
+    lin_place(id, mt, nt, 8, 8, m0, n0);
+    i8_params<T, 4>((float*)(own + 4096), w, bias, (n0 + wn * 4) * 32);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        acc[i][j] = i32x16{};
+        asm volatile("" : "+a"(acc[i][j]));  // a register set each, now
+      }
+    for (int s = n; s > 0; s -= 2) {
+      const uint32_t other = PAIR - 2 * off;  // from this pair to the other one (off: 0 or PAIR)
+      i8_step0<0>(acc, f0, f1, bw + f1at, ba + f1at, v + 4, at(1), dst + PAIR - off + ST + 4096);
+      next_pair();
+      i8_step1<ST>(acc, f1, f0, bw + f0at, ba + f0at, v, at(0), dst + off);
+      i8_step0<ST>(acc, f0, f1, bw + f1at, ba + f1at, v + 4, at(0), dst + off + 4096);
+      bw += other, ba += other;
+      i8_step1<0>(acc, f1, f0, bw + f0at, ba + f0at, v, at(1), dst + off + ST);
+      off = PAIR - off;
+    }
+    // the last products' registers are readable after 18 cycles of issue
+    asm volatile("s_nop 15\n\ts_nop 15" : I8_ACC);
+    i8_store<T, 4, 4, GELU, VEC>(acc, own, (const float*)(own + 4096), a, out, ldo, (m0 + wm * 4) * 32,
+                                 (n0 + wn * 4) * 32, w.rows);
+    id += step;
+    if (id >= end) break;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// ---- the 128 x 128 tile ------------------------------------------------------
+// The same with a whole stage a step: eight products, the next stage's eight
+// fragment reads and the DMA of the stage four further on.  Two work-groups fit a
+// CU.
+#define I8_Q(c, i, j) "v_mfma_i32_32x32x32_i8 %[c" #i #j "], %[w" #c #i "], %[a" #c #j "], %[c" #i #j "]\n\t"
+#define I8_MID_STEP                                                                                     \
+  "s_mov_b32 m0, %[m]\n\ts_waitcnt vmcnt(8)\n\ts_barrier\n\t" I8_Q(0, 0, 0) I8_R("x00", "bw0", "o0")    \
+      I8_R("y00", "ba0", "o0") I8_Q(0, 0, 1) I8_R("x01", "bw0", "o1") I8_R("y01", "ba0", "o1")          \
+          I8_Q(0, 1, 1) I8_D(0) I8_R("x10", "bw1", "o0") I8_Q(0, 1, 0) I8_R("y10", "ba1", "o0") I8_D(1) \
+              I8_Q(1, 0, 0) I8_R("x11", "bw1", "o1") I8_R("y11", "ba1", "o1") I8_Q(1, 0, 1) I8_D(2)     \
+                  I8_Q(1, 1, 1) I8_D(3) I8_Q(1, 1, 0) "s_waitcnt lgkmcnt(0)"
+struct I8MidFrags {
+  i32x4 w[2][2], a[2][2];  // [fragment of the stage][block]
+};
+#define I8_MID_NEXT(nx)                                                                                 \
+  [x00] "=&v"(nx.w[0][0]), [x01] "=&v"(nx.w[0][1]), [x10] "=&v"(nx.w[1][0]), [x11] "=&v"(nx.w[1][1]),   \
+      [y00] "=&v"(nx.a[0][0]), [y01] "=&v"(nx.a[0][1]), [y10] "=&v"(nx.a[1][0]), [y11] "=&v"(nx.a[1][1])
+// OFF: where the next stage lies
+template <int OFF>
+__device__ inline void i8_mid_step(i32x16 (&acc)[2][2], const I8MidFrags& f, I8MidFrags& nx, uint32_t bw0,
+                                   uint32_t bw1, uint32_t ba0, uint32_t ba1, const uint32_t (&v)[4], const char* g,
+                                   uint32_t m) {
+  asm volatile(I8_MID_STEP
+               : [c00] "+v"(acc[0][0]), [c01] "+v"(acc[0][1]), [c10] "+v"(acc[1][0]), [c11] "+v"(acc[1][1]),
+                 I8_MID_NEXT(nx)
+               : [w00] "v"(f.w[0][0]), [w01] "v"(f.w[0][1]), [w10] "v"(f.w[1][0]), [w11] "v"(f.w[1][1]),
+                 [a00] "v"(f.a[0][0]), [a01] "v"(f.a[0][1]), [a10] "v"(f.a[1][0]), [a11] "v"(f.a[1][1]),
+                 [bw0] "v"(bw0), [bw1] "v"(bw1), [ba0] "v"(ba0), [ba1] "v"(ba1), [o0] "n"(OFF), [o1] "n"(OFF + 2048),
+                 I8_DMA_IN
+               : "memory", "scc");
+}
+
+template <typename T, bool GELU, bool VEC>
+__global__ __launch_bounds__(256, 2) void i8_mid_kernel(I8Mat a, I8Mat w, const uint16_t* __restrict__ bias,
+                                                        uint16_t* __restrict__ out, long long ldo, int n, int mt,
+                                                        int nt, int per_xcd) {
+  constexpr int ST = I8Tile<2, 2>::STAGE, PAIR = 2 * ST;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * ST];
+  __shared__ __attribute__((aligned(16))) float par[4][128];
+  const int id = lin_first(per_xcd);
+  if (id >= lin_end(mt, nt, per_xcd)) return;
+  int m0, n0;
+  lin_place(id, mt, nt, 4, 4, m0, n0);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wn = wave & 1, wm = wave >> 1;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lin_lds_t*)lds;
+  const I8Mat& x = wave < 2 ? w : a;
+  const int first = 32 * (wave < 2 ? n0 : m0), last = x.rows - 1 - first;
+  const char* g = x.codes + first * x.stride;
+  uint32_t v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = 64 * (wave & 1) + 16 * i + (lane >> 2);
+    v[i] = (uint32_t)(min(row, last) * x.stride) + 16 * ((lane & 3) ^ i8_swz(row));
+  }
+  const uint32_t dst = lds0 + wave * 4096;
+  // (past the last stage it is fetched again, so that the counts of loads in flight stay)
+  auto at = [&](int s) { return g + (size_t)min(s, n - 1) * 64; };
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %[v], %[g]" ::[m] "s"(
+                       dst + s * ST + i * 1024),
+                   [v] "v"(v[i]), [g] "s"(at(s))
+                   : "memory");
+  i8_params<T, 2>(par[wave], w, bias, (n0 + wn * 2) * 32);
+  i32x16 acc[2][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) acc[i][j] = i32x16{};
+  const uint32_t row = (lane & 31) * 64, hh = lane >> 5, z = i8_swz(lane & 31);
+  const uint32_t at0 = row + 16 * (hh ^ z), at1 = row + 16 * ((2 + hh) ^ z);
+  uint32_t bw0 = lds0 + wn * 4096 + at0, bw1 = lds0 + wn * 4096 + at1;
+  uint32_t ba0 = lds0 + 8192 + wm * 4096 + at0, ba1 = lds0 + 8192 + wm * 4096 + at1, off = 0;
+  I8MidFrags f0, f1;
+  asm volatile("s_waitcnt vmcnt(12)\n\ts_barrier\n\t" I8_R("x00", "bw0", "o0") I8_R("x01", "bw0", "o1")
+               I8_R("x10", "bw1", "o0") I8_R("x11", "bw1", "o1") I8_R("y00", "ba0", "o0") I8_R("y01", "ba0", "o1")
+               I8_R("y10", "ba1", "o0") I8_R("y11", "ba1", "o1") "s_waitcnt lgkmcnt(0)"
+               : I8_MID_NEXT(f0)
+               : [bw0] "v"(bw0), [bw1] "v"(bw1), [ba0] "v"(ba0), [ba1] "v"(ba1), [o0] "n"(0), [o1] "n"(2048)
+               : "memory");
+  for (int s = 0; s < n; s += 2) {
+    const uint32_t other = PAIR - 2 * off;  // from this pair of stages to the other one
+    i8_mid_step<ST>(acc, f0, f1, bw0, bw1, ba0, ba1, v, at(s + 4), dst + off);
+    bw0 += other, bw1 += other, ba0 += other, ba1 += other;
+    i8_mid_step<0>(acc, f1, f0, bw0, bw1, ba0, ba1, v, at(s + 5), dst + off + ST);
+    off = PAIR - off;
+  }
+  // every load has landed and every wave's reads are done: LDS is free; the products' registers are
+  // readable
+  asm volatile("s_nop 15\n\ts_nop 15\n\ts_waitcnt vmcnt(0)\n\ts_barrier"
+               : "+v"(acc[0][0]), "+v"(acc[0][1]), "+v"(acc[1][0]), "+v"(acc[1][1])
+               :
+               : "memory");
+  i8_store<T, 2, 2, GELU, VEC>(acc, lds + wave * 4096, par[wave], a, out, ldo, (m0 + wm * 2) * 32, (n0 + wn * 2) * 32,
+                               w.rows);
+}
+
+// tiles of 64 TW x 64 TA
+template <typename T, int TW, int TA>
+static int i8_tile_launch(const I8Mat& a, const I8Mat& w, const uint16_t* bias, int act, uint16_t* out,
+                          long long ldo, int units, hipStream_t st) {
+  const int mt = cdiv(a.blocks, 2 * TA), nt = cdiv(w.blocks, 2 * TW);
+  const long long tiles = (long long)mt * nt;
+  if (tiles > (1 << 23)) {  // 2^31 threads of 128 x 128 tiles; as many large ones are a TB of outputs
+    t2t_set_error("int8_product: M=%d N=%d", a.rows, w.rows);
+    return T2T_ERR_UNSUPPORTED;
+  }
+  const int per = cdiv(tiles, 8);
+  auto launch = [&](auto kernel, int slots) {
+    hipLaunchKernelGGL(kernel, dim3(8 * slots), dim3(256), 0, st, a, w, bias, out, ldo, 2 * units, mt, nt, per);
+  };
+  auto form = [&](auto G, auto V) {
+    constexpr bool GELU = decltype(G)::value, VEC = decltype(V)::value;
+    if constexpr (TW == 4)  // fills a CU: 32 work-groups an XCD, which go through the tiles
+      launch(i8_big_kernel<T, GELU, VEC>, per < 32 ? per : 32);
+    else
+      launch(i8_mid_kernel<T, GELU, VEC>, per);
+  };
+  const bool gelu = act == T2T_ACT_GELU_TANH;
+  const bool vec = w.rows % 8 == 0 && ldo % 8 == 0 && (uintptr_t)out % 16 == 0;
+  if (gelu)
+    vec ? form(std::true_type{}, std::true_type{}) : form(std::true_type{}, std::false_type{});
+  else
+    vec ? form(std::false_type{}, std::true_type{}) : form(std::false_type{}, std::false_type{});
+  T2T_LAUNCH_CHECK("int8_product");
+  return T2T_OK;
+}
+
 template <typename T>
 static int i8_product(const I8Mat& a, const I8Mat& w, const uint16_t* bias, int act, uint16_t* out, long long ldo,
                       int units, hipStream_t st) {
-  return i8_split_launch<T, 2>(a, w, bias, act, out, ldo, units, st);
+  const long long big = (long long)cdiv(a.blocks, 8) * cdiv(w.blocks, 8);
+  const long long mid = (long long)cdiv(a.blocks, 4) * cdiv(w.blocks, 4);
+  if ((long long)a.blocks * w.blocks <= 512) return i8_split_launch<T, 2>(a, w, bias, act, out, ldo, units, st);
+  if (big >= 256 && 4 * big <= mid + mid / 4) return i8_tile_launch<T, 4, 4>(a, w, bias, act, out, ldo, units, st);
+  return i8_tile_launch<T, 2, 2>(a, w, bias, act, out, ldo, units, st);
 }
 
 static int i8_check_product(const char* what, const void* w_codes, long long w_stride, const float* w_scales,

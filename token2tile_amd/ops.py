@@ -1286,9 +1286,9 @@ class Int8:
                              f"behind them, got {rows} x {wide}")
         _check(scales, (rows,), _f32, "scales", dev)
         stride = codes.stride(0) if rows > 1 else wide
-        if codes.stride(1) != 1 or stride < wide or stride % 16 or codes.data_ptr() % 16:
-            raise ValueError(f"t2t: the rows of codes must be contiguous, 16-byte aligned and apart, got strides "
-                             f"{tuple(codes.stride())}")
+        if codes.stride(1) != 1 or not wide <= stride <= 2 ** 23 or stride % 16 or codes.data_ptr() % 16:
+            raise ValueError(f"t2t: the rows of codes must be contiguous, 16-byte aligned and apart (at most 8 MiB), got "
+                             f"strides {tuple(codes.stride())}")
         if rows and _near(*_span(codes), ((scales.data_ptr(), scales.nbytes),)) and _meet(codes, scales):
             raise ValueError("t2t: scales shares memory with codes")
         self._set(codes, scales, cols)
