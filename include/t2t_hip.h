@@ -512,33 +512,34 @@ int t2t_mxfp4_linear(const void* x, int dtype, long long x_row_stride, const voi
 
 /* ---- 8-bit linear layers -------------------------------------------------- */
 /* Matrices [M, K] (M <= 2^30, K < 2^17) of whole numbers -127 .. 127 with one
- * fp32 scale a row.  No counterpart in the reference.  codes: row m at m *
- * stride bytes (16-byte aligned, a multiple of 16, at most 2^23), columns K .. Kp - 1 of
- * every row zero, Kp = t2t_int8_row_bytes(K) = K rounded up to 128 <= stride.
- * Code -128 is taken as it stands. */
-size_t t2t_int8_row_bytes(int K);
+ * fp32 scale a row.  No counterpart in the reference.  Codes are held in the order
+ * of the products' tiles, blocks of 16 rows x 64 columns:
+ *   codes [ceil(M / 16)][Kp / 64][16][4][16] bytes, Kp = K rounded up to 128: chunk
+ *         c (columns 16 c .. + 15) of row r of a block at place c ^ ((r >> 2) & 3)
+ * Columns K .. Kp - 1 are zero; rows from M on may hold anything.  Code -128 is taken
+ * as it stands.  Byte count of the codes (0 for an empty matrix). */
+size_t t2t_int8_code_bytes(int M, int K);
 /* x [M, K] fp16 / bf16, row m at m * row_stride (elements; any alignment).  A
  * row's scale is max|x| / 127 in fp32, at least 2^-120; codes are x / scale to
  * nearest, ties to even (the exact quotient); a row with an inf or NaN gets
- * scale NaN and codes 0.  Columns K .. Kp - 1 of codes are written (0). */
-int t2t_int8_quantize(const void* x, int dtype, long long row_stride, void* codes,
-                      long long code_stride, float* scales, int M, int K, void* stream);
+ * scale NaN and codes 0.  Rows from M on are not written. */
+int t2t_int8_quantize(const void* x, int dtype, long long row_stride, void* codes, float* scales,
+                      int M, int K, void* stream);
 /* code * scale, rounded once -> out [M, K] fp16 / bf16. */
-int t2t_int8_dequantize(const void* codes, long long code_stride, const float* scales, void* out,
-                        int dtype, long long row_stride, int M, int K, void* stream);
+int t2t_int8_dequantize(const void* codes, const float* scales, void* out, int dtype,
+                        long long row_stride, int M, int K, void* stream);
 /* out [M, N] (dtype) = act((sum_k A W) w_scales[n] a_scales[m] + bias[n]): A [M, K]
  * and W [N, K] in 8 bits, bias [N] in dtype or NULL, act as for MXFP4; sums in
  * 32-bit integers (exact), the rest in fp32, rounded once.  Row m of out at m *
  * out_row_stride. */
-int t2t_int8_product(const void* a_codes, long long a_stride, const float* a_scales,
-                     const void* w_codes, long long w_stride, const float* w_scales,
-                     const void* bias, int act, void* out, int dtype, long long out_row_stride,
-                     int M, int N, int K, void* stream);
+int t2t_int8_product(const void* a_codes, const float* a_scales, const void* w_codes,
+                     const float* w_scales, const void* bias, int act, void* out, int dtype,
+                     long long out_row_stride, int M, int N, int K, void* stream);
 /* t2t_int8_quantize of x into the workspace and t2t_int8_product.  out and ws
  * share no memory with another argument. */
 size_t t2t_int8_linear_ws_bytes(int M, int N, int K);
 int t2t_int8_linear(const void* x, int dtype, long long x_row_stride, const void* w_codes,
-                    long long w_stride, const float* w_scales, const void* bias, int act, void* out,
+                    const float* w_scales, const void* bias, int act, void* out,
                     long long out_row_stride, int M, int N, int K, void* ws, size_t ws_bytes,
                     void* stream);
 

@@ -46,10 +46,19 @@ def i8_ref(x):
 def _check_codes(t, x):
     n, s = i8_ref(x)
     M, K = x.shape
-    assert t.shape == (M, K) and t.codes.shape == (M, -(-K // 128) * 128)
-    assert torch.equal(t.scales.double().nan_to_num(-1.0), s.nan_to_num(-1.0))
-    assert torch.equal(t.codes[:, :K].double(), n)
-    assert not bool(t.codes[:, K:].any())
+    assert t.shape == (M, K) and torch.equal(t.scales.double().nan_to_num(-1.0), s.nan_to_num(-1.0))
+    wide = _rows(t)
+    assert torch.equal(wide[:M, :K].double(), n) and not bool(wide[:M, K:].any())
+    assert torch.equal(t.to_codes(), wide[:M, :K])
+
+
+def _rows(t):
+    """All codes of a matrix in rows, by the layout's definition: chunk c of row r at
+    place c ^ ((r >> 2) & 3) of its block of 16 rows x 64 columns."""
+    M, K = -(-t.rows // 16) * 16, -(-t.cols // 128) * 128
+    r, c = torch.arange(M)[:, None], torch.arange(K)[None]
+    at = ((r // 16 * (K // 64) + c // 64) * 16 + r % 16) * 64 + ((c // 16 % 4) ^ (r // 4 % 4)) * 16 + c % 16
+    return t.codes[at.to(t.codes.device)]
 
 
 # ---------------------------------------------------------------------------
@@ -59,28 +68,30 @@ def test_entries_reject_bad_arguments():
     from token2tile_amd import _lib
     L = _lib.lib()
     p, odd = ctypes.c_void_p(32), ctypes.c_void_p(40)
-    assert [L.t2t_int8_row_bytes(k) for k in (0, 1, 128, 129, 131071, 131072)] == [0, 128, 128, 256, 131072, 0]
+    bytes_of = L.t2t_int8_code_bytes
+    assert [bytes_of(1, k) for k in (0, 1, 128, 129, 131071, 131072)] == [0, 2048, 2048, 4096, 16 * 131072, 0]
+    assert [bytes_of(m, 100) for m in (-1, 0, 16, 17)] == [0, 0, 2048, 4096]
 
-    def quant(x=p, dtype=1, stride=300, codes=p, cs=384, scales=p, M=4, K=300):
-        return L.t2t_int8_quantize(x, dtype, stride, codes, cs, scales, M, K, None)
-    assert quant(dtype=7) == 1 and quant(stride=299) == 1 and quant(codes=odd) == 1 and quant(cs=383) == 1
-    assert quant(cs=368) == 1 and quant(K=0) == 1 and quant(K=1 << 17, stride=1 << 17, cs=1 << 18) == 1
+    def quant(x=p, dtype=1, stride=300, codes=p, scales=p, M=4, K=300):
+        return L.t2t_int8_quantize(x, dtype, stride, codes, scales, M, K, None)
+    assert quant(dtype=7) == 1 and quant(stride=299) == 1 and quant(codes=odd) == 1 and quant(scales=ctypes.c_void_p(6)) == 1
+    assert quant(K=0) == 1 and quant(K=1 << 17, stride=1 << 17) == 1
     assert quant(M=-1) == 1 and quant(M=(1 << 30) + 1) == 1
     assert quant(scales=None) == 1 and b"null" in L.t2t_last_error() and quant(x=None) == 1
     assert quant(M=0, x=None) == 0
 
-    def deq(dtype=1, stride=300, out=p, cs=384):
-        return L.t2t_int8_dequantize(p, cs, p, out, dtype, stride, 4, 300, None)
-    assert deq(dtype=2) == 1 and deq(stride=299) == 1 and deq(out=None) == 1 and deq(cs=256) == 1
+    def deq(dtype=1, stride=300, out=p, codes=p):
+        return L.t2t_int8_dequantize(codes, p, out, dtype, stride, 4, 300, None)
+    assert deq(dtype=2) == 1 and deq(stride=299) == 1 and deq(out=None) == 1 and deq(codes=odd) == 1
 
-    def prod(a=p, st=384, w=p, act=0, out=p, dtype=1, ldo=40, M=4, N=40, K=300):
-        return L.t2t_int8_product(a, st, p, w, st, p, None, act, out, dtype, ldo, M, N, K, None)
+    def prod(a=p, w=p, act=0, out=p, dtype=1, ldo=40, M=4, N=40, K=300):
+        return L.t2t_int8_product(a, p, w, p, None, act, out, dtype, ldo, M, N, K, None)
     assert prod(act=2) == 1 and prod(dtype=3) == 1 and prod(ldo=39) == 1 and prod(N=0) == 1 and prod(w=None) == 1
-    assert prod(a=odd) == 1 and prod(st=400 - 32) == 1 and prod(out=None) == 1
+    assert prod(a=odd) == 1 and prod(w=odd) == 1 and prod(out=None) == 1
     assert prod(M=0, a=None, out=None) == 0
 
     def lin(ws=p, nb=1 << 20, M=4, K=300, x=p):
-        return L.t2t_int8_linear(x, 1, 300, p, 384, p, None, 0, p, 40, M, 40, K, ws, nb, None)
+        return L.t2t_int8_linear(x, 1, 300, p, p, None, 0, p, 40, M, 40, K, ws, nb, None)
     assert lin(ws=None) == 2 and lin(nb=100) == 2 and b"workspace" in L.t2t_last_error()
     assert lin(ws=odd) == 1 and lin(x=None) == 1 and lin(M=0, ws=None) == 0
 
@@ -99,7 +110,7 @@ def test_the_workspace_never_falls(step):
 def test_cpu_tensors_are_refused():
     x = torch.zeros(4, 64, dtype=torch.bfloat16)
     for f in (lambda: ops.int8_quantize(x), lambda: ops.int8_linear(x, x), lambda: ops.int8_dequantize(x),
-              lambda: ops.Int8(torch.zeros(4, 128, dtype=torch.int8), torch.zeros(4))):
+              lambda: ops.Int8.from_codes(torch.zeros(4, 128, dtype=torch.int8), torch.zeros(4))):
         with pytest.raises(ValueError, match="t2t"):
             f()
 
@@ -114,8 +125,8 @@ def launches(monkeypatch):
 
 
 def _cpu(rows, cols, fill=3):
-    w = -(-cols // 128) * 128
-    return ops.Int8(torch.full((rows, w), fill, dtype=torch.int8), torch.ones(rows), cols)
+    n = -(-rows // 16) * 16 * (-(-cols // 128) * 128)
+    return ops.Int8(torch.full((n,), fill, dtype=torch.int8), torch.ones(rows), rows, cols)
 
 
 @pytest.mark.parametrize("how", ["copy", "deepcopy", "pickle"])
@@ -128,12 +139,12 @@ def test_a_copied_matrix_is_read_at_its_own_address(launches, how):
     ops.int8_quantize(x, out=c)
     ops.int8_linear(x, c)
     ops.int8_linear(c, c)
-    mine = [c.codes.data_ptr(), 128, c.scales.data_ptr()]
-    at = {"t2t_int8_dequantize": [0], "t2t_int8_quantize": [3], "t2t_int8_linear": [3], "t2t_int8_product": [0, 3]}
+    mine = [c.codes.data_ptr(), c.scales.data_ptr()]
+    at = {"t2t_int8_dequantize": [0], "t2t_int8_quantize": [3], "t2t_int8_linear": [3], "t2t_int8_product": [0, 2]}
     assert [name for name, _, _ in launches] == list(at)
     for name, _, args in launches:
         for i in at[name]:
-            assert list(args[i:i + 3]) == mine, name
+            assert list(args[i:i + 2]) == mine, name
 
 
 def test_every_tensor_of_a_call_is_recorded_on_its_stream(launches):
@@ -148,13 +159,13 @@ def test_every_tensor_of_a_call_is_recorded_on_its_stream(launches):
 
 
 @pytest.mark.parametrize("bad", ["k", "type", "stride", "none", "bias", "bias_type", "act", "dtype", "dtype_q", "out",
-                                 "out_type", "out_twice", "weight", "ws", "out_q", "codes", "cols", "wide", "scales",
-                                 "scales_shape", "align", "rows", "in_x", "in_w", "in_bias", "ws_x", "ws_out",
-                                 "q_in_x", "d_in_codes", "apart"])
+                                 "out_type", "out_twice", "weight", "ws", "out_q", "codes", "cols", "size", "scales",
+                                 "scales_shape", "align", "rows", "code_type", "code_dim", "code_cols", "in_x", "in_w",
+                                 "in_bias", "ws_x", "ws_out", "q_in_x", "d_in_codes", "apart"])
 def test_refused(launches, bad):
     z = lambda *s, dtype=torch.bfloat16: torch.zeros(*s, dtype=dtype)  # noqa: E731
     i8, f32 = torch.int8, torch.float32
-    W, x = _cpu(40, 100), z(6, 100)
+    W, V, x = _cpu(40, 100), _cpu(10, 100), z(6, 100)
     buf = z(4000)
     big = torch.zeros(1 << 14, dtype=torch.uint8)
     calls = {
@@ -173,22 +184,25 @@ def test_refused(launches, bad):
         "weight": lambda: ops.int8_linear(x, z(40, 100)),
         "ws": lambda: ops.int8_linear(x, W, ws=z(1 << 16)),
         "out_q": lambda: ops.int8_quantize(x, out=W),
-        "codes": lambda: ops.Int8(z(4, 128), torch.zeros(4)),
-        "cols": lambda: ops.Int8(z(4, 128, dtype=i8), torch.zeros(4), 129),
-        "wide": lambda: ops.Int8(z(4, 256, dtype=i8), torch.zeros(4), 100),
-        "scales": lambda: ops.Int8(z(4, 128, dtype=i8), torch.zeros(4, dtype=F64)),
-        "scales_shape": lambda: ops.Int8(z(4, 128, dtype=i8), torch.zeros(4, 1)),
-        "align": lambda: ops.Int8(z(4 * 128 + 16, dtype=i8)[8:520].view(4, 128), torch.zeros(4)),
-        "rows": lambda: ops.Int8(z(1, 128, dtype=i8).expand(4, 128), torch.zeros(4)),
+        "codes": lambda: ops.Int8(z(2048), torch.zeros(4), 4, 100),
+        "cols": lambda: ops.Int8(z(1 << 21, dtype=i8), torch.zeros(4), 4, 1 << 17),
+        "size": lambda: ops.Int8(z(2048, dtype=i8), torch.zeros(4), 4, 129),
+        "scales": lambda: ops.Int8(z(2048, dtype=i8), torch.zeros(4, dtype=F64), 4, 100),
+        "scales_shape": lambda: ops.Int8(z(2048, dtype=i8), torch.zeros(4, 1), 4, 100),
+        "align": lambda: ops.Int8(z(2056, dtype=i8)[8:], torch.zeros(4), 4, 100),
+        "rows": lambda: ops.Int8(z(2048, dtype=i8), torch.zeros(4), -1, 100),
+        "code_type": lambda: ops.Int8.from_codes(z(4, 100), torch.zeros(4)),
+        "code_dim": lambda: ops.Int8.from_codes(z(400, dtype=i8), torch.zeros(4)),
+        "code_cols": lambda: ops.Int8.from_codes(z(4, 0, dtype=i8), torch.zeros(4)),
         "in_x": lambda: ops.int8_linear(buf[:600].view(6, 100), W, out=buf[500:740].view(6, 40)),
-        "in_w": lambda: ops.int8_linear(x, W, out=W.codes.view(torch.bfloat16).view(-1)[:240].view(6, 40)),
+        "in_w": lambda: ops.int8_linear(x, W, out=W.codes.view(torch.bfloat16)[:240].view(6, 40)),
         "in_bias": lambda: ops.int8_linear(x, W, buf[:40], out=buf[39:279].view(6, 40)),
         "ws_x": lambda: ops.int8_linear(big[:1200].view(torch.bfloat16).view(6, 100), W, ws=big[512:]),
         "ws_out": lambda: ops.int8_linear(x, W, out=big[:480].view(torch.bfloat16).view(6, 40), ws=big[256:]),
         "q_in_x": lambda: ops.int8_quantize(
-            buf[:256].view(2, 128), out=ops.Int8(buf[128:256].view(i8).view(2, 128), torch.zeros(2))),
-        "d_in_codes": lambda: ops.int8_dequantize(W, out=W.codes.view(torch.bfloat16).expand(40, 64)[:, :1].expand(40, 100)),
-        "apart": lambda: ops.Int8(big[:512].view(i8).view(4, 128), big[:16].view(f32))}
+            buf[:256].view(2, 128), out=ops.Int8(buf[128:1152].view(i8), torch.zeros(2), 2, 128)),
+        "d_in_codes": lambda: ops.int8_dequantize(V, out=V.codes.view(torch.bfloat16)[:1000].view(10, 100)),
+        "apart": lambda: ops.Int8(big[:2048].view(i8), big[:16].view(f32), 4, 128)}
     with pytest.raises(ValueError, match="t2t"):
         calls[bad]()
     assert not launches
@@ -258,13 +272,11 @@ def test_quantize_nonfinite_rows_views_and_buffers(dev):
     t = ops.int8_quantize(x)
     _check_codes(t, x)
     assert bool(t.scales[[3, 9, 11]].isnan().all()) and bool(ops.int8_dequantize(t)[9].isnan().all())
-    # into a caller's matrix with rows apart, and values into a strided view
-    codes = torch.full((72, 512), 9, device=dev, dtype=torch.int8)
-    out = ops.Int8(codes[1:71, 128:384], torch.empty(70, device=dev), 200)
+    # into a caller's matrix: rows behind the last stay as they were; values into a strided view
+    out = ops.Int8(torch.full((80 * 256,), 9, device=dev, dtype=torch.int8), torch.empty(70, device=dev), 70, 200)
     assert ops.int8_quantize(x, out=out) is out
-    assert torch.equal(out.codes, t.codes) and torch.equal(out.scales.nan_to_num(7), t.scales.nan_to_num(7))
-    codes[1:71, 128:384] = 9
-    assert bool((codes == 9).all())
+    _check_codes(out, x)
+    assert bool((_rows(out)[70:] == 9).all()) and torch.equal(out.scales.nan_to_num(7), t.scales.nan_to_num(7))
     buf = torch.full((72, 301), 9.0, device=dev, dtype=dt)
     ops.int8_dequantize(t, out=buf[1:71, 5:205])
     assert torch.equal(buf[1:71, 5:205].nan_to_num(3), ops.int8_dequantize(t).nan_to_num(3))
@@ -280,10 +292,11 @@ def test_quantize_more_rows_than_work_groups(dev):
     x = _randn(_gen(dev, 1), 1 << 20, 8).half()
     x = torch.cat((x, x, x, x, x[:37]))
     t = ops.int8_quantize(x)
+    codes = t.to_codes()
     n, s = i8_ref(x[:1 << 20])
     for i in range(4):
-        assert torch.equal(t.codes[i << 20:(i + 1) << 20, :8].double(), n)
-    assert torch.equal(t.codes[4 << 20:, :8].double(), n[:37]) and torch.equal(t.scales[4 << 20:].double(), s[:37])
+        assert torch.equal(codes[i << 20:(i + 1) << 20].double(), n)
+    assert torch.equal(codes[4 << 20:].double(), n[:37]) and torch.equal(t.scales[4 << 20:].double(), s[:37])
 
 
 # ---------------------------------------------------------------------------
@@ -308,8 +321,8 @@ def _linear_ref(a, sa, w, sw, b, act):
 
 def _check_linear(got, x, W, b, act):
     """x: what came in (quantised here by the definition), or an Int8 matrix."""
-    a, sa = (x.codes[:, :x.cols], x.scales) if isinstance(x, ops.Int8) else i8_ref(x)
-    ref, tol = _linear_ref(a, sa, W.codes[:, :W.cols], W.scales, b, act)
+    a, sa = (x.to_codes(), x.scales) if isinstance(x, ops.Int8) else i8_ref(x)
+    ref, tol = _linear_ref(a, sa, W.to_codes(), W.scales, b, act)
     tol = tol + _half_step(ref, got.dtype) * (1 + 2.0 ** -7)
     bad = ~((got.double() - ref).abs() <= tol)
     assert not bool(bad.any()), (int(bad.sum()), bad.nonzero()[:4].tolist())
@@ -352,18 +365,23 @@ TILES = [(3, 40, 96), (40, 100, 700), (1000, 1536, 512), (1000, 1531, 800), (410
 @pytest.mark.parametrize("M,N,K", TILES)
 def test_linear_into_views(dev, M, N, K, dt, act):
     """Outputs of any stride and address get the bits of a contiguous one, nothing
-    around them is written, and weights may have rows apart."""
+    around them is written, and what stands behind the last rows of the operands has
+    no part."""
     dt = HALF[dt]
     x, w, b = _operands(dev, M, N, K, dt, M + N)
     W = ops.int8_quantize(w)
     y = ops.int8_linear(x, W, b, activation=act)
     _check_linear(y, x, W, b, act)
     X = ops.int8_quantize(x)
-    wide = torch.full((N, W.codes.shape[1] + 48), 77, device=dev, dtype=torch.int8)
-    wide[:, 16:-32] = W.codes
-    V = ops.Int8(wide[:, 16:-32], W.scales, K)
-    assert torch.equal(ops.int8_linear(x, V, b, activation=act), y)
-    assert torch.equal(ops.int8_linear(V, X, activation=act, dtype=dt), ops.int8_linear(W, X, activation=act, dtype=dt))
+    assert torch.equal(ops.int8_linear(ops.int8_quantize(x), ops.Int8.from_codes(W.to_codes(), W.scales), b,
+                                       activation=act, dtype=dt), y)
+    full = []
+    for t in (X, W):
+        wide = _rows(t)
+        wide[t.rows:] = 77
+        codes = ops.Int8.from_codes(wide, torch.ones(wide.shape[0], device=dev)).codes
+        full.append(ops.Int8(codes, t.scales, *t.shape))
+    assert torch.equal(ops.int8_linear(*full, b, activation=act, dtype=dt), y)
     for off, width in ((16, N + 24 - N % 8), (4, N + 24 - N % 8), (8, N + 17 - N % 2), (3, N + 17 - N % 2)):
         buf = torch.full((M + 2, width), 5.0, device=dev, dtype=dt)
         out = buf[1:M + 1, off:off + N]
@@ -400,16 +418,13 @@ def test_linear_of_the_longest_sums(dev, M, N):
     """Codes of the largest magnitude over the longest rows, -128 among them: the
     sums fill 31 bits and are exact."""
     K = 131071 if M < 1000 else 20001
-    w = -(-K // 128) * 128
-    def full(rows, code):
-        t = torch.zeros(rows, w, device=dev, dtype=torch.int8)
-        t[:, :K] = code
-        return t
+    full = lambda n, code: torch.full((n, K), code, device=dev, dtype=torch.int8)  # noqa: E731
     ones = lambda n: torch.ones(n, device=dev)  # noqa: E731
-    A = ops.Int8(full(M, -128), 2.0 ** -20 * ones(M), K)
-    A.codes[1::2, :K] = 127
+    a = full(M, -128)
+    a[1::2] = 127
+    A = ops.Int8.from_codes(a, 2.0 ** -20 * ones(M))
     for code, values in ((-128, (16384, -16256)), (127, (-16256, 16129))):
-        y = ops.int8_linear(A, ops.Int8(full(N, code), ones(N), K), dtype=torch.bfloat16)
+        y = ops.int8_linear(A, ops.Int8.from_codes(full(N, code), ones(N)), dtype=torch.bfloat16)
         for i, v in enumerate(values):
             want = torch.tensor(float(v * K), dtype=F64).float().mul(2.0 ** -20).to(torch.bfloat16)
             assert bool((y[i::2] == want.to(dev)).all())

@@ -155,14 +155,13 @@ SIGNATURES = {
     "t2t_mxfp4_linear_ws_bytes": (c_size_t, [c_int, c_int, c_int]),
     "t2t_mxfp4_linear": (c_int, [_P, c_int, c_longlong, _P, _P, _P, c_int, _P, c_longlong, c_int, c_int,
                                  c_int, _P, c_size_t, _P]),
-    "t2t_int8_row_bytes": (c_size_t, [c_int]),
-    "t2t_int8_quantize": (c_int, [_P, c_int, c_longlong, _P, c_longlong, _P, c_int, c_int, _P]),
-    "t2t_int8_dequantize": (c_int, [_P, c_longlong, _P, _P, c_int, c_longlong, c_int, c_int, _P]),
-    "t2t_int8_product": (c_int, [_P, c_longlong, _P, _P, c_longlong, _P, _P, c_int, _P, c_int, c_longlong,
-                                 c_int, c_int, c_int, _P]),
+    "t2t_int8_code_bytes": (c_size_t, [c_int, c_int]),
+    "t2t_int8_quantize": (c_int, [_P, c_int, c_longlong, _P, _P, c_int, c_int, _P]),
+    "t2t_int8_dequantize": (c_int, [_P, _P, _P, c_int, c_longlong, c_int, c_int, _P]),
+    "t2t_int8_product": (c_int, [_P] * 5 + [c_int, _P, c_int, c_longlong] + [c_int] * 3 + [_P]),
     "t2t_int8_linear_ws_bytes": (c_size_t, [c_int, c_int, c_int]),
-    "t2t_int8_linear": (c_int, [_P, c_int, c_longlong, _P, c_longlong, _P, _P, c_int, _P, c_longlong, c_int,
-                                c_int, c_int, _P, c_size_t, _P]),
+    "t2t_int8_linear": (c_int, [_P, c_int, c_longlong, _P, _P, _P, c_int, _P, c_longlong, c_int, c_int,
+                                c_int, _P, c_size_t, _P]),
     "t2t_cache_append": (c_int, [ctypes.POINTER(RotaryTensor)] * 3 + [c_int, _P, _P, _P, c_int, c_int, c_int,
                                                                      c_longlong] + [c_int] * 4 + [c_float, _P]),
     "t2t_cache_attention_ws_bytes": (c_size_t, [c_int, c_int, c_longlong, c_int, c_int, c_int, c_longlong]),

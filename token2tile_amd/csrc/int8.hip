@@ -2,8 +2,13 @@
 // token of the activations, a channel of the weights); quantisation, the values
 // back, and the linear layer on the 8-bit MFMA.
 //
-// An 8-bit matrix [M, K]: codes in rows, row m at m * stride bytes (a multiple of
-// 16), columns K .. Kp - 1 zero, Kp = K rounded up to 128; scales [M].
+// Layout of the codes of a matrix [M, K]: blocks of 16 rows x 64 columns, 1 KB each,
+//   [ceil(M / 16)][Kp / 64][16 rows][4 chunks of 16 bytes], Kp = K rounded up to 128,
+// chunk c of row r at place c ^ ((r >> 2) & 3).  It is the order in which the tiles
+// lie in LDS (the places let the operand reads of sixteen rows meet all banks), so a
+// tile is fetched in whole kilobytes: from plain rows, 64 bytes of each at a time,
+// every fetch took half lines, and 75,600 x 13,824 x 5,120 5.09 ms.  Columns K .. Kp -
+// 1 are zero, rows from M on anything.
 #include "t2t_linear.h"
 #include <type_traits>
 
@@ -13,22 +18,24 @@ typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 #define I8_MAX_K 131071  // 2^7 2^7 K stays below 2^31
 static inline int i8_kp(int K) { return (K + 127) / 128 * 128; }
+// where column c of row r lies, blk bytes to 16 rows (Kp * 16)
+__host__ __device__ static inline int i8_swz(int row) { return (row >> 2) & 3; }
+__device__ inline long long i8_at(long long r, int c, long long blk) {
+  return (r >> 4) * blk + ((c >> 6) << 10) + ((int)(r & 15) << 6) + ((((c >> 4) & 3) ^ i8_swz((int)r)) << 4) + (c & 15);
+}
 
-extern "C" size_t t2t_int8_row_bytes(int K) { return K < 1 || K > I8_MAX_K ? 0 : (size_t)i8_kp(K); }
+extern "C" size_t t2t_int8_code_bytes(int M, int K) {
+  return M < 1 || M > (1 << 30) || K < 1 || K > I8_MAX_K ? 0 : ((size_t)M + 15) / 16 * 16 * i8_kp(K);
+}
 
 static int i8_check_sizes(const char* what, int M, int K) {
   T2T_REQUIRE(M >= 0 && M <= (1 << 30) && K >= 1 && K <= I8_MAX_K, "%s: M=%d K=%d (M <= 2^30, 1 <= K < 2^17)",
               what, M, K);
   return T2T_OK;
 }
-static int i8_check_matrix(const char* what, const void* codes, long long stride, const void* scales, int M,
-                           int K) {
+static int i8_check_matrix(const char* what, const void* codes, const void* scales) {
   T2T_REQUIRE(codes && scales, "%s: null pointer", what);
-  // (a tile's rows are addressed by 32-bit offsets)
-  T2T_REQUIRE((uintptr_t)codes % 16 == 0 && stride % 16 == 0 && stride >= i8_kp(K) && stride <= (1 << 23) &&
-                  (uintptr_t)scales % 4 == 0,
-              "%s: rows of codes must be 16-byte aligned, hold K rounded up to 128 and lie within 8 MiB, stride %lld",
-              what, stride);
+  T2T_REQUIRE((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 4 == 0, "%s: codes must be 16-byte aligned", what);
   return T2T_OK;
 }
 // a 16-bit matrix
@@ -117,8 +124,8 @@ __device__ inline uint32_t i8_top(uint32_t top, const u32x4& v) {  // both halve
 // one read of x, one write of the codes.
 template <typename T, int TPR, int I>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void i8_quantize_kernel(
-    const uint16_t* __restrict__ x, long long row_stride, char* __restrict__ codes, long long stride,
-    float* __restrict__ scales, int M, int K, int Kp) {
+    const uint16_t* __restrict__ x, long long row_stride, char* __restrict__ codes, float* __restrict__ scales, int M,
+    int K, int Kp) {
   constexpr int ROWS = TPR < 256 ? 256 / TPR : 1;
   __shared__ uint32_t tops[16];
   const int t = threadIdx.x % TPR;
@@ -142,25 +149,24 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void i8_quantize_kernel(
     }
     const bool bad = top >= I8Inf<T>::bits;
     const I8Scale k = i8_scale(T::to_f((uint16_t)top));
-    char* dst = codes + row * stride;
 #pragma unroll
     for (int i = 0; i < I; ++i) {
       const int c = 8 * (t + i * TPR);
-      if (c < Kp) *(u32x2*)(dst + c) = bad ? u32x2{0u, 0u} : i8_codes<T>(v[i], k);
+      if (c < Kp) *(u32x2*)(codes + i8_at(row, c, 16LL * Kp)) = bad ? u32x2{0u, 0u} : i8_codes<T>(v[i], k);
     }
     if (t == 0) scales[row] = bad ? __builtin_nanf("") : k.s;
   }
 }
 
 template <typename T>
-static void i8_quantize_launch(const uint16_t* x, long long row_stride, char* codes, long long stride,
-                               float* scales, int M, int K, hipStream_t st) {
+static void i8_quantize_launch(const uint16_t* x, long long row_stride, char* codes, float* scales, int M, int K,
+                               hipStream_t st) {
   const int Kp = i8_kp(K);
   auto go = [&](auto tpr, auto its) {
     constexpr int TPR = decltype(tpr)::value, I = decltype(its)::value, ROWS = TPR < 256 ? 256 / TPR : 1;
     const int wgs = cdiv(M, ROWS);
     hipLaunchKernelGGL((i8_quantize_kernel<T, TPR, I>), dim3(wgs < (1 << 20) ? wgs : 1 << 20),
-                       dim3(TPR < 256 ? 256 : TPR), 0, st, x, row_stride, codes, stride, scales, M, K, Kp);
+                       dim3(TPR < 256 ? 256 : TPR), 0, st, x, row_stride, codes, scales, M, K, Kp);
   };
 #define I8_GO(TPR, I) go(std::integral_constant<int, TPR>{}, std::integral_constant<int, I>{})
   if (Kp <= 512) I8_GO(64, 1);
@@ -175,15 +181,15 @@ static void i8_quantize_launch(const uint16_t* x, long long row_stride, char* co
 #undef I8_GO
 }
 
-extern "C" int t2t_int8_quantize(const void* x, int dtype, long long row_stride, void* codes,
-                                 long long code_stride, float* scales, int M, int K, void* stream) {
+extern "C" int t2t_int8_quantize(const void* x, int dtype, long long row_stride, void* codes, float* scales, int M,
+                                 int K, void* stream) {
   int rc = i8_check_sizes("int8_quantize", M, K);
   if (rc != T2T_OK || M == 0) return rc;
   rc = i8_check_rows("int8_quantize", x, dtype, row_stride, M, K);
-  if (rc == T2T_OK) rc = i8_check_matrix("int8_quantize", codes, code_stride, scales, M, K);
+  if (rc == T2T_OK) rc = i8_check_matrix("int8_quantize", codes, scales);
   if (rc != T2T_OK) return rc;
   (dtype == T2T_BF16 ? i8_quantize_launch<BF16T> : i8_quantize_launch<F16T>)(
-      (const uint16_t*)x, row_stride, (char*)codes, code_stride, scales, M, K, (hipStream_t)stream);
+      (const uint16_t*)x, row_stride, (char*)codes, scales, M, K, (hipStream_t)stream);
   T2T_LAUNCH_CHECK("int8_quantize");
   return T2T_OK;
 }
@@ -192,14 +198,14 @@ extern "C" int t2t_int8_quantize(const void* x, int dtype, long long row_stride,
 // the values back: eight a thread.  Bound: writing them.
 // ---------------------------------------------------------------------------
 template <typename T>
-__global__ __launch_bounds__(256) void i8_dequantize_kernel(const char* __restrict__ codes, long long stride,
+__global__ __launch_bounds__(256) void i8_dequantize_kernel(const char* __restrict__ codes, long long blk,
                                                             const float* __restrict__ scales,
                                                             uint16_t* __restrict__ out, long long row_stride,
                                                             long long units, int per_row, int K) {
   for (long long u = (long long)blockIdx.x * 256 + threadIdx.x; u < units; u += (long long)gridDim.x * 256) {
     const long long row = u / per_row;
     const int c = 8 * (int)(u - row * per_row);
-    const u32x2 v = *(const u32x2*)(codes + row * stride + c);
+    const u32x2 v = *(const u32x2*)(codes + i8_at(row, c, blk));
     const float s = scales[row];
     float f[8];
 #pragma unroll
@@ -210,18 +216,18 @@ __global__ __launch_bounds__(256) void i8_dequantize_kernel(const char* __restri
   }
 }
 
-extern "C" int t2t_int8_dequantize(const void* codes, long long code_stride, const float* scales, void* out,
-                                   int dtype, long long row_stride, int M, int K, void* stream) {
+extern "C" int t2t_int8_dequantize(const void* codes, const float* scales, void* out, int dtype, long long row_stride,
+                                   int M, int K, void* stream) {
   int rc = i8_check_sizes("int8_dequantize", M, K);
   if (rc != T2T_OK || M == 0) return rc;
   rc = i8_check_rows("int8_dequantize", out, dtype, row_stride, M, K);
-  if (rc == T2T_OK) rc = i8_check_matrix("int8_dequantize", codes, code_stride, scales, M, K);
+  if (rc == T2T_OK) rc = i8_check_matrix("int8_dequantize", codes, scales);
   if (rc != T2T_OK) return rc;
   const int per_row = (K + 7) / 8;
   const long long units = (long long)M * per_row, wgs = (units + 255) / 256;
   const dim3 grid((unsigned)(wgs < (1 << 20) ? wgs : 1 << 20));
   auto kernel = dtype == T2T_BF16 ? i8_dequantize_kernel<BF16T> : i8_dequantize_kernel<F16T>;
-  hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, (const char*)codes, code_stride, scales,
+  hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, (const char*)codes, 16LL * i8_kp(K), scales,
                      (uint16_t*)out, row_stride, units, per_row, K);
   T2T_LAUNCH_CHECK("int8_dequantize");
   return T2T_OK;
@@ -234,7 +240,7 @@ extern "C" int t2t_int8_dequantize(const void* codes, long long code_stride, con
 // ---------------------------------------------------------------------------
 struct I8Mat {
   const char* codes;
-  long long stride;
+  long long blk;  // bytes of 16 rows
   const float* scales;
   int rows, blocks;  // rows, row blocks of 32
 };
@@ -261,17 +267,20 @@ __global__ __launch_bounds__(512) void i8_split_kernel(I8Mat a, I8Mat w, const u
   lin_place(id, mt, nt, 1, 1, mb, nb);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = mb * 32 + (lane & 31), feat = nb * 32 + (lane & 31);
-  // (any order of the columns will do that is the same for both: a lane takes 64 bytes of a unit)
-  const char* pw = w.codes + min(feat, w.rows - 1) * w.stride + 64 * (lane >> 5);
-  const char* pa = a.codes + min(row, a.rows - 1) * a.stride + 64 * (lane >> 5);
+  // (rows past the last are read from its block of sixteen, and not stored)
+  const char* pw = w.codes + (min(feat, w.rows - 1) >> 4) * w.blk + (feat & 15) * 64;
+  const char* pa = a.codes + (min(row, a.rows - 1) >> 4) * a.blk + (row & 15) * 64;
+  int at[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) at[i] = (i >> 1) * 1024 + (((2 * (i & 1) + (lane >> 5)) ^ i8_swz(lane)) << 4);
   struct Unit {
     i32x4 w[4], a[4];
   };
   auto load = [&](int s, Unit& t) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      t.w[i] = *(const i32x4*)(pw + (size_t)s * 128 + 16 * i);
-      t.a[i] = *(const i32x4*)(pa + (size_t)s * 128 + 16 * i);
+      t.w[i] = *(const i32x4*)(pw + (size_t)s * 2048 + at[i]);
+      t.a[i] = *(const i32x4*)(pa + (size_t)s * 2048 + at[i]);
     }
   };
   i32x16 acc = {};
@@ -329,15 +338,12 @@ static int i8_split_launch(const I8Mat& a, const I8Mat& w, const uint16_t* bias,
 // ---- tiles staged through LDS ------------------------------------------------
 // Tiles of 64 TW features x 64 TA tokens, four waves of 32 TW x 32 TA each (2 x 2).
 // The weights are the A operand, so a lane holds one token's features 8 (i / 4) +
-// 4 (l / 32) + i % 4 of a block.  A stage is 64 columns: rows of 64 bytes, weights
-// before tokens, fetched by DMA (1 KB, sixteen rows, an instruction; the lane fetches
-// the 16 bytes that belong at its place).  16-byte chunk c of row r lies at c ^ ((r
-// >> 2) & 3), so that the fragment reads (row l % 32, chunk 2 s + l / 32 in lane l for
-// step s) meet all banks.  Four stages are kept.
+// 4 (l / 32) + i % 4 of a block.  A stage is 64 columns, the blocks of the weights
+// before those of the tokens, fetched as they are by DMA (1 KB an instruction); step
+// s of a stage reads row l % 32, chunk 2 s + l / 32 in lane l.  Four stages are kept.
 template <int TW, int TA> struct I8Tile {
   static constexpr int STAGE = 64 * (TW + TA) * 64;
 };
-__device__ inline int i8_swz(int row) { return (row >> 2) & 3; }
 
 // A wave's 32 TA tokens from m on, 32 TW features from n on: 32 tokens x 64 features at a time are
 // scaled, packed, turned through 4 KB of LDS of the wave's own (16-byte chunk c of token t at c ^ (t &
@@ -491,7 +497,7 @@ __global__ __launch_bounds__(256, 1) void i8_big_kernel(I8Mat a, I8Mat w, const 
   if (id >= end) return;
 
   // the stream of stages (n a tile, an even number): tile ld, its stage ls; this wave fetches 128 rows
-  // of the weights (waves 0 and 1) or the tokens, KB i those from 16 i on
+  // of the weights (waves 0 and 1) or the tokens, KB i the block i of them
   const char* g;
   uint32_t v[8];
   int ld = id, ls = 0;
@@ -499,13 +505,10 @@ __global__ __launch_bounds__(256, 1) void i8_big_kernel(I8Mat a, I8Mat w, const 
     int m0, n0;
     lin_place(ld, mt, nt, 8, 8, m0, n0);
     const I8Mat& x = wave < 2 ? w : a;
-    const int first = 32 * (wave < 2 ? n0 : m0), last = x.rows - 1 - first;
-    g = x.codes + first * x.stride;
+    const int first = 2 * (wave < 2 ? n0 : m0), last = (x.rows - 1) / 16 - first;
+    g = x.codes + first * x.blk;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int row = 128 * (wave & 1) + 16 * i + (lane >> 2);
-      v[i] = (uint32_t)(min(row, last) * x.stride) + 16 * ((lane & 3) ^ i8_swz(row));
-    }
+    for (int i = 0; i < 8; ++i) v[i] = (uint32_t)(min(8 * (wave & 1) + i, last) * x.blk) + 16 * lane;
   };
   auto next_pair = [&]() {
     if (ld >= end) return;
@@ -521,7 +524,7 @@ __global__ __launch_bounds__(256, 1) void i8_big_kernel(I8Mat a, I8Mat w, const 
       for (int i = 0; i < 8; ++i) v[i] = 0;
     }
   };
-  auto at = [&](int odd) { return g + (size_t)(ls + odd) * 64; };
+  auto at = [&](int odd) { return g + (size_t)(ls + odd) * 1024; };
   const uint32_t dst = lds0 + wave * 8192;
   auto issue = [&](uint32_t off, int i) {  // KB i of a pair
     asm volatile("s_mov_b32 m0, %[m]\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %[v], %[g]" ::[m] "s"(
@@ -630,17 +633,14 @@ __global__ __launch_bounds__(256, 2) void i8_mid_kernel(I8Mat a, I8Mat w, const 
   const int wn = wave & 1, wm = wave >> 1;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lin_lds_t*)lds;
   const I8Mat& x = wave < 2 ? w : a;
-  const int first = 32 * (wave < 2 ? n0 : m0), last = x.rows - 1 - first;
-  const char* g = x.codes + first * x.stride;
+  const int first = 2 * (wave < 2 ? n0 : m0), last = (x.rows - 1) / 16 - first;
+  const char* g = x.codes + first * x.blk;
   uint32_t v[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = 64 * (wave & 1) + 16 * i + (lane >> 2);
-    v[i] = (uint32_t)(min(row, last) * x.stride) + 16 * ((lane & 3) ^ i8_swz(row));
-  }
+  for (int i = 0; i < 4; ++i) v[i] = (uint32_t)(min(4 * (wave & 1) + i, last) * x.blk) + 16 * lane;
   const uint32_t dst = lds0 + wave * 4096;
   // (past the last stage it is fetched again, so that the counts of loads in flight stay)
-  auto at = [&](int s) { return g + (size_t)min(s, n - 1) * 64; };
+  auto at = [&](int s) { return g + (size_t)min(s, n - 1) * 1024; };
 #pragma unroll
   for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -724,8 +724,8 @@ static int i8_product(const I8Mat& a, const I8Mat& w, const uint16_t* bias, int 
   return i8_tile_launch<T, 2, 2>(a, w, bias, act, out, ldo, units, st);
 }
 
-static int i8_check_product(const char* what, const void* w_codes, long long w_stride, const float* w_scales,
-                            int act, const void* out, int dtype, long long out_row_stride, int M, int N, int K) {
+static int i8_check_product(const char* what, const void* w_codes, const float* w_scales, int act, const void* out,
+                            int dtype, long long out_row_stride, int M, int N, int K) {
   int rc = i8_check_sizes(what, M, K);
   if (rc != T2T_OK) return rc;
   T2T_REQUIRE(act == T2T_ACT_NONE || act == T2T_ACT_GELU_TANH, "%s: activation %d", what, act);
@@ -733,19 +733,19 @@ static int i8_check_product(const char* what, const void* w_codes, long long w_s
   T2T_REQUIRE(dtype == T2T_F16 || dtype == T2T_BF16, "%s: dtype %d", what, dtype);
   if (M == 0) return T2T_OK;
   rc = i8_check_rows(what, out, dtype, out_row_stride, M, N);
-  return rc != T2T_OK ? rc : i8_check_matrix(what, w_codes, w_stride, w_scales, N, K);
+  return rc != T2T_OK ? rc : i8_check_matrix(what, w_codes, w_scales);
 }
 
-extern "C" int t2t_int8_product(const void* a_codes, long long a_stride, const float* a_scales,
-                                const void* w_codes, long long w_stride, const float* w_scales, const void* bias,
-                                int act, void* out, int dtype, long long out_row_stride, int M, int N, int K,
-                                void* stream) {
-  int rc = i8_check_product("int8_product", w_codes, w_stride, w_scales, act, out, dtype, out_row_stride, M, N, K);
+extern "C" int t2t_int8_product(const void* a_codes, const float* a_scales, const void* w_codes,
+                                const float* w_scales, const void* bias, int act, void* out, int dtype,
+                                long long out_row_stride, int M, int N, int K, void* stream) {
+  int rc = i8_check_product("int8_product", w_codes, w_scales, act, out, dtype, out_row_stride, M, N, K);
   if (rc != T2T_OK || M == 0) return rc;
-  rc = i8_check_matrix("int8_product", a_codes, a_stride, a_scales, M, K);
+  rc = i8_check_matrix("int8_product", a_codes, a_scales);
   if (rc != T2T_OK) return rc;
-  const I8Mat a{(const char*)a_codes, a_stride, a_scales, M, cdiv(M, 32)};
-  const I8Mat w{(const char*)w_codes, w_stride, w_scales, N, cdiv(N, 32)};
+  const long long blk = 16LL * i8_kp(K);
+  const I8Mat a{(const char*)a_codes, blk, a_scales, M, cdiv(M, 32)};
+  const I8Mat w{(const char*)w_codes, blk, w_scales, N, cdiv(N, 32)};
   return (dtype == T2T_BF16 ? i8_product<BF16T> : i8_product<F16T>)(a, w, (const uint16_t*)bias, act, (uint16_t*)out,
                                                                    out_row_stride, i8_kp(K) / 128,
                                                                    (hipStream_t)stream);
@@ -754,15 +754,16 @@ extern "C" int t2t_int8_product(const void* a_codes, long long a_stride, const f
 // codes, then scales
 extern "C" size_t t2t_int8_linear_ws_bytes(int M, int N, int K) {
   (void)N;
-  return M < 1 || M > (1 << 30) || K < 1 || K > I8_MAX_K ? 0 : (size_t)M * i8_kp(K) + t2t_align256((size_t)M * 4);
+  const size_t codes = t2t_int8_code_bytes(M, K);
+  return codes ? codes + t2t_align256((size_t)M * 4) : 0;
 }
 
 extern "C" int t2t_int8_linear(const void* x, int dtype, long long x_row_stride, const void* w_codes,
-                               long long w_stride, const float* w_scales, const void* bias, int act, void* out,
+                               const float* w_scales, const void* bias, int act, void* out,
                                long long out_row_stride, int M, int N, int K, void* ws, size_t ws_bytes,
                                void* stream) {
   // everything before the first launch
-  int rc = i8_check_product("int8_linear", w_codes, w_stride, w_scales, act, out, dtype, out_row_stride, M, N, K);
+  int rc = i8_check_product("int8_linear", w_codes, w_scales, act, out, dtype, out_row_stride, M, N, K);
   if (rc != T2T_OK || M == 0) return rc;
   rc = i8_check_rows("int8_linear", x, dtype, x_row_stride, M, K);
   if (rc != T2T_OK) return rc;
@@ -772,9 +773,8 @@ extern "C" int t2t_int8_linear(const void* x, int dtype, long long x_row_stride,
     return T2T_ERR_WORKSPACE;
   }
   T2T_REQUIRE((uintptr_t)ws % 16 == 0, "int8_linear: workspace must be 16-byte aligned");
-  float* scales = (float*)((char*)ws + (size_t)M * i8_kp(K));
-  rc = t2t_int8_quantize(x, dtype, x_row_stride, ws, i8_kp(K), scales, M, K, stream);
+  float* scales = (float*)((char*)ws + t2t_int8_code_bytes(M, K));
+  rc = t2t_int8_quantize(x, dtype, x_row_stride, ws, scales, M, K, stream);
   if (rc != T2T_OK) return rc;
-  return t2t_int8_product(ws, i8_kp(K), scales, w_codes, w_stride, w_scales, bias, act, out, dtype, out_row_stride,
-                          M, N, K, stream);
+  return t2t_int8_product(ws, scales, w_codes, w_scales, bias, act, out, dtype, out_row_stride, M, N, K, stream);
 }

@@ -1266,62 +1266,67 @@ _I8_MAX_COLS = 2 ** 17 - 1  # the sums stay in 32 bits
 
 
 class Int8:
-    """A matrix [rows, cols] in 8 bits (``int8_quantize``, or the codes and scales of
-    a checkpoint): ``codes`` int8 [rows, cols rounded up to 128] with zeros from
-    column ``cols`` on (which is not checked), rows of contiguous codes, 16-byte
-    aligned; ``scales`` fp32 [rows].  Element (i, j) stands for codes[i, j] *
-    scales[i].  Both are on the GPU and are checked here, once."""
+    """A matrix [rows, cols] in 8 bits: whole numbers -127 .. 127 and an fp32 scale
+    for each row (``int8_quantize``; ``from_codes`` for those of a checkpoint).
+    ``codes`` (int8) and ``scales`` are the buffers on the GPU, the codes in the
+    order of the products' tiles (include/t2t_hip.h); they are checked here, once."""
 
     # (addresses and device are the buffers' at each call: a copied, pickled or loaded matrix has others)
-    __slots__ = ("_codes", "_scales", "_cols")
+    __slots__ = ("_codes", "_scales", "_rows", "_cols")
 
-    def __init__(self, codes, scales, cols=None):
+    def __init__(self, codes, scales, rows, cols):
+        rows, cols = int(rows), int(cols)
+        if not (0 <= rows <= 2 ** 30 and 1 <= cols <= _I8_MAX_COLS):
+            raise ValueError(f"t2t: an 8-bit matrix has 1 to 2^17 - 1 columns, got {rows} x {cols}")
         dev = _dev(codes)
-        if codes.dtype != torch.int8 or codes.dim() != 2:
-            raise ValueError(f"t2t: codes must be an int8 matrix, got {codes.dtype} {tuple(codes.shape)}")
-        rows, wide = codes.shape
-        cols = wide if cols is None else int(cols)
-        if not (0 <= rows <= 2 ** 30 and 1 <= cols <= _I8_MAX_COLS and wide == _i8_cols(cols)):
-            raise ValueError(f"t2t: {cols} columns (1 to 2^17 - 1) are held as {_i8_cols(max(cols, 1))} with zeros "
-                             f"behind them, got {rows} x {wide}")
+        _check(codes, (_i8_bytes(rows, cols),), torch.int8, "codes", dev)
         _check(scales, (rows,), _f32, "scales", dev)
-        stride = codes.stride(0) if rows > 1 else wide
-        if codes.stride(1) != 1 or not wide <= stride <= 2 ** 23 or stride % 16 or codes.data_ptr() % 16:
-            raise ValueError(f"t2t: the rows of codes must be contiguous, 16-byte aligned and apart (at most 8 MiB), got "
-                             f"strides {tuple(codes.stride())}")
-        if rows and _near(*_span(codes), ((scales.data_ptr(), scales.nbytes),)) and _meet(codes, scales):
+        if rows and codes.data_ptr() % 16:
+            raise ValueError("t2t: codes must be 16-byte aligned")
+        if _near(*_span(codes), ((scales.data_ptr(), scales.nbytes),)):
             raise ValueError("t2t: scales shares memory with codes")
-        self._set(codes, scales, cols)
+        self._set(codes, scales, rows, cols)
 
-    def _set(self, codes, scales, cols):
-        self._codes, self._scales, self._cols = codes, scales, cols
+    def _set(self, codes, scales, rows, cols):
+        self._codes, self._scales, self._rows, self._cols = codes, scales, rows, cols
         return self
+
+    @classmethod
+    def from_codes(cls, codes, scales):
+        """From whole numbers int8 [rows, cols] in rows and their scales fp32 [rows],
+        which are copied."""
+        if not isinstance(codes, torch.Tensor) or codes.dtype != torch.int8 or codes.dim() != 2:
+            raise ValueError("t2t: codes must be an int8 [rows, cols] tensor")
+        rows, cols = codes.shape
+        if not 1 <= cols <= _I8_MAX_COLS:
+            raise ValueError(f"t2t: an 8-bit matrix has 1 to 2^17 - 1 columns, got {rows} x {cols}")
+        wide = codes.new_zeros(-(-rows // 16) * 16, -(-cols // 128) * 128)
+        wide[:rows, :cols] = codes
+        blocks = wide.view(-1, 4, 4, wide.shape[1] // 64, 4, 16)     # row r as (r / 4, r % 4)
+        blocks = torch.stack([blocks[:, i][..., [c ^ i for c in range(4)], :] for i in range(4)], 1)
+        return cls(blocks.permute(0, 3, 1, 2, 4, 5).contiguous().view(-1), scales.clone(), rows, cols)
+
+    def to_codes(self):
+        """The whole numbers in rows, int8 [rows, cols]."""
+        blocks = self._codes.view(-(-self._rows // 16), -(-self._cols // 128) * 2, 4, 4, 4, 16)
+        blocks = torch.stack([blocks[:, :, i][..., [c ^ i for c in range(4)], :] for i in range(4)], 2)
+        wide = blocks.permute(0, 2, 3, 1, 4, 5).reshape(-(-self._rows // 16) * 16, -(-self._cols // 128) * 128)
+        return wide[:self._rows, :self._cols].contiguous()
 
     codes = property(lambda self: self._codes)
     scales = property(lambda self: self._scales)
-    rows = property(lambda self: self._codes.shape[0])
+    rows = property(lambda self: self._rows)
     cols = property(lambda self: self._cols)
-    shape = property(lambda self: (self._codes.shape[0], self._cols))
+    shape = property(lambda self: (self._rows, self._cols))
     device = property(lambda self: self._codes.device)
 
     def __repr__(self):
-        return f"Int8({self.rows} x {self._cols}, {self.device})"
+        return f"Int8({self._rows} x {self._cols}, {self.device})"
 
 
-def _i8_cols(cols):
-    """Columns that are held (t2t_int8_row_bytes)."""
-    return (cols + 127) & ~127
-
-
-def _i8_args(t):
-    """Addresses and row stride of an Int8 matrix."""
-    codes = t._codes
-    return codes.data_ptr(), codes.stride(0) if codes.shape[0] > 1 else codes.shape[1], t._scales.data_ptr()
-
-
-def _i8_spans(t):
-    p, end = _span(t._codes)
-    return [(p, end - p), (t._scales.data_ptr(), t._scales.nbytes)]
+def _i8_bytes(rows, cols):
+    """Bytes of the codes (t2t_int8_code_bytes)."""
+    return -(-rows // 16) * 16 * (-(-cols // 128) * 128)
 
 
 def _x_span(x, rows, cols, stride):
@@ -1338,16 +1343,17 @@ def int8_quantize(x, out=None, stream=None):
     M, K, stride = _mx_rows(x, "x", dev, 2)
     if not (1 <= K <= _I8_MAX_COLS and M <= 2 ** 30):
         raise ValueError(f"t2t: x must have 1 to 2^17 - 1 columns, got {M} x {K}")
-    if out is None:
-        out = Int8.__new__(Int8)._set(_empty(stream, (M, _i8_cols(K)), torch.int8, dev),
-                                      _empty(stream, (M,), _f32, dev), K)
+    given = out is not None
+    if not given:
+        out = Int8.__new__(Int8)._set(_empty(stream, (_i8_bytes(M, K),), torch.int8, dev),
+                                      _empty(stream, (M,), _f32, dev), M, K)
     elif not isinstance(out, Int8) or out.shape != (M, K) or _dev(out._codes) != dev:
         raise ValueError(f"t2t: out must be an Int8 matrix {M} x {K} on {dev}, got {out!r}")
-    elif _near(*_span(x), _i8_spans(out)):
-        _apart((out._codes, out._scales), ("out.codes", "out.scales"), (None, None, x))
-    pc, cs, ps = _i8_args(out)
-    _launch("t2t_int8_quantize", dev, stream, (x, out._codes, out._scales), x.data_ptr(), dtype_code(x.dtype),
-            stride, pc, cs, ps, M, K)
+    codes, scales = out._codes, out._scales
+    px, pc, ps = x.data_ptr(), codes.data_ptr(), scales.data_ptr()
+    if given and _near(px, px + 2 * ((M - 1) * stride + K), ((pc, codes.nbytes), (ps, scales.nbytes))):
+        _apart((codes, scales), ("out.codes", "out.scales"), (None, None, x))
+    _launch("t2t_int8_quantize", dev, stream, (x, codes, scales), px, dtype_code(x.dtype), stride, pc, ps, M, K)
     return out
 
 
@@ -1356,7 +1362,8 @@ def int8_dequantize(t, dtype=torch.bfloat16, out=None, stream=None):
     rounded once."""
     if not isinstance(t, Int8):
         raise ValueError("t2t: expected an Int8 matrix")
-    dev = _dev(t._codes)
+    codes, scales = t._codes, t._scales
+    dev = codes.device if codes.is_cuda else _dev(codes)
     _on(stream, dev)
     code = _mx_dtype(dtype)
     if out is None:
@@ -1366,10 +1373,9 @@ def int8_dequantize(t, dtype=torch.bfloat16, out=None, stream=None):
         M, K, stride = _mx_rows(out, "out", dev, 2)
         if (M, K) != t.shape or out.dtype != dtype:
             raise ValueError(f"t2t: out must be {dtype} {t.shape}, got {out.dtype} {tuple(out.shape)}")
-        _apart((out,), ("out",), (None, t._codes, t._scales))
-    pc, cs, ps = _i8_args(t)
-    _launch("t2t_int8_dequantize", dev, stream, (t._codes, t._scales, out), pc, cs, ps, out.data_ptr(), code,
-            stride, *t.shape)
+        _apart((out,), ("out",), (None, codes, scales))
+    _launch("t2t_int8_dequantize", dev, stream, (codes, scales, out), codes.data_ptr(), scales.data_ptr(),
+            out.data_ptr(), code, stride, *t.shape)
     return out
 
 
@@ -1391,13 +1397,13 @@ def int8_linear(x, weight, bias=None, *, activation=None, dtype=None, out=None, 
     wc, wsc = weight._codes, weight._scales
     dev = wc.device if wc.is_cuda else _dev(wc)
     _on(stream, dev)
-    N = wc.shape[0]
+    N = weight._rows
     shared = isinstance(x, Int8)
     if shared:
         xs = x._codes, x._scales
         if xs[0].device != dev:
             raise ValueError(f"t2t: x must be on {dev}")
-        M, K = x.shape
+        M, K = x._rows, x._cols
         shape = (M, N)
         dt = torch.bfloat16 if dtype is None else dtype
         code = _mx_dtype(dt)
@@ -1413,11 +1419,11 @@ def int8_linear(x, weight, bias=None, *, activation=None, dtype=None, out=None, 
         raise ValueError(f"t2t: activation {activation!r} (None or gelu_tanh)")
     if bias is not None and not _is(bias, (N,), dt, dev):
         _check(bias, (N,), dt, "bias", dev)
-    args = *_i8_args(weight), None if bias is None else bias.data_ptr()
+    args = wc.data_ptr(), wsc.data_ptr(), None if bias is None else bias.data_ptr()
     spans = None  # of the inputs, where the caller brings an output or a workspace
     if out is not None or ws is not None:
-        spans = _i8_spans(weight) + [(args[3], 2 * N)] * (bias is not None)
-        spans += _i8_spans(x) if shared else [_x_span(x, M, K, stride)]
+        spans = [(args[0], wc.nbytes), (args[1], wsc.nbytes)] + [(args[2], 2 * N)] * (bias is not None)
+        spans += [(t.data_ptr(), t.nbytes) for t in xs] if shared else [_x_span(x, M, K, stride)]
     if out is None:
         out = _empty(stream, shape, dt, dev) if stream is not None or shared else x.new_empty(shape)
         ostride, po = N, out.data_ptr()
@@ -1426,12 +1432,12 @@ def int8_linear(x, weight, bias=None, *, activation=None, dtype=None, out=None, 
         if tuple(out.shape) != shape or out.dtype != dt:
             raise ValueError(f"t2t: out must be {dt} {shape}, got {out.dtype} {tuple(out.shape)}")
         po = out.data_ptr()
-        if _near(*_span(out), spans):
+        if _near(po, po + 2 * ((M - 1) * ostride + N), spans):
             _apart((out,), ("out",), (None, *(xs if shared else (x,)), wc, wsc, bias))
     args = *args, _ACTIVATIONS[activation], po
     if shared:
-        _launch("t2t_int8_product", dev, stream, (*xs, wc, wsc, bias, out), *_i8_args(x), *args, code, ostride,
-                M, N, K)
+        _launch("t2t_int8_product", dev, stream, (*xs, wc, wsc, bias, out), xs[0].data_ptr(), xs[1].data_ptr(), *args,
+                code, ostride, M, N, K)
     else:
         need = int8_linear_ws_bytes(M, N, K)
         if ws is not None:
