@@ -10,7 +10,16 @@
 #include <type_traits>
 
 typedef __attribute__((address_space(3))) void ca_lds_t;
-typedef const __attribute__((address_space(1))) void ca_glb_t;
+
+// 1 KB to LDS, 16 bytes a lane in the order of the lanes.  (In assembly: of the builtin the compiler
+// knows no more than that it writes LDS, and has the transposing reads wait for every one in flight.
+// The waits and barriers that order them are written out.)
+__device__ inline void ca_dma(const char* from, uint16_t* to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(
+                   __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(ca_lds_t*)to)),
+               "v"(from)
+               : "memory");
+}
 
 #define CA_NONE (-1.0e30f)  // the running maximum before any key: finite, so that rows of hidden keys add 0
 
@@ -25,6 +34,7 @@ struct CacheArgs {
   int B, N, T, HQ, HK, G, pages, page, shift, width, mask_cols, causal;
   float c;  // scale log2(e)
   int S;    // most parts of a sequence's keys
+  int tiles, items;  // row blocks; with the parts and key heads
   float* opart;
   float* mlpart;
 };
@@ -110,20 +120,20 @@ struct CacheState {
   float m, l;
 };
 
-// the four operand parts of 32 keys and dim block nb, from the transposing reads: lane l gets dim l %
-// 32 of keys 16 i / 2 + 8 (i % 2) + 4 (l / 32) + 0 .. 3
-template <int D, int BASE>
-__device__ inline void ca_vread(u32x2 (&f)[4], uint32_t a) {
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %4 offset:%c5\n\t"
-      "ds_read_b64_tr_b16 %1, %4 offset:%c6\n\t"
-      "ds_read_b64_tr_b16 %2, %4 offset:%c7\n\t"
-      "ds_read_b64_tr_b16 %3, %4 offset:%c8"
-      : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f[2]), "=&v"(f[3])
-      : "v"(a), "n"(BASE), "n"(BASE + 16 * D), "n"(BASE + 32 * D), "n"(BASE + 48 * D));
+// the four operand parts of 32 keys and a block of dims, from the transposing reads: in a 16-lane group
+// lane i gets, in slot k, element i % 4 of the 8 bytes that lane 4 k + i / 4 addresses.  Lane l
+// addresses key 8 r + 4 (l / 32) + (l % 16) / 4 at dims 16 ((l / 16) % 2) + 4 (l % 4) .. + 3 and so gets
+// dim l % 32 of keys 8 r + 4 (l / 32) + 0 .. 3, the order the weights are packed in.
+__device__ inline int ca_trkey(int lane) { return 4 * (lane >> 5) + ((lane & 15) >> 2); }
+template <int D> __device__ inline int ca_trat(int lane, int nb) {  // halves; + 8 r D for r
+  const int key = ca_trkey(lane), dim = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  return key * D + 8 * ((4 * nb + (dim >> 3)) ^ ca_vswz<D>(key)) + (dim & 7);
 }
-#define CA_WAIT4(f, n) \
-  asm volatile("s_waitcnt lgkmcnt(" #n ")" : "+v"(f[0]), "+v"(f[1]), "+v"(f[2]), "+v"(f[3]))
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+__device__ inline u32x2 ca_trread(const uint16_t* p) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (__attribute__((address_space(3))) s16x4*)p));
+}
 
 // The lane's row in the mask: hidden are positions past the length, new ones past `last` (causal)
 // and, with a mask, those it does not name.
@@ -135,7 +145,33 @@ struct CacheSight {
     if (!mask || pos < first) return true;
     return pos - first < cols && mask[pos - first] != 0;
   }
+  // of four positions from pos on, a bit each
+  __device__ uint32_t sees4(int pos) const {
+    const int i = pos - first;
+    if (mask && i >= 0 && i + 3 < cols && pos + 3 <= last) {
+      uint32_t x;
+      __builtin_memcpy(&x, mask + i, 4);
+      return (uint32_t)((x & 0xffu) != 0) | (uint32_t)((x & 0xff00u) != 0) << 1 | (uint32_t)((x & 0xff0000u) != 0) << 2 |
+             (uint32_t)((x & 0xff000000u) != 0) << 3;
+    }
+    uint32_t x = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x |= (uint32_t)sees(pos + e) << e;
+    return x;
+  }
 };
+
+// Which part, key head and row block a work-group takes.  Consecutive work-groups go to the eight XCDs
+// in turn: each takes a run of items, the row blocks of one part and key head next to each other, which
+// then share their keys in its L2.  (Under causal the last row blocks, which see the most, go first.)
+__device__ inline bool ca_item(const CacheArgs& A, int& part, int& kh, int& tile) {
+  const int per = (A.items + 7) / 8, id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+  if (id >= min(A.items, ((int)(blockIdx.x & 7) + 1) * per)) return false;
+  tile = id % A.tiles;
+  if (A.causal) tile = A.tiles - 1 - tile;
+  part = id / A.tiles % A.S, kh = id / A.tiles / A.S;
+  return true;
+}
 
 // s -> weights against the running maximum (exp2 scales exactly, so it only has to keep the weights in
 // the range of T: it moves where they leave it, and the sums so far with it)
@@ -177,11 +213,11 @@ __device__ inline void ca_weights(CacheState<T, D>& w, const f32x16 (&s)[NK], u3
 }
 
 // Whether a tile's operand parts hold an inf or NaN, and those parts without them
-template <typename T>
-__device__ inline bool ca_clean(u32x2 (&f)[4]) {
+template <typename T, int N>
+__device__ inline bool ca_clean(u32x2 (&f)[N]) {
   bool any = false;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const uint32_t lo = (f[i][e] & CaType<T>::inf) == CaType<T>::inf ? 0u : f[i][e] & 0xffffu;
@@ -205,7 +241,8 @@ __global__ __launch_bounds__(256, 1) void ca_few_kernel(CacheArgs A) {
   __shared__ float sM[WAVES][32], sL[WAVES][32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int jl = lane & 31, hh = lane >> 5;
-  const int part = blockIdx.x % A.S, kh = blockIdx.x / A.S % A.HK, tile = blockIdx.x / A.S / A.HK;
+  int part, kh, tile;
+  if (!ca_item(A, part, kh, tile)) return;
   CacheRows w;
   if (!ca_rows<32>(A, tile, w)) return;
   const int parts = ca_parts(w.L, A.S);
@@ -238,18 +275,14 @@ __global__ __launch_bounds__(256, 1) void ca_few_kernel(CacheArgs A) {
     for (int i = 0; i < 32 / RPI; ++i) {
       const int row = RPI * i + lane / LPR;
       const size_t at = (size_t)(uint32_t)__shfl((int)off, row, 64) * 16;
-      __builtin_amdgcn_global_load_lds((ca_glb_t*)(kbase + at + 16 * ((lane & (LPR - 1)) ^ ca_kswz<D>(row))),
-                                       (ca_lds_t*)(dk + i * 512), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((ca_glb_t*)(vbase + at + 16 * ((lane & (LPR - 1)) ^ ca_vswz<D>(row))),
-                                       (ca_lds_t*)(dv + i * 512), 16, 0, 0);
+      ca_dma(kbase + at + 16 * ((lane & (LPR - 1)) ^ ca_kswz<D>(row)), dk + i * 512);
+      ca_dma(vbase + at + 16 * ((lane & (LPR - 1)) ^ ca_vswz<D>(row)), dv + i * 512);
     }
   };
-  const int trkey = 4 * hh + ((lane & 15) >> 2), trdim = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
   // BAD: lanes whose key's table entry lies outside the cache
   auto step = [&](int t, uint64_t bad, auto BUF) __attribute__((always_inline)) {
     const uint16_t* sk = (decltype(BUF)::value ? sK1 : sK0) + wave * TILE;
     const uint16_t* sv = (decltype(BUF)::value ? sV1 : sV0) + wave * TILE;
-    const uint32_t va = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint16_t*)sv;
     f32x16 s[1] = {zero16()};
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
@@ -272,8 +305,9 @@ __global__ __launch_bounds__(256, 1) void ca_few_kernel(CacheArgs A) {
 #pragma unroll
     for (int nb = 0; nb < D / 32; ++nb) {
       u32x2 f[4];
-      ca_vread<D, 0>(f, va + 2 * (trkey * D + 8 * ((4 * nb + (trdim >> 3)) ^ ca_vswz<D>(trkey)) + (trdim & 7)));
-      CA_WAIT4(f, 0);
+      const uint16_t* at = sv + ca_trat<D>(lane, nb);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = ca_trread(at + 8 * i * D);
       if (hide) odd |= ca_clean<T>(f);
 #pragma unroll
       for (int mm = 0; mm < 2; ++mm)
@@ -377,12 +411,364 @@ __global__ __launch_bounds__(256, 1) void ca_few_kernel(CacheArgs A) {
   if (A.lse && d0 == 0) A.lse[at] = lt == 0.f ? -__builtin_inff() : 0.6931471805599453f * (sM[0][rr] + __log2f(lt));
 }
 
+// c += a b with c in accumulation registers (the compiler's choice moved them back and forth).  The
+// operands have been written long before; who reads c waits.
+template <typename T> __device__ inline void ca_mfma_a(f32x16& c, const u32x4& a, const u32x4& b) {
+  if constexpr (T::code == T2T_BF16)
+    asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  else
+    asm("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+
+// ---- many rows: a work-group's waves share the keys --------------------------
+// 128 RB packed rows a work-group, 32 RB a wave; tiles of 64 keys, fetched by all
+// waves for all (DMA, one barrier a tile).  Tiles of which every row sees every key
+// go through a pipeline of half tiles: a turn computes the scores of the next half,
+// the weights of this one and the sums of the last, in steps of RB products each with
+// the weights' vector operations between them: a SIMD holds one wave, and the matrix
+// unit has work while the exponentials are taken.  The other tiles follow, one after
+// the other.
+template <typename T, int D, int RB>
+__global__ __launch_bounds__(256, 1) void ca_many_kernel(CacheArgs A) {
+  constexpr int ROWS = 128 * RB, LPR = D / 8, RPI = 64 / LPR, NB = D / 32, NS = D / 16;
+  constexpr int PAIRS = 8 * RB;  // of weights in a half tile
+  __shared__ __attribute__((aligned(1024))) uint16_t sK0[64 * D], sK1[64 * D], sV0[64 * D], sV1[64 * D];
+  __shared__ uint32_t sBad[2][4];  // a wave's sixteen keys whose table entry lies outside the cache
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int jl = lane & 31, hh = lane >> 5;
+  int part, kh, tile;
+  if (!ca_item(A, part, kh, tile)) return;
+  CacheRows w;
+  if (!ca_rows<ROWS>(A, tile, w)) return;
+  const int parts = ca_parts(w.L, A.S);
+  if (part >= parts) return;
+  const int wr0 = w.r0 + 32 * RB * wave;      // the wave's first row
+  const bool live = wr0 < w.rows;             // (of the wave)
+  u32x4 q[RB][NS];
+  f32x16 o[RB][NB];
+  float m[RB], l[RB];
+  auto row_of = [&](int b, int& tok, int& head) {
+    const int r = min(wr0 + 32 * b + jl, w.rows - 1);
+    tok = r / A.G, head = kh * A.G + r - tok * A.G;
+  };
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    int tok, head;
+    row_of(b, tok, head);
+    const char* qr = ca_token(A.q, A, w, A.q_batch, A.q_row, tok) + head * A.q_head + 16 * hh;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) q[b][s] = *(const u32x4*)(qr + 32 * s);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) o[b][nb] = zero16();
+    m[b] = CA_NONE, l[b] = 0.f;
+  }
+  // keys that some row of the work-group sees; from `plain` on not every row sees every key
+  const int tok0 = w.r0 / A.G, tok1 = (min(w.r0 + ROWS, w.rows) - 1) / A.G;
+  const int keys = A.causal ? min(w.L, w.first + tok1 + 1) : w.L;
+  const int plain = max(0, A.mask ? w.first : A.causal ? w.first + tok0 + 1 : w.L);
+  const int all = max(0, (keys + 63) / 64);
+  const int t0 = (int)((long long)part * all / parts), nt = (int)((long long)(part + 1) * all / parts) - t0;
+  const char* kbase = A.k + kh * A.kv_head;
+  const char* vbase = A.v + kh * A.kv_head;
+  const int32_t* table = A.table + w.b * A.table_row;
+  // tiles of the pipeline: none where an entry of the table lies outside the cache
+  int nf = min(nt, max(0, plain / 64 - t0));
+  {
+    bool bad = false;
+    const int e0 = nf > 0 ? 64 * t0 / A.page : 0, e1 = nf > 0 ? (64 * (t0 + nf) - 1) / A.page : -1;
+    for (int e = e0 + threadIdx.x; e <= e1; e += 256) bad |= (uint32_t)table[e] >= (uint32_t)A.pages;
+    if (__syncthreads_or(bad)) nf = 0;
+  }
+
+  // this wave fetches keys 16 wave .. + 15 of every tile; lane l looks key l % 16 up
+  auto pos_of = [&](int t) { return min(64 * (t0 + t) + 16 * wave + (lane & 15), w.L - 1); };
+  auto fetch = [&](const char* base, uint16_t* to, uint32_t off, auto KEYS) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 16 / RPI; ++i) {
+      const int in = RPI * i + lane / LPR, row = 16 * wave + in;
+      const size_t at = (size_t)(uint32_t)__shfl((int)off, in, 64) * 16;
+      const int swz = decltype(KEYS)::value ? ca_kswz<D>(row) : ca_vswz<D>(row);
+      ca_dma(base + at + 16 * ((lane & (LPR - 1)) ^ swz), to + (16 * wave + RPI * i) * D);
+    }
+  };
+  using Yes = std::true_type;
+  using No = std::false_type;
+  // where the lane's operands lie (halves): K of step s, V of dim block nb
+  auto kat = [&](int s) { return jl * D + 8 * ((2 * s + hh) ^ ca_kswz<D>(jl)); };
+  auto vat = [&](int nb) { return ca_trat<D>(lane, nb); };
+  // the rare move of the running maximum: S are the half tile's scores, whose weights left the range
+  auto move = [&](int b, const f32x16& S) __attribute__((always_inline)) {
+    float mr = -__builtin_inff();
+#pragma unroll
+    for (int a = 0; a < 16; ++a) mr = __builtin_elementwise_maximum(mr, S[a]);
+    const float mx = half_max(mr) * A.c - CaType<T>::top;
+    const float mnew = mx > m[b] || mx != mx ? mx : m[b];
+    const float alpha = __builtin_amdgcn_exp2f(m[b] - mnew);
+    m[b] = mnew;
+    l[b] *= alpha;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int a = 0; a < 16; ++a) o[b][nb][a] *= alpha;
+  };
+  // weight pair i of 8 RB: rows i / 8, elements 2 (i % 8), + 1
+  auto weigh = [&](int i, const f32x16 (&S)[RB], u32x4 (&P)[RB][2], float (&lt)[RB]) __attribute__((always_inline)) {
+    const int b = i / 8, a = 2 * (i % 8);
+    const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[b][a], A.c, -m[b]));
+    const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[b][a + 1], A.c, -m[b]));
+    const uint32_t pk = Pk<T>::pack(x0, x1);
+    lt[b] = Pk<T>::sum2(pk, lt[b]);
+    P[b][a / 8][(a % 8) / 2] = pk;
+  };
+  // the sums are in accumulation registers, written by the assembly below, whose results are
+  // readable after 18 cycles of issue
+  auto ready = [&]() __attribute__((always_inline)) {
+    asm volatile("s_nop 15\n\ts_nop 15");
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) asm volatile("" : "+a"(o[b][nb]));
+  };
+  auto settle = [&](const f32x16 (&S)[RB], u32x4 (&P)[RB][2], float (&lt)[RB]) __attribute__((always_inline)) {
+    bool far = false;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) far |= !(lt[b] <= CaType<T>::limit);
+    if (__builtin_amdgcn_readfirstlane((int)(__ballot(far) != 0ull))) {
+      ready();
+#pragma unroll
+      for (int b = 0; b < RB; ++b) move(b, S[b]), lt[b] = 0.f;
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) weigh(i, S, P, lt);
+    }
+#pragma unroll
+    for (int b = 0; b < RB; ++b) l[b] += lt[b];
+  };
+  auto scores = [&](f32x16 (&S)[RB], const uint16_t* kt) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const u32x4 f = *(const u32x4*)(kt + kat(s));
+#pragma unroll
+      for (int b = 0; b < RB; ++b) S[b] = Mfma<T>::run(f, q[b][s], s ? S[b] : zero16());
+    }
+  };
+  // One turn: S of this half tile's scores -> P, the scores SX of the half tile in kt, the sums of the
+  // one in vt with its weights PP.
+  auto turn = [&](const f32x16 (&S)[RB], f32x16 (&SX)[RB], u32x4 (&P)[RB][2], const u32x4 (&PP)[RB][2],
+                  const uint16_t* kt, const uint16_t* vt) __attribute__((always_inline)) {
+    constexpr int AHEAD = 2, STEPS = NS;
+    static_assert(NS == 2 * NB, "a turn's steps come in pairs");
+    float lt[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) lt[b] = 0.f;
+    u32x4 kf[AHEAD + 1];
+    u32x2 vf[AHEAD + 1][2];
+    auto rdk = [&](int i) __attribute__((always_inline)) { kf[i % (AHEAD + 1)] = *(const u32x4*)(kt + kat(i)); };
+    auto rdv = [&](int i) __attribute__((always_inline)) {
+      const uint16_t* at = vt + vat(i / 2) + 16 * (i % 2) * D;
+      vf[i % (AHEAD + 1)][0] = ca_trread(at);
+      vf[i % (AHEAD + 1)][1] = ca_trread(at + 8 * D);
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) rdv(i), rdk(i);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (i + AHEAD < STEPS) rdv(i + AHEAD);
+      const u32x2 f0 = vf[i % (AHEAD + 1)][0], f1 = vf[i % (AHEAD + 1)][1];
+      const u32x4 f{f0[0], f0[1], f1[0], f1[1]};
+#pragma unroll
+      for (int b = 0; b < RB; ++b) ca_mfma_a<T>(o[b][i / 2], f, PP[b][i % 2]);
+#pragma unroll
+      for (int j = (2 * i) * PAIRS / (2 * STEPS); j < (2 * i + 1) * PAIRS / (2 * STEPS); ++j) weigh(j, S, P, lt);
+      __builtin_amdgcn_sched_barrier(0);
+      if (i + AHEAD < STEPS) rdk(i + AHEAD);
+#pragma unroll
+      for (int b = 0; b < RB; ++b) SX[b] = Mfma<T>::run(kf[i % (AHEAD + 1)], q[b][i], i ? SX[b] : zero16());
+#pragma unroll
+      for (int j = (2 * i + 1) * PAIRS / (2 * STEPS); j < (2 * i + 2) * PAIRS / (2 * STEPS); ++j) weigh(j, S, P, lt);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    settle(S, P, lt);
+  };
+
+  if (nf > 0) {
+    f32x16 s0[RB], s1[RB];
+    u32x4 p0[RB][2], p1[RB][2];
+    bool ok;
+    auto find = [&](int t, uint32_t entry) { return ca_offset(A, entry, pos_of(t), ok); };
+    // (tiles past the last of the pipeline are fetched like it, and not used)
+    auto last = [&](int t) { return min(t, nf - 1); };
+    // offsets of tiles t + 1 and t + 2; the table's entry of tile t + 3
+    uint32_t off0 = find(0, ca_entry(A, table, pos_of(0))), off1 = find(last(1), ca_entry(A, table, pos_of(last(1)))),
+             off2 = find(last(2), ca_entry(A, table, pos_of(last(2)))), entry = ca_entry(A, table, pos_of(last(3)));
+    fetch(kbase, sK0, off0, Yes{});
+    // before the first half tile: values and weights of zero
+    for (int i = threadIdx.x; i < 8 * D; i += 256) *(u32x4*)(sV1 + 8 * i) = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) p1[b][i] = u32x4{0u, 0u, 0u, 0u};
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    fetch(kbase, sK1, off1, Yes{});
+    fetch(vbase, sV0, off0, No{});
+    if (live) scores(s0, sK0);
+    // tile t, whose first half's scores are there; K of t + 1 and V of t have been asked for
+    auto round = [&](int t, uint16_t* kt, uint16_t* kx, uint16_t* vt, uint16_t* vw) __attribute__((always_inline)) {
+      if (live) turn(s0, s1, p0, p1, kt + 32 * D, vw + 32 * D);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      const uint32_t off3 = find(last(t + 3), entry);  // (here, where no load is under way)
+      fetch(kbase, kt, off2, Yes{});
+      fetch(vbase, vw, off1, No{});
+      entry = ca_entry(A, table, pos_of(last(t + 4)));
+      off1 = off2, off2 = off3;
+      if (live) turn(s1, s0, p1, p0, kx, vt);
+    };
+    for (int t = 0; t < nf; t += 2) {
+      round(t, sK0, sK1, sV0, sV1);
+      if (t + 1 < nf) round(t + 1, sK1, sK0, sV1, sV0);
+    }
+    // the last half tile's sums
+    if (live) {
+      const uint16_t* vt = (nf & 1 ? sV0 : sV1) + 32 * D;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int mm = 0; mm < 2; ++mm) {
+          const uint16_t* at = vt + vat(nb) + 16 * mm * D;
+          const u32x2 f0 = ca_trread(at), f1 = ca_trread(at + 8 * D);
+#pragma unroll
+          for (int b = 0; b < RB; ++b) ca_mfma_a<T>(o[b][nb], u32x4{f0[0], f0[1], f1[0], f1[1]}, p1[b][mm]);
+        }
+      ready();
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
+
+  // ---- tiles with hidden keys: those of a row are not seen, and an inf or NaN among their values
+  // (left out of the products, where a weight of 0 would make it NaN) goes to the rows that see it
+  if (nf < nt) {
+    CacheSight sight[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      int tok, head;
+      row_of(b, tok, head);
+      sight[b] = CacheSight{
+          A.mask ? A.mask + (A.offsets ? (w.row0 + tok) * A.mask_row : w.b * A.mask_batch + tok * A.mask_row) : nullptr,
+          w.first, A.causal ? w.first + tok : w.L - 1, A.mask_cols};
+    }
+    auto ask = [&](int t, uint16_t* kt, uint16_t* vt) __attribute__((always_inline)) {
+      bool ok;
+      const uint32_t off = ca_offset(A, ca_entry(A, table, pos_of(t)), pos_of(t), ok);
+      const uint64_t bad = __ballot(!ok);
+      if (lane == 0) sBad[t & 1][wave] = (uint32_t)bad & 0xffffu;
+      fetch(kbase, kt, off, Yes{});
+      fetch(vbase, vt, off, No{});
+    };
+    auto hidden = [&](int t, int kb, const uint16_t* kt, const uint16_t* vt) __attribute__((always_inline)) {
+      const int base = 64 * (t0 + t) + 32 * kb;
+      f32x16 S[RB];
+      u32x4 P[RB][2];
+      uint32_t seen[RB];
+      float lt[RB];
+      scores(S, kt);
+#pragma unroll
+      for (int b = 0; b < RB; ++b) {
+        uint32_t x = 0;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int j = 8 * g + 4 * hh;
+          x |= sight[b].sees4(base + j) << j;
+        }
+        x |= half_partner(x);
+        x &= ~(sBad[t & 1][2 * kb] | sBad[t & 1][2 * kb + 1] << 16);
+        seen[b] = x;
+#pragma unroll
+        for (int a = 0; a < 16; ++a)
+          if (!(x >> (8 * (a / 4) + 4 * hh + a % 4) & 1)) S[b][a] = -__builtin_inff();
+        lt[b] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) weigh(i, S, P, lt);
+      settle(S, P, lt);
+      bool odd = false;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int mm = 0; mm < 2; ++mm) {
+          const uint16_t* at = vt + vat(nb) + 16 * mm * D;
+          u32x2 f[2] = {ca_trread(at), ca_trread(at + 8 * D)};
+          odd |= ca_clean<T>(f);
+#pragma unroll
+          for (int b = 0; b < RB; ++b)
+            o[b][nb] = Mfma<T>::run(u32x4{f[0][0], f[0][1], f[1][0], f[1][1]}, P[b][mm], o[b][nb]);
+        }
+      if (__ballot(odd)) {
+        for (int j = 0; j < 32; ++j)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int a = 0; a < 16; ++a) {
+              const int d = 32 * nb + 8 * (a / 4) + 4 * hh + a % 4;
+              const uint16_t u = vt[j * D + 8 * ((d >> 3) ^ ca_vswz<D>(j)) + (d & 7)];
+              if ((u & CaType<T>::inf) == CaType<T>::inf)
+#pragma unroll
+                for (int b = 0; b < RB; ++b)
+                  if (seen[b] >> j & 1) o[b][nb][a] += T::to_f(u);
+            }
+      }
+    };
+    ask(nf, sK0, sV0);
+    for (int t = nf; t < nt; ++t) {
+      const bool even = !((t - nf) & 1);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (t + 1 < nt) ask(t + 1, even ? sK1 : sK0, even ? sV1 : sV0);
+      if (live)
+#pragma clang loop unroll(disable)
+        for (int kb = 0; kb < 2; ++kb) hidden(t, kb, (even ? sK0 : sK1) + 32 * kb * D, (even ? sV0 : sV1) + 32 * kb * D);
+    }
+  }
+  if (!live) return;
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const float lt = half_sum(l[b]);
+    if (wr0 + 32 * b + jl >= w.rows) continue;
+    int tok, head;
+    row_of(b, tok, head);
+    const long long at = (w.row0 + tok) * A.HQ + head;
+    if (parts > 1) {
+      const long long pr = (long long)part * A.T * A.HQ + at;
+      float* op = A.opart + pr * D + 4 * hh;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *(f32x4*)(op + 32 * nb + 8 * g) = f32x4{o[b][nb][4 * g], o[b][nb][4 * g + 1], o[b][nb][4 * g + 2], o[b][nb][4 * g + 3]};
+      if (hh == 0) A.mlpart[2 * pr] = m[b], A.mlpart[2 * pr + 1] = lt;
+      continue;
+    }
+    const float inv = lt == 0.f ? 0.f : 1.f / lt;
+    char* dst = (char*)ca_token(A.out, A, w, A.o_batch, A.o_row, tok) + head * A.o_head + 8 * hh;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *(u32x2*)(dst + 64 * nb + 16 * g) = u32x2{Pk<T>::pack(o[b][nb][4 * g] * inv, o[b][nb][4 * g + 1] * inv),
+                                                  Pk<T>::pack(o[b][nb][4 * g + 2] * inv, o[b][nb][4 * g + 3] * inv)};
+    if (A.lse && hh == 0) A.lse[at] = lt == 0.f ? -__builtin_inff() : 0.6931471805599453f * (m[b] + __log2f(lt));
+  }
+}
+
 // joins the parts of a row block's rows, eight threads a row
-template <typename T, int D>
+template <typename T, int D, int ROWS>
 __global__ __launch_bounds__(256) void ca_combine_kernel(CacheArgs A) {
   const int kh = blockIdx.x % A.HK, tile = blockIdx.x / A.HK;
   CacheRows w;
-  if (!ca_rows<32>(A, tile, w)) return;
+  if (!ca_rows<ROWS>(A, tile, w)) return;
+  w.r0 += 32 * blockIdx.y;
   const int parts = ca_parts(w.L, A.S), rr = threadIdx.x >> 3, d0 = (threadIdx.x & 7) * (D / 8);
   if (parts < 2 || w.r0 + rr >= w.rows) return;  // (its work-group has written the rows)
   const int tok = (w.r0 + rr) / A.G, head = kh * A.G + w.r0 + rr - tok * A.G;
@@ -410,6 +796,12 @@ __global__ __launch_bounds__(256) void ca_combine_kernel(CacheArgs A) {
   if (A.lse && d0 == 0) A.lse[at] = total == 0.f ? -__builtin_inff() : 0.6931471805599453f * (M + __log2f(total));
 }
 
+// Packed rows of a row block: by the rows that a sequence may have (all of them, where they are not
+// known to the host).
+static int ca_block(int ragged, int B, long long T, int G) {
+  const long long rows = (ragged ? T : T / B) * G;
+  return rows <= 64 ? 32 : rows <= 128 ? 128 : 256;
+}
 // Most parts of a sequence's keys: as many as bring the launch to two rounds of work-groups, of
 // CA_PART keys at least.
 static int ca_split(long long tiles, int HK, long long keys) {
@@ -418,15 +810,16 @@ static int ca_split(long long tiles, int HK, long long keys) {
   const long long s = (512 + wgs - 1) / wgs;
   return (int)(s < most ? (s < 64 ? s : 64) : (most < 64 ? most : 64));
 }
-// row blocks of 32 packed rows
-static long long ca_tiles(int ragged, int B, long long T, int G) {
-  return ragged ? T * G / 32 + B : B * ((T / B * G + 31) / 32);
+// row blocks of `block` packed rows
+static long long ca_tiles(int block, int ragged, int B, long long T, int G) {
+  return ragged ? T * G / block + B : B * ((T / B * G + block - 1) / block);
 }
 static size_t ca_ws(int S, long long rows, int D) { return S < 2 ? 0 : (size_t)S * rows * (D + 2) * 4; }
 
 extern "C" size_t t2t_cache_attention_ws_bytes(int ragged, int B, long long T, int HQ, int HK, int D, long long keys) {
   if (B < 1 || T < 1 || HK < 1 || HQ < HK || keys < 1) return 0;
-  return ca_ws(ca_split(ca_tiles(ragged, B, T, HQ / HK), HK, keys), T * HQ, D);
+  const int G = HQ / HK, block = ca_block(ragged, B, T, G);
+  return ca_ws(ca_split(ca_tiles(block, ragged, B, T, G), HK, keys), T * HQ, D);
 }
 
 extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -466,7 +859,8 @@ extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, 
   A.pages = a->pages, A.page = a->page_size, A.width = a->width, A.mask_cols = a->mask_cols, A.causal = a->causal;
   A.shift = (a->page_size & (a->page_size - 1)) ? -1 : __builtin_ctz(a->page_size);
   A.c = a->scale * 1.4426950408889634f;
-  const long long tiles = ca_tiles(a->offsets != nullptr, a->B, T, A.G);
+  const int ragged = a->offsets != nullptr, block = ca_block(ragged, a->B, T, A.G);
+  const long long tiles = ca_tiles(block, ragged, a->B, T, A.G);
   const long long keys = (long long)a->width * a->page_size;
   A.S = ca_split(tiles, a->HK, keys < 1 ? 1 : keys);
   // (as many parts as the workspace holds)
@@ -480,12 +874,18 @@ extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, 
     t2t_set_error("cache_attention: %lld row blocks of %d heads", tiles, a->HK);
     return T2T_ERR_UNSUPPORTED;
   }
+  A.tiles = (int)tiles, A.items = (int)(tiles * a->HK * A.S);
   auto run = [&](auto t, auto d) {
     using TT = decltype(t);
     constexpr int D = decltype(d)::value;
-    hipLaunchKernelGGL((ca_few_kernel<TT, D>), dim3((unsigned)(tiles * a->HK * A.S)), dim3(256), 0, (hipStream_t)stream, A);
-    if (A.S > 1)
-      hipLaunchKernelGGL((ca_combine_kernel<TT, D>), dim3((unsigned)(tiles * a->HK)), dim3(256), 0, (hipStream_t)stream, A);
+    auto go = [&](auto kernel, auto join) {
+      hipLaunchKernelGGL(kernel, dim3((A.items + 7) / 8 * 8), dim3(256), 0, (hipStream_t)stream, A);
+      if (A.S > 1)
+        hipLaunchKernelGGL(join, dim3((unsigned)(tiles * a->HK), block / 32), dim3(256), 0, (hipStream_t)stream, A);
+    };
+    if (block == 32) go(ca_few_kernel<TT, D>, ca_combine_kernel<TT, D, 32>);
+    else if (block == 128) go(ca_many_kernel<TT, D, 1>, ca_combine_kernel<TT, D, 128>);
+    else go(ca_many_kernel<TT, D, 2>, ca_combine_kernel<TT, D, 256>);
   };
   using D64 = std::integral_constant<int, 64>;
   using D128 = std::integral_constant<int, 128>;
