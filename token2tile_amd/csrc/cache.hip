@@ -21,6 +21,14 @@ __device__ inline void ca_dma(const char* from, uint16_t* to) {
                : "memory");
 }
 
+// the same from a scalar base and an offset a lane
+__device__ inline void ca_dma_at(const char* base, uint32_t off, uint16_t* to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(
+                   __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(ca_lds_t*)to)),
+               "v"(off), "s"(base)
+               : "memory");
+}
+
 #define CA_NONE (-1.0e30f)  // the running maximum before any key: finite, so that rows of hidden keys add 0
 
 struct CacheArgs {
@@ -428,7 +436,7 @@ template <typename T> __device__ inline void ca_mfma_a(f32x16& c, const u32x4& a
 // the weights' vector operations between them: a SIMD holds one wave, and the matrix
 // unit has work while the exponentials are taken.  The other tiles follow, one after
 // the other.
-template <typename T, int D, int RB>
+template <typename T, int D, int RB, bool P16>
 __global__ __launch_bounds__(256, 1) void ca_many_kernel(CacheArgs A) {
   constexpr int ROWS = 128 * RB, LPR = D / 8, RPI = 64 / LPR, NB = D / 32, NS = D / 16;
   constexpr int PAIRS = 8 * RB;  // of weights in a half tile
@@ -491,6 +499,16 @@ __global__ __launch_bounds__(256, 1) void ca_many_kernel(CacheArgs A) {
       ca_dma(base + at + 16 * ((lane & (LPR - 1)) ^ swz), to + (16 * wave + RPI * i) * D);
     }
   };
+  // with P16 sixteen keys lie in one page, one stride apart: a scalar base, and offsets that stay
+  uint32_t koff[P16 ? 16 / RPI : 1], voff[P16 ? 16 / RPI : 1];
+  if constexpr (P16) {
+#pragma unroll
+    for (int i = 0; i < 16 / RPI; ++i) {
+      const int in = RPI * i + lane / LPR, row = 16 * wave + in;
+      koff[i] = (uint32_t)(in * A.kv_row) + 16 * ((lane & (LPR - 1)) ^ ca_kswz<D>(row));
+      voff[i] = (uint32_t)(in * A.kv_row) + 16 * ((lane & (LPR - 1)) ^ ca_vswz<D>(row));
+    }
+  }
   using Yes = std::true_type;
   using No = std::false_type;
   // where the lane's operands lie (halves): K of step s, V of dim block nb
@@ -533,7 +551,7 @@ __global__ __launch_bounds__(256, 1) void ca_many_kernel(CacheArgs A) {
     bool far = false;
 #pragma unroll
     for (int b = 0; b < RB; ++b) far |= !(lt[b] <= CaType<T>::limit);
-    if (__builtin_amdgcn_readfirstlane((int)(__ballot(far) != 0ull))) {
+    if (__ballot(far)) {
       ready();
 #pragma unroll
       for (int b = 0; b < RB; ++b) move(b, S[b]), lt[b] = 0.f;
@@ -552,56 +570,115 @@ __global__ __launch_bounds__(256, 1) void ca_many_kernel(CacheArgs A) {
     }
   };
   // One turn: S of this half tile's scores -> P, the scores SX of the half tile in kt, the sums of the
-  // one in vt with its weights PP.
+  // one in vt with its weights PP.  Operands are read AHEAD steps before their products; the first
+  // ones by the turn before, which at `mid`, with all its own reads done, meets the other waves where
+  // the next turn's tiles have to be there.  extra(i): what else step i issues.
+  constexpr int AHEAD = 3, STEPS = NS;
+  static_assert(NS == 2 * NB && STEPS >= AHEAD, "a turn's steps come in pairs");
+  u32x4 kf[AHEAD + 1];
+  u32x2 vf[AHEAD + 1][2];
+  auto rdk = [&](const uint16_t* kt, int i) __attribute__((always_inline)) {
+    kf[i % (AHEAD + 1)] = *(const u32x4*)(kt + kat(i));
+  };
+  auto rdv = [&](const uint16_t* vt, int i) __attribute__((always_inline)) {
+    const uint16_t* at = vt + vat(i / 2) + 16 * (i % 2) * D;
+    vf[i % (AHEAD + 1)][0] = ca_trread(at);
+    vf[i % (AHEAD + 1)][1] = ca_trread(at + 8 * D);
+  };
   auto turn = [&](const f32x16 (&S)[RB], f32x16 (&SX)[RB], u32x4 (&P)[RB][2], const u32x4 (&PP)[RB][2],
-                  const uint16_t* kt, const uint16_t* vt) __attribute__((always_inline)) {
-    constexpr int AHEAD = 2, STEPS = NS;
-    static_assert(NS == 2 * NB, "a turn's steps come in pairs");
-    float lt[RB];
+                  const uint16_t* kt, const uint16_t* vt, const uint16_t* kn, const uint16_t* vn, auto mid, auto extra)
+      __attribute__((always_inline)) {
+    static_assert(STEPS % (AHEAD + 1) == 0, "the ring goes on from turn to turn");
+    float lt[RB], x0[2], x1[2];
 #pragma unroll
     for (int b = 0; b < RB; ++b) lt[b] = 0.f;
-    u32x4 kf[AHEAD + 1];
-    u32x2 vf[AHEAD + 1][2];
-    auto rdk = [&](int i) __attribute__((always_inline)) { kf[i % (AHEAD + 1)] = *(const u32x4*)(kt + kat(i)); };
-    auto rdv = [&](int i) __attribute__((always_inline)) {
-      const uint16_t* at = vt + vat(i / 2) + 16 * (i % 2) * D;
-      vf[i % (AHEAD + 1)][0] = ca_trread(at);
-      vf[i % (AHEAD + 1)][1] = ca_trread(at + 8 * D);
+    // the weights' operations, a slot behind each product: of pair j the products and the first
+    // exponential, then the second, with the packing and sum of the pair before
+    constexpr int SLOTS = 2 * STEPS * RB, EACH = SLOTS / PAIRS;  // 2 (D = 128), 1
+    auto pack = [&](int j) __attribute__((always_inline)) {
+      const int b = j / 8, a = 2 * (j % 8);
+      P[b][a / 8][(a % 8) / 2] = Pk<T>::pack(x0[j & 1], x1[j & 1]);
     };
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) rdv(i), rdk(i);
+    auto add = [&](int j) __attribute__((always_inline)) {
+      const int b = j / 8, a = 2 * (j % 8);
+      lt[b] = Pk<T>::sum2(P[b][a / 8][(a % 8) / 2], lt[b]);
+    };
+    auto slot = [&](int n) __attribute__((always_inline)) {
+      const int j = n / EACH, b = j / 8, a = 2 * (j % 8);
+      if (EACH == 1 || n % 2 == 0) {
+        x0[j & 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[b][a], A.c, -m[b]));
+        x1[j & 1] = __builtin_fmaf(S[b][a + 1], A.c, -m[b]);
+        if (j) pack(j - 1);
+      }
+      if (EACH == 1 || n % 2 == 1) {
+        x1[j & 1] = __builtin_amdgcn_exp2f(x1[j & 1]);
+        if (j) add(j - 1);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
       __builtin_amdgcn_sched_barrier(0);
-      if (i + AHEAD < STEPS) rdv(i + AHEAD);
+      if (i == STEPS - AHEAD) mid();
+      rdk(i + AHEAD < STEPS ? kt : kn, (i + AHEAD) % STEPS);
+      rdv(i + AHEAD < STEPS ? vt : vn, (i + AHEAD) % STEPS);
+      extra(i);
+      __builtin_amdgcn_sched_barrier(0);
       const u32x2 f0 = vf[i % (AHEAD + 1)][0], f1 = vf[i % (AHEAD + 1)][1];
       const u32x4 f{f0[0], f0[1], f1[0], f1[1]};
 #pragma unroll
-      for (int b = 0; b < RB; ++b) ca_mfma_a<T>(o[b][i / 2], f, PP[b][i % 2]);
+      for (int b = 0; b < RB; ++b) {
+        SX[b] = Mfma<T>::run(kf[i % (AHEAD + 1)], q[b][i], i ? SX[b] : zero16());
+        __builtin_amdgcn_sched_barrier(0);
+        slot(2 * RB * i + b);
+      }
 #pragma unroll
-      for (int j = (2 * i) * PAIRS / (2 * STEPS); j < (2 * i + 1) * PAIRS / (2 * STEPS); ++j) weigh(j, S, P, lt);
-      __builtin_amdgcn_sched_barrier(0);
-      if (i + AHEAD < STEPS) rdk(i + AHEAD);
-#pragma unroll
-      for (int b = 0; b < RB; ++b) SX[b] = Mfma<T>::run(kf[i % (AHEAD + 1)], q[b][i], i ? SX[b] : zero16());
-#pragma unroll
-      for (int j = (2 * i + 1) * PAIRS / (2 * STEPS); j < (2 * i + 2) * PAIRS / (2 * STEPS); ++j) weigh(j, S, P, lt);
+      for (int b = 0; b < RB; ++b) {
+        ca_mfma_a<T>(o[b][i / 2], f, PP[b][i % 2]);
+        __builtin_amdgcn_sched_barrier(0);
+        slot(2 * RB * i + RB + b);
+      }
     }
-    __builtin_amdgcn_sched_barrier(0);
+    pack(PAIRS - 1);
+    add(PAIRS - 1);
     settle(S, P, lt);
   };
 
   if (nf > 0) {
     f32x16 s0[RB], s1[RB];
     u32x4 p0[RB][2], p1[RB][2];
-    bool ok;
-    auto find = [&](int t, uint32_t entry) { return ca_offset(A, entry, pos_of(t), ok); };
     // (tiles past the last of the pipeline are fetched like it, and not used)
     auto last = [&](int t) { return min(t, nf - 1); };
-    // offsets of tiles t + 1 and t + 2; the table's entry of tile t + 3
-    uint32_t off0 = find(0, ca_entry(A, table, pos_of(0))), off1 = find(last(1), ca_entry(A, table, pos_of(last(1)))),
-             off2 = find(last(2), ca_entry(A, table, pos_of(last(2)))), entry = ca_entry(A, table, pos_of(last(3)));
-    fetch(kbase, sK0, off0, Yes{});
+    auto look = [&](int t) { return ca_entry(A, table, P16 ? 64 * (t0 + last(t)) + 16 * wave : pos_of(last(t))); };
+    auto find = [&](int t, uint32_t entry) {
+      if constexpr (P16) {
+        const int pos = 64 * (t0 + last(t)) + 16 * wave;
+        entry = __builtin_amdgcn_readfirstlane(entry);
+        return (long long)entry * A.kv_page + (A.shift >= 0 ? pos & (A.page - 1) : pos % A.page) * A.kv_row;
+      } else {
+        bool ok;
+        return ca_offset(A, entry, pos_of(last(t)), ok);
+      }
+    };
+    auto one = [&](const char* base, uint16_t* to, auto off, int i, auto KEYS) __attribute__((always_inline)) {
+      to += (16 * wave + RPI * i) * D;
+      if constexpr (P16) {
+        ca_dma_at(base + off, decltype(KEYS)::value ? koff[i] : voff[i], to);
+      } else {
+        const int in = RPI * i + lane / LPR, row = 16 * wave + in;
+        const size_t at = (size_t)(uint32_t)__shfl((int)off, in, 64) * 16;
+        const int swz = decltype(KEYS)::value ? ca_kswz<D>(row) : ca_vswz<D>(row);
+        ca_dma(base + at + 16 * ((lane & (LPR - 1)) ^ swz), to);
+      }
+    };
+    auto whole = [&](const char* base, uint16_t* to, auto off, auto KEYS) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 16 / RPI; ++i) one(base, to, off, i, KEYS);
+    };
+    // where tiles t + 1 and t + 2 lie; the table's entry of tile t + 3
+    auto off0 = find(0, look(0)), off1 = find(1, look(1)), off2 = find(2, look(2));
+    uint32_t entry = look(3);
+    whole(kbase, sK0, off0, Yes{});
     // before the first half tile: values and weights of zero
     for (int i = threadIdx.x; i < 8 * D; i += 256) *(u32x4*)(sV1 + 8 * i) = u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
@@ -610,20 +687,35 @@ __global__ __launch_bounds__(256, 1) void ca_many_kernel(CacheArgs A) {
       for (int i = 0; i < 2; ++i) p1[b][i] = u32x4{0u, 0u, 0u, 0u};
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    fetch(kbase, sK1, off1, Yes{});
-    fetch(vbase, sV0, off0, No{});
-    if (live) scores(s0, sK0);
+    whole(kbase, sK1, off1, Yes{});
+    whole(vbase, sV0, off0, No{});
+    if (live) {
+      scores(s0, sK0);
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) rdk(sK0 + 32 * D, i), rdv(sV1 + 32 * D, i);
+    }
+    // every wave's reads of the tiles before are done, and the loads that have been asked for are there
+    auto meet = [&]() __attribute__((always_inline)) {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+    auto nothing = [&](int) __attribute__((always_inline)) {};
+    auto none = [&]() __attribute__((always_inline)) {};
     // tile t, whose first half's scores are there; K of t + 1 and V of t have been asked for
     auto round = [&](int t, uint16_t* kt, uint16_t* kx, uint16_t* vt, uint16_t* vw) __attribute__((always_inline)) {
-      if (live) turn(s0, s1, p0, p1, kt + 32 * D, vw + 32 * D);
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      const uint32_t off3 = find(last(t + 3), entry);  // (here, where no load is under way)
-      fetch(kbase, kt, off2, Yes{});
-      fetch(vbase, vw, off1, No{});
-      entry = ca_entry(A, table, pos_of(last(t + 4)));
+      if (live) turn(s0, s1, p0, p1, kt + 32 * D, vw + 32 * D, kx, vt, meet, nothing);
+      else meet();
+      const auto off3 = find(t + 3, entry);  // (here, where no load is under way)
+      auto ask = [&](int i) __attribute__((always_inline)) {
+        if (i < 16 / RPI) one(kbase, kt, off2, i, Yes{}), one(vbase, vw, off1, i, No{});
+      };
+      if (live) {
+        turn(s1, s0, p1, p0, kx, vt, kx + 32 * D, vt + 32 * D, none, ask);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16 / RPI; ++i) ask(i);
+      }
+      entry = look(t + 4);
       off1 = off2, off2 = off3;
-      if (live) turn(s1, s0, p1, p0, kx, vt);
     };
     for (int t = 0; t < nf; t += 2) {
       round(t, sK0, sK1, sV0, sV1);
@@ -875,6 +967,8 @@ extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, 
     return T2T_ERR_UNSUPPORTED;
   }
   A.tiles = (int)tiles, A.items = (int)(tiles * a->HK * A.S);
+  // sixteen keys from a multiple of sixteen on lie in one page, at 32-bit offsets
+  const bool p16 = a->page_size % 16 == 0 && A.kv_row < (1 << 27);
   auto run = [&](auto t, auto d) {
     using TT = decltype(t);
     constexpr int D = decltype(d)::value;
@@ -884,8 +978,10 @@ extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, 
         hipLaunchKernelGGL(join, dim3((unsigned)(tiles * a->HK), block / 32), dim3(256), 0, (hipStream_t)stream, A);
     };
     if (block == 32) go(ca_few_kernel<TT, D>, ca_combine_kernel<TT, D, 32>);
-    else if (block == 128) go(ca_many_kernel<TT, D, 1>, ca_combine_kernel<TT, D, 128>);
-    else go(ca_many_kernel<TT, D, 2>, ca_combine_kernel<TT, D, 256>);
+    else if (block == 128) p16 ? go(ca_many_kernel<TT, D, 1, true>, ca_combine_kernel<TT, D, 128>)
+                               : go(ca_many_kernel<TT, D, 1, false>, ca_combine_kernel<TT, D, 128>);
+    else p16 ? go(ca_many_kernel<TT, D, 2, true>, ca_combine_kernel<TT, D, 256>)
+             : go(ca_many_kernel<TT, D, 2, false>, ca_combine_kernel<TT, D, 256>);
   };
   using D64 = std::integral_constant<int, 64>;
   using D128 = std::integral_constant<int, 128>;
