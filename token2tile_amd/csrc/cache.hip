@@ -193,9 +193,8 @@ __device__ inline void ca_weights(CacheState<T, D>& w, const f32x16 (&s)[NK], u3
       for (int a = 0; a < 16; a += 2) {
         const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][a], c, nm));
         const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][a + 1], c, nm));
-        const uint32_t pk = Pk<T>::pack(p0, p1);
-        acc = Pk<T>::sum2(pk, acc);
-        p[2 * kb + a / 8][(a % 8) / 2] = pk;
+        acc += p0 + p1;
+        p[2 * kb + a / 8][(a % 8) / 2] = Pk<T>::pack(p0, p1);
       }
     return acc;
   };
@@ -534,9 +533,8 @@ __global__ __launch_bounds__(256, 1) void ca_many_kernel(CacheArgs A) {
     const int b = i / 8, a = 2 * (i % 8);
     const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[b][a], A.c, -m[b]));
     const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[b][a + 1], A.c, -m[b]));
-    const uint32_t pk = Pk<T>::pack(x0, x1);
-    lt[b] = Pk<T>::sum2(pk, lt[b]);
-    P[b][a / 8][(a % 8) / 2] = pk;
+    lt[b] += x0 + x1;
+    P[b][a / 8][(a % 8) / 2] = Pk<T>::pack(x0, x1);
   };
   // the sums are in accumulation registers, written by the assembly below, whose results are
   // readable after 18 cycles of issue
@@ -599,10 +597,7 @@ __global__ __launch_bounds__(256, 1) void ca_many_kernel(CacheArgs A) {
       const int b = j / 8, a = 2 * (j % 8);
       P[b][a / 8][(a % 8) / 2] = Pk<T>::pack(x0[j & 1], x1[j & 1]);
     };
-    auto add = [&](int j) __attribute__((always_inline)) {
-      const int b = j / 8, a = 2 * (j % 8);
-      lt[b] = Pk<T>::sum2(P[b][a / 8][(a % 8) / 2], lt[b]);
-    };
+    auto add = [&](int j) __attribute__((always_inline)) { lt[j / 8] += x0[j & 1] + x1[j & 1]; };
     auto slot = [&](int n) __attribute__((always_inline)) {
       const int j = n / EACH, b = j / 8, a = 2 * (j % 8);
       if (EACH == 1 || n % 2 == 0) {
