@@ -418,29 +418,41 @@ __global__ __launch_bounds__(256, 1) void ca_few_kernel(CacheArgs A) {
   if (A.lse && d0 == 0) A.lse[at] = lt == 0.f ? -__builtin_inff() : 0.6931471805599453f * (sM[0][rr] + __log2f(lt));
 }
 
-// c += a b with c in accumulation registers (the compiler's choice moved them back and forth).  The
-// operands have been written long before; who reads c waits.
-template <typename T> __device__ inline void ca_mfma_a(f32x16& c, const u32x4& a, const u32x4& b) {
-  if constexpr (T::code == T2T_BF16)
-    asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
-  else
-    asm("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+// The products of the pipeline below, with the sums in accumulation registers and the queries where
+// there is room (the compiler's choice moved them back and forth).  Two wait states come before each:
+// the compiler may have moved an operand just before, and does not know what this is.  Who reads a
+// result waits, or comes two products later.
+#define CA_MFMA(dst, c, dst_, q_)                                                                       \
+  if constexpr (T::code == T2T_BF16)                                                                    \
+    asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, " c : dst_(dst) : "v"(a), q_(b));               \
+  else                                                                                                  \
+    asm("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, " c : dst_(dst) : "v"(a), q_(b))
+template <typename T> __device__ inline void ca_mfma_sum(f32x16& c, const u32x4& a, const u32x4& b) {
+  CA_MFMA(c, "%0", "+a", "v");
 }
+template <typename T, int D, bool FIRST>
+__device__ inline void ca_mfma_score(f32x16& c, const u32x4& a, const u32x4& b) {
+  if constexpr (FIRST && D == 128) { CA_MFMA(c, "0", "=&v", "a"); }
+  else if constexpr (D == 128) { CA_MFMA(c, "%0", "+v", "a"); }
+  else if constexpr (FIRST) { CA_MFMA(c, "0", "=&v", "v"); }
+  else { CA_MFMA(c, "%0", "+v", "v"); }
+}
+#undef CA_MFMA
 
 // ---- many rows: a work-group's waves share the keys --------------------------
-// 128 RB packed rows a work-group, 32 RB a wave; tiles of 64 keys, fetched by all
-// waves for all (DMA, one barrier a tile).  Tiles of which every row sees every key
-// go through a pipeline of half tiles: a turn computes the scores of the next half,
-// the weights of this one and the sums of the last, in steps of RB products each with
-// the weights' vector operations between them: a SIMD holds one wave, and the matrix
-// unit has work while the exponentials are taken.  The other tiles follow, one after
-// the other.
-template <typename T, int D, int RB, bool P16>
-__global__ __launch_bounds__(256, 1) void ca_many_kernel(CacheArgs A) {
-  constexpr int ROWS = 128 * RB, LPR = D / 8, RPI = 64 / LPR, NB = D / 32, NS = D / 16;
-  constexpr int PAIRS = 8 * RB;  // of weights in a half tile
+// 32 W packed rows a work-group of W waves; tiles of 64 keys, fetched by all waves for
+// all (DMA, one barrier a tile).  Tiles of which every row sees every key go through a
+// pipeline of half tiles: a turn computes the scores of the next half, the weights of
+// this one and the sums of the last, product by product with the weights' vector
+// operations between them, so that the matrix unit has work while the exponentials
+// are taken.  The other tiles follow, one after the other.
+template <typename T, int D, int W, bool P16>
+__global__ __launch_bounds__(64 * W, 2) void ca_many_kernel(CacheArgs A) {
+  constexpr int ROWS = 32 * W, LPR = D / 8, RPI = 64 / LPR, NB = D / 32, NS = D / 16;
+  constexpr int KW = 64 / W, IPW = KW / RPI;  // keys of a tile that a wave fetches, in so many instructions
+  static_assert(IPW >= 1, "whole instructions");
   __shared__ __attribute__((aligned(1024))) uint16_t sK0[64 * D], sK1[64 * D], sV0[64 * D], sV1[64 * D];
-  __shared__ uint32_t sBad[2][4];  // a wave's sixteen keys whose table entry lies outside the cache
+  __shared__ uint32_t sBad[2][W];  // a wave's keys whose table entry lies outside the cache
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int jl = lane & 31, hh = lane >> 5;
   int part, kh, tile;
@@ -449,26 +461,19 @@ __global__ __launch_bounds__(256, 1) void ca_many_kernel(CacheArgs A) {
   if (!ca_rows<ROWS>(A, tile, w)) return;
   const int parts = ca_parts(w.L, A.S);
   if (part >= parts) return;
-  const int wr0 = w.r0 + 32 * RB * wave;      // the wave's first row
-  const bool live = wr0 < w.rows;             // (of the wave)
-  u32x4 q[RB][NS];
-  f32x16 o[RB][NB];
-  float m[RB], l[RB];
-  auto row_of = [&](int b, int& tok, int& head) {
-    const int r = min(wr0 + 32 * b + jl, w.rows - 1);
-    tok = r / A.G, head = kh * A.G + r - tok * A.G;
-  };
-#pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    int tok, head;
-    row_of(b, tok, head);
+  const int wr0 = w.r0 + 32 * wave;  // the wave's first row
+  const bool live = wr0 < w.rows;    // (of the wave)
+  const int r = min(wr0 + jl, w.rows - 1), tok = r / A.G, head = kh * A.G + r - tok * A.G;
+  u32x4 q[NS];
+  f32x16 o[NB];
+  float m = CA_NONE, l = 0.f;
+  {
     const char* qr = ca_token(A.q, A, w, A.q_batch, A.q_row, tok) + head * A.q_head + 16 * hh;
 #pragma unroll
-    for (int s = 0; s < NS; ++s) q[b][s] = *(const u32x4*)(qr + 32 * s);
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) o[b][nb] = zero16();
-    m[b] = CA_NONE, l[b] = 0.f;
+    for (int s = 0; s < NS; ++s) q[s] = *(const u32x4*)(qr + 32 * s);
   }
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) o[nb] = zero16();
   // keys that some row of the work-group sees; from `plain` on not every row sees every key
   const int tok0 = w.r0 / A.G, tok1 = (min(w.r0 + ROWS, w.rows) - 1) / A.G;
   const int keys = A.causal ? min(w.L, w.first + tok1 + 1) : w.L;
@@ -483,96 +488,89 @@ __global__ __launch_bounds__(256, 1) void ca_many_kernel(CacheArgs A) {
   {
     bool bad = false;
     const int e0 = nf > 0 ? 64 * t0 / A.page : 0, e1 = nf > 0 ? (64 * (t0 + nf) - 1) / A.page : -1;
-    for (int e = e0 + threadIdx.x; e <= e1; e += 256) bad |= (uint32_t)table[e] >= (uint32_t)A.pages;
+    for (int e = e0 + threadIdx.x; e <= e1; e += 64 * W) bad |= (uint32_t)table[e] >= (uint32_t)A.pages;
     if (__syncthreads_or(bad)) nf = 0;
   }
 
-  // this wave fetches keys 16 wave .. + 15 of every tile; lane l looks key l % 16 up
-  auto pos_of = [&](int t) { return min(64 * (t0 + t) + 16 * wave + (lane & 15), w.L - 1); };
-  auto fetch = [&](const char* base, uint16_t* to, uint32_t off, auto KEYS) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 16 / RPI; ++i) {
-      const int in = RPI * i + lane / LPR, row = 16 * wave + in;
-      const size_t at = (size_t)(uint32_t)__shfl((int)off, in, 64) * 16;
-      const int swz = decltype(KEYS)::value ? ca_kswz<D>(row) : ca_vswz<D>(row);
-      ca_dma(base + at + 16 * ((lane & (LPR - 1)) ^ swz), to + (16 * wave + RPI * i) * D);
-    }
-  };
+  // this wave fetches keys KW wave .. of every tile; lane l looks key l % KW up
+  auto pos_of = [&](int t) { return min(64 * (t0 + t) + KW * wave + (lane & (KW - 1)), w.L - 1); };
   // with P16 sixteen keys lie in one page, one stride apart: a scalar base, and offsets that stay
-  uint32_t koff[P16 ? 16 / RPI : 1], voff[P16 ? 16 / RPI : 1];
+  uint32_t koff[P16 ? IPW : 1], voff[P16 ? IPW : 1];
   if constexpr (P16) {
 #pragma unroll
-    for (int i = 0; i < 16 / RPI; ++i) {
-      const int in = RPI * i + lane / LPR, row = 16 * wave + in;
+    for (int i = 0; i < IPW; ++i) {
+      const int in = RPI * i + lane / LPR, row = KW * wave + in;
       koff[i] = (uint32_t)(in * A.kv_row) + 16 * ((lane & (LPR - 1)) ^ ca_kswz<D>(row));
       voff[i] = (uint32_t)(in * A.kv_row) + 16 * ((lane & (LPR - 1)) ^ ca_vswz<D>(row));
     }
   }
   using Yes = std::true_type;
   using No = std::false_type;
+  // 1 KB of a tile's keys (values) to LDS: off is where the wave's keys lie (P16) or the lane's key
+  auto one = [&](const char* base, uint16_t* to, auto off, int i, auto KEYS) __attribute__((always_inline)) {
+    to += (KW * wave + RPI * i) * D;
+    if constexpr (sizeof(off) == 8) {
+      ca_dma_at(base + off, decltype(KEYS)::value ? koff[P16 ? i : 0] : voff[P16 ? i : 0], to);
+    } else {
+      const int in = RPI * i + lane / LPR, row = KW * wave + in;
+      const size_t at = (size_t)(uint32_t)__shfl((int)off, in, 64) * 16;
+      const int swz = decltype(KEYS)::value ? ca_kswz<D>(row) : ca_vswz<D>(row);
+      ca_dma(base + at + 16 * ((lane & (LPR - 1)) ^ swz), to);
+    }
+  };
+  auto whole = [&](const char* base, uint16_t* to, auto off, auto KEYS) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < IPW; ++i) one(base, to, off, i, KEYS);
+  };
   // where the lane's operands lie (halves): K of step s, V of dim block nb
   auto kat = [&](int s) { return jl * D + 8 * ((2 * s + hh) ^ ca_kswz<D>(jl)); };
   auto vat = [&](int nb) { return ca_trat<D>(lane, nb); };
-  // the rare move of the running maximum: S are the half tile's scores, whose weights left the range
-  auto move = [&](int b, const f32x16& S) __attribute__((always_inline)) {
-    float mr = -__builtin_inff();
-#pragma unroll
-    for (int a = 0; a < 16; ++a) mr = __builtin_elementwise_maximum(mr, S[a]);
-    const float mx = half_max(mr) * A.c - CaType<T>::top;
-    const float mnew = mx > m[b] || mx != mx ? mx : m[b];
-    const float alpha = __builtin_amdgcn_exp2f(m[b] - mnew);
-    m[b] = mnew;
-    l[b] *= alpha;
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int a = 0; a < 16; ++a) o[b][nb][a] *= alpha;
-  };
-  // weight pair i of 8 RB: rows i / 8, elements 2 (i % 8), + 1
-  auto weigh = [&](int i, const f32x16 (&S)[RB], u32x4 (&P)[RB][2], float (&lt)[RB]) __attribute__((always_inline)) {
-    const int b = i / 8, a = 2 * (i % 8);
-    const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[b][a], A.c, -m[b]));
-    const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[b][a + 1], A.c, -m[b]));
-    lt[b] += x0 + x1;
-    P[b][a / 8][(a % 8) / 2] = Pk<T>::pack(x0, x1);
+  // weight pair i of 8: elements 2 i, + 1
+  auto weigh = [&](int i, const f32x16& S, u32x4 (&P)[2], float& lt) __attribute__((always_inline)) {
+    const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[2 * i], A.c, -m));
+    const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[2 * i + 1], A.c, -m));
+    lt += x0 + x1;
+    P[i / 4][i % 4] = Pk<T>::pack(x0, x1);
   };
   // the sums are in accumulation registers, written by the assembly below, whose results are
   // readable after 18 cycles of issue
   auto ready = [&]() __attribute__((always_inline)) {
     asm volatile("s_nop 15\n\ts_nop 15");
 #pragma unroll
-    for (int b = 0; b < RB; ++b)
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) asm volatile("" : "+a"(o[b][nb]));
+    for (int nb = 0; nb < NB; ++nb) asm volatile("" : "+a"(o[nb]));
   };
-  auto settle = [&](const f32x16 (&S)[RB], u32x4 (&P)[RB][2], float (&lt)[RB]) __attribute__((always_inline)) {
-    bool far = false;
-#pragma unroll
-    for (int b = 0; b < RB; ++b) far |= !(lt[b] <= CaType<T>::limit);
-    if (__ballot(far)) {
+  // a half tile's weights have left the range: the maximum moves, and they are taken again
+  auto settle = [&](const f32x16& S, u32x4 (&P)[2], float& lt) __attribute__((always_inline)) {
+    if (__ballot(!(lt <= CaType<T>::limit))) {
       ready();
+      float mr = -__builtin_inff();
 #pragma unroll
-      for (int b = 0; b < RB; ++b) move(b, S[b]), lt[b] = 0.f;
+      for (int a = 0; a < 16; ++a) mr = __builtin_elementwise_maximum(mr, S[a]);
+      const float mx = half_max(mr) * A.c - CaType<T>::top;
+      const float mnew = mx > m || mx != mx ? mx : m;
+      const float alpha = __builtin_amdgcn_exp2f(m - mnew);
+      m = mnew;
+      l *= alpha;
 #pragma unroll
-      for (int i = 0; i < PAIRS; ++i) weigh(i, S, P, lt);
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int a = 0; a < 16; ++a) o[nb][a] *= alpha;
+      lt = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) weigh(i, S, P, lt);
     }
-#pragma unroll
-    for (int b = 0; b < RB; ++b) l[b] += lt[b];
+    l += lt;
   };
-  auto scores = [&](f32x16 (&S)[RB], const uint16_t* kt) __attribute__((always_inline)) {
+  auto scores = [&](f32x16& S, const uint16_t* kt) __attribute__((always_inline)) {
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      const u32x4 f = *(const u32x4*)(kt + kat(s));
-#pragma unroll
-      for (int b = 0; b < RB; ++b) S[b] = Mfma<T>::run(f, q[b][s], s ? S[b] : zero16());
-    }
+    for (int s = 0; s < NS; ++s) S = Mfma<T>::run(*(const u32x4*)(kt + kat(s)), q[s], s ? S : zero16());
   };
   // One turn: S of this half tile's scores -> P, the scores SX of the half tile in kt, the sums of the
   // one in vt with its weights PP.  Operands are read AHEAD steps before their products; the first
   // ones by the turn before, which at `mid`, with all its own reads done, meets the other waves where
   // the next turn's tiles have to be there.  extra(i): what else step i issues.
   constexpr int AHEAD = 3, STEPS = NS;
-  static_assert(NS == 2 * NB && STEPS >= AHEAD, "a turn's steps come in pairs");
+  static_assert(NS == 2 * NB && STEPS % (AHEAD + 1) == 0, "the ring of operands goes on from turn to turn");
   u32x4 kf[AHEAD + 1];
   u32x2 vf[AHEAD + 1][2];
   auto rdk = [&](const uint16_t* kt, int i) __attribute__((always_inline)) {
@@ -583,31 +581,25 @@ __global__ __launch_bounds__(256, 1) void ca_many_kernel(CacheArgs A) {
     vf[i % (AHEAD + 1)][0] = ca_trread(at);
     vf[i % (AHEAD + 1)][1] = ca_trread(at + 8 * D);
   };
-  auto turn = [&](const f32x16 (&S)[RB], f32x16 (&SX)[RB], u32x4 (&P)[RB][2], const u32x4 (&PP)[RB][2],
-                  const uint16_t* kt, const uint16_t* vt, const uint16_t* kn, const uint16_t* vn, auto mid, auto extra)
+  auto turn = [&](const f32x16& S, f32x16& SX, u32x4 (&P)[2], const u32x4 (&PP)[2], const uint16_t* kt,
+                  const uint16_t* vt, const uint16_t* kn, const uint16_t* vn, auto mid, auto extra)
       __attribute__((always_inline)) {
-    static_assert(STEPS % (AHEAD + 1) == 0, "the ring goes on from turn to turn");
-    float lt[RB], x0[2], x1[2];
-#pragma unroll
-    for (int b = 0; b < RB; ++b) lt[b] = 0.f;
+    float lt = 0.f, x0[2], x1[2];
     // the weights' operations, a slot behind each product: of pair j the products and the first
-    // exponential, then the second, with the packing and sum of the pair before
-    constexpr int SLOTS = 2 * STEPS * RB, EACH = SLOTS / PAIRS;  // 2 (D = 128), 1
-    auto pack = [&](int j) __attribute__((always_inline)) {
-      const int b = j / 8, a = 2 * (j % 8);
-      P[b][a / 8][(a % 8) / 2] = Pk<T>::pack(x0[j & 1], x1[j & 1]);
-    };
-    auto add = [&](int j) __attribute__((always_inline)) { lt[j / 8] += x0[j & 1] + x1[j & 1]; };
+    // exponential, then the second, with the packing and sum of the pair before (in ordinary
+    // additions: a dot product of the packed pair waits for the matrix unit)
+    constexpr int EACH = 2 * STEPS / 8;  // slots of a pair: 2 (D = 128), 1
+    auto pack = [&](int j) __attribute__((always_inline)) { P[j / 4][j % 4] = Pk<T>::pack(x0[j & 1], x1[j & 1]); };
     auto slot = [&](int n) __attribute__((always_inline)) {
-      const int j = n / EACH, b = j / 8, a = 2 * (j % 8);
+      const int j = n / EACH;
       if (EACH == 1 || n % 2 == 0) {
-        x0[j & 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[b][a], A.c, -m[b]));
-        x1[j & 1] = __builtin_fmaf(S[b][a + 1], A.c, -m[b]);
+        x0[j & 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[2 * j], A.c, -m));
+        x1[j & 1] = __builtin_fmaf(S[2 * j + 1], A.c, -m);
         if (j) pack(j - 1);
       }
       if (EACH == 1 || n % 2 == 1) {
         x1[j & 1] = __builtin_amdgcn_exp2f(x1[j & 1]);
-        if (j) add(j - 1);
+        if (j) lt += x0[(j - 1) & 1] + x1[(j - 1) & 1];
       }
       __builtin_amdgcn_sched_barrier(0);
     };
@@ -619,35 +611,29 @@ __global__ __launch_bounds__(256, 1) void ca_many_kernel(CacheArgs A) {
       rdv(i + AHEAD < STEPS ? vt : vn, (i + AHEAD) % STEPS);
       extra(i);
       __builtin_amdgcn_sched_barrier(0);
+      if (i == 0) ca_mfma_score<T, D, true>(SX, kf[0], q[0]);
+      else ca_mfma_score<T, D, false>(SX, kf[i % (AHEAD + 1)], q[i]);
+      __builtin_amdgcn_sched_barrier(0);
+      slot(2 * i);
       const u32x2 f0 = vf[i % (AHEAD + 1)][0], f1 = vf[i % (AHEAD + 1)][1];
-      const u32x4 f{f0[0], f0[1], f1[0], f1[1]};
-#pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        SX[b] = Mfma<T>::run(kf[i % (AHEAD + 1)], q[b][i], i ? SX[b] : zero16());
-        __builtin_amdgcn_sched_barrier(0);
-        slot(2 * RB * i + b);
-      }
-#pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        ca_mfma_a<T>(o[b][i / 2], f, PP[b][i % 2]);
-        __builtin_amdgcn_sched_barrier(0);
-        slot(2 * RB * i + RB + b);
-      }
+      ca_mfma_sum<T>(o[i / 2], u32x4{f0[0], f0[1], f1[0], f1[1]}, PP[i % 2]);
+      __builtin_amdgcn_sched_barrier(0);
+      slot(2 * i + 1);
     }
-    pack(PAIRS - 1);
-    add(PAIRS - 1);
+    pack(7);
+    lt += x0[1] + x1[1];
     settle(S, P, lt);
   };
 
   if (nf > 0) {
-    f32x16 s0[RB], s1[RB];
-    u32x4 p0[RB][2], p1[RB][2];
+    f32x16 s0, s1;
+    u32x4 p0[2], p1[2];
     // (tiles past the last of the pipeline are fetched like it, and not used)
     auto last = [&](int t) { return min(t, nf - 1); };
-    auto look = [&](int t) { return ca_entry(A, table, P16 ? 64 * (t0 + last(t)) + 16 * wave : pos_of(last(t))); };
+    auto look = [&](int t) { return ca_entry(A, table, P16 ? 64 * (t0 + last(t)) + KW * wave : pos_of(last(t))); };
     auto find = [&](int t, uint32_t entry) {
       if constexpr (P16) {
-        const int pos = 64 * (t0 + last(t)) + 16 * wave;
+        const int pos = 64 * (t0 + last(t)) + KW * wave;
         entry = __builtin_amdgcn_readfirstlane(entry);
         return (long long)entry * A.kv_page + (A.shift >= 0 ? pos & (A.page - 1) : pos % A.page) * A.kv_row;
       } else {
@@ -655,31 +641,13 @@ __global__ __launch_bounds__(256, 1) void ca_many_kernel(CacheArgs A) {
         return ca_offset(A, entry, pos_of(last(t)), ok);
       }
     };
-    auto one = [&](const char* base, uint16_t* to, auto off, int i, auto KEYS) __attribute__((always_inline)) {
-      to += (16 * wave + RPI * i) * D;
-      if constexpr (P16) {
-        ca_dma_at(base + off, decltype(KEYS)::value ? koff[i] : voff[i], to);
-      } else {
-        const int in = RPI * i + lane / LPR, row = 16 * wave + in;
-        const size_t at = (size_t)(uint32_t)__shfl((int)off, in, 64) * 16;
-        const int swz = decltype(KEYS)::value ? ca_kswz<D>(row) : ca_vswz<D>(row);
-        ca_dma(base + at + 16 * ((lane & (LPR - 1)) ^ swz), to);
-      }
-    };
-    auto whole = [&](const char* base, uint16_t* to, auto off, auto KEYS) __attribute__((always_inline)) {
-#pragma unroll
-      for (int i = 0; i < 16 / RPI; ++i) one(base, to, off, i, KEYS);
-    };
     // where tiles t + 1 and t + 2 lie; the table's entry of tile t + 3
     auto off0 = find(0, look(0)), off1 = find(1, look(1)), off2 = find(2, look(2));
     uint32_t entry = look(3);
     whole(kbase, sK0, off0, Yes{});
     // before the first half tile: values and weights of zero
-    for (int i = threadIdx.x; i < 8 * D; i += 256) *(u32x4*)(sV1 + 8 * i) = u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int b = 0; b < RB; ++b)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) p1[b][i] = u32x4{0u, 0u, 0u, 0u};
+    for (int i = threadIdx.x; i < 8 * D; i += 64 * W) *(u32x4*)(sV1 + 8 * i) = u32x4{0u, 0u, 0u, 0u};
+    p1[0] = p1[1] = u32x4{0u, 0u, 0u, 0u};
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     whole(kbase, sK1, off1, Yes{});
@@ -701,13 +669,13 @@ __global__ __launch_bounds__(256, 1) void ca_many_kernel(CacheArgs A) {
       else meet();
       const auto off3 = find(t + 3, entry);  // (here, where no load is under way)
       auto ask = [&](int i) __attribute__((always_inline)) {
-        if (i < 16 / RPI) one(kbase, kt, off2, i, Yes{}), one(vbase, vw, off1, i, No{});
+        if (i < IPW) one(kbase, kt, off2, i, Yes{}), one(vbase, vw, off1, i, No{});
       };
       if (live) {
         turn(s1, s0, p1, p0, kx, vt, kx + 32 * D, vt + 32 * D, none, ask);
       } else {
 #pragma unroll
-        for (int i = 0; i < 16 / RPI; ++i) ask(i);
+        for (int i = 0; i < IPW; ++i) ask(i);
       }
       entry = look(t + 4);
       off1 = off2, off2 = off3;
@@ -725,8 +693,7 @@ __global__ __launch_bounds__(256, 1) void ca_many_kernel(CacheArgs A) {
         for (int mm = 0; mm < 2; ++mm) {
           const uint16_t* at = vt + vat(nb) + 16 * mm * D;
           const u32x2 f0 = ca_trread(at), f1 = ca_trread(at + 8 * D);
-#pragma unroll
-          for (int b = 0; b < RB; ++b) ca_mfma_a<T>(o[b][nb], u32x4{f0[0], f0[1], f1[0], f1[1]}, p1[b][mm]);
+          ca_mfma_sum<T>(o[nb], u32x4{f0[0], f0[1], f1[0], f1[1]}, p1[mm]);
         }
       ready();
     }
@@ -737,48 +704,38 @@ __global__ __launch_bounds__(256, 1) void ca_many_kernel(CacheArgs A) {
   // ---- tiles with hidden keys: those of a row are not seen, and an inf or NaN among their values
   // (left out of the products, where a weight of 0 would make it NaN) goes to the rows that see it
   if (nf < nt) {
-    CacheSight sight[RB];
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      int tok, head;
-      row_of(b, tok, head);
-      sight[b] = CacheSight{
-          A.mask ? A.mask + (A.offsets ? (w.row0 + tok) * A.mask_row : w.b * A.mask_batch + tok * A.mask_row) : nullptr,
-          w.first, A.causal ? w.first + tok : w.L - 1, A.mask_cols};
-    }
+    const CacheSight sight{
+        A.mask ? A.mask + (A.offsets ? (w.row0 + tok) * A.mask_row : w.b * A.mask_batch + tok * A.mask_row) : nullptr,
+        w.first, A.causal ? w.first + tok : w.L - 1, A.mask_cols};
     auto ask = [&](int t, uint16_t* kt, uint16_t* vt) __attribute__((always_inline)) {
       bool ok;
       const uint32_t off = ca_offset(A, ca_entry(A, table, pos_of(t)), pos_of(t), ok);
       const uint64_t bad = __ballot(!ok);
-      if (lane == 0) sBad[t & 1][wave] = (uint32_t)bad & 0xffffu;
-      fetch(kbase, kt, off, Yes{});
-      fetch(vbase, vt, off, No{});
+      if (lane == 0) sBad[t & 1][wave] = (uint32_t)bad & ((1u << KW) - 1u);
+      whole(kbase, kt, off, Yes{});
+      whole(vbase, vt, off, No{});
     };
     auto hidden = [&](int t, int kb, const uint16_t* kt, const uint16_t* vt) __attribute__((always_inline)) {
       const int base = 64 * (t0 + t) + 32 * kb;
-      f32x16 S[RB];
-      u32x4 P[RB][2];
-      uint32_t seen[RB];
-      float lt[RB];
+      f32x16 S;
+      u32x4 P[2];
       scores(S, kt);
+      uint32_t seen = 0, bad = 0;
 #pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        uint32_t x = 0;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int j = 8 * g + 4 * hh;
-          x |= sight[b].sees4(base + j) << j;
-        }
-        x |= half_partner(x);
-        x &= ~(sBad[t & 1][2 * kb] | sBad[t & 1][2 * kb + 1] << 16);
-        seen[b] = x;
-#pragma unroll
-        for (int a = 0; a < 16; ++a)
-          if (!(x >> (8 * (a / 4) + 4 * hh + a % 4) & 1)) S[b][a] = -__builtin_inff();
-        lt[b] = 0.f;
+      for (int g = 0; g < 4; ++g) {
+        const int j = 8 * g + 4 * hh;
+        seen |= sight.sees4(base + j) << j;
       }
+      seen |= half_partner(seen);
 #pragma unroll
-      for (int i = 0; i < PAIRS; ++i) weigh(i, S, P, lt);
+      for (int x = 0; x < W / 2; ++x) bad |= sBad[t & 1][W / 2 * kb + x] << (KW * x);
+      seen &= ~bad;
+#pragma unroll
+      for (int a = 0; a < 16; ++a)
+        if (!(seen >> (8 * (a / 4) + 4 * hh + a % 4) & 1)) S[a] = -__builtin_inff();
+      float lt = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) weigh(i, S, P, lt);
       settle(S, P, lt);
       bool odd = false;
 #pragma unroll
@@ -788,9 +745,7 @@ __global__ __launch_bounds__(256, 1) void ca_many_kernel(CacheArgs A) {
           const uint16_t* at = vt + vat(nb) + 16 * mm * D;
           u32x2 f[2] = {ca_trread(at), ca_trread(at + 8 * D)};
           odd |= ca_clean<T>(f);
-#pragma unroll
-          for (int b = 0; b < RB; ++b)
-            o[b][nb] = Mfma<T>::run(u32x4{f[0][0], f[0][1], f[1][0], f[1][1]}, P[b][mm], o[b][nb]);
+          o[nb] = Mfma<T>::run(u32x4{f[0][0], f[0][1], f[1][0], f[1][1]}, P[mm], o[nb]);
         }
       if (__ballot(odd)) {
         for (int j = 0; j < 32; ++j)
@@ -800,53 +755,45 @@ __global__ __launch_bounds__(256, 1) void ca_many_kernel(CacheArgs A) {
             for (int a = 0; a < 16; ++a) {
               const int d = 32 * nb + 8 * (a / 4) + 4 * hh + a % 4;
               const uint16_t u = vt[j * D + 8 * ((d >> 3) ^ ca_vswz<D>(j)) + (d & 7)];
-              if ((u & CaType<T>::inf) == CaType<T>::inf)
-#pragma unroll
-                for (int b = 0; b < RB; ++b)
-                  if (seen[b] >> j & 1) o[b][nb][a] += T::to_f(u);
+              if ((u & CaType<T>::inf) == CaType<T>::inf && (seen >> j & 1)) o[nb][a] += T::to_f(u);
             }
       }
     };
-    ask(nf, sK0, sV0);
+    ask(nf, (nf & 1) ? sK1 : sK0, (nf & 1) ? sV1 : sV0);
     for (int t = nf; t < nt; ++t) {
-      const bool even = !((t - nf) & 1);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
-      if (t + 1 < nt) ask(t + 1, even ? sK1 : sK0, even ? sV1 : sV0);
+      if (t + 1 < nt) ask(t + 1, (t & 1) ? sK0 : sK1, (t & 1) ? sV0 : sV1);
       if (live)
 #pragma clang loop unroll(disable)
-        for (int kb = 0; kb < 2; ++kb) hidden(t, kb, (even ? sK0 : sK1) + 32 * kb * D, (even ? sV0 : sV1) + 32 * kb * D);
+        for (int kb = 0; kb < 2; ++kb)
+          hidden(t, kb, ((t & 1) ? sK1 : sK0) + 32 * kb * D, ((t & 1) ? sV1 : sV0) + 32 * kb * D);
     }
   }
   if (!live) return;
-#pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    const float lt = half_sum(l[b]);
-    if (wr0 + 32 * b + jl >= w.rows) continue;
-    int tok, head;
-    row_of(b, tok, head);
-    const long long at = (w.row0 + tok) * A.HQ + head;
-    if (parts > 1) {
-      const long long pr = (long long)part * A.T * A.HQ + at;
-      float* op = A.opart + pr * D + 4 * hh;
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *(f32x4*)(op + 32 * nb + 8 * g) = f32x4{o[b][nb][4 * g], o[b][nb][4 * g + 1], o[b][nb][4 * g + 2], o[b][nb][4 * g + 3]};
-      if (hh == 0) A.mlpart[2 * pr] = m[b], A.mlpart[2 * pr + 1] = lt;
-      continue;
-    }
-    const float inv = lt == 0.f ? 0.f : 1.f / lt;
-    char* dst = (char*)ca_token(A.out, A, w, A.o_batch, A.o_row, tok) + head * A.o_head + 8 * hh;
+  const float lt = half_sum(l);
+  if (wr0 + jl >= w.rows) return;
+  const long long at = (w.row0 + tok) * A.HQ + head;
+  if (parts > 1) {
+    const long long pr = (long long)part * A.T * A.HQ + at;
+    float* op = A.opart + pr * D + 4 * hh;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        *(u32x2*)(dst + 64 * nb + 16 * g) = u32x2{Pk<T>::pack(o[b][nb][4 * g] * inv, o[b][nb][4 * g + 1] * inv),
-                                                  Pk<T>::pack(o[b][nb][4 * g + 2] * inv, o[b][nb][4 * g + 3] * inv)};
-    if (A.lse && hh == 0) A.lse[at] = lt == 0.f ? -__builtin_inff() : 0.6931471805599453f * (m[b] + __log2f(lt));
+        *(f32x4*)(op + 32 * nb + 8 * g) = f32x4{o[nb][4 * g], o[nb][4 * g + 1], o[nb][4 * g + 2], o[nb][4 * g + 3]};
+    if (hh == 0) A.mlpart[2 * pr] = m, A.mlpart[2 * pr + 1] = lt;
+    return;
   }
+  const float inv = lt == 0.f ? 0.f : 1.f / lt;
+  char* dst = (char*)ca_token(A.out, A, w, A.o_batch, A.o_row, tok) + head * A.o_head + 8 * hh;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *(u32x2*)(dst + 64 * nb + 16 * g) = u32x2{Pk<T>::pack(o[nb][4 * g] * inv, o[nb][4 * g + 1] * inv),
+                                                Pk<T>::pack(o[nb][4 * g + 2] * inv, o[nb][4 * g + 3] * inv)};
+  if (A.lse && hh == 0) A.lse[at] = lt == 0.f ? -__builtin_inff() : 0.6931471805599453f * (m + __log2f(lt));
 }
 
 // joins the parts of a row block's rows, eight threads a row
@@ -967,16 +914,17 @@ extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, 
   auto run = [&](auto t, auto d) {
     using TT = decltype(t);
     constexpr int D = decltype(d)::value;
-    auto go = [&](auto kernel, auto join) {
-      hipLaunchKernelGGL(kernel, dim3((A.items + 7) / 8 * 8), dim3(256), 0, (hipStream_t)stream, A);
+    auto go = [&](auto kernel, int threads, auto join) {
+      hipLaunchKernelGGL(kernel, dim3((A.items + 7) / 8 * 8), dim3(threads), 0, (hipStream_t)stream, A);
       if (A.S > 1)
         hipLaunchKernelGGL(join, dim3((unsigned)(tiles * a->HK), block / 32), dim3(256), 0, (hipStream_t)stream, A);
     };
-    if (block == 32) go(ca_few_kernel<TT, D>, ca_combine_kernel<TT, D, 32>);
-    else if (block == 128) p16 ? go(ca_many_kernel<TT, D, 1, true>, ca_combine_kernel<TT, D, 128>)
-                               : go(ca_many_kernel<TT, D, 1, false>, ca_combine_kernel<TT, D, 128>);
-    else p16 ? go(ca_many_kernel<TT, D, 2, true>, ca_combine_kernel<TT, D, 256>)
-             : go(ca_many_kernel<TT, D, 2, false>, ca_combine_kernel<TT, D, 256>);
+    if (block == 32)
+      go(ca_few_kernel<TT, D>, 256, ca_combine_kernel<TT, D, 32>);
+    else if (block == 128)
+      go(p16 ? ca_many_kernel<TT, D, 4, true> : ca_many_kernel<TT, D, 4, false>, 256, ca_combine_kernel<TT, D, 128>);
+    else
+      go(p16 ? ca_many_kernel<TT, D, 8, true> : ca_many_kernel<TT, D, 8, false>, 512, ca_combine_kernel<TT, D, 256>);
   };
   using D64 = std::integral_constant<int, 64>;
   using D128 = std::integral_constant<int, 128>;
