@@ -11,14 +11,16 @@
 
 typedef __attribute__((address_space(3))) void ca_lds_t;
 
-// 1 KB to LDS, 16 bytes a lane in the order of the lanes.  (In assembly: of the builtin the compiler
+// 1 KB to LDS, 16 bytes a lane in the order of the lanes; ONCE: of what no other work-group reads
+// (sixteen tokens over 32,760 keys: 302 us, 326 without).  (In assembly: of the builtin the compiler
 // knows no more than that it writes LDS, and has the transposing reads wait for every one in flight.
 // The waits and barriers that order them are written out.)
-__device__ inline void ca_dma(const char* from, uint16_t* to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(
-                   __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(ca_lds_t*)to)),
-               "v"(from)
-               : "memory");
+template <bool ONCE = false> __device__ inline void ca_dma(const char* from, uint16_t* to) {
+  const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(ca_lds_t*)to);
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(at), "v"(from) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory");
 }
 
 // the same from a scalar base and an offset a lane
@@ -41,15 +43,16 @@ struct CacheArgs {
   long long table_row, mask_batch, mask_row;
   int B, N, T, HQ, HK, G, pages, page, shift, width, mask_cols, causal;
   float c;  // scale log2(e)
-  int S;    // most parts of a sequence's keys
+  int S, part;  // most parts of a sequence's keys, keys of one
   int tiles, items;  // row blocks; with the parts and key heads
   float* opart;
   float* mlpart;
 };
 
-// parts that a sequence of L keys goes in
+// Parts that a sequence of L keys goes in: of one size, that of the table's keys in S parts, so that all
+// work-groups have about the same to do; CA_PART keys at least.
 #define CA_PART 512
-__device__ inline int ca_parts(int L, int S) { return min(S, max(1, (L + CA_PART - 1) / CA_PART)); }
+__device__ inline int ca_parts(const CacheArgs& A, int L) { return L < 1 ? 1 : (L - 1) / A.part + 1; }
 
 // A work-group's rows: row block `tile` of ROWS packed rows (token, head of the group) of a
 // sequence.  Sequence b owns blocks from offsets[b] G / ROWS + b on, at least as many as it needs.
@@ -235,14 +238,40 @@ __device__ inline bool ca_clean(u32x2 (&f)[N]) {
   return any;
 }
 
+// D / 8 dims from d0 on of packed row r, of a part of its keys or (part < 0) of all: the sums, or the
+// result
+template <typename T, int D>
+__device__ inline void ca_row(const CacheArgs& A, const CacheRows& w, int kh, int r, int part, float m, float l, int d0,
+                              const float (&o)[D / 8]) {
+  const int tok = r / A.G, head = kh * A.G + r - tok * A.G;
+  const long long at = (w.row0 + tok) * A.HQ + head;
+  if (part >= 0) {
+    const long long pr = (long long)part * A.T * A.HQ + at;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+      *(f32x4*)(A.opart + pr * D + d0 + 4 * i) = f32x4{o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]};
+    if (d0 == 0) A.mlpart[2 * pr] = m, A.mlpart[2 * pr + 1] = l;
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  char* dst = (char*)ca_token(A.out, A, w, A.o_batch, A.o_row, tok) + head * A.o_head + 2 * d0;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i)
+    *(u32x4*)(dst + 16 * i) =
+        u32x4{Pk<T>::pack(o[8 * i] * inv, o[8 * i + 1] * inv), Pk<T>::pack(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
+              Pk<T>::pack(o[8 * i + 4] * inv, o[8 * i + 5] * inv), Pk<T>::pack(o[8 * i + 6] * inv, o[8 * i + 7] * inv)};
+  if (A.lse && d0 == 0) A.lse[at] = l == 0.f ? -__builtin_inff() : 0.6931471805599453f * (m + __log2f(l));
+}
+
 // ---- few rows: a work-group's waves take the keys in turn --------------------
 // 32 packed rows a work-group, 32 keys a tile; a wave fetches its own tiles (DMA to
 // its own LDS, one ahead) and keeps sums of its own, which meet at the end.  Where
 // the row blocks are few, a sequence's keys go in parts to several work-groups,
-// whose sums ca_combine_kernel joins.
+// whose sums ca_combine_kernel joins.  Two waves a work-group, two work-groups a CU:
+// one's start and end pass under the other's loads.
 template <typename T, int D>
-__global__ __launch_bounds__(256, 1) void ca_few_kernel(CacheArgs A) {
-  constexpr int WAVES = 4, TILE = 32 * D, LPR = D / 8, RPI = 64 / LPR;  // lanes a row, rows an instruction
+__global__ __launch_bounds__(128, 1) void ca_few_kernel(CacheArgs A) {
+  constexpr int WAVES = 2, TILE = 32 * D, LPR = D / 8, RPI = 64 / LPR;  // lanes a row, rows an instruction
   __shared__ __attribute__((aligned(1024))) uint16_t sK0[WAVES * TILE], sK1[WAVES * TILE];
   __shared__ __attribute__((aligned(1024))) uint16_t sV0[WAVES * TILE], sV1[WAVES * TILE];
   __shared__ float sM[WAVES][32], sL[WAVES][32];
@@ -252,7 +281,7 @@ __global__ __launch_bounds__(256, 1) void ca_few_kernel(CacheArgs A) {
   if (!ca_item(A, part, kh, tile)) return;
   CacheRows w;
   if (!ca_rows<32>(A, tile, w)) return;
-  const int parts = ca_parts(w.L, A.S);
+  const int parts = ca_parts(A, w.L);
   if (part >= parts) return;
   const int r = min(w.r0 + jl, w.rows - 1), tok = r / A.G, head = kh * A.G + r - tok * A.G;
   CacheSight sight{A.mask ? A.mask + (A.offsets ? (w.row0 + tok) * A.mask_row : w.b * A.mask_batch + tok * A.mask_row)
@@ -282,8 +311,8 @@ __global__ __launch_bounds__(256, 1) void ca_few_kernel(CacheArgs A) {
     for (int i = 0; i < 32 / RPI; ++i) {
       const int row = RPI * i + lane / LPR;
       const size_t at = (size_t)(uint32_t)__shfl((int)off, row, 64) * 16;
-      ca_dma(kbase + at + 16 * ((lane & (LPR - 1)) ^ ca_kswz<D>(row)), dk + i * 512);
-      ca_dma(vbase + at + 16 * ((lane & (LPR - 1)) ^ ca_vswz<D>(row)), dv + i * 512);
+      ca_dma<true>(kbase + at + 16 * ((lane & (LPR - 1)) ^ ca_kswz<D>(row)), dk + i * 512);
+      ca_dma<true>(vbase + at + 16 * ((lane & (LPR - 1)) ^ ca_vswz<D>(row)), dv + i * 512);
     }
   };
   // BAD: lanes whose key's table entry lies outside the cache
@@ -372,7 +401,7 @@ __global__ __launch_bounds__(256, 1) void ca_few_kernel(CacheArgs A) {
 #pragma unroll
   for (int x = 0; x < WAVES; ++x) total += sL[x][jl] * __builtin_amdgcn_exp2f(sM[x][jl] - M);
   const float mine = __builtin_amdgcn_exp2f(st.m - M);
-  auto sums = [&](int x) { return (float*)(x < 2 ? sK0 : sK1) + (x & 1) * 32 * D; };
+  auto sums = [&](int x) { return (float*)(x ? sK1 : sK0); };
   float* to = sums(wave);
 #pragma unroll
   for (int nb = 0; nb < D / 32; ++nb)
@@ -382,40 +411,23 @@ __global__ __launch_bounds__(256, 1) void ca_few_kernel(CacheArgs A) {
       *(f32x4*)(to + jl * D + 4 * ch) = f32x4{st.o[nb][4 * g] * mine, st.o[nb][4 * g + 1] * mine,
                                               st.o[nb][4 * g + 2] * mine, st.o[nb][4 * g + 3] * mine};
     }
-  if (wave == 0 && hh == 0) sM[0][jl] = M;
   __syncthreads();
-  if (wave == 0 && hh == 0) sL[0][jl] = total;
+  if (wave == 0 && hh == 0) sM[0][jl] = M, sL[0][jl] = total;
   __syncthreads();
   // a row by eight threads, D / 8 dims each
-  const int rr = threadIdx.x >> 3, d0 = (threadIdx.x & 7) * (D / 8);
-  if (w.r0 + rr >= w.rows) return;
-  const int tok2 = (w.r0 + rr) / A.G, head2 = kh * A.G + w.r0 + rr - tok2 * A.G;
-  const float lt = sL[0][rr];
-  const long long at = (w.row0 + tok2) * A.HQ + head2;
-  float o[D / 8];
+  for (int rr = threadIdx.x >> 3; rr < 32; rr += 8 * WAVES) {
+    if (w.r0 + rr >= w.rows) return;
+    const int d0 = (threadIdx.x & 7) * (D / 8);
+    float o[D / 8];
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < D / 32; ++i) {
+      const int ch = 4 * ((d0 / 4 + i) ^ (rr & 15));
+      const f32x4 x = *(const f32x4*)(sums(0) + rr * D + ch) + *(const f32x4*)(sums(1) + rr * D + ch);
 #pragma unroll
-    for (int y = 0; y < WAVES; ++y) x += *(const f32x4*)(sums(y) + rr * D + 4 * ((d0 / 4 + i) ^ (rr & 15)));
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[4 * i + e] = x[e];
+      for (int e = 0; e < 4; ++e) o[4 * i + e] = x[e];
+    }
+    ca_row<T, D>(A, w, kh, w.r0 + rr, parts > 1 ? part : -1, sM[0][rr], sL[0][rr], d0, o);
   }
-  if (parts > 1) {
-    const long long pr = (long long)part * A.T * A.HQ + at;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-      *(f32x4*)(A.opart + pr * D + d0 + 4 * i) = f32x4{o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]};
-    if (d0 == 0) A.mlpart[2 * pr] = sM[0][rr], A.mlpart[2 * pr + 1] = lt;
-    return;
-  }
-  const float inv = lt == 0.f ? 0.f : 1.f / lt;
-  char* dst = (char*)ca_token(A.out, A, w, A.o_batch, A.o_row, tok2) + head2 * A.o_head + 2 * d0;
-#pragma unroll
-  for (int i = 0; i < D / 64; ++i)
-    *(u32x4*)(dst + 16 * i) = u32x4{Pk<T>::pack(o[8 * i] * inv, o[8 * i + 1] * inv), Pk<T>::pack(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
-                                    Pk<T>::pack(o[8 * i + 4] * inv, o[8 * i + 5] * inv), Pk<T>::pack(o[8 * i + 6] * inv, o[8 * i + 7] * inv)};
-  if (A.lse && d0 == 0) A.lse[at] = lt == 0.f ? -__builtin_inff() : 0.6931471805599453f * (sM[0][rr] + __log2f(lt));
 }
 
 // The products of the pipeline below, with the sums in accumulation registers and the queries where
@@ -459,7 +471,7 @@ __global__ __launch_bounds__(64 * W, 2) void ca_many_kernel(CacheArgs A) {
   if (!ca_item(A, part, kh, tile)) return;
   CacheRows w;
   if (!ca_rows<ROWS>(A, tile, w)) return;
-  const int parts = ca_parts(w.L, A.S);
+  const int parts = ca_parts(A, w.L);
   if (part >= parts) return;
   const int wr0 = w.r0 + 32 * wave;  // the wave's first row
   const bool live = wr0 < w.rows;    // (of the wave)
@@ -796,38 +808,51 @@ __global__ __launch_bounds__(64 * W, 2) void ca_many_kernel(CacheArgs A) {
   if (A.lse && hh == 0) A.lse[at] = lt == 0.f ? -__builtin_inff() : 0.6931471805599453f * (m + __log2f(lt));
 }
 
-// joins the parts of a row block's rows, eight threads a row
+// joins the parts of a row block's rows, 32 lanes a row: a lane weighs two parts and sums D / 32 dims
 template <typename T, int D, int ROWS>
 __global__ __launch_bounds__(256) void ca_combine_kernel(CacheArgs A) {
-  const int kh = blockIdx.x % A.HK, tile = blockIdx.x / A.HK;
+  const int kh = blockIdx.x % A.HK, tile = blockIdx.x / A.HK, lane = threadIdx.x & 31;
   CacheRows w;
   if (!ca_rows<ROWS>(A, tile, w)) return;
-  w.r0 += 32 * blockIdx.y;
-  const int parts = ca_parts(w.L, A.S), rr = threadIdx.x >> 3, d0 = (threadIdx.x & 7) * (D / 8);
-  if (parts < 2 || w.r0 + rr >= w.rows) return;  // (its work-group has written the rows)
-  const int tok = (w.r0 + rr) / A.G, head = kh * A.G + w.r0 + rr - tok * A.G;
+  const int parts = ca_parts(A, w.L), r = w.r0 + 8 * blockIdx.y + (threadIdx.x >> 5);
+  if (parts < 2 || r >= w.rows) return;  // (its work-group has written the rows)
+  const int tok = r / A.G, head = kh * A.G + r - tok * A.G;
   const long long at = (w.row0 + tok) * A.HQ + head, step = (long long)A.T * A.HQ;
-  float M = CA_NONE, total = 0.f, o[D / 8];
-  for (int i = 0; i < parts; ++i) M = __builtin_elementwise_maximum(M, A.mlpart[2 * (at + i * step)]);
+  float m[2], l[2], M, total;
 #pragma unroll
-  for (int e = 0; e < D / 8; ++e) o[e] = 0.f;
-  for (int i = 0; i < parts; ++i) {
-    const float a = __builtin_amdgcn_exp2f(A.mlpart[2 * (at + i * step)] - M);
-    total = __builtin_fmaf(a, A.mlpart[2 * (at + i * step) + 1], total);
+  for (int i = 0; i < 2; ++i) {
+    const bool on = lane + 32 * i < parts;
+    const u32x2 v = on ? *(const u32x2*)(A.mlpart + 2 * (at + (lane + 32 * i) * step)) : u32x2{0u, 0u};
+    m[i] = on ? __builtin_bit_cast(float, (uint32_t)v[0]) : CA_NONE;
+    l[i] = __builtin_bit_cast(float, (uint32_t)v[1]);
+  }
+  M = __builtin_elementwise_maximum(m[0], m[1]);
 #pragma unroll
-    for (int e = 0; e < D / 8; e += 4) {
-      const f32x4 x = *(const f32x4*)(A.opart + (at + i * step) * D + d0 + e);
+  for (int d = 1; d < 32; d <<= 1) M = __builtin_elementwise_maximum(M, __shfl_xor(M, d, 32));
 #pragma unroll
-      for (int f = 0; f < 4; ++f) o[e + f] = __builtin_fmaf(a, x[f], o[e + f]);
+  for (int i = 0; i < 2; ++i) m[i] = __builtin_amdgcn_exp2f(m[i] - M);
+  total = m[0] * l[0] + m[1] * l[1];
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) total += __shfl_xor(total, d, 32);
+  typedef float vec __attribute__((ext_vector_type(D / 32)));
+  vec o = {};
+  const float* src = A.opart + at * D + D / 32 * lane;
+  for (int i = 0; i < parts; i += 8) {
+    vec x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = *(const vec*)(src + min(i + e, parts - 1) * step * D);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float a = __shfl(i < 32 ? m[0] : m[1], (i + e) & 31, 32);  // (0 past the last)
+#pragma unroll
+      for (int f = 0; f < D / 32; ++f) o[f] = i + e < parts ? __builtin_fmaf(a, x[e][f], o[f]) : o[f];
     }
   }
   const float inv = total == 0.f ? 0.f : 1.f / total;
-  char* dst = (char*)ca_token(A.out, A, w, A.o_batch, A.o_row, tok) + head * A.o_head + 2 * d0;
+  char* dst = (char*)ca_token(A.out, A, w, A.o_batch, A.o_row, tok) + head * A.o_head + D / 16 * lane;
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i)
-    *(u32x4*)(dst + 16 * i) = u32x4{Pk<T>::pack(o[8 * i] * inv, o[8 * i + 1] * inv), Pk<T>::pack(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
-                                    Pk<T>::pack(o[8 * i + 4] * inv, o[8 * i + 5] * inv), Pk<T>::pack(o[8 * i + 6] * inv, o[8 * i + 7] * inv)};
-  if (A.lse && d0 == 0) A.lse[at] = total == 0.f ? -__builtin_inff() : 0.6931471805599453f * (M + __log2f(total));
+  for (int f = 0; f < D / 32; f += 2) *(uint32_t*)(dst + 2 * f) = Pk<T>::pack(o[f] * inv, o[f + 1] * inv);
+  if (A.lse && lane == 0) A.lse[at] = total == 0.f ? -__builtin_inff() : 0.6931471805599453f * (M + __log2f(total));
 }
 
 // Packed rows of a row block: by the rows that a sequence may have (all of them, where they are not
@@ -836,13 +861,19 @@ static int ca_block(int ragged, int B, long long T, int G) {
   const long long rows = (ragged ? T : T / B) * G;
   return rows <= 64 ? 32 : rows <= 128 ? 128 : 256;
 }
-// Most parts of a sequence's keys: as many as bring the launch to two rounds of work-groups, of
-// CA_PART keys at least.
-static int ca_split(long long tiles, int HK, long long keys) {
-  const long long wgs = tiles * HK, most = (keys + CA_PART - 1) / CA_PART;
-  if (wgs >= 512 || most < 2) return 1;
-  const long long s = (512 + wgs - 1) / wgs;
-  return (int)(s < most ? (s < 64 ? s : 64) : (most < 64 ? most : 64));
+// Most parts of a sequence's keys, of CA_PART keys at least: as many as bring a small launch to a round
+// of work-groups (256 at once; with few rows two of 512, as sequences differ in length), and a larger
+// one to rounds that are nearly full.
+static int ca_split(int block, long long tiles, int HK, long long keys) {
+  const long long wgs = tiles * HK, slots = block == 32 ? 512 : 256;
+  long long most = (keys + CA_PART - 1) / CA_PART, s = 1;
+  most = most < 64 ? most : 64;
+  if (wgs < slots) {
+    s = ((block == 32 ? 2 : 1) * slots + wgs - 1) / wgs;
+  } else if (wgs < 4 * slots) {
+    while (s < 4 && 20 * wgs * s < 17 * ((wgs * s + slots - 1) / slots) * slots) ++s;
+  }
+  return (int)(s < most ? s : most < 1 ? 1 : most);
 }
 // row blocks of `block` packed rows
 static long long ca_tiles(int block, int ragged, int B, long long T, int G) {
@@ -853,7 +884,7 @@ static size_t ca_ws(int S, long long rows, int D) { return S < 2 ? 0 : (size_t)S
 extern "C" size_t t2t_cache_attention_ws_bytes(int ragged, int B, long long T, int HQ, int HK, int D, long long keys) {
   if (B < 1 || T < 1 || HK < 1 || HQ < HK || keys < 1) return 0;
   const int G = HQ / HK, block = ca_block(ragged, B, T, G);
-  return ca_ws(ca_split(ca_tiles(block, ragged, B, T, G), HK, keys), T * HQ, D);
+  return ca_ws(ca_split(block, ca_tiles(block, ragged, B, T, G), HK, keys), T * HQ, D);
 }
 
 extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -896,7 +927,7 @@ extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, 
   const int ragged = a->offsets != nullptr, block = ca_block(ragged, a->B, T, A.G);
   const long long tiles = ca_tiles(block, ragged, a->B, T, A.G);
   const long long keys = (long long)a->width * a->page_size;
-  A.S = ca_split(tiles, a->HK, keys < 1 ? 1 : keys);
+  A.S = ca_split(block, tiles, a->HK, keys < 1 ? 1 : keys);
   // (as many parts as the workspace holds)
   while (A.S > 1 && (!ws || ws_bytes < ca_ws(A.S, T * a->HQ, a->D))) --A.S;
   if (A.S > 1) {
@@ -904,7 +935,8 @@ extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, 
     A.opart = (float*)ws;
     A.mlpart = A.opart + (size_t)A.S * T * a->HQ * a->D;
   }
-  if (tiles * a->HK * A.S > (1 << 23)) {  // 2^31 threads
+  A.part = A.S > 1 ? (int)((keys + A.S - 1) / A.S) : INT_MAX;
+  if (tiles * a->HK * A.S > (1 << 22)) {  // 2^31 threads
     t2t_set_error("cache_attention: %lld row blocks of %d heads", tiles, a->HK);
     return T2T_ERR_UNSUPPORTED;
   }
@@ -917,10 +949,10 @@ extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, 
     auto go = [&](auto kernel, int threads, auto join) {
       hipLaunchKernelGGL(kernel, dim3((A.items + 7) / 8 * 8), dim3(threads), 0, (hipStream_t)stream, A);
       if (A.S > 1)
-        hipLaunchKernelGGL(join, dim3((unsigned)(tiles * a->HK), block / 32), dim3(256), 0, (hipStream_t)stream, A);
+        hipLaunchKernelGGL(join, dim3((unsigned)(tiles * a->HK), block / 8), dim3(256), 0, (hipStream_t)stream, A);
     };
     if (block == 32)
-      go(ca_few_kernel<TT, D>, 256, ca_combine_kernel<TT, D, 32>);
+      go(ca_few_kernel<TT, D>, 128, ca_combine_kernel<TT, D, 32>);
     else if (block == 128)
       go(p16 ? ca_many_kernel<TT, D, 4, true> : ca_many_kernel<TT, D, 4, false>, 256, ca_combine_kernel<TT, D, 128>);
     else
