@@ -535,8 +535,9 @@ int t2t_int8_dequantize(const void* codes, const float* scales, void* out, int d
 int t2t_int8_product(const void* a_codes, const float* a_scales, const void* w_codes,
                      const float* w_scales, const void* bias, int act, void* out, int dtype,
                      long long out_row_stride, int M, int N, int K, void* stream);
-/* t2t_int8_quantize of x into the workspace and t2t_int8_product.  out and ws
- * share no memory with another argument. */
+/* t2t_int8_quantize of x into the workspace and t2t_int8_product (one launch and no
+ * workspace where M <= 2 and M * Kp <= 32768).  out and ws share no memory with
+ * another argument. */
 size_t t2t_int8_linear_ws_bytes(int M, int N, int K);
 int t2t_int8_linear(const void* x, int dtype, long long x_row_stride, const void* w_codes,
                     const float* w_scales, const void* bias, int act, void* out,

@@ -90,7 +90,7 @@ def test_entries_reject_bad_arguments():
     assert prod(a=odd) == 1 and prod(w=odd) == 1 and prod(out=None) == 1
     assert prod(M=0, a=None, out=None) == 0
 
-    def lin(ws=p, nb=1 << 20, M=4, K=300, x=p):
+    def lin(ws=p, nb=1 << 20, M=40, K=300, x=p):
         return L.t2t_int8_linear(x, 1, 300, p, p, None, 0, p, 40, M, 40, K, ws, nb, None)
     assert lin(ws=None) == 2 and lin(nb=100) == 2 and b"workspace" in L.t2t_last_error()
     assert lin(ws=odd) == 1 and lin(x=None) == 1 and lin(M=0, ws=None) == 0
@@ -148,7 +148,7 @@ def test_a_copied_matrix_is_read_at_its_own_address(launches, how):
 
 
 def test_every_tensor_of_a_call_is_recorded_on_its_stream(launches):
-    M, K, N, dt = 5, 100, 40, torch.bfloat16
+    M, K, N, dt = 50, 100, 40, torch.bfloat16
     W, x, b, out = _cpu(N, K), torch.zeros(M, K, dtype=dt), torch.zeros(N, dtype=dt), torch.zeros(M, N, dtype=dt)
     ws = torch.empty(ops.int8_linear_ws_bytes(M, N, K) + 64, dtype=torch.uint8)
     ops.int8_linear(x, W, b, out=out, ws=ws, stream=type("S", (), {"device": x.device})())
@@ -197,8 +197,8 @@ def test_refused(launches, bad):
         "in_x": lambda: ops.int8_linear(buf[:600].view(6, 100), W, out=buf[500:740].view(6, 40)),
         "in_w": lambda: ops.int8_linear(x, W, out=W.codes.view(torch.bfloat16)[:240].view(6, 40)),
         "in_bias": lambda: ops.int8_linear(x, W, buf[:40], out=buf[39:279].view(6, 40)),
-        "ws_x": lambda: ops.int8_linear(big[:1200].view(torch.bfloat16).view(6, 100), W, ws=big[512:]),
-        "ws_out": lambda: ops.int8_linear(x, W, out=big[:480].view(torch.bfloat16).view(6, 40), ws=big[256:]),
+        "ws_x": lambda: ops.int8_linear(big[:1800].view(torch.bfloat16).view(9, 100), W, ws=big[512:]),
+        "ws_out": lambda: ops.int8_linear(z(9, 100), W, out=big[:720].view(torch.bfloat16).view(9, 40), ws=big[256:]),
         "q_in_x": lambda: ops.int8_quantize(
             buf[:256].view(2, 128), out=ops.Int8(buf[128:1152].view(i8), torch.zeros(2), 2, 128)),
         "d_in_codes": lambda: ops.int8_dequantize(V, out=V.codes.view(torch.bfloat16)[:1000].view(10, 100)),
@@ -334,7 +334,7 @@ def _operands(dev, M, N, K, dt, seed):
     return x, (_randn(g, N, K) * K ** -0.5).to(dt), _randn(g, N).to(dt)
 
 
-SIZES = [(1, 1, 1), (1, 64, 64), (1, 5120, 512), (2, 33, 95), (5, 96, 256), (16, 48, 1024), (17, 31, 300),
+SIZES = [(1, 1, 1), (1, 64, 64), (1, 5000, 33000), (3, 70, 10001), (8, 100, 4097), (9, 100, 4097), (1, 5120, 512), (2, 33, 95), (5, 96, 256), (16, 48, 1024), (17, 31, 300),
          (31, 100, 288), (32, 32, 1571), (33, 257, 512), (64, 640, 2048), (100, 72, 5120), (129, 130, 161),
          (257, 513, 256), (600, 1000, 321), (1000, 1536, 1536), (2049, 776, 64), (4099, 2041, 1571),
          (33, 20481, 256), (700, 1100, 512), (16385, 1030, 1057), (4100, 4200, 1024), (70000, 1025, 96)]

@@ -879,12 +879,17 @@ static int ca_split(int block, long long tiles, int HK, long long keys) {
 static long long ca_tiles(int block, int ragged, int B, long long T, int G) {
   return ragged ? T * G / block + B : B * ((T / B * G + block - 1) / block);
 }
+// (those of a ragged batch that hold rows: about as many)
+static long long ca_full(int block, int ragged, int B, long long T, int G) {
+  const long long n = (T * G + block - 1) / block;
+  return ragged ? (n > B ? n : B) : ca_tiles(block, ragged, B, T, G);
+}
 static size_t ca_ws(int S, long long rows, int D) { return S < 2 ? 0 : (size_t)S * rows * (D + 2) * 4; }
 
 extern "C" size_t t2t_cache_attention_ws_bytes(int ragged, int B, long long T, int HQ, int HK, int D, long long keys) {
   if (B < 1 || T < 1 || HK < 1 || HQ < HK || keys < 1) return 0;
   const int G = HQ / HK, block = ca_block(ragged, B, T, G);
-  return ca_ws(ca_split(block, ca_tiles(block, ragged, B, T, G), HK, keys), T * HQ, D);
+  return ca_ws(ca_split(block, ca_full(block, ragged, B, T, G), HK, keys), T * HQ, D);
 }
 
 extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -927,7 +932,7 @@ extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, 
   const int ragged = a->offsets != nullptr, block = ca_block(ragged, a->B, T, A.G);
   const long long tiles = ca_tiles(block, ragged, a->B, T, A.G);
   const long long keys = (long long)a->width * a->page_size;
-  A.S = ca_split(block, tiles, a->HK, keys < 1 ? 1 : keys);
+  A.S = ca_split(block, ca_full(block, ragged, a->B, T, A.G), a->HK, keys < 1 ? 1 : keys);
   // (as many parts as the workspace holds)
   while (A.S > 1 && (!ws || ws_bytes < ca_ws(A.S, T * a->HQ, a->D))) --A.S;
   if (A.S > 1) {

@@ -254,13 +254,26 @@ __device__ inline float i8_out(int acc, float sw, float sa, float bias) {
 // ---- small launches: the columns split over the waves ------------------------
 // 32 features x 32 tokens a work-group; its eight waves take units of 128 columns
 // in turn, loaded straight into registers, DEPTH units ahead.  The waves' sums
-// meet in LDS.
-template <typename T, int DEPTH, bool GELU>
-__global__ __launch_bounds__(512) void i8_split_kernel(I8Mat a, I8Mat w, const uint16_t* __restrict__ bias,
+// meet in LDS.  With X16 the tokens come in 16 bits, and every work-group quantises
+// them into LDS first, under the loads of its first weights, in the place of a launch
+// before this one.
+#define I8_X16_BYTES 32768  // codes that the LDS holds
+struct I8Src {
+  I8Mat m;            // in 8 bits (its row count in either case), or
+  const uint16_t* x;  // in 16 bits
+  long long stride;
+  int K;
+};
+
+template <typename T, int DEPTH, bool GELU, bool X16>
+__global__ __launch_bounds__(512) void i8_split_kernel(I8Src a, I8Mat w, const uint16_t* __restrict__ bias,
                                                        uint16_t* __restrict__ out, long long ldo, int units,
                                                        int mt, int nt, int per_xcd) {
   constexpr int WAVES = 8;
   __shared__ i32x4 part[WAVES][4][64];
+  __shared__ __attribute__((aligned(16))) char codes[X16 ? I8_X16_BYTES + 32 * 16 : 16];
+  __shared__ uint32_t tops[X16 ? 32 : 1][WAVES];
+  __shared__ float scales[X16 ? 32 : 1];
   const int id = lin_first(per_xcd);
   if (id >= lin_end(mt, nt, per_xcd)) return;
   int mb, nb;
@@ -269,7 +282,7 @@ __global__ __launch_bounds__(512) void i8_split_kernel(I8Mat a, I8Mat w, const u
   const int row = mb * 32 + (lane & 31), feat = nb * 32 + (lane & 31);
   // (rows past the last are read from its block of sixteen, and not stored)
   const char* pw = w.codes + (min(feat, w.rows - 1) >> 4) * w.blk + (feat & 15) * 64;
-  const char* pa = a.codes + (min(row, a.rows - 1) >> 4) * a.blk + (row & 15) * 64;
+  const char* pa = X16 ? nullptr : a.m.codes + (min(row, a.m.rows - 1) >> 4) * a.m.blk + (row & 15) * 64;
   int at[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) at[i] = (i >> 1) * 1024 + (((2 * (i & 1) + (lane >> 5)) ^ i8_swz(lane)) << 4);
@@ -280,7 +293,15 @@ __global__ __launch_bounds__(512) void i8_split_kernel(I8Mat a, I8Mat w, const u
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       t.w[i] = *(const i32x4*)(pw + (size_t)s * 2048 + at[i]);
-      t.a[i] = *(const i32x4*)(pa + (size_t)s * 2048 + at[i]);
+      if constexpr (!X16) t.a[i] = *(const i32x4*)(pa + (size_t)s * 2048 + at[i]);
+    }
+  };
+  const int pitch = 128 * units + 16;  // of the codes' rows in LDS
+  auto fetch = [&](int s, Unit& t) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      t.a[i] = i32x4{};
+      if (row < a.m.rows) t.a[i] = *(const i32x4*)(codes + row * pitch + 128 * s + 64 * (i >> 1) + 32 * (i & 1) + 16 * (lane >> 5));
     }
   };
   i32x16 acc = {};
@@ -288,13 +309,37 @@ __global__ __launch_bounds__(512) void i8_split_kernel(I8Mat a, I8Mat w, const u
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d)
     if (wave + d * WAVES < units) load(wave + d * WAVES, ring[d]);
+  if constexpr (X16) {
+    for (int r = 0; r < a.m.rows; ++r) {
+      uint32_t top = 0;
+      for (int c = 8 * threadIdx.x; c < a.K; c += 8 * 64 * WAVES) top = i8_top(top, i8_load(a.x + r * a.stride + c, a.K - c));
+      top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
+      if (lane == 0) tops[r][wave] = top;
+    }
+    __syncthreads();
+    for (int r = 0; r < a.m.rows; ++r) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int x = 0; x < WAVES; ++x) top = max(top, tops[r][x]);
+      const bool bad = top >= I8Inf<T>::bits;
+      const I8Scale k = i8_scale(T::to_f((uint16_t)top));
+      for (int c = 8 * threadIdx.x; c < 128 * units; c += 8 * 64 * WAVES)
+        *(u32x2*)(codes + r * pitch + c) = bad ? u32x2{0u, 0u} : i8_codes<T>(i8_load(a.x + r * a.stride + c, a.K - c), k);
+      if (threadIdx.x == 0) scales[r] = bad ? __builtin_nanf("") : k.s;
+    }
+    __syncthreads();
+  }
   for (int s = wave; s < units; s += DEPTH * WAVES) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
       Unit& t = ring[d];
-      if (s + d * WAVES < units)
+      if (s + d * WAVES < units) {
+        if constexpr (X16) fetch(s + d * WAVES, t);
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(t.w[i], t.a[i], acc, 0, 0, 0);
+      }
       if (s + (d + DEPTH) * WAVES < units) load(s + (d + DEPTH) * WAVES, t);
     }
   }
@@ -308,8 +353,8 @@ __global__ __launch_bounds__(512) void i8_split_kernel(I8Mat a, I8Mat w, const u
   i32x4 v = part[0][q][lane];
 #pragma unroll
   for (int x = 1; x < WAVES; ++x) v += part[x][q][lane];
-  if (row < a.rows && f < w.rows) {
-    const float sa = a.scales[row];
+  if (row < a.m.rows && f < w.rows) {
+    const float sa = X16 ? scales[row] : a.m.scales[row];
     float y[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -320,17 +365,18 @@ __global__ __launch_bounds__(512) void i8_split_kernel(I8Mat a, I8Mat w, const u
   }
 }
 
-template <typename T, int DEPTH>
-static int i8_split_launch(const I8Mat& a, const I8Mat& w, const uint16_t* bias, int act, uint16_t* out,
+template <typename T, int DEPTH, bool X16>
+static int i8_split_launch(const I8Src& a, const I8Mat& w, const uint16_t* bias, int act, uint16_t* out,
                            long long ldo, int units, hipStream_t st) {
-  const long long tiles = (long long)a.blocks * w.blocks;
+  const long long tiles = (long long)a.m.blocks * w.blocks;
   if ((tiles + 7) / 8 > (1 << 19)) {  // 2^31 threads
-    t2t_set_error("int8_product: M=%d N=%d", a.rows, w.rows);
+    t2t_set_error("int8_product: M=%d N=%d", a.m.rows, w.rows);
     return T2T_ERR_UNSUPPORTED;
   }
   const int per = cdiv(tiles, 8);
-  auto kernel = act == T2T_ACT_GELU_TANH ? i8_split_kernel<T, DEPTH, true> : i8_split_kernel<T, DEPTH, false>;
-  hipLaunchKernelGGL(kernel, dim3(8 * per), dim3(512), 0, st, a, w, bias, out, ldo, units, a.blocks, w.blocks, per);
+  auto kernel =
+      act == T2T_ACT_GELU_TANH ? i8_split_kernel<T, DEPTH, true, X16> : i8_split_kernel<T, DEPTH, false, X16>;
+  hipLaunchKernelGGL(kernel, dim3(8 * per), dim3(512), 0, st, a, w, bias, out, ldo, units, a.m.blocks, w.blocks, per);
   T2T_LAUNCH_CHECK("int8_product");
   return T2T_OK;
 }
@@ -719,7 +765,7 @@ static int i8_product(const I8Mat& a, const I8Mat& w, const uint16_t* bias, int 
                       int units, hipStream_t st) {
   const long long big = (long long)cdiv(a.blocks, 8) * cdiv(w.blocks, 8);
   const long long mid = (long long)cdiv(a.blocks, 4) * cdiv(w.blocks, 4);
-  if ((long long)a.blocks * w.blocks <= 512) return i8_split_launch<T, 2>(a, w, bias, act, out, ldo, units, st);
+  if ((long long)a.blocks * w.blocks <= 512) return i8_split_launch<T, 4, false>(I8Src{a, nullptr, 0, 0}, w, bias, act, out, ldo, units, st);
   if (big >= 256 && 4 * big <= mid + mid / 4) return i8_tile_launch<T, 4, 4>(a, w, bias, act, out, ldo, units, st);
   return i8_tile_launch<T, 2, 2>(a, w, bias, act, out, ldo, units, st);
 }
@@ -751,11 +797,15 @@ extern "C" int t2t_int8_product(const void* a_codes, const float* a_scales, cons
                                                                    (hipStream_t)stream);
 }
 
+// Few rows are quantised by the product itself: every work-group does it again (5120 x 5120, one row: 7.0
+// us, two 8.0, four 11.1; with a launch before it 10.0 throughout).
+static bool i8_few(int M, int K) { return M <= 2 && M * i8_kp(K) <= I8_X16_BYTES; }
+
 // codes, then scales
 extern "C" size_t t2t_int8_linear_ws_bytes(int M, int N, int K) {
   (void)N;
   const size_t codes = t2t_int8_code_bytes(M, K);
-  return codes ? codes + t2t_align256((size_t)M * 4) : 0;
+  return codes && !i8_few(M, K) ? codes + t2t_align256((size_t)M * 4) : 0;
 }
 
 extern "C" int t2t_int8_linear(const void* x, int dtype, long long x_row_stride, const void* w_codes,
@@ -767,6 +817,12 @@ extern "C" int t2t_int8_linear(const void* x, int dtype, long long x_row_stride,
   if (rc != T2T_OK || M == 0) return rc;
   rc = i8_check_rows("int8_linear", x, dtype, x_row_stride, M, K);
   if (rc != T2T_OK) return rc;
+  if (i8_few(M, K)) {
+    const I8Src a{I8Mat{nullptr, 0, nullptr, M, 1}, (const uint16_t*)x, x_row_stride, K};
+    const I8Mat w{(const char*)w_codes, 16LL * i8_kp(K), w_scales, N, cdiv(N, 32)};
+    return (dtype == T2T_BF16 ? i8_split_launch<BF16T, 5, true> : i8_split_launch<F16T, 5, true>)(
+        a, w, (const uint16_t*)bias, act, (uint16_t*)out, out_row_stride, i8_kp(K) / 128, (hipStream_t)stream);
+  }
   const size_t need = t2t_int8_linear_ws_bytes(M, N, K);
   if (!ws || ws_bytes < need) {
     t2t_set_error("int8_linear: workspace %zu < %zu bytes", ws ? ws_bytes : (size_t)0, need);

@@ -1380,7 +1380,8 @@ def int8_dequantize(t, dtype=torch.bfloat16, out=None, stream=None):
 
 
 def int8_linear_ws_bytes(M, N, K):
-    """Workspace of int8_linear for a 16-bit x of M rows."""
+    """Workspace of int8_linear for a 16-bit x of M rows (0 where the product
+    quantises them itself)."""
     return size_query("t2t_int8_linear_ws_bytes", M, N, K)
 
 
