@@ -44,7 +44,6 @@ struct CacheArgs {
   int B, N, T, HQ, HK, G, pages, page, shift, width, mask_cols, causal;
   float c;  // scale log2(e)
   int S, part;  // most parts of a sequence's keys, keys of one
-  int tiles, items;  // row blocks; with the parts and key heads
   float* opart;
   float* mlpart;
 };
@@ -54,40 +53,47 @@ struct CacheArgs {
 #define CA_PART 512
 __device__ inline int ca_parts(const CacheArgs& A, int L) { return L < 1 ? 1 : (L - 1) / A.part + 1; }
 
-// A work-group's rows: row block `tile` of ROWS packed rows (token, head of the group) of a
-// sequence.  Sequence b owns blocks from offsets[b] G / ROWS + b on, at least as many as it needs.
+// A work-group's rows: a row block of ROWS packed rows (token, head of the group) of a sequence.
 struct CacheRows {
   int b, n, L, first;   // sequence, its new tokens, keys, older keys
   int r0, rows;         // packed rows from r0 on, how many there are in the sequence
   long long row0;       // its first row among all
 };
-template <int ROWS>
-__device__ inline bool ca_rows(const CacheArgs& A, int tile, CacheRows& w) {
-  int first_tile;
+// sequence b: offsets and lengths are held to what there is
+__device__ inline void ca_sequence(const CacheArgs& A, int b, CacheRows& w) {
+  w.b = b;
   if (A.offsets) {
-    const int lane = __lane_id();
-    int count = 0;
-    for (int b0 = 0; b0 < A.B; b0 += 64) {
-      const int b = b0 + lane;
-      const long long off = b < A.B ? min(max(A.offsets[b], 0), A.T) : 0;
-      count += __popcll(__ballot(b < A.B && off * A.G / ROWS + b <= tile));
-    }
-    w.b = max(count - 1, 0);
-    const int lo = min(max(A.offsets[w.b], 0), A.T), hi = min(max(A.offsets[w.b + 1], 0), A.T);
+    const int lo = min(max(A.offsets[b], 0), A.T), hi = min(max(A.offsets[b + 1], 0), A.T);
     w.row0 = lo, w.n = max(hi - lo, 0);
-    first_tile = (int)((long long)lo * A.G / ROWS) + w.b;
   } else {
-    const int per = (int)(((long long)A.N * A.G + ROWS - 1) / ROWS);
-    w.b = tile / per;
-    w.row0 = (long long)w.b * A.N, w.n = A.N;
-    first_tile = w.b * per;
+    w.row0 = (long long)b * A.N, w.n = A.N;
   }
   w.rows = w.n * A.G;
-  w.r0 = (tile - first_tile) * ROWS;
-  if (w.b >= A.B || w.r0 < 0 || w.r0 >= w.rows) return false;
-  w.L = min((long long)max(A.lengths[w.b], 0), (long long)A.width * A.page);
+  w.L = (int)min((long long)max(A.lengths[b], 0), (long long)A.width * A.page);
   w.first = w.L - w.n;
-  return true;
+}
+// Row block `tile` of a launch that does not go by the parts: sequence b owns blocks from offsets[b] G
+// / ROWS + b on, at least as many as it needs.
+template <int ROWS>
+__device__ inline bool ca_rows(const CacheArgs& A, int tile, CacheRows& w) {
+  const int per = A.offsets ? 0 : (int)(((long long)A.N * A.G + ROWS - 1) / ROWS);
+  int b, first;
+  if (A.offsets) {
+    int count = 0;
+    for (int b0 = 0; b0 < A.B; b0 += 64) {
+      const int x = b0 + (int)__lane_id();
+      const long long off = x < A.B ? min(max(A.offsets[x], 0), A.T) : 0;
+      count += __popcll(__ballot(x < A.B && off * A.G / ROWS + x <= tile));
+    }
+    b = max(count - 1, 0);
+    first = (int)((long long)min(max(A.offsets[b], 0), A.T) * A.G / ROWS) + b;
+  } else {
+    b = tile / per, first = b * per;
+  }
+  if (b >= A.B) return false;
+  ca_sequence(A, b, w);
+  w.r0 = (tile - first) * ROWS;
+  return w.r0 >= 0 && w.r0 < w.rows;
 }
 __device__ inline const char* ca_token(const char* p, const CacheArgs& A, const CacheRows& w, long long batch,
                                        long long row, int i) {
@@ -146,41 +152,89 @@ __device__ inline u32x2 ca_trread(const uint16_t* p) {
                                        (__attribute__((address_space(3))) s16x4*)p));
 }
 
-// The lane's row in the mask: hidden are positions past the length, new ones past `last` (causal)
-// and, with a mask, those it does not name.
+// What the lane's row sees: positions up to `last` (the length's, or under causal its own), and of the
+// new ones, with a mask, those it names.
 struct CacheSight {
   const uint8_t* mask;  // the row's bytes for new token 0, or NULL
   int first, last, cols;
-  __device__ bool sees(int pos) const {
-    if (pos > last) return false;
-    if (!mask || pos < first) return true;
-    return pos - first < cols && mask[pos - first] != 0;
-  }
-  // of four positions from pos on, a bit each
-  __device__ uint32_t sees4(int pos) const {
+  // four positions' bytes of the mask, not 0 where they are seen
+  __device__ uint32_t peek(int pos) const {
     const int i = pos - first;
-    if (mask && i >= 0 && i + 3 < cols && pos + 3 <= last) {
-      uint32_t x;
+    uint32_t x = 0x01010101u;
+    if (i >= 0 && i + 3 < cols) {
       __builtin_memcpy(&x, mask + i, 4);
-      return (uint32_t)((x & 0xffu) != 0) | (uint32_t)((x & 0xff00u) != 0) << 1 | (uint32_t)((x & 0xff0000u) != 0) << 2 |
-             (uint32_t)((x & 0xff000000u) != 0) << 3;
-    }
-    uint32_t x = 0;
+    } else if (i > -4) {
+      x = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x |= (uint32_t)sees(pos + e) << e;
+      for (int e = 0; e < 4; ++e)
+        if (i + e < 0 || (i + e < cols && mask[i + e])) x |= 1u << (8 * e);
+    }
     return x;
+  }
+  // a bit for each of the 32 positions from base on; raw: peek() of base + 8 g + 4 (lane / 32)
+  __device__ uint32_t bits(int base, const uint32_t (&raw)[4]) const {
+    uint32_t seen = 0;
+    if (mask) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const uint32_t x = (((raw[g] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | raw[g]) >> 7 & 0x01010101u;
+        seen |= (x * 0x01020408u >> 24 & 0xfu) << (8 * g + 4 * (__lane_id() >> 5));
+      }
+      seen |= half_partner(seen);
+    } else {
+      seen = 0xffffffffu;
+    }
+    const int n = last - base + 1;
+    return n >= 32 ? seen : n <= 0 ? 0u : seen & ((1u << n) - 1u);
   }
 };
 
-// Which part, key head and row block a work-group takes.  Consecutive work-groups go to the eight XCDs
-// in turn: each takes a run of items, the row blocks of one part and key head next to each other, which
-// then share their keys in its L2.  (Under causal the last row blocks, which see the most, go first.)
-__device__ inline bool ca_item(const CacheArgs& A, int& part, int& kh, int& tile) {
-  const int per = (A.items + 7) / 8, id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-  if (id >= min(A.items, ((int)(blockIdx.x & 7) + 1) * per)) return false;
-  tile = id % A.tiles;
-  if (A.causal) tile = A.tiles - 1 - tile;
-  part = id / A.tiles % A.S, kh = id / A.tiles / A.S;
+// Which key head, sequence, part and row block a work-group takes.  Those that there are (row blocks
+// times parts of every sequence, which the lanes count) come without gaps, so that the launch's spare
+// work-groups are its last: dealt among the others, they left CUs without work while others had two.
+// Consecutive work-groups go to the eight XCDs in turn: each takes a run of items, the row blocks of
+// one part and key head next to each other, which then share their keys in its L2.  (Under causal the
+// last row blocks, which see the most, go first.)
+template <int ROWS>
+__device__ inline bool ca_item(const CacheArgs& A, int& part, int& parts, int& kh, CacheRows& w) {
+  const int lane = __lane_id();
+  auto blocks = [&](const CacheRows& x) { return (x.rows + ROWS - 1) / ROWS; };
+  auto items = [&](int b) {
+    if (b >= A.B) return 0;
+    CacheRows x;
+    ca_sequence(A, b, x);
+    return blocks(x) * ca_parts(A, x.L);
+  };
+  const bool alike = !A.offsets && A.S == 1;
+  long long each = 0;  // items of a key head
+  if (alike)
+    each = (long long)A.B * (((long long)A.N * A.G + ROWS - 1) / ROWS);
+  else
+    for (int b0 = 0; b0 < A.B; b0 += 64) each += wave_sum(items(b0 + lane));
+  const int all = (int)(each * A.HK), per = (all + 7) / 8, in = (int)(blockIdx.x >> 3);
+  const int id = (int)(blockIdx.x & 7) * per + in;
+  if (in >= per || id >= all) return false;
+  kh = id / (int)each;
+  int local = id - kh * (int)each, b = 0;
+  if (alike) {
+    const int n = (int)each / A.B;
+    b = local / n, local -= b * n;
+  } else {
+    for (int b0 = 0; b0 < A.B; b0 += 64) {
+      const int n = items(b0 + lane), end = wave_incl_scan(n), sum = __builtin_amdgcn_readlane(end, 63);
+      if (local < sum) {  // (the same for the wave)
+        const int at = __ffsll((unsigned long long)__ballot(end > local)) - 1;
+        b = b0 + at;
+        local -= __builtin_amdgcn_readlane(end, at) - __builtin_amdgcn_readlane(n, at);
+        break;
+      }
+      local -= sum;
+    }
+  }
+  ca_sequence(A, b, w);
+  const int n = blocks(w), tile = local % n;
+  part = local / n, parts = ca_parts(A, w.L);
+  w.r0 = (A.causal ? n - 1 - tile : tile) * ROWS;
   return true;
 }
 
@@ -277,12 +331,9 @@ __global__ __launch_bounds__(128, 1) void ca_few_kernel(CacheArgs A) {
   __shared__ float sM[WAVES][32], sL[WAVES][32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int jl = lane & 31, hh = lane >> 5;
-  int part, kh, tile;
-  if (!ca_item(A, part, kh, tile)) return;
+  int part, parts, kh;
   CacheRows w;
-  if (!ca_rows<32>(A, tile, w)) return;
-  const int parts = ca_parts(A, w.L);
-  if (part >= parts) return;
+  if (!ca_item<32>(A, part, parts, kh, w)) return;
   const int r = min(w.r0 + jl, w.rows - 1), tok = r / A.G, head = kh * A.G + r - tok * A.G;
   CacheSight sight{A.mask ? A.mask + (A.offsets ? (w.row0 + tok) * A.mask_row : w.b * A.mask_batch + tok * A.mask_row)
                           : nullptr,
@@ -324,16 +375,15 @@ __global__ __launch_bounds__(128, 1) void ca_few_kernel(CacheArgs A) {
     for (int i = 0; i < D / 16; ++i)
       s[0] = Mfma<T>::run(*(const u32x4*)(sk + jl * D + 8 * ((2 * i + hh) ^ ca_kswz<D>(jl))), st.q[i], s[0]);
     const bool hide = 32 * t + 32 > (masked ? w.first : w.L) || bad;  // (of the wave)
-    uint32_t seen = 0;  // by the lane's row, of all 32 keys
+    uint32_t seen = 0;  // by the lane's row
     if (hide) {
+      uint32_t raw[4];
 #pragma unroll
-      for (int a = 0; a < 16; ++a) {
-        const int j = 8 * (a / 4) + 4 * hh + a % 4;
-        const bool see = sight.sees(32 * t + j) && !(bad >> j & 1);
-        seen |= (uint32_t)see << j;
-        if (!see) s[0][a] = -__builtin_inff();
-      }
-      seen |= half_partner(seen);
+      for (int g = 0; g < 4; ++g) raw[g] = A.mask ? sight.peek(32 * t + 8 * g + 4 * hh) : 0u;
+      seen = sight.bits(32 * t, raw) & ~(uint32_t)bad;
+#pragma unroll
+      for (int a = 0; a < 16; ++a)
+        if (!(seen >> (8 * (a / 4) + 4 * hh + a % 4) & 1)) s[0][a] = -__builtin_inff();
     }
     u32x4 p[2];
     ca_weights<T, D, 1>(st, s, p, A.c);
@@ -430,8 +480,8 @@ __global__ __launch_bounds__(128, 1) void ca_few_kernel(CacheArgs A) {
   }
 }
 
-// The products of the pipeline below, with the sums in accumulation registers and the queries where
-// there is room (the compiler's choice moved them back and forth).  Two wait states come before each:
+// The products of the pipeline below, with the sums and the queries in accumulation registers (the
+// compiler's choice moved them back and forth).  Two wait states come before each:
 // the compiler may have moved an operand just before, and does not know what this is.  Who reads a
 // result waits, or comes two products later.
 #define CA_MFMA(dst, c, dst_, q_)                                                                       \
@@ -442,12 +492,10 @@ __global__ __launch_bounds__(128, 1) void ca_few_kernel(CacheArgs A) {
 template <typename T> __device__ inline void ca_mfma_sum(f32x16& c, const u32x4& a, const u32x4& b) {
   CA_MFMA(c, "%0", "+a", "v");
 }
-template <typename T, int D, bool FIRST>
+template <typename T, bool FIRST>
 __device__ inline void ca_mfma_score(f32x16& c, const u32x4& a, const u32x4& b) {
-  if constexpr (FIRST && D == 128) { CA_MFMA(c, "0", "=&v", "a"); }
-  else if constexpr (D == 128) { CA_MFMA(c, "%0", "+v", "a"); }
-  else if constexpr (FIRST) { CA_MFMA(c, "0", "=&v", "v"); }
-  else { CA_MFMA(c, "%0", "+v", "v"); }
+  if constexpr (FIRST) { CA_MFMA(c, "0", "=&v", "a"); }
+  else { CA_MFMA(c, "%0", "+v", "a"); }
 }
 #undef CA_MFMA
 
@@ -463,23 +511,30 @@ __global__ __launch_bounds__(64 * W, 2) void ca_many_kernel(CacheArgs A) {
   constexpr int ROWS = 32 * W, LPR = D / 8, RPI = 64 / LPR, NB = D / 32, NS = D / 16;
   constexpr int KW = 64 / W, IPW = KW / RPI;  // keys of a tile that a wave fetches, in so many instructions
   static_assert(IPW >= 1, "whole instructions");
-  __shared__ __attribute__((aligned(1024))) uint16_t sK0[64 * D], sK1[64 * D], sV0[64 * D], sV1[64 * D];
+  constexpr int NBUF = 2;  // tiles that are kept (three gained nothing)
+  __shared__ __attribute__((aligned(1024))) uint16_t sK[NBUF * 64 * D], sV[NBUF * 64 * D];
   __shared__ uint32_t sBad[2][W];  // a wave's keys whose table entry lies outside the cache
+  __shared__ uint32_t sOdd[2][W];  // whether its values hold an inf or NaN
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int jl = lane & 31, hh = lane >> 5;
-  int part, kh, tile;
-  if (!ca_item(A, part, kh, tile)) return;
+  int part, parts, kh;
   CacheRows w;
-  if (!ca_rows<ROWS>(A, tile, w)) return;
-  const int parts = ca_parts(A, w.L);
-  if (part >= parts) return;
+  if (!ca_item<ROWS>(A, part, parts, kh, w)) return;
   const int wr0 = w.r0 + 32 * wave;  // the wave's first row
   const bool live = wr0 < w.rows;    // (of the wave)
-  const int r = min(wr0 + jl, w.rows - 1), tok = r / A.G, head = kh * A.G + r - tok * A.G;
   u32x4 q[NS];
   f32x16 o[NB];
   float m = CA_NONE, l = 0.f;
+  // the lane's row (looked up again after the pipeline, which has no registers to spare)
+  auto row_of = [&](int& tok, int& head) {
+    int x = wr0 + jl;
+    asm volatile("" : "+v"(x));
+    x = min(x, w.rows - 1);
+    tok = x / A.G, head = kh * A.G + x - tok * A.G;
+  };
   {
+    int tok, head;
+    row_of(tok, head);
     const char* qr = ca_token(A.q, A, w, A.q_batch, A.q_row, tok) + head * A.q_head + 16 * hh;
 #pragma unroll
     for (int s = 0; s < NS; ++s) q[s] = *(const u32x4*)(qr + 32 * s);
@@ -535,8 +590,19 @@ __global__ __launch_bounds__(64 * W, 2) void ca_many_kernel(CacheArgs A) {
     for (int i = 0; i < IPW; ++i) one(base, to, off, i, KEYS);
   };
   // where the lane's operands lie (halves): K of step s, V of dim block nb
-  auto kat = [&](int s) { return jl * D + 8 * ((2 * s + hh) ^ ca_kswz<D>(jl)); };
-  auto vat = [&](int nb) { return ca_trat<D>(lane, nb); };
+  int ka[NS], va[NB];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    ka[s] = jl * D + 8 * ((2 * s + hh) ^ ca_kswz<D>(jl));
+    asm volatile("" : "+v"(ka[s]));  // (one register each: not put together again at every read)
+  }
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    va[nb] = ca_trat<D>(lane, nb);
+    asm volatile("" : "+v"(va[nb]));
+  }
+  auto kat = [&](int s) { return ka[s]; };
+  auto vat = [&](int nb) { return va[nb]; };
   // weight pair i of 8: elements 2 i, + 1
   auto weigh = [&](int i, const f32x16& S, u32x4 (&P)[2], float& lt) __attribute__((always_inline)) {
     const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[2 * i], A.c, -m));
@@ -623,8 +689,8 @@ __global__ __launch_bounds__(64 * W, 2) void ca_many_kernel(CacheArgs A) {
       rdv(i + AHEAD < STEPS ? vt : vn, (i + AHEAD) % STEPS);
       extra(i);
       __builtin_amdgcn_sched_barrier(0);
-      if (i == 0) ca_mfma_score<T, D, true>(SX, kf[0], q[0]);
-      else ca_mfma_score<T, D, false>(SX, kf[i % (AHEAD + 1)], q[i]);
+      if (i == 0) ca_mfma_score<T, true>(SX, kf[0], q[0]);
+      else ca_mfma_score<T, false>(SX, kf[i % (AHEAD + 1)], q[i]);
       __builtin_amdgcn_sched_barrier(0);
       slot(2 * i);
       const u32x2 f0 = vf[i % (AHEAD + 1)][0], f1 = vf[i % (AHEAD + 1)][1];
@@ -642,46 +708,67 @@ __global__ __launch_bounds__(64 * W, 2) void ca_many_kernel(CacheArgs A) {
     u32x4 p0[2], p1[2];
     // (tiles past the last of the pipeline are fetched like it, and not used)
     auto last = [&](int t) { return min(t, nf - 1); };
-    auto look = [&](int t) { return ca_entry(A, table, P16 ? 64 * (t0 + last(t)) + KW * wave : pos_of(last(t))); };
-    auto find = [&](int t, uint32_t entry) {
+#pragma unroll
+    for (int s = 0; s < NS; ++s) asm volatile("" : "+a"(q[s]));
+    // where the wave's keys of a tile lie.  P16: its entry is a lane's of `entries`, those of tiles t0 +
+    // 64 i + lane, which are loaded once in 64 tiles
+    int first = 0;
+    uint32_t entries = 0;
+    auto look = [&](int t) {
+      first = t;
+      entries = ca_entry(A, table, 64 * (t0 + last(t + lane)) + KW * wave);
+      asm volatile("" : "+v"(entries));  // (waited for here, not wherever it may be needed)
+    };
+    auto find = [&](int t) {
       if constexpr (P16) {
+        if (t >= first + 64) look(t);
+        const uint32_t entry = __builtin_amdgcn_readlane(entries, t - first);
         const int pos = 64 * (t0 + last(t)) + KW * wave;
-        entry = __builtin_amdgcn_readfirstlane(entry);
         return (long long)entry * A.kv_page + (A.shift >= 0 ? pos & (A.page - 1) : pos % A.page) * A.kv_row;
       } else {
         bool ok;
-        return ca_offset(A, entry, pos_of(last(t)), ok);
+        const int pos = pos_of(last(t));
+        return ca_offset(A, ca_entry(A, table, pos), pos, ok);
       }
     };
-    // where tiles t + 1 and t + 2 lie; the table's entry of tile t + 3
-    auto off0 = find(0, look(0)), off1 = find(1, look(1)), off2 = find(2, look(2));
-    uint32_t entry = look(3);
-    whole(kbase, sK0, off0, Yes{});
-    // before the first half tile: values and weights of zero
-    for (int i = threadIdx.x; i < 8 * D; i += 64 * W) *(u32x4*)(sV1 + 8 * i) = u32x4{0u, 0u, 0u, 0u};
-    p1[0] = p1[1] = u32x4{0u, 0u, 0u, 0u};
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    whole(kbase, sK1, off1, Yes{});
-    whole(vbase, sV0, off0, No{});
-    if (live) {
-      scores(s0, sK0);
+    if constexpr (P16) look(0);
+    // K of tile s + NBUF and V of tile s + NBUF - 1, the ones that round s asks for; offv: where the
+    // latter lies
+    auto offv = find(0), offk = offv;
+    whole(kbase, sK, offk, Yes{});
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) rdk(sK0 + 32 * D, i), rdv(sV1 + 32 * D, i);
+    for (int s = 1 - NBUF; s < 0; ++s) {
+      offk = find(s + NBUF);
+      whole(kbase, sK + (s + NBUF) * 64 * D, offk, Yes{});
+      whole(vbase, sV + (s + NBUF - 1) * 64 * D, offv, No{});
+      offv = offk;
     }
-    // every wave's reads of the tiles before are done, and the loads that have been asked for are there
+    // before the first half tile: values and weights of zero
+    for (int i = threadIdx.x; i < 8 * D; i += 64 * W) *(u32x4*)(sV + (NBUF - 1) * 64 * D + 8 * i) = u32x4{0u, 0u, 0u, 0u};
+    p1[0] = p1[1] = u32x4{0u, 0u, 0u, 0u};
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NBUF - 1) * 2 * IPW) : "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the zeros
+    __builtin_amdgcn_s_barrier();
+    if (live) {
+      scores(s0, sK);
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) rdk(sK + 32 * D, i), rdv(sV + (NBUF - 1) * 64 * D + 32 * D, i);
+    }
+    // every wave's reads of the tiles before are done, and the loads that have to be there are
     auto meet = [&]() __attribute__((always_inline)) {
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NBUF - 2) * 2 * IPW) : "memory");
     };
     auto nothing = [&](int) __attribute__((always_inline)) {};
     auto none = [&]() __attribute__((always_inline)) {};
-    // tile t, whose first half's scores are there; K of t + 1 and V of t have been asked for
-    auto round = [&](int t, uint16_t* kt, uint16_t* kx, uint16_t* vt, uint16_t* vw) __attribute__((always_inline)) {
+    // tile t, in buffer B, whose first half's scores are there
+    auto round = [&](int t, auto BUF) __attribute__((always_inline)) {
+      constexpr int B = decltype(BUF)::value, BX = (B + 1) % NBUF, BW = (B + NBUF - 1) % NBUF;
+      uint16_t *kt = sK + B * 64 * D, *kx = sK + BX * 64 * D, *vt = sV + B * 64 * D, *vw = sV + BW * 64 * D;
+      offk = find(t + NBUF);
       if (live) turn(s0, s1, p0, p1, kt + 32 * D, vw + 32 * D, kx, vt, meet, nothing);
       else meet();
-      const auto off3 = find(t + 3, entry);  // (here, where no load is under way)
       auto ask = [&](int i) __attribute__((always_inline)) {
-        if (i < IPW) one(kbase, kt, off2, i, Yes{}), one(vbase, vw, off1, i, No{});
+        if (i < IPW) one(kbase, kt, offk, i, Yes{}), one(vbase, vw, offv, i, No{});
       };
       if (live) {
         turn(s1, s0, p1, p0, kx, vt, kx + 32 * D, vt + 32 * D, none, ask);
@@ -689,16 +776,17 @@ __global__ __launch_bounds__(64 * W, 2) void ca_many_kernel(CacheArgs A) {
 #pragma unroll
         for (int i = 0; i < IPW; ++i) ask(i);
       }
-      entry = look(t + 4);
-      off1 = off2, off2 = off3;
+      offv = offk;
     };
+    using B0 = std::integral_constant<int, 0>;
+    using B1 = std::integral_constant<int, 1>;
     for (int t = 0; t < nf; t += 2) {
-      round(t, sK0, sK1, sV0, sV1);
-      if (t + 1 < nf) round(t + 1, sK1, sK0, sV1, sV0);
+      round(t, B0{});
+      if (t + 1 < nf) round(t + 1, B1{});
     }
     // the last half tile's sums
     if (live) {
-      const uint16_t* vt = (nf & 1 ? sV0 : sV1) + 32 * D;
+      const uint16_t* vt = sV + ((nf - 1) % NBUF * 64 + 32) * D;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -715,33 +803,31 @@ __global__ __launch_bounds__(64 * W, 2) void ca_many_kernel(CacheArgs A) {
 
   // ---- tiles with hidden keys: those of a row are not seen, and an inf or NaN among their values
   // (left out of the products, where a weight of 0 would make it NaN) goes to the rows that see it
+  int tok, head;
+  row_of(tok, head);
   if (nf < nt) {
     const CacheSight sight{
         A.mask ? A.mask + (A.offsets ? (w.row0 + tok) * A.mask_row : w.b * A.mask_batch + tok * A.mask_row) : nullptr,
         w.first, A.causal ? w.first + tok : w.L - 1, A.mask_cols};
-    auto ask = [&](int t, uint16_t* kt, uint16_t* vt) __attribute__((always_inline)) {
+    auto at = [&](uint16_t* x, int t) { return x + (t & 1) * 64 * D; };
+    uint32_t raw[2][4] = {};
+    auto ask = [&](int t) __attribute__((always_inline)) {
       bool ok;
       const uint32_t off = ca_offset(A, ca_entry(A, table, pos_of(t)), pos_of(t), ok);
       const uint64_t bad = __ballot(!ok);
       if (lane == 0) sBad[t & 1][wave] = (uint32_t)bad & ((1u << KW) - 1u);
-      whole(kbase, kt, off, Yes{});
-      whole(vbase, vt, off, No{});
+      whole(kbase, at(sK, t), off, Yes{});
+      whole(vbase, at(sV, t), off, No{});
+      if (A.mask)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) raw[kb][g] = sight.peek(64 * (t0 + t) + 32 * kb + 8 * g + 4 * hh);
     };
-    auto hidden = [&](int t, int kb, const uint16_t* kt, const uint16_t* vt) __attribute__((always_inline)) {
-      const int base = 64 * (t0 + t) + 32 * kb;
+    auto hidden = [&](uint32_t seen, bool odd, const uint16_t* kt, const uint16_t* vt) __attribute__((always_inline)) {
       f32x16 S;
       u32x4 P[2];
       scores(S, kt);
-      uint32_t seen = 0, bad = 0;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int j = 8 * g + 4 * hh;
-        seen |= sight.sees4(base + j) << j;
-      }
-      seen |= half_partner(seen);
-#pragma unroll
-      for (int x = 0; x < W / 2; ++x) bad |= sBad[t & 1][W / 2 * kb + x] << (KW * x);
-      seen &= ~bad;
 #pragma unroll
       for (int a = 0; a < 16; ++a)
         if (!(seen >> (8 * (a / 4) + 4 * hh + a % 4) & 1)) S[a] = -__builtin_inff();
@@ -749,17 +835,16 @@ __global__ __launch_bounds__(64 * W, 2) void ca_many_kernel(CacheArgs A) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) weigh(i, S, P, lt);
       settle(S, P, lt);
-      bool odd = false;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int mm = 0; mm < 2; ++mm) {
-          const uint16_t* at = vt + vat(nb) + 16 * mm * D;
-          u32x2 f[2] = {ca_trread(at), ca_trread(at + 8 * D)};
-          odd |= ca_clean<T>(f);
+          const uint16_t* x = vt + vat(nb) + 16 * mm * D;
+          u32x2 f[2] = {ca_trread(x), ca_trread(x + 8 * D)};
+          if (odd) ca_clean<T>(f);
           o[nb] = Mfma<T>::run(u32x4{f[0][0], f[0][1], f[1][0], f[1][1]}, P[mm], o[nb]);
         }
-      if (__ballot(odd)) {
+      if (odd) {
         for (int j = 0; j < 32; ++j)
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb)
@@ -771,15 +856,31 @@ __global__ __launch_bounds__(64 * W, 2) void ca_many_kernel(CacheArgs A) {
             }
       }
     };
-    ask(nf, (nf & 1) ? sK1 : sK0, (nf & 1) ? sV1 : sV0);
+    ask(nf);
     for (int t = nf; t < nt; ++t) {
+      uint32_t seen[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) seen[kb] = sight.bits(64 * (t0 + t) + 32 * kb, raw[kb]);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      {  // (this wave's own keys have landed)
+        u32x2 v[KW * D / 256];
+#pragma unroll
+        for (int i = 0; i < KW * D / 256; ++i) v[i] = *(const u32x2*)(at(sV, t) + KW * wave * D + 256 * i + 4 * lane);
+        const uint64_t any = __ballot(ca_clean<T>(v));
+        if (lane == 0) sOdd[t & 1][wave] = any != 0;
+      }
       __syncthreads();
-      if (t + 1 < nt) ask(t + 1, (t & 1) ? sK0 : sK1, (t & 1) ? sV0 : sV1);
+      uint32_t bad[2] = {0, 0}, odd = 0;
+#pragma unroll
+      for (int x = 0; x < W; ++x) bad[x / (W / 2)] |= sBad[t & 1][x] << (KW * (x % (W / 2))), odd |= sOdd[t & 1][x];
+      if (t + 1 < nt) ask(t + 1);
       if (live)
 #pragma clang loop unroll(disable)
-        for (int kb = 0; kb < 2; ++kb)
-          hidden(t, kb, ((t & 1) ? sK1 : sK0) + 32 * kb * D, ((t & 1) ? sV1 : sV0) + 32 * kb * D);
+        for (int kb = 0; kb < 2; ++kb) {
+          const uint32_t see = (kb ? seen[1] : seen[0]) & ~(kb ? bad[1] : bad[0]);
+          if (__ballot(see != 0))
+            hidden(see, __builtin_amdgcn_readfirstlane(odd), at(sK, t) + 32 * kb * D, at(sV, t) + 32 * kb * D);
+        }
     }
   }
   if (!live) return;
@@ -945,14 +1046,14 @@ extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, 
     t2t_set_error("cache_attention: %lld row blocks of %d heads", tiles, a->HK);
     return T2T_ERR_UNSUPPORTED;
   }
-  A.tiles = (int)tiles, A.items = (int)(tiles * a->HK * A.S);
+  const int items = (int)(tiles * a->HK * A.S);
   // sixteen keys from a multiple of sixteen on lie in one page, at 32-bit offsets
   const bool p16 = a->page_size % 16 == 0 && A.kv_row < (1 << 27);
   auto run = [&](auto t, auto d) {
     using TT = decltype(t);
     constexpr int D = decltype(d)::value;
     auto go = [&](auto kernel, int threads, auto join) {
-      hipLaunchKernelGGL(kernel, dim3((A.items + 7) / 8 * 8), dim3(threads), 0, (hipStream_t)stream, A);
+      hipLaunchKernelGGL(kernel, dim3((items + 7) / 8 * 8), dim3(threads), 0, (hipStream_t)stream, A);
       if (A.S > 1)
         hipLaunchKernelGGL(join, dim3((unsigned)(tiles * a->HK), block / 8), dim3(256), 0, (hipStream_t)stream, A);
     };

@@ -121,20 +121,23 @@ __device__ inline uint32_t i8_top(uint32_t top, const u32x4& v) {  // both halve
 }
 
 // TPR threads a row, which stays in registers between its maximum and its codes:
-// one read of x, one write of the codes.
-template <typename T, int TPR, int I>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void i8_quantize_kernel(
+// one read of x, one write of the codes.  A work-group has several rows where it can:
+// a row writes half lines (64 bytes of every block), its neighbour the other halves
+// (75,600 x 5,120: XX us with four rows, 239 with one).
+template <typename T, int TPR, int I, int ROWS>
+__global__ __launch_bounds__(TPR * ROWS) void i8_quantize_kernel(
     const uint16_t* __restrict__ x, long long row_stride, char* __restrict__ codes, float* __restrict__ scales, int M,
     int K, int Kp) {
-  constexpr int ROWS = TPR < 256 ? 256 / TPR : 1;
   __shared__ uint32_t tops[16];
   const int t = threadIdx.x % TPR;
-  for (long long row = (long long)blockIdx.x * ROWS + threadIdx.x / TPR; row < M; row += (long long)gridDim.x * ROWS) {
+  for (long long row0 = (long long)blockIdx.x * ROWS; row0 < M; row0 += (long long)gridDim.x * ROWS) {
+    const long long row = row0 + threadIdx.x / TPR;
+    if (TPR == 64 && row >= M) return;
     const uint16_t* src = x + row * row_stride;
     u32x4 v[I];
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < I; ++i) v[i] = i8_load(src + 8 * (t + i * TPR), K - 8 * (t + i * TPR));
+    for (int i = 0; i < I; ++i) v[i] = i8_load(src + 8 * (t + i * TPR), row < M ? K - 8 * (t + i * TPR) : 0);
 #pragma unroll
     for (int i = 0; i < I; ++i) top = i8_top(top, v[i]);
     top = max(top & 0xffffu, top >> 16);
@@ -145,16 +148,16 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void i8_quantize_kernel(
       if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < TPR / 64; ++w) top = max(top, tops[w]);
+      for (int w = 0; w < TPR / 64; ++w) top = max(top, tops[threadIdx.x / TPR * (TPR / 64) + w]);
     }
     const bool bad = top >= I8Inf<T>::bits;
     const I8Scale k = i8_scale(T::to_f((uint16_t)top));
 #pragma unroll
     for (int i = 0; i < I; ++i) {
       const int c = 8 * (t + i * TPR);
-      if (c < Kp) *(u32x2*)(codes + i8_at(row, c, 16LL * Kp)) = bad ? u32x2{0u, 0u} : i8_codes<T>(v[i], k);
+      if (c < Kp && row < M) *(u32x2*)(codes + i8_at(row, c, 16LL * Kp)) = bad ? u32x2{0u, 0u} : i8_codes<T>(v[i], k);
     }
-    if (t == 0) scales[row] = bad ? __builtin_nanf("") : k.s;
+    if (t == 0 && row < M) scales[row] = bad ? __builtin_nanf("") : k.s;
   }
 }
 
@@ -162,22 +165,27 @@ template <typename T>
 static void i8_quantize_launch(const uint16_t* x, long long row_stride, char* codes, float* scales, int M, int K,
                                hipStream_t st) {
   const int Kp = i8_kp(K);
-  auto go = [&](auto tpr, auto its) {
-    constexpr int TPR = decltype(tpr)::value, I = decltype(its)::value, ROWS = TPR < 256 ? 256 / TPR : 1;
+  auto go = [&](auto tpr, auto its, auto rows) {
+    constexpr int TPR = decltype(tpr)::value, I = decltype(its)::value, ROWS = decltype(rows)::value;
     const int wgs = cdiv(M, ROWS);
-    hipLaunchKernelGGL((i8_quantize_kernel<T, TPR, I>), dim3(wgs < (1 << 20) ? wgs : 1 << 20),
-                       dim3(TPR < 256 ? 256 : TPR), 0, st, x, row_stride, codes, scales, M, K, Kp);
+    hipLaunchKernelGGL((i8_quantize_kernel<T, TPR, I, ROWS>), dim3(wgs < (1 << 20) ? wgs : 1 << 20), dim3(TPR * ROWS),
+                       0, st, x, row_stride, codes, scales, M, K, Kp);
   };
-#define I8_GO(TPR, I) go(std::integral_constant<int, TPR>{}, std::integral_constant<int, I>{})
-  if (Kp <= 512) I8_GO(64, 1);
-  else if (Kp <= 1024) I8_GO(64, 2);
-  else if (Kp <= 2048) I8_GO(64, 4);
-  else if (Kp <= 4096) I8_GO(256, 2);
-  else if (Kp <= 6144) I8_GO(256, 3);
-  else if (Kp <= 8192) I8_GO(256, 4);
-  else if (Kp <= 16384) I8_GO(256, 8);
-  else if (Kp <= 32768) I8_GO(1024, 4);
-  else I8_GO(1024, 16);
+#define I8_GO(TPR, I, ROWS) \
+  go(std::integral_constant<int, TPR>{}, std::integral_constant<int, I>{}, std::integral_constant<int, ROWS>{})
+  const bool many = M >= 1024;  // else more threads take a row (1 x 5,120: 2.5 us)
+  if (Kp <= 512) I8_GO(64, 1, 4);
+  else if (Kp <= 1024) I8_GO(64, 2, 4);
+  else if (Kp <= 1536 && many) I8_GO(64, 3, 4);
+  else if (Kp <= 2048) I8_GO(64, 4, 4);
+  else if (Kp <= 3584 && many) I8_GO(64, 7, 4);
+  else if (Kp <= 5120 && many) I8_GO(64, 10, 4);
+  else if (Kp <= 4096) I8_GO(256, 2, 1);
+  else if (Kp <= 6144) I8_GO(256, 3, 2);
+  else if (Kp <= 8192) I8_GO(256, 4, 2);
+  else if (Kp <= 14336) I8_GO(256, 7, 2);
+  else if (Kp <= 32768) I8_GO(1024, 4, 1);
+  else I8_GO(1024, 16, 1);
 #undef I8_GO
 }
 
@@ -195,17 +203,22 @@ extern "C" int t2t_int8_quantize(const void* x, int dtype, long long row_stride,
 }
 
 // ---------------------------------------------------------------------------
-// the values back: eight a thread.  Bound: writing them.
+// the values back: eight a thread, the codes read in order, so that a row of a
+// block is stored whole (128 bytes).  Bound: writing them.
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(256) void i8_dequantize_kernel(const char* __restrict__ codes, long long blk,
                                                             const float* __restrict__ scales,
                                                             uint16_t* __restrict__ out, long long row_stride,
-                                                            long long units, int per_row, int K) {
+                                                            long long units, int M, int K) {
+  const int per = (int)(blk >> 3);  // units of 16 rows
   for (long long u = (long long)blockIdx.x * 256 + threadIdx.x; u < units; u += (long long)gridDim.x * 256) {
-    const long long row = u / per_row;
-    const int c = 8 * (int)(u - row * per_row);
-    const u32x2 v = *(const u32x2*)(codes + i8_at(row, c, blk));
+    const long long rb = u / per;
+    const int in = (int)(u - rb * per), r = in >> 3 & 15;
+    const int c = 64 * (in >> 7) + 16 * ((in >> 1 & 3) ^ i8_swz(r)) + 8 * (in & 1);
+    const long long row = 16 * rb + r;
+    if (row >= M || c >= K) continue;
+    const u32x2 v = *(const u32x2*)(codes + 8 * u);
     const float s = scales[row];
     float f[8];
 #pragma unroll
@@ -223,12 +236,11 @@ extern "C" int t2t_int8_dequantize(const void* codes, const float* scales, void*
   rc = i8_check_rows("int8_dequantize", out, dtype, row_stride, M, K);
   if (rc == T2T_OK) rc = i8_check_matrix("int8_dequantize", codes, scales);
   if (rc != T2T_OK) return rc;
-  const int per_row = (K + 7) / 8;
-  const long long units = (long long)M * per_row, wgs = (units + 255) / 256;
+  const long long units = (long long)(t2t_int8_code_bytes(M, K) / 8), wgs = (units + 255) / 256;
   const dim3 grid((unsigned)(wgs < (1 << 20) ? wgs : 1 << 20));
   auto kernel = dtype == T2T_BF16 ? i8_dequantize_kernel<BF16T> : i8_dequantize_kernel<F16T>;
   hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, (const char*)codes, 16LL * i8_kp(K), scales,
-                     (uint16_t*)out, row_stride, units, per_row, K);
+                     (uint16_t*)out, row_stride, units, M, K);
   T2T_LAUNCH_CHECK("int8_dequantize");
   return T2T_OK;
 }
