@@ -282,7 +282,19 @@ def test_a_copied_cache_is_read_at_its_own_address(launches):
     assert c.k.data_ptr() != a["cache"].k.data_ptr()
     ops.cache_append(**{**a, "cache": c})
     (_, _, args), = launches
-    assert args[1].out == c.k.data_ptr() and args[2].out == c.v.data_ptr()
+    from token2tile_amd import _lib
+    k, v = (_lib.RotaryTensor.from_buffer_copy(x) for x in args[1:3])
+    assert k.out == c.k.data_ptr() and v.out == c.v.data_ptr()
+
+
+def test_arguments_as_bytes_are_the_structs():
+    from token2tile_amd import _lib
+    for packer, struct in ((_lib.ROTARY_TENSOR, _lib.RotaryTensor),
+                           (_lib.CACHE_ATTENTION_ARGS, _lib.CacheAttentionArgs)):
+        names = [n for n, _ in struct._fields_]
+        values = list(range(1, len(names) + 1))
+        a = struct.from_buffer_copy(packer.pack(*values))
+        assert packer.size == ctypes.sizeof(struct) and [getattr(a, n) for n in names] == values
 
 
 # ---------------------------------------------------------------------------

@@ -211,6 +211,7 @@ __device__ inline bool ca_item(const CacheArgs& A, int& part, int& parts, int& k
     each = (long long)A.B * (((long long)A.N * A.G + ROWS - 1) / ROWS);
   else
     for (int b0 = 0; b0 < A.B; b0 += 64) each += wave_sum(items(b0 + lane));
+  if (each * A.HK > gridDim.x) return false;  // (offsets that go back, whose sequences overlap)
   const int all = (int)(each * A.HK), per = (all + 7) / 8, in = (int)(blockIdx.x >> 3);
   const int id = (int)(blockIdx.x & 7) * per + in;
   if (in >= per || id >= all) return false;

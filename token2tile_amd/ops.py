@@ -8,6 +8,7 @@ library and CUDA (ROCm) tensors.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from contextlib import nullcontext
 from dataclasses import dataclass
@@ -715,6 +716,7 @@ def fit_chol(Mq, Mk, floor, small, stream=None):
 # (single-token calls are bound by the host: checks are written for few
 # operations, and a matrix in MXFP4 is checked once, when it is made)
 _functions = {}
+_sizes_of = functools.lru_cache(1024)(size_query)  # (of sizes alone)
 
 
 def _launch(name, dev, stream, tensors, *args):
@@ -1009,9 +1011,9 @@ def _rotary_arg(x, out, weight, norm, name, dev, stream, B, N, D, dtype):
             _check(weight, wshape, dtype, f"{name}_weight", dev)
     elif weight is not None:
         raise ValueError(f"t2t: {name}_weight without a norm")
-    return out, _lib.RotaryTensor(x.data_ptr(), xs[0] if nd == 4 else 0, xs[-3], xs[-2], out.data_ptr(),
-                                  os[0] if nd == 4 else 0, os[-3], os[-2],
-                                  None if weight is None else weight.data_ptr(), H)
+    return out, _lib.ROTARY_TENSOR.pack(x.data_ptr(), xs[0] if nd == 4 else 0, xs[-3], xs[-2], out.data_ptr(),
+                                        os[0] if nd == 4 else 0, os[-3], os[-2],
+                                        0 if weight is None else weight.data_ptr(), H)
 
 
 def rotary(q, k, cos, sin, *, layout="interleaved", inverse=False, norm=None, q_weight=None,
@@ -1382,7 +1384,7 @@ def int8_dequantize(t, dtype=torch.bfloat16, out=None, stream=None):
 def int8_linear_ws_bytes(M, N, K):
     """Workspace of int8_linear for a 16-bit x of M rows (0 where the product
     quantises them itself)."""
-    return size_query("t2t_int8_linear_ws_bytes", M, N, K)
+    return _sizes_of("t2t_int8_linear_ws_bytes", M, N, K)
 
 
 def int8_linear(x, weight, bias=None, *, activation=None, dtype=None, out=None, ws=None, stream=None):
@@ -1462,7 +1464,7 @@ class PagedCache:
     contiguous channels; both may be views of one tensor), 16-byte aligned.  Slot
     page * page_size + i is row i of a page.  They are checked here, once."""
 
-    __slots__ = ("_k", "_v")
+    __slots__ = ("_k", "_v", "_strides", "_bytes")
 
     def __init__(self, k, v):
         dev = _dev(k)
@@ -1483,7 +1485,7 @@ class PagedCache:
         if not (_scattered(k) and _scattered(v)) or _near(*_span(k), ((_span(v)[0], _span(v)[1] - _span(v)[0]),)) \
                 and (_same_view(k, v) or _meet(k, v)):
             raise ValueError("t2t: the cache holds an element twice")
-        self._k, self._v = k, v
+        self._k, self._v, self._strides, self._bytes = k, v, st, _span(k)[1] - _span(k)[0]
 
     k = property(lambda self: self._k)
     v = property(lambda self: self._v)
@@ -1508,6 +1510,9 @@ def _cache_of(cache):
     return k, cache._v, k.device if k.is_cuda else _dev(k)
 
 
+_SLOT_BITS = {_i32: 32, torch.int64: 64}
+
+
 def cache_append(q, k, v, cos, sin, cache, slots, *, layout="interleaved", norm=None, q_weight=None,
                  k_weight=None, eps=1e-6, out=None, stream=None):
     """New tokens' k, normed and rotated as by ``rotary``, and v into their slots of
@@ -1527,23 +1532,24 @@ def cache_append(q, k, v, cos, sin, cache, slots, *, layout="interleaved", norm=
     if not isinstance(k, torch.Tensor) or k.dim() != 3:
         raise ValueError("t2t: k must be a [T, heads, D] tensor")
     T = k.shape[0]
-    for t, name in ((k, "k"), (v, "v")):
-        if (not isinstance(t, torch.Tensor) or t.shape != (T, H, D) or t.dtype != dt or t.device != dev
-                or t.stride(2) != 1):
-            raise ValueError(f"t2t: {name} must be a {dt} [{T}, {H}, {D}] tensor on {dev} with contiguous channels")
+    shape, ks = (T, H, D), k.stride()
+    if (k.shape != shape or k.dtype != dt or k.device != dev or ks[2] != 1 or not isinstance(v, torch.Tensor)
+            or v.shape != shape or v.dtype != dt or v.device != dev or v.stride(2) != 1):
+        raise ValueError(f"t2t: k and v must be {dt} [{T}, {H}, {D}] tensors on {dev} with contiguous channels")
+    vs = v.stride()
     if layout not in _ROPE_LAYOUTS or norm not in _ROPE_NORMS:
         raise ValueError(f"t2t: layout {layout!r} (interleaved or half), norm {norm!r} (None, token or head)")
     if not (math.isfinite(eps) and eps >= 0.0):
         raise ValueError(f"t2t: eps must be at least 0, got {eps}")
-    R = 2 * cos.shape[-1] if isinstance(cos, torch.Tensor) and cos.dim() else 0
-    if not 2 <= R <= D:
-        raise ValueError(f"t2t: {R} of {D} channels rotated (2 <= R <= D)")
+    P = cos.shape[-1] if isinstance(cos, torch.Tensor) and cos.dim() else 0
+    if not 1 <= P <= D // 2:
+        raise ValueError(f"t2t: {2 * P} of {D} channels rotated (2 <= R <= D)")
     for t, name in ((cos, "cos"), (sin, "sin")):
-        if not _is(t, (T, R // 2), _f32, dev):
-            _check(t, (T, R // 2), _f32, name, dev)
+        if not _is(t, (T, P), _f32, dev):
+            _check(t, (T, P), _f32, name, dev)
     if T >= 2 ** 31:
         raise ValueError(f"t2t: {T} tokens")
-    bits = {_i32: 32, torch.int64: 64}.get(slots.dtype) if isinstance(slots, torch.Tensor) else None
+    bits = _SLOT_BITS.get(slots.dtype) if isinstance(slots, torch.Tensor) else None
     if bits is None or not _is(slots, (T,), slots.dtype, dev):
         _check(slots, (T,), (_i32, torch.int64), "slots", dev)
     if norm is not None:
@@ -1552,31 +1558,38 @@ def cache_append(q, k, v, cos, sin, cache, slots, *, layout="interleaved", norm=
             _check(k_weight, wshape, dt, "k_weight", dev)
     elif k_weight is not None:
         raise ValueError("t2t: k_weight without a norm")
-    cs = _cache_strides(ck)
-    ks, vs = k.stride(), v.stride()
-    tk = _lib.RotaryTensor(k.data_ptr(), 0, ks[0], ks[1], ck.data_ptr(), *cs,
-                           None if k_weight is None else k_weight.data_ptr(), H)
-    tv = _lib.RotaryTensor(v.data_ptr(), 0, vs[0], vs[1], cv.data_ptr(), *cs, None, H)
+    # the cache (and a caller's output) apart from everything that is read
+    pk, pv, pck, pcv, pcos, psin, ps = (k.data_ptr(), v.data_ptr(), ck.data_ptr(), cv.data_ptr(), cos.data_ptr(),
+                                        sin.data_ptr(), slots.data_ptr())
+    kn, n = (T - 1) * ks[0] + (H - 1) * ks[1] + D, 4 * T * P
+    at = [(pk, 2 * kn), (pv, 2 * ((T - 1) * vs[0] + (H - 1) * vs[1] + D)), (pcos, n), (psin, n), (ps, T * bits >> 3)]
+    pw = None
+    if k_weight is not None:
+        pw = k_weight.data_ptr()
+        at.append((pw, 2 * k_weight.shape[0]))
+    cs = cache._strides
+    pack = _lib.ROTARY_TENSOR.pack
     oq = tq = None
     if q is not None:
         if not isinstance(q, torch.Tensor) or q.dim() != 3:
             raise ValueError("t2t: q must be a [T, heads, D] tensor")
         oq, tq = _rotary_arg(q, out, q_weight, norm, "q", dev, stream, 1, T, D, dt)
+        qs = q.stride()
+        at.append((q.data_ptr(), 2 * ((T - 1) * qs[0] + (q.shape[1] - 1) * qs[1] + D)))
+        if q_weight is not None:
+            at.append((q_weight.data_ptr(), q_weight.nbytes))
     elif out is not None or q_weight is not None:
         raise ValueError("t2t: out and q_weight belong to q")
-    # the cache (and a caller's output) apart from everything that is read
     ins = (q, k, v, cos, sin, q_weight, k_weight, slots)
-    at = [(p, e - p) for p, e in (_span(t) for t in ins if t is not None)]
-    if out is not None and q is not out:
-        at.append((lambda p, e: (p, e - p))(*_span(oq)))
-    if out is not None or _near(*_span(ck), at) or _near(*_span(cv), at):
-        if out is not None:
-            _apart((oq, ck, cv), ("the output of q", "the cache", "the cache"), ins[:1] + (None, None) + ins[1:])
-        else:
+    kend, vend = pck + cache._bytes, pcv + cache._bytes
+    for p, n in at if out is None and T else ():
+        if p < kend and pck < p + n or p < vend and pcv < p + n:
             _apart((ck, cv), ("the cache", "the cache"), (None, None) + ins)
-    _launch("t2t_cache_append", dev, stream, (*ins, ck, cv, oq), tq, tk, tv, dtype_code(dt), cos.data_ptr(),
-            sin.data_ptr(), slots.data_ptr(), bits, pages, page, T, D, R, _ROPE_LAYOUTS[layout], _ROPE_NORMS[norm],
-            eps)
+    if out is not None:
+        _apart((oq, ck, cv), ("the output of q", "the cache", "the cache"), ins[:1] + (None, None) + ins[1:])
+    _launch("t2t_cache_append", dev, stream, (*ins, ck, cv, oq), tq, pack(pk, 0, ks[0], ks[1], pck, *cs, pw or 0, H),
+            pack(pv, 0, vs[0], vs[1], pcv, *cs, 0, H), dtype_code(dt), pcos, psin, ps, bits, pages, page, T, D, 2 * P,
+            _ROPE_LAYOUTS[layout], _ROPE_NORMS[norm], eps)
     return oq
 
 
@@ -1584,8 +1597,8 @@ def cache_attention_ws_bytes(B, T, Hq, cache, width, ragged=False):
     """Workspace of cache_attention for T rows in all of B sequences (``ragged``: with
     offsets) whose page tables are ``width`` pages wide."""
     k = cache._k
-    return size_query("t2t_cache_attention_ws_bytes", bool(ragged), B, T, Hq, k.shape[2], k.shape[3],
-                      width * k.shape[1])
+    return _sizes_of("t2t_cache_attention_ws_bytes", bool(ragged), B, T, Hq, k.shape[2], k.shape[3],
+                     width * k.shape[1])
 
 
 def cache_attention(q, cache, page_table, lengths, *, offsets=None, mask=None, causal=False, scale=None,
@@ -1656,33 +1669,35 @@ def cache_attention(q, cache, page_table, lengths, *, offsets=None, mask=None, c
         raise ValueError(f"t2t: scale must be above 0, got {scale}")
     qs = _attn_strides(q, "q")
     if out is None:
-        o = q.new_empty(q.shape) if stream is None else _empty(stream, q.shape, dt, dev)
+        o = (_empty(stream, q.shape, dt, dev) if stream is not None
+             else torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape))
     else:
         o = out
         if not isinstance(o, torch.Tensor) or o.shape != q.shape or o.dtype != dt or o.device != dev:
             raise ValueError(f"t2t: out must be a {dt} {tuple(q.shape)} tensor on {dev}")
         if not _scattered(o):
             raise ValueError("t2t: out holds an element twice")
-    os = _attn_strides(o, "out")
+    os = qs if out is None and q.is_contiguous() else _attn_strides(o, "out")
     lse = _empty(stream, (*lead, Hq), _f32, dev) if return_lse else None
     need = cache_attention_ws_bytes(B, T, Hq, cache, width, ragged) if T and B else 0
-    if ws is not None:
+    given = ws is not None
+    if given:
         ws = _ws_for(ws, need, dev, stream)
     elif need:
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if stream is None else _ws(need, dev, stream)
     ins = (q, ck, cv, page_table, lengths, offsets, mask)
     if out is not None:
         _apart((o,), ("out",), (None, *ins))
-    if ws is not None and need:
+    if given and need:
         at = ws.data_ptr()
         if _near(at, at + need, [(p, e - p) for p, e in (_span(t) for t in (*ins, o) if t is not None)]):
             _apart((ws[:need],), ("ws",), (None, *ins, o))
     ms = mask.stride() if mask is not None else (0, 0, 0)
-    args = _lib.CacheAttentionArgs(
-        ctypes.sizeof(_lib.CacheAttentionArgs), q.data_ptr(), ck.data_ptr(), cv.data_ptr(), o.data_ptr(),
-        None if lse is None else lse.data_ptr(), page_table.data_ptr() or None, lengths.data_ptr() or None,
-        offsets.data_ptr() if ragged else None, None if mask is None else mask.data_ptr() or q.data_ptr(), *qs, *os,
-        *_cache_strides(ck), page_table.stride(0), 0 if ragged else ms[0], ms[-2], B, N, Hq, Hk, D, dtype_code(dt),
+    args = _lib.CACHE_ATTENTION_ARGS.pack(
+        _lib.CACHE_ATTENTION_ARGS.size, q.data_ptr(), ck.data_ptr(), cv.data_ptr(), o.data_ptr(),
+        0 if lse is None else lse.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
+        offsets.data_ptr() if ragged else 0, 0 if mask is None else mask.data_ptr() or q.data_ptr(), *qs, *os,
+        *cache._strides, page_table.stride(0), 0 if ragged else ms[0], ms[-2], B, N, Hq, Hk, D, dtype_code(dt),
         pages, page, width, mask.shape[-1] if mask is not None else 0, bool(causal), scale)
     _launch("t2t_cache_attention", dev, stream, (*ins, o, lse, ws), args, None if ws is None else ws.data_ptr(),
             0 if ws is None else ws.numel())
@@ -1691,8 +1706,14 @@ def cache_attention(q, cache, page_table, lengths, *, offsets=None, mask=None, c
 
 def _attn_strides(t, name):
     """Strides of sequences, tokens and heads of [B, N, H, D] or [T, H, D]."""
-    st = tuple(s if n > 1 else 0 for s, n in zip(t.stride(), t.shape))[:-1]
-    if (t.stride(-1) != 1 or any(s % 8 for s in st) or t.data_ptr() % 16) and t.numel():
+    st = t.stride()
+    if t.is_contiguous():
+        st = st[:-1]
+        bad = t.data_ptr() % 16
+    else:
+        st = tuple(s if n > 1 else 0 for s, n in zip(st, t.shape))[:-1]
+        bad = (t.stride(-1) != 1 or any(s % 8 for s in st) or t.data_ptr() % 16) and t.numel()
+    if bad:
         raise ValueError(f"t2t: {name} must have contiguous channels and 16-byte aligned rows, got strides "
                          f"{tuple(t.stride())}")
     return st if len(st) == 3 else (0, *st)
