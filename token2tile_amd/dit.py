@@ -8,8 +8,10 @@ Its self-attention runs either dense (torch SDPA) or through
 profile, dense prefix and mask-refresh reuse, so one denoising step can be
 timed both ways on the same weights and inputs.
 
-With ``mxfp4`` the blocks' linear layers run on MXFP4 operands, and with
-``fused_rope`` the RMSNorm and rotary embedding of q and k in one launch.
+With ``mxfp4`` the blocks' linear layers run on MXFP4 operands, with ``int8`` on
+8-bit ones, and with ``fused_rope`` the RMSNorm and rotary embedding of q and k in
+one launch.  A ``ChunkCache`` generates a video chunk by chunk: each chunk's tokens
+attend to their own and the earlier chunks' keys in a paged cache.
 
 ``python -m token2tile_amd.dit`` prints one JSON line with the per-step times
 at the Wan2.1-14B 720p shape (40 blocks, hidden 5120, 40 heads, FFN 13824,
@@ -40,6 +42,7 @@ class DiTConfig:
     grid: tuple[int, int, int] = (21, 45, 80)  # latent frames x height x width (720p)
     eps: float = 1e-6
     mxfp4: bool = False       # the blocks' linear layers in MXFP4 (ops.mxfp4_linear)
+    int8: bool = False        # the blocks' linear layers in 8 bits (ops.int8_linear)
     fused_rope: bool = False  # q/k RMSNorm and rotary embedding in one launch (ops.rotary)
 
     @property
@@ -86,22 +89,33 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
     return (xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps)).to(x.dtype) * weight
 
 
-class MxFp4Linear(torch.nn.Module):
-    """A linear layer whose weight is kept in MXFP4 (its codes and scales are
+class _FewBitLinear(torch.nn.Module):
+    """A linear layer whose weight is kept in fewer bits (its codes and scales are
     buffers: moved, copied, saved and loaded with the module); its input is
-    quantised at the call, or comes as an ``ops.MxFp4`` that several layers share
-    (the output's leading dimensions are then flattened)."""
+    quantised at the call, or comes as a matrix that several layers share (the
+    output's leading dimensions are then flattened)."""
 
     def __init__(self, linear: torch.nn.Linear):
         super().__init__()
-        from token2tile_amd import ops
-        w = ops.mxfp4_quantize(linear.weight.detach())
+        w = self.quantize(linear.weight.detach())
         self.out_features, self.in_features = w.shape
         self.register_buffer("weight_codes", w.codes)
         self.register_buffer("weight_scales", w.scales)
         # of the outputs' type, which the module's conversions change with the bias
         self.register_buffer("_like", linear.weight.detach().new_empty(0), persistent=False)
         self.bias = linear.bias
+
+    def _dtype(self, x):
+        return None if isinstance(x, torch.Tensor) else self._like.dtype
+
+
+class MxFp4Linear(_FewBitLinear):
+    """In MXFP4, input and weight (``ops.MxFp4``)."""
+
+    @staticmethod
+    def quantize(x):
+        from token2tile_amd import ops
+        return ops.mxfp4_quantize(x)
 
     @property
     def weight(self):
@@ -110,16 +124,64 @@ class MxFp4Linear(torch.nn.Module):
 
     def forward(self, x, activation=None):
         from token2tile_amd import ops
-        return ops.mxfp4_linear(x, self.weight, self.bias, activation=activation,
-                                dtype=self._like.dtype if isinstance(x, ops.MxFp4) else None)
+        return ops.mxfp4_linear(x, self.weight, self.bias, activation=activation, dtype=self._dtype(x))
+
+
+class Int8Linear(_FewBitLinear):
+    """In 8 bits, a scale for each token and channel (``ops.Int8``)."""
+
+    def _apply(self, fn, *args, **kw):
+        # conversions of the module to a 16-bit type leave the scales in 32 bits, as they are
+        scales = self.weight_scales
+        super()._apply(fn, *args, **kw)
+        if self.weight_scales.dtype != scales.dtype:
+            self.weight_scales = scales.to(self.weight_scales.device)
+        return self
+
+    @staticmethod
+    def quantize(x):
+        from token2tile_amd import ops
+        return ops.int8_quantize(x)
+
+    @property
+    def weight(self):
+        from token2tile_amd import ops
+        return ops.Int8(self.weight_codes, self.weight_scales, self.out_features, self.in_features)
+
+    def forward(self, x, activation=None):
+        from token2tile_amd import ops
+        return ops.int8_linear(x, self.weight, self.bias, activation=activation, dtype=self._dtype(x))
 
 
 def _shared(x, layer):
-    """x as ``layer`` and its neighbours take it: in MXFP4 once for all of them."""
-    if isinstance(layer, MxFp4Linear):
+    """x as ``layer`` and its neighbours take it: in few bits once for all of them."""
+    return layer.quantize(x) if isinstance(layer, _FewBitLinear) else x
+
+
+class ChunkCache:
+    """The keys and values of a stack's self-attention for generation chunk by
+    chunk: a paged cache for each block, with room for ``tokens`` (default: the
+    configuration's), and the positions of the chunk at hand."""
+
+    def __init__(self, cfg: DiTConfig, device, dtype=torch.bfloat16, tokens=None, page_size=64):
         from token2tile_amd import ops
-        return ops.mxfp4_quantize(x)
-    return x
+        self.tokens = cfg.tokens if tokens is None else tokens
+        pages = -(-self.tokens // page_size)
+        self.blocks = []
+        for _ in range(cfg.blocks):
+            k, v = torch.zeros(2, pages, page_size, cfg.heads, cfg.head_dim, dtype=dtype, device=device)
+            self.blocks.append(ops.PagedCache(k, v))
+        self.table = torch.arange(pages, dtype=torch.int32, device=device)[None]
+        self.slots = self.lengths = None
+
+    def at(self, start, n):
+        """Tokens ``start`` .. ``start + n - 1`` come next (again, at each step of a
+        chunk's denoising): their slots are theirs, and they see all before them."""
+        if not (0 <= start and 1 <= n and start + n <= self.tokens):
+            raise ValueError(f"tokens {start} .. {start + n - 1} of a cache for {self.tokens}")
+        dev = self.table.device
+        self.slots = torch.arange(start, start + n, dtype=torch.int32, device=dev)
+        self.lengths = torch.full((1,), start + n, dtype=torch.int32, device=dev)
 
 
 class Block(torch.nn.Module):
@@ -146,10 +208,10 @@ class Block(torch.nn.Module):
         self.ffn2 = torch.nn.Linear(Fh, D)
         self.attn_impl = attn_impl  # None: dense SDPA
 
-    def quantize_(self):
-        """The block's linear layers in MXFP4, in the place of the 16-bit ones."""
+    def quantize_(self, layer=MxFp4Linear):
+        """The block's linear layers as ``layer``, in the place of the 16-bit ones."""
         for name in ("q", "k", "v", "o", "cq", "ck", "cv", "co", "ffn1", "ffn2"):
-            setattr(self, name, MxFp4Linear(getattr(self, name)))
+            setattr(self, name, layer(getattr(self, name)))
 
     def qkv(self, x, rope):
         """q, k (normed and rotated) and v [B, N, H, d] of the self-attention."""
@@ -166,6 +228,19 @@ class Block(torch.nn.Module):
         q = rms_norm(q, self.norm_q, self.cfg.eps).view(B, N, H, d)
         k = rms_norm(k, self.norm_k, self.cfg.eps).view(B, N, H, d)
         return apply_rope(q, *rope), apply_rope(k, *rope), v
+
+    def chunk_attention(self, x, rope, cache):
+        """The self-attention of a chunk, behind the chunks that the cache holds."""
+        from token2tile_amd import ops
+        B, N, D = x.shape
+        H, d = self.cfg.heads, self.cfg.head_dim
+        x = _shared(x, self.q)
+        q, k, v = (y(x).view(N, H, d) for y in (self.q, self.k, self.v))
+        own = cache.blocks[self.index]
+        q = ops.cache_append(q, k, v, *rope, own, cache.slots, norm="token", q_weight=self.norm_q,
+                             k_weight=self.norm_k, eps=self.cfg.eps, out=q)
+        o = ops.cache_attention(q.view(B, N, H, d), own, cache.table, cache.lengths)
+        return self.o(o.view(B, N, D))
 
     def self_attention(self, x, rope, attn_metadata):
         B, N, D = x.shape
@@ -187,14 +262,15 @@ class Block(torch.nn.Module):
         o = F.scaled_dot_product_attention(q, k, v).transpose(1, 2).reshape(B, N, D)
         return self.co(o)
 
-    def forward(self, x, t_emb, ctx, rope, attn_metadata):
+    def forward(self, x, t_emb, ctx, rope, attn_metadata, cache=None):
         e = (self.modulation + t_emb[:, None, :]).chunk(6, dim=1)  # 6 x [B, 1, D]
         D = self.cfg.hidden
         h = F.layer_norm(x, (D,), eps=self.cfg.eps) * (1 + e[1]) + e[0]
-        x = x + self.self_attention(h, rope, attn_metadata) * e[2]
+        a = self.self_attention(h, rope, attn_metadata) if cache is None else self.chunk_attention(h, rope, cache)
+        x = x + a * e[2]
         x = x + self.cross_attention(self.norm3(x), ctx)
         h = F.layer_norm(x, (D,), eps=self.cfg.eps) * (1 + e[4]) + e[3]
-        if isinstance(self.ffn1, MxFp4Linear):
+        if isinstance(self.ffn1, _FewBitLinear):
             y = self.ffn1(h, activation="gelu_tanh")
         else:
             y = F.gelu(self.ffn1(h), approximate="tanh")
@@ -209,6 +285,8 @@ class WanDiT(torch.nn.Module):
 
     def __init__(self, cfg: DiTConfig, sparse: bool, device, dtype=torch.bfloat16, tie=0.0):
         super().__init__()
+        if cfg.mxfp4 and cfg.int8:
+            raise ValueError("linear layers in MXFP4 or in 8 bits, not both")
         self.cfg = cfg
         impls = [None] * cfg.blocks
         if sparse:
@@ -229,9 +307,9 @@ class WanDiT(torch.nn.Module):
                 for blk in self.blocks:
                     blk.k.weight.mul_(math.sqrt(1.0 - tie * tie)).add_(tie * blk.q.weight)
         self.to(dtype)
-        if cfg.mxfp4:
+        if cfg.mxfp4 or cfg.int8:
             for blk in self.blocks:
-                blk.quantize_()
+                blk.quantize_(MxFp4Linear if cfg.mxfp4 else Int8Linear)
         self.rope = rope_tables(cfg, device)
 
     @torch.no_grad()
@@ -239,6 +317,17 @@ class WanDiT(torch.nn.Module):
         for blk in self.blocks:
             md = metadata_for_layer(blk.index) if metadata_for_layer is not None else None
             x = blk(x, t_emb, ctx, self.rope, md)
+        return x
+
+    @torch.no_grad()
+    def forward_chunk(self, x, t_emb, ctx, cache: ChunkCache, start):
+        """Tokens ``start`` .. of the video (x [1, n, hidden]; by whole frames, for
+        chunks that see all of themselves) behind those the cache holds."""
+        n = x.shape[1]
+        cache.at(start, n)
+        rope = tuple(t[start:start + n] for t in self.rope)
+        for blk in self.blocks:
+            x = blk(x, t_emb, ctx, rope, None, cache)
         return x
 
 
@@ -299,6 +388,29 @@ def run(cfg: DiTConfig, steps, device, *, sparse: bool, profile="auto", budget_k
     return times
 
 
+def run_chunks(cfg: DiTConfig, frames, device, steps=2, seed=0):
+    """Time the block stack over a video in chunks of ``frames`` latent frames, each
+    ``steps`` times (its denoising steps); returns the ms of each chunk's last."""
+    torch.manual_seed(seed)
+    model = WanDiT(cfg, False, device)
+    g = torch.Generator(device=device).manual_seed(seed + 1)
+    r = lambda *shape: torch.randn(*shape, generator=g, device=device, dtype=torch.bfloat16)  # noqa: E731
+    x, ctx, t_emb = r(1, cfg.tokens, cfg.hidden), r(1, cfg.context_tokens, cfg.hidden), 0.1 * r(1, cfg.hidden)
+    cache, n = ChunkCache(cfg, device), frames * cfg.grid[1] * cfg.grid[2]
+    times = []
+    for start in range(0, cfg.tokens, n):
+        for _ in range(steps):
+            torch.cuda.synchronize(device)
+            t0 = time.perf_counter()
+            y = model.forward_chunk(x[:, start:start + n], t_emb, ctx, cache, start)
+            torch.cuda.synchronize(device)
+            ms = (time.perf_counter() - t0) * 1e3
+        times.append(ms)
+        print(f"[dit] tokens {start} .. {min(start + n, cfg.tokens) - 1}: {ms:.1f} ms", file=sys.stderr, flush=True)
+        assert bool(torch.isfinite(y).all()), "non-finite DiT output"
+    return times
+
+
 WINDOWS = ((12, 21), (21, 31), (31, 41), (41, 50))  # the backend's budget windows
 
 
@@ -311,13 +423,31 @@ def main(argv=None):
                    help="tied q/k weights and a smooth latent (local attention); default: random")
     p.add_argument("--mxfp4", action="store_true",
                    help="the blocks' linear layers in MXFP4; default: bf16")
+    p.add_argument("--int8", action="store_true",
+                   help="the blocks' linear layers in 8 bits; default: bf16")
+    p.add_argument("--chunk", type=int, default=0, metavar="FRAMES",
+                   help="time generation in chunks of that many latent frames (dense attention over a paged cache) "
+                        "instead of whole steps")
     p.add_argument("--fused-rope", action="store_true",
                    help="q/k norm and rotary embedding in one launch; default: torch")
     args = p.parse_args(argv)
     if not torch.cuda.is_available():
         sys.exit("the DiT harness needs a ROCm GPU")
     dev = torch.device("cuda", 0)
-    cfg = DiTConfig(blocks=args.blocks, mxfp4=args.mxfp4, fused_rope=args.fused_rope)
+    if args.mxfp4 and args.int8:
+        p.error("--mxfp4 or --int8")
+    cfg = DiTConfig(blocks=args.blocks, mxfp4=args.mxfp4, int8=args.int8, fused_rope=args.fused_rope)
+    linear = {"linear": "mxfp4"} if cfg.mxfp4 else {"linear": "int8"} if cfg.int8 else {}
+    if args.chunk:
+        if not 1 <= args.chunk <= cfg.grid[0]:
+            p.error(f"--chunk: 1 to {cfg.grid[0]} frames")
+        times = run_chunks(cfg, args.chunk, dev)
+        print(json.dumps({"metric": "Wan2.1-14B DiT denoising step of a chunk (one CFG branch), ms",
+                          "config": {"blocks": cfg.blocks, "hidden": cfg.hidden, "heads": cfg.heads, "ffn": cfg.ffn,
+                                     "tokens": cfg.tokens, "chunk_frames": args.chunk, "dtype": "bf16",
+                                     "weights": "random"},
+                          **linear, "chunk_ms": [round(t, 1) for t in times]}), flush=True)
+        return
     dense = run(cfg, [0, 1, 2], dev, sparse=False, structured=args.structured)
     d_ms = (dense[1] + dense[2]) / 2
     torch.cuda.empty_cache()
@@ -344,7 +474,7 @@ def main(argv=None):
                       "dtype": "bf16",
                       "weights": "random, k tied to q (0.9), smooth latent" if args.structured
                       else "random", "attention_profile": "auto"},
-           **({"linear": "mxfp4"} if cfg.mxfp4 else {}), **({"rope": "fused"} if cfg.fused_rope else {}),
+           **linear, **({"rope": "fused"} if cfg.fused_rope else {}),
            "dense_ms_per_step": round(d_ms, 1),
            "t2t_step_ms": {str(k): round(v, 1) for k, v in sparse.items()},
            "t2t_ms_per_step_by_window": [round(w, 1) for w in win_ms],
