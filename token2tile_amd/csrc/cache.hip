@@ -49,8 +49,8 @@ struct CacheArgs {
 };
 
 // Parts that a sequence of L keys goes in: of one size, that of the table's keys in S parts, so that all
-// work-groups have about the same to do; CA_PART keys at least.
-#define CA_PART 512
+// work-groups have about the same to do; CA_PART keys at least (a tile of each of two waves).
+#define CA_PART 64
 __device__ inline int ca_parts(const CacheArgs& A, int L) { return L < 1 ? 1 : (L - 1) / A.part + 1; }
 
 // A work-group's rows: a row block of ROWS packed rows (token, head of the group) of a sequence.
@@ -957,25 +957,31 @@ __global__ __launch_bounds__(256) void ca_combine_kernel(CacheArgs A) {
   if (A.lse && lane == 0) A.lse[at] = total == 0.f ? -__builtin_inff() : 0.6931471805599453f * (M + __log2f(total));
 }
 
-// Packed rows of a row block: by the rows that a sequence may have (all of them, where they are not
-// known to the host).
-static int ca_block(int ragged, int B, long long T, int G) {
-  const long long rows = (ragged ? T : T / B) * G;
-  return rows <= 64 ? 32 : rows <= 128 ? 128 : 256;
-}
-// Most parts of a sequence's keys, of CA_PART keys at least: as many as bring a small launch to a round
-// of work-groups (256 at once; with few rows two of 512, as sequences differ in length), and a larger
-// one to rounds that are nearly full.
-static int ca_split(int block, long long tiles, int HK, long long keys) {
-  const long long wgs = tiles * HK, slots = block == 32 ? 512 : 256;
-  long long most = (keys + CA_PART - 1) / CA_PART, s = 1;
-  most = most < 64 ? most : 64;
-  if (wgs < slots) {
-    s = ((block == 32 ? 2 : 1) * slots + wgs - 1) / wgs;
-  } else if (wgs < 4 * slots) {
-    while (s < 4 && 20 * wgs * s < 17 * ((wgs * s + slots - 1) / slots) * slots) ++s;
-  }
-  return (int)(s < most ? s : most < 1 ? 1 : most);
+// Packed rows of a row block and most parts of a sequence's keys, by the least time of an estimate.
+// Measured as graphs of ten launches, us, D = 128:
+//   rows a sequence, keys, key heads x sequences     blocks of 32      128      256
+//   32, 32,000, 40                                            154      170      199
+//   48, 32,000, 40                                            249      158      199
+//   128, 32,000, 40                                           414      164      206
+//   400, 1,000, 320                                           214      102       90
+//   4,680, 32,760, 12                                           -      865      823
+// so 32 where a sequence has no more rows, else 128 or 256.  Parts: a work-group alone goes through its
+// keys at its latency, so there should be about as many as run at once, but a further round costs its
+// own, and the parts' sums are written and read again:
+//   1 row, 32,760 keys, 40 heads     S = 6: 165   12 (480 work-groups): 118   13 (520): 164   26: 139
+//   1,560 rows, 9,360, 12 (256)      S = 1: 195    2: 121    3 (252 work-groups): 103    4: 138
+//   400 rows, 1,000, 320 (256)       S = 1:  90    2: 155
+//   1 row, 1,000, 8                  S = 2:  19    8: 12
+// The estimate: a key of a work-group takes the longer the more run beside it (they share the memory
+// and the power); the constants are fitted to such measurements.
+static double ca_time(int block, long long wgs, int S, double keys, double rows) {
+  const int slots = block == 256 ? 256 : 512;  // work-groups at once
+  auto key = [&](long long n) { return block == 32 ? 22e-3 + 45e-6 * n : block == 128 ? 14e-3 + 30e-6 * n : 20e-3 + 20e-6 * n; };
+  const long long n = wgs * S, full = n / slots, rest = n % slots;
+  const double part = 64.0 * (long long)((keys / S + 63) / 64), start = block == 256 ? 3.5 : 2.0;
+  double us = (double)full * (part * key(slots) + start);
+  if (rest) us += part * key(rest) + start;
+  return S < 2 ? us : us + 3.0 + 0.1 * S + 0.23e-3 * S * rows;  // (the join: launched, its loads, its bytes)
 }
 // row blocks of `block` packed rows
 static long long ca_tiles(int block, int ragged, int B, long long T, int G) {
@@ -986,12 +992,33 @@ static long long ca_full(int block, int ragged, int B, long long T, int G) {
   const long long n = (T * G + block - 1) / block;
   return ragged ? (n > B ? n : B) : ca_tiles(block, ragged, B, T, G);
 }
+struct CachePlan {
+  int block, S;
+};
+static CachePlan ca_plan(int ragged, int B, long long T, int HQ, int HK, long long keys) {
+  const int G = HQ / HK;
+  // (of a ragged batch: twice the mean, as its sequences are not known to the host)
+  long long rows = (T + B - 1) / B * G * (ragged ? 2 : 1);
+  if (rows > T * G) rows = T * G;
+  const long long parts = (keys + CA_PART - 1) / CA_PART, most = parts < 1 ? 1 : parts < 64 ? parts : 64;
+  CachePlan best{rows <= 32 ? 32 : 128, 1};
+  double least = 0.0;
+  for (int block = best.block; block <= (rows <= 128 ? best.block : 256); block *= 2) {
+    const long long wgs = ca_full(block, ragged, B, T, G) * HK, slots = block == 256 ? 256 : 512;
+    for (int i = 0; i < 11; ++i) {  // 1, 2, 3 and eighths of all that run at once
+      const long long S = i < 3 ? i + 1 : (i - 2) * slots / 8 / wgs;
+      if (S < 1 || S > most) continue;
+      const double us = ca_time(block, wgs, (int)S, (double)keys, (double)T * HQ);
+      if (least == 0.0 || us < least) least = us, best = CachePlan{block, (int)S};
+    }
+  }
+  return best;
+}
 static size_t ca_ws(int S, long long rows, int D) { return S < 2 ? 0 : (size_t)S * rows * (D + 2) * 4; }
 
 extern "C" size_t t2t_cache_attention_ws_bytes(int ragged, int B, long long T, int HQ, int HK, int D, long long keys) {
   if (B < 1 || T < 1 || HK < 1 || HQ < HK || keys < 1) return 0;
-  const int G = HQ / HK, block = ca_block(ragged, B, T, G);
-  return ca_ws(ca_split(block, ca_full(block, ragged, B, T, G), HK, keys), T * HQ, D);
+  return ca_ws(ca_plan(ragged, B, T, HQ, HK, keys).S, T * HQ, D);
 }
 
 extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -1031,10 +1058,12 @@ extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, 
   A.pages = a->pages, A.page = a->page_size, A.width = a->width, A.mask_cols = a->mask_cols, A.causal = a->causal;
   A.shift = (a->page_size & (a->page_size - 1)) ? -1 : __builtin_ctz(a->page_size);
   A.c = a->scale * 1.4426950408889634f;
-  const int ragged = a->offsets != nullptr, block = ca_block(ragged, a->B, T, A.G);
-  const long long tiles = ca_tiles(block, ragged, a->B, T, A.G);
+  const int ragged = a->offsets != nullptr;
   const long long keys = (long long)a->width * a->page_size;
-  A.S = ca_split(block, ca_full(block, ragged, a->B, T, A.G), a->HK, keys < 1 ? 1 : keys);
+  const CachePlan plan = ca_plan(ragged, a->B, T, a->HQ, a->HK, keys);
+  const int block = plan.block;
+  const long long tiles = ca_tiles(block, ragged, a->B, T, A.G);
+  A.S = plan.S;
   // (as many parts as the workspace holds)
   while (A.S > 1 && (!ws || ws_bytes < ca_ws(A.S, T * a->HQ, a->D))) --A.S;
   if (A.S > 1) {
