@@ -337,7 +337,8 @@ def _operands(dev, M, N, K, dt, seed):
 SIZES = [(1, 1, 1), (1, 64, 64), (1, 5000, 33000), (3, 70, 10001), (8, 100, 4097), (9, 100, 4097), (1, 5120, 512), (2, 33, 95), (5, 96, 256), (16, 48, 1024), (17, 31, 300),
          (31, 100, 288), (32, 32, 1571), (33, 257, 512), (64, 640, 2048), (100, 72, 5120), (129, 130, 161),
          (257, 513, 256), (600, 1000, 321), (1000, 1536, 1536), (2049, 776, 64), (4099, 2041, 1571),
-         (33, 20481, 256), (700, 1100, 512), (16385, 1030, 1057), (4100, 4200, 1024), (70000, 1025, 96)]
+         (33, 20481, 256), (700, 1100, 512), (16385, 1030, 1057), (4100, 4200, 1024), (70000, 1025, 96),
+         (3900, 4091, 1057), (3969, 4096, 320), (8000, 4060, 96)]
 
 
 @pytest.mark.gpu
@@ -357,7 +358,8 @@ def test_linear(dev, M, N, K, dt, bias, act):
 
 
 # forms of every size of tile, ragged in both directions
-TILES = [(3, 40, 96), (40, 100, 700), (1000, 1536, 512), (1000, 1531, 800), (4100, 4200, 1024), (4100, 4195, 1057)]
+TILES = [(3, 40, 96), (40, 100, 700), (1000, 1536, 512), (1000, 1531, 800), (4100, 4200, 1024), (4100, 4195, 1057),
+         (3900, 4088, 512), (3969, 4091, 705)]
 
 
 @pytest.mark.gpu
@@ -413,7 +415,7 @@ def test_linear_of_nonfinite_rows(dev, M, N, K):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("M,N", [(2, 40), (40, 200), (600, 1000), (4100, 4200)])
+@pytest.mark.parametrize("M,N", [(2, 40), (40, 200), (600, 1000), (4100, 4200), (3900, 4090)])
 def test_linear_of_the_longest_sums(dev, M, N):
     """Codes of the largest magnitude over the longest rows, -128 among them: the
     sums fill 31 bits and are exact."""

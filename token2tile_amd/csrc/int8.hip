@@ -123,7 +123,7 @@ __device__ inline uint32_t i8_top(uint32_t top, const u32x4& v) {  // both halve
 // TPR threads a row, which stays in registers between its maximum and its codes:
 // one read of x, one write of the codes.  A work-group has several rows where it can:
 // a row writes half lines (64 bytes of every block), its neighbour the other halves
-// (75,600 x 5,120: XX us with four rows, 239 with one).
+// (75,600 x 5,120: 228 us with four rows, 239 with one).
 template <typename T, int TPR, int I, int ROWS>
 __global__ __launch_bounds__(TPR * ROWS) void i8_quantize_kernel(
     const uint16_t* __restrict__ x, long long row_stride, char* __restrict__ codes, float* __restrict__ scales, int M,
@@ -772,13 +772,27 @@ static int i8_tile_launch(const I8Mat& a, const I8Mat& w, const uint16_t* bias, 
   return T2T_OK;
 }
 
+// Which tile, measured in graphs of twenty launches, us (K = 5,120 / 1,536):
+//                       32 x 32 blocks     split       128 x 128       256 x 256
+//   96 x 5,120                       480  13.2 /  6.2   15.2 /  7.2    46.6 / 19.3
+//   128 x 5,120                      640  18.6 /  8.6   15.4 /  7.3    46.6 / 19.8
+//   2,048 x 5,120 (160 of 256 x 256)                    55.5 / 20.9    53.2 / 24.4
+//   3,000 x 5,120 (240)                                 75.9 / 28.1    66.1 / 27.5
+//   4,096 x 4,096 (256)                                 78.6 / 29.7    70.1 / 28.7
+//   9,000 x 2,048 (288)                                 90.9 / 34.1     110 / 44.1
+//   2,700 x 13,824 (594)                                 185 / 70.3     172 / 67.1
+// The small tiles' time goes with their number (two fit a CU, of which one goes on while the other
+// starts or ends); the large ones go by rounds of 256, of which a full one takes that of 890 small tiles
+// and an empty one more than half of it.
 template <typename T>
 static int i8_product(const I8Mat& a, const I8Mat& w, const uint16_t* bias, int act, uint16_t* out, long long ldo,
                       int units, hipStream_t st) {
-  const long long big = (long long)cdiv(a.blocks, 8) * cdiv(w.blocks, 8);
+  if ((long long)a.blocks * w.blocks <= 512)
+    return i8_split_launch<T, 4, false>(I8Src{a, nullptr, 0, 0}, w, bias, act, out, ldo, units, st);
+  const long long big = (long long)cdiv(a.blocks, 8) * cdiv(w.blocks, 8), rest = big % 256;
   const long long mid = (long long)cdiv(a.blocks, 4) * cdiv(w.blocks, 4);
-  if ((long long)a.blocks * w.blocks <= 512) return i8_split_launch<T, 4, false>(I8Src{a, nullptr, 0, 0}, w, bias, act, out, ldo, units, st);
-  if (big >= 256 && 4 * big <= mid + mid / 4) return i8_tile_launch<T, 4, 4>(a, w, bias, act, out, ldo, units, st);
+  if (big / 256 * 890 + (rest ? 470 + 420 * rest / 256 : 0) < mid + 25)
+    return i8_tile_launch<T, 4, 4>(a, w, bias, act, out, ldo, units, st);
   return i8_tile_launch<T, 2, 2>(a, w, bias, act, out, ldo, units, st);
 }
 
