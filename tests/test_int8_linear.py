@@ -214,6 +214,24 @@ def test_refused(launches, bad):
 # every count of values a thread, the borders between them, rows of one value and of odd widths
 WIDTHS = [1, 2, 7, 8, 9, 127, 128, 129, 511, 513, 1023, 1531, 2048, 2049, 4096, 4097, 5120, 6145, 8192, 8200, 16385,
           32769, 131071]
+MANY = [300, 1000, 1531, 2041, 5120, 16000]  # of rows enough that fewer threads take each
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", HALF)
+@pytest.mark.parametrize("K", MANY)
+def test_quantize_many_rows(dev, K, dt):
+    g, dt, M = _gen(dev, K), HALF[dt], 1027
+    x = (_randn(g, M, K) * torch.exp(2 * _randn(g, M, 1))).to(dt)
+    x[5, K // 2] = math.inf
+    t = ops.int8_quantize(x)
+    few = ops.int8_quantize(x[1000:])
+    assert bool(t.scales[5].isnan()) and not bool(t.to_codes()[5].any())
+    assert torch.equal(t.to_codes()[1000:], few.to_codes()) and torch.equal(t.scales[1000:], few.scales)
+    x[5] = 0
+    t.scales[5] = 2.0 ** -120
+    n, s = i8_ref(x)
+    assert torch.equal(t.to_codes().double(), n) and torch.equal(t.scales.double(), s)
 
 
 @pytest.mark.gpu

@@ -123,7 +123,7 @@ __device__ inline uint32_t i8_top(uint32_t top, const u32x4& v) {  // both halve
 // TPR threads a row, which stays in registers between its maximum and its codes:
 // one read of x, one write of the codes.  A work-group has several rows where it can:
 // a row writes half lines (64 bytes of every block), its neighbour the other halves
-// (75,600 x 5,120: 228 us with four rows, 239 with one).
+// (75,600 x 5,120: 217 us with two rows, 260 with one).
 template <typename T, int TPR, int I, int ROWS>
 __global__ __launch_bounds__(TPR * ROWS) void i8_quantize_kernel(
     const uint16_t* __restrict__ x, long long row_stride, char* __restrict__ codes, float* __restrict__ scales, int M,
@@ -173,17 +173,19 @@ static void i8_quantize_launch(const uint16_t* x, long long row_stride, char* co
   };
 #define I8_GO(TPR, I, ROWS) \
   go(std::integral_constant<int, TPR>{}, std::integral_constant<int, I>{}, std::integral_constant<int, ROWS>{})
-  const bool many = M >= 1024;  // else more threads take a row (1 x 5,120: 2.5 us)
+  // enough threads a row that its loads come at once (us, 10 x 16 bytes a thread of 64 against 3 of 256,
+  // K = 5,120: 64 rows 7.3 and 4.0, 2,048 rows 11.9 and 9.3, 75,600 rows 225 and 217); more shorten
+  // small launches alone (K = 1,536, 3 of 64 against 1 of 256: 256 rows 3.7 and 3.1, 4,680 rows 7.0 and 10.1)
+  const bool many = M >= 1024;
   if (Kp <= 512) I8_GO(64, 1, 4);
   else if (Kp <= 1024) I8_GO(64, 2, 4);
-  else if (Kp <= 1536 && many) I8_GO(64, 3, 4);
-  else if (Kp <= 2048) I8_GO(64, 4, 4);
-  else if (Kp <= 3584 && many) I8_GO(64, 7, 4);
-  else if (Kp <= 5120 && many) I8_GO(64, 10, 4);
-  else if (Kp <= 4096) I8_GO(256, 2, 1);
+  else if (Kp <= 2048 && !many) I8_GO(256, 1, 2);
+  else if (Kp <= 1536) I8_GO(64, 3, 4);
+  else if (Kp <= 2048) I8_GO(128, 2, 4);
+  else if (Kp <= 4096) I8_GO(256, 2, 2);
   else if (Kp <= 6144) I8_GO(256, 3, 2);
   else if (Kp <= 8192) I8_GO(256, 4, 2);
-  else if (Kp <= 14336) I8_GO(256, 7, 2);
+  else if (Kp <= 16384) I8_GO(512, 4, 2);
   else if (Kp <= 32768) I8_GO(1024, 4, 1);
   else I8_GO(1024, 16, 1);
 #undef I8_GO
