@@ -84,11 +84,12 @@ def test_entries_reject_bad_arguments():
 def test_workspace_bytes():
     from token2tile_amd import _lib
     f = _lib.lib().t2t_cache_attention_ws_bytes
-    assert f(0, 1, 1, 40, 8, 128, 100) == 0                  # one part
-    assert f(0, 1, 4680, 40, 40, 128, 32768) == 0            # enough rows
-    one = f(0, 1, 1, 40, 8, 128, 1 << 16)
+    assert f(0, 0, 1, 1, 40, 8, 128, 100) == 0               # one part
+    assert f(0, 0, 1, 4680, 40, 40, 128, 32768) == 0         # enough rows
+    one = f(0, 0, 1, 1, 40, 8, 128, 1 << 16)
     assert one >= 2 * 40 * 130 * 4 and one % (40 * 130 * 4) == 0
-    assert f(0, 0, 0, 40, 8, 128, 100) == 0 and f(1, 4, 61, 32, 8, 64, 20000) > 0
+    assert f(0, 0, 0, 0, 40, 8, 128, 100) == 0 and f(1, 0, 4, 61, 32, 8, 64, 20000) > 0
+    assert f(0, 1, 1, 8192, 8, 8, 128, 8192) > f(0, 0, 1, 8192, 8, 8, 128, 8192) == 0  # row blocks that differ
 
 
 def test_cpu_tensors_are_refused():
@@ -526,6 +527,46 @@ UNIFORM = [  # lengths, N, Hq, Hk, D, page
     ([61, 200], 61, 4, 2, 128, 16), ([129, 130], 129, 2, 2, 128, 64), ([1000], 300, 4, 4, 128, 64),
     ([90, 1500, 700], 33, 6, 2, 64, 256), ([3000], 1, 40, 1, 128, 16), ([2500], 700, 3, 3, 64, 48),
     ([4200], 1030, 2, 2, 128, 16)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,L,Hq,Hk,D,page,frame,cols", [
+    (300, 300, 2, 1, 128, 16, 50, 300), (300, 1000, 4, 1, 64, 48, 70, 299), (700, 1500, 3, 3, 128, 64, 64, 700),
+    (1300, 1300, 2, 2, 128, 64, 500, 1300), (1100, 900, 2, 2, 64, 16, 300, 1100), (2100, 2500, 2, 1, 128, 256, 33, 2600),
+    (900, 5000, 1, 1, 128, 1, 400, 257), (600, 700, 2, 2, 128, 16, 600, 256)])
+@pytest.mark.parametrize("kind", ["frames", "window", "holes"])
+def test_attention_of_frames(dev, N, L, Hq, Hk, D, page, frame, cols, kind):
+    """Masks that most of the new keys pass: tokens see their frame and those before it, or the frame and the one
+    before alone, or all but single keys, one of them an inf; rows that see no new key; any byte but 0 is true."""
+    g, dt = _gen(dev, 21), torch.bfloat16
+    pages, table = _pages(g, [L, L - 1], page)
+    cache = _cache(g, pages, page, Hk, D, dt)
+    q = _randn(g, 2, N, Hq, D).to(dt)
+    f = torch.arange(N, device=dev) // frame
+    see = f[:, None] >= f[None]
+    if kind == "window":
+        see = see & (f[:, None] <= f[None] + 1)
+    if kind == "holes":
+        see = torch.ones_like(see)
+        see[torch.arange(0, N, 7), torch.arange(0, N, 7) * 5 % N] = False
+        see[:, N // 2] = False
+    see = see[None].repeat(2, 1, 1)
+    see[1, N // 3] = False
+    byte = torch.randint(1, 256, (2, N, cols + 3), generator=g, device=dev).to(torch.uint8)
+    byte[:, :, :min(N, cols)] *= see[:, :, :cols]
+    mask = byte.view(torch.bool)[:, :, :cols]            # (rows at any address)
+    if kind == "holes" and N // 2 < cols and L >= N:
+        at = L - N + N // 2
+        cache.v[table[0, at // page], at % page, 0, 3] = math.inf
+    lengths = torch.tensor([L, L - 1], dtype=I32, device=dev)
+    out, lse = ops.cache_attention(q, cache, table, lengths, mask=mask, return_lse=True)
+    full = torch.zeros(2, N, max(cols, N), dtype=torch.bool, device=dev)
+    full[:, :, :min(N, cols)] = see[:, :, :cols]
+    _check_attention(out, lse, attention_ref(q, cache, table, [L, L - 1], [N, N], full))
+    # the same rows, ragged
+    off = torch.tensor([0, N, 2 * N], dtype=I32, device=dev)
+    again = ops.cache_attention(q.flatten(0, 1), cache, table, lengths, offsets=off, mask=mask.flatten(0, 1))
+    _check_attention(again, lse, attention_ref(q, cache, table, [L, L - 1], [N, N], full))
 
 
 @pytest.mark.gpu

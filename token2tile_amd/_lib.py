@@ -169,7 +169,7 @@ SIGNATURES = {
                                 c_int, _P, c_size_t, _P]),
     "t2t_cache_append": (c_int, [_P] * 3 + [c_int, _P, _P, _P, c_int, c_int, c_int, c_longlong] + [c_int] * 4
                          + [c_float, _P]),
-    "t2t_cache_attention_ws_bytes": (c_size_t, [c_int, c_int, c_longlong, c_int, c_int, c_int, c_longlong]),
+    "t2t_cache_attention_ws_bytes": (c_size_t, [c_int, c_int, c_int, c_longlong, c_int, c_int, c_int, c_longlong]),
     "t2t_cache_attention": (c_int, [_P, _P, c_size_t, _P]),
 }
 

@@ -51,6 +51,7 @@ struct CacheArgs {
 // Parts that a sequence of L keys goes in: of one size, that of the table's keys in S parts, so that all
 // work-groups have about the same to do; CA_PART keys at least (a tile of each of two waves).
 #define CA_PART 64
+#define CA_SPAN 256  // columns of a mask from which on the many-row form searches it
 __device__ inline int ca_parts(const CacheArgs& A, int L) { return L < 1 ? 1 : (L - 1) / A.part + 1; }
 
 // A work-group's rows: a row block of ROWS packed rows (token, head of the group) of a sequence.
@@ -500,13 +501,68 @@ __device__ inline void ca_mfma_score(f32x16& c, const u32x4& a, const u32x4& b) 
 }
 #undef CA_MFMA
 
+// The new tokens that all of a work-group's tokens tok0 .. tok1 see, up to the first that one does not,
+// and one behind the last that any sees: columns of the mask's rows at `rows`, of cols >= 16.  A wave
+// takes every W-th row, eight at once, and a KB of each from either end until it has met its column.
+template <int W>
+__device__ inline void ca_span(const uint8_t* rows, long long stride, int count, int cols, int (&sFirst)[W],
+                               int (&sLast)[W], int& first, int& last) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  auto flags = [](uint32_t x) { return (((x & 0x7f7f7f7fu) + 0x7f7f7f7fu) | x) & 0x80808080u; };  // of bytes that are not 0
+  auto gather = [&](int col, uint32_t (&f)[4], auto ALL) {
+    for (int r = wave; r < count; r += 8 * W) {
+      u32x4 x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) __builtin_memcpy(&x[i], rows + min(r + i * W, count - 1) * stride + col, 16);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t y = flags(x[i][e]);
+          f[e] = decltype(ALL)::value ? f[e] & y : f[e] | y;
+        }
+    }
+  };
+  int lo = cols, hi = 0;
+  for (int b = 0; b < cols && lo == cols; b += 1024) {
+    const int col = min(b + 16 * lane, cols - 16);
+    uint32_t f[4] = {~0u, ~0u, ~0u, ~0u};
+    gather(col, f, std::true_type{});
+#pragma unroll
+    for (int e = 3; e >= 0; --e) {
+      const uint32_t none = ~f[e] & 0x80808080u;
+      if (none) lo = col + 4 * e + (__builtin_ctz(none) >> 3);
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) lo = min(lo, __shfl_xor(lo, d, 64));
+  }
+  for (int b = cols; b > 0 && hi == 0; b -= 1024) {
+    const int col = max(b - 1024 + 16 * lane, 0);
+    uint32_t f[4] = {0u, 0u, 0u, 0u};
+    gather(col, f, std::false_type{});
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (f[e]) hi = col + 4 * e + 4 - (__builtin_clz(f[e]) >> 3);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) hi = max(hi, __shfl_xor(hi, d, 64));
+  }
+  if (lane == 0) sFirst[wave] = lo, sLast[wave] = hi;
+  __syncthreads();
+  first = cols, last = 0;
+#pragma unroll
+  for (int x = 0; x < W; ++x) first = min(first, sFirst[x]), last = max(last, sLast[x]);
+}
+
 // ---- many rows: a work-group's waves share the keys --------------------------
 // 32 W packed rows a work-group of W waves; tiles of 64 keys, fetched by all waves for
 // all (DMA, one barrier a tile).  Tiles of which every row sees every key go through a
 // pipeline of half tiles: a turn computes the scores of the next half, the weights of
 // this one and the sums of the last, product by product with the weights' vector
 // operations between them, so that the matrix unit has work while the exponentials
-// are taken.  The other tiles follow, one after the other.
+// are taken.  The other tiles follow, one after the other.  Under a mask the pipeline
+// goes on through the new tokens that all of the work-group's rows see, and the tiles
+// behind the last that one of them sees are not fetched (4,096 tokens in eight frames
+// over 8,192 keys, 16 heads: 246 us, 479 with every tile of new tokens looked through).
 template <typename T, int D, int W, bool P16>
 __global__ __launch_bounds__(64 * W, 2) void ca_many_kernel(CacheArgs A) {
   constexpr int ROWS = 32 * W, LPR = D / 8, RPI = 64 / LPR, NB = D / 32, NS = D / 16;
@@ -545,9 +601,20 @@ __global__ __launch_bounds__(64 * W, 2) void ca_many_kernel(CacheArgs A) {
   // keys that some row of the work-group sees; from `plain` on not every row sees every key
   const int tok0 = w.r0 / A.G, tok1 = (min(w.r0 + ROWS, w.rows) - 1) / A.G;
   const int keys = A.causal ? min(w.L, w.first + tok1 + 1) : w.L;
-  const int plain = max(0, A.mask ? w.first : A.causal ? w.first + tok0 + 1 : w.L);
+  int plain = max(0, A.mask ? w.first : A.causal ? w.first + tok0 + 1 : w.L);
   const int all = max(0, (keys + 63) / 64);
-  const int t0 = (int)((long long)part * all / parts), nt = (int)((long long)(part + 1) * all / parts) - t0;
+  const int t0 = (int)((long long)part * all / parts);
+  int nt = (int)((long long)(part + 1) * all / parts) - t0;
+  const int cols = min(A.mask_cols, w.n);
+  if (A.mask && 64 * (t0 + nt) > w.first) {
+    __shared__ int sFirst[W], sLast[W];
+    int c0 = 0, c1 = cols;
+    if (cols >= CA_SPAN)  // (fewer are not worth the search)
+      ca_span<W>(A.mask + (A.offsets ? (w.row0 + tok0) * A.mask_row : w.b * A.mask_batch + tok0 * A.mask_row), A.mask_row,
+                 tok1 - tok0 + 1, cols, sFirst, sLast, c0, c1);
+    plain = max(0, w.first + c0);
+    nt = max(0, min(nt, (max(0, w.first + c1) + 63) / 64 - t0));
+  }
   const char* kbase = A.k + kh * A.kv_head;
   const char* vbase = A.v + kh * A.kv_head;
   const int32_t* table = A.table + w.b * A.table_row;
@@ -974,13 +1041,16 @@ __global__ __launch_bounds__(256) void ca_combine_kernel(CacheArgs A) {
 //   1 row, 1,000, 8                  S = 2:  19    8: 12
 // The estimate: a key of a work-group takes the longer the more run beside it (they share the memory
 // and the power); the constants are fitted to such measurements.
-static double ca_time(int block, long long wgs, int S, double keys, double rows) {
+// Under causal the first row blocks see few keys: the longest work-group's time, or their mean's over
+// all rounds (8,192 rows over as many keys, 8 heads: S = 1: 193 us, 2: 170).
+static double ca_time(int block, long long wgs, int S, double keys, double rows, double mean) {
   const int slots = block == 256 ? 256 : 512;  // work-groups at once
   auto key = [&](long long n) { return block == 32 ? 22e-3 + 45e-6 * n : block == 128 ? 14e-3 + 30e-6 * n : 20e-3 + 20e-6 * n; };
   const long long n = wgs * S, full = n / slots, rest = n % slots;
   const double part = 64.0 * (long long)((keys / S + 63) / 64), start = block == 256 ? 3.5 : 2.0;
   double us = (double)full * (part * key(slots) + start);
   if (rest) us += part * key(rest) + start;
+  if (mean < 1.0 && full) us = part * key(slots) * (mean * n > slots ? mean * n / slots : 1.0) + start;
   return S < 2 ? us : us + 3.0 + 0.1 * S + 0.23e-3 * S * rows;  // (the join: launched, its loads, its bytes)
 }
 // row blocks of `block` packed rows
@@ -995,20 +1065,22 @@ static long long ca_full(int block, int ragged, int B, long long T, int G) {
 struct CachePlan {
   int block, S;
 };
-static CachePlan ca_plan(int ragged, int B, long long T, int HQ, int HK, long long keys) {
+static CachePlan ca_plan(int ragged, int B, long long T, int HQ, int HK, long long keys, int causal) {
   const int G = HQ / HK;
   // (of a ragged batch: twice the mean, as its sequences are not known to the host)
   long long rows = (T + B - 1) / B * G * (ragged ? 2 : 1);
   if (rows > T * G) rows = T * G;
   const long long parts = (keys + CA_PART - 1) / CA_PART, most = parts < 1 ? 1 : parts < 64 ? parts : 64;
   CachePlan best{rows <= 32 ? 32 : 128, 1};
+  // (what a row block sees on average, of the keys)
+  const double mean = causal ? 1.0 - 0.5 * (double)rows / G / (double)(keys > rows / G ? keys : rows / G) : 1.0;
   double least = 0.0;
   for (int block = best.block; block <= (rows <= 128 ? best.block : 256); block *= 2) {
     const long long wgs = ca_full(block, ragged, B, T, G) * HK, slots = block == 256 ? 256 : 512;
     for (int i = 0; i < 11; ++i) {  // 1, 2, 3 and eighths of all that run at once
       const long long S = i < 3 ? i + 1 : (i - 2) * slots / 8 / wgs;
       if (S < 1 || S > most) continue;
-      const double us = ca_time(block, wgs, (int)S, (double)keys, (double)T * HQ);
+      const double us = ca_time(block, wgs, (int)S, (double)keys, (double)T * HQ, mean);
       if (least == 0.0 || us < least) least = us, best = CachePlan{block, (int)S};
     }
   }
@@ -1016,9 +1088,9 @@ static CachePlan ca_plan(int ragged, int B, long long T, int HQ, int HK, long lo
 }
 static size_t ca_ws(int S, long long rows, int D) { return S < 2 ? 0 : (size_t)S * rows * (D + 2) * 4; }
 
-extern "C" size_t t2t_cache_attention_ws_bytes(int ragged, int B, long long T, int HQ, int HK, int D, long long keys) {
+extern "C" size_t t2t_cache_attention_ws_bytes(int ragged, int causal, int B, long long T, int HQ, int HK, int D, long long keys) {
   if (B < 1 || T < 1 || HK < 1 || HQ < HK || keys < 1) return 0;
-  return ca_ws(ca_plan(ragged, B, T, HQ, HK, keys).S, T * HQ, D);
+  return ca_ws(ca_plan(ragged, B, T, HQ, HK, keys, causal).S, T * HQ, D);
 }
 
 extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -1060,7 +1132,7 @@ extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, 
   A.c = a->scale * 1.4426950408889634f;
   const int ragged = a->offsets != nullptr;
   const long long keys = (long long)a->width * a->page_size;
-  const CachePlan plan = ca_plan(ragged, a->B, T, a->HQ, a->HK, keys);
+  const CachePlan plan = ca_plan(ragged, a->B, T, a->HQ, a->HK, keys, a->causal);
   const int block = plan.block;
   const long long tiles = ca_tiles(block, ragged, a->B, T, A.G);
   A.S = plan.S;
