@@ -32,7 +32,8 @@ FLAGS = [
 
 # per-file extra compiler flags.  kmeans.hip: MFMA accumulators in VGPRs
 # rather than AGPRs; the assignment's min tree reads all 16 per block, and the
-# AGPR form spent 16 v_accvgpr_read per block on moving them out
+# AGPR form spent 16 v_accvgpr_read per block on moving them out.  cache.hip: the
+# same for scores; what belongs in AGPRs (queries, sums) is put there by name
 EXTRA: dict = {"kmeans.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "cache.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 

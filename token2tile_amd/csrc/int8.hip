@@ -121,7 +121,8 @@ __device__ inline uint32_t i8_top(uint32_t top, const u32x4& v) {  // both halve
 }
 
 // TPR threads a row, which stays in registers between its maximum and its codes:
-// one read of x, one write of the codes.  A work-group has several rows where it can:
+// one read of x, one write of the codes, which bound it (75,600 x 5,120: 5.3 TB/s).  A
+// work-group has several rows where it can:
 // a row writes half lines (64 bytes of every block), its neighbour the other halves
 // (75,600 x 5,120: 217 us with two rows, 260 with one).
 template <typename T, int TPR, int I, int ROWS>
@@ -206,7 +207,7 @@ extern "C" int t2t_int8_quantize(const void* x, int dtype, long long row_stride,
 
 // ---------------------------------------------------------------------------
 // the values back: eight a thread, the codes read in order, so that a row of a
-// block is stored whole (128 bytes).  Bound: writing them.
+// block is stored whole (128 bytes).  Bound: writing them (75,600 x 5,120: 205 us, 5.7 TB/s).
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(256) void i8_dequantize_kernel(const char* __restrict__ codes, long long blk,
@@ -270,7 +271,8 @@ __device__ inline float i8_out(int acc, float sw, float sa, float bias) {
 // in turn, loaded straight into registers, DEPTH units ahead.  The waves' sums
 // meet in LDS.  With X16 the tokens come in 16 bits, and every work-group quantises
 // them into LDS first, under the loads of its first weights, in the place of a launch
-// before this one.
+// before this one.  Bound: the weights' loads, of which 160 of 256 CUs have one round
+// each (1 x 5,120 x 5,120: 7.0 us, 3.7 TB/s).
 #define I8_X16_BYTES 32768  // codes that the LDS holds
 struct I8Src {
   I8Mat m;            // in 8 bits (its row count in either case), or
@@ -538,6 +540,11 @@ __device__ inline void i8_step1(i32x16 (&acc)[4][4], const I8Frags& f, I8Frags& 
                : "memory", "scc");
 }
 
+// 256 x 256 for four waves of 128 x 128: a step's sixteen products take 512 cycles, the
+// eight fragments that they need 256 of LDS reads a CU (waves of 64 x 64: as many as the
+// products).  Bound: the matrix units are busy for 69% of the cycles, and the clock falls
+// under their load (75,600 x 13,824 x 5,120 with GELU: 4.2 ms, 2.5 POP/s; a large library
+// product in 8 bits 2.1).
 // Work-groups stay for many tiles.  The DMA runs four stages ahead of the products
 // as one stream over all of them, so a tile's first stages are loaded under the last
 // products and the epilogue of the one before; the epilogue has LDS of its own.
@@ -649,7 +656,9 @@ __global__ __launch_bounds__(256, 1) void i8_big_kernel(I8Mat a, I8Mat w, const 
 // ---- the 128 x 128 tile ------------------------------------------------------
 // The same with a whole stage a step: eight products, the next stage's eight
 // fragment reads and the DMA of the stage four further on.  Two work-groups fit a
-// CU.
+// CU, and one's products pass under the other's start and epilogue.  Bound: 0.43 us a
+// stage with two on every CU (2.7 POP/s), and about 6 us beside the stages, of which the
+// outputs' bytes are a half (4,680 x 1,536 x 1,536: 15.4 us).
 #define I8_Q(c, i, j) "v_mfma_i32_32x32x32_i8 %[c" #i #j "], %[w" #c #i "], %[a" #c #j "], %[c" #i #j "]\n\t"
 #define I8_MID_STEP                                                                                     \
   "s_mov_b32 m0, %[m]\n\ts_waitcnt vmcnt(8)\n\ts_barrier\n\t" I8_Q(0, 0, 0) I8_R("x00", "bw0", "o0")    \
