@@ -750,6 +750,35 @@ def test_attention_offsets_that_are_no_offsets(dev):
     for off in ([0, 100, 5, 1 << 30, -1], [-9, -4, 0, 60, 60], [40, 30, 20, 10, 0]):
         ops.cache_attention(q, cache, table, lengths, offsets=torch.tensor(off, dtype=I32, device=dev), out=buf[10:50])
         assert bool((buf[:10] == 7.0).all() and (buf[50:] == 7.0).all())
+    for B in (65, 700):
+        many, lens = table[:1].repeat(B, 1), lengths[:1].repeat(B)
+        for lo, hi in ((-50, 100), (0, 40), (1 << 30, (1 << 31) - 1), (-(1 << 31), 0)):
+            off = torch.randint(lo, hi, (B + 1,), generator=g, device=dev).to(I32)
+            for offsets in (off, off.sort(descending=True).values, off.sort().values):
+                ops.cache_attention(q, cache, many, lens, offsets=offsets, causal=True, out=buf[10:50])
+                assert bool((buf[:10] == 7.0).all() and (buf[50:] == 7.0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,most,Hq,Hk,D", [(65, 1, 4, 4, 64), (300, 3, 8, 2, 128), (4100, 1, 2, 2, 64), (130, 40, 10, 5, 128),
+                                            (70, 300, 4, 2, 64)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_of_many_ragged_sequences(dev, B, most, Hq, Hk, D, causal):
+    g, dt, page, r = _gen(dev, 30), torch.bfloat16, 16, random.Random(B)
+    rows = [r.choice([0, 1, most, r.randint(0, most)]) for _ in range(B)]
+    lens = [n + r.choice([0, 0, 5, 90]) for n in rows]
+    rows[-1], lens[-1] = 0, 30
+    pages, table = _pages(g, lens, page)
+    cache = _cache(g, pages, page, Hk, D, dt)
+    T = sum(rows)
+    q = _randn(g, T + 3, Hq, D).to(dt)
+    offsets = torch.tensor([0] + rows, device=dev).cumsum(0).to(I32)
+    buf = torch.full((T + 3, Hq, D), 7.0, device=dev, dtype=dt)
+    out, lse = ops.cache_attention(q, cache, table, torch.tensor(lens, dtype=I32, device=dev), offsets=offsets,
+                                   causal=causal, out=buf, return_lse=True)
+    qs = [q[a:a + n] for a, n in zip(offsets.tolist(), rows)]
+    _check_attention(out[:T], lse[:T], attention_ref(qs, cache, table, lens, rows, causal=causal))
+    assert bool((buf[T:] == 7.0).all())
 
 
 @pytest.mark.gpu

@@ -206,6 +206,31 @@ __device__ inline bool ca_item(const CacheArgs& A, int& part, int& parts, int& k
     ca_sequence(A, b, x);
     return blocks(x) * ca_parts(A, x.L);
   };
+  if (A.offsets && A.S == 1 && A.B > 64) {
+    // (to count many sequences would take longer than a work-group's own part: 4,096 of one token over 200
+    // keys 3.3 ms.  Sequence b owns row blocks from offsets[b] G / ROWS + b on, which is at least as many as
+    // it needs, and the lanes look for the last one that starts no later)
+    const long long tiles = (long long)A.T * A.G / ROWS + A.B;
+    const int all = (int)(tiles * A.HK), per = (all + 7) / 8, in = (int)(blockIdx.x >> 3);
+    const int id = (int)(blockIdx.x & 7) * per + in;
+    if (in >= per || id >= all) return false;
+    kh = id / (int)tiles;
+    const int local = id - kh * (int)tiles;
+    auto start = [&](int b) { return (long long)min(max(A.offsets[b], 0), A.T) * A.G / ROWS + b; };
+    int lo = 0, n = A.B;
+    while (n > 1) {
+      const int step = (n + 63) / 64, at = lane * step;
+      const bool on = at < n && start(lo + min(at, n - 1)) <= local;
+      const int started = __popcll(__ballot(on)), skip = max(started - 1, 0) * step;
+      lo += skip, n = min(step, n - skip);
+    }
+    ca_sequence(A, lo, w);
+    const long long tile = local - start(lo);
+    const int n_blocks = blocks(w);
+    part = 0, parts = 1;
+    w.r0 = (int)(A.causal ? n_blocks - 1 - tile : tile) * ROWS;
+    return tile >= 0 && tile < n_blocks;
+  }
   const bool alike = !A.offsets && A.S == 1;
   long long each = 0;  // items of a key head
   if (alike)

@@ -1661,7 +1661,7 @@ def cache_attention(q, cache, page_table, lengths, *, offsets=None, mask=None, c
             raise ValueError("t2t: a mask and causal")
         if (not isinstance(mask, torch.Tensor) or mask.dtype != torch.bool or mask.device != dev
                 or mask.dim() != len(lead) + 1 or tuple(mask.shape[:-1]) != lead
-                or (mask.shape[-1] > 1 and mask.stride(-1) != 1)):
+                or (mask.shape[-1] > 1 and mask.stride(-1) != 1) or mask.shape[-1] >= 2 ** 31):
             raise ValueError(f"t2t: mask must be a bool {[*lead, 'columns']} tensor on {dev} with contiguous rows")
     if scale is None:
         scale = D ** -0.5
