@@ -87,7 +87,7 @@ def test_workspace_bytes():
     assert f(0, 0, 1, 1, 40, 8, 128, 100) == 0               # one part
     assert f(0, 0, 1, 4680, 40, 40, 128, 32768) == 0         # enough rows
     one = f(0, 0, 1, 1, 40, 8, 128, 1 << 16)
-    assert one >= 2 * 40 * 130 * 4 and one % (40 * 130 * 4) == 0
+    assert one >= 2 * 40 * 130 * 4 and one % (40 * 130 * 4) == 16  # parts, and their size
     assert f(0, 0, 0, 0, 40, 8, 128, 100) == 0 and f(1, 0, 4, 61, 32, 8, 64, 20000) > 0
     assert f(0, 1, 1, 8192, 8, 8, 128, 8192) > f(0, 0, 1, 8192, 8, 8, 128, 8192) == 0  # row blocks that differ
 
@@ -757,6 +757,47 @@ def test_attention_offsets_that_are_no_offsets(dev):
             for offsets in (off, off.sort(descending=True).values, off.sort().values):
                 ops.cache_attention(q, cache, many, lens, offsets=offsets, causal=True, out=buf[10:50])
                 assert bool((buf[:10] == 7.0).all() and (buf[50:] == 7.0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,N,Hq,Hk,D,ragged", [(1, 1, 8, 8, 128, False), (16, 1, 40, 8, 128, False), (16, 2, 8, 2, 64, True),
+                                                (70, 1, 8, 8, 64, False), (70, 1, 16, 8, 128, True), (3, 61, 8, 2, 128, True),
+                                                (5, 200, 4, 4, 64, False)])
+def test_attention_of_unequal_lengths_in_a_captured_call(dev, B, N, Hq, Hk, D, ragged):
+    """One long sequence among short ones, tables much wider than they are (behind them entries
+    outside the cache), lengths that change from replay to replay, an empty sequence."""
+    g, dt, page, W = _gen(dev, 31), torch.bfloat16, 16, 700
+    cache = _cache(g, 900, page, Hk, D, dt)
+    q = _randn(g, B, N, Hq, D).to(dt)
+    kw = dict(offsets=torch.arange(0, B * N + 1, N, device=dev, dtype=I32)) if ragged else {}
+    x = q.flatten(0, 1) if ragged else q
+    table = torch.empty(B, W, dtype=I32, device=dev)
+    lengths = torch.empty(B, dtype=I32, device=dev)
+    r = random.Random(B)
+
+    def fill(longest):
+        lens = [r.choice([1, 0, 7, 64, 65, 300]) for _ in range(B)]
+        lens[r.randrange(B)] = longest
+        lengths.copy_(torch.tensor(lens, dtype=I32))
+        table.copy_(torch.randint(0, 900, (B, W), generator=g, device=dev))
+        table.masked_fill_(torch.arange(W, device=dev)[None] * page >= lengths[:, None], -1)
+        return lens
+    fill(500)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        ops.cache_attention(x, cache, table, lengths, **kw)
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out, lse = ops.cache_attention(x, cache, table, lengths, return_lse=True, **kw)
+    torch.cuda.synchronize()
+    for longest in (11000, 1, 4097, 640):
+        lens = fill(longest)
+        graph.replay()
+        torch.cuda.synchronize()
+        _check_attention(out, lse, attention_ref(q, cache, table, lens, [N] * B))
+        again, lse2 = ops.cache_attention(x, cache, table, lengths, return_lse=True, **kw)
+        assert torch.equal(again, out) and torch.equal(lse2, lse)
 
 
 @pytest.mark.gpu

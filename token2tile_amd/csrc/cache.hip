@@ -43,16 +43,21 @@ struct CacheArgs {
   long long table_row, mask_batch, mask_row;
   int B, N, T, HQ, HK, G, pages, page, shift, width, mask_cols, causal;
   float c;  // scale log2(e)
-  int S, part;  // most parts of a sequence's keys, keys of one
+  int S, target;  // most parts of a sequence's keys; work-groups of a key head that are aimed at
   float* opart;
   float* mlpart;
+  int* size;  // keys of a part, as the launch has found it
 };
 
-// Parts that a sequence of L keys goes in: of one size, that of the table's keys in S parts, so that all
-// work-groups have about the same to do; CA_PART keys at least (a tile of each of two waves).
+// A sequence's keys go in parts of one size, so that all work-groups have about the same to do. The
+// launch finds the size from the lengths themselves (ca_part): a table is as wide as its longest
+// sequence may become, above all in a captured graph, and lengths differ (single tokens of 40 heads over
+// 8, parts by the lengths and by the table's width: one of 4,000 keys in a table for 65,536 14.1 and 26.6
+// us, one of 32,000 keys and fifteen of 1,000 50 and 207; with equal lengths it costs 0.5). CA_PART keys
+// at least, a tile of each of two waves.
 #define CA_PART 64
 #define CA_SPAN 256  // columns of a mask from which on the many-row form searches it
-__device__ inline int ca_parts(const CacheArgs& A, int L) { return L < 1 ? 1 : (L - 1) / A.part + 1; }
+__device__ inline int ca_parts(int size, int L) { return L < 1 ? 1 : (L - 1) / size + 1; }
 
 // A work-group's rows: a row block of ROWS packed rows (token, head of the group) of a sequence.
 struct CacheRows {
@@ -190,6 +195,57 @@ struct CacheSight {
   }
 };
 
+// Row blocks and keys of the sequences, a lane each, 64 at a time; up to 64 are loaded once.
+template <int ROWS> struct CacheBatch {
+  const CacheArgs& A;
+  int n, L;
+  __device__ CacheBatch(const CacheArgs& a) : A(a), n(0), L(0) {
+    if (A.B <= 64) load(0);
+  }
+  __device__ void load(int b0) {
+    const int b = b0 + (int)__lane_id();
+    n = L = 0;
+    if (b >= A.B) return;
+    CacheRows w;
+    ca_sequence(A, b, w);
+    n = (w.rows + ROWS - 1) / ROWS, L = w.L;
+  }
+  __device__ void at(int b0) {
+    if (A.B > 64) load(b0);
+  }
+};
+// Keys of a part: the smallest size (in CA_PART keys, to a sixteenth) at which the row blocks' parts are
+// no more than the launch aims at, and a sequence's no more than the workspace has room for.
+template <int ROWS> __device__ inline int ca_part(CacheBatch<ROWS>& s) {
+  const CacheArgs& A = s.A;
+  if (A.S == 1) return INT_MAX;
+  auto units = [&]() { return max(s.L - 1, 0) / CA_PART + 1; };
+  // over the lanes; past 2^23 a lane's is enough to be too many (a launch has fewer work-groups)
+  auto all = [&](int x) { return wave_sum((int)min((long long)s.n * x, 1ll << 23)); };
+  int total = 0, hi = 1;
+  for (int b0 = 0; b0 < A.B; b0 += 64) {
+    s.at(b0);
+    total = min(total + all(units()), 1 << 30);
+    hi = max(hi, __builtin_amdgcn_readlane(wave_incl_max(s.n ? units() : 0), 63));
+  }
+  auto fits = [&](int p) {
+    int parts = 0;
+    for (int b0 = 0; b0 < A.B; b0 += 64) s.at(b0), parts = min(parts + all((units() + p - 1) / p), 1 << 30);
+    return parts <= A.target;
+  };
+  int lo = max(min((total - 1) / A.target + 1, hi), max((hi - 1) / A.S + 1, 1));
+  if (lo < hi && !fits(lo)) {
+    ++lo;
+    while (hi - lo > lo / 16) {
+      const int mid = lo + (hi - lo) / 2;
+      if (fits(mid)) hi = mid;
+      else lo = mid + 1;
+    }
+    lo = hi;
+  }
+  return lo * CA_PART;
+}
+
 // Which key head, sequence, part and row block a work-group takes.  Those that there are (row blocks
 // times parts of every sequence, which the lanes count) come without gaps, so that the launch's spare
 // work-groups are its last: dealt among the others, they left CUs without work while others had two.
@@ -200,12 +256,6 @@ template <int ROWS>
 __device__ inline bool ca_item(const CacheArgs& A, int& part, int& parts, int& kh, CacheRows& w) {
   const int lane = __lane_id();
   auto blocks = [&](const CacheRows& x) { return (x.rows + ROWS - 1) / ROWS; };
-  auto items = [&](int b) {
-    if (b >= A.B) return 0;
-    CacheRows x;
-    ca_sequence(A, b, x);
-    return blocks(x) * ca_parts(A, x.L);
-  };
   if (A.offsets && A.S == 1 && A.B > 64) {
     // (to count many sequences would take longer than a work-group's own part: 4,096 of one token over 200
     // keys 3.3 ms.  Sequence b owns row blocks from offsets[b] G / ROWS + b on, which is at least as many as
@@ -233,10 +283,15 @@ __device__ inline bool ca_item(const CacheArgs& A, int& part, int& parts, int& k
   }
   const bool alike = !A.offsets && A.S == 1;
   long long each = 0;  // items of a key head
-  if (alike)
+  CacheBatch<ROWS> s(A);
+  int size = INT_MAX;
+  if (alike) {
     each = (long long)A.B * (((long long)A.N * A.G + ROWS - 1) / ROWS);
-  else
-    for (int b0 = 0; b0 < A.B; b0 += 64) each += wave_sum(items(b0 + lane));
+  } else {
+    size = ca_part(s);
+    for (int b0 = 0; b0 < A.B; b0 += 64) s.at(b0), each += wave_sum(s.n * ca_parts(size, s.L));
+    if (A.S > 1 && blockIdx.x == 0 && threadIdx.x == 0) *A.size = size;
+  }
   if (each * A.HK > gridDim.x) return false;  // (offsets that go back, whose sequences overlap)
   const int all = (int)(each * A.HK), per = (all + 7) / 8, in = (int)(blockIdx.x >> 3);
   const int id = (int)(blockIdx.x & 7) * per + in;
@@ -248,7 +303,8 @@ __device__ inline bool ca_item(const CacheArgs& A, int& part, int& parts, int& k
     b = local / n, local -= b * n;
   } else {
     for (int b0 = 0; b0 < A.B; b0 += 64) {
-      const int n = items(b0 + lane), end = wave_incl_scan(n), sum = __builtin_amdgcn_readlane(end, 63);
+      s.at(b0);
+      const int n = s.n * ca_parts(size, s.L), end = wave_incl_scan(n), sum = __builtin_amdgcn_readlane(end, 63);
       if (local < sum) {  // (the same for the wave)
         const int at = __ffsll((unsigned long long)__ballot(end > local)) - 1;
         b = b0 + at;
@@ -258,9 +314,10 @@ __device__ inline bool ca_item(const CacheArgs& A, int& part, int& parts, int& k
       local -= sum;
     }
   }
-  ca_sequence(A, b, w);
+  ca_sequence(A, __builtin_amdgcn_readfirstlane(b), w);
+  local = __builtin_amdgcn_readfirstlane(local), kh = __builtin_amdgcn_readfirstlane(kh);
   const int n = blocks(w), tile = local % n;
-  part = local / n, parts = ca_parts(A, w.L);
+  part = local / n, parts = ca_parts(size, w.L);
   w.r0 = (A.causal ? n - 1 - tile : tile) * ROWS;
   return true;
 }
@@ -577,6 +634,7 @@ __device__ inline void ca_span(const uint8_t* rows, long long stride, int count,
   first = cols, last = 0;
 #pragma unroll
   for (int x = 0; x < W; ++x) first = min(first, sFirst[x]), last = max(last, sLast[x]);
+  first = __builtin_amdgcn_readfirstlane(first), last = __builtin_amdgcn_readfirstlane(last);
 }
 
 // ---- many rows: a work-group's waves share the keys --------------------------
@@ -635,8 +693,8 @@ __global__ __launch_bounds__(64 * W, 2) void ca_many_kernel(CacheArgs A) {
   const int keys = A.causal ? min(w.L, w.first + tok1 + 1) : w.L;
   int plain = max(0, A.mask ? w.first : A.causal ? w.first + tok0 + 1 : w.L);
   const int all = max(0, (keys + 63) / 64);
-  const int t0 = (int)((long long)part * all / parts);
-  int nt = (int)((long long)(part + 1) * all / parts) - t0;
+  const int t0 = __builtin_amdgcn_readfirstlane((int)((long long)part * all / parts));
+  int nt = __builtin_amdgcn_readfirstlane((int)((long long)(part + 1) * all / parts)) - t0;
   const int cols = min(A.mask_cols, w.n);
   if (A.mask && 64 * (t0 + nt) > w.first) {
     __shared__ int sFirst[W], sLast[W];
@@ -657,6 +715,7 @@ __global__ __launch_bounds__(64 * W, 2) void ca_many_kernel(CacheArgs A) {
     const int e0 = nf > 0 ? 64 * t0 / A.page : 0, e1 = nf > 0 ? (64 * (t0 + nf) - 1) / A.page : -1;
     for (int e = e0 + threadIdx.x; e <= e1; e += 64 * W) bad |= (uint32_t)table[e] >= (uint32_t)A.pages;
     if (__syncthreads_or(bad)) nf = 0;
+    nf = __builtin_amdgcn_readfirstlane(nf);
   }
 
   // this wave fetches keys KW wave .. of every tile; lane l looks key l % KW up
@@ -1015,7 +1074,7 @@ __global__ __launch_bounds__(256) void ca_combine_kernel(CacheArgs A) {
   const int kh = blockIdx.x % A.HK, tile = blockIdx.x / A.HK, lane = threadIdx.x & 31;
   CacheRows w;
   if (!ca_rows<ROWS>(A, tile, w)) return;
-  const int parts = ca_parts(A, w.L), r = w.r0 + 8 * blockIdx.y + (threadIdx.x >> 5);
+  const int parts = min(ca_parts(max(*A.size, 1), w.L), A.S), r = w.r0 + 8 * blockIdx.y + (threadIdx.x >> 5);
   if (parts < 2 || r >= w.rows) return;  // (its work-group has written the rows)
   const int tok = r / A.G, head = kh * A.G + r - tok * A.G;
   const long long at = (w.row0 + tok) * A.HQ + head, step = (long long)A.T * A.HQ;
@@ -1095,15 +1154,15 @@ static long long ca_full(int block, int ragged, int B, long long T, int G) {
   return ragged ? (n > B ? n : B) : ca_tiles(block, ragged, B, T, G);
 }
 struct CachePlan {
-  int block, S;
+  int block, S, target;
 };
-static CachePlan ca_plan(int ragged, int B, long long T, int HQ, int HK, long long keys, int causal) {
+static CachePlan ca_plan(int ragged, int B, long long T, int HQ, int HK, long long keys, int D, int causal) {
   const int G = HQ / HK;
   // (of a ragged batch: twice the mean, as its sequences are not known to the host)
   long long rows = (T + B - 1) / B * G * (ragged ? 2 : 1);
   if (rows > T * G) rows = T * G;
   const long long parts = (keys + CA_PART - 1) / CA_PART, most = parts < 1 ? 1 : parts < 64 ? parts : 64;
-  CachePlan best{rows <= 32 ? 32 : 128, 1};
+  CachePlan best{rows <= 32 ? 32 : 128, 1, 0};
   // (what a row block sees on average, of the keys)
   const double mean = causal ? 1.0 - 0.5 * (double)rows / G / (double)(keys > rows / G ? keys : rows / G) : 1.0;
   double least = 0.0;
@@ -1113,16 +1172,26 @@ static CachePlan ca_plan(int ragged, int B, long long T, int HQ, int HK, long lo
       const long long S = i < 3 ? i + 1 : (i - 2) * slots / 8 / wgs;
       if (S < 1 || S > most) continue;
       const double us = ca_time(block, wgs, (int)S, (double)keys, (double)T * HQ, mean);
-      if (least == 0.0 || us < least) least = us, best = CachePlan{block, (int)S};
+      if (least == 0.0 || us < least) least = us, best = CachePlan{block, (int)S, 0};
     }
+  }
+  // work-groups of a key head; the parts' number goes by them, and a long sequence among short ones may
+  // take more than its share
+  const long long full = ca_full(best.block, ragged, B, T, G);
+  best.target = (int)(best.S * full);
+  if (B > 1 && (best.S > 1 || (best.block == 32 && full * HK < 2048 && keys >= 2048))) {
+    // (where there are enough without parts, a round more of them for the long sequences')
+    const long long room = (32 << 20) / (T * HQ * (D + 2) * 4);
+    if (best.S == 1) best.target += 512 / HK;
+    if (room > best.S) best.S = (int)(room < most ? room : most);
   }
   return best;
 }
-static size_t ca_ws(int S, long long rows, int D) { return S < 2 ? 0 : (size_t)S * rows * (D + 2) * 4; }
+static size_t ca_ws(int S, long long rows, int D) { return S < 2 ? 0 : (size_t)S * rows * (D + 2) * 4 + 16; }
 
 extern "C" size_t t2t_cache_attention_ws_bytes(int ragged, int causal, int B, long long T, int HQ, int HK, int D, long long keys) {
   if (B < 1 || T < 1 || HK < 1 || HQ < HK || keys < 1) return 0;
-  return ca_ws(ca_plan(ragged, B, T, HQ, HK, keys, causal).S, T * HQ, D);
+  return ca_ws(ca_plan(ragged, B, T, HQ, HK, keys, D, causal).S, T * HQ, D);
 }
 
 extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -1164,7 +1233,7 @@ extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, 
   A.c = a->scale * 1.4426950408889634f;
   const int ragged = a->offsets != nullptr;
   const long long keys = (long long)a->width * a->page_size;
-  const CachePlan plan = ca_plan(ragged, a->B, T, a->HQ, a->HK, keys, a->causal);
+  const CachePlan plan = ca_plan(ragged, a->B, T, a->HQ, a->HK, keys, a->D, a->causal);
   const int block = plan.block;
   const long long tiles = ca_tiles(block, ragged, a->B, T, A.G);
   A.S = plan.S;
@@ -1174,13 +1243,16 @@ extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, 
     T2T_REQUIRE((uintptr_t)ws % 16 == 0, "cache_attention: workspace must be 16-byte aligned");
     A.opart = (float*)ws;
     A.mlpart = A.opart + (size_t)A.S * T * a->HQ * a->D;
+    A.size = (int*)(A.mlpart + (size_t)A.S * T * a->HQ * 2);
   }
-  A.part = A.S > 1 ? (int)((keys + A.S - 1) / A.S) : INT_MAX;
-  if (tiles * a->HK * A.S > (1 << 22)) {  // 2^31 threads
+  A.target = plan.target;
+  // (no more work-groups have anything to do: ca_part's, or one part for every row block)
+  const long long most = (A.S > 1 && A.target > tiles ? A.target : tiles) * a->HK;
+  if (most > (1 << 22)) {  // 2^31 threads
     t2t_set_error("cache_attention: %lld row blocks of %d heads", tiles, a->HK);
     return T2T_ERR_UNSUPPORTED;
   }
-  const int items = (int)(tiles * a->HK * A.S);
+  const int items = (int)most;
   // sixteen keys from a multiple of sixteen on lie in one page, at 32-bit offsets
   const bool p16 = a->page_size % 16 == 0 && A.kv_row < (1 << 27);
   auto run = [&](auto t, auto d) {
