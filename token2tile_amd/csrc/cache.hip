@@ -1133,15 +1133,18 @@ __global__ __launch_bounds__(256) void ca_combine_kernel(CacheArgs A) {
 // The estimate: a key of a work-group takes the longer the more run beside it (they share the memory
 // and the power); the constants are fitted to such measurements.
 // Under causal the first row blocks see few keys: the longest work-group's time, or their mean's over
-// all rounds (8,192 rows over as many keys, 8 heads: S = 1: 193 us, 2: 170).
-static double ca_time(int block, long long wgs, int S, double keys, double rows, double mean) {
+// all rounds (8,192 rows over as many keys, 8 heads: S = 1: 193 us, 2: 170).  Tiles with hidden keys
+// are not pipelined: `extra` us a work-group, more with more rows, so that short sequences under a mask
+// go by 128 (653 rows over as many keys, 27 x 40 heads, D = 64, 128 and 256: plain 272 and 279, causal 235
+// and 279, frames 423 and 542; 4,096 rows in frames over 8,192 keys, 16: 255 and 242).
+static double ca_time(int block, long long wgs, int S, double keys, double rows, double mean, double extra) {
   const int slots = block == 256 ? 256 : 512;  // work-groups at once
   auto key = [&](long long n) { return block == 32 ? 22e-3 + 45e-6 * n : block == 128 ? 14e-3 + 30e-6 * n : 20e-3 + 20e-6 * n; };
   const long long n = wgs * S, full = n / slots, rest = n % slots;
-  const double part = 64.0 * (long long)((keys / S + 63) / 64), start = block == 256 ? 3.5 : 2.0;
+  const double part = 64.0 * (long long)((keys / S + 63) / 64), start = (block == 256 ? 5.0 : 2.5) + extra;
   double us = (double)full * (part * key(slots) + start);
   if (rest) us += part * key(rest) + start;
-  if (mean < 1.0 && full) us = part * key(slots) * (mean * n > slots ? mean * n / slots : 1.0) + start;
+  if (mean < 1.0 && full) us = part * key(slots) * (mean * n > slots ? mean * n / slots : 1.0) + start * n / slots;
   return S < 2 ? us : us + 3.0 + 0.1 * S + 0.23e-3 * S * rows;  // (the join: launched, its loads, its bytes)
 }
 // row blocks of `block` packed rows
@@ -1156,7 +1159,7 @@ static long long ca_full(int block, int ragged, int B, long long T, int G) {
 struct CachePlan {
   int block, S, target;
 };
-static CachePlan ca_plan(int ragged, int B, long long T, int HQ, int HK, long long keys, int D, int causal) {
+static CachePlan ca_plan(int ragged, int B, long long T, int HQ, int HK, long long keys, int D, int hidden) {
   const int G = HQ / HK;
   // (of a ragged batch: twice the mean, as its sequences are not known to the host)
   long long rows = (T + B - 1) / B * G * (ragged ? 2 : 1);
@@ -1164,14 +1167,16 @@ static CachePlan ca_plan(int ragged, int B, long long T, int HQ, int HK, long lo
   const long long parts = (keys + CA_PART - 1) / CA_PART, most = parts < 1 ? 1 : parts < 64 ? parts : 64;
   CachePlan best{rows <= 32 ? 32 : 128, 1, 0};
   // (what a row block sees on average, of the keys)
-  const double mean = causal ? 1.0 - 0.5 * (double)rows / G / (double)(keys > rows / G ? keys : rows / G) : 1.0;
+  const double mean = hidden == 1 ? 1.0 - 0.5 * (double)rows / G / (double)(keys > rows / G ? keys : rows / G) : 1.0;
   double least = 0.0;
   for (int block = best.block; block <= (rows <= 128 ? best.block : 256); block *= 2) {
     const long long wgs = ca_full(block, ragged, B, T, G) * HK, slots = block == 256 ? 256 : 512;
+    const double fresh = (double)(rows / G) / 600.0, wide = block == 256 ? 1.0 : 0.0;
+    const double extra = block == 32 || !hidden ? 0.0 : (hidden == 1 ? 7.0 + 1.5 * wide : 20.0 + 7.0 * wide) * (fresh < 1.0 ? fresh : 1.0);
     for (int i = 0; i < 11; ++i) {  // 1, 2, 3 and eighths of all that run at once
       const long long S = i < 3 ? i + 1 : (i - 2) * slots / 8 / wgs;
       if (S < 1 || S > most) continue;
-      const double us = ca_time(block, wgs, (int)S, (double)keys, (double)T * HQ, mean);
+      const double us = ca_time(block, wgs, (int)S, (double)keys, (double)T * HQ, mean, extra);
       if (least == 0.0 || us < least) least = us, best = CachePlan{block, (int)S, 0};
     }
   }
@@ -1189,9 +1194,10 @@ static CachePlan ca_plan(int ragged, int B, long long T, int HQ, int HK, long lo
 }
 static size_t ca_ws(int S, long long rows, int D) { return S < 2 ? 0 : (size_t)S * rows * (D + 2) * 4 + 16; }
 
-extern "C" size_t t2t_cache_attention_ws_bytes(int ragged, int causal, int B, long long T, int HQ, int HK, int D, long long keys) {
+extern "C" size_t t2t_cache_attention_ws_bytes(int ragged, int hidden, int B, long long T, int HQ, int HK, int D,
+                                               long long keys) {
   if (B < 1 || T < 1 || HK < 1 || HQ < HK || keys < 1) return 0;
-  return ca_ws(ca_plan(ragged, B, T, HQ, HK, keys, D, causal).S, T * HQ, D);
+  return ca_ws(ca_plan(ragged, B, T, HQ, HK, keys, D, hidden).S, T * HQ, D);
 }
 
 extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -1233,7 +1239,7 @@ extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, 
   A.c = a->scale * 1.4426950408889634f;
   const int ragged = a->offsets != nullptr;
   const long long keys = (long long)a->width * a->page_size;
-  const CachePlan plan = ca_plan(ragged, a->B, T, a->HQ, a->HK, keys, a->D, a->causal);
+  const CachePlan plan = ca_plan(ragged, a->B, T, a->HQ, a->HK, keys, a->D, a->causal ? 1 : a->mask ? 2 : 0);
   const int block = plan.block;
   const long long tiles = ca_tiles(block, ragged, a->B, T, A.G);
   A.S = plan.S;

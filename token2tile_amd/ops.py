@@ -1593,12 +1593,12 @@ def cache_append(q, k, v, cos, sin, cache, slots, *, layout="interleaved", norm=
     return oq
 
 
-def cache_attention_ws_bytes(B, T, Hq, cache, width, ragged=False, causal=False):
+def cache_attention_ws_bytes(B, T, Hq, cache, width, ragged=False, causal=False, masked=False):
     """Workspace of cache_attention for T rows in all of B sequences (``ragged``: with
-    offsets) whose page tables are ``width`` pages wide."""
+    offsets; ``masked``: with a mask) whose page tables are ``width`` pages wide."""
     k = cache._k
-    return _sizes_of("t2t_cache_attention_ws_bytes", bool(ragged), bool(causal), B, T, Hq, k.shape[2], k.shape[3],
-                     width * k.shape[1])
+    return _sizes_of("t2t_cache_attention_ws_bytes", bool(ragged), 1 if causal else 2 if masked else 0, B, T, Hq,
+                     k.shape[2], k.shape[3], width * k.shape[1])
 
 
 def cache_attention(q, cache, page_table, lengths, *, offsets=None, mask=None, causal=False, scale=None,
@@ -1679,7 +1679,7 @@ def cache_attention(q, cache, page_table, lengths, *, offsets=None, mask=None, c
             raise ValueError("t2t: out holds an element twice")
     os = qs if out is None and q.is_contiguous() else _attn_strides(o, "out")
     lse = _empty(stream, (*lead, Hq), _f32, dev) if return_lse else None
-    need = cache_attention_ws_bytes(B, T, Hq, cache, width, ragged, causal) if T and B else 0
+    need = cache_attention_ws_bytes(B, T, Hq, cache, width, ragged, causal, mask is not None) if T and B else 0
     given = ws is not None
     if given:
         ws = _ws_for(ws, need, dev, stream)
