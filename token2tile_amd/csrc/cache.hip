@@ -586,48 +586,54 @@ __device__ inline void ca_mfma_score(f32x16& c, const u32x4& a, const u32x4& b) 
 
 // The new tokens that all of a work-group's tokens tok0 .. tok1 see, up to the first that one does not,
 // and one behind the last that any sees: columns of the mask's rows at `rows`, of cols >= 16.  A wave
-// takes every W-th row, eight at once, and a KB of each from either end until it has met its column.
+// takes every W-th row, sixteen at once, and a KB of each from either end until it has met its column.
 template <int W>
 __device__ inline void ca_span(const uint8_t* rows, long long stride, int count, int cols, int (&sFirst)[W],
                                int (&sLast)[W], int& first, int& last) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   auto flags = [](uint32_t x) { return (((x & 0x7f7f7f7fu) + 0x7f7f7f7fu) | x) & 0x80808080u; };  // of bytes that are not 0
-  auto gather = [&](int col, uint32_t (&f)[4], auto ALL) {
-    for (int r = wave; r < count; r += 8 * W) {
-      u32x4 x[8];
+  constexpr int AT_ONCE = 16;
+  auto gather = [&](int col, uint32_t (&every)[4], uint32_t (&any)[4]) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) __builtin_memcpy(&x[i], rows + min(r + i * W, count - 1) * stride + col, 16);
+    for (int e = 0; e < 4; ++e) every[e] = ~0u, any[e] = 0u;
+    for (int r = wave; r < count; r += AT_ONCE * W) {
+      u32x4 x[AT_ONCE];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < AT_ONCE; ++i) __builtin_memcpy(&x[i], rows + min(r + i * W, count - 1) * stride + col, 16);
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t y = flags(x[i][e]);
-          f[e] = decltype(ALL)::value ? f[e] & y : f[e] | y;
+          every[e] &= y, any[e] |= y;
         }
     }
   };
   int lo = cols, hi = 0;
+  uint32_t every[4], any[4];
+  auto behind = [&](int col) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (any[e]) hi = col + 4 * e + 4 - (__builtin_clz(any[e]) >> 3);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) hi = max(hi, __shfl_xor(hi, d, 64));
+  };
   for (int b = 0; b < cols && lo == cols; b += 1024) {
     const int col = min(b + 16 * lane, cols - 16);
-    uint32_t f[4] = {~0u, ~0u, ~0u, ~0u};
-    gather(col, f, std::true_type{});
+    gather(col, every, any);
 #pragma unroll
     for (int e = 3; e >= 0; --e) {
-      const uint32_t none = ~f[e] & 0x80808080u;
+      const uint32_t none = ~every[e] & 0x80808080u;
       if (none) lo = col + 4 * e + (__builtin_ctz(none) >> 3);
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) lo = min(lo, __shfl_xor(lo, d, 64));
+    if (cols <= 1024) behind(col);  // (all columns at once)
   }
-  for (int b = cols; b > 0 && hi == 0; b -= 1024) {
+  for (int b = cols; cols > 1024 && b > 0 && hi == 0; b -= 1024) {
     const int col = max(b - 1024 + 16 * lane, 0);
-    uint32_t f[4] = {0u, 0u, 0u, 0u};
-    gather(col, f, std::false_type{});
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (f[e]) hi = col + 4 * e + 4 - (__builtin_clz(f[e]) >> 3);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) hi = max(hi, __shfl_xor(hi, d, 64));
+    gather(col, every, any);
+    behind(col);
   }
   if (lane == 0) sFirst[wave] = lo, sLast[wave] = hi;
   __syncthreads();
@@ -983,10 +989,8 @@ __global__ __launch_bounds__(64 * W, 2) void ca_many_kernel(CacheArgs A) {
 #pragma unroll
           for (int g = 0; g < 4; ++g) raw[kb][g] = sight.peek(64 * (t0 + t) + 32 * kb + 8 * g + 4 * hh);
     };
-    auto hidden = [&](uint32_t seen, bool odd, const uint16_t* kt, const uint16_t* vt) __attribute__((always_inline)) {
-      f32x16 S;
+    auto hidden = [&](uint32_t seen, bool odd, f32x16& S, const uint16_t* vt) __attribute__((always_inline)) {
       u32x4 P[2];
-      scores(S, kt);
 #pragma unroll
       for (int a = 0; a < 16; ++a)
         if (!(seen >> (8 * (a / 4) + 4 * hh + a % 4) & 1)) S[a] = -__builtin_inff();
@@ -1033,13 +1037,29 @@ __global__ __launch_bounds__(64 * W, 2) void ca_many_kernel(CacheArgs A) {
 #pragma unroll
       for (int x = 0; x < W; ++x) bad[x / (W / 2)] |= sBad[t & 1][x] << (KW * (x % (W / 2))), odd |= sOdd[t & 1][x];
       if (t + 1 < nt) ask(t + 1);
-      if (live)
+      seen[0] &= ~bad[0], seen[1] &= ~bad[1];
+      if (!live) continue;
+      if constexpr (D == 128) {  // (no registers for both halves' scores)
 #pragma clang loop unroll(disable)
         for (int kb = 0; kb < 2; ++kb) {
-          const uint32_t see = (kb ? seen[1] : seen[0]) & ~(kb ? bad[1] : bad[0]);
-          if (__ballot(see != 0))
-            hidden(see, __builtin_amdgcn_readfirstlane(odd), at(sK, t) + 32 * kb * D, at(sV, t) + 32 * kb * D);
+          const uint32_t see = kb ? seen[1] : seen[0];
+          if (!__ballot(see != 0)) continue;
+          f32x16 S;
+          scores(S, at(sK, t) + 32 * kb * D);
+          hidden(see, __builtin_amdgcn_readfirstlane(odd), S, at(sV, t) + 32 * kb * D);
         }
+      } else if (__ballot((seen[0] | seen[1]) != 0)) {
+        f32x16 S[2];  // (of both halves in turn, as a product waits for the one before of its half)
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+            S[kb] = Mfma<T>::run(*(const u32x4*)(at(sK, t) + 32 * kb * D + kat(s)), q[s], s ? S[kb] : zero16());
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+          if (__ballot(seen[kb] != 0))
+            hidden(seen[kb], __builtin_amdgcn_readfirstlane(odd), S[kb], at(sV, t) + 32 * kb * D);
+      }
     }
   }
   if (!live) return;
@@ -1135,8 +1155,9 @@ __global__ __launch_bounds__(256) void ca_combine_kernel(CacheArgs A) {
 // Under causal the first row blocks see few keys: the longest work-group's time, or their mean's over
 // all rounds (8,192 rows over as many keys, 8 heads: S = 1: 193 us, 2: 170).  Tiles with hidden keys
 // are not pipelined: `extra` us a work-group, more with more rows, so that short sequences under a mask
-// go by 128 (653 rows over as many keys, 27 x 40 heads, D = 64, 128 and 256: plain 272 and 279, causal 235
-// and 279, frames 423 and 542; 4,096 rows in frames over 8,192 keys, 16: 255 and 242).
+// go by 128 (blocks of 128 and 256: 653 rows over as many keys, 27 x 40 heads, D = 64, plain 272 and 279,
+// causal 235 and 279; 3,306 rows in frames over as many, 3 x 24 heads, 405 and 457; 4,096 in frames over
+// 8,192, 16 heads, 255 and 242).
 static double ca_time(int block, long long wgs, int S, double keys, double rows, double mean, double extra) {
   const int slots = block == 256 ? 256 : 512;  // work-groups at once
   auto key = [&](long long n) { return block == 32 ? 22e-3 + 45e-6 * n : block == 128 ? 14e-3 + 30e-6 * n : 20e-3 + 20e-6 * n; };
@@ -1172,7 +1193,7 @@ static CachePlan ca_plan(int ragged, int B, long long T, int HQ, int HK, long lo
   for (int block = best.block; block <= (rows <= 128 ? best.block : 256); block *= 2) {
     const long long wgs = ca_full(block, ragged, B, T, G) * HK, slots = block == 256 ? 256 : 512;
     const double fresh = (double)(rows / G) / 600.0, wide = block == 256 ? 1.0 : 0.0;
-    const double extra = block == 32 || !hidden ? 0.0 : (hidden == 1 ? 7.0 + 1.5 * wide : 20.0 + 7.0 * wide) * (fresh < 1.0 ? fresh : 1.0);
+    const double extra = block == 32 || !hidden ? 0.0 : (hidden == 1 ? 7.0 + 1.5 * wide : 20.0 + 13.0 * wide) * (fresh < 1.0 ? fresh : 1.0);
     for (int i = 0; i < 11; ++i) {  // 1, 2, 3 and eighths of all that run at once
       const long long S = i < 3 ? i + 1 : (i - 2) * slots / 8 / wgs;
       if (S < 1 || S > most) continue;
