@@ -250,8 +250,11 @@ template <int ROWS> __device__ inline int ca_part(CacheBatch<ROWS>& s) {
 // times parts of every sequence, which the lanes count) come without gaps, so that the launch's spare
 // work-groups are its last: dealt among the others, they left CUs without work while others had two.
 // Consecutive work-groups go to the eight XCDs in turn: each takes a run of items, the row blocks of
-// one part and key head next to each other, which then share their keys in its L2.  (Under causal the
-// last row blocks, which see the most, go first.)
+// one part and key head next to each other, which then share their keys in its L2.  Under causal the
+// last row blocks, which see the most, go first: of a uniform batch without parts, and where there are
+// fewer key heads and sequences than XCDs, items are dealt one by one, all heads' and sequences' longest
+// before their next (8,184 tokens of 24 heads over one: 400 us, 580 in runs, of which an XCD had long ones
+// alone; 4 x 2,000 tokens of 16 heads 96 and 118; with as many heads as XCDs a head stays on its XCD).
 template <int ROWS>
 __device__ inline bool ca_item(const CacheArgs& A, int& part, int& parts, int& kh, CacheRows& w) {
   const int lane = __lane_id();
@@ -294,13 +297,19 @@ __device__ inline bool ca_item(const CacheArgs& A, int& part, int& parts, int& k
   }
   if (each * A.HK > gridDim.x) return false;  // (offsets that go back, whose sequences overlap)
   const int all = (int)(each * A.HK), per = (all + 7) / 8, in = (int)(blockIdx.x >> 3);
-  const int id = (int)(blockIdx.x & 7) * per + in;
+  const bool deal = A.causal && (alike || A.HK * A.B < 8);
+  const int id = deal ? (int)blockIdx.x : (int)(blockIdx.x & 7) * per + in;
   if (in >= per || id >= all) return false;
-  kh = id / (int)each;
-  int local = id - kh * (int)each, b = 0;
+  kh = deal ? id % A.HK : id / (int)each;
+  int local = deal ? id / A.HK : id - kh * (int)each, b = 0;
   if (alike) {
     const int n = (int)each / A.B;
-    b = local / n, local -= b * n;
+    if (deal) {
+      const int x = local / A.B;
+      b = local - x * A.B, local = x;
+    } else {
+      b = local / n, local -= b * n;
+    }
   } else {
     for (int b0 = 0; b0 < A.B; b0 += 64) {
       s.at(b0);
