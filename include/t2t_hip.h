@@ -589,8 +589,8 @@ typedef struct t2t_cache_attention_args {
   int B, N, HQ, HK, D, dtype, pages, page_size, width, mask_cols, causal;
   float scale;
 } t2t_cache_attention_args;
-/* hidden: 1 causal, 2 with a mask, else 0; T: rows of q in all; keys: width * page_size.  (With less, or none, a long
- * sequence's keys go to fewer work-groups.) */
+/* hidden: 1 causal, 2 with a mask, else 0; T: rows of q in all; keys: width *
+ * page_size.  (With less, or none, a long sequence's keys go to fewer work-groups.) */
 size_t t2t_cache_attention_ws_bytes(int ragged, int hidden, int B, long long T, int HQ, int HK, int D,
                                     long long keys);
 int t2t_cache_attention(const t2t_cache_attention_args* args, void* ws, size_t ws_bytes,
