@@ -231,6 +231,28 @@ def test_attention_refused(launches, bad):
     assert not launches
 
 
+def test_a_workspace_of_any_size_is_the_one_that_is_used(launches):
+    """A caller's workspace is passed on with its own byte count, never replaced."""
+    a = _attend_args(width=200)
+    need = ops.cache_attention_ws_bytes(3, 12, 4, a["cache"], 200)
+    buf = torch.zeros(need + 64, dtype=torch.uint8)
+    for n in (0, 1, need // 2, need - 1, need, need + 64):
+        ws = buf[:n]
+        ops.cache_attention(**a, ws=ws)
+        name, tensors, args = launches.pop()
+        assert args[1:] == (ws.data_ptr(), n) and any(t is ws for t in tensors)
+    with pytest.raises(ValueError, match="aligned"):
+        ops.cache_attention(**a, ws=buf[4:])
+    # a small one that shares memory with an input
+    a["q"] = buf[:6144].view(torch.bfloat16).view(3, 4, 4, 64)
+    with pytest.raises(ValueError, match="shares memory"):
+        ops.cache_attention(**a, ws=buf[6128:6160])
+    ops.cache_attention(**a, ws=buf[6144:6160])
+    short = _attend_args(width=1)  # (no workspace asked for: nothing of it is used)
+    assert ops.cache_attention_ws_bytes(3, 12, 4, short["cache"], 1) == 0
+    ops.cache_attention(**short, ws=buf[4:])
+
+
 @pytest.mark.parametrize("kind", ["k", "v", "page_table", "lengths", "offsets", "mask"])
 def test_an_output_apart_from_every_input(launches, kind):
     buf = torch.zeros(1 << 16, dtype=torch.uint8)
@@ -735,6 +757,34 @@ def test_attention_does_not_depend_on_the_company(dev, N, Hq, Hk):
     # an empty table
     got, lse = ops.cache_attention(q, cache, table[:, :0], far, return_lse=True)
     assert not bool(got.any()) and bool(torch.isneginf(lse).all())
+
+
+@pytest.mark.gpu  # (row blocks of 32, 128 and 256, each in several parts)
+@pytest.mark.parametrize("N,Hq,Hk,D,ragged", [(1, 8, 2, 128, False), (7, 4, 2, 64, True), (61, 8, 4, 128, True),
+                                              (100, 4, 4, 64, False), (500, 6, 6, 128, False), (500, 4, 4, 64, True)])
+def test_attention_with_any_workspace(dev, N, Hq, Hk, D, ragged):
+    """The whole workspace, one short of it, those of seven, three and two parts and none (one part): results
+    within the bounds, and nothing written outside the bytes that were given."""
+    g, dt, page, lens = _gen(dev, 41), torch.bfloat16, 64, [9000, 1, 5000]
+    pages, table = _pages(g, lens, page)
+    cache = _cache(g, pages, page, Hk, D, dt)
+    q = _randn(g, 3, N, Hq, D).to(dt)
+    lengths = torch.tensor(lens, dtype=I32, device=dev)
+    kw = dict(offsets=torch.arange(0, 3 * N + 1, N, device=dev, dtype=I32)) if ragged else {}
+    x = q.flatten(0, 1) if ragged else q
+    ref = attention_ref(q, cache, table, lens, [N] * 3)
+    need = ops.cache_attention_ws_bytes(3, 3 * N, Hq, cache, table.shape[1], ragged)
+    part = 3 * N * Hq * (D + 2) * 4
+    assert need >= 2 * part + 16
+    for n in (need, need - 1, 7 * part + 16, 3 * part + 16, 2 * part + 16, 2 * part + 15, 1, 0):
+        n = min(n, need)
+        buf = torch.full((n + 256,), 0xAB, dtype=torch.uint8, device=dev)
+        print(N, D, "workspace", n, flush=True)
+        out, lse = ops.cache_attention(x, cache, table, lengths, return_lse=True, ws=buf[:n], **kw)
+        _check_attention(out, lse, ref)
+        assert bool((buf[n:] == 0xAB).all())
+        if n < 2 * part + 16:
+            assert bool((buf == 0xAB).all())
 
 
 @pytest.mark.gpu

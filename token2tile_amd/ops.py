@@ -1624,7 +1624,8 @@ def cache_attention(q, cache, page_table, lengths, *, offsets=None, mask=None, c
     the type for the second product.  Returns out (of q's shape), or (out, lse) with
     the natural logarithms of the softmax's sums, fp32 [..., Hq].  ``out``: contiguous
     channels, 16-byte aligned rows; it and ``ws`` share no memory with another
-    argument."""
+    argument.  A ``ws`` (uint8, 16-byte aligned) is never replaced: with fewer bytes
+    than cache_attention_ws_bytes a long sequence's keys go to fewer work-groups."""
     ck, cv, dev = _cache_of(cache)
     _on(stream, dev)
     pages, page, Hk, D = ck.shape
@@ -1680,18 +1681,21 @@ def cache_attention(q, cache, page_table, lengths, *, offsets=None, mask=None, c
     os = qs if out is None and q.is_contiguous() else _attn_strides(o, "out")
     lse = _empty(stream, (*lead, Hq), _f32, dev) if return_lse else None
     need = cache_attention_ws_bytes(B, T, Hq, cache, width, ragged, causal, mask is not None) if T and B else 0
-    given = ws is not None
-    if given:
-        ws = _ws_for(ws, need, dev, stream)
+    held = 0  # bytes that the launch may use of a caller's workspace
+    if ws is not None:
+        ws = _ws_for(ws, 0, dev, stream)
+        held = min(need, ws.numel())
+        if held and ws.data_ptr() % 16:
+            raise ValueError("t2t: ws must be 16-byte aligned")
     elif need:
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if stream is None else _ws(need, dev, stream)
     ins = (q, ck, cv, page_table, lengths, offsets, mask)
     if out is not None:
         _apart((o,), ("out",), (None, *ins))
-    if given and need:
+    if held:
         at = ws.data_ptr()
-        if _near(at, at + need, [(p, e - p) for p, e in (_span(t) for t in (*ins, o) if t is not None)]):
-            _apart((ws[:need],), ("ws",), (None, *ins, o))
+        if _near(at, at + held, [(p, e - p) for p, e in (_span(t) for t in (*ins, o) if t is not None)]):
+            _apart((ws[:held],), ("ws",), (None, *ins, o))
     ms = mask.stride() if mask is not None else (0, 0, 0)
     args = _lib.CACHE_ATTENTION_ARGS.pack(
         _lib.CACHE_ATTENTION_ARGS.size, q.data_ptr(), ck.data_ptr(), cv.data_ptr(), o.data_ptr(),
