@@ -575,8 +575,9 @@ int t2t_cache_append(const t2t_rotary_tensor* q, const t2t_rotary_tensor* k,
  * lse (or NULL) [rows, HQ] fp32 contiguous: natural log of the softmax's sum, -inf
  * for rows that see nothing.  fp16 or bf16, D 64 or 128, all strides multiples of
  * 8 elements and pointers 16-byte aligned, one head's keys within 64 GiB; sums and
- * softmax in fp32, weights rounded to the type for the second product.  out and ws
- * share no memory with another argument. */
+ * softmax in fp32, weights rounded to the type for the second product.  Values
+ * up to 2^127 / keys and scores (scale q . k) up to 2^26 are in range: past these a row
+ * may hold anything.  out and ws share no memory with another argument. */
 typedef struct t2t_cache_attention_args {
   size_t struct_bytes; /* sizeof(t2t_cache_attention_args) */
   const void *q, *k, *v;

@@ -717,6 +717,52 @@ def test_attention_shifted_by_a_large_score(dev, N, causal):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("size", [2.0 ** 100, 2.0 ** -100])
+@pytest.mark.parametrize("N,L,D,kind", [(1, 900, 64, "all"), (1, 9000, 128, "all"), (40, 900, 128, "causal"),
+                                        (200, 900, 64, "mask"), (200, 9000, 128, "all"), (3000, 3000, 64, "causal")])
+def test_attention_of_large_and_small_values(dev, N, L, D, kind, size):
+    """Scores that rise by hundreds along the keys, over values far from 1 on either side: what is summed stays in
+    range (a weight's error and half steps are relative, so the bounds are those of ordinary values)."""
+    g, dt, page = _gen(dev, 4), torch.bfloat16, 16
+    pages, table = _pages(g, [L], page)
+    cache = _cache(g, pages, page, 2, D, dt)
+    cache.v.mul_(size)
+    at = torch.arange(L, device=dev)
+    cache.k[table[0, at // page].long(), at % page, :, 0] = (at * 45 // L).to(dt)[:, None]
+    q = (0.3 * _randn(g, 1, N, 2, D)).to(dt)
+    q[..., 0] = 40.0
+    lengths = torch.tensor([L], dtype=I32, device=dev)
+    mask = torch.rand(1, N, N, generator=g, device=dev) < 0.5 if kind == "mask" else None
+    out, lse = ops.cache_attention(q, cache, table, lengths, mask=mask, causal=kind == "causal", return_lse=True)
+    _check_attention(out, lse, attention_ref([q[0]], cache, table, [L], [N], mask, kind == "causal"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", HALF)
+@pytest.mark.parametrize("N,L", [(1, 1500), (3, 70), (200, 900), (3000, 3000)])
+def test_attention_of_scores_as_large_as_documented(dev, N, L, dt):
+    """Scores of up to 2^26 in magnitude, the same for all keys of a head: the mean of its values."""
+    g, dt, page, D = _gen(dev, 12), HALF[dt], 16, 64
+    pages, table = _pages(g, [L], page)
+    cache = _cache(g, pages, page, 4, D, dt)
+    cache.k.zero_()
+    cache.k[..., 0] = torch.tensor([2.0 ** 15, -2.0 ** 15, 2.0 ** 13, -2.0 ** 9], device=dev)
+    q = torch.zeros(1, N, 4, D, device=dev)
+    q[..., 0] = 2.0 ** 13 * (1 + torch.rand(1, N, 4, generator=g, device=dev))
+    q = q.to(dt)
+    lengths = torch.tensor([L], dtype=I32, device=dev)
+    out, lse = ops.cache_attention(q, cache, table, lengths, return_lse=True)
+    at = torch.arange(L, device=dev)
+    v = cache.v[table[0, at // page].long(), at % page].double()         # [L, 4, D]
+    mean = v.mean(0).expand_as(out[0])
+    # equal weights, half a step of the type off their sum; L fp32 additions; the result's half step
+    tol = mean.abs() * torch.finfo(dt).eps / 2 + (L + 80) * 2.0 ** -24 * v.abs().mean(0) + _half_step(mean, dt) * (1 + 2.0 ** -6)
+    assert bool(((out[0].double() - mean).abs() <= tol).all())
+    s = q[0, :, :, 0].double() * cache.k[0, 0, :, 0].double() / 8 + math.log(L)
+    assert bool(((lse[0].double() - s).abs() <= 2.0 ** -22 * s.abs() + 1e-3).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("scale", [1e-6, 0.02, 1.0])
 def test_attention_scales(dev, scale):
     g, dt, L = _gen(dev, 8), torch.bfloat16, 333

@@ -125,7 +125,10 @@ __device__ inline uint32_t ca_offset(const CacheArgs& A, uint32_t entry, int pos
 
 template <typename T> struct CaType;
 template <> struct CaType<BF16T> {
-  static constexpr float top = 0.f, limit = 0x1p64f;  // log2 of the largest weight, most of a tile's sum
+  // log2 of the largest weight as the maximum moves, and the most that a lane's weights of a half tile (16
+  // keys) may add up to before it moves again.  Weights are then 1 on average at most, so the sums stay
+  // below keys x max |v| (with 2^64 for the limit, values of 2^100 overflowed where scores rose by 45)
+  static constexpr float top = -10.f, limit = 16.f;
   static constexpr uint32_t inf = 0x7f80u;
 };
 template <> struct CaType<F16T> {
