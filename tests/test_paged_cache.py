@@ -92,6 +92,17 @@ def test_workspace_bytes():
     assert f(0, 1, 1, 8192, 8, 8, 128, 8192) > f(0, 0, 1, 8192, 8, 8, 128, 8192) == 0  # row blocks that differ
 
 
+def test_parts_where_they_help():
+    """Many sequences are counted by every work-group: no parts where those are many and the keys few."""
+    from token2tile_amd import _lib
+    f = _lib.lib().t2t_cache_attention_ws_bytes
+    for ragged in (0, 1):
+        for B, Hk, keys in ((64, 1, 1024), (128, 1, 1024), (256, 1, 1024), (400, 1, 4096), (128, 8, 4096), (1500, 1, 16384)):
+            assert f(ragged, 0, B, B, 8, Hk, 128, keys) > 0, (B, Hk, keys)
+        for B, Hk, keys in ((400, 1, 2048), (1024, 1, 4096), (2000, 1, 4096), (2000, 1, 16384), (400, 8, 4096), (400, 8, 16384)):
+            assert f(ragged, 0, B, B, 8, Hk, 128, keys) == 0, (B, Hk, keys)
+
+
 def test_cpu_tensors_are_refused():
     z = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="t2t"):
@@ -831,6 +842,32 @@ def test_attention_with_any_workspace(dev, N, Hq, Hk, D, ragged):
         assert bool((buf[n:] == 0xAB).all())
         if n < 2 * part + 16:
             assert bool((buf == 0xAB).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,N,Hq,Hk,D,W,kind", [
+    (65, 1, 8, 8, 128, 100, "all"), (300, 1, 8, 1, 128, 250, "all"), (600, 2, 4, 1, 64, 500, "causal"),
+    (200, 3, 8, 2, 128, 200, "mask"), (70, 130, 2, 2, 64, 300, "causal"), (1000, 1, 2, 2, 64, 40, "all")])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_attention_of_many_sequences_of_unequal_lengths(dev, B, N, Hq, Hk, D, W, kind, ragged):
+    """More sequences than a wave counts at once, a few of them long, in parts (but for the last)."""
+    g, dt, page, r = _gen(dev, 43), torch.bfloat16, 16, random.Random(B)
+    cache = _cache(g, 500, page, Hk, D, dt)
+    q = _randn(g, B, N, Hq, D).to(dt)
+    lens = [r.choice([0, 1, 5, 64, 65, 130]) for _ in range(B)]
+    for b in (0, B // 2, B - 1):
+        lens[b] = W * page - b % 7
+    table = torch.randint(0, 500, (B, W), generator=g, device=dev).to(I32)
+    lengths = torch.tensor(lens, dtype=I32, device=dev)
+    need = ops.cache_attention_ws_bytes(B, B * N, Hq, cache, W, ragged, kind == "causal", kind == "mask")
+    assert (need == 0) == (B == 1000)
+    mask = torch.rand(B, N, N, generator=g, device=dev) < 0.5 if kind == "mask" else None
+    kw = dict(causal=kind == "causal")
+    if ragged:
+        kw["offsets"] = torch.arange(0, B * N + 1, N, device=dev, dtype=I32)
+    out, lse = ops.cache_attention(q.flatten(0, 1) if ragged else q, cache, table, lengths, return_lse=True,
+                                   mask=mask.flatten(0, 1) if ragged and mask is not None else mask, **kw)
+    _check_attention(out, lse, attention_ref(q, cache, table, lens, [N] * B, mask, kind == "causal"))
 
 
 @pytest.mark.gpu

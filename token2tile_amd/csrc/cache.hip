@@ -1192,6 +1192,21 @@ static long long ca_full(int block, int ragged, int B, long long T, int G) {
 struct CachePlan {
   int block, S, target;
 };
+// Whether parts may help.  Past 64 sequences every work-group counts them through memory, several times over,
+// which costs more than parts gain where the work-groups are enough without and the keys few (one token a
+// sequence over tables of so many keys; us with and without parts, equal and random lengths, and four that
+// are eight times the others):
+//   sequences, key heads, keys      equal     random    four long
+//   256, 1, 1,024                   36   34   32   32   17   29
+//   400, 1, 2,048                  114   81   81   67   37   55
+//   400, 1, 4,096                  182  148  115  118   47  104
+//   2,000, 1, 4,096                820  632  664  368  237  159
+//   2,000, 1, 16,384              2580 2433 1657 1451  476  618
+//   128, 8, 4,096                  344  330  211  222   88  139
+//   400, 8, 4,096                 1084 1042  759  557  356  207
+static bool ca_divides(int B, long long wgs, long long keys) {
+  return B <= 64 || wgs <= 256 || (wgs < 2048 && keys >= 10LL * B);
+}
 static CachePlan ca_plan(int ragged, int B, long long T, int HQ, int HK, long long keys, int D, int hidden) {
   const int G = HQ / HK;
   // (of a ragged batch: twice the mean, as its sequences are not known to the host)
@@ -1208,7 +1223,7 @@ static CachePlan ca_plan(int ragged, int B, long long T, int HQ, int HK, long lo
     const double extra = block == 32 || !hidden ? 0.0 : (hidden == 1 ? 7.0 + 1.5 * wide : 20.0 + 13.0 * wide) * (fresh < 1.0 ? fresh : 1.0);
     for (int i = 0; i < 11; ++i) {  // 1, 2, 3 and eighths of all that run at once
       const long long S = i < 3 ? i + 1 : (i - 2) * slots / 8 / wgs;
-      if (S < 1 || S > most) continue;
+      if (S < 1 || S > most || (S > 1 && !ca_divides(B, wgs, keys))) continue;
       const double us = ca_time(block, wgs, (int)S, (double)keys, (double)T * HQ, mean, extra);
       if (least == 0.0 || us < least) least = us, best = CachePlan{block, (int)S, 0};
     }
@@ -1217,7 +1232,7 @@ static CachePlan ca_plan(int ragged, int B, long long T, int HQ, int HK, long lo
   // take more than its share
   const long long full = ca_full(best.block, ragged, B, T, G);
   best.target = (int)(best.S * full);
-  if (B > 1 && (best.S > 1 || (best.block == 32 && full * HK < 2048 && keys >= 2048))) {
+  if (B > 1 && (best.S > 1 || (best.block == 32 && full * HK < 2048 && keys >= 2048 && ca_divides(B, full * HK, keys)))) {
     // (where there are enough without parts, a round more of them for the long sequences')
     const long long room = (32 << 20) / (T * HQ * (D + 2) * 4);
     if (best.S == 1) best.target += 512 / HK;
