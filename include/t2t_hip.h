@@ -577,7 +577,7 @@ int t2t_cache_append(const t2t_rotary_tensor* q, const t2t_rotary_tensor* k,
  * 8 elements and pointers 16-byte aligned, one head's keys within 64 GiB; sums and
  * softmax in fp32, weights rounded to the type for the second product.  Values
  * up to 2^127 / keys and scores (scale q . k) up to 2^26 are in range: past these a row
- * may hold anything.  out and ws share no memory with another argument. */
+ * may hold anything.  0 < scale, and scale log2(e) finite in fp32.  out and ws share no memory with another argument. */
 typedef struct t2t_cache_attention_args {
   size_t struct_bytes; /* sizeof(t2t_cache_attention_args) */
   const void *q, *k, *v;

@@ -264,6 +264,26 @@ def test_a_workspace_of_any_size_is_the_one_that_is_used(launches):
     ops.cache_attention(**short, ws=buf[4:])
 
 
+@pytest.mark.parametrize("scale", [1e39, 1e-50, 2.5e38, -1e39, math.inf])
+def test_scales_that_fp32_does_not_hold(launches, scale):
+    """Not in 32 bits, or not times log2(e): refused before the launch, as every scale that is no number above 0."""
+    with pytest.raises(ValueError, match="scale"):
+        ops.cache_attention(**_attend_args(), scale=scale)
+    assert not launches
+    for good in (2.3e38, 1e-45, 1):
+        ops.cache_attention(**_attend_args(), scale=good)
+    assert len(launches) == 3
+
+
+def test_the_entry_refuses_a_scale_without_room():
+    from token2tile_amd import _lib
+    a = _lib.CacheAttentionArgs(struct_bytes=ctypes.sizeof(_lib.CacheAttentionArgs), q=32, k=32, v=32, out=32, table=32,
+                                lengths=32, q_batch=512, q_row=256, q_head=128, out_batch=512, out_row=256, out_head=128,
+                                kv_page=4096, kv_row=256, kv_head=128, table_row=4, B=2, N=2, HQ=2, HK=2, D=128, dtype=1,
+                                pages=8, page_size=16, width=4, scale=2.5e38)
+    assert _lib.lib().t2t_cache_attention(ctypes.byref(a), None, 0, None) == 1
+
+
 @pytest.mark.parametrize("kind", ["k", "v", "page_table", "lengths", "offsets", "mask"])
 def test_an_output_apart_from_every_input(launches, kind):
     buf = torch.zeros(1 << 16, dtype=torch.uint8)

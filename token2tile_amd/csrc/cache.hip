@@ -1262,7 +1262,7 @@ extern "C" int t2t_cache_attention(const t2t_cache_attention_args* a, void* ws, 
   T2T_REQUIRE(T * a->HQ <= INT_MAX, "cache_attention: %lld rows of %d heads", T, a->HQ);
   T2T_REQUIRE(a->pages >= 1 && a->page_size >= 1 && a->width >= 0 && (long long)a->width * a->page_size <= INT_MAX - 64,
               "cache_attention: %d pages of %d, %d a sequence", a->pages, a->page_size, a->width);
-  T2T_REQUIRE(a->scale > 0.f && a->scale < __builtin_inff(), "cache_attention: scale %g", a->scale);
+  T2T_REQUIRE(a->scale > 0.f && a->scale * 1.4426950408889634f < __builtin_inff(), "cache_attention: scale %g", a->scale);
   T2T_REQUIRE(!(a->mask && a->causal), "cache_attention: a mask and causal");
   T2T_REQUIRE(!a->mask || a->mask_cols >= 0, "cache_attention: mask of %d columns", a->mask_cols);
   T2T_REQUIRE(a->q && a->k && a->v && a->out && a->lengths && (a->table || a->width == 0),

@@ -1620,7 +1620,7 @@ def cache_attention(q, cache, page_table, lengths, *, offsets=None, mask=None, c
     is not seen has no part whatever it holds; keys in pages outside the cache are not
     seen, and lengths are held to what the table has room for.
 
-    ``scale`` (default D^-0.5) above 0.  fp32 sums and softmax, its weights rounded to
+    ``scale`` (default D^-0.5) above 0, at most 2.3e38.  fp32 sums and softmax, its weights rounded to
     the type for the second product.  Returns out (of q's shape), or (out, lse) with
     the natural logarithms of the softmax's sums, fp32 [..., Hq].  ``out``: contiguous
     channels, 16-byte aligned rows; it and ``ws`` share no memory with another
@@ -1666,8 +1666,8 @@ def cache_attention(q, cache, page_table, lengths, *, offsets=None, mask=None, c
             raise ValueError(f"t2t: mask must be a bool {[*lead, 'columns']} tensor on {dev} with contiguous rows")
     if scale is None:
         scale = D ** -0.5
-    elif not (math.isfinite(scale) and scale > 0.0):
-        raise ValueError(f"t2t: scale must be above 0, got {scale}")
+    elif not 2.0 ** -150 < scale <= 2.3e38:  # (in fp32 above 0, and finite times log2(e))
+        raise ValueError(f"t2t: scale must be above 0 and within fp32, got {scale}")
     qs = _attn_strides(q, "q")
     if out is None:
         o = (_empty(stream, q.shape, dt, dev) if stream is not None
