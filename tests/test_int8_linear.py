@@ -208,6 +208,14 @@ def test_refused(launches, bad):
     assert not launches
 
 
+@pytest.mark.parametrize("scales", [None, [1.0] * 4, 1.0])
+def test_scales_of_a_checkpoint_are_a_tensor(launches, scales):
+    with pytest.raises(ValueError, match="t2t"):
+        ops.Int8.from_codes(torch.zeros(4, 100, dtype=torch.int8), scales)
+    W = ops.Int8.from_codes(torch.zeros(4, 100, dtype=torch.int8), torch.arange(8.0)[::2])  # (of any stride)
+    assert W.scales.tolist() == [0.0, 2.0, 4.0, 6.0] and W.scales.is_contiguous()
+
+
 # ---------------------------------------------------------------------------
 # quantisation
 # ---------------------------------------------------------------------------

@@ -1299,6 +1299,8 @@ class Int8:
         which are copied."""
         if not isinstance(codes, torch.Tensor) or codes.dtype != torch.int8 or codes.dim() != 2:
             raise ValueError("t2t: codes must be an int8 [rows, cols] tensor")
+        if not isinstance(scales, torch.Tensor):
+            raise ValueError("t2t: scales must be an fp32 [rows] tensor")
         rows, cols = codes.shape
         if not 1 <= cols <= _I8_MAX_COLS:
             raise ValueError(f"t2t: an 8-bit matrix has 1 to 2^17 - 1 columns, got {rows} x {cols}")
