@@ -136,7 +136,7 @@ template <> struct CaType<F16T> {
   static constexpr uint32_t inf = 0x7c00u;
 };
 
-// ---- one tile of NK x 32 keys for 32 rows ------------------------------------
+// ---- 32 keys for 32 rows -----------------------------------------------------
 // S^T = K Q^T and O^T = V^T P^T: lane l holds row l % 32 throughout, keys 8 (a / 4)
 // + 4 (l / 32) + a % 4 of a 32-key block in element a, dims likewise.
 template <typename T, int D>
@@ -335,29 +335,26 @@ __device__ inline bool ca_item(const CacheArgs& A, int& part, int& parts, int& k
 }
 
 // s -> weights against the running maximum (exp2 scales exactly, so it only has to keep the weights in
-// the range of T: it moves where they leave it, and the sums so far with it)
-template <typename T, int D, int NK>
-__device__ inline void ca_weights(CacheState<T, D>& w, const f32x16 (&s)[NK], u32x4 (&p)[2 * NK], float c) {
+// the range of T: it moves where they leave it, and the sums so far with it).  The many-row kernel's
+// weigh() and settle() are the same steps between its products: they change together.
+template <typename T, int D>
+__device__ inline void ca_weights(CacheState<T, D>& w, const f32x16& s, u32x4 (&p)[2], float c) {
   auto expo = [&](float nm) __attribute__((always_inline)) {
     float acc = 0.f;
 #pragma unroll
-    for (int kb = 0; kb < NK; ++kb)
-#pragma unroll
-      for (int a = 0; a < 16; a += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][a], c, nm));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][a + 1], c, nm));
-        acc += p0 + p1;
-        p[2 * kb + a / 8][(a % 8) / 2] = Pk<T>::pack(p0, p1);
-      }
+    for (int a = 0; a < 16; a += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[a], c, nm));
+      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[a + 1], c, nm));
+      acc += p0 + p1;
+      p[a / 8][(a % 8) / 2] = Pk<T>::pack(p0, p1);
+    }
     return acc;
   };
   float lt = expo(-w.m);
   if (__builtin_amdgcn_readfirstlane((int)(__ballot(!(lt <= CaType<T>::limit)) != 0ull))) {
     float mr = -__builtin_inff();
 #pragma unroll
-    for (int kb = 0; kb < NK; ++kb)
-#pragma unroll
-      for (int a = 0; a < 16; ++a) mr = __builtin_elementwise_maximum(mr, s[kb][a]);
+    for (int a = 0; a < 16; ++a) mr = __builtin_elementwise_maximum(mr, s[a]);
     const float mx = half_max(mr) * c - CaType<T>::top;
     const float mnew = mx > w.m || mx != mx ? mx : w.m;
     const float alpha = __builtin_amdgcn_exp2f(w.m - mnew);
@@ -467,10 +464,10 @@ __global__ __launch_bounds__(128, 1) void ca_few_kernel(CacheArgs A) {
   auto step = [&](int t, uint64_t bad, auto BUF) __attribute__((always_inline)) {
     const uint16_t* sk = (decltype(BUF)::value ? sK1 : sK0) + wave * TILE;
     const uint16_t* sv = (decltype(BUF)::value ? sV1 : sV0) + wave * TILE;
-    f32x16 s[1] = {zero16()};
+    f32x16 s = zero16();
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
-      s[0] = Mfma<T>::run(*(const u32x4*)(sk + jl * D + 8 * ((2 * i + hh) ^ ca_kswz<D>(jl))), st.q[i], s[0]);
+      s = Mfma<T>::run(*(const u32x4*)(sk + jl * D + 8 * ((2 * i + hh) ^ ca_kswz<D>(jl))), st.q[i], s);
     const bool hide = 32 * t + 32 > (masked ? w.first : w.L) || bad;  // (of the wave)
     uint32_t seen = 0;  // by the lane's row
     if (hide) {
@@ -480,10 +477,10 @@ __global__ __launch_bounds__(128, 1) void ca_few_kernel(CacheArgs A) {
       seen = sight.bits(32 * t, raw) & ~(uint32_t)bad;
 #pragma unroll
       for (int a = 0; a < 16; ++a)
-        if (!(seen >> (8 * (a / 4) + 4 * hh + a % 4) & 1)) s[0][a] = -__builtin_inff();
+        if (!(seen >> (8 * (a / 4) + 4 * hh + a % 4) & 1)) s[a] = -__builtin_inff();
     }
     u32x4 p[2];
-    ca_weights<T, D, 1>(st, s, p, A.c);
+    ca_weights<T, D>(st, s, p, A.c);
     bool odd = false;
 #pragma unroll
     for (int nb = 0; nb < D / 32; ++nb) {
@@ -794,7 +791,8 @@ __global__ __launch_bounds__(64 * W, 2) void ca_many_kernel(CacheArgs A) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) asm volatile("" : "+a"(o[nb]));
   };
-  // a half tile's weights have left the range: the maximum moves, and they are taken again
+  // a half tile's weights have left the range: the maximum moves, and they are taken again (as in
+  // ca_weights)
   auto settle = [&](const f32x16& S, u32x4 (&P)[2], float& lt) __attribute__((always_inline)) {
     if (__ballot(!(lt <= CaType<T>::limit))) {
       ready();
