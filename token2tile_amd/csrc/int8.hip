@@ -121,7 +121,8 @@ __device__ inline uint32_t i8_top(uint32_t top, const u32x4& v) {  // both halve
 }
 
 // TPR threads a row, which stays in registers between its maximum and its codes:
-// one read of x, one write of the codes, which bound it (75,600 x 5,120: 5.3 TB/s).  A
+// one read of x, one write of the codes, which bound it (75,600 x 5,120: 4.6 to 5.5 TB/s; 4,099 x
+// 1,531 is one round of waves, each a chain of loads, maximum and codes: 8.5 us, 7.6 at 1,536 columns).  A
 // work-group has several rows where it can:
 // a row writes half lines (64 bytes of every block), its neighbour the other halves
 // (75,600 x 5,120: 217 us with two rows, 260 with one).
@@ -272,7 +273,7 @@ __device__ inline float i8_out(int acc, float sw, float sa, float bias) {
 // meet in LDS.  With X16 the tokens come in 16 bits, and every work-group quantises
 // them into LDS first, under the loads of its first weights, in the place of a launch
 // before this one.  Bound: the weights' loads, of which 160 of 256 CUs have one round
-// each (1 x 5,120 x 5,120: 7.0 us, 3.7 TB/s).
+// each (1 x 5,120 x 5,120: 10.5 us with weights from memory, 2.5 TB/s; 7.4 on one weight again and again).
 #define I8_X16_BYTES 32768  // codes that the LDS holds
 struct I8Src {
   I8Mat m;            // in 8 bits (its row count in either case), or
@@ -834,8 +835,8 @@ extern "C" int t2t_int8_product(const void* a_codes, const float* a_scales, cons
                                                                    (hipStream_t)stream);
 }
 
-// Few rows are quantised by the product itself: every work-group does it again (5120 x 5120, one row: 7.0
-// us, two 8.0, four 11.1; with a launch before it 10.0 throughout).
+// Few rows are quantised by the product itself: every work-group does it again (5120 x 5120, weights
+// from memory: one row 10.5 us, two 11.8, three 14.5, four 14.8; with a launch before it 14.4, 14.1, 14.2, 14.8).
 static bool i8_few(int M, int K) { return M <= 2 && M * i8_kp(K) <= I8_X16_BYTES; }
 
 // codes, then scales

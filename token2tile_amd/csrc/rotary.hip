@@ -203,7 +203,8 @@ __device__ inline typename RopeVec<V>::type rope_pack(const float (&f)[V]) {
 // The forms with SLOTS are those of an append: the first tensor's rows go to their slots (its out
 // strides are the cache's), the second, if any, is an ordinary one, and the grid's last row of
 // work-groups stores v.  Bound: one read and one write of every element (4,680 tokens of 40 heads:
-// 68 us, 4.2 TB/s; 10,007 of 32 and 8, head norm, 96 of 128: 43.5 us, 5.7 TB/s; a token: 4.9 us).
+// 72 us, 4.0 TB/s; 10,007 of 32 and 8, head norm, 96 of 128: 52 us, 4.8 TB/s; 68 and 43.5 on inputs just
+// seen; four tokens: 4.9 us).
 struct RopeSlots {
   const void* slots;
   int wide;               // 64-bit slots
